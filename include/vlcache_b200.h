@@ -370,6 +370,98 @@ int vlc_content_hash_host(const void* data, int64_t nbytes, const void* header, 
                           uint64_t* digest);
 uint64_t vlc_xxh64(const void* data, int64_t nbytes, uint64_t seed);
 
+/* --------------------------------------------------------------------------
+ * Rotary embedding at positions with several axes (time, height, width) fused with the
+ * KV scatter.  No counterpart in the reference (get_rope ignores rope_scaling,
+ * nanovllm/layers/rotary_embedding.py:51-71); the rotation is HF transformers'
+ * apply_multimodal_rotary_pos_emb (modeling_qwen2_5_vl.py:627-665).
+ *   positions [num_axes][axis_stride] int64, num_axes 1 .. 4 (axis_stride 0: one row for
+ *   every axis); sections[num_axes] pairs per axis, in order, summing to head_dim / 2: rotate-half pair j takes the position of
+ *   the axis whose section holds it.
+ * Everything else as vlc_rope_store_kvcache, whose result it gives, bit for bit, when a
+ * row's positions are equal on all axes.  A row with a position outside the table on any
+ * axis is recorded (VLC_DEV_ERR_POSITION) and its q and k are not stored.
+ * ------------------------------------------------------------------------ */
+int vlc_mrope_store_kvcache(const int64_t* positions, int64_t axis_stride, int num_axes, const int32_t* sections,
+                            const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, const void* key,
+                            int64_t key_stride, const void* value, int64_t value_stride,
+                            const float* cos_sin_cache, int64_t max_position, void* k_cache, void* v_cache,
+                            const int32_t* slot_mapping, int64_t num_slots, void* k_out, int64_t k_out_stride,
+                            int num_tokens, int num_heads, int num_kv_heads, int head_dim, void* stream);
+
+/* --------------------------------------------------------------------------
+ * The KV cache in 4 bits.  No counterpart in the reference.
+ * A head's row of 128 dims is 8 groups of 16; a group holds one e4m3 scale s and 16 e2m1
+ * codes (two per byte, the even dim in the low nibble).  With g a power of two per cache
+ * (k_scale, v_scale; 2^-64 .. 2^64):
+ *   s = e4m3(min(max|x / g| / 6, 448)),  code = e2m1(x / g / s),  value = g * s * code,
+ * rounded to nearest even; codes are 0 where s is 0, magnitudes above 6 become 6, a NaN
+ * makes its whole group NaN.  Every value is exact in bf16.  Choose g so that max|x| / g
+ * stays below 2688 and the small groups' max|x| / g above 6 * 2^-6.
+ * Page of one layer's K or V: [num_kv_heads][block_size * 64 code bytes | block_size * 8
+ * scale bytes], block_size a multiple of 64; caches [num_pages] such pages, contiguous.
+ * Slot -> page slot / block_size, row slot % block_size, as in the bf16 cache.
+ *
+ * vlc_rope_store_kvcache_fp4: vlc_mrope_store_kvcache with its k and v rows quantised into
+ *   such a cache (num_axes = 1, sections = {64}: the one-axis rotation).  The key is
+ *   rounded to bf16 first, as the bf16 cache holds it.
+ * vlc_store_kvcache_fp4: the rows without a rotation (vlc_store_kvcache's contract).
+ * vlc_gather_kvcache_fp4: the values of keys 0 .. len_b - 1 of every sequence, row
+ *   cu_seqlens_k[b] + j of k_out / v_out ([total_k, num_kv_heads, 128] bf16, row stride
+ *   out_row_stride elements), for num_layers layers (layer l of the caches at
+ *   l * layer_stride bytes, of the outputs at l * out_layer_stride elements).
+ *   cu_seqlens_k: device, num_seqs + 1.  Keys of a bad table entry read as 0 and are
+ *   recorded (VLC_DEV_ERR_BLOCK_RANGE); rows past total_k are recorded
+ *   (VLC_DEV_ERR_LENGTH) and not written.
+ * vlc_mrope_shift_fp4: vlc_mrope_shift in such a cache: K rows of src_slots rotated by the
+ *   delta, rounded to bf16, quantised again, written to dst_slots (NULL: in place); V rows
+ *   copied when dst_slots is given.  A group whose 16 pairs the delta does not turn keeps
+ *   its bits.  layer_stride in bytes.
+ * vlc_decode_attn_fp4: vlc_decode_attn over such a cache: f16 products of exact K / V
+ *   values with q (scaled per head by a power of two) and P, fp32 sums.  Keys of a chunk of
+ *   64 whose table entry is bad are left out and recorded.
+ * ------------------------------------------------------------------------ */
+int vlc_rope_store_kvcache_fp4(const int64_t* positions, int64_t axis_stride, int num_axes, const int32_t* sections,
+                               const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, const void* key,
+                               int64_t key_stride, const void* value, int64_t value_stride,
+                               const float* cos_sin_cache, int64_t max_position, void* k_cache, void* v_cache,
+                               const int32_t* slot_mapping, int64_t num_pages, int block_size, float k_scale,
+                               float v_scale, int num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                               void* stream);
+int vlc_store_kvcache_fp4(const void* key, int64_t key_stride, const void* value, int64_t value_stride, void* k_cache,
+                          void* v_cache, const int32_t* slot_mapping, int64_t num_pages, int block_size,
+                          float k_scale, float v_scale, int num_tokens, int num_kv_heads, int head_dim, void* stream);
+int vlc_gather_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t layer_stride, int num_layers,
+                           int64_t num_pages, int block_size, int num_kv_heads, int head_dim,
+                           const int32_t* block_tables, int64_t block_table_stride, int block_table_width,
+                           const int32_t* cu_seqlens_k, int num_seqs, int64_t total_k, float k_scale, float v_scale,
+                           void* k_out, void* v_out, int64_t out_row_stride, int64_t out_layer_stride, void* stream);
+int vlc_mrope_shift_fp4(void* k_cache, void* v_cache, int64_t layer_stride, int num_layers, int64_t num_pages,
+                        int block_size, int num_kv_heads, int head_dim, const int32_t* src_slots,
+                        const int32_t* dst_slots, int num_rows, const int32_t* delta_thw,
+                        const int32_t* mrope_section, float rope_theta, void* stream);
+int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_seqs, int num_heads, const void* k_cache,
+                        const void* v_cache, int64_t num_pages, int block_size, int num_kv_heads, int head_dim,
+                        const int32_t* block_tables, int64_t block_table_stride, int block_table_width,
+                        const int32_t* context_lens, int max_context_len, float softmax_scale, float k_scale,
+                        float v_scale, void* out, int64_t out_seq_stride, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+int64_t vlc_decode_fp4_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int max_context_len);
+
+/* --------------------------------------------------------------------------
+ * Pages.  vlc_copy_pages: in each of num_planes planes (one layer's K or V: num_pages
+ * pages of page_bytes, planes plane_stride bytes apart) page dst_pages[i] becomes a copy
+ * of page src_pages[i] (device lists; a pair of -1 is skipped).  All in one launch and in
+ * no order: destinations differ, and none is another pair's source.  An index out of
+ * range is recorded (VLC_DEV_ERR_BLOCK_RANGE) and its pair skipped.
+ * vlc_remap_block_tables: every entry p of a table (row stride row_stride) becomes
+ * page_map[p]; -1 stays, an entry out of range is recorded and stays.
+ * ------------------------------------------------------------------------ */
+int vlc_copy_pages(void* base, int64_t plane_stride, int num_planes, int64_t page_bytes, int64_t num_pages,
+                   const int32_t* src_pages, const int32_t* dst_pages, int num_pairs, void* stream);
+int vlc_remap_block_tables(int32_t* block_tables, int64_t row_stride, int num_rows, int width,
+                           const int32_t* page_map, int num_pages, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,23 @@ SIGNATURES: dict[str, tuple] = {
     "vlc_qkv_rope_store_kvcache": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp,
                                            c_vp, c_vp, c_i64, c_int, c_int, c_int, c_int, c_int, c_vp, c_i64,
                                            c_vp]),
+    "vlc_mrope_store_kvcache": (c_int, [c_vp, c_i64, c_int, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,
+                                        c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_int, c_int, c_int, c_int,
+                                        c_vp]),
+    "vlc_rope_store_kvcache_fp4": (c_int, [c_vp, c_i64, c_int, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp,
+                                           c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_float, c_float,
+                                           c_int, c_int, c_int, c_int, c_vp]),
+    "vlc_store_kvcache_fp4": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_float, c_float,
+                                      c_int, c_int, c_int, c_vp]),
+    "vlc_gather_kvcache_fp4": (c_int, [c_vp, c_vp, c_i64, c_int, c_i64, c_int, c_int, c_int, c_vp, c_i64, c_int, c_vp,
+                                       c_int, c_i64, c_float, c_float, c_vp, c_vp, c_i64, c_i64, c_vp]),
+    "vlc_mrope_shift_fp4": (c_int, [c_vp, c_vp, c_i64, c_int, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_int, c_vp,
+                                    c_vp, c_float, c_vp]),
+    "vlc_decode_attn_fp4": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_i64,
+                                    c_int, c_vp, c_int, c_float, c_float, c_float, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "vlc_decode_fp4_workspace_size": (c_i64, [c_int, c_int, c_int, c_int]),
+    "vlc_copy_pages": (c_int, [c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_int, c_vp]),
+    "vlc_remap_block_tables": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_int, c_vp]),
 }
 
 

@@ -12,6 +12,9 @@ Host side of the hot path, mirroring nano-vllm's model runner / engine:
     padded block tables, positions, vectorised, plus the attention plan, all built from
     host data so no device read is needed during the step;
   * ``prepare_decode``        — model_runner.py:322-338.
+  * ``kv_format="fp4"``       — the cache in 4 bits, uint8 ``[2, L, num_blocks, Hk, block_size * 72]``
+    (no counterpart in the reference; include/vlcache_b200.h has the layout): the same
+    ``copy_image_kv`` and ``Attention`` calls work on it.
 """
 from __future__ import annotations
 
@@ -42,12 +45,13 @@ class CacheBudget:
 def cache_budget(num_layers: int, num_kv_heads: int, head_dim: int, hidden_size: int, *, block_size: int = BLOCK_SIZE,
                  dtype=torch.bfloat16, gpu_memory_utilization: float = 0.9, encoder_cache_ratio: float = 0.2,
                  mem_info: tuple[int, int] | None = None, peak_bytes: int | None = None,
-                 current_bytes: int | None = None) -> CacheBudget:
+                 current_bytes: int | None = None, kv_format: str = "bf16") -> CacheBudget:
     """The reference's sizing rule (model_runner.py:130-151):
     ``available = total * gpu_memory_utilization - used - peak + current`` (used = total -
     free; peak / current = torch's allocated-bytes statistics), ``encoder_cache_ratio`` of
     it for the encoder cache (blocks of ``block_size`` tokens x ``hidden_size``), the rest
-    for KV blocks of ``2 * layers * block_size * Hk * head_dim`` elements.  The memory
+    for KV blocks of ``2 * layers * block_size * Hk * head_dim`` elements (72 bytes per
+    row and head with ``kv_format="fp4"``).  The memory
     figures default to the current device's; pass them to size for another budget."""
     if mem_info is None:
         free, total = torch.cuda.mem_get_info()
@@ -59,7 +63,8 @@ def cache_budget(num_layers: int, num_kv_heads: int, head_dim: int, hidden_size:
         current_bytes = stats.get("allocated_bytes.all.current", 0) if current_bytes is None else current_bytes
     itemsize = torch.empty((), dtype=dtype).element_size()
     used = total - free
-    kv_block_bytes = 2 * num_layers * block_size * num_kv_heads * head_dim * itemsize
+    row_bytes = ops.FP4_ROW_BYTES if _is_fp4(kv_format, head_dim) else head_dim * itemsize
+    kv_block_bytes = 2 * num_layers * block_size * num_kv_heads * row_bytes
     encoder_block_bytes = block_size * hidden_size * itemsize
     available = total * gpu_memory_utilization - used - peak_bytes + current_bytes
     encoder_memory = available * encoder_cache_ratio
@@ -71,16 +76,28 @@ def cache_budget(num_layers: int, num_kv_heads: int, head_dim: int, hidden_size:
     return budget
 
 
+def _is_fp4(kv_format: str, head_dim: int) -> bool:
+    if kv_format not in ("bf16", "fp4"):
+        raise ValueError(f"kv_format {kv_format!r}: bf16 or fp4")
+    if kv_format == "fp4" and head_dim != ops.HEAD_DIM:
+        raise ValueError(f"the 4-bit cache has head_dim {ops.HEAD_DIM}")
+    return kv_format == "fp4"
+
+
 def allocate_kv_cache(model: torch.nn.Module | None, num_layers: int, num_blocks: int | None, num_kv_heads: int,
                       head_dim: int = 128, block_size: int = BLOCK_SIZE, dtype=torch.bfloat16,
                       device="cuda", *, hidden_size: int | None = None, gpu_memory_utilization: float = 0.9,
-                      encoder_cache_ratio: float = 0.2) -> torch.Tensor:
+                      encoder_cache_ratio: float = 0.2, kv_format: str = "bf16") -> torch.Tensor:
     """``[2, L, num_blocks, block_size, Hk, D]`` with per-layer views handed to every module
     that has ``k_cache`` / ``v_cache`` (model_runner.py:152-158), plus the module's
     ``layer_id``.  ``num_blocks=None`` sizes the pool from the device's free memory with
     the reference's rule (``cache_budget``, which needs ``hidden_size`` for the encoder
     cache share); the tensor's ``budget`` attribute then holds the block counts, the
-    encoder-cache block count included."""
+    encoder-cache block count included.  ``kv_format="fp4"`` makes the 4-bit cache (the
+    modules' ``k_scale`` / ``v_scale`` are its powers of two)."""
+    fp4 = _is_fp4(kv_format, head_dim)
+    if fp4 and block_size % 64:
+        raise ValueError("the 4-bit cache needs a block size that is a multiple of 64")
     budget = None
     if num_blocks is None:
         if hidden_size is None:
@@ -88,10 +105,14 @@ def allocate_kv_cache(model: torch.nn.Module | None, num_layers: int, num_blocks
         with torch.cuda.device(torch.device(device)):
             budget = cache_budget(num_layers, num_kv_heads, head_dim, hidden_size, block_size=block_size, dtype=dtype,
                                   gpu_memory_utilization=gpu_memory_utilization,
-                                  encoder_cache_ratio=encoder_cache_ratio)
+                                  encoder_cache_ratio=encoder_cache_ratio, kv_format=kv_format)
         num_blocks = budget.num_kvcache_blocks
-    kv_cache = torch.empty(2, num_layers, num_blocks, block_size, num_kv_heads, head_dim, dtype=dtype,
-                           device=device)
+    if fp4:
+        kv_cache = torch.empty(2, num_layers, num_blocks, num_kv_heads, block_size * ops.FP4_ROW_BYTES,
+                               dtype=torch.uint8, device=device)
+    else:
+        kv_cache = torch.empty(2, num_layers, num_blocks, block_size, num_kv_heads, head_dim, dtype=dtype,
+                               device=device)
     kv_cache.budget = budget
     if model is not None:
         layer_id = 0
@@ -142,6 +163,27 @@ def check_reuse_slots(old_slots, new_slots) -> None:
                          "different positions); move the rows through a fresh page first")
 
 
+def copy_pages(kv_cache: torch.Tensor, src_pages, dst_pages) -> None:
+    """Copy whole pages of every layer (host lists; ``PagePool.fork`` and ``PagePool.compact``
+    return such lists), after checking them: destinations differ, and none is the source
+    of another pair."""
+    src, dst = np.asarray(src_pages, dtype=np.int64).ravel(), np.asarray(dst_pages, dtype=np.int64).ravel()
+    if src.shape != dst.shape:
+        raise ValueError("source and destination page lists differ in length")
+    if len(src) == 0:
+        return
+    pages = kv_cache.shape[2]
+    if min(src.min(), dst.min()) < 0 or max(src.max(), dst.max()) >= pages:
+        raise ValueError(f"page outside the cache's {pages}")
+    if len(np.unique(dst)) != len(dst):
+        raise ValueError("a page is the destination of two copies")
+    moved = src != dst
+    if np.intersect1d(src[moved], dst[moved]).size:
+        raise ValueError("a page is the source of one copy and the destination of another")
+    up = torch.from_numpy(np.stack([src, dst]).astype(np.int32)).pin_memory().to(kv_cache.device, non_blocking=True)
+    ops.copy_kv_pages(kv_cache, up[0], up[1])
+
+
 def copy_image_kv(kv_cache: torch.Tensor, old_slots, new_slots, delta_thw=(0, 0, 0),
                   shift: MRopeShift | None = None) -> None:
     """Move reused image K/V rows (all layers) to new slots, rotating K by ``delta_thw``.
@@ -176,7 +218,7 @@ def copy_image_kv_per_layer(kv_cache: torch.Tensor, src_slots: torch.Tensor, dst
     events = []
     with torch.cuda.stream(stream):
         for layer in range(kv_cache.shape[1]):
-            if src_slots.numel():
+            if src_slots.numel():   # either cache format
                 sh.shift_layer(kv_cache[0, layer], kv_cache[1, layer], src_slots, dst_slots, delta_thw)
             ev = torch.cuda.Event()
             ev.record(stream)

@@ -11,6 +11,11 @@ Optionally ``forward(q, k, v, positions=..., rotary_emb=...)`` takes q/k before 
 and rotates them in the scatter launch (vlc_rope_store_kvcache): the caller's
 ``q, k = self.rotary_emb(positions, q, k); o = self.attn(q, k, v)``
 (nanovllm/models/qwen3.py:84-86) becomes one call with the same result.
+A ``rotary_emb`` with several axes (``layers.rotary_embedding.MRotaryEmbedding``) takes its
+``positions`` as ``[axes, tokens]``.
+A 4-bit cache (``allocate_kv_cache(..., kv_format="fp4")``: ``k_cache`` / ``v_cache`` uint8) is
+written by vlc_rope_store_kvcache_fp4 / vlc_store_kvcache_fp4 and read by the 4-bit prefill
+and decode; ``k_scale`` / ``v_scale`` are its powers of two.
 ``forward(q, None, None)`` attends over a cache that already holds this step's K/V
 (stored by ``layers.linear.QKVParallelLinear.forward_rope_store``, which fuses the
 QKV projection, RoPE and the scatter).
@@ -29,6 +34,19 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
                   slot_mapping: torch.Tensor):
     """Scatter new K/V rows into the paged cache by slot (-1 skipped).  Bit-exact copy."""
     ops.store_kvcache(key, value, k_cache, v_cache, slot_mapping)
+
+
+def rope_store(positions, q, k, v, rotary_emb: nn.Module, attn: nn.Module, slot_mapping) -> torch.Tensor:
+    """Rotate q and k and scatter k and v into ``attn``'s cache, whatever its format and the
+    rotation's axes, in one launch; returns the rotated q."""
+    section = getattr(rotary_emb, "mrope_section", None)
+    table, k_cache, v_cache = rotary_emb.cos_sin_cache, attn.k_cache, attn.v_cache
+    if k_cache.dtype == torch.uint8:
+        return ops.rope_store_kvcache_fp4(positions, q, k, v, table, k_cache, v_cache, slot_mapping, section,
+                                          attn.k_scale, attn.v_scale)
+    if section is not None:
+        return ops.mrope_store_kvcache(positions, q, k, v, table, k_cache, v_cache, slot_mapping, section)
+    return ops.rope_store_kvcache(positions, q, k, v, table, k_cache, v_cache, slot_mapping)
 
 
 def _prefill_plan(context: Context, num_heads: int, num_kv_heads: int, device: torch.device) -> ops.PrefillPlan:
@@ -68,6 +86,7 @@ class Attention(nn.Module):
         self.scale = scale
         self.num_kv_heads = num_kv_heads
         self.k_cache = self.v_cache = torch.tensor([])
+        self.k_scale = self.v_scale = 1.0  # powers of two that a 4-bit cache's values are divided by
         self.layer_id = None  # set by engine.kv_cache.allocate_kv_cache (or the caller)
 
     def forward(self, q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None,
@@ -85,23 +104,30 @@ class Attention(nn.Module):
             assert self.layer_id is not None, "kv_ready needs Attention.layer_id"
             torch.cuda.current_stream().wait_event(context.kv_ready[self.layer_id])
         have_cache = bool(k_cache.numel() and v_cache.numel()) and k is not None
+        fp4 = k_cache.dtype == torch.uint8
         if rotary_emb is not None:
             assert positions is not None, "rotary_emb needs the positions"
             if have_cache and (context.block_tables is not None or not context.is_prefill):
                 # K/V are read back from the cache: rotate and scatter in one launch
-                q = ops.rope_store_kvcache(positions, q, k, v, rotary_emb.cos_sin_cache, k_cache, v_cache,
-                                           context.slot_mapping)
+                q = rope_store(positions, q, k, v, rotary_emb, self, context.slot_mapping)
                 have_cache = False  # stored
             else:                   # cold prefill reads the in-flight K: rotate it too
                 q, k = rotary_emb(positions, q, k)
         stored_plain = False  # k / v hold exactly the rows store_kvcache copied into the cache
-        if have_cache:
+        if have_cache and fp4:
+            ops.store_kvcache_fp4(k, v, k_cache, v_cache, context.slot_mapping, self.k_scale, self.v_scale)
+        elif have_cache:
             store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)
             stored_plain = True
         if context.is_prefill:
             plan = _prefill_plan(context, self.num_heads, self.num_kv_heads, q.device)
-            ws = _workspace(context, plan.workspace_bytes, q.device)
-            if context.block_tables is not None:    # prefix cache / warm request: paged K/V
+            paged = context.block_tables is not None
+            ws = _workspace(context, ops.prefill_fp4_workspace_bytes(plan, self.num_kv_heads) if fp4 and paged
+                            else plan.workspace_bytes, q.device)
+            if paged and fp4:
+                o = ops.prefill_attention_fp4(q, k_cache, v_cache, context.block_tables, context.cu_seqlens_k, plan,
+                                              self.scale, self.k_scale, self.v_scale, workspace=ws)
+            elif paged:                             # prefix cache / warm request: paged K/V
                 # k / v (when given) are the rows just stored: self-attention sequences read
                 # them directly and do not wait for the scatter
                 inflight = k is not None and stored_plain
@@ -113,7 +139,14 @@ class Attention(nn.Module):
         else:    # decode
             max_len = context.max_context_len
             if max_len is None:
-                max_len = context.block_tables.size(1) * k_cache.shape[1]
+                max_len = context.block_tables.size(1) * (k_cache.shape[-1] // ops.FP4_ROW_BYTES if fp4
+                                                          else k_cache.shape[1])
+            if fp4:
+                ws = _workspace(context, ops.decode_fp4_workspace_bytes(q.shape[0], self.num_heads, self.num_kv_heads,
+                                                                        max_len), q.device)
+                o = ops.decode_attention_fp4(q, k_cache, v_cache, context.block_tables, context.context_lens, max_len,
+                                             self.scale, self.k_scale, self.v_scale, workspace=ws)
+                return o.unsqueeze(1)
             ws = _workspace(context, ops.decode_workspace_bytes(q.shape[0], self.num_heads, self.num_kv_heads,
                                                                 max_len), q.device)
             o = ops.decode_attention(q, k_cache, v_cache, context.block_tables, context.context_lens, max_len,

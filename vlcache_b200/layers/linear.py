@@ -22,6 +22,7 @@ from torch import nn
 
 from .. import ops
 from ..utils.context import get_context
+from .attention import rope_store
 
 
 def divide(numerator: int, denominator: int) -> int:
@@ -104,8 +105,14 @@ class QKVParallelLinear(ColumnParallelLinear):
                            attn: nn.Module) -> torch.Tensor:
         """qkv_proj + rotary_emb + store_kvcache for this step's rows: returns the roped q
         ``[tokens, num_heads, head_size]``; the roped k and the v rows are in ``attn``'s
-        cache at the context's ``slot_mapping``, so call ``attn`` without K/V to store."""
+        cache at the context's ``slot_mapping``, so call ``attn`` without K/V to store.  With
+        a 4-bit cache or a rotation of several axes the projection is one launch and the
+        rotation with the scatter another."""
         context = get_context()
+        if attn.k_cache.dtype == torch.uint8 or getattr(rotary_emb, "mrope_section", None) is not None:
+            qkv = self(x.reshape(-1, x.shape[-1])).view(-1, self.num_heads + 2 * self.num_kv_heads, self.head_size)
+            q, k, v = qkv.split((self.num_heads, self.num_kv_heads, self.num_kv_heads), dim=1)
+            return rope_store(positions, q, k, v, rotary_emb, attn, context.slot_mapping)
         return ops.qkv_rope_store_kvcache(x.reshape(-1, x.shape[-1]), self.weight, self.bias, positions,
                                           rotary_emb.cos_sin_cache, attn.k_cache, attn.v_cache,
                                           context.slot_mapping, self.num_heads, self.num_kv_heads)

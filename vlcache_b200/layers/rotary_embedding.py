@@ -15,7 +15,13 @@ uses the t, h or w position of the token, by ``mrope_section`` = [16, 24, 24].  
 cached image reappears at a different place in the prompt every vision position
 moves by the same offset per section, and since R(p + d) = R(d) R(p) per pair the
 cached K only needs one extra rotation by d.  ``MRopeShift`` applies it on the GPU
-(vlc_mrope_shift), in place or while moving the rows to the new request's pages.
+(vlc_mrope_shift), in place or while moving the rows to the new request's pages; in a
+4-bit cache through vlc_mrope_shift_fp4.
+
+``MRotaryEmbedding`` / ``get_mrope`` rotate new rows at positions of several axes, which a
+model trained with M-RoPE needs for its image rows: the same table and call as
+``RotaryEmbedding`` with positions ``[axes, N]``, and accepted wherever the attention and
+projection layers take a ``rotary_emb``.
 """
 from __future__ import annotations
 
@@ -68,6 +74,31 @@ def _rope_cached(head_size: int, rotary_dim: int, max_position: int, base: float
     return RotaryEmbedding(head_size, rotary_dim, max_position, base)
 
 
+class MRotaryEmbedding(RotaryEmbedding):
+    """Rotate-half RoPE at positions of several axes: pair j of the split takes the position
+    of the axis whose section of ``mrope_section`` (pairs per axis) holds it (HF
+    modeling_qwen2_5_vl.py:627-665)."""
+
+    def __init__(self, head_size: int, rotary_dim: int, max_position_embeddings: int, base: float,
+                 mrope_section=ops.DEFAULT_MROPE_SECTION) -> None:
+        super().__init__(head_size, rotary_dim, max_position_embeddings, base)
+        self.mrope_section = tuple(int(x) for x in mrope_section)
+        if min(self.mrope_section) < 0 or sum(self.mrope_section) != rotary_dim // 2:
+            raise ValueError(f"mrope_section {self.mrope_section} does not sum to {rotary_dim // 2} pairs")
+
+    def forward(self, positions: torch.Tensor, query: torch.Tensor,
+                key: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """query [N, H, D], key [N, Hk, D] bf16 and int64 positions [axes, N] -> new rotated tensors."""
+        return ops.mrotary_embedding(positions, query, key, self.cos_sin_cache, self.mrope_section)
+
+
+@lru_cache(1)
+def get_mrope(head_size: int, rotary_dim: int, max_position: int, base: float,
+              mrope_section: tuple[int, ...] = ops.DEFAULT_MROPE_SECTION) -> MRotaryEmbedding:
+    """Shared instance per configuration, as ``get_rope``."""
+    return MRotaryEmbedding(head_size, rotary_dim, max_position, base, mrope_section)
+
+
 def image_position_delta(old_start: int, new_start: int, time_interval: int = 1) -> tuple[int, int, int]:
     """(dt, dh, dw) when an image's first vision position moves from ``old_start`` to
     ``new_start``: t = start * time_interval, h = start + row, w = start + col
@@ -85,9 +116,17 @@ class MRopeShift:
     def shift_layer(self, k_cache: torch.Tensor, v_cache: torch.Tensor | None, src_slots: torch.Tensor,
                     dst_slots: torch.Tensor | None, delta_thw) -> None:
         """One layer; in place when ``dst_slots`` is None."""
+        if k_cache.dtype == torch.uint8:
+            ops.mrope_shift_layer_fp4(k_cache, v_cache, src_slots, dst_slots, delta_thw, self.mrope_section,
+                                      self.rope_theta)
+            return
         ops.mrope_shift(k_cache, v_cache, src_slots, dst_slots, delta_thw, self.mrope_section, self.rope_theta)
 
     def shift_all_layers(self, kv_cache: torch.Tensor, src_slots: torch.Tensor, dst_slots: torch.Tensor | None,
                          delta_thw) -> None:
-        """Every layer of a ``[2, L, NB, BS, Hk, D]`` cache in one launch."""
+        """Every layer of a ``[2, L, NB, BS, Hk, D]`` (or 4-bit ``[2, L, NB, Hk, BS * 72]``) cache
+        in one launch."""
+        if kv_cache.dtype == torch.uint8:
+            ops.mrope_shift_fp4(kv_cache, src_slots, dst_slots, delta_thw, self.mrope_section, self.rope_theta)
+            return
         ops.mrope_shift_all_layers(kv_cache, src_slots, dst_slots, delta_thw, self.mrope_section, self.rope_theta)

@@ -6,6 +6,7 @@ the CPU are rejected (there is no CPU path in the product).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -185,10 +186,13 @@ def mrope_shift_all_layers(kv_cache: torch.Tensor, src_slots: torch.Tensor, dst_
 # --------------------------------------------------------------------------- prefill
 @dataclass
 class PrefillPlan:
-    """Host plan (numpy int32) plus its device copy and workspace size (bytes)."""
+    """Host plan (numpy int32) plus its device copy and workspace size (bytes), and the key
+    rows and sequences it was built for."""
     host: np.ndarray
     dev: torch.Tensor | None
     workspace_bytes: int
+    total_k: int = 0
+    num_seqs: int = 0
 
     @property
     def host_ptr(self) -> int:
@@ -257,7 +261,7 @@ def build_prefill_plan(cu_seqlens_q, cu_seqlens_k, num_heads: int, num_kv_heads:
     dev = None
     if device is not None:
         dev = torch.from_numpy(plan).pin_memory().to(device, non_blocking=True)
-    return PrefillPlan(host=plan, dev=dev, workspace_bytes=ws)
+    return PrefillPlan(host=plan, dev=dev, workspace_bytes=ws, total_k=int(ck[-1]), num_seqs=nseq)
 
 
 def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor | None,
@@ -547,3 +551,355 @@ def xxh64(data: bytes | np.ndarray, seed: int = 0) -> int:
     arr = np.frombuffer(bytes(data), dtype=np.uint8) if not isinstance(data, np.ndarray) else \
         np.ascontiguousarray(data).reshape(-1).view(np.uint8)
     return int(lib().vlc_xxh64(ctypes.c_void_p(arr.ctypes.data if arr.size else 0), arr.size, seed))
+
+
+# --------------------------------------------------------------------------- several-axes rotary
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _on_device_of(first: torch.Tensor, *others: torch.Tensor | None):
+    """Context in which the tensors' (one) device is the current one."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError("vlcache_b200 ops run on CUDA tensors only (no CPU fallback)")
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}: one call takes one device")
+    return _SAME_DEVICE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _rows(t: torch.Tensor, name: str) -> None:
+    """``t`` is bf16 [N, heads, D] with contiguous heads (any token stride)."""
+    _need(t.dtype == torch.bfloat16 and t.dim() == 3, f"{name}: bf16 [tokens, heads, head_dim]")
+    n, h, d = t.shape
+    _need(t.stride(2) == 1 and (h == 1 or t.stride(1) == d), f"{name}: the heads of a token must be contiguous")
+
+
+def _token_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _rotary_args(positions, query, key, cos_sin_cache, sections):
+    """Checks shared by the rotating ops; returns (axes, sections array, axis stride, table rows)."""
+    _rows(query, "query")
+    _rows(key, "key")
+    n, _, d = query.shape
+    _need(key.shape[0] == n and key.shape[2] == d, "query and key: the same tokens and head_dim")
+    if sections is None:
+        _need(positions.dim() == 1, "positions [tokens] (or [axes, tokens] with mrope_section)")
+        sections = (d // 2,)
+    sections = tuple(int(x) for x in sections)
+    axes = len(sections)
+    _need(positions.shape == (axes, n) or (axes == 1 and positions.shape == (n,)), f"positions: [{axes}, {n}]")
+    _need(positions.dtype == torch.int64 and (n <= 1 or positions.stride(-1) == 1), "positions: int64, tokens contiguous")
+    _need(cos_sin_cache.dtype == torch.float32 and cos_sin_cache.is_contiguous()
+          and cos_sin_cache.shape[-1] == d and cos_sin_cache.numel() == cos_sin_cache.shape[0] * d,
+          "cos_sin_cache: contiguous fp32 [positions, (1,) head_dim]")
+    stride = positions.stride(0) if axes > 1 else n   # 0: one row of positions for every axis
+    return axes, (ctypes.c_int32 * axes)(*sections), stride, cos_sin_cache.shape[0]
+
+
+def _q_out(query: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    _rows(out, "out")
+    _need(out.shape == query.shape, "out: query's shape")
+    return out
+
+
+def _slots(slot_mapping: torch.Tensor, n: int) -> None:
+    _need(slot_mapping.dtype == torch.int32 and slot_mapping.numel() == n and slot_mapping.is_contiguous(),
+          "slot_mapping: contiguous int32, one per token")
+
+
+def mrotary_embedding(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, cos_sin_cache: torch.Tensor,
+                      mrope_section=DEFAULT_MROPE_SECTION) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotate-half RoPE of ``query`` [N, H, D] and ``key`` [N, Hk, D] at ``positions``
+    [axes, N] (time, height, width): pair j takes the position of the axis whose section of
+    ``mrope_section`` (pairs per axis, summing to D / 2) holds it.  Returns new tensors;
+    with equal positions on all axes they are ``rotary_embedding``'s, bit for bit."""
+    with _on_device_of(query, positions, key, cos_sin_cache):
+        axes, sec, stride, max_pos = _rotary_args(positions, query, key, cos_sin_cache, mrope_section)
+        n, h, d = query.shape
+        hk = key.shape[1]
+        q_out, k_out = _q_out(query, None), torch.empty(key.shape, dtype=key.dtype, device=key.device)
+        st = lib().vlc_mrope_store_kvcache(_ptr(positions), stride, axes, sec, _ptr(query), _token_stride(query),
+                                           _ptr(q_out), h * d, _ptr(key), _token_stride(key), None, 0,
+                                           _ptr(cos_sin_cache), max_pos, None, None, None, 0, _ptr(k_out), hk * d, n,
+                                           h, hk, d, _stream())
+    check("vlc_mrope_store_kvcache", st)
+    return q_out, k_out
+
+
+def mrope_store_kvcache(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                        cos_sin_cache: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                        slot_mapping: torch.Tensor, mrope_section=DEFAULT_MROPE_SECTION,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """``mrotary_embedding`` fused with the paged KV scatter, in one launch: returns the
+    rotated query (into ``out`` when given; it may be ``query``) and writes the rotated key
+    and the value rows to ``k_cache`` / ``v_cache`` row ``slot_mapping[i]`` (-1 skipped)."""
+    with _on_device_of(query, positions, key, value, cos_sin_cache, k_cache, v_cache, slot_mapping, out):
+        axes, sec, stride, max_pos = _rotary_args(positions, query, key, cos_sin_cache, mrope_section)
+        n, h, d = query.shape
+        hk = key.shape[1]
+        _rows(value, "value")
+        _need(value.shape == key.shape, "value: key's shape")
+        _need(k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16 and k_cache.is_contiguous()
+              and v_cache.is_contiguous() and k_cache.shape == v_cache.shape and k_cache.shape[-2:] == (hk, d),
+              "k_cache / v_cache: contiguous bf16 [.., num_kv_heads, head_dim]")
+        _slots(slot_mapping, n)
+        out = _q_out(query, out)
+        st = lib().vlc_mrope_store_kvcache(_ptr(positions), stride, axes, sec, _ptr(query), _token_stride(query),
+                                           _ptr(out), _token_stride(out), _ptr(key), _token_stride(key), _ptr(value),
+                                           _token_stride(value), _ptr(cos_sin_cache), max_pos, _ptr(k_cache),
+                                           _ptr(v_cache), _ptr(slot_mapping), k_cache.numel() // (hk * d), None, 0, n,
+                                           h, hk, d, _stream())
+    check("vlc_mrope_store_kvcache", st)
+    return out
+
+
+# --------------------------------------------------------------------------- the KV cache in 4 bits
+FP4_ROW_BYTES = 72   # of one head's row: 64 of e2m1 codes, 8 of e4m3 scales (include/vlcache_b200.h)
+
+
+def _fp4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dims=(3,)) -> tuple[int, int, int]:
+    """(pages, KV heads, block size) of 4-bit caches uint8 [(layers,) pages, Hk, block * 72]."""
+    for t in (k_cache, v_cache):
+        _need(t.dtype == torch.uint8 and t.dim() in dims, "a 4-bit cache is uint8 [pages, num_kv_heads, block_size * 72]")
+        _need(t[0].is_contiguous() if t.dim() == 4 else t.is_contiguous(), "4-bit caches must be contiguous")
+    _need(k_cache.shape == v_cache.shape, "k_cache and v_cache: the same shape")
+    pages, hk, row = k_cache.shape[-3:]
+    _need(row % FP4_ROW_BYTES == 0 and row > 0, "a 4-bit page is block_size * 72 bytes a head")
+    return pages, hk, row // FP4_ROW_BYTES
+
+
+def _tables(block_tables: torch.Tensor, num_seqs: int) -> tuple[int, int]:
+    """(row stride, width) of int32 block tables [num_seqs, width]."""
+    _need(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == num_seqs,
+          f"block_tables: int32 [{num_seqs}, width]")
+    width = block_tables.shape[1]
+    _need(width <= 1 or block_tables.stride(1) == 1, "block_tables: rows must be contiguous")
+    return (block_tables.stride(0) if num_seqs > 1 else width), width
+
+
+def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      slot_mapping: torch.Tensor, k_scale: float = 1.0, v_scale: float = 1.0) -> None:
+    """``store_kvcache`` into a 4-bit cache (uint8 [pages, Hk, block * 72]): each group of 16
+    dims becomes e2m1 codes and an e4m3 scale.  ``k_scale`` / ``v_scale``: the cache's
+    powers of two (include/vlcache_b200.h says how values are held)."""
+    with _on_device_of(key, value, k_cache, v_cache, slot_mapping):
+        _rows(key, "key")
+        _rows(value, "value")
+        n, hk, d = key.shape
+        _need(value.shape == key.shape, "value: key's shape")
+        pages, heads, block = _fp4_caches(k_cache, v_cache)
+        _need(heads == hk, "the caches' num_kv_heads")
+        _slots(slot_mapping, n)
+        st = lib().vlc_store_kvcache_fp4(_ptr(key), _token_stride(key), _ptr(value), _token_stride(value),
+                                         _ptr(k_cache), _ptr(v_cache), _ptr(slot_mapping), pages, block,
+                                         float(k_scale), float(v_scale), n, hk, d, _stream())
+    check("vlc_store_kvcache_fp4", st)
+
+
+def rope_store_kvcache_fp4(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                           cos_sin_cache: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           slot_mapping: torch.Tensor, mrope_section=None, k_scale: float = 1.0,
+                           v_scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``rope_store_kvcache`` (or, with ``mrope_section``, ``mrope_store_kvcache``) into a 4-bit
+    cache, in one launch: returns the rotated query; the rotated key, rounded to bf16, and
+    the value are quantised into row ``slot_mapping[i]`` (-1 skipped), the same bytes as
+    rotating first and ``store_kvcache_fp4`` after."""
+    with _on_device_of(query, positions, key, value, cos_sin_cache, k_cache, v_cache, slot_mapping, out):
+        axes, sec, stride, max_pos = _rotary_args(positions, query, key, cos_sin_cache, mrope_section)
+        n, h, d = query.shape
+        hk = key.shape[1]
+        _rows(value, "value")
+        _need(value.shape == key.shape, "value: key's shape")
+        pages, heads, block = _fp4_caches(k_cache, v_cache)
+        _need(heads == hk, "the caches' num_kv_heads")
+        _slots(slot_mapping, n)
+        out = _q_out(query, out)
+        st = lib().vlc_rope_store_kvcache_fp4(_ptr(positions), stride, axes, sec, _ptr(query), _token_stride(query),
+                                              _ptr(out), _token_stride(out), _ptr(key), _token_stride(key),
+                                              _ptr(value), _token_stride(value), _ptr(cos_sin_cache), max_pos,
+                                              _ptr(k_cache), _ptr(v_cache), _ptr(slot_mapping), pages, block,
+                                              float(k_scale), float(v_scale), n, h, hk, d, _stream())
+    check("vlc_rope_store_kvcache_fp4", st)
+    return out
+
+
+def gather_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                       cu_seqlens_k: torch.Tensor, total_k: int, k_scale: float = 1.0, v_scale: float = 1.0,
+                       k_out: torch.Tensor | None = None,
+                       v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values of a 4-bit cache's keys and values, in bf16 (exact): row cu_seqlens_k[b] + j
+    of the outputs [total_k, Hk, 128] is key j of sequence b.  With caches of several layers
+    ([layers, pages, Hk, block * 72], e.g. ``kv_cache[0]``, ``kv_cache[1]``) the outputs are
+    [layers, total_k, Hk, 128].  ``total_k`` is cu_seqlens_k's last entry, on the host."""
+    with _on_device_of(k_cache, v_cache, block_tables, cu_seqlens_k, k_out, v_out):
+        pages, hk, block = _fp4_caches(k_cache, v_cache, dims=(3, 4))
+        layers = k_cache.shape[0] if k_cache.dim() == 4 else 1
+        layer_stride = k_cache.stride(0) if k_cache.dim() == 4 and layers > 1 else 0
+        _need(k_cache.dim() == 3 or layers <= 1 or k_cache.stride(0) == v_cache.stride(0),
+              "k_cache and v_cache: the same layer stride")
+        _need(cu_seqlens_k.dtype == torch.int32 and cu_seqlens_k.dim() == 1 and cu_seqlens_k.is_contiguous()
+              and cu_seqlens_k.numel() >= 1, "cu_seqlens_k: contiguous int32 [num_seqs + 1]")
+        seqs = cu_seqlens_k.numel() - 1
+        stride, width = _tables(block_tables, seqs)
+        shape = (total_k, hk, HEAD_DIM) if k_cache.dim() == 3 else (layers, total_k, hk, HEAD_DIM)
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
+        if v_out is None:
+            v_out = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
+        for t in (k_out, v_out):
+            _need(t.shape == shape and t.dtype == torch.bfloat16 and t.is_contiguous(),
+                  f"k_out / v_out: contiguous bf16 {list(shape)}")
+        row = hk * HEAD_DIM
+        st = lib().vlc_gather_kvcache_fp4(_ptr(k_cache), _ptr(v_cache), layer_stride, layers, pages, block, hk,
+                                          HEAD_DIM, _ptr(block_tables), stride, width, _ptr(cu_seqlens_k), seqs,
+                                          total_k, float(k_scale), float(v_scale), _ptr(k_out), _ptr(v_out), row,
+                                          total_k * row, _stream())
+    check("vlc_gather_kvcache_fp4", st)
+    return k_out, v_out
+
+
+def _shift_fp4(k, v, layers, layer_stride, src_slots, dst_slots, delta_thw, mrope_section, rope_theta) -> int:
+    pages, hk, block = _fp4_caches(k, k if v is None else v, dims=(3, 4))
+    n = src_slots.numel()
+    for t in (src_slots, dst_slots):
+        _need(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n),
+              "src_slots / dst_slots: contiguous int32 of one length")
+    d = (ctypes.c_int32 * 3)(*[int(x) for x in delta_thw])
+    sec = (ctypes.c_int32 * 3)(*[int(x) for x in mrope_section])
+    return lib().vlc_mrope_shift_fp4(_ptr(k), _ptr(v), layer_stride, layers, pages, block, hk, HEAD_DIM,
+                                     _ptr(src_slots), _ptr(dst_slots), n, d, sec, float(rope_theta), _stream())
+
+
+def mrope_shift_fp4(kv_cache: torch.Tensor, src_slots: torch.Tensor, dst_slots: torch.Tensor | None, delta_thw,
+                    mrope_section=DEFAULT_MROPE_SECTION, rope_theta: float = 1e6) -> None:
+    """``mrope_shift_all_layers`` in a 4-bit cache uint8 [2, L, pages, Hk, block * 72], one
+    launch: K rows of ``src_slots`` turned by the position delta to ``dst_slots`` (None: in
+    place), V rows copied.  A turned row is rounded to bf16 and quantised again; groups of
+    16 pairs whose delta is 0 keep their bits, so a zero delta copies.  No destination may
+    be another row's source (``engine.kv_cache.check_reuse_slots``)."""
+    with _on_device_of(kv_cache, src_slots, dst_slots):
+        _need(kv_cache.dim() == 5 and kv_cache.shape[0] == 2 and kv_cache.is_contiguous(),
+              "kv_cache: contiguous uint8 [2, layers, pages, Hk, block * 72]")
+        st = _shift_fp4(kv_cache[0], kv_cache[1], kv_cache.shape[1], kv_cache.stride(1), src_slots, dst_slots,
+                        delta_thw, mrope_section, rope_theta)
+    check("vlc_mrope_shift_fp4", st)
+
+
+def mrope_shift_layer_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor | None, src_slots: torch.Tensor,
+                          dst_slots: torch.Tensor | None, delta_thw, mrope_section=DEFAULT_MROPE_SECTION,
+                          rope_theta: float = 1e6) -> None:
+    """``mrope_shift_fp4`` of one layer's caches uint8 [pages, Hk, block * 72] (``v_cache`` None:
+    K alone)."""
+    with _on_device_of(k_cache, v_cache, src_slots, dst_slots):
+        _need(k_cache.dim() == 3, "a 4-bit cache is uint8 [pages, num_kv_heads, block_size * 72]")
+        st = _shift_fp4(k_cache, v_cache, 1, 0, src_slots, dst_slots, delta_thw, mrope_section, rope_theta)
+    check("vlc_mrope_shift_fp4", st)
+
+
+def decode_fp4_workspace_bytes(num_seqs: int, num_heads: int, num_kv_heads: int, max_context_len: int) -> int:
+    return int(lib().vlc_decode_fp4_workspace_size(num_seqs, num_heads, num_kv_heads, max_context_len))
+
+
+def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                         context_lens: torch.Tensor, max_context_len: int, softmax_scale: float,
+                         k_scale: float = 1.0, v_scale: float = 1.0, out: torch.Tensor | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``decode_attention`` over a 4-bit cache: one query token per sequence, q / out [B, H, 128]
+    (q may be [B, 1, H, 128]); sequences of length 0 give zeros.  ``max_context_len`` bounds
+    the lengths on the host and sizes the grid; ``workspace`` as ``decode_fp4_workspace_bytes``."""
+    with _on_device_of(q, k_cache, v_cache, block_tables, context_lens, out, workspace):
+        if q.dim() == 4:
+            _need(q.shape[1] == 1, "q: one token per sequence")
+            q = q.squeeze(1)
+        _rows(q, "q")
+        b, h, d = q.shape
+        pages, hk, block = _fp4_caches(k_cache, v_cache)
+        stride, width = _tables(block_tables, b)
+        _need(context_lens.dtype == torch.int32 and context_lens.numel() == b and context_lens.is_contiguous(),
+              "context_lens: contiguous int32, one per sequence")
+        out = _q_out(q, out)
+        need = decode_fp4_workspace_bytes(b, h, hk, max_context_len)
+        if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        st = lib().vlc_decode_attn_fp4(_ptr(q), _token_stride(q), b, h, _ptr(k_cache), _ptr(v_cache), pages, block, hk,
+                                       d, _ptr(block_tables), stride, width, _ptr(context_lens), int(max_context_len),
+                                       float(softmax_scale), float(k_scale), float(v_scale), _ptr(out),
+                                       _token_stride(out), _ptr(workspace), ws_bytes, _stream())
+    check("vlc_decode_attn_fp4", st)
+    return out
+
+
+def prefill_fp4_workspace_bytes(plan: PrefillPlan, num_kv_heads: int) -> int:
+    """Workspace of ``prefill_attention_fp4``: the plan's, and the keys and values in bf16."""
+    return _round_up(plan.workspace_bytes, 256) + 2 * plan.total_k * num_kv_heads * HEAD_DIM * 2
+
+
+def _round_up(n: int, to: int) -> int:
+    return (n + to - 1) // to * to
+
+
+def prefill_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                          cu_seqlens_k: torch.Tensor, plan: PrefillPlan, softmax_scale: float, k_scale: float = 1.0,
+                          v_scale: float = 1.0, out: torch.Tensor | None = None,
+                          workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``prefill_attention`` over a 4-bit cache: the sequences' keys and values are read back
+    to bf16 once (``gather_kvcache_fp4``, exact), then the tcgen05 attention kernel runs on
+    them.  A prompt's query tiles share each key, so one conversion per key costs less than
+    one per tile, and the dense rows mostly stay in L2.  ``cu_seqlens_k``: the plan's, on the
+    device; ``workspace``: uint8, ``prefill_fp4_workspace_bytes``."""
+    with _on_device_of(q, k_cache, v_cache, block_tables, cu_seqlens_k, out, workspace):
+        _rows(q, "q")
+        pages, hk, block = _fp4_caches(k_cache, v_cache)
+        _need(cu_seqlens_k.numel() == plan.num_seqs + 1, "cu_seqlens_k: the plan's sequences")
+        need = prefill_fp4_workspace_bytes(plan, hk)
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        workspace = workspace.view(-1).view(torch.uint8)
+        at = _round_up(plan.workspace_bytes, 256)
+        kv = workspace[at:need].view(torch.bfloat16).view(2, plan.total_k, hk, HEAD_DIM)
+        gather_kvcache_fp4(k_cache, v_cache, block_tables, cu_seqlens_k, plan.total_k, k_scale, v_scale, kv[0], kv[1])
+        return prefill_attention(q, kv[0], kv[1], None, plan, softmax_scale, out=out, workspace=workspace[:at])
+
+
+# --------------------------------------------------------------------------- pages
+def copy_kv_pages(kv_cache: torch.Tensor, src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
+    """Page ``dst_pages[i]`` becomes a copy of page ``src_pages[i]`` in every layer's K and V, in
+    one launch: ``kv_cache[:, :, dst] = kv_cache[:, :, src]`` for a cache [2, L, pages, ...] of
+    either format.  Pages of the lists (device int32) are copied in no order: destinations
+    differ and none is another pair's source (``engine.page_pool`` makes such lists); pairs
+    of -1 are skipped."""
+    with _on_device_of(kv_cache, src_pages, dst_pages):
+        _need(kv_cache.dim() >= 4 and kv_cache.is_contiguous(), "kv_cache: contiguous [2, layers, pages, ...]")
+        n = src_pages.numel()
+        for t in (src_pages, dst_pages):
+            _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n,
+                  "src_pages / dst_pages: contiguous int32 of one length")
+        planes, pages = kv_cache.shape[0] * kv_cache.shape[1], kv_cache.shape[2]
+        item = kv_cache.element_size()
+        st = lib().vlc_copy_pages(_ptr(kv_cache), kv_cache.stride(1) * item, planes, kv_cache.stride(2) * item, pages,
+                                  _ptr(src_pages), _ptr(dst_pages), n, _stream())
+    check("vlc_copy_pages", st)
+
+
+def remap_block_tables(block_tables: torch.Tensor, page_map: torch.Tensor) -> None:
+    """Every entry p of the device block tables becomes ``page_map[p]`` (int32 [pages]); -1 stays."""
+    with _on_device_of(block_tables, page_map):
+        _need(block_tables.dtype == torch.int32 and block_tables.dim() == 2, "block_tables: int32 [rows, width]")
+        rows, width = block_tables.shape
+        _need(width <= 1 or block_tables.stride(1) == 1, "block_tables: rows must be contiguous")
+        _need(page_map.dtype == torch.int32 and page_map.dim() == 1 and page_map.is_contiguous(),
+              "page_map: contiguous int32 [pages]")
+        st = lib().vlc_remap_block_tables(_ptr(block_tables), block_tables.stride(0) if rows > 1 else width, rows,
+                                          width, _ptr(page_map), page_map.numel(), _stream())
+    check("vlc_remap_block_tables", st)
