@@ -14,15 +14,21 @@
 //   * e2m1 pairs convert to f16 pairs in one instruction and one multiplication by the scale makes
 //     the exact value; V pairs hold the same dim of two keys, made by exchanging nibbles first.
 //   * P^T in the layout of a B operand is S^T's accumulator transposed: one movmatrix an 8 x 8 tile.
-// Layout of the work: grid (split of the keys, KV head, sequence), a warp takes chunks of CH keys
-// of the CTA's split through a ring of its own (TMA tiles with the 64-byte swizzle for the codes,
-// plain bulk copies for the scales), with its own running maximum and sum; the warps of a CTA join
-// through shared memory, the splits in decode_fp4_combine_kernel.
+// Layout of the work: the keys of all (sequence, KV head) pairs, in chunks of 64, form one line that
+// the grid's warps share out evenly, each a contiguous run of it.  The shares are equal whatever
+// the lengths are (a grid of fixed splits left SMs idle at its end, paid a prologue and a join
+// every few chunks and merged in shared memory: 267 us for 256 sequences of 2700 .. 10700 keys, 28
+// query and 4 KV heads, against 196 us now).  A warp works alone: its own ring of chunks (TMA
+// tiles with the 64-byte swizzle for the codes, plain bulk copies for the scales, issued by its
+// lane 0), its own running maximum and sums, no barrier with any other warp.  A pair that a warp
+// has to itself is written out; the parts of a pair that several warps share go to the workspace
+// and decode_fp4_combine_kernel, launched as a programmatic dependent, joins them.
 //
 // f16 operands: K and V are exact in f16.  q is scaled per head by a power of two that puts its
 // largest element in [2^14, 2^15), so elements down to 2^-28 of it convert exactly; the power goes
-// into the softmax scale.  P is 2^15 exp(s - max), so that it rounds to 11 bits down to 2^-29 of
-// the largest; the factor is in P's sum too and cancels.  Sums are fp32.
+// into the softmax scale.  P is 2^12 exp(s - m) with m within 2^3 of the running maximum, so that it
+// rounds to 11 bits down to 2^-26 of the largest; the factor is in P's sum too (an MMA with ones
+// takes it) and cancels.  Sums are fp32.
 #include <algorithm>
 #include <cmath>
 
@@ -35,15 +41,19 @@ namespace decode_fp4 {
 using fp4::HD;
 constexpr int CH = 64;                          // keys a step of a warp
 constexpr int TILES = CH / 16;
-constexpr int WARPS = 4;
-constexpr int STAGES = 3;
+constexpr int WARPS = 2;                        // a block's warps share nothing but the launch
+constexpr int STAGES = 2;
 constexpr int CODE_TILE = CH * fp4::CODE_BYTES;
 constexpr int SCALE_TILE = CH * fp4::SCALE_BYTES;
 constexpr int STAGE_BYTES = 2 * (CODE_TILE + SCALE_TILE);
-constexpr int RING_BYTES = WARPS * STAGES * STAGE_BYTES;
-constexpr int SMEM_BYTES = RING_BYTES + 1024;
+constexpr int SMEM_BYTES = WARPS * STAGES * STAGE_BYTES + 512;  // + alignment to the swizzle's period
 constexpr int MAX_GROUP = 16;
-constexpr float P_SHIFT = 15.f;
+constexpr int MIN_SHARE = 2;                    // chunks a warp takes at least
+constexpr float P_SHIFT = 12.f;
+constexpr float SLACK = 3.f;                    // log2 that the maximum may grow by before O is rescaled
+
+// Blocks an SM holds: 12 warps of up to 168 registers with 8 query heads, 8 warps with 16.
+constexpr int blocks_per_sm(int NT) { return NT == 1 ? 6 : 4; }
 
 struct Params {
   CUtensorMap tm_k, tm_v;  // bytes {64, block_size, pages * Hk}, box {64, CH, 1}
@@ -57,14 +67,15 @@ struct Params {
   int block_size;
   int num_pages;
   const int32_t* context_lens;
-  int split_keys, max_splits;
+  int num_seqs, max_len;
   int group, num_heads, num_kv_heads;
-  float scale_log2;  // softmax scale * log2(e) * g_k
+  float scale_log2;  // |softmax scale| * log2(e) * g_k
+  float q_sign;      // the softmax scale's sign
   float v_scale;
   __nv_bfloat16* out;
   int64_t out_seq_stride;
-  float* part_o;   // [num_seqs][max_splits][num_heads][HD]
-  float* part_ml;  // [num_seqs][max_splits][num_heads][2]
+  int num_warps;
+  float* parts;  // [num_warps][2][group][HD] sums, then [num_warps][2][group][2] (maximum, sum of P)
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -117,154 +128,74 @@ __device__ __forceinline__ uint32_t swizzled(int key, int piece) {
   return key * 64 + ((piece ^ ((key >> 1) & 3)) << 4);
 }
 
+// Chunks of a sequence.  A length past the host's bound is cut to it (recorded by the caller).
+__device__ __forceinline__ int chunks_of(int len, int max_len) { return (min(max(len, 0), max_len) + CH - 1) / CH; }
+
+// How the line of chunks is shared: chunks a warp, from the total and the warps of the grid.
+__device__ __forceinline__ int64_t share_of(int64_t total, int num_warps) {
+  return max((total + num_warps - 1) / num_warps, (int64_t)MIN_SHARE);
+}
+
+// A query head group's state of a warp: S^T, O^T and the softmax, and the step over one chunk.
 template <int NT>  // 8-head column tiles
-__global__ void __launch_bounds__(WARPS * 32, 2) decode_fp4_kernel(const __grid_constant__ Params p) {
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_all[WARPS * STAGES];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int split = blockIdx.x, g = blockIdx.y, b = blockIdx.z;
-  const int G = p.group;
-  int len = __ldg(p.context_lens + b);
-  // As in the bf16 decode: a length past the keys that the grid covers is recorded and cut.
-  const int cap = p.max_splits * p.split_keys;
-  if (len > cap) {
-    if (split == 0 && g == 0 && threadIdx.x == 0) record_error(VLC_DEV_ERR_LENGTH);
-    len = cap;
-  }
-  const int nsplit = len > 0 ? (len + p.split_keys - 1) / p.split_keys : 0;
-  if (split >= nsplit) {
-    if (len <= 0 && split == 0) {  // an empty sequence: zeros
-      for (int i = threadIdx.x; i < G * HD / 2; i += blockDim.x)
-        reinterpret_cast<uint32_t*>(p.out + (int64_t)b * p.out_seq_stride + (int64_t)g * G * HD)[i] = 0;
-    }
-    return;
-  }
-  const int warp = warp_id(), lane = lane_id();
-  const int r = lane >> 2, t = lane & 3;
-  uint64_t* const full = full_all + warp * STAGES;
-  if (lane == 0) {
-#pragma unroll
-    for (int s = 0; s < STAGES; ++s) mbar_init(full + s, 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
+struct State {
+  uint32_t qb[NT][16];      // Q as B fragments: dims 32t .. 32t + 31 of head r (and 8 + r)
+  float scale[NT][2];       // of scores, heads 2t and 2t + 1
+  float o[NT][8][4];        // m-tile i: dims 16r + 2i (0, 1) and 16r + 2i + 1 (2, 3) of heads 2t, 2t + 1
+  float l[NT][4];           // sums of P: 0 and 1 of heads 2t, 2t + 1
+  float m[NT][2];           // the maximum that P is relative to
 
-  const int k_begin = split * p.split_keys;
-  const int k_end = min(len, k_begin + p.split_keys);
-  const int nchunks = (k_end - k_begin + CH - 1) / CH;
-  const int mine = nchunks > warp ? (nchunks - warp + WARPS - 1) / WARPS : 0;  // chunks warp, warp + WARPS, ..
-  uint8_t* const ring = smem + warp * (STAGES * STAGE_BYTES);
-  const int32_t* const table = p.block_tables + (int64_t)b * p.table_stride;
-
-  // Page of the warp's i-th chunk, or -1 when the table has no usable page there: such a chunk is
-  // recorded and left out.
-  auto page_of = [&](int i) {
-    const int index = (k_begin + (warp + i * WARPS) * CH) / p.block_size;
-    const int page = index < p.table_width ? __ldg(table + index) : -1;
-    return page >= 0 && page < p.num_pages ? page : -1;
-  };
-  auto issue = [&](int i) {  // one lane
-    const int page = page_of(i);
-    if (page < 0) {
-      record_error(VLC_DEV_ERR_BLOCK_RANGE);
-      return;
-    }
-    uint64_t* bar = full + i % STAGES;
-    uint8_t* st = ring + (i % STAGES) * STAGE_BYTES;
-    const int row = (k_begin + (warp + i * WARPS) * CH) % p.block_size;
-    const int piece = page * p.num_kv_heads + g;
-    const int64_t scales = fp4::head_offset(page, p.num_kv_heads, g, p.block_size) +
-                           fp4::scale_offset(row, p.block_size);
-    mbar_expect_tx(bar, STAGE_BYTES);
-    tma_load_3d(st, &p.tm_k, bar, 0, row, piece);
-    bulk_load_1d(st + 2 * CODE_TILE, p.k_cache + scales, SCALE_TILE, bar);
-    tma_load_3d(st + CODE_TILE, &p.tm_v, bar, 0, row, piece);
-    bulk_load_1d(st + 2 * CODE_TILE + SCALE_TILE, p.v_cache + scales, SCALE_TILE, bar);
-  };
-  auto arrived = [&](int i) {
-    const bool ok = mbar_wait_bounded(full + i % STAGES, (uint32_t)(i / STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 22,
-                                      VLC_WAIT_LIMIT_CYCLES);
-    return __all_sync(0xffffffffu, ok) != 0;
-  };
-  if (lane == 0) {
-    for (int i = 0; i < min(STAGES, mine); ++i) issue(i);
-  }
-
-  // Q as B fragments: lane (r, t) holds dims 32t .. 32t + 31 of head r (and 8 + r); head powers.
-  uint32_t qb[NT][16];
-  float head_scale[NT][2];  // of heads 2t and 2t + 1
+  __device__ __forceinline__ void start(const __nv_bfloat16* q, int G, int r, int t, float scale_log2, float sign) {
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int h = n * 8 + r;
-    uint4 u[4] = {};
-    if (h < G) {
-      const uint4* src =
-          reinterpret_cast<const uint4*>(p.q + (int64_t)b * p.q_seq_stride + (int64_t)(g * G + h) * HD + 32 * t);
+    for (int n = 0; n < NT; ++n) {
+      const int h = n * 8 + r;
+      uint4 u[4] = {};
+      if (h < G) {
+        const uint4* src = reinterpret_cast<const uint4*>(q + (int64_t)h * HD + 32 * t);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = __ldg(src + i);
-    }
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(u);
-    uint32_t top = 0;  // largest bf16 magnitude
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^(141 - e) for a largest element with exponent field e puts it in [2^14, 2^15); e is kept
-    // where both that power and its inverse are normal.  All-zero and non-finite rows: power 1.
-    int e = (int)(top >> 7);
-    e = (top == 0 || e == 255) ? 141 : max(e, 15);
-    const float up = __uint_as_float((uint32_t)(127 + 141 - e) << 23);
-    const float down = __uint_as_float((uint32_t)(127 - 141 + e) << 23);
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      qb[n][i] = pack_f16x2(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up);
-    head_scale[n][0] = p.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t);      // lane of head 2t
-    head_scale[n][1] = p.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t + 4);  // of head 2t + 1
-  }
-
-  float o[NT][8][4];
-  float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.f;
-  }
-  const uint32_t ring_u = smem_u32(ring);
-  const int kr = tile_key(r);
-  // V fragment columns 2t, 2t + 1 (and 8 more): keys of S^T's rows 2t and 2t + 1
-  const int kv0 = tile_key(2 * t), kv1 = tile_key(2 * t + 1);
-
-  for (int i = 0; i < mine; ++i) {
-    if (page_of(i) < 0) {
-      if (lane == 0) {
-        mbar_arrive(full + i % STAGES);  // nothing was issued: the barrier's phase is turned over here
-        if (i + STAGES < mine) issue(i + STAGES);
+        for (int i = 0; i < 4; ++i) u[i] = __ldg(src + i);
       }
-      __syncwarp();
-      continue;
+      const uint32_t w[16] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w,
+                              u[2].x, u[2].y, u[2].z, u[2].w, u[3].x, u[3].y, u[3].z, u[3].w};
+      uint32_t top = 0;  // largest bf16 magnitude
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^(141 - e) for a largest element with exponent field e puts it in [2^14, 2^15); e is kept
+      // where both that power and its inverse are normal.  All-zero and non-finite rows: power 1.
+      int e = (int)(top >> 7);
+      e = (top == 0 || e == 255) ? 141 : max(e, 15);
+      const float up = __uint_as_float((uint32_t)(127 + 141 - e) << 23) * sign;
+      const float down = __uint_as_float((uint32_t)(127 - 141 + e) << 23);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        qb[n][i] = pack_f16x2(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up);
+      scale[n][0] = scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t);      // lane of head 2t
+      scale[n][1] = scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t + 4);  // of head 2t + 1
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      l[n][0] = l[n][1] = l[n][2] = l[n][3] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
     }
-    if (!arrived(i)) {  // recorded; the copies still in flight are given the same time before the warp leaves
-      for (int x = i + 1; x < min(i + STAGES, mine); ++x)
-        if (page_of(x) >= 0) arrived(x);
-      break;
-    }
-    const uint32_t st = ring_u + (i % STAGES) * STAGE_BYTES;
-    const int valid = k_end - (k_begin + (warp + i * WARPS) * CH);  // keys of the chunk that count
+  }
 
+  // One chunk at `st`.  CUT: only its first `valid` keys count.
+  template <bool CUT>
+  __device__ __forceinline__ void step(uint32_t st, int valid, int r, int t) {
+    const int kr = tile_key(r);
+    const uint32_t k_codes = st + swizzled(kr, t), k_scales = st + 2 * CODE_TILE + kr * 8 + 2 * t;
     // ---- S^T = K Q^T
     float s[TILES][NT][4];
 #pragma unroll
     for (int kt = 0; kt < TILES; ++kt) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) s[kt][n][0] = s[kt][n][1] = s[kt][n][2] = s[kt][n][3] = 0.f;
-      const int k0 = kt * 16 + kr, k1 = k0 + 8;
-      uint32_t c0[4], c1[4];
-      lds128(st + swizzled(k0, t), c0);
-      lds128(st + swizzled(k1, t), c1);
-      const uint32_t f0 = fp4::scales2_f16(lds_u16(st + 2 * CODE_TILE + k0 * 8 + 2 * t));
-      const uint32_t f1 = fp4::scales2_f16(lds_u16(st + 2 * CODE_TILE + k1 * 8 + 2 * t));
+      uint32_t c0[4], c1[4];  // keys kr and kr + 8 of the tile (8 keys on, the swizzle is the same)
+      lds128(k_codes + kt * 1024, c0);
+      lds128(k_codes + kt * 1024 + 512, c1);
+      const uint32_t f0 = fp4::scales2_f16(lds_u16(k_scales + kt * 128));
+      const uint32_t f1 = fp4::scales2_f16(lds_u16(k_scales + kt * 128 + 64));
 #pragma unroll
       for (int w = 0; w < 4; ++w) {  // four bytes: k-steps 2w and 2w + 1
         const uint32_t sc0 = __byte_perm(f0, 0, w < 2 ? 0x1010 : 0x3232);
@@ -286,7 +217,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) decode_fp4_kernel(const __grid_
         }
       }
     }
-    // ---- running softmax, log2 domain; lane holds keys of rows r, r + 8 for heads 2t, 2t + 1
+    // ---- running softmax, log2 domain; a lane holds keys of rows r, r + 8 for heads 2t, 2t + 1
     uint32_t pb[TILES][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -294,65 +225,76 @@ __global__ void __launch_bounds__(WARPS * 32, 2) decode_fp4_kernel(const __grid_
 #pragma unroll
       for (int kt = 0; kt < TILES; ++kt) {
         float(&x)[4] = s[kt][n];
-        x[0] *= head_scale[n][0];
-        x[1] *= head_scale[n][1];
-        x[2] *= head_scale[n][0];
-        x[3] *= head_scale[n][1];
-        if (valid < CH) {
+        if (CUT) {
           if (kt * 16 + kr >= valid) x[0] = x[1] = -INFINITY;
           if (kt * 16 + kr + 8 >= valid) x[2] = x[3] = -INFINITY;
         }
-        top0 = fmaxf(top0, fmaxf(x[0], x[2]));
-        top1 = fmaxf(top1, fmaxf(x[1], x[3]));
+        top0 = fmax3(top0, x[0], x[2]);
+        top1 = fmax3(top1, x[1], x[3]);
       }
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
         top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, d));
         top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, d));
       }
-      const float m0 = fmaxf(m[n][0], top0), m1 = fmaxf(m[n][1], top1);
-      // (-inf: no key so far)
-      const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m[n][0] - m0);
-      const float f1 = m1 == -INFINITY ? 0.f : fast_exp2(m[n][1] - m1);
-      const float r0 = m0 == -INFINITY ? 0.f : m0 - P_SHIFT, r1 = m1 == -INFINITY ? 0.f : m1 - P_SHIFT;
-      m[n][0] = m0;
-      m[n][1] = m1;
-      float l0 = 0.f, l1 = 0.f;
+      top0 *= scale[n][0];
+      top1 *= scale[n][1];
+      if (__any_sync(0xffffffffu, top0 > m[n][0] + SLACK || top1 > m[n][1] + SLACK)) {
+        const float m0 = fmaxf(m[n][0], top0), m1 = fmaxf(m[n][1], top1);
+        const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m[n][0] - m0);  // (-inf: no key so far)
+        const float f1 = m1 == -INFINITY ? 0.f : fast_exp2(m[n][1] - m1);
+        m[n][0] = m0;
+        m[n][1] = m1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          o[n][i][0] *= f0;
+          o[n][i][1] *= f1;
+          o[n][i][2] *= f0;
+          o[n][i][3] *= f1;
+        }
+        l[n][0] *= f0;
+        l[n][1] *= f1;
+      }
+      const float r0 = m[n][0] == -INFINITY ? 0.f : P_SHIFT - m[n][0];
+      const float r1 = m[n][1] == -INFINITY ? 0.f : P_SHIFT - m[n][1];
 #pragma unroll
       for (int kt = 0; kt < TILES; ++kt) {
         float(&x)[4] = s[kt][n];
-        x[0] = fast_exp2(x[0] - r0);
-        x[1] = fast_exp2(x[1] - r1);
-        x[2] = fast_exp2(x[2] - r0);
-        x[3] = fast_exp2(x[3] - r1);
-        l0 += x[0] + x[2];
-        l1 += x[1] + x[3];
+        x[0] = fast_exp2(fmaf(x[0], scale[n][0], r0));
+        x[1] = fast_exp2(fmaf(x[1], scale[n][1], r1));
+        x[2] = fast_exp2(fmaf(x[2], scale[n][0], r0));
+        x[3] = fast_exp2(fmaf(x[3], scale[n][1], r1));
+        if (CUT) {  // (not left to exp2(-inf): a scale of 0 would make it exp2(NaN))
+          if (kt * 16 + kr >= valid) x[0] = x[1] = 0.f;
+          if (kt * 16 + kr + 8 >= valid) x[2] = x[3] = 0.f;
+        }
         pb[kt][n][0] = transpose8x8(pack_f16x2(x[0], x[1]));
         pb[kt][n][1] = transpose8x8(pack_f16x2(x[2], x[3]));
       }
-      l[n][0] = l[n][0] * f0 + l0;
-      l[n][1] = l[n][1] * f1 + l1;
-#pragma unroll
-      for (int mt = 0; mt < 8; ++mt) {
-        o[n][mt][0] *= f0;
-        o[n][mt][1] *= f1;
-        o[n][mt][2] *= f0;
-        o[n][mt][3] *= f1;
-      }
     }
-    // ---- O^T += V^T P^T
+    // ---- O^T += V^T P^T; V's columns 2t, 2t + 1 (and 8 more) are the keys of S^T's rows of that number
+    const int kv[2] = {tile_key(2 * t), tile_key(2 * t + 1)};
+    uint32_t v_codes[2], v_scales[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      v_codes[x] = st + CODE_TILE + swizzled(kv[x], r >> 1) + 8 * (r & 1);
+      v_scales[x] = st + 2 * CODE_TILE + SCALE_TILE + kv[x] * 8 + r;
+    }
+    const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
     for (int kt = 0; kt < TILES; ++kt) {
-      const int key[4] = {kt * 16 + kv0, kt * 16 + kv1, kt * 16 + 8 + kv0, kt * 16 + 8 + kv1};
       uint32_t c[4][2], sb[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        lds64(st + CODE_TILE + swizzled(key[x], r >> 1) + 8 * (r & 1), c[x][0], c[x][1]);
-        sb[x] = lds_u8(st + 2 * CODE_TILE + SCALE_TILE + key[x] * 8 + r);
+        lds64(v_codes[x & 1] + kt * 1024 + (x >> 1) * 512, c[x][0], c[x][1]);
+        sb[x] = lds_u8(v_scales[x & 1] + kt * 128 + (x >> 1) * 64);
         // rows past the end may hold anything: their P is 0, and a scale of 0 makes V 0
-        if (valid < CH && key[x] >= valid) sb[x] = 0;
+        if (CUT && kt * 16 + kv[x & 1] + (x >> 1) * 8 >= valid) sb[x] = 0;
       }
-      const uint32_t sc01 = fp4::scales2_f16(sb[0] | (sb[1] << 8)), sc23 = fp4::scales2_f16(sb[2] | (sb[3] << 8));
+      const uint32_t sc01 = fp4::scales2_f16(__byte_perm(sb[0], sb[1], 0x0040));
+      const uint32_t sc23 = fp4::scales2_f16(__byte_perm(sb[2], sb[3], 0x0040));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_f16(l[n], ones, pb[kt][n][0], pb[kt][n][1]);
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         // bytes of {key 0 or 2, key 1 or 3} x {low nibbles: dims 16r + 2i, high: 16r + 2i + 1}
@@ -373,123 +315,287 @@ __global__ void __launch_bounds__(WARPS * 32, 2) decode_fp4_kernel(const __grid_
         }
       }
     }
-    __syncwarp();  // every lane has read the stage
-    if (lane == 0 && i + STAGES < mine) issue(i + STAGES);
   }
+};
 
-  // ---- join the warps: every copy into the ring was waited for, its memory is free
+template <int NT>
+__global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_all[WARPS * STAGES];
+  __shared__ int valid_all[WARPS * STAGES];
+  pdl_launch_dependents();  // the join waits for this grid's end before it reads
+  const int warp = warp_id(), lane = lane_id();
+  const int r = lane >> 2, t = lane & 3;
+  const int G = p.group, Hk = p.num_kv_heads;
+  const int64_t my = (int64_t)blockIdx.x * WARPS + warp;
+  uint64_t* const full = full_all + warp * STAGES;
+  volatile int* const valid_of = valid_all + warp * STAGES;
+
+  // ---- this warp's run [c0, c1) of the line, and the sequence that c0 lies in
+  int64_t total = 0;
+  for (int i = lane; i < p.num_seqs; i += 32) {
+    const int len = __ldg(p.context_lens + i);
+    if (my == 0 && len > p.max_len) record_error(VLC_DEV_ERR_LENGTH);
+    total += chunks_of(len, p.max_len);
+  }
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int d = 1; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+  total *= Hk;
+  const int64_t share = share_of(total, p.num_warps);
+  const int64_t c0 = my * share;
+  if (my >= p.num_warps || c0 >= total) return;
+  const int count = (int)(min(c0 + share, total) - c0);
+  int seq = 0;
+  int64_t at = c0;  // c0's place among the chunks from the sequence's first on
+  for (int base = 0;; base += 32) {
+    int64_t n = base + lane < p.num_seqs ? (int64_t)chunks_of(__ldg(p.context_lens + base + lane), p.max_len) * Hk : 0;
+    int64_t upto = n;
 #pragma unroll
-    for (int d = 4; d < 32; d <<= 1) {
-      l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], d);
-      l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], d);
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
     }
-  __syncthreads();
-  constexpr int HEADS = NT * 8;
-  float* sm_o = reinterpret_cast<float*>(smem);        // [WARPS][HEADS][HD]
-  float* sm_ml = sm_o + WARPS * HEADS * HD;            // [WARPS][HEADS][2]
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int h = n * 8 + 2 * t;
-    float* d0 = sm_o + (warp * HEADS + h) * HD + 16 * r;
-#pragma unroll
-    for (int mt = 0; mt < 8; ++mt) {
-      *reinterpret_cast<float2*>(d0 + 2 * mt) = make_float2(o[n][mt][0], o[n][mt][2]);
-      *reinterpret_cast<float2*>(d0 + HD + 2 * mt) = make_float2(o[n][mt][1], o[n][mt][3]);
+    const uint32_t past = __ballot_sync(0xffffffffu, upto > at);
+    if (past) {
+      const int first = __ffs(past) - 1;
+      seq = base + first;
+      at -= __shfl_sync(0xffffffffu, upto - n, first);
+      break;
     }
-    if (r == 0) {
+    at -= __shfl_sync(0xffffffffu, upto, 31);
+    if (base + 32 >= p.num_seqs) return;  // not reached: c0 < total
+  }
+  int len = min(__ldg(p.context_lens + seq), p.max_len);
+  int n = (len + CH - 1) / CH;
+  int head = (int)(at / n), j = (int)(at - (int64_t)head * n);
+
+  uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 511) & ~uintptr_t(511)) +
+                        warp * (STAGES * STAGE_BYTES);
+  if (lane == 0) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        sm_ml[(warp * HEADS + h + x) * 2] = m[n][x];
-        sm_ml[(warp * HEADS + h + x) * 2 + 1] = l[n][x];
+    for (int s = 0; s < STAGES; ++s) mbar_init(full + s, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+
+  // ---- the issuing side (lane 0): a cursor of its own, STAGES chunks ahead of the other
+  struct {
+    int seq, head, j, n, len, row, index, page;
+  } ahead = {seq, head, j, n, len, (j * CH) % p.block_size, (j * CH) / p.block_size, 0};
+  auto load_page = [&]() {
+    ahead.page = ahead.index < p.table_width ? __ldg(p.block_tables + ahead.seq * p.table_stride + ahead.index) : -1;
+  };
+  if (lane == 0) load_page();
+  auto issue = [&](int i, bool more) {
+    uint64_t* bar = full + i % STAGES;
+    uint8_t* st = ring + (i % STAGES) * STAGE_BYTES;
+    const bool good = ahead.page >= 0 && ahead.page < p.num_pages;
+    // keys of the chunk that count: none where the table has no usable page (recorded)
+    valid_of[i % STAGES] = good ? min(CH, ahead.len - ahead.j * CH) : 0;
+    if (good) {
+      const int piece = ahead.page * Hk + ahead.head;
+      const int64_t scales = fp4::head_offset(ahead.page, Hk, ahead.head, p.block_size) +
+                             fp4::scale_offset(ahead.row, p.block_size);
+      mbar_expect_tx(bar, STAGE_BYTES);
+      tma_load_3d(st, &p.tm_k, bar, 0, ahead.row, piece);
+      bulk_load_1d(st + 2 * CODE_TILE, p.k_cache + scales, SCALE_TILE, bar);
+      tma_load_3d(st + CODE_TILE, &p.tm_v, bar, 0, ahead.row, piece);
+      bulk_load_1d(st + 2 * CODE_TILE + SCALE_TILE, p.v_cache + scales, SCALE_TILE, bar);
+    } else {
+      record_error(VLC_DEV_ERR_BLOCK_RANGE);
+      mbar_arrive(bar);
+    }
+    if (!more) return;
+    if (++ahead.j < ahead.n) {
+      ahead.row += CH;
+      if (ahead.row < p.block_size) return;
+      ahead.row = 0;
+      ++ahead.index;
+    } else {
+      ahead.j = ahead.row = ahead.index = 0;
+      if (++ahead.head == Hk) {
+        ahead.head = 0;
+        do {
+          ahead.len = min(__ldg(p.context_lens + ++ahead.seq), p.max_len);
+        } while (ahead.len <= 0);  // a chunk follows: so does a sequence with keys
+        ahead.n = (ahead.len + CH - 1) / CH;
       }
     }
+    load_page();  // used at the next issue
+  };
+  if (lane == 0) {
+    for (int i = 0; i < min(STAGES, count); ++i) issue(i, i + 1 < count);
   }
-  __syncthreads();
-  // four dims a thread, heads over the warps
-  for (int h = warp; h < G; h += WARPS) {
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, sm_ml[(w * HEADS + h) * 2]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float f = fast_exp2(sm_ml[(w * HEADS + h) * 2] - ref);
-      L += f * sm_ml[(w * HEADS + h) * 2 + 1];
-      const float4 x = reinterpret_cast<const float4*>(sm_o + (w * HEADS + h) * HD)[lane];
-      acc.x += f * x.x;
-      acc.y += f * x.y;
-      acc.z += f * x.z;
-      acc.w += f * x.w;
+  auto arrived = [&](int i) {
+    const bool ok = mbar_wait_bounded(full + i % STAGES, (uint32_t)(i / STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 22,
+                                      VLC_WAIT_LIMIT_CYCLES);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
+
+  const uint32_t ring_u = smem_u32(ring);
+  State<NT> state;
+  auto q_of = [&]() { return p.q + (int64_t)seq * p.q_seq_stride + (int64_t)head * G * HD; };
+  state.start(q_of(), G, r, t, p.scale_log2, p.q_sign);
+  int begin = j;       // first chunk of the pair that is in the state
+  int first_slot = 0;  // the part's slot: 0 for the one that holds the warp's first chunk
+
+  for (int i = 0; i < count; ++i) {
+    if (!arrived(i)) {  // recorded; the copies still in flight are given the same time before the warp leaves
+      for (int x = i + 1; x < min(i + STAGES, count); ++x) arrived(x);
+      return;
     }
-    const int head = g * G + h;
-    if (nsplit == 1) {
-      const float inv = L != 0.f ? p.v_scale / L : 0.f;
-      uint2 u;
-      u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-      u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-      reinterpret_cast<uint2*>(p.out + (int64_t)b * p.out_seq_stride + (int64_t)head * HD)[lane] = u;
-    } else {
-      const int64_t pi = ((int64_t)b * p.max_splits + split) * p.num_heads + head;
-      reinterpret_cast<float4*>(p.part_o + pi * HD)[lane] = acc;
-      if (lane == 0) reinterpret_cast<float2*>(p.part_ml)[pi] = make_float2(M, L);
+    const uint32_t st = ring_u + (i % STAGES) * STAGE_BYTES;
+    const int valid = valid_of[i % STAGES];
+    if (valid == CH) state.template step<false>(st, valid, r, t);
+    else state.template step<true>(st, valid, r, t);
+    __syncwarp();  // every lane has read the stage
+    if (lane == 0 && i + STAGES < count) issue(i + STAGES, i + STAGES + 1 < count);
+    if (++j < n && i + 1 < count) continue;
+
+    // ---- the pair ends, or the run does
+    const bool whole = begin == 0 && j == n;
+    float* const part_o = p.parts + (my * 2 + first_slot) * G * HD;
+    float2* const part_ml = reinterpret_cast<float2*>(p.parts + (int64_t)p.num_warps * 2 * G * HD) +
+                            (my * 2 + first_slot) * G;
+#pragma unroll
+    for (int x = 0; x < NT * 2; ++x) {
+      const int nt = x >> 1, odd = x & 1;
+      const int h = nt * 8 + 2 * t + odd;
+      if (h >= G) continue;
+      const float sum = state.l[nt][odd];
+      if (whole) {
+        const float inv = sum != 0.f ? p.v_scale / sum : 0.f;
+        uint32_t u[8];
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt)
+          u[mt] = pack_bf16x2(state.o[nt][mt][odd] * inv, state.o[nt][mt][2 + odd] * inv);
+        uint4* dst = reinterpret_cast<uint4*>(p.out + (int64_t)seq * p.out_seq_stride + ((int64_t)head * G + h) * HD +
+                                              16 * r);
+        dst[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        dst[1] = make_uint4(u[4], u[5], u[6], u[7]);
+      } else {
+        float4* dst = reinterpret_cast<float4*>(part_o + h * HD + 16 * r);
+#pragma unroll
+        for (int mt = 0; mt < 8; mt += 2)
+          dst[mt / 2] = make_float4(state.o[nt][mt][odd], state.o[nt][mt][2 + odd], state.o[nt][mt + 1][odd],
+                                    state.o[nt][mt + 1][2 + odd]);
+        if (r == 0) part_ml[h] = make_float2(state.m[nt][odd], sum);
+      }
     }
+    if (i + 1 == count) break;
+    j = begin = 0;
+    first_slot = 1;
+    if (++head == Hk) {
+      head = 0;
+      do {
+        len = min(__ldg(p.context_lens + ++seq), p.max_len);
+      } while (len <= 0);
+      n = (len + CH - 1) / CH;
+    }
+    state.start(q_of(), G, r, t, p.scale_log2, p.q_sign);
   }
 }
 
-// Joins the splits of each (sequence, head): one warp a head, four dims a lane.
-__global__ void __launch_bounds__(128) decode_fp4_combine_kernel(const float* __restrict__ part_o,
-                                                                 const float* __restrict__ part_ml,
-                                                                 const int32_t* __restrict__ context_lens,
-                                                                 int split_keys, int max_splits, int num_heads,
-                                                                 float v_scale, __nv_bfloat16* __restrict__ out,
+// Joins the parts of the pairs that several warps shared and writes zeros for empty sequences.
+// Grid (sequence, heads): a block's eight warps take eight heads, or one head's parts in turn
+// (spread) where a pair has many.  Lanes: four dims each.
+__global__ void __launch_bounds__(256) decode_fp4_combine_kernel(const float* parts, const int32_t* context_lens,
+                                                                 int num_seqs, int max_len, int num_warps,
+                                                                 int num_heads, int num_kv_heads, int spread,
+                                                                 float v_scale, __nv_bfloat16* out,
                                                                  int64_t out_seq_stride) {
-  const int b = blockIdx.x;
-  const int h = blockIdx.y * 4 + warp_id();
-  const int lane = lane_id();
-  if (h >= num_heads) return;
-  const int len = min(__ldg(context_lens + b), max_splits * split_keys);
-  const int nsplit = len > 0 ? (len + split_keys - 1) / split_keys : 0;
-  if (nsplit <= 1) return;  // written by the decode kernel
-  const float2* ml = reinterpret_cast<const float2*>(part_ml) + (int64_t)b * max_splits * num_heads + h;
-  const float4* po = reinterpret_cast<const float4*>(part_o) + ((int64_t)b * max_splits * num_heads + h) * (HD / 4);
-  float M = -INFINITY;
-  for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, ml[(int64_t)s * num_heads].x);
+  __shared__ int64_t s_sum[2][8];
+  __shared__ float4 s_o[8][32];
+  __shared__ float2 s_ml[8];
+  const int seq = blockIdx.x, warp = warp_id(), lane = lane_id();
+  int64_t total = 0, before = 0;
+  for (int i = threadIdx.x; i < num_seqs; i += 256) {
+    const int c = chunks_of(__ldg(context_lens + i), max_len);
+    total += c;
+    if (i < seq) before += c;
+  }
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-  const float ref = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
+  for (int d = 1; d < 32; d <<= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, d);
+    before += __shfl_xor_sync(0xffffffffu, before, d);
+  }
+  if (lane == 0) {
+    s_sum[0][warp] = total;
+    s_sum[1][warp] = before;
+  }
+  __syncthreads();
+  total = before = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    total += s_sum[0][w];
+    before += s_sum[1][w];
+  }
+  // Every block waits, those with nothing to join too: what follows in the stream may rely on this
+  // grid's end for the decode kernel's.
+  pdl_wait();
+  const int h = spread ? blockIdx.y : blockIdx.y * 8 + warp;
+  const int n = chunks_of(__ldg(context_lens + seq), max_len);
+  const int G = num_heads / num_kv_heads;
+  if (h < num_heads && n == 0 && (!spread || warp == 0))
+    reinterpret_cast<uint2*>(out + (int64_t)seq * out_seq_stride + (int64_t)h * HD)[lane] = make_uint2(0, 0);
+  if (n == 0) return;
+  const int64_t share = share_of(total * num_kv_heads, num_warps);
+  const int64_t f0 = before * num_kv_heads + (int64_t)(min(h, num_heads - 1) / G) * n;  // the pair's chunks
+  const int64_t w0 = f0 / share, w1 = (f0 + n - 1) / share;                              // its warps
+  if (spread ? w0 == w1 : (h >= num_heads || w0 == w1)) return;  // (spread: for all warps alike)
+  // a part's slot is 0 unless the pair starts inside the warp's run
+  const int64_t skip = f0 == w0 * share ? 0 : 1;
+  const float* base = parts + (int64_t)(h % G) * HD;
+  const float2* ml = reinterpret_cast<const float2*>(parts + (int64_t)num_warps * 2 * G * HD) + h % G;
+  auto slot = [&](int64_t w) { return (w * 2 + (w == w0 ? skip : 0)) * G; };
+  const int step = spread ? 8 : 1;
+  float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int s = 0; s < nsplit; ++s) {
-    const float2 x = ml[(int64_t)s * num_heads];
-    const float4 v = po[(int64_t)s * num_heads * (HD / 4) + lane];
-    const float f = fast_exp2(x.x - ref);
-    L += f * x.y;
-    acc.x += f * v.x;
-    acc.y += f * v.y;
-    acc.z += f * v.z;
-    acc.w += f * v.w;
+  for (int64_t w = w0 + (spread ? warp : 0); w <= w1; w += step) {
+    const float2 x = ml[slot(w)];
+    const float4 v = reinterpret_cast<const float4*>(base + slot(w) * HD)[lane];
+    const float m = fmaxf(M, x.x);
+    const float f = m == -INFINITY ? 0.f : fast_exp2(M - m), g = m == -INFINITY ? 0.f : fast_exp2(x.x - m);
+    M = m;
+    L = L * f + g * x.y;
+    acc.x = acc.x * f + g * v.x;
+    acc.y = acc.y * f + g * v.y;
+    acc.z = acc.z * f + g * v.z;
+    acc.w = acc.w * f + g * v.w;
+  }
+  if (spread) {
+    s_o[warp][lane] = acc;
+    if (lane == 0) s_ml[warp] = make_float2(M, L);
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) M = fmaxf(M, s_ml[w].x);
+    L = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const float g = M == -INFINITY ? 0.f : fast_exp2(s_ml[w].x - M);
+      const float4 v = s_o[w][lane];
+      L += g * s_ml[w].y;
+      acc.x += g * v.x;
+      acc.y += g * v.y;
+      acc.z += g * v.z;
+      acc.w += g * v.w;
+    }
   }
   const float inv = L != 0.f ? v_scale / L : 0.f;
   uint2 u;
   u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
   u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-  reinterpret_cast<uint2*>(out + (int64_t)b * out_seq_stride + (int64_t)h * HD)[lane] = u;
+  reinterpret_cast<uint2*>(out + (int64_t)seq * out_seq_stride + (int64_t)h * HD)[lane] = u;
 }
 
-// Keys of a split: from host values only, so that the grid is fixed for graph capture.
-static int choose_split_keys(int num_seqs, int num_kv_heads, int max_context_len, int num_sms) {
-  const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
-  const int64_t target = 8LL * num_sms;
-  const int64_t splits = std::max<int64_t>(1, (target + pairs - 1) / pairs);
-  const int64_t step = WARPS * CH;
-  int64_t sk = (max_context_len + splits - 1) / splits;
-  sk = (sk + step - 1) / step * step;
-  return (int)std::max<int64_t>(512, std::min<int64_t>(sk, 2048));
+// Warps of the grid: from host values only, so that it is fixed for graph capture.
+static int grid_warps(int num_seqs, int num_heads, int num_kv_heads, int max_context_len, int num_sms) {
+  const int64_t most = (int64_t)num_seqs * num_kv_heads * (((int64_t)max_context_len + CH - 1) / CH);
+  const int64_t resident = (int64_t)num_sms * WARPS * blocks_per_sm(num_heads / num_kv_heads <= 8 ? 1 : 2);
+  return (int)std::max<int64_t>(1, std::min(resident, (most + MIN_SHARE - 1) / MIN_SHARE));
 }
 
 static bool power_of_two(float g) {
@@ -504,11 +610,9 @@ using namespace vlc;
 using namespace vlc::decode_fp4;
 
 extern "C" int64_t vlc_decode_fp4_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int max_context_len) {
-  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_context_len <= 0) return 0;
-  const int sk = choose_split_keys(num_seqs, num_kv_heads, max_context_len, vlc_num_sms());
-  const int64_t max_splits = ((int64_t)max_context_len + sk - 1) / sk;
-  if (max_splits <= 1) return 0;
-  return (int64_t)num_seqs * max_splits * num_heads * (HD + 2) * (int64_t)sizeof(float);
+  if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_context_len < 0) return 0;
+  const int64_t warps = grid_warps(num_seqs, num_heads, num_kv_heads, std::max(max_context_len, 1), vlc_num_sms());
+  return warps * 2 * (num_heads / num_kv_heads) * (HD + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_seqs, int num_heads,
@@ -531,13 +635,12 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return VLC_ERR_ALIGN;
   if (num_pages <= 0 || num_pages > 0x7fffffff / block_size || num_pages * num_kv_heads > 0x7fffffff)
     return VLC_ERR_SHAPE;
-  if (num_kv_heads > 65535 || num_seqs > 65535) return VLC_ERR_SHAPE;
+  if (num_kv_heads > 65535 || num_seqs > 65535 || num_heads > 65535) return VLC_ERR_SHAPE;
   if (max_context_len == 0) max_context_len = 1;
-  const int sk = choose_split_keys(num_seqs, num_kv_heads, max_context_len, vlc_num_sms());
-  const int max_splits = (max_context_len + sk - 1) / sk;
+  const int warps = grid_warps(num_seqs, num_heads, num_kv_heads, max_context_len, vlc_num_sms());
   const int64_t need = vlc_decode_fp4_workspace_size(num_seqs, num_heads, num_kv_heads, max_context_len);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return VLC_ERR_WORKSPACE;
-  if (need > 0 && !aligned16(workspace)) return VLC_ERR_ALIGN;
+  if (!workspace || workspace_bytes < need) return VLC_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return VLC_ERR_ALIGN;
 
   Params p;
   const uint64_t dims[3] = {(uint64_t)fp4::CODE_BYTES, (uint64_t)block_size, (uint64_t)(num_pages * num_kv_heads)};
@@ -555,20 +658,21 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   p.block_size = block_size;
   p.num_pages = (int)num_pages;
   p.context_lens = context_lens;
-  p.split_keys = sk;
-  p.max_splits = max_splits;
+  p.num_seqs = num_seqs;
+  p.max_len = max_context_len;
   p.group = G;
   p.num_heads = num_heads;
   p.num_kv_heads = num_kv_heads;
-  p.scale_log2 = softmax_scale * 1.4426950408889634f * k_scale;
+  p.scale_log2 = std::fabs(softmax_scale) * 1.4426950408889634f * k_scale;
+  p.q_sign = softmax_scale < 0.f ? -1.f : 1.f;
   p.v_scale = v_scale;
   p.out = (__nv_bfloat16*)out;
   p.out_seq_stride = out_seq_stride;
-  p.part_o = (float*)workspace;
-  p.part_ml = workspace ? p.part_o + (int64_t)num_seqs * max_splits * num_heads * HD : nullptr;
+  p.num_warps = warps;
+  p.parts = (float*)workspace;
 
   static std::atomic<uint64_t> smem1{0}, smem2{0};
-  const dim3 grid(max_splits, num_kv_heads, num_seqs);
+  const int grid = (warps + WARPS - 1) / WARPS;
   cudaStream_t st = (cudaStream_t)stream;
   if (G <= 8) {
     if (ensure_dynamic_smem((const void*)decode_fp4_kernel<1>, SMEM_BYTES, smem1) != VLC_OK) return VLC_ERR_CUDA;
@@ -577,10 +681,24 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
     if (ensure_dynamic_smem((const void*)decode_fp4_kernel<2>, SMEM_BYTES, smem2) != VLC_OK) return VLC_ERR_CUDA;
     decode_fp4_kernel<2><<<grid, WARPS * 32, SMEM_BYTES, st>>>(p);
   }
-  const int rc = launch_status();
-  if (rc != VLC_OK || max_splits <= 1) return rc;
-  const dim3 cg(num_seqs, (num_heads + 3) / 4);
-  decode_fp4_combine_kernel<<<cg, 128, 0, st>>>(p.part_o, p.part_ml, context_lens, sk, max_splits, num_heads, v_scale,
-                                              p.out, out_seq_stride);
-  return launch_status();
+  int rc = launch_status();
+  if (rc != VLC_OK) return rc;
+  // Few pairs: each has many parts, and a block takes one head's.
+  const int spread = warps > 8ll * num_seqs * num_kv_heads ? 1 : 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(num_seqs, spread ? num_heads : (num_heads + 7) / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, decode_fp4_combine_kernel, (const float*)p.parts, context_lens, num_seqs,
+                         max_context_len, warps, num_heads, num_kv_heads, spread, v_scale, p.out,
+                         out_seq_stride) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return VLC_ERR_CUDA;
+  }
+  return VLC_OK;
 }
