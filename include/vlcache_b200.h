@@ -419,7 +419,8 @@ int vlc_mrope_store_kvcache(const int64_t* positions, int64_t axis_stride, int n
  *   its bits.  layer_stride in bytes.
  * vlc_decode_attn_fp4: vlc_decode_attn over such a cache: f16 products of exact K / V
  *   values with q (scaled per head by a power of two) and P, fp32 sums.  Keys of a chunk of
- *   64 whose table entry is bad are left out and recorded.
+ *   64 whose table entry is bad are left out and recorded.  The workspace, 32-byte aligned,
+ *   holds the parts of keys split over the grid; calls that may overlap take one each.
  * ------------------------------------------------------------------------ */
 int vlc_rope_store_kvcache_fp4(const int64_t* positions, int64_t axis_stride, int num_axes, const int32_t* sections,
                                const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, const void* key,

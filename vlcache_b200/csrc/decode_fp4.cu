@@ -18,7 +18,7 @@
 // the grid's warps share out evenly, each a contiguous run of it.  The shares are equal whatever
 // the lengths are (a grid of fixed splits left SMs idle at its end, paid a prologue and a join
 // every few chunks and merged in shared memory: 267 us for 256 sequences of 2700 .. 10700 keys, 28
-// query and 4 KV heads, against 196 us now).  A warp works alone: its own ring of chunks (TMA
+// query and 4 KV heads, against 183 us now).  A warp works alone: its own ring of chunks (TMA
 // tiles with the 64-byte swizzle for the codes, plain bulk copies for the scales, issued by its
 // lane 0), its own running maximum and sums, no barrier with any other warp.  A pair that a warp
 // has to itself is written out; the parts of a pair that several warps share go to the workspace
@@ -48,7 +48,6 @@ constexpr int SCALE_TILE = CH * fp4::SCALE_BYTES;
 constexpr int STAGE_BYTES = 2 * (CODE_TILE + SCALE_TILE);
 constexpr int SMEM_BYTES = WARPS * STAGES * STAGE_BYTES + 512;  // + alignment to the swizzle's period
 constexpr int MAX_GROUP = 16;
-constexpr int MIN_SHARE = 2;                    // chunks a warp takes at least
 constexpr float P_SHIFT = 12.f;
 constexpr float SLACK = 3.f;                    // log2 that the maximum may grow by before O is rescaled
 
@@ -89,14 +88,20 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, __half2 b) {
+  const __half2 d = __hmul2(as_half2(a), b);
+  return *reinterpret_cast<const uint32_t*>(&d);
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+// Bits of a where the mask is set, of b elsewhere: one instruction.
+__device__ __forceinline__ uint32_t select_bits(uint32_t mask, uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xca;" : "=r"(d) : "r"(mask), "r"(a), "r"(b));
   return d;
 }
 __device__ __forceinline__ uint32_t lds_u8(uint32_t a) {
@@ -131,10 +136,18 @@ __device__ __forceinline__ uint32_t swizzled(int key, int piece) {
 // Chunks of a sequence.  A length past the host's bound is cut to it (recorded by the caller).
 __device__ __forceinline__ int chunks_of(int len, int max_len) { return (min(max(len, 0), max_len) + CH - 1) / CH; }
 
-// How the line of chunks is shared: chunks a warp, from the total and the warps of the grid.
-__device__ __forceinline__ int64_t share_of(int64_t total, int num_warps) {
-  return max((total + num_warps - 1) / num_warps, (int64_t)MIN_SHARE);
-}
+// How the line of `total` chunks is shared: every warp takes each() of them and the first extra()
+// one more.
+struct Shares {
+  int64_t each, extra;
+  __device__ __forceinline__ Shares(int64_t total, int num_warps) : each(total / num_warps), extra(total % num_warps) {}
+  __device__ __forceinline__ int64_t first(int64_t warp) const { return warp * each + min(warp, extra); }
+  __device__ __forceinline__ int64_t count(int64_t warp) const { return each + (warp < extra ? 1 : 0); }
+  __device__ __forceinline__ int64_t warp_of(int64_t chunk) const {
+    const int64_t big = extra * (each + 1);
+    return chunk < big ? chunk / (each + 1) : extra + (chunk - big) / each;
+  }
+};
 
 // A query head group's state of a warp: S^T, O^T and the softmax, and the step over one chunk.
 template <int NT>  // 8-head column tiles
@@ -144,6 +157,7 @@ struct State {
   float o[NT][8][4];        // m-tile i: dims 16r + 2i (0, 1) and 16r + 2i + 1 (2, 3) of heads 2t, 2t + 1
   float l[NT][4];           // sums of P: 0 and 1 of heads 2t, 2t + 1
   float m[NT][2];           // the maximum that P is relative to
+  float shift[NT][2];       // P_SHIFT - m (0 before the first key)
 
   __device__ __forceinline__ void start(const __nv_bfloat16* q, int G, int r, int t, float scale_log2, float sign) {
 #pragma unroll
@@ -177,6 +191,7 @@ struct State {
       for (int i = 0; i < 8; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
       l[n][0] = l[n][1] = l[n][2] = l[n][3] = 0.f;
       m[n][0] = m[n][1] = -INFINITY;
+      shift[n][0] = shift[n][1] = 0.f;
     }
   }
 
@@ -194,12 +209,13 @@ struct State {
       uint32_t c0[4], c1[4];  // keys kr and kr + 8 of the tile (8 keys on, the swizzle is the same)
       lds128(k_codes + kt * 1024, c0);
       lds128(k_codes + kt * 1024 + 512, c1);
-      const uint32_t f0 = fp4::scales2_f16(lds_u16(k_scales + kt * 128));
-      const uint32_t f1 = fp4::scales2_f16(lds_u16(k_scales + kt * 128 + 64));
+      const __half2 f0 = as_half2(fp4::scales2_f16(lds_u16(k_scales + kt * 128)));
+      const __half2 f1 = as_half2(fp4::scales2_f16(lds_u16(k_scales + kt * 128 + 64)));
 #pragma unroll
       for (int w = 0; w < 4; ++w) {  // four bytes: k-steps 2w and 2w + 1
-        const uint32_t sc0 = __byte_perm(f0, 0, w < 2 ? 0x1010 : 0x3232);
-        const uint32_t sc1 = __byte_perm(f1, 0, w < 2 ? 0x1010 : 0x3232);
+        // (a half on both sides of a multiplication is an operand's form, not an instruction)
+        const __half2 sc0 = w < 2 ? __low2half2(f0) : __high2half2(f0);
+        const __half2 sc1 = w < 2 ? __low2half2(f1) : __high2half2(f1);
         uint32_t h0[4], h1[4];
         fp4::decode8(c0[w], h0);
         fp4::decode8(c1[w], h1);
@@ -232,19 +248,22 @@ struct State {
         top0 = fmax3(top0, x[0], x[2]);
         top1 = fmax3(top1, x[1], x[3]);
       }
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, d));
-        top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, d));
-      }
       top0 *= scale[n][0];
       top1 *= scale[n][1];
+      // The lanes' own maxima tell whether any grew past the slack; only then are they joined.
       if (__any_sync(0xffffffffu, top0 > m[n][0] + SLACK || top1 > m[n][1] + SLACK)) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, d));
+          top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, d));
+        }
         const float m0 = fmaxf(m[n][0], top0), m1 = fmaxf(m[n][1], top1);
         const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m[n][0] - m0);  // (-inf: no key so far)
         const float f1 = m1 == -INFINITY ? 0.f : fast_exp2(m[n][1] - m1);
         m[n][0] = m0;
         m[n][1] = m1;
+        shift[n][0] = m0 == -INFINITY ? 0.f : P_SHIFT - m0;
+        shift[n][1] = m1 == -INFINITY ? 0.f : P_SHIFT - m1;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           o[n][i][0] *= f0;
@@ -255,15 +274,13 @@ struct State {
         l[n][0] *= f0;
         l[n][1] *= f1;
       }
-      const float r0 = m[n][0] == -INFINITY ? 0.f : P_SHIFT - m[n][0];
-      const float r1 = m[n][1] == -INFINITY ? 0.f : P_SHIFT - m[n][1];
 #pragma unroll
       for (int kt = 0; kt < TILES; ++kt) {
         float(&x)[4] = s[kt][n];
-        x[0] = fast_exp2(fmaf(x[0], scale[n][0], r0));
-        x[1] = fast_exp2(fmaf(x[1], scale[n][1], r1));
-        x[2] = fast_exp2(fmaf(x[2], scale[n][0], r0));
-        x[3] = fast_exp2(fmaf(x[3], scale[n][1], r1));
+        x[0] = fast_exp2(fmaf(x[0], scale[n][0], shift[n][0]));
+        x[1] = fast_exp2(fmaf(x[1], scale[n][1], shift[n][1]));
+        x[2] = fast_exp2(fmaf(x[2], scale[n][0], shift[n][0]));
+        x[3] = fast_exp2(fmaf(x[3], scale[n][1], shift[n][1]));
         if (CUT) {  // (not left to exp2(-inf): a scale of 0 would make it exp2(NaN))
           if (kt * 16 + kr >= valid) x[0] = x[1] = 0.f;
           if (kt * 16 + kr + 8 >= valid) x[2] = x[3] = 0.f;
@@ -291,17 +308,18 @@ struct State {
         // rows past the end may hold anything: their P is 0, and a scale of 0 makes V 0
         if (CUT && kt * 16 + kv[x & 1] + (x >> 1) * 8 >= valid) sb[x] = 0;
       }
-      const uint32_t sc01 = fp4::scales2_f16(__byte_perm(sb[0], sb[1], 0x0040));
-      const uint32_t sc23 = fp4::scales2_f16(__byte_perm(sb[2], sb[3], 0x0040));
+      const __half2 sc01 = as_half2(fp4::scales2_f16(__byte_perm(sb[0], sb[1], 0x0040)));
+      const __half2 sc23 = as_half2(fp4::scales2_f16(__byte_perm(sb[2], sb[3], 0x0040)));
 #pragma unroll
       for (int n = 0; n < NT; ++n) mma_f16(l[n], ones, pb[kt][n][0], pb[kt][n][1]);
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         // bytes of {key 0 or 2, key 1 or 3} x {low nibbles: dims 16r + 2i, high: 16r + 2i + 1}
-        const uint32_t lo01 = (c[0][w] & 0x0f0f0f0fu) | ((c[1][w] << 4) & 0xf0f0f0f0u);
-        const uint32_t hi01 = ((c[0][w] >> 4) & 0x0f0f0f0fu) | (c[1][w] & 0xf0f0f0f0u);
-        const uint32_t lo23 = (c[2][w] & 0x0f0f0f0fu) | ((c[3][w] << 4) & 0xf0f0f0f0u);
-        const uint32_t hi23 = ((c[2][w] >> 4) & 0x0f0f0f0fu) | (c[3][w] & 0xf0f0f0f0u);
+        constexpr uint32_t LOW = 0x0f0f0f0fu;
+        const uint32_t lo01 = select_bits(LOW, c[0][w], c[1][w] << 4);
+        const uint32_t hi01 = select_bits(LOW, c[0][w] >> 4, c[1][w]);
+        const uint32_t lo23 = select_bits(LOW, c[2][w], c[3][w] << 4);
+        const uint32_t hi23 = select_bits(LOW, c[2][w] >> 4, c[3][w]);
         uint32_t a0[4], a1[4], a2[4], a3[4];
         fp4::decode8(lo01, a0);
         fp4::decode8(hi01, a1);
@@ -341,10 +359,10 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
   total *= Hk;
-  const int64_t share = share_of(total, p.num_warps);
-  const int64_t c0 = my * share;
-  if (my >= p.num_warps || c0 >= total) return;
-  const int count = (int)(min(c0 + share, total) - c0);
+  const Shares shares(total, p.num_warps);
+  const int64_t c0 = shares.first(my);
+  const int count = (int)shares.count(my);
+  if (my >= p.num_warps || count == 0) return;
   int seq = 0;
   int64_t at = c0;  // c0's place among the chunks from the sequence's first on
   for (int base = 0;; base += 32) {
@@ -380,56 +398,60 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
 
   // ---- the issuing side (lane 0): a cursor of its own, STAGES chunks ahead of the other
   struct {
-    int seq, head, j, n, len, row, index, page;
-  } ahead = {seq, head, j, n, len, (j * CH) % p.block_size, (j * CH) / p.block_size, 0};
+    int seq, head, left, keys;  // chunks and keys of the pair from here on
+    int row, index;             // row in the page, page of the sequence
+    int page;                   // its number in the cache, loaded when the cursor comes to it
+  } ahead = {seq, head, n - j, len - j * CH, (j * CH) % p.block_size, (j * CH) / p.block_size, 0};
   auto load_page = [&]() {
     ahead.page = ahead.index < p.table_width ? __ldg(p.block_tables + ahead.seq * p.table_stride + ahead.index) : -1;
   };
   if (lane == 0) load_page();
-  auto issue = [&](int i, bool more) {
-    uint64_t* bar = full + i % STAGES;
-    uint8_t* st = ring + (i % STAGES) * STAGE_BYTES;
-    const bool good = ahead.page >= 0 && ahead.page < p.num_pages;
-    // keys of the chunk that count: none where the table has no usable page (recorded)
-    valid_of[i % STAGES] = good ? min(CH, ahead.len - ahead.j * CH) : 0;
-    if (good) {
+  const int head_bytes = p.block_size * fp4::ROW_BYTES;
+  auto issue = [&](int stage, bool more) {
+    uint64_t* bar = full + stage;
+    uint8_t* st = ring + stage * STAGE_BYTES;
+    if ((uint32_t)ahead.page < (uint32_t)p.num_pages) {
       const int piece = ahead.page * Hk + ahead.head;
-      const int64_t scales = fp4::head_offset(ahead.page, Hk, ahead.head, p.block_size) +
-                             fp4::scale_offset(ahead.row, p.block_size);
+      const int64_t scales = (int64_t)piece * head_bytes + fp4::scale_offset(ahead.row, p.block_size);
+      valid_of[stage] = min(CH, ahead.keys);
       mbar_expect_tx(bar, STAGE_BYTES);
       tma_load_3d(st, &p.tm_k, bar, 0, ahead.row, piece);
       bulk_load_1d(st + 2 * CODE_TILE, p.k_cache + scales, SCALE_TILE, bar);
       tma_load_3d(st + CODE_TILE, &p.tm_v, bar, 0, ahead.row, piece);
       bulk_load_1d(st + 2 * CODE_TILE + SCALE_TILE, p.v_cache + scales, SCALE_TILE, bar);
-    } else {
+    } else {  // the table has no usable page there: recorded, and none of the chunk's keys counts
+      valid_of[stage] = 0;
       record_error(VLC_DEV_ERR_BLOCK_RANGE);
       mbar_arrive(bar);
     }
     if (!more) return;
-    if (++ahead.j < ahead.n) {
-      ahead.row += CH;
+    ahead.row += CH;
+    ahead.keys -= CH;
+    if (--ahead.left > 0) {
       if (ahead.row < p.block_size) return;
       ahead.row = 0;
       ++ahead.index;
     } else {
-      ahead.j = ahead.row = ahead.index = 0;
+      ahead.row = ahead.index = 0;
       if (++ahead.head == Hk) {
         ahead.head = 0;
         do {
-          ahead.len = min(__ldg(p.context_lens + ++ahead.seq), p.max_len);
-        } while (ahead.len <= 0);  // a chunk follows: so does a sequence with keys
-        ahead.n = (ahead.len + CH - 1) / CH;
+          ++ahead.seq;
+        } while (__ldg(p.context_lens + ahead.seq) <= 0);  // a chunk follows: so does a sequence with keys
       }
+      ahead.keys = min(__ldg(p.context_lens + ahead.seq), p.max_len);
+      ahead.left = (ahead.keys + CH - 1) / CH;
     }
     load_page();  // used at the next issue
   };
   if (lane == 0) {
     for (int i = 0; i < min(STAGES, count); ++i) issue(i, i + 1 < count);
   }
+  // Whether chunk i came (recorded where it did not).
   auto arrived = [&](int i) {
-    const bool ok = mbar_wait_bounded(full + i % STAGES, (uint32_t)(i / STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 22,
-                                      VLC_WAIT_LIMIT_CYCLES);
-    return __all_sync(0xffffffffu, ok) != 0;
+    const uint32_t parity = (uint32_t)(i / STAGES) & 1u;
+    if (mbar_try_wait(full + i % STAGES, parity)) return true;
+    return mbar_wait_bounded(full + i % STAGES, parity, VLC_DEV_ERR_TIMEOUT + 22, VLC_WAIT_LIMIT_CYCLES);
   };
 
   const uint32_t ring_u = smem_u32(ring);
@@ -440,7 +462,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
   int first_slot = 0;  // the part's slot: 0 for the one that holds the warp's first chunk
 
   for (int i = 0; i < count; ++i) {
-    if (!arrived(i)) {  // recorded; the copies still in flight are given the same time before the warp leaves
+    if (!__all_sync(0xffffffffu, arrived(i))) {  // the copies still in flight are given the same time
       for (int x = i + 1; x < min(i + STAGES, count); ++x) arrived(x);
       return;
     }
@@ -449,7 +471,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
     if (valid == CH) state.template step<false>(st, valid, r, t);
     else state.template step<true>(st, valid, r, t);
     __syncwarp();  // every lane has read the stage
-    if (lane == 0 && i + STAGES < count) issue(i + STAGES, i + STAGES + 1 < count);
+    if (lane == 0 && i + STAGES < count) issue(i % STAGES, i + STAGES + 1 < count);
     if (++j < n && i + 1 < count) continue;
 
     // ---- the pair ends, or the run does
@@ -474,11 +496,16 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
         dst[0] = make_uint4(u[0], u[1], u[2], u[3]);
         dst[1] = make_uint4(u[4], u[5], u[6], u[7]);
       } else {
-        float4* dst = reinterpret_cast<float4*>(part_o + h * HD + 16 * r);
 #pragma unroll
-        for (int mt = 0; mt < 8; mt += 2)
-          dst[mt / 2] = make_float4(state.o[nt][mt][odd], state.o[nt][mt][2 + odd], state.o[nt][mt + 1][odd],
-                                    state.o[nt][mt + 1][2 + odd]);
+        for (int mt = 0; mt < 8; mt += 4) {  // 32 bytes a store: whole sectors
+          uint32_t u[8];
+#pragma unroll
+          for (int x4 = 0; x4 < 4; ++x4) {
+            u[2 * x4] = __float_as_uint(state.o[nt][mt + x4][odd]);
+            u[2 * x4 + 1] = __float_as_uint(state.o[nt][mt + x4][2 + odd]);
+          }
+          st_global_v8(part_o + h * HD + 16 * r + 2 * mt, u);
+        }
         if (r == 0) part_ml[h] = make_float2(state.m[nt][odd], sum);
       }
     }
@@ -497,16 +524,17 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
 }
 
 // Joins the parts of the pairs that several warps shared and writes zeros for empty sequences.
-// Grid (sequence, heads): a block's eight warps take eight heads, or one head's parts in turn
-// (spread) where a pair has many.  Lanes: four dims each.
-__global__ void __launch_bounds__(256) decode_fp4_combine_kernel(const float* parts, const int32_t* context_lens,
+// SPREAD (few pairs of many parts): a block takes a quarter of one head's dims; its 32 groups of
+// eight lanes take the parts in turn.  Otherwise a block takes eight heads, a warp each.
+template <bool SPREAD>
+__global__ void __launch_bounds__(256, SPREAD ? 3 : 6) decode_fp4_combine_kernel(const float* parts, const int32_t* context_lens,
                                                                  int num_seqs, int max_len, int num_warps,
-                                                                 int num_heads, int num_kv_heads, int spread,
-                                                                 float v_scale, __nv_bfloat16* out,
-                                                                 int64_t out_seq_stride) {
+                                                                 int num_heads, int num_kv_heads, float v_scale,
+                                                                 __nv_bfloat16* out, int64_t out_seq_stride) {
   __shared__ int64_t s_sum[2][8];
-  __shared__ float4 s_o[8][32];
-  __shared__ float2 s_ml[8];
+  __shared__ float s_max[8];
+  __shared__ float4 s_o[8][8];
+  __shared__ float s_l[8];
   const int seq = blockIdx.x, warp = warp_id(), lane = lane_id();
   int64_t total = 0, before = 0;
   for (int i = threadIdx.x; i < num_seqs; i += 256) {
@@ -530,72 +558,90 @@ __global__ void __launch_bounds__(256) decode_fp4_combine_kernel(const float* pa
     total += s_sum[0][w];
     before += s_sum[1][w];
   }
+  const int n = chunks_of(__ldg(context_lens + seq), max_len);
+  const int h = SPREAD ? blockIdx.y : blockIdx.y * 8 + warp;
+  const int G = num_heads / num_kv_heads;
+  // dims: 32 z + 4 (lane % 8) of a quarter, or 4 lane
+  const int dim4 = SPREAD ? blockIdx.z * 8 + (lane & 7) : lane;
   // Every block waits, those with nothing to join too: what follows in the stream may rely on this
   // grid's end for the decode kernel's.
   pdl_wait();
-  const int h = spread ? blockIdx.y : blockIdx.y * 8 + warp;
-  const int n = chunks_of(__ldg(context_lens + seq), max_len);
-  const int G = num_heads / num_kv_heads;
-  if (h < num_heads && n == 0 && (!spread || warp == 0))
-    reinterpret_cast<uint2*>(out + (int64_t)seq * out_seq_stride + (int64_t)h * HD)[lane] = make_uint2(0, 0);
-  if (n == 0) return;
-  const int64_t share = share_of(total * num_kv_heads, num_warps);
-  const int64_t f0 = before * num_kv_heads + (int64_t)(min(h, num_heads - 1) / G) * n;  // the pair's chunks
-  const int64_t w0 = f0 / share, w1 = (f0 + n - 1) / share;                              // its warps
-  if (spread ? w0 == w1 : (h >= num_heads || w0 == w1)) return;  // (spread: for all warps alike)
-  // a part's slot is 0 unless the pair starts inside the warp's run
-  const int64_t skip = f0 == w0 * share ? 0 : 1;
-  const float* base = parts + (int64_t)(h % G) * HD;
-  const float2* ml = reinterpret_cast<const float2*>(parts + (int64_t)num_warps * 2 * G * HD) + h % G;
-  auto slot = [&](int64_t w) { return (w * 2 + (w == w0 ? skip : 0)) * G; };
-  const int step = spread ? 8 : 1;
-  float M = -INFINITY, L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int64_t w = w0 + (spread ? warp : 0); w <= w1; w += step) {
-    const float2 x = ml[slot(w)];
-    const float4 v = reinterpret_cast<const float4*>(base + slot(w) * HD)[lane];
-    const float m = fmaxf(M, x.x);
-    const float f = m == -INFINITY ? 0.f : fast_exp2(M - m), g = m == -INFINITY ? 0.f : fast_exp2(x.x - m);
-    M = m;
-    L = L * f + g * x.y;
-    acc.x = acc.x * f + g * v.x;
-    acc.y = acc.y * f + g * v.y;
-    acc.z = acc.z * f + g * v.z;
-    acc.w = acc.w * f + g * v.w;
+  if (h >= num_heads) return;
+  uint2* const dst = reinterpret_cast<uint2*>(out + (int64_t)seq * out_seq_stride + (int64_t)h * HD) + dim4;
+  if (n == 0) {
+    if (!SPREAD || threadIdx.x < 8) *dst = make_uint2(0, 0);
+    return;
   }
-  if (spread) {
-    s_o[warp][lane] = acc;
-    if (lane == 0) s_ml[warp] = make_float2(M, L);
-    __syncthreads();
-    if (warp) return;
+  const Shares shares(total * num_kv_heads, num_warps);
+  const int64_t f0 = before * num_kv_heads + (int64_t)(h / G) * n;           // the pair's first chunk
+  const int64_t w0 = shares.warp_of(f0);                                     // its first warp
+  const int count = (int)(shares.warp_of(f0 + n - 1) - w0) + 1;              // and their number
+  if (count == 1) return;
+  // parts are G apart, but the first warp's lies one slot on when its run begins before the pair
+  const int64_t first = (w0 * 2 + (f0 == shares.first(w0) ? 0 : 1)) * G + h % G, rest = w0 * 2 * G + h % G;
+  const float4* po = reinterpret_cast<const float4*>(parts) + dim4;
+  const float2* ml = reinterpret_cast<const float2*>(parts + (int64_t)num_warps * 2 * G * HD);
+  auto slot = [&](int i) { return i == 0 ? first : rest + (int64_t)i * 2 * G; };
+
+  float M = -INFINITY;
+  for (int i = SPREAD ? threadIdx.x : lane; i < count; i += SPREAD ? 256 : 32) M = fmaxf(M, ml[slot(i)].x);
 #pragma unroll
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, s_ml[w].x);
+  for (int d = 1; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  if (SPREAD) {
+    if (lane == 0) s_max[warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) M = fmaxf(M, s_max[w]);
+  }
+  const float ref = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll (SPREAD ? 8 : 2)
+  for (int i = SPREAD ? threadIdx.x >> 3 : 0; i < count; i += SPREAD ? 32 : 1) {
+    const int64_t s = slot(i);
+    const float2 x = ml[s];
+    const float4 v = po[s * (HD / 4)];
+    const float f = fast_exp2(x.x - ref);
+    L += f * x.y;
+    acc.x += f * v.x;
+    acc.y += f * v.y;
+    acc.z += f * v.z;
+    acc.w += f * v.w;
+  }
+  if (SPREAD) {
+#pragma unroll
+    for (int d = 8; d < 32; d <<= 1) {
+      L += __shfl_xor_sync(0xffffffffu, L, d);
+      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, d);
+      acc.y += __shfl_xor_sync(0xffffffffu, acc.y, d);
+      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, d);
+      acc.w += __shfl_xor_sync(0xffffffffu, acc.w, d);
+    }
+    if (lane < 8) s_o[warp][lane] = acc;
+    if (lane == 0) s_l[warp] = L;
+    __syncthreads();
+    if (threadIdx.x >= 8) return;
     L = 0.f;
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      const float g = M == -INFINITY ? 0.f : fast_exp2(s_ml[w].x - M);
       const float4 v = s_o[w][lane];
-      L += g * s_ml[w].y;
-      acc.x += g * v.x;
-      acc.y += g * v.y;
-      acc.z += g * v.z;
-      acc.w += g * v.w;
+      L += s_l[w];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
     }
   }
   const float inv = L != 0.f ? v_scale / L : 0.f;
-  uint2 u;
-  u.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-  u.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-  reinterpret_cast<uint2*>(out + (int64_t)seq * out_seq_stride + (int64_t)h * HD)[lane] = u;
+  *dst = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
 // Warps of the grid: from host values only, so that it is fixed for graph capture.
 static int grid_warps(int num_seqs, int num_heads, int num_kv_heads, int max_context_len, int num_sms) {
   const int64_t most = (int64_t)num_seqs * num_kv_heads * (((int64_t)max_context_len + CH - 1) / CH);
   const int64_t resident = (int64_t)num_sms * WARPS * blocks_per_sm(num_heads / num_kv_heads <= 8 ? 1 : 2);
-  return (int)std::max<int64_t>(1, std::min(resident, (most + MIN_SHARE - 1) / MIN_SHARE));
+  return (int)std::max<int64_t>(1, std::min(resident, most));
 }
 
 static bool power_of_two(float g) {
@@ -640,7 +686,7 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   const int warps = grid_warps(num_seqs, num_heads, num_kv_heads, max_context_len, vlc_num_sms());
   const int64_t need = vlc_decode_fp4_workspace_size(num_seqs, num_heads, num_kv_heads, max_context_len);
   if (!workspace || workspace_bytes < need) return VLC_ERR_WORKSPACE;
-  if (!aligned16(workspace)) return VLC_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(workspace) % 32) return VLC_ERR_ALIGN;
 
   Params p;
   const uint64_t dims[3] = {(uint64_t)fp4::CODE_BYTES, (uint64_t)block_size, (uint64_t)(num_pages * num_kv_heads)};
@@ -683,10 +729,10 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   }
   int rc = launch_status();
   if (rc != VLC_OK) return rc;
-  // Few pairs: each has many parts, and a block takes one head's.
-  const int spread = warps > 8ll * num_seqs * num_kv_heads ? 1 : 0;
+  // Few pairs: each has many parts, which several blocks read.
+  const bool spread = warps > 8ll * num_seqs * num_kv_heads;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(num_seqs, spread ? num_heads : (num_heads + 7) / 8);
+  cfg.gridDim = spread ? dim3(num_seqs, num_heads, 4) : dim3(num_seqs, (num_heads + 7) / 8);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -694,9 +740,9 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, decode_fp4_combine_kernel, (const float*)p.parts, context_lens, num_seqs,
-                         max_context_len, warps, num_heads, num_kv_heads, spread, v_scale, p.out,
-                         out_seq_stride) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, spread ? decode_fp4_combine_kernel<true> : decode_fp4_combine_kernel<false>,
+                         (const float*)p.parts, context_lens, num_seqs, max_context_len, warps, num_heads,
+                         num_kv_heads, v_scale, p.out, out_seq_stride) != cudaSuccess) {
     (void)cudaGetLastError();
     return VLC_ERR_CUDA;
   }
