@@ -30,6 +30,29 @@ def test_oracle_values_fit_bf16():
     assert torch.equal(v.to(torch.bfloat16).double(), v) and torch.equal(v.to(torch.float16).double(), v)
 
 
+def test_quantising_without_division_is_exact():
+    """The kernels' arithmetic, in numpy's fp32, over every bf16 magnitude and every scale: a
+    product with the reciprocal put on the grid of 2^-11 rounds to e2m1 as the exact quotient
+    does, and a product with 1/6 rounds to e4m3 as the quotient by 6 does.  The reciprocal is
+    taken one step high and low too, as an approximate one may be."""
+    f = np.float32
+    x = np.arange(0x7f80, dtype=np.uint32)
+    x = (x << 16).view(f)                                            # all finite magnitudes
+    top = np.minimum(x.astype(np.float64) / 6, 448)
+    with np.errstate(over="ignore"):
+        assert np.array_equal(fp4.nearest(np.minimum(x * (f(1) / f(6)), f(448)).astype(np.float64), fp4.E4M3),
+                              fp4.nearest(top, fp4.E4M3))
+        grid = f(1.5 * 4096)
+        for s in fp4.E4M3[1:]:
+            y = x[x <= 20 * s]                                       # the codes stop at 6
+            want = fp4.nearest(y.astype(np.float64) / s, fp4.E2M1)
+            inv = f(1) / f(s)
+            for i in (inv, np.nextafter(inv, f(0)), np.nextafter(inv, f(4096))):
+                for sign in (f(1), f(-1)):
+                    q = (y.astype(np.float64) * sign * i + grid).astype(f) - grid   # one rounding, as fma has
+                    assert np.array_equal(fp4.nearest(np.abs(q.astype(np.float64)), fp4.E2M1), want)
+
+
 def test_oracle_pages_round_trip():
     r = np.random.default_rng(0)
     pages = r.integers(0, 256, size=(3, 2, 64 * fp4.ROW), dtype=np.uint8)

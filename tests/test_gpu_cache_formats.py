@@ -94,6 +94,43 @@ def test_mrope_store_matches_oracle(ops, sections, N, H, Hk):
     assert np.array_equal(_bits(dvc).reshape(512, Hk, D), vc_ref)
 
 
+@pytest.mark.parametrize("N,H,Hk,sections", [(4011, 28, 4, (16, 24, 24)), (12001, 6, 1, (22, 21, 21)),
+                                             (6001, 16, 2, (64,))])
+def test_mrope_many_tokens_are_few_tokens_rows(ops, N, H, Hk, sections):
+    """A prompt's rows come out as they do in calls of a few tokens each, into either cache and
+    without one: skipped slots, bad slots and bad positions among them."""
+    from vlcache_b200.layers.rotary_embedding import rope_cos_sin_cache
+    g = _gen(N)
+    table = rope_cos_sin_cache(D, 1024, 1e6).cuda()
+    pos = torch.randint(0, 1024, (len(sections), N), generator=g)
+    pos[-1, 77] = 1024
+    pos, qkv = pos.cuda(), torch.randn(N, H + 2 * Hk, D, generator=g).to(torch.bfloat16).cuda()
+    q, k, v = qkv.split((H, Hk, Hk), 1)
+    pages = (N + 255) // 256 + 1
+    slots = torch.randperm(pages * 256, generator=g)[:N].to(torch.int32)
+    slots[::11], slots[5] = -1, pages * 256
+    slots = slots.cuda()
+    zeros = lambda fmt: [torch.zeros(*((pages, 256, Hk, D) if fmt == "bf16" else (pages, Hk, 256 * 72)),  # noqa: E731
+                                     dtype=torch.bfloat16 if fmt == "bf16" else torch.uint8, device="cuda")
+                         for _ in "kv"]
+    rows = [slice(i, i + 100) for i in range(0, N, 100)]
+    for fmt, store in (("bf16", ops.mrope_store_kvcache), ("fp4", ops.rope_store_kvcache_fp4)):
+        many, few = zeros(fmt), zeros(fmt)
+        out, parts = torch.zeros(N, H, D, dtype=torch.bfloat16, device="cuda"), torch.zeros_like(q)
+        store(pos, q, k, v, table, *many, slots, sections, out=out)
+        assert ops.device_error(reset=True) in (101, 103)
+        for r in rows:
+            store(pos[:, r], q[r], k[r], v[r], table, *few, slots[r], sections, out=parts[r])
+        assert ops.device_error(reset=True) in (101, 103)
+        assert torch.equal(out, parts) and bool(out[-1].any()) and not bool(out[77].any())
+        assert all(torch.equal(a, b) and bool(a.any()) for a, b in zip(many, few))
+    good = pos.clamp(max=1023)
+    a, b = ops.mrotary_embedding(good, q, k, table, sections)
+    for r in rows:
+        x, y = ops.mrotary_embedding(good[:, r], q[r], k[r], table, sections)
+        assert torch.equal(a[r], x) and torch.equal(b[r], y)
+
+
 def test_mrope_on_equal_axes_is_rope(ops):
     """Text rows: equal positions on every axis (one row, broadcast) give the one-axis bits."""
     from vlcache_b200.layers.rotary_embedding import rope_cos_sin_cache
@@ -399,8 +436,8 @@ def test_decode_fp4_strided_graph_streams(ops):
     out_wide = torch.zeros(3, H * D + 8, dtype=torch.bfloat16, device="cuda")
     out = out_wide[:, :H * D].view(3, H, D)
     ctx, table = torch.tensor(lens, dtype=torch.int32).cuda(), bt.cuda()
-    call = lambda o, w: ops.decode_attention_fp4(q, dk, dv, table, ctx, 3072, SCALE, out=o, workspace=w)  # noqa: E731
-    ws = [torch.empty(ops.decode_fp4_workspace_bytes(3, H, Hk, 3072), dtype=torch.uint8, device="cuda") for _ in "ab"]
+    call = lambda o, w: ops.decode_attention_fp4(q, dk, dv, table, ctx, 3328, SCALE, out=o, workspace=w)  # noqa: E731
+    ws = [torch.empty(ops.decode_fp4_workspace_bytes(3, H, Hk, 3328), dtype=torch.uint8, device="cuda") for _ in "ab"]
     assert ws[0].numel() > 0
     eager = call(None, None)
     assert torch.equal(call(out, ws[0]), eager) and not bool(out_wide[:, H * D:].any())

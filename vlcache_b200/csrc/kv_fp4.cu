@@ -15,28 +15,30 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Eight values of a group (codes of four bytes, one scale) as floats; exact.
-__device__ __forceinline__ void values8(uint32_t codes, uint32_t scale_byte, float (&v)[8]) {
+// Eight values of a group (codes of four bytes, its scale in both halves) as packed fp32 pairs; exact.
+__device__ __forceinline__ void values8(uint32_t codes, uint32_t scale2, uint64_t (&v)[4]) {
   uint32_t h[4];
   fp4::decode8(codes, h);
-  const uint32_t s = fp4::scales2_f16((scale_byte & 0xff) * 0x0101u);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t x = hmul2(h[i], s);
+    const uint32_t x = hmul2(h[i], scale2);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    v[i] = f2_pack(f.x, f.y);
   }
+}
+__device__ __forceinline__ uint32_t both_halves(uint32_t scale_byte) {
+  return fp4::scales2_f16((scale_byte & 0xff) * 0x0101u);
 }
 
 // ---------------------------------------------------------------------------
 // Read-back: row cu_seqlens_k[b] + j of the output is key j of sequence b, for every head, in
 // bf16 (exact: value = g * s * code).  Bound by the bf16 rows written (256 of the 328 bytes a row
-// and head moves).  A block takes 64 rows of one head, K or V, of one layer: sixteen lanes a row,
-// eight dims a lane, so a warp reads two rows' 128 bytes of codes and writes two rows' 256-byte
-// pieces; a lane has its four rows' loads in flight at once.
+// and head moves).  A block takes 64 rows of one head, K and V, of one layer: eight lanes a row, a
+// scale's group of 16 dims a lane, so a warp reads four rows' 256 bytes of codes and a lane writes
+// 32 bytes at once; all of a lane's loads (two rows of K and of V) are issued before the first use.
 // Block x is given sequence b and tile i with x = cu[b] / 64 + b + i: those starts leave every
 // sequence room for its ceil(len / 64) tiles, and a block past the last of them has nothing to do.
+// 2556 rows of 2 heads in 36 layers (121 MB): GATHER_US us.
 // ---------------------------------------------------------------------------
 struct GatherParams {
   const uint8_t* cache[2];
@@ -53,6 +55,7 @@ struct GatherParams {
   float scale[2];
   __nv_bfloat16* out[2];
   int64_t out_row_stride, out_layer_stride;
+  bool wide;  // outputs 32-byte aligned
 };
 
 __global__ void __launch_bounds__(256) gather_fp4_kernel(const __grid_constant__ GatherParams p) {
@@ -67,44 +70,59 @@ __global__ void __launch_bounds__(256) gather_fp4_kernel(const __grid_constant__
   const int len = __ldg(p.cu_seqlens_k + lo + 1) - (int)begin;
   const int64_t j0 = ((int64_t)blockIdx.x - (begin / TILE + lo)) * TILE;
   if (j0 < 0 || j0 >= len) return;
-  const int head = blockIdx.y;
-  const int layer = blockIdx.z >> 1, which = blockIdx.z & 1;
-  const int table_index = (int)(j0 / p.block_size);
+  const int head = blockIdx.y, layer = blockIdx.z;
+  const int table_index = (int)j0 / p.block_size;
   const int page = table_index < p.table_width ? __ldg(p.block_tables + lo * p.table_stride + table_index) : -1;
   const bool bad = page < 0 || page >= p.num_pages;
   if (bad && threadIdx.x == 0) record_error(VLC_DEV_ERR_BLOCK_RANGE);
   if ((begin < 0 || begin + len > p.total_k) && threadIdx.x == 0) record_error(VLC_DEV_ERR_LENGTH);
-  const uint8_t* src = p.cache[which] + layer * p.layer_stride +
-                       fp4::head_offset(bad ? 0 : page, p.num_kv_heads, head, p.block_size);
-  const int row0 = (int)(j0 % p.block_size);
-  const int c = threadIdx.x & 15;
-  constexpr int N = TILE / 16;
-  uint32_t codes[N], scales[N];
-  bool live[N];
+  const int64_t src = layer * p.layer_stride + fp4::head_offset(bad ? 0 : page, p.num_kv_heads, head, p.block_size);
+  const int row0 = (int)j0 - table_index * p.block_size;
+  const int c = threadIdx.x & 7;
+  uint2 codes[2][2];
+  uint32_t scales[2][2];
+  bool live[2];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int r = i * 16 + (threadIdx.x >> 4);
+  for (int i = 0; i < 2; ++i) {
+    const int r = i * 32 + (threadIdx.x >> 3);
     live[i] = j0 + r < len && begin >= 0 && begin + j0 + r < p.total_k;
-    codes[i] = scales[i] = 0;
-    if (live[i] && !bad) {
-      codes[i] = __ldg(reinterpret_cast<const uint32_t*>(src + fp4::code_offset(row0 + r)) + c);
-      scales[i] = __ldg(src + fp4::scale_offset(row0 + r, p.block_size) + (c >> 1));
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      codes[i][w] = make_uint2(0, 0);
+      scales[i][w] = 0;
+      if (live[i] && !bad) {
+        codes[i][w] = __ldg(reinterpret_cast<const uint2*>(p.cache[w] + src + fp4::code_offset(row0 + r)) + c);
+        scales[i][w] = __ldg(p.cache[w] + src + fp4::scale_offset(row0 + r, p.block_size) + c);
+      }
     }
   }
-  const float g = p.scale[which];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < 2; ++i) {
     if (!live[i]) continue;
-    const int r = i * 16 + (threadIdx.x >> 4);
-    float v[8];
-    values8(codes[i], scales[i], v);
-    uint4 u;
-    u.x = pack_bf16x2(v[0] * g, v[1] * g);
-    u.y = pack_bf16x2(v[2] * g, v[3] * g);
-    u.z = pack_bf16x2(v[4] * g, v[5] * g);
-    u.w = pack_bf16x2(v[6] * g, v[7] * g);
-    __nv_bfloat16* dst = p.out[which] + layer * p.out_layer_stride + (begin + j0 + r) * p.out_row_stride + head * HD;
-    *reinterpret_cast<uint4*>(dst + 8 * c) = u;
+    const int64_t at = layer * p.out_layer_stride + (begin + j0 + i * 32 + (threadIdx.x >> 3)) * p.out_row_stride +
+                       head * HD + 16 * c;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const uint32_t s = both_halves(scales[i][w]);
+      const uint64_t g = f2_pack(p.scale[w], p.scale[w]);
+      uint64_t v[2][4];
+      values8(codes[i][w].x, s, v[0]);
+      values8(codes[i][w].y, s, v[1]);
+      uint32_t u[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        float a, b;
+        f2_unpack(f2_mul(v[x >> 2][x & 3], g), a, b);
+        u[x] = pack_bf16x2(a, b);
+      }
+      if (p.wide) {
+        st_global_v8(p.out[w] + at, u);
+      } else {
+        uint4* dst = reinterpret_cast<uint4*>(p.out[w] + at);
+        dst[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        dst[1] = make_uint4(u[4], u[5], u[6], u[7]);
+      }
+    }
   }
 }
 
@@ -114,10 +132,12 @@ __global__ void __launch_bounds__(256) gather_fp4_kernel(const __grid_constant__
 // copied.  K is dequantised (exact), rotated in fp32 with every product and sum rounded by itself,
 // rounded to bf16 as a bf16 cache would hold it, and quantised again.  A group of 16 pairs that
 // the delta does not turn keeps its codes and scales: quantising again would move it.
-// Bound by HBM (288 bytes read and written per row and head).  Lanes: eight a row, eight pairs a
-// lane (dims 8c.. and 64 + 8c..), four consecutive rows a warp, kRows such rows a lane, all loads
+// 288 bytes are read and written per row and head; at the copy rate that leaves an SM some 25
+// instructions a byte-row lane, so the arithmetic counts as much: packed products, no division
+// (fp4.cuh), a row's pages found once for all of a lane's heads.  Lanes: eight a row, eight pairs a
+// lane (dims 8c.. and 64 + 8c..), four consecutive rows a warp, kHeads heads a lane, all loads
 // first; rows of an image lie next to each other in their pages, so a warp's loads are runs of
-// 256 bytes.
+// 256 bytes.  2556 rows of 2 heads in 36 layers (53 MB): SHIFT_US us.
 // ---------------------------------------------------------------------------
 struct ShiftParams {
   uint8_t* k_cache;
@@ -131,90 +151,88 @@ struct ShiftParams {
   float cos[HD / 2], sin[HD / 2];
 };
 
-constexpr int kRows = 2;
+constexpr int kHeads = 2;
 
 __global__ void __launch_bounds__(256) shift_fp4_kernel(const __grid_constant__ ShiftParams p) {
-  __shared__ float s_cos[HD / 2], s_sin[HD / 2];
+  __shared__ __align__(8) float s_cos[HD / 2], s_sin[HD / 2];
   if (threadIdx.x < HD / 2) {
     s_cos[threadIdx.x] = p.cos[threadIdx.x];
     s_sin[threadIdx.x] = p.sin[threadIdx.x];
   }
   __syncthreads();
-  const int head = blockIdx.y, layer = blockIdx.z;
+  const int head0 = blockIdx.y * kHeads, layer = blockIdx.z;
   const int c = threadIdx.x & 7;
   uint8_t* const k = p.k_cache + layer * p.layer_stride;
   uint8_t* const v = p.v_cache ? p.v_cache + layer * p.layer_stride : nullptr;
-  const int64_t num_slots = (int64_t)p.num_pages * p.block_size;
-  int64_t from[kRows], to[kRows];  // the head's piece of the page
-  int from_row[kRows], to_row[kRows];
-  bool live[kRows];
-  uint32_t lo[kRows], hi[kRows], s_lo[kRows], s_hi[kRows];
-  uint2 vc[kRows];
-  uint8_t vs[kRows];
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int r = (blockIdx.x * kRows + i) * 32 + (threadIdx.x >> 3);
-    live[i] = r < p.num_rows;
-    if (!live[i]) continue;
-    const int src = __ldg(p.src_slots + r);
-    const int dst = p.dst_slots ? __ldg(p.dst_slots + r) : src;
-    if (src < 0 || dst < 0 || src >= num_slots || dst >= num_slots) {
-      if (c == 0 && head == 0 && layer == 0) record_error(VLC_DEV_ERR_SLOT_RANGE);
-      live[i] = false;
-      continue;
-    }
-    from_row[i] = src % p.block_size;
-    to_row[i] = dst % p.block_size;
-    from[i] = fp4::head_offset(src / p.block_size, p.num_kv_heads, head, p.block_size);
-    to[i] = fp4::head_offset(dst / p.block_size, p.num_kv_heads, head, p.block_size);
-    const uint8_t* kc = k + from[i] + fp4::code_offset(from_row[i]);
-    lo[i] = reinterpret_cast<const uint32_t*>(kc)[c];
-    hi[i] = reinterpret_cast<const uint32_t*>(kc)[8 + c];
-    const uint8_t* ks = k + from[i] + fp4::scale_offset(from_row[i], p.block_size);
-    s_lo[i] = ks[c >> 1];
-    s_hi[i] = ks[4 + (c >> 1)];
-    if (v) {
-      vc[i] = reinterpret_cast<const uint2*>(v + from[i] + fp4::code_offset(from_row[i]))[c];
-      vs[i] = v[from[i] + fp4::scale_offset(from_row[i], p.block_size) + c];
+  const int r = blockIdx.x * 32 + (threadIdx.x >> 3);
+  bool live = r < p.num_rows;
+  int src = 0, dst = 0;
+  if (live) {
+    src = __ldg(p.src_slots + r);
+    dst = p.dst_slots ? __ldg(p.dst_slots + r) : src;
+    const uint32_t num_slots = (uint32_t)p.num_pages * (uint32_t)p.block_size;
+    if ((uint32_t)src >= num_slots || (uint32_t)dst >= num_slots) {
+      if (c == 0 && head0 == 0 && layer == 0) record_error(VLC_DEV_ERR_SLOT_RANGE);
+      live = false;
     }
   }
+  const int head_bytes = p.block_size * fp4::ROW_BYTES;
+  const int src_page = src / p.block_size, src_row = src - src_page * p.block_size;
+  const int dst_page = dst / p.block_size, dst_row = dst - dst_page * p.block_size;
+  const int64_t from = ((int64_t)src_page * p.num_kv_heads + head0) * head_bytes;
+  const int64_t to = ((int64_t)dst_page * p.num_kv_heads + head0) * head_bytes;
+  const int from_codes = fp4::code_offset(src_row), from_scales = fp4::scale_offset(src_row, p.block_size);
+  const int to_codes = fp4::code_offset(dst_row), to_scales = fp4::scale_offset(dst_row, p.block_size);
+  uint32_t lo[kHeads], hi[kHeads], s_lo[kHeads], s_hi[kHeads];
+  uint2 vc[kHeads];
+  uint8_t vs[kHeads];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    float x1[8], x2[8];
-    if (live[i]) {
-      values8(lo[i], s_lo[i], x1);
-      values8(hi[i], s_hi[i], x2);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x1[e] = x2[e] = 0.f;
+  for (int i = 0; i < kHeads; ++i) {
+    lo[i] = hi[i] = s_lo[i] = s_hi[i] = 0;
+    if (!live || head0 + i >= p.num_kv_heads) continue;
+    const uint8_t* kf = k + from + i * head_bytes;
+    lo[i] = reinterpret_cast<const uint32_t*>(kf + from_codes)[c];
+    hi[i] = reinterpret_cast<const uint32_t*>(kf + from_codes)[8 + c];
+    s_lo[i] = kf[from_scales + (c >> 1)];
+    s_hi[i] = kf[from_scales + 4 + (c >> 1)];
+    if (v) {
+      const uint8_t* vf = v + from + i * head_bytes;
+      vc[i] = reinterpret_cast<const uint2*>(vf + from_codes)[c];
+      vs[i] = vf[from_scales + c];
     }
+  }
+  uint64_t cs[4], sn[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float cs = s_cos[8 * c + e], sn = s_sin[8 * c + e];
-      const float y1 = __fsub_rn(__fmul_rn(x1[e], cs), __fmul_rn(x2[e], sn));
-      const float y2 = __fadd_rn(__fmul_rn(x2[e], cs), __fmul_rn(x1[e], sn));
-      x1[e] = __bfloat162float(__float2bfloat16_rn(y1));
-      x2[e] = __bfloat162float(__float2bfloat16_rn(y2));
-    }
-    uint32_t m1 = fp4::absmax8_bits(x1), m2 = fp4::absmax8_bits(x2);
+  for (int i = 0; i < 4; ++i) {
+    cs[i] = *reinterpret_cast<const uint64_t*>(s_cos + 8 * c + 2 * i);
+    sn[i] = *reinterpret_cast<const uint64_t*>(s_sin + 8 * c + 2 * i);
+  }
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    uint64_t x1[4], x2[4];
+    values8(lo[i], both_halves(s_lo[i]), x1);
+    values8(hi[i], both_halves(s_hi[i]), x2);
+    fp4::rotate8(x1, x2, cs, sn);
+    const uint4 y1 = fp4::pack8(x1), y2 = fp4::pack8(x2);
+    uint32_t m1 = fp4::absmax8(y1), m2 = fp4::absmax8(y2);
     m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
     m2 = max(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
-    if (!live[i]) continue;
+    if (!live || head0 + i >= p.num_kv_heads) continue;
     if ((p.turned >> (c >> 1)) & 1) {
-      s_lo[i] = fp4::encode_scale(__uint_as_float(m1));
-      s_hi[i] = fp4::encode_scale(__uint_as_float(m2));
-      lo[i] = fp4::quantise8(x1, s_lo[i]);
-      hi[i] = fp4::quantise8(x2, s_hi[i]);
+      s_lo[i] = fp4::encode_scale(m1, 1.f);
+      s_hi[i] = fp4::encode_scale(m2, 1.f);
+      lo[i] = fp4::quantise8(y1, fp4::inverse_scale(s_lo[i], 1.f));
+      hi[i] = fp4::quantise8(y2, fp4::inverse_scale(s_hi[i], 1.f));
     }
-    uint32_t* kc = reinterpret_cast<uint32_t*>(k + to[i] + fp4::code_offset(to_row[i]));
-    kc[c] = lo[i];
-    kc[8 + c] = hi[i];
-    uint8_t* ks = k + to[i] + fp4::scale_offset(to_row[i], p.block_size);
-    if ((c & 1) == 0) ks[c >> 1] = (uint8_t)s_lo[i];
-    else ks[4 + (c >> 1)] = (uint8_t)s_hi[i];
+    uint8_t* kt = k + to + i * head_bytes;
+    reinterpret_cast<uint32_t*>(kt + to_codes)[c] = lo[i];
+    reinterpret_cast<uint32_t*>(kt + to_codes)[8 + c] = hi[i];
+    if ((c & 1) == 0) kt[to_scales + (c >> 1)] = (uint8_t)s_lo[i];
+    else kt[to_scales + 4 + (c >> 1)] = (uint8_t)s_hi[i];
     if (v) {
-      reinterpret_cast<uint2*>(v + to[i] + fp4::code_offset(to_row[i]))[c] = vc[i];
-      v[to[i] + fp4::scale_offset(to_row[i], p.block_size) + c] = vs[i];
+      uint8_t* vt = v + to + i * head_bytes;
+      reinterpret_cast<uint2*>(vt + to_codes)[c] = vc[i];
+      vt[to_scales + c] = vs[i];
     }
   }
 }
@@ -273,7 +291,9 @@ extern "C" int vlc_gather_kvcache_fp4(const void* k_cache, const void* v_cache, 
   p.out[1] = (__nv_bfloat16*)v_out;
   p.out_row_stride = out_row_stride;
   p.out_layer_stride = out_layer_stride;
-  const dim3 grid((unsigned)(total_k / TILE + num_seqs), num_kv_heads, 2 * num_layers);
+  p.wide = reinterpret_cast<uintptr_t>(k_out) % 32 == 0 && reinterpret_cast<uintptr_t>(v_out) % 32 == 0 &&
+           out_row_stride % 16 == 0 && out_layer_stride % 16 == 0;
+  const dim3 grid((unsigned)(total_k / TILE + num_seqs), num_kv_heads, num_layers);
   gather_fp4_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(p);
   return launch_status();
 }
@@ -313,7 +333,7 @@ extern "C" int vlc_mrope_shift_fp4(void* k_cache, void* v_cache, int64_t layer_s
     p.sin[j] = (float)sin(a);
     if (delta_thw[axis] != 0) p.turned |= 1u << (j / fp4::GROUP);
   }
-  const dim3 grid((num_rows + 32 * kRows - 1) / (32 * kRows), num_kv_heads, num_layers);
+  const dim3 grid((num_rows + 31) / 32, (num_kv_heads + kHeads - 1) / kHeads, num_layers);
   shift_fp4_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(p);
   return launch_status();
 }

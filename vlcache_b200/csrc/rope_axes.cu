@@ -9,11 +9,18 @@
 // kernel of this library does, so that equal positions on all axes give its bits.  The 4-bit
 // cache holds the quantised bf16 row: the same rows whether the rotation is fused or not.
 //
-// Bound by HBM: each row element is read once and written once.  A warp takes one token and
-// `kIters` groups of four consecutive heads (query, key and value heads counted through): eight
-// lanes a head, eight pairs a lane, so a group's loads are 128-byte pieces, and every load of the
-// warp's groups is issued before the first use.  A lane's cos/sin values depend on the token and
-// its pairs only: they are loaded once and serve all its heads.
+// Bound by HBM: each row element is read once and written once.  Two kernels:
+//  * rope_axes_kernel, few tokens: a warp takes one token and kIters groups of four consecutive
+//    heads (query, key and value heads counted through), eight lanes a head, eight pairs a lane;
+//    every load of the warp's groups is issued before the first use, the cos/sin values are loaded
+//    once for them.  A decode step's tokens spread over as many SMs as there are slices.
+//  * rope_stream_kernel, many tokens: the same slices taken by persistent warps.  Every lane keeps
+//    the row pieces of its next two slices in flight into a place of its own in shared memory
+//    (16-byte asynchronous copies: no registers, no barrier, only its own copies to wait for), and
+//    loads the positions two slices and the table values one slice ahead.
+//    10617 tokens of 28 + 4 + 4 heads into bf16 pages: 35.3 us against 41 with the first kernel
+//    (196 MB, 31 us at the copy rate); whole tokens brought and taken by bulk copies into rings of
+//    eight warps measured 41 too, each token waiting for the stores of the one before.
 #include <cmath>
 
 #include "fp4.cuh"
@@ -57,28 +64,109 @@ struct Params {
   int warps_per_token;
 };
 
-__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+// cos and sin of pairs 8c .. 8c + 7 as packed pairs, from the table rows of the axes.
+template <typename RowOf>
+__device__ __forceinline__ void load_angles(const Params& p, int c, RowOf row_of, uint64_t (&cs)[4],
+                                            uint64_t (&sn)[4]) {
+  if (!p.mixed) {
+    int x = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = __bfloat1622float2(h[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
+    for (int i = 1; i < kMaxAxes; ++i)
+      if (i < p.num_axes && 8 * c >= p.section_end[i - 1]) x = i;
+    const float4* row = reinterpret_cast<const float4*>(row_of(x));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 u = row[2 * c + i], v = row[HALF / 4 + 2 * c + i];
+      cs[2 * i] = f2_pack(u.x, u.y);
+      cs[2 * i + 1] = f2_pack(u.z, u.w);
+      sn[2 * i] = f2_pack(v.x, v.y);
+      sn[2 * i + 1] = f2_pack(v.z, v.w);
+    }
+  } else {
+    float u[8], v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = 8 * c + i;
+      int x = 0;
+#pragma unroll
+      for (int k = 1; k < kMaxAxes; ++k)
+        if (k < p.num_axes && j >= p.section_end[k - 1]) x = k;
+      u[i] = row_of(x)[j];
+      v[i] = row_of(x)[HALF + j];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      cs[i] = f2_pack(u[2 * i], u[2 * i + 1]);
+      sn[i] = f2_pack(v[2 * i], v[2 * i + 1]);
+    }
   }
 }
 
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint4 u;
-  u.x = pack_bf16x2(f[0], f[1]);
-  u.y = pack_bf16x2(f[2], f[3]);
-  u.z = pack_bf16x2(f[4], f[5]);
-  u.w = pack_bf16x2(f[6], f[7]);
-  return u;
+// Dims 8c .. (a) and 64 + 8c .. (b) of a head's row into its place in the 4-bit cache.  The groups
+// are c / 2 and 4 + c / 2, each shared by two neighbouring lanes: all lanes of the warp come here,
+// those without a row (dst null) too.
+__device__ __forceinline__ void store_fp4(uint8_t* dst, const uint4& a, const uint4& b, float inv_g, int c, int row,
+                                          int block_size) {
+  uint32_t m1 = fp4::absmax8(a), m2 = fp4::absmax8(b);
+  m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
+  m2 = max(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
+  if (!dst) return;
+  const uint32_t s1 = fp4::encode_scale(m1, inv_g), s2 = fp4::encode_scale(m2, inv_g);
+  uint32_t* codes = reinterpret_cast<uint32_t*>(dst + fp4::code_offset(row));
+  codes[c] = fp4::quantise8(a, fp4::inverse_scale(s1, inv_g));
+  codes[8 + c] = fp4::quantise8(b, fp4::inverse_scale(s2, inv_g));
+  uint8_t* scales = dst + fp4::scale_offset(row, block_size);
+  if ((c & 1) == 0) scales[c >> 1] = (uint8_t)s1;
+  else scales[4 + (c >> 1)] = (uint8_t)s2;
+}
+
+// Eight pairs of a head's row (a: dims 8c.., b: 64 + 8c..) to where they belong: turned when the
+// head is a query or key head, and quantised for the 4-bit cache.  All lanes of a warp come here.
+template <int SINK, bool ROTATE>
+__device__ __forceinline__ void put_head(const Params& p, int64_t token, int head, int c, uint4 a, uint4 b,
+                                         const uint64_t (&cs)[4], const uint64_t (&sn)[4], bool placed, bool stored,
+                                         int slot) {
+  const int q_heads = ROTATE ? p.num_heads : 0;
+  const bool is_q = head < q_heads;
+  const bool is_k = !is_q && head < q_heads + p.num_kv_heads;
+  const bool is_v = !is_q && !is_k && head < q_heads + 2 * p.num_kv_heads;
+  if (ROTATE && (is_q || is_k)) {
+    uint64_t x1[4], x2[4];
+    fp4::unpack8(a, x1);
+    fp4::unpack8(b, x2);
+    fp4::rotate8(x1, x2, cs, sn);
+    a = fp4::pack8(x1);
+    b = fp4::pack8(x2);
+  }
+  const int kv_head = head - q_heads - (is_v ? p.num_kv_heads : 0);
+  const bool keep = stored && ((is_k && placed) || is_v);  // a row for the cache
+  __nv_bfloat16* dst = nullptr;
+  if (is_q) {
+    if (placed) dst = p.q_out + token * p.q_out_stride + head * HD;
+  } else if (SINK == kRows) {
+    if (is_k && placed) dst = (__nv_bfloat16*)p.k_cache + token * p.k_out_stride + kv_head * HD;
+  } else if (SINK == kBf16Cache) {
+    if (keep) dst = (__nv_bfloat16*)(is_v ? p.v_cache : p.k_cache) + ((int64_t)slot * p.num_kv_heads + kv_head) * HD;
+  }
+  if (dst) {
+    *reinterpret_cast<uint4*>(dst + 8 * c) = a;
+    *reinterpret_cast<uint4*>(dst + HALF + 8 * c) = b;
+  }
+  if (SINK == kFp4Cache && __any_sync(0xffffffffu, is_k || is_v)) {
+    uint8_t* row = nullptr;
+    int at = 0;
+    if (keep) {
+      const int page = slot / p.block_size;
+      at = slot - page * p.block_size;
+      row = (uint8_t*)(is_v ? p.v_cache : p.k_cache) + fp4::head_offset(page, p.num_kv_heads, kv_head, p.block_size);
+    }
+    store_fp4(row, a, b, is_v ? p.v_inv_scale : p.k_inv_scale, c, at, p.block_size);
+  }
 }
 
 // ROTATE false: no positions and no query heads (the plain 4-bit scatter).
 template <int SINK, bool ROTATE>
-__global__ void __launch_bounds__(kWarps * 32) rope_axes_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kWarps * 32, 4) rope_axes_kernel(const __grid_constant__ Params p) {
   pdl_launch_dependents();  // the attention that follows may start its prologue
   const int64_t warp = (int64_t)blockIdx.x * kWarps + warp_id();
   const int64_t token = warp / p.warps_per_token;
@@ -115,7 +203,7 @@ __global__ void __launch_bounds__(kWarps * 32) rope_axes_kernel(const __grid_con
     stored = slot >= 0 && slot < p.num_slots;
     if (!stored && slot != -1 && lane == 0 && slice == 0) record_error(VLC_DEV_ERR_SLOT_RANGE);
   }
-  float cv[8], sv[8];
+  uint64_t cs[4], sn[4];
   bool placed = true;  // every axis' position is inside the table
   if (ROTATE) {
     int64_t pos[kMaxAxes];
@@ -124,103 +212,134 @@ __global__ void __launch_bounds__(kWarps * 32) rope_axes_kernel(const __grid_con
       pos[x] = x < p.num_axes ? __ldg(p.positions + x * p.axis_stride + token) : 0;
       placed = placed && pos[x] >= 0 && pos[x] < p.max_position;
     }
-    if (!placed) {
-      if (lane == 0 && slice == 0) record_error(VLC_DEV_ERR_POSITION);
+    if (!placed && lane == 0 && slice == 0) record_error(VLC_DEV_ERR_POSITION);
+    load_angles(
+        p, c, [&](int x) {
+          int64_t at = pos[0];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) cv[i] = sv[i] = 0.f;
-    } else if (!p.mixed) {
-      int64_t at = pos[0];
-#pragma unroll
-      for (int x = 1; x < kMaxAxes; ++x)
-        if (x < p.num_axes && 8 * c >= p.section_end[x - 1]) at = pos[x];
-      const float4* row = reinterpret_cast<const float4*>(p.cos_sin + at * HD);
-      *reinterpret_cast<float4*>(&cv[0]) = __ldg(row + 2 * c);
-      *reinterpret_cast<float4*>(&cv[4]) = __ldg(row + 2 * c + 1);
-      *reinterpret_cast<float4*>(&sv[0]) = __ldg(row + HALF / 4 + 2 * c);
-      *reinterpret_cast<float4*>(&sv[4]) = __ldg(row + HALF / 4 + 2 * c + 1);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = 8 * c + i;
-        int64_t at = pos[0];
-#pragma unroll
-        for (int x = 1; x < kMaxAxes; ++x)
-          if (x < p.num_axes && j >= p.section_end[x - 1]) at = pos[x];
-        cv[i] = __ldg(p.cos_sin + at * HD + j);
-        sv[i] = __ldg(p.cos_sin + at * HD + HALF + j);
-      }
-    }
+          for (int i = 1; i < kMaxAxes; ++i)
+            if (x == i) at = pos[i];
+          return p.cos_sin + (placed ? at : 0) * HD;
+        }, cs, sn);
   }
-  const int64_t page = SINK == kFp4Cache ? slot / p.block_size : 0;
-  const int row = SINK == kFp4Cache ? (int)(slot - page * p.block_size) : 0;
+#pragma unroll
+  for (int it = 0; it < kIters; ++it)
+    put_head<SINK, ROTATE>(p, token, first + it * 4, c, a[it], b[it], cs, sn, placed, stored, slot);
+}
 
-#pragma unroll
-  for (int it = 0; it < kIters; ++it) {
-    const int head = first + it * 4;
-    const bool is_q = head < q_heads;
-    const bool is_k = !is_q && head < q_heads + p.num_kv_heads;
-    const bool is_v = !is_q && !is_k && head < all_heads;
-    float x1[8], x2[8];
-    if (ROTATE && (is_q || is_k)) {
-      unpack8(a[it], x1);
-      unpack8(b[it], x2);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y1 = __fsub_rn(__fmul_rn(x1[i], cv[i]), __fmul_rn(x2[i], sv[i]));
-        const float y2 = __fadd_rn(__fmul_rn(x2[i], cv[i]), __fmul_rn(x1[i], sv[i]));
-        x1[i] = y1;
-        x2[i] = y2;
-      }
-      a[it] = pack8(x1);
-      b[it] = pack8(x2);
+constexpr int kStreamWarps = 20;   // one block an SM: 102 registers a thread
+constexpr int kStreamStages = 3;   // slices of rows a lane has in shared memory
+constexpr int kStreamBytes = kStreamWarps * kStreamStages * kIters * 2 * 32 * 16;
+
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+template <int SINK>
+__global__ void __launch_bounds__(kStreamWarps * 32, 1) rope_stream_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(16) uint4 rows[];  // [warp][stage][2 it + half][lane]
+  pdl_launch_dependents();
+  const int lane = lane_id(), c = lane & 7;
+  uint4* const mine = rows + (warp_id() * kStreamStages) * (kIters * 2 * 32) + lane;
+  const int heads = p.num_heads + 2 * p.num_kv_heads;
+  // Slices of a token: this warp's are every (blocks * warps)-th of all.
+  struct Unit {
+    int token, slice;
+  };
+  const int per_token = p.warps_per_token;
+  const int stride = gridDim.x * kStreamWarps, stride_tokens = stride / per_token,
+            stride_slices = stride - stride_tokens * per_token;
+  auto after = [&](const Unit& u) {
+    Unit n{u.token + stride_tokens, u.slice + stride_slices};
+    if (n.slice >= per_token) {
+      n.slice -= per_token;
+      ++n.token;
     }
-    if (is_q) {
-      if (placed) {
-        __nv_bfloat16* dst = p.q_out + token * p.q_out_stride + head * HD;
-        *reinterpret_cast<uint4*>(dst + 8 * c) = a[it];
-        *reinterpret_cast<uint4*>(dst + HALF + 8 * c) = b[it];
-      }
-    }
-    if (SINK != kFp4Cache) {
-      const int kv_head = head - q_heads - (is_v ? p.num_kv_heads : 0);
-      __nv_bfloat16* dst = nullptr;
-      if (SINK == kRows) {
-        if (is_k && placed) dst = (__nv_bfloat16*)p.k_cache + token * p.k_out_stride + kv_head * HD;
-      } else if (stored && ((is_k && placed) || is_v)) {
-        dst = (__nv_bfloat16*)(is_v ? p.v_cache : p.k_cache) + ((int64_t)slot * p.num_kv_heads + kv_head) * HD;
-      }
-      if (dst) {
-        *reinterpret_cast<uint4*>(dst + 8 * c) = a[it];
-        *reinterpret_cast<uint4*>(dst + HALF + 8 * c) = b[it];
-      }
-    } else if (__any_sync(0xffffffffu, is_k || is_v)) {
-      // Lane c holds dims 8c.. of group c / 2 and dims 64 + 8c.. of group 4 + c / 2: a group's
-      // maximum is that of two neighbouring lanes.
-      const float inv = is_v ? p.v_inv_scale : p.k_inv_scale;
-      unpack8(a[it], x1);
-      unpack8(b[it], x2);
+    return n;
+  };
+  auto copy_rows = [&](const Unit& u, int stage) {
+    if (u.token < p.num_tokens) {
+      const int first = u.slice * (kIters * 4) + (lane >> 3);
+      const int64_t token = u.token;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x1[i] *= inv;
-        x2[i] *= inv;
-      }
-      uint32_t m1 = fp4::absmax8_bits(x1), m2 = fp4::absmax8_bits(x2);
-      m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
-      m2 = max(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
-      if (stored && ((is_k && placed) || is_v)) {
-        const int kv_head = head - q_heads - (is_v ? p.num_kv_heads : 0);
-        const uint32_t s1 = fp4::encode_scale(__uint_as_float(m1));
-        const uint32_t s2 = fp4::encode_scale(__uint_as_float(m2));
-        uint8_t* dst = (uint8_t*)(is_v ? p.v_cache : p.k_cache) +
-                       fp4::head_offset(page, p.num_kv_heads, kv_head, p.block_size);
-        uint32_t* codes = reinterpret_cast<uint32_t*>(dst + fp4::code_offset(row));
-        codes[c] = fp4::quantise8(x1, s1);
-        codes[8 + c] = fp4::quantise8(x2, s2);
-        uint8_t* scales = dst + fp4::scale_offset(row, p.block_size);
-        if ((c & 1) == 0) scales[c >> 1] = (uint8_t)s1;
-        else scales[4 + (c >> 1)] = (uint8_t)s2;
+      for (int it = 0; it < kIters; ++it) {
+        const int head = first + it * 4;
+        const __nv_bfloat16* src;
+        if (head < p.num_heads) src = p.q + token * p.q_stride + head * HD;
+        else if (head < p.num_heads + p.num_kv_heads) src = p.key + token * p.key_stride + (head - p.num_heads) * HD;
+        else if (SINK != kRows && head < heads)
+          src = p.value + token * p.value_stride + (head - p.num_heads - p.num_kv_heads) * HD;
+        else continue;
+        uint4* dst = mine + (stage * kIters + it) * 64;
+        copy_async16(dst, src + 8 * c);
+        copy_async16(dst + 32, src + HALF + 8 * c);
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int64_t pos[kMaxAxes];  // of the slice after the next, and its slot
+  int slot_after = -1;
+  auto load_positions = [&](const Unit& u) {
+    const int64_t token = u.token < p.num_tokens ? u.token : 0;
+#pragma unroll
+    for (int x = 0; x < kMaxAxes; ++x) pos[x] = x < p.num_axes ? __ldg(p.positions + x * p.axis_stride + token) : 0;
+    if (SINK != kRows) slot_after = __ldg(p.slot_mapping + token);
+  };
+  uint64_t cs_next[4], sn_next[4];  // of the next slice
+  bool placed_next;
+  int slot_next = -1;
+  auto load_table = [&]() {
+    placed_next = true;
+#pragma unroll
+    for (int x = 0; x < kMaxAxes; ++x) placed_next = placed_next && pos[x] >= 0 && pos[x] < p.max_position;
+    slot_next = slot_after;
+    load_angles(
+        p, c, [&](int x) {
+          int64_t at = pos[0];
+#pragma unroll
+          for (int i = 1; i < kMaxAxes; ++i)
+            if (x == i) at = pos[i];
+          return p.cos_sin + (placed_next ? at : 0) * HD;
+        }, cs_next, sn_next);
+  };
+
+  const int start = warp_id() * gridDim.x + blockIdx.x;
+  Unit u0{start / per_token, start % per_token}, u1 = after(u0), u2 = after(u1);
+  static_assert(kStreamStages == 3, "rows are two slices ahead, as positions are");
+  copy_rows(u0, 0);
+  copy_rows(u1, 1);
+  load_positions(u0);
+  load_table();
+  load_positions(u1);
+  for (int stage = 0; u0.token < p.num_tokens; stage = stage == 2 ? 0 : stage + 1) {
+    uint64_t cs[4], sn[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      cs[i] = cs_next[i];
+      sn[i] = sn_next[i];
+    }
+    const bool placed = placed_next;
+    const int slot = slot_next;
+    load_table();
+    load_positions(u2);
+    copy_rows(u2, stage == 0 ? 2 : stage - 1);
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
+
+    const int token = u0.token;
+    const int first = u0.slice * (kIters * 4) + (lane >> 3);
+    const bool stored = slot >= 0 && slot < p.num_slots;
+    if (lane == 0 && u0.slice == 0) {
+      if (!placed) record_error(VLC_DEV_ERR_POSITION);
+      if (SINK != kRows && !stored && slot != -1) record_error(VLC_DEV_ERR_SLOT_RANGE);
+    }
+#pragma unroll
+    for (int it = 0; it < kIters; ++it) {
+      const uint4* src = mine + (stage * kIters + it) * 64;
+      put_head<SINK, true>(p, token, first + it * 4, c, src[0], src[32], cs, sn, placed, stored, slot);
+    }
+    u0 = u1;
+    u1 = u2;
+    u2 = after(u2);
   }
 }
 
@@ -249,6 +368,19 @@ template <int SINK, bool ROTATE>
 static int launch(Params& p, cudaStream_t stream) {
   const int heads = (ROTATE ? p.num_heads : 0) + (SINK == kRows ? 1 : 2) * p.num_kv_heads;
   p.warps_per_token = (heads + 4 * kIters - 1) / (4 * kIters);
+  if constexpr (ROTATE) {
+    // Where every persistent warp gets four slices and more: below, filling and draining their copies
+    // costs more than it saves (36 heads: 3001 tokens 14.0 against 12.7 us, 4500 tokens 17.0 against
+    // 18.5; 20 heads: 4500 tokens 13.0 against 11.4).
+    const int sms = vlc_num_sms();
+    if ((int64_t)p.num_tokens * p.warps_per_token >= 4ll * sms * kStreamWarps && p.num_tokens <= 0x3fffffff) {
+      static std::atomic<uint64_t> smem_set{0};
+      if (ensure_dynamic_smem((const void*)rope_stream_kernel<SINK>, kStreamBytes, smem_set) != VLC_OK)
+        return VLC_ERR_CUDA;
+      rope_stream_kernel<SINK><<<sms, kStreamWarps * 32, kStreamBytes, stream>>>(p);
+      return launch_status();
+    }
+  }
   const int64_t grid = ((int64_t)p.num_tokens * p.warps_per_token + kWarps - 1) / kWarps;
   if (grid > 0x7fffffff) return VLC_ERR_SHAPE;
   rope_axes_kernel<SINK, ROTATE><<<(unsigned)grid, kWarps * 32, 0, stream>>>(p);
