@@ -644,6 +644,10 @@ static int grid_warps(int num_seqs, int num_heads, int num_kv_heads, int max_con
   return (int)std::max<int64_t>(1, std::min(resident, most));
 }
 
+static int64_t workspace_bytes_for(int64_t warps, int group) {
+  return warps * 2 * group * (HD + 2) * (int64_t)sizeof(float);
+}
+
 static bool power_of_two(float g) {
   int e;
   return std::isfinite(g) && g > 0.f && std::frexp(g, &e) == 0.5f && e >= -63 && e <= 65;
@@ -657,8 +661,9 @@ using namespace vlc::decode_fp4;
 
 extern "C" int64_t vlc_decode_fp4_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int max_context_len) {
   if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_context_len < 0) return 0;
-  const int64_t warps = grid_warps(num_seqs, num_heads, num_kv_heads, std::max(max_context_len, 1), vlc_num_sms());
-  return warps * 2 * (num_heads / num_kv_heads) * (HD + 2) * (int64_t)sizeof(float);
+  return workspace_bytes_for(
+      grid_warps(num_seqs, num_heads, num_kv_heads, std::max(max_context_len, 1), vlc_num_sms()),
+      num_heads / num_kv_heads);
 }
 
 extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_seqs, int num_heads,
@@ -684,7 +689,7 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   if (num_kv_heads > 65535 || num_seqs > 65535 || num_heads > 65535) return VLC_ERR_SHAPE;
   if (max_context_len == 0) max_context_len = 1;
   const int warps = grid_warps(num_seqs, num_heads, num_kv_heads, max_context_len, vlc_num_sms());
-  const int64_t need = vlc_decode_fp4_workspace_size(num_seqs, num_heads, num_kv_heads, max_context_len);
+  const int64_t need = workspace_bytes_for(warps, G);
   if (!workspace || workspace_bytes < need) return VLC_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 32) return VLC_ERR_ALIGN;
 

@@ -147,13 +147,14 @@ struct ShiftParams {
   const int32_t* src_slots;
   const int32_t* dst_slots;
   int num_rows;
+  int block_shift;  // log2 of a block size that is a power of two, else -1
   uint32_t turned;  // bit m: group m of 16 pairs turns
   float cos[HD / 2], sin[HD / 2];
 };
 
 constexpr int kHeads = 2;
 
-__global__ void __launch_bounds__(256) shift_fp4_kernel(const __grid_constant__ ShiftParams p) {
+__global__ void __launch_bounds__(256, 4) shift_fp4_kernel(const __grid_constant__ ShiftParams p) {
   __shared__ __align__(8) float s_cos[HD / 2], s_sin[HD / 2];
   if (threadIdx.x < HD / 2) {
     s_cos[threadIdx.x] = p.cos[threadIdx.x];
@@ -177,8 +178,9 @@ __global__ void __launch_bounds__(256) shift_fp4_kernel(const __grid_constant__ 
     }
   }
   const int head_bytes = p.block_size * fp4::ROW_BYTES;
-  const int src_page = src / p.block_size, src_row = src - src_page * p.block_size;
-  const int dst_page = dst / p.block_size, dst_row = dst - dst_page * p.block_size;
+  const int src_page = p.block_shift >= 0 ? src >> p.block_shift : src / p.block_size;
+  const int dst_page = p.block_shift >= 0 ? dst >> p.block_shift : dst / p.block_size;
+  const int src_row = src - src_page * p.block_size, dst_row = dst - dst_page * p.block_size;
   const int64_t from = ((int64_t)src_page * p.num_kv_heads + head0) * head_bytes;
   const int64_t to = ((int64_t)dst_page * p.num_kv_heads + head0) * head_bytes;
   const int from_codes = fp4::code_offset(src_row), from_scales = fp4::scale_offset(src_row, p.block_size);
@@ -325,6 +327,9 @@ extern "C" int vlc_mrope_shift_fp4(void* k_cache, void* v_cache, int64_t layer_s
   p.src_slots = src_slots;
   p.dst_slots = dst_slots;
   p.num_rows = num_rows;
+  p.block_shift = -1;
+  for (int s = 6; s < 31; ++s)
+    if (block_size == 1 << s) p.block_shift = s;
   p.turned = 0;
   for (int j = 0; j < HD / 2; ++j) {
     const int axis = j < mrope_section[0] ? 0 : (j < mrope_section[0] + mrope_section[1] ? 1 : 2);

@@ -6,7 +6,6 @@ the CPU are rejected (there is no CPU path in the product).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -554,62 +553,85 @@ def xxh64(data: bytes | np.ndarray, seed: int = 0) -> int:
 
 
 # --------------------------------------------------------------------------- several-axes rotary
-_SAME_DEVICE = contextlib.nullcontext()
-
-
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
 
 
-def _on_device_of(first: torch.Tensor, *others: torch.Tensor | None):
-    """Context in which the tensors' (one) device is the current one."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise ValueError("vlcache_b200 ops run on CUDA tensors only (no CPU fallback)")
+def _device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """Index of the CUDA device that all the tensors are on."""
+    dev = first.get_device()
     for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}: one call takes one device")
-    return _SAME_DEVICE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {first.device} and {t.device}: one call takes one device")
+    if dev < 0:
+        raise ValueError("vlcache_b200 ops run on CUDA tensors only (no CPU fallback)")
+    return dev
 
 
-def _rows(t: torch.Tensor, name: str) -> None:
-    """``t`` is bf16 [N, heads, D] with contiguous heads (any token stride)."""
-    _need(t.dtype == torch.bfloat16 and t.dim() == 3, f"{name}: bf16 [tokens, heads, head_dim]")
-    n, h, d = t.shape
-    _need(t.stride(2) == 1 and (h == 1 or t.stride(1) == d), f"{name}: the heads of a token must be contiguous")
+def _launch(dev: int, name: str, *args) -> None:
+    """Call a C-ABI entry point on device ``dev`` and its current stream (the last argument)."""
+    fn = getattr(lib(), name)
+    if dev == torch.cuda.current_device():
+        status = fn(*args, _stream())
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _stream())
+    if status != 0:
+        check(name, status)
 
 
-def _token_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int, int]:
+    """(tokens, heads, head_dim, token stride) of bf16 rows [tokens, heads, head_dim] with
+    contiguous heads (any token stride)."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype != torch.bfloat16 or len(shape) != 3:
+        raise ValueError(f"{name}: bf16 [tokens, heads, head_dim]")
+    n, h, d = shape
+    if stride[2] != 1 or (h > 1 and stride[1] != d):
+        raise ValueError(f"{name}: the heads of a token must be contiguous")
+    return n, h, d, stride[0] if n > 1 else h * d
 
 
-def _rotary_args(positions, query, key, cos_sin_cache, sections):
-    """Checks shared by the rotating ops; returns (axes, sections array, axis stride, table rows)."""
-    _rows(query, "query")
-    _rows(key, "key")
-    n, _, d = query.shape
-    _need(key.shape[0] == n and key.shape[2] == d, "query and key: the same tokens and head_dim")
+_SECTIONS: dict = {}   # pairs per axis -> the C array of them
+
+
+def _rotary_args(positions, cos_sin_cache, sections, n: int, d: int):
+    """Positions and table of the rotating ops; returns (axis stride, axes, sections array, table rows)."""
     if sections is None:
         _need(positions.dim() == 1, "positions [tokens] (or [axes, tokens] with mrope_section)")
         sections = (d // 2,)
-    sections = tuple(int(x) for x in sections)
+    sections = tuple(sections)
+    array = _SECTIONS.get(sections)
+    if array is None:
+        if len(_SECTIONS) > 64:
+            _SECTIONS.clear()
+        array = _SECTIONS[sections] = (ctypes.c_int32 * len(sections))(*[int(x) for x in sections])
     axes = len(sections)
-    _need(positions.shape == (axes, n) or (axes == 1 and positions.shape == (n,)), f"positions: [{axes}, {n}]")
-    _need(positions.dtype == torch.int64 and (n <= 1 or positions.stride(-1) == 1), "positions: int64, tokens contiguous")
-    _need(cos_sin_cache.dtype == torch.float32 and cos_sin_cache.is_contiguous()
-          and cos_sin_cache.shape[-1] == d and cos_sin_cache.numel() == cos_sin_cache.shape[0] * d,
-          "cos_sin_cache: contiguous fp32 [positions, (1,) head_dim]")
-    stride = positions.stride(0) if axes > 1 else n   # 0: one row of positions for every axis
-    return axes, (ctypes.c_int32 * axes)(*sections), stride, cos_sin_cache.shape[0]
+    shape, stride = positions.shape, positions.stride()
+    _need(shape == (axes, n) or (axes == 1 and shape == (n,)), f"positions: [{axes}, {n}]")
+    _need(positions.dtype == torch.int64 and (n <= 1 or stride[-1] == 1), "positions: int64, tokens contiguous")
+    rows = cos_sin_cache.shape[0]
+    _need(cos_sin_cache.dtype == torch.float32 and cos_sin_cache.is_contiguous() and cos_sin_cache.shape[-1] == d
+          and cos_sin_cache.numel() == rows * d, "cos_sin_cache: contiguous fp32 [positions, (1,) head_dim]")
+    return stride[0] if axes > 1 else n, axes, array, rows   # stride 0: one row of positions for every axis
 
 
-def _q_out(query: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+def _q_out(query: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Tensor, int]:
+    """The output in query's shape, a new one unless given, and its token stride."""
     if out is None:
-        return torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    _rows(out, "out")
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        return out, out.shape[1] * out.shape[2]
     _need(out.shape == query.shape, "out: query's shape")
-    return out
+    return out, _rows(out, "out")[3]
+
+
+def _kv_rows(key: torch.Tensor, value: torch.Tensor, n: int, d: int) -> tuple[int, int, int]:
+    """(KV heads, key's token stride, value's) of n tokens' key and value rows."""
+    nk, hk, dk, ks = _rows(key, "key")
+    _need(nk == n and dk == d, "query and key: the same tokens and head_dim")
+    _need(value.shape == key.shape, "value: key's shape")
+    return hk, ks, _rows(value, "value")[3]
 
 
 def _slots(slot_mapping: torch.Tensor, n: int) -> None:
@@ -623,16 +645,15 @@ def mrotary_embedding(positions: torch.Tensor, query: torch.Tensor, key: torch.T
     [axes, N] (time, height, width): pair j takes the position of the axis whose section of
     ``mrope_section`` (pairs per axis, summing to D / 2) holds it.  Returns new tensors;
     with equal positions on all axes they are ``rotary_embedding``'s, bit for bit."""
-    with _on_device_of(query, positions, key, cos_sin_cache):
-        axes, sec, stride, max_pos = _rotary_args(positions, query, key, cos_sin_cache, mrope_section)
-        n, h, d = query.shape
-        hk = key.shape[1]
-        q_out, k_out = _q_out(query, None), torch.empty(key.shape, dtype=key.dtype, device=key.device)
-        st = lib().vlc_mrope_store_kvcache(_ptr(positions), stride, axes, sec, _ptr(query), _token_stride(query),
-                                           _ptr(q_out), h * d, _ptr(key), _token_stride(key), None, 0,
-                                           _ptr(cos_sin_cache), max_pos, None, None, None, 0, _ptr(k_out), hk * d, n,
-                                           h, hk, d, _stream())
-    check("vlc_mrope_store_kvcache", st)
+    dev = _device(query, positions, key, cos_sin_cache)
+    n, h, d, qs = _rows(query, "query")
+    nk, hk, dk, ks = _rows(key, "key")
+    _need(nk == n and dk == d, "query and key: the same tokens and head_dim")
+    axis, axes, sec, max_pos = _rotary_args(positions, cos_sin_cache, mrope_section, n, d)
+    q_out, k_out = _q_out(query, None)[0], _q_out(key, None)[0]
+    _launch(dev, "vlc_mrope_store_kvcache", positions.data_ptr(), axis, axes, sec, query.data_ptr(), qs,
+            q_out.data_ptr(), h * d, key.data_ptr(), ks, None, 0, cos_sin_cache.data_ptr(), max_pos, None, None, None,
+            0, k_out.data_ptr(), hk * d, n, h, hk, d)
     return q_out, k_out
 
 
@@ -643,23 +664,20 @@ def mrope_store_kvcache(positions: torch.Tensor, query: torch.Tensor, key: torch
     """``mrotary_embedding`` fused with the paged KV scatter, in one launch: returns the
     rotated query (into ``out`` when given; it may be ``query``) and writes the rotated key
     and the value rows to ``k_cache`` / ``v_cache`` row ``slot_mapping[i]`` (-1 skipped)."""
-    with _on_device_of(query, positions, key, value, cos_sin_cache, k_cache, v_cache, slot_mapping, out):
-        axes, sec, stride, max_pos = _rotary_args(positions, query, key, cos_sin_cache, mrope_section)
-        n, h, d = query.shape
-        hk = key.shape[1]
-        _rows(value, "value")
-        _need(value.shape == key.shape, "value: key's shape")
-        _need(k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16 and k_cache.is_contiguous()
-              and v_cache.is_contiguous() and k_cache.shape == v_cache.shape and k_cache.shape[-2:] == (hk, d),
-              "k_cache / v_cache: contiguous bf16 [.., num_kv_heads, head_dim]")
-        _slots(slot_mapping, n)
-        out = _q_out(query, out)
-        st = lib().vlc_mrope_store_kvcache(_ptr(positions), stride, axes, sec, _ptr(query), _token_stride(query),
-                                           _ptr(out), _token_stride(out), _ptr(key), _token_stride(key), _ptr(value),
-                                           _token_stride(value), _ptr(cos_sin_cache), max_pos, _ptr(k_cache),
-                                           _ptr(v_cache), _ptr(slot_mapping), k_cache.numel() // (hk * d), None, 0, n,
-                                           h, hk, d, _stream())
-    check("vlc_mrope_store_kvcache", st)
+    dev = _device(query, positions, key, value, cos_sin_cache, k_cache, v_cache, slot_mapping, out)
+    n, h, d, qs = _rows(query, "query")
+    hk, ks, vs = _kv_rows(key, value, n, d)
+    axis, axes, sec, max_pos = _rotary_args(positions, cos_sin_cache, mrope_section, n, d)
+    shape = k_cache.shape
+    _need(k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16 and k_cache.is_contiguous()
+          and v_cache.is_contiguous() and shape == v_cache.shape and shape[-2:] == (hk, d),
+          "k_cache / v_cache: contiguous bf16 [.., num_kv_heads, head_dim]")
+    _slots(slot_mapping, n)
+    out, os = _q_out(query, out)
+    _launch(dev, "vlc_mrope_store_kvcache", positions.data_ptr(), axis, axes, sec, query.data_ptr(), qs,
+            out.data_ptr(), os, key.data_ptr(), ks, value.data_ptr(), vs, cos_sin_cache.data_ptr(), max_pos,
+            k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), k_cache.numel() // (hk * d), None, 0, n,
+            h, hk, d)
     return out
 
 
@@ -667,24 +685,30 @@ def mrope_store_kvcache(positions: torch.Tensor, query: torch.Tensor, key: torch
 FP4_ROW_BYTES = 72   # of one head's row: 64 of e2m1 codes, 8 of e4m3 scales (include/vlcache_b200.h)
 
 
-def _fp4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dims=(3,)) -> tuple[int, int, int]:
-    """(pages, KV heads, block size) of 4-bit caches uint8 [(layers,) pages, Hk, block * 72]."""
-    for t in (k_cache, v_cache):
-        _need(t.dtype == torch.uint8 and t.dim() in dims, "a 4-bit cache is uint8 [pages, num_kv_heads, block_size * 72]")
-        _need(t[0].is_contiguous() if t.dim() == 4 else t.is_contiguous(), "4-bit caches must be contiguous")
-    _need(k_cache.shape == v_cache.shape, "k_cache and v_cache: the same shape")
-    pages, hk, row = k_cache.shape[-3:]
-    _need(row % FP4_ROW_BYTES == 0 and row > 0, "a 4-bit page is block_size * 72 bytes a head")
-    return pages, hk, row // FP4_ROW_BYTES
+def _fp4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dims: int = 3) -> tuple[int, int, int]:
+    """(pages, KV heads, block size) of 4-bit caches uint8 [pages, Hk, block * 72], or with
+    ``dims`` 4 of layers of them."""
+    shape = k_cache.shape
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8 or len(shape) != dims:
+        raise ValueError("a 4-bit cache is uint8 [pages, num_kv_heads, block_size * 72]")
+    _need(v_cache.shape == shape, "k_cache and v_cache: the same shape")
+    if dims == 4 and shape[0] > 0:   # the layers may lie apart
+        _need(k_cache[0].is_contiguous() and v_cache[0].is_contiguous(), "4-bit caches must be contiguous")
+    else:
+        _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "4-bit caches must be contiguous")
+    block = shape[-1] // FP4_ROW_BYTES
+    _need(block > 0 and shape[-1] == block * FP4_ROW_BYTES, "a 4-bit page is block_size * 72 bytes a head")
+    return shape[-3], shape[-2], block
 
 
 def _tables(block_tables: torch.Tensor, num_seqs: int) -> tuple[int, int]:
     """(row stride, width) of int32 block tables [num_seqs, width]."""
-    _need(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.shape[0] == num_seqs,
-          f"block_tables: int32 [{num_seqs}, width]")
-    width = block_tables.shape[1]
-    _need(width <= 1 or block_tables.stride(1) == 1, "block_tables: rows must be contiguous")
-    return (block_tables.stride(0) if num_seqs > 1 else width), width
+    shape, stride = block_tables.shape, block_tables.stride()
+    if block_tables.dtype != torch.int32 or len(shape) != 2 or shape[0] != num_seqs:
+        raise ValueError(f"block_tables: int32 [{num_seqs}, width]")
+    width = shape[1]
+    _need(width <= 1 or stride[1] == 1, "block_tables: rows must be contiguous")
+    return (stride[0] if num_seqs > 1 else width), width
 
 
 def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -692,18 +716,15 @@ def store_kvcache_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     """``store_kvcache`` into a 4-bit cache (uint8 [pages, Hk, block * 72]): each group of 16
     dims becomes e2m1 codes and an e4m3 scale.  ``k_scale`` / ``v_scale``: the cache's
     powers of two (include/vlcache_b200.h says how values are held)."""
-    with _on_device_of(key, value, k_cache, v_cache, slot_mapping):
-        _rows(key, "key")
-        _rows(value, "value")
-        n, hk, d = key.shape
-        _need(value.shape == key.shape, "value: key's shape")
-        pages, heads, block = _fp4_caches(k_cache, v_cache)
-        _need(heads == hk, "the caches' num_kv_heads")
-        _slots(slot_mapping, n)
-        st = lib().vlc_store_kvcache_fp4(_ptr(key), _token_stride(key), _ptr(value), _token_stride(value),
-                                         _ptr(k_cache), _ptr(v_cache), _ptr(slot_mapping), pages, block,
-                                         float(k_scale), float(v_scale), n, hk, d, _stream())
-    check("vlc_store_kvcache_fp4", st)
+    dev = _device(key, value, k_cache, v_cache, slot_mapping)
+    n, hk, d, ks = _rows(key, "key")
+    _need(value.shape == key.shape, "value: key's shape")
+    vs = _rows(value, "value")[3]
+    pages, heads, block = _fp4_caches(k_cache, v_cache)
+    _need(heads == hk, "the caches' num_kv_heads")
+    _slots(slot_mapping, n)
+    _launch(dev, "vlc_store_kvcache_fp4", key.data_ptr(), ks, value.data_ptr(), vs, k_cache.data_ptr(),
+            v_cache.data_ptr(), slot_mapping.data_ptr(), pages, block, float(k_scale), float(v_scale), n, hk, d)
 
 
 def rope_store_kvcache_fp4(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -714,22 +735,18 @@ def rope_store_kvcache_fp4(positions: torch.Tensor, query: torch.Tensor, key: to
     cache, in one launch: returns the rotated query; the rotated key, rounded to bf16, and
     the value are quantised into row ``slot_mapping[i]`` (-1 skipped), the same bytes as
     rotating first and ``store_kvcache_fp4`` after."""
-    with _on_device_of(query, positions, key, value, cos_sin_cache, k_cache, v_cache, slot_mapping, out):
-        axes, sec, stride, max_pos = _rotary_args(positions, query, key, cos_sin_cache, mrope_section)
-        n, h, d = query.shape
-        hk = key.shape[1]
-        _rows(value, "value")
-        _need(value.shape == key.shape, "value: key's shape")
-        pages, heads, block = _fp4_caches(k_cache, v_cache)
-        _need(heads == hk, "the caches' num_kv_heads")
-        _slots(slot_mapping, n)
-        out = _q_out(query, out)
-        st = lib().vlc_rope_store_kvcache_fp4(_ptr(positions), stride, axes, sec, _ptr(query), _token_stride(query),
-                                              _ptr(out), _token_stride(out), _ptr(key), _token_stride(key),
-                                              _ptr(value), _token_stride(value), _ptr(cos_sin_cache), max_pos,
-                                              _ptr(k_cache), _ptr(v_cache), _ptr(slot_mapping), pages, block,
-                                              float(k_scale), float(v_scale), n, h, hk, d, _stream())
-    check("vlc_rope_store_kvcache_fp4", st)
+    dev = _device(query, positions, key, value, cos_sin_cache, k_cache, v_cache, slot_mapping, out)
+    n, h, d, qs = _rows(query, "query")
+    hk, ks, vs = _kv_rows(key, value, n, d)
+    axis, axes, sec, max_pos = _rotary_args(positions, cos_sin_cache, mrope_section, n, d)
+    pages, heads, block = _fp4_caches(k_cache, v_cache)
+    _need(heads == hk, "the caches' num_kv_heads")
+    _slots(slot_mapping, n)
+    out, os = _q_out(query, out)
+    _launch(dev, "vlc_rope_store_kvcache_fp4", positions.data_ptr(), axis, axes, sec, query.data_ptr(), qs,
+            out.data_ptr(), os, key.data_ptr(), ks, value.data_ptr(), vs, cos_sin_cache.data_ptr(), max_pos,
+            k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), pages, block, float(k_scale),
+            float(v_scale), n, h, hk, d)
     return out
 
 
@@ -741,43 +758,41 @@ def gather_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table
     of the outputs [total_k, Hk, 128] is key j of sequence b.  With caches of several layers
     ([layers, pages, Hk, block * 72], e.g. ``kv_cache[0]``, ``kv_cache[1]``) the outputs are
     [layers, total_k, Hk, 128].  ``total_k`` is cu_seqlens_k's last entry, on the host."""
-    with _on_device_of(k_cache, v_cache, block_tables, cu_seqlens_k, k_out, v_out):
-        pages, hk, block = _fp4_caches(k_cache, v_cache, dims=(3, 4))
-        layers = k_cache.shape[0] if k_cache.dim() == 4 else 1
-        layer_stride = k_cache.stride(0) if k_cache.dim() == 4 and layers > 1 else 0
-        _need(k_cache.dim() == 3 or layers <= 1 or k_cache.stride(0) == v_cache.stride(0),
-              "k_cache and v_cache: the same layer stride")
-        _need(cu_seqlens_k.dtype == torch.int32 and cu_seqlens_k.dim() == 1 and cu_seqlens_k.is_contiguous()
-              and cu_seqlens_k.numel() >= 1, "cu_seqlens_k: contiguous int32 [num_seqs + 1]")
-        seqs = cu_seqlens_k.numel() - 1
-        stride, width = _tables(block_tables, seqs)
-        shape = (total_k, hk, HEAD_DIM) if k_cache.dim() == 3 else (layers, total_k, hk, HEAD_DIM)
-        if k_out is None:
-            k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
-        if v_out is None:
-            v_out = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
-        for t in (k_out, v_out):
-            _need(t.shape == shape and t.dtype == torch.bfloat16 and t.is_contiguous(),
-                  f"k_out / v_out: contiguous bf16 {list(shape)}")
-        row = hk * HEAD_DIM
-        st = lib().vlc_gather_kvcache_fp4(_ptr(k_cache), _ptr(v_cache), layer_stride, layers, pages, block, hk,
-                                          HEAD_DIM, _ptr(block_tables), stride, width, _ptr(cu_seqlens_k), seqs,
-                                          total_k, float(k_scale), float(v_scale), _ptr(k_out), _ptr(v_out), row,
-                                          total_k * row, _stream())
-    check("vlc_gather_kvcache_fp4", st)
+    dev = _device(k_cache, v_cache, block_tables, cu_seqlens_k, k_out, v_out)
+    many = k_cache.dim() == 4
+    pages, hk, block = _fp4_caches(k_cache, v_cache, 4 if many else 3)
+    layers = k_cache.shape[0] if many else 1
+    layer_stride = k_cache.stride(0) if layers > 1 else 0
+    _need(layers <= 1 or v_cache.stride(0) == layer_stride, "k_cache and v_cache: the same layer stride")
+    _need(cu_seqlens_k.dtype == torch.int32 and cu_seqlens_k.dim() == 1 and cu_seqlens_k.is_contiguous()
+          and cu_seqlens_k.numel() >= 1, "cu_seqlens_k: contiguous int32 [num_seqs + 1]")
+    seqs = cu_seqlens_k.numel() - 1
+    stride, width = _tables(block_tables, seqs)
+    shape = (layers, total_k, hk, HEAD_DIM) if many else (total_k, hk, HEAD_DIM)
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
+    if v_out is None:
+        v_out = torch.empty_like(k_out, memory_format=torch.contiguous_format)
+    for t in (k_out, v_out):
+        if t.shape != shape or t.dtype != torch.bfloat16 or not t.is_contiguous():
+            raise ValueError(f"k_out / v_out: contiguous bf16 {list(shape)}")
+    row = hk * HEAD_DIM
+    _launch(dev, "vlc_gather_kvcache_fp4", k_cache.data_ptr(), v_cache.data_ptr(), layer_stride, layers, pages, block,
+            hk, HEAD_DIM, block_tables.data_ptr(), stride, width, cu_seqlens_k.data_ptr(), seqs, total_k,
+            float(k_scale), float(v_scale), k_out.data_ptr(), v_out.data_ptr(), row, total_k * row)
     return k_out, v_out
 
 
-def _shift_fp4(k, v, layers, layer_stride, src_slots, dst_slots, delta_thw, mrope_section, rope_theta) -> int:
-    pages, hk, block = _fp4_caches(k, k if v is None else v, dims=(3, 4))
+def _shift_fp4(dev, k, v, layers, layer_stride, src_slots, dst_slots, delta_thw, mrope_section, rope_theta) -> None:
+    pages, hk, block = _fp4_caches(k, k if v is None else v, k.dim())
     n = src_slots.numel()
     for t in (src_slots, dst_slots):
         _need(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n),
               "src_slots / dst_slots: contiguous int32 of one length")
     d = (ctypes.c_int32 * 3)(*[int(x) for x in delta_thw])
     sec = (ctypes.c_int32 * 3)(*[int(x) for x in mrope_section])
-    return lib().vlc_mrope_shift_fp4(_ptr(k), _ptr(v), layer_stride, layers, pages, block, hk, HEAD_DIM,
-                                     _ptr(src_slots), _ptr(dst_slots), n, d, sec, float(rope_theta), _stream())
+    _launch(dev, "vlc_mrope_shift_fp4", k.data_ptr(), _ptr(v), layer_stride, layers, pages, block, hk, HEAD_DIM,
+            src_slots.data_ptr(), _ptr(dst_slots), n, d, sec, float(rope_theta))
 
 
 def mrope_shift_fp4(kv_cache: torch.Tensor, src_slots: torch.Tensor, dst_slots: torch.Tensor | None, delta_thw,
@@ -787,12 +802,11 @@ def mrope_shift_fp4(kv_cache: torch.Tensor, src_slots: torch.Tensor, dst_slots: 
     place), V rows copied.  A turned row is rounded to bf16 and quantised again; groups of
     16 pairs whose delta is 0 keep their bits, so a zero delta copies.  No destination may
     be another row's source (``engine.kv_cache.check_reuse_slots``)."""
-    with _on_device_of(kv_cache, src_slots, dst_slots):
-        _need(kv_cache.dim() == 5 and kv_cache.shape[0] == 2 and kv_cache.is_contiguous(),
-              "kv_cache: contiguous uint8 [2, layers, pages, Hk, block * 72]")
-        st = _shift_fp4(kv_cache[0], kv_cache[1], kv_cache.shape[1], kv_cache.stride(1), src_slots, dst_slots,
-                        delta_thw, mrope_section, rope_theta)
-    check("vlc_mrope_shift_fp4", st)
+    dev = _device(kv_cache, src_slots, dst_slots)
+    _need(kv_cache.dim() == 5 and kv_cache.shape[0] == 2 and kv_cache.is_contiguous(),
+          "kv_cache: contiguous uint8 [2, layers, pages, Hk, block * 72]")
+    _shift_fp4(dev, kv_cache[0], kv_cache[1], kv_cache.shape[1], kv_cache.stride(1), src_slots, dst_slots, delta_thw,
+               mrope_section, rope_theta)
 
 
 def mrope_shift_layer_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor | None, src_slots: torch.Tensor,
@@ -800,10 +814,9 @@ def mrope_shift_layer_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor | None, s
                           rope_theta: float = 1e6) -> None:
     """``mrope_shift_fp4`` of one layer's caches uint8 [pages, Hk, block * 72] (``v_cache`` None:
     K alone)."""
-    with _on_device_of(k_cache, v_cache, src_slots, dst_slots):
-        _need(k_cache.dim() == 3, "a 4-bit cache is uint8 [pages, num_kv_heads, block_size * 72]")
-        st = _shift_fp4(k_cache, v_cache, 1, 0, src_slots, dst_slots, delta_thw, mrope_section, rope_theta)
-    check("vlc_mrope_shift_fp4", st)
+    dev = _device(k_cache, v_cache, src_slots, dst_slots)
+    _need(k_cache.dim() == 3, "a 4-bit cache is uint8 [pages, num_kv_heads, block_size * 72]")
+    _shift_fp4(dev, k_cache, v_cache, 1, 0, src_slots, dst_slots, delta_thw, mrope_section, rope_theta)
 
 
 def decode_fp4_workspace_bytes(num_seqs: int, num_heads: int, num_kv_heads: int, max_context_len: int) -> int:
@@ -816,27 +829,25 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``decode_attention`` over a 4-bit cache: one query token per sequence, q / out [B, H, 128]
     (q may be [B, 1, H, 128]); sequences of length 0 give zeros.  ``max_context_len`` bounds
-    the lengths on the host and sizes the grid; ``workspace`` as ``decode_fp4_workspace_bytes``."""
-    with _on_device_of(q, k_cache, v_cache, block_tables, context_lens, out, workspace):
-        if q.dim() == 4:
-            _need(q.shape[1] == 1, "q: one token per sequence")
-            q = q.squeeze(1)
-        _rows(q, "q")
-        b, h, d = q.shape
-        pages, hk, block = _fp4_caches(k_cache, v_cache)
-        stride, width = _tables(block_tables, b)
-        _need(context_lens.dtype == torch.int32 and context_lens.numel() == b and context_lens.is_contiguous(),
-              "context_lens: contiguous int32, one per sequence")
-        out = _q_out(q, out)
-        need = decode_fp4_workspace_bytes(b, h, hk, max_context_len)
-        if need > 0 and (workspace is None or workspace.numel() * workspace.element_size() < need):
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        st = lib().vlc_decode_attn_fp4(_ptr(q), _token_stride(q), b, h, _ptr(k_cache), _ptr(v_cache), pages, block, hk,
-                                       d, _ptr(block_tables), stride, width, _ptr(context_lens), int(max_context_len),
-                                       float(softmax_scale), float(k_scale), float(v_scale), _ptr(out),
-                                       _token_stride(out), _ptr(workspace), ws_bytes, _stream())
-    check("vlc_decode_attn_fp4", st)
+    the lengths on the host and sizes the grid; ``workspace``: ``decode_fp4_workspace_bytes``,
+    32-byte aligned, one per call in flight."""
+    dev = _device(q, k_cache, v_cache, block_tables, context_lens, out, workspace)
+    if q.dim() == 4:
+        _need(q.shape[1] == 1, "q: one token per sequence")
+        q = q.squeeze(1)
+    b, h, d, qs = _rows(q, "q")
+    pages, hk, block = _fp4_caches(k_cache, v_cache)
+    stride, width = _tables(block_tables, b)
+    _need(context_lens.dtype == torch.int32 and context_lens.numel() == b and context_lens.is_contiguous(),
+          "context_lens: contiguous int32, one per sequence")
+    out, os = _q_out(q, out)
+    need = lib().vlc_decode_fp4_workspace_size(b, h, hk, max_context_len)
+    if need > 0 and (workspace is None or workspace.nbytes < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _launch(dev, "vlc_decode_attn_fp4", q.data_ptr(), qs, b, h, k_cache.data_ptr(), v_cache.data_ptr(), pages, block,
+            hk, d, block_tables.data_ptr(), stride, width, context_lens.data_ptr(), int(max_context_len),
+            float(softmax_scale), float(k_scale), float(v_scale), out.data_ptr(), os, _ptr(workspace),
+            0 if workspace is None else workspace.nbytes)
     return out
 
 
@@ -858,18 +869,22 @@ def prefill_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     them.  A prompt's query tiles share each key, so one conversion per key costs less than
     one per tile, and the dense rows mostly stay in L2.  ``cu_seqlens_k``: the plan's, on the
     device; ``workspace``: uint8, ``prefill_fp4_workspace_bytes``."""
-    with _on_device_of(q, k_cache, v_cache, block_tables, cu_seqlens_k, out, workspace):
-        _rows(q, "q")
-        pages, hk, block = _fp4_caches(k_cache, v_cache)
-        _need(cu_seqlens_k.numel() == plan.num_seqs + 1, "cu_seqlens_k: the plan's sequences")
-        need = prefill_fp4_workspace_bytes(plan, hk)
-        if workspace is None or workspace.numel() * workspace.element_size() < need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        workspace = workspace.view(-1).view(torch.uint8)
-        at = _round_up(plan.workspace_bytes, 256)
-        kv = workspace[at:need].view(torch.bfloat16).view(2, plan.total_k, hk, HEAD_DIM)
-        gather_kvcache_fp4(k_cache, v_cache, block_tables, cu_seqlens_k, plan.total_k, k_scale, v_scale, kv[0], kv[1])
-        return prefill_attention(q, kv[0], kv[1], None, plan, softmax_scale, out=out, workspace=workspace[:at])
+    dev = _device(q, k_cache, v_cache, block_tables, cu_seqlens_k, out, workspace)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return prefill_attention_fp4(q, k_cache, v_cache, block_tables, cu_seqlens_k, plan, softmax_scale, k_scale,
+                                         v_scale, out, workspace)
+    _rows(q, "q")
+    _, hk, _ = _fp4_caches(k_cache, v_cache)
+    _need(cu_seqlens_k.numel() == plan.num_seqs + 1, "cu_seqlens_k: the plan's sequences")
+    need = prefill_fp4_workspace_bytes(plan, hk)
+    if workspace is None or workspace.nbytes < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    workspace = workspace.view(-1).view(torch.uint8)
+    at = _round_up(plan.workspace_bytes, 256)
+    k, v = workspace[at:need].view(torch.bfloat16).view(2, plan.total_k, hk, HEAD_DIM).unbind()
+    gather_kvcache_fp4(k_cache, v_cache, block_tables, cu_seqlens_k, plan.total_k, k_scale, v_scale, k, v)
+    return prefill_attention(q, k, v, None, plan, softmax_scale, out=out, workspace=workspace[:at])
 
 
 # --------------------------------------------------------------------------- pages
@@ -879,27 +894,23 @@ def copy_kv_pages(kv_cache: torch.Tensor, src_pages: torch.Tensor, dst_pages: to
     either format.  Pages of the lists (device int32) are copied in no order: destinations
     differ and none is another pair's source (``engine.page_pool`` makes such lists); pairs
     of -1 are skipped."""
-    with _on_device_of(kv_cache, src_pages, dst_pages):
-        _need(kv_cache.dim() >= 4 and kv_cache.is_contiguous(), "kv_cache: contiguous [2, layers, pages, ...]")
-        n = src_pages.numel()
-        for t in (src_pages, dst_pages):
-            _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n,
-                  "src_pages / dst_pages: contiguous int32 of one length")
-        planes, pages = kv_cache.shape[0] * kv_cache.shape[1], kv_cache.shape[2]
-        item = kv_cache.element_size()
-        st = lib().vlc_copy_pages(_ptr(kv_cache), kv_cache.stride(1) * item, planes, kv_cache.stride(2) * item, pages,
-                                  _ptr(src_pages), _ptr(dst_pages), n, _stream())
-    check("vlc_copy_pages", st)
+    dev = _device(kv_cache, src_pages, dst_pages)
+    _need(kv_cache.dim() >= 4 and kv_cache.is_contiguous(), "kv_cache: contiguous [2, layers, pages, ...]")
+    n = src_pages.numel()
+    for t in (src_pages, dst_pages):
+        _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n,
+              "src_pages / dst_pages: contiguous int32 of one length")
+    shape, stride, item = kv_cache.shape, kv_cache.stride(), kv_cache.element_size()
+    _launch(dev, "vlc_copy_pages", kv_cache.data_ptr(), stride[1] * item, shape[0] * shape[1], stride[2] * item,
+            shape[2], src_pages.data_ptr(), dst_pages.data_ptr(), n)
 
 
 def remap_block_tables(block_tables: torch.Tensor, page_map: torch.Tensor) -> None:
     """Every entry p of the device block tables becomes ``page_map[p]`` (int32 [pages]); -1 stays."""
-    with _on_device_of(block_tables, page_map):
-        _need(block_tables.dtype == torch.int32 and block_tables.dim() == 2, "block_tables: int32 [rows, width]")
-        rows, width = block_tables.shape
-        _need(width <= 1 or block_tables.stride(1) == 1, "block_tables: rows must be contiguous")
-        _need(page_map.dtype == torch.int32 and page_map.dim() == 1 and page_map.is_contiguous(),
-              "page_map: contiguous int32 [pages]")
-        st = lib().vlc_remap_block_tables(_ptr(block_tables), block_tables.stride(0) if rows > 1 else width, rows,
-                                          width, _ptr(page_map), page_map.numel(), _stream())
-    check("vlc_remap_block_tables", st)
+    dev = _device(block_tables, page_map)
+    rows = block_tables.shape[0]
+    stride, width = _tables(block_tables, rows)
+    _need(page_map.dtype == torch.int32 and page_map.dim() == 1 and page_map.is_contiguous(),
+          "page_map: contiguous int32 [pages]")
+    _launch(dev, "vlc_remap_block_tables", block_tables.data_ptr(), stride, rows, width, page_map.data_ptr(),
+            page_map.numel())
