@@ -372,6 +372,20 @@ def test_decode_fp4_extreme_magnitudes(ops, size, qsize):
     _check_attention(out, q, kc, vc, bt, [1, 1], lens, scale, 1.0, 1.0, 2.0 ** -11)
 
 
+def test_decode_fp4_order_and_sharing_of_the_caches(ops):
+    """K before V, V before K, and one cache for both give what each place holds."""
+    lens, H, Hk = [400, 129], 16, 2
+    kc, vc, bt = _paged(37, lens, Hk, 64, poison=False)
+    q = torch.randn(2, H, D, generator=_gen(9)).to(torch.bfloat16)
+    ctx = torch.tensor(lens, dtype=torch.int32).cuda()
+    call = lambda k, v: ops.decode_attention_fp4(q.cuda(), k, v, bt.cuda(), ctx, 400, SCALE)  # noqa: E731
+    a, b = torch.stack([kc, vc]).cuda(), torch.stack([vc, kc]).cuda()
+    first, second = call(a[0], a[1]), call(b[1], b[0])
+    assert torch.equal(first, second)
+    _check_attention(first, q, kc, vc, bt, [1, 1], lens, SCALE, 1.0, 1.0, 2.0 ** -11)
+    _check_attention(call(a[0], a[0]), q, kc, kc, bt, [1, 1], lens, SCALE, 1.0, 1.0, 2.0 ** -11)
+
+
 def test_decode_fp4_flat_and_peaked(ops):
     """One key far above a flat rest: the rest's weights, 2^-26 of the peak each and below f16's
     smallest number, still add up (65536 of them are 2^-10 of the whole)."""

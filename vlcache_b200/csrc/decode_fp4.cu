@@ -18,7 +18,7 @@
 // the grid's warps share out evenly, each a contiguous run of it.  The shares are equal whatever
 // the lengths are (a grid of fixed splits left SMs idle at its end, paid a prologue and a join
 // every few chunks and merged in shared memory: 267 us for 256 sequences of 2700 .. 10700 keys, 28
-// query and 4 KV heads, against 183 us now).  A warp works alone: its own ring of chunks (TMA
+// query and 4 KV heads, against 178 us now).  A warp works alone: its own ring of chunks (TMA
 // tiles with the 64-byte swizzle for the codes, plain bulk copies for the scales, issued by its
 // lane 0), its own running maximum and sums, no barrier with any other warp.  A pair that a warp
 // has to itself is written out; the parts of a pair that several warps share go to the workspace
@@ -55,9 +55,13 @@ constexpr float SLACK = 3.f;                    // log2 that the maximum may gro
 constexpr int blocks_per_sm(int NT) { return NT == 1 ? 6 : 4; }
 
 struct Params {
-  CUtensorMap tm_k, tm_v;  // bytes {64, block_size, pages * Hk}, box {64, CH, 1}
-  const uint8_t* k_cache;
-  const uint8_t* v_cache;
+  // K's and V's codes {64, block_size, pages * Hk} and scales {64, block_size / 8, pages * Hk}, in
+  // bytes (boxes {64, CH} and {64, CH / 8}).  Joined, codes[0] and scales[0] have a fourth dimension,
+  // the two caches, whose stride is their distance: a chunk is then two copies instead of four (183
+  // -> 179 us for 256 sequences).  v_first: V lies before K.
+  CUtensorMap codes[2], scales[2];
+  bool joined;
+  bool v_first;
   const __nv_bfloat16* q;
   int64_t q_seq_stride;
   const int32_t* block_tables;
@@ -74,7 +78,10 @@ struct Params {
   __nv_bfloat16* out;
   int64_t out_seq_stride;
   int num_warps;
-  float* parts;  // [num_warps][2][group][HD] sums, then [num_warps][2][group][2] (maximum, sum of P)
+  // Workspace: a warp's first pair and its last leave parts when they are not whole.
+  float* parts;    // [num_warps][2][group][HD] sums of P V
+  float2* part_ml;  // [num_warps][2][group] (maximum, sum of P)
+  int2* places;    // [num_seqs][num_kv_heads] of each pair with keys: (slot of its first part, parts)
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -197,9 +204,12 @@ struct State {
 
   // One chunk at `st`.  CUT: only its first `valid` keys count.
   template <bool CUT>
-  __device__ __forceinline__ void step(uint32_t st, int valid, int r, int t) {
+  __device__ __forceinline__ void step(uint32_t st, uint32_t k_at, int valid, int r, int t) {
     const int kr = tile_key(r);
-    const uint32_t k_codes = st + swizzled(kr, t), k_scales = st + 2 * CODE_TILE + kr * 8 + 2 * t;
+    // k_at: 0 or 1, K's place among the two
+    const uint32_t k_codes = st + k_at * CODE_TILE + swizzled(kr, t);
+    const uint32_t k_scales = st + 2 * CODE_TILE + k_at * SCALE_TILE + kr * 8 + 2 * t;
+    const uint32_t v_at = k_at ^ 1;
     // ---- S^T = K Q^T
     float s[TILES][NT][4];
 #pragma unroll
@@ -294,8 +304,8 @@ struct State {
     uint32_t v_codes[2], v_scales[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      v_codes[x] = st + CODE_TILE + swizzled(kv[x], r >> 1) + 8 * (r & 1);
-      v_scales[x] = st + 2 * CODE_TILE + SCALE_TILE + kv[x] * 8 + r;
+      v_codes[x] = st + v_at * CODE_TILE + swizzled(kv[x], r >> 1) + 8 * (r & 1);
+      v_scales[x] = st + 2 * CODE_TILE + v_at * SCALE_TILE + kv[x] * 8 + r;
     }
     const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
@@ -406,19 +416,19 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
     ahead.page = ahead.index < p.table_width ? __ldg(p.block_tables + ahead.seq * p.table_stride + ahead.index) : -1;
   };
   if (lane == 0) load_page();
-  const int head_bytes = p.block_size * fp4::ROW_BYTES;
   auto issue = [&](int stage, bool more) {
     uint64_t* bar = full + stage;
     uint8_t* st = ring + stage * STAGE_BYTES;
     if ((uint32_t)ahead.page < (uint32_t)p.num_pages) {
       const int piece = ahead.page * Hk + ahead.head;
-      const int64_t scales = (int64_t)piece * head_bytes + fp4::scale_offset(ahead.row, p.block_size);
       valid_of[stage] = min(CH, ahead.keys);
       mbar_expect_tx(bar, STAGE_BYTES);
-      tma_load_3d(st, &p.tm_k, bar, 0, ahead.row, piece);
-      bulk_load_1d(st + 2 * CODE_TILE, p.k_cache + scales, SCALE_TILE, bar);
-      tma_load_3d(st + CODE_TILE, &p.tm_v, bar, 0, ahead.row, piece);
-      bulk_load_1d(st + 2 * CODE_TILE + SCALE_TILE, p.v_cache + scales, SCALE_TILE, bar);
+      tma_load_4d(st, &p.codes[0], bar, 0, ahead.row, piece, 0);
+      tma_load_4d(st + 2 * CODE_TILE, &p.scales[0], bar, 0, ahead.row >> 3, piece, 0);
+      if (!p.joined) {
+        tma_load_4d(st + CODE_TILE, &p.codes[1], bar, 0, ahead.row, piece, 0);
+        tma_load_4d(st + 2 * CODE_TILE + SCALE_TILE, &p.scales[1], bar, 0, ahead.row >> 3, piece, 0);
+      }
     } else {  // the table has no usable page there: recorded, and none of the chunk's keys counts
       valid_of[stage] = 0;
       record_error(VLC_DEV_ERR_BLOCK_RANGE);
@@ -458,6 +468,14 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
   State<NT> state;
   auto q_of = [&]() { return p.q + (int64_t)seq * p.q_seq_stride + (int64_t)head * G * HD; };
   state.start(q_of(), G, r, t, p.scale_log2, p.q_sign);
+  // The warp with a pair's first chunk notes where its parts will be: one for each warp up to that of
+  // its last chunk, in slot 0 but for this warp's.
+  auto note = [&](int64_t chunk, int slot) {
+    if (lane == 0)
+      p.places[(int64_t)seq * Hk + head] =
+          make_int2((int)my * 2 + slot, (int)(shares.warp_of(chunk + n - 1) - my) + 1);
+  };
+  if (j == 0) note(c0, 0);
   int begin = j;       // first chunk of the pair that is in the state
   int first_slot = 0;  // the part's slot: 0 for the one that holds the warp's first chunk
 
@@ -468,8 +486,8 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
     }
     const uint32_t st = ring_u + (i % STAGES) * STAGE_BYTES;
     const int valid = valid_of[i % STAGES];
-    if (valid == CH) state.template step<false>(st, valid, r, t);
-    else state.template step<true>(st, valid, r, t);
+    if (valid == CH) state.template step<false>(st, p.v_first, valid, r, t);
+    else state.template step<true>(st, p.v_first, valid, r, t);
     __syncwarp();  // every lane has read the stage
     if (lane == 0 && i + STAGES < count) issue(i % STAGES, i + STAGES + 1 < count);
     if (++j < n && i + 1 < count) continue;
@@ -477,8 +495,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
     // ---- the pair ends, or the run does
     const bool whole = begin == 0 && j == n;
     float* const part_o = p.parts + (my * 2 + first_slot) * G * HD;
-    float2* const part_ml = reinterpret_cast<float2*>(p.parts + (int64_t)p.num_warps * 2 * G * HD) +
-                            (my * 2 + first_slot) * G;
+    float2* const part_ml = p.part_ml + (my * 2 + first_slot) * G;
 #pragma unroll
     for (int x = 0; x < NT * 2; ++x) {
       const int nt = x >> 1, odd = x & 1;
@@ -519,122 +536,118 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
       } while (len <= 0);
       n = (len + CH - 1) / CH;
     }
+    note(c0 + i + 1, 1);
     state.start(q_of(), G, r, t, p.scale_log2, p.q_sign);
   }
 }
 
+// A running (maximum, sum of P, four dims of O) and its union with another part's.
+struct Joined {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float m2, float l2, const float4& o2) {
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
+    const float f = fast_exp2(m - ref), g = fast_exp2(m2 - ref);
+    m = top;
+    l = l * f + l2 * g;
+    o = make_float4(o.x * f + o2.x * g, o.y * f + o2.y * g, o.z * f + o2.z * g, o.w * f + o2.w * g);
+  }
+  __device__ __forceinline__ uint2 result(float v_scale) const {
+    const float inv = l != 0.f ? v_scale / l : 0.f;
+    return make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  }
+};
+
 // Joins the parts of the pairs that several warps shared and writes zeros for empty sequences.
 // SPREAD (few pairs of many parts): a block takes a quarter of one head's dims; its 32 groups of
-// eight lanes take the parts in turn.  Otherwise a block takes eight heads, a warp each.
+// eight lanes take the parts in turn.  Otherwise a block takes 16 heads of a sequence, a warp every
+// eighth of them.  The decode kernel fills the SMs to its end, so what a block does before the wait
+// is not hidden: where a pair's parts are was noted by the warp that began it.
 template <bool SPREAD>
-__global__ void __launch_bounds__(256, SPREAD ? 3 : 6) decode_fp4_combine_kernel(const float* parts, const int32_t* context_lens,
-                                                                 int num_seqs, int max_len, int num_warps,
+__global__ void __launch_bounds__(256, 3) decode_fp4_combine_kernel(const float* parts, const float2* part_ml,
+                                                                 const int2* places, const int32_t* context_lens,
                                                                  int num_heads, int num_kv_heads, float v_scale,
                                                                  __nv_bfloat16* out, int64_t out_seq_stride) {
-  __shared__ int64_t s_sum[2][8];
-  __shared__ float s_max[8];
   __shared__ float4 s_o[8][8];
-  __shared__ float s_l[8];
+  __shared__ float2 s_ml[8];
   const int seq = blockIdx.x, warp = warp_id(), lane = lane_id();
-  int64_t total = 0, before = 0;
-  for (int i = threadIdx.x; i < num_seqs; i += 256) {
-    const int c = chunks_of(__ldg(context_lens + i), max_len);
-    total += c;
-    if (i < seq) before += c;
-  }
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, d);
-    before += __shfl_xor_sync(0xffffffffu, before, d);
-  }
-  if (lane == 0) {
-    s_sum[0][warp] = total;
-    s_sum[1][warp] = before;
-  }
-  __syncthreads();
-  total = before = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    total += s_sum[0][w];
-    before += s_sum[1][w];
-  }
-  const int n = chunks_of(__ldg(context_lens + seq), max_len);
-  const int h = SPREAD ? blockIdx.y : blockIdx.y * 8 + warp;
   const int G = num_heads / num_kv_heads;
   // dims: 32 z + 4 (lane % 8) of a quarter, or 4 lane
   const int dim4 = SPREAD ? blockIdx.z * 8 + (lane & 7) : lane;
+  const float4* po = reinterpret_cast<const float4*>(parts) + dim4;
+  uint2* const dst = reinterpret_cast<uint2*>(out + (int64_t)seq * out_seq_stride) + dim4;
+  const bool empty = __ldg(context_lens + seq) <= 0;
   // Every block waits, those with nothing to join too: what follows in the stream may rely on this
   // grid's end for the decode kernel's.
   pdl_wait();
-  if (h >= num_heads) return;
-  uint2* const dst = reinterpret_cast<uint2*>(out + (int64_t)seq * out_seq_stride + (int64_t)h * HD) + dim4;
-  if (n == 0) {
-    if (!SPREAD || threadIdx.x < 8) *dst = make_uint2(0, 0);
-    return;
-  }
-  const Shares shares(total * num_kv_heads, num_warps);
-  const int64_t f0 = before * num_kv_heads + (int64_t)(h / G) * n;           // the pair's first chunk
-  const int64_t w0 = shares.warp_of(f0);                                     // its first warp
-  const int count = (int)(shares.warp_of(f0 + n - 1) - w0) + 1;              // and their number
-  if (count == 1) return;
-  // parts are G apart, but the first warp's lies one slot on when its run begins before the pair
-  const int64_t first = (w0 * 2 + (f0 == shares.first(w0) ? 0 : 1)) * G + h % G, rest = w0 * 2 * G + h % G;
-  const float4* po = reinterpret_cast<const float4*>(parts) + dim4;
-  const float2* ml = reinterpret_cast<const float2*>(parts + (int64_t)num_warps * 2 * G * HD);
-  auto slot = [&](int i) { return i == 0 ? first : rest + (int64_t)i * 2 * G; };
-
-  float M = -INFINITY;
-  for (int i = SPREAD ? threadIdx.x : lane; i < count; i += SPREAD ? 256 : 32) M = fmaxf(M, ml[slot(i)].x);
+  constexpr int HEADS = SPREAD ? 1 : 2;  // of a warp
+  int64_t first[HEADS], rest[HEADS];     // rows of parts: part i > 0 is at rest + 2 G i
+  int count[HEADS];                      // parts of the head
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-  if (SPREAD) {
-    if (lane == 0) s_max[warp] = M;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, s_max[w]);
+  for (int x = 0; x < HEADS; ++x) {
+    const int h = SPREAD ? blockIdx.y : blockIdx.y * 16 + x * 8 + warp;
+    int2 place = make_int2(0, 0);
+    if (h < num_heads && !empty) place = places[(int64_t)seq * num_kv_heads + h / G];
+    first[x] = (int64_t)place.x * G + h % G;
+    rest[x] = (int64_t)(place.x & ~1) * G + h % G;
+    count[x] = place.y;
   }
-  const float ref = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll (SPREAD ? 8 : 2)
-  for (int i = SPREAD ? threadIdx.x >> 3 : 0; i < count; i += SPREAD ? 32 : 1) {
-    const int64_t s = slot(i);
-    const float2 x = ml[s];
-    const float4 v = po[s * (HD / 4)];
-    const float f = fast_exp2(x.x - ref);
-    L += f * x.y;
-    acc.x += f * v.x;
-    acc.y += f * v.y;
-    acc.z += f * v.z;
-    acc.w += f * v.w;
-  }
-  if (SPREAD) {
+  if constexpr (SPREAD) {
+    if (empty && threadIdx.x < 8) dst[blockIdx.y * (HD / 4)] = make_uint2(0, 0);
+    if (count[0] <= 1) return;  // empty, or written by its warp
+    Joined sum;
+#pragma unroll 4
+    for (int i = threadIdx.x >> 3; i < count[0]; i += 32) {
+      const int64_t s = i == 0 ? first[0] : rest[0] + (int64_t)i * 2 * G;
+      const float2 x = part_ml[s];
+      const float4 v = po[s * (HD / 4)];
+      sum.add(x.x, x.y, v);
+    }
 #pragma unroll
     for (int d = 8; d < 32; d <<= 1) {
-      L += __shfl_xor_sync(0xffffffffu, L, d);
-      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, d);
-      acc.y += __shfl_xor_sync(0xffffffffu, acc.y, d);
-      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, d);
-      acc.w += __shfl_xor_sync(0xffffffffu, acc.w, d);
+      const float m = __shfl_xor_sync(0xffffffffu, sum.m, d), l = __shfl_xor_sync(0xffffffffu, sum.l, d);
+      float4 v;
+      v.x = __shfl_xor_sync(0xffffffffu, sum.o.x, d);
+      v.y = __shfl_xor_sync(0xffffffffu, sum.o.y, d);
+      v.z = __shfl_xor_sync(0xffffffffu, sum.o.z, d);
+      v.w = __shfl_xor_sync(0xffffffffu, sum.o.w, d);
+      sum.add(m, l, v);
     }
-    if (lane < 8) s_o[warp][lane] = acc;
-    if (lane == 0) s_l[warp] = L;
+    if (lane < 8) s_o[warp][lane] = sum.o;
+    if (lane == 0) s_ml[warp] = make_float2(sum.m, sum.l);
     __syncthreads();
     if (threadIdx.x >= 8) return;
-    L = 0.f;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const float4 v = s_o[w][lane];
-      L += s_l[w];
-      acc.x += v.x;
-      acc.y += v.y;
-      acc.z += v.z;
-      acc.w += v.w;
+    for (int w = 1; w < 8; ++w) sum.add(s_ml[w].x, s_ml[w].y, s_o[w][lane]);
+    dst[blockIdx.y * (HD / 4)] = sum.result(v_scale);
+  }
+  if constexpr (!SPREAD) {
+    constexpr int PARTS = 3;  // loads of that many parts of both heads at once: mostly all there are
+    Joined sum[HEADS];
+    for (int i0 = 0; i0 < max(count[0], count[1]); i0 += PARTS) {
+      float2 x[HEADS][PARTS];
+      float4 v[HEADS][PARTS];
+#pragma unroll
+      for (int y = 0; y < HEADS; ++y)
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          if (count[y] <= 1 || i0 + i >= count[y]) continue;
+          const int64_t s = i0 + i == 0 ? first[y] : rest[y] + (int64_t)(i0 + i) * 2 * G;
+          x[y][i] = part_ml[s];
+          v[y][i] = po[s * (HD / 4)];
+        }
+#pragma unroll
+      for (int y = 0; y < HEADS; ++y)
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i)
+          if (count[y] > 1 && i0 + i < count[y]) sum[y].add(x[y][i].x, x[y][i].y, v[y][i]);
+    }
+#pragma unroll
+    for (int y = 0; y < HEADS; ++y) {
+      const int h = blockIdx.y * 16 + y * 8 + warp;
+      if (h < num_heads && count[y] != 1) dst[h * (HD / 4)] = sum[y].result(v_scale);  // (0 parts: zeros)
     }
   }
-  const float inv = L != 0.f ? v_scale / L : 0.f;
-  *dst = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
 // Warps of the grid: from host values only, so that it is fixed for graph capture.
@@ -644,8 +657,8 @@ static int grid_warps(int num_seqs, int num_heads, int num_kv_heads, int max_con
   return (int)std::max<int64_t>(1, std::min(resident, most));
 }
 
-static int64_t workspace_bytes_for(int64_t warps, int group) {
-  return warps * 2 * group * (HD + 2) * (int64_t)sizeof(float);
+static int64_t workspace_bytes_for(int64_t warps, int group, int64_t pairs) {
+  return warps * 2 * group * (HD + 2) * (int64_t)sizeof(float) + pairs * (int64_t)sizeof(int2);
 }
 
 static bool power_of_two(float g) {
@@ -663,7 +676,7 @@ extern "C" int64_t vlc_decode_fp4_workspace_size(int num_seqs, int num_heads, in
   if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_context_len < 0) return 0;
   return workspace_bytes_for(
       grid_warps(num_seqs, num_heads, num_kv_heads, std::max(max_context_len, 1), vlc_num_sms()),
-      num_heads / num_kv_heads);
+      num_heads / num_kv_heads, (int64_t)num_seqs * num_kv_heads);
 }
 
 extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_seqs, int num_heads,
@@ -689,18 +702,34 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   if (num_kv_heads > 65535 || num_seqs > 65535 || num_heads > 65535) return VLC_ERR_SHAPE;
   if (max_context_len == 0) max_context_len = 1;
   const int warps = grid_warps(num_seqs, num_heads, num_kv_heads, max_context_len, vlc_num_sms());
-  const int64_t need = workspace_bytes_for(warps, G);
+  const int64_t need = workspace_bytes_for(warps, G, (int64_t)num_seqs * num_kv_heads);
   if (!workspace || workspace_bytes < need) return VLC_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 32) return VLC_ERR_ALIGN;
 
   Params p;
-  const uint64_t dims[3] = {(uint64_t)fp4::CODE_BYTES, (uint64_t)block_size, (uint64_t)(num_pages * num_kv_heads)};
-  const uint64_t strides[2] = {(uint64_t)fp4::CODE_BYTES, (uint64_t)block_size * fp4::ROW_BYTES};
-  const uint32_t box[3] = {(uint32_t)fp4::CODE_BYTES, (uint32_t)CH, 1};
-  if (encode_tmap_u8(&p.tm_k, k_cache, 3, dims, strides, box, 64) != VLC_OK) return VLC_ERR_CUDA;
-  if (encode_tmap_u8(&p.tm_v, v_cache, 3, dims, strides, box, 64) != VLC_OK) return VLC_ERR_CUDA;
-  p.k_cache = (const uint8_t*)k_cache;
-  p.v_cache = (const uint8_t*)v_cache;
+  const uint8_t* caches[2] = {(const uint8_t*)k_cache, (const uint8_t*)v_cache};
+  const uint64_t pieces = (uint64_t)(num_pages * num_kv_heads), page_head = (uint64_t)block_size * fp4::ROW_BYTES;
+  p.v_first = caches[1] < caches[0];
+  if (p.v_first) std::swap(caches[0], caches[1]);
+  const uint64_t apart = (uint64_t)(caches[1] - caches[0]);
+  p.joined = apart > 0 && apart < 1ull << 40;  // as a tensor map's strides may be
+  if (!p.joined && p.v_first) {
+    std::swap(caches[0], caches[1]);
+    p.v_first = false;
+  }
+  for (int i = 0; i < (p.joined ? 1 : 2); ++i) {
+    const uint64_t both = p.joined ? 2 : 1, last = p.joined ? apart : pieces * page_head;
+    const uint64_t dims[4] = {(uint64_t)fp4::CODE_BYTES, (uint64_t)block_size, pieces, both};
+    const uint64_t strides[3] = {(uint64_t)fp4::CODE_BYTES, page_head, last};
+    const uint32_t box[4] = {(uint32_t)fp4::CODE_BYTES, (uint32_t)CH, 1, (uint32_t)both};
+    if (encode_tmap_u8(&p.codes[i], caches[i], 4, dims, strides, box, 64) != VLC_OK) return VLC_ERR_CUDA;
+    const uint64_t sdims[4] = {64, (uint64_t)block_size / 8, pieces, both};
+    const uint64_t sstrides[3] = {64, page_head, last};
+    const uint32_t sbox[4] = {64, (uint32_t)CH / 8, 1, (uint32_t)both};
+    if (encode_tmap_u8(&p.scales[i], caches[i] + (int64_t)block_size * fp4::CODE_BYTES, 4, sdims, sstrides, sbox, 0) !=
+        VLC_OK)
+      return VLC_ERR_CUDA;
+  }
   p.q = (const __nv_bfloat16*)q;
   p.q_seq_stride = q_seq_stride;
   p.block_tables = block_tables;
@@ -721,6 +750,8 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   p.out_seq_stride = out_seq_stride;
   p.num_warps = warps;
   p.parts = (float*)workspace;
+  p.part_ml = (float2*)(p.parts + (int64_t)warps * 2 * G * HD);
+  p.places = (int2*)(p.part_ml + (int64_t)warps * 2 * G);
 
   static std::atomic<uint64_t> smem1{0}, smem2{0};
   const int grid = (warps + WARPS - 1) / WARPS;
@@ -737,7 +768,7 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   // Few pairs: each has many parts, which several blocks read.
   const bool spread = warps > 8ll * num_seqs * num_kv_heads;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = spread ? dim3(num_seqs, num_heads, 4) : dim3(num_seqs, (num_heads + 7) / 8);
+  cfg.gridDim = spread ? dim3(num_seqs, num_heads, 4) : dim3(num_seqs, (num_heads + 15) / 16);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -746,8 +777,8 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, spread ? decode_fp4_combine_kernel<true> : decode_fp4_combine_kernel<false>,
-                         (const float*)p.parts, context_lens, num_seqs, max_context_len, warps, num_heads,
-                         num_kv_heads, v_scale, p.out, out_seq_stride) != cudaSuccess) {
+                         (const float*)p.parts, (const float2*)p.part_ml, (const int2*)p.places, context_lens,
+                         num_heads, num_kv_heads, v_scale, p.out, out_seq_stride) != cudaSuccess) {
     (void)cudaGetLastError();
     return VLC_ERR_CUDA;
   }

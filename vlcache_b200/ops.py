@@ -868,23 +868,32 @@ def prefill_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     to bf16 once (``gather_kvcache_fp4``, exact), then the tcgen05 attention kernel runs on
     them.  A prompt's query tiles share each key, so one conversion per key costs less than
     one per tile, and the dense rows mostly stay in L2.  ``cu_seqlens_k``: the plan's, on the
-    device; ``workspace``: uint8, ``prefill_fp4_workspace_bytes``."""
+    device; ``workspace``: ``prefill_fp4_workspace_bytes``, 256-byte aligned, one per call in
+    flight."""
     dev = _device(q, k_cache, v_cache, block_tables, cu_seqlens_k, out, workspace)
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return prefill_attention_fp4(q, k_cache, v_cache, block_tables, cu_seqlens_k, plan, softmax_scale, k_scale,
-                                         v_scale, out, workspace)
-    _rows(q, "q")
-    _, hk, _ = _fp4_caches(k_cache, v_cache)
-    _need(cu_seqlens_k.numel() == plan.num_seqs + 1, "cu_seqlens_k: the plan's sequences")
+    n, h, d, qs = _rows(q, "q")
+    pages, hk, block = _fp4_caches(k_cache, v_cache)
+    seqs, total_k = plan.num_seqs, plan.total_k
+    _need(cu_seqlens_k.dtype == torch.int32 and cu_seqlens_k.is_contiguous() and cu_seqlens_k.numel() == seqs + 1,
+          "cu_seqlens_k: contiguous int32, the plan's sequences")
+    stride, width = _tables(block_tables, seqs)
+    out, os = _q_out(q, out)
     need = prefill_fp4_workspace_bytes(plan, hk)
     if workspace is None or workspace.nbytes < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    workspace = workspace.view(-1).view(torch.uint8)
-    at = _round_up(plan.workspace_bytes, 256)
-    k, v = workspace[at:need].view(torch.bfloat16).view(2, plan.total_k, hk, HEAD_DIM).unbind()
-    gather_kvcache_fp4(k_cache, v_cache, block_tables, cu_seqlens_k, plan.total_k, k_scale, v_scale, k, v)
-    return prefill_attention(q, k, v, None, plan, softmax_scale, out=out, workspace=workspace[:at])
+    _need(workspace.is_contiguous(), "workspace: contiguous")
+    if plan.dev is None or plan.dev.device != q.device:
+        plan.dev = torch.from_numpy(plan.host).to(q.device)
+    row = hk * HEAD_DIM
+    k = workspace.data_ptr() + _round_up(plan.workspace_bytes, 256)
+    v = k + 2 * total_k * row
+    _launch(dev, "vlc_gather_kvcache_fp4", k_cache.data_ptr(), v_cache.data_ptr(), 0, 1, pages, block, hk, d,
+            block_tables.data_ptr(), stride, width, cu_seqlens_k.data_ptr(), seqs, total_k, float(k_scale),
+            float(v_scale), k, v, row, 0)
+    _launch(dev, "vlc_prefill_attn", q.data_ptr(), qs, n, h, k, v, row, row, total_k, hk, d, None, 0, 0,
+            plan.dev.data_ptr(), plan.host_ptr, float(softmax_scale), out.data_ptr(), os, workspace.data_ptr(),
+            plan.workspace_bytes)
+    return out
 
 
 # --------------------------------------------------------------------------- pages
