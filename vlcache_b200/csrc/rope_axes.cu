@@ -18,7 +18,7 @@
 //    the row pieces of its next two slices in flight into a place of its own in shared memory
 //    (16-byte asynchronous copies: no registers, no barrier, only its own copies to wait for), and
 //    loads the positions two slices and the table values one slice ahead.
-//    10617 tokens of 28 + 4 + 4 heads into bf16 pages: 35.3 us against 41 with the first kernel
+//    10617 tokens of 28 + 4 + 4 heads into bf16 pages: 34.6 us against 41 with the first kernel
 //    (196 MB, 31 us at the copy rate); whole tokens brought and taken by bulk copies into rings of
 //    eight warps measured 41 too, each token waiting for the stores of the one before.
 #include <cmath>
@@ -59,6 +59,7 @@ struct Params {
   const int32_t* slot_mapping;
   int64_t num_slots;
   int block_size;
+  int block_shift;  // log2 of a block size that is a power of two, else -1
   float k_inv_scale, v_inv_scale;
   int num_tokens, num_heads, num_kv_heads;
   int warps_per_token;
@@ -156,7 +157,7 @@ __device__ __forceinline__ void put_head(const Params& p, int64_t token, int hea
     uint8_t* row = nullptr;
     int at = 0;
     if (keep) {
-      const int page = slot / p.block_size;
+      const int page = p.block_shift >= 0 ? slot >> p.block_shift : slot / p.block_size;
       at = slot - page * p.block_size;
       row = (uint8_t*)(is_v ? p.v_cache : p.k_cache) + fp4::head_offset(page, p.num_kv_heads, kv_head, p.block_size);
     }
@@ -277,30 +278,37 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 1) rope_stream_kernel(const
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  int64_t pos[kMaxAxes];  // of the slice after the next, and its slot
+  // A lane's eight pairs belong to one axis (sections that split them go to the other kernel); that
+  // every axis' position is inside the table is seen by the lanes together.
+  int own = 0;
+#pragma unroll
+  for (int x = 1; x < kMaxAxes; ++x)
+    if (x < p.num_axes && 8 * c >= p.section_end[x - 1]) own = x;
+  const int64_t* const own_positions = p.positions + own * p.axis_stride;
+  const int64_t* const any_positions = p.positions + min(lane & 3, p.num_axes - 1) * p.axis_stride;
+  int64_t own_pos, any_pos;  // of the slice after the next, and its slot
   int slot_after = -1;
   auto load_positions = [&](const Unit& u) {
-    const int64_t token = u.token < p.num_tokens ? u.token : 0;
-#pragma unroll
-    for (int x = 0; x < kMaxAxes; ++x) pos[x] = x < p.num_axes ? __ldg(p.positions + x * p.axis_stride + token) : 0;
+    const int token = u.token < p.num_tokens ? u.token : 0;
+    own_pos = __ldg(own_positions + token);
+    any_pos = __ldg(any_positions + token);
     if (SINK != kRows) slot_after = __ldg(p.slot_mapping + token);
   };
   uint64_t cs_next[4], sn_next[4];  // of the next slice
   bool placed_next;
   int slot_next = -1;
   auto load_table = [&]() {
-    placed_next = true;
-#pragma unroll
-    for (int x = 0; x < kMaxAxes; ++x) placed_next = placed_next && pos[x] >= 0 && pos[x] < p.max_position;
+    placed_next = __all_sync(0xffffffffu, (uint64_t)any_pos < (uint64_t)p.max_position);
     slot_next = slot_after;
-    load_angles(
-        p, c, [&](int x) {
-          int64_t at = pos[0];
+    const float4* row = reinterpret_cast<const float4*>(p.cos_sin + (placed_next ? own_pos : 0) * HD) + 2 * c;
 #pragma unroll
-          for (int i = 1; i < kMaxAxes; ++i)
-            if (x == i) at = pos[i];
-          return p.cos_sin + (placed_next ? at : 0) * HD;
-        }, cs_next, sn_next);
+    for (int i = 0; i < 2; ++i) {
+      const float4 u = __ldg(row + i), v = __ldg(row + HALF / 4 + i);
+      cs_next[2 * i] = f2_pack(u.x, u.y);
+      cs_next[2 * i + 1] = f2_pack(u.z, u.w);
+      sn_next[2 * i] = f2_pack(v.x, v.y);
+      sn_next[2 * i + 1] = f2_pack(v.z, v.w);
+    }
   };
 
   const int start = warp_id() * gridDim.x + blockIdx.x;
@@ -373,7 +381,8 @@ static int launch(Params& p, cudaStream_t stream) {
     // costs more than it saves (36 heads: 3001 tokens 14.0 against 12.7 us, 4500 tokens 17.0 against
     // 18.5; 20 heads: 4500 tokens 13.0 against 11.4).
     const int sms = vlc_num_sms();
-    if ((int64_t)p.num_tokens * p.warps_per_token >= 4ll * sms * kStreamWarps && p.num_tokens <= 0x3fffffff) {
+    if ((int64_t)p.num_tokens * p.warps_per_token >= 4ll * sms * kStreamWarps && p.num_tokens <= 0x3fffffff &&
+        !p.mixed) {
       static std::atomic<uint64_t> smem_set{0};
       if (ensure_dynamic_smem((const void*)rope_stream_kernel<SINK>, kStreamBytes, smem_set) != VLC_OK)
         return VLC_ERR_CUDA;
@@ -441,6 +450,9 @@ static int fp4_args(Params& p, int64_t num_pages, int block_size, float k_scale,
   if (num_pages <= 0 || num_pages > 0x7fffffff / block_size) return VLC_ERR_SHAPE;
   if (!power_of_two(k_scale) || !power_of_two(v_scale)) return VLC_ERR_UNSUPPORTED;
   p.block_size = block_size;
+  p.block_shift = -1;
+  for (int s = 6; s < 31; ++s)
+    if (block_size == 1 << s) p.block_shift = s;
   p.k_inv_scale = 1.f / k_scale;
   p.v_inv_scale = 1.f / v_scale;
   return VLC_OK;
