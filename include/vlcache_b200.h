@@ -399,7 +399,8 @@ int vlc_mrope_store_kvcache(const int64_t* positions, int64_t axis_stride, int n
  * makes its whole group NaN.  Every value is exact in bf16.  Choose g so that max|x| / g
  * stays below 2688 and the small groups' max|x| / g above 6 * 2^-6.
  * Page of one layer's K or V: [num_kv_heads][block_size * 64 code bytes | block_size * 8
- * scale bytes], block_size a multiple of 64; caches [num_pages] such pages, contiguous.
+ * scale bytes], block_size a multiple of 64, at most 2^20; caches [num_pages] such pages,
+ * contiguous.  The slots that one call writes differ.
  * Slot -> page slot / block_size, row slot % block_size, as in the bf16 cache.
  *
  * vlc_rope_store_kvcache_fp4: vlc_mrope_store_kvcache with its k and v rows quantised into

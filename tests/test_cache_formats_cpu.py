@@ -227,6 +227,9 @@ REFUSALS = [
     ("vlc_decode_attn_fp4", DECODE4, dict(heads=5), SHAPE),
     ("vlc_decode_attn_fp4", DECODE4, dict(heads=34, q_stride=34 * 128, out_stride=34 * 128), UNSUPPORTED),  # 17 a head
     ("vlc_decode_attn_fp4", DECODE4, dict(block=32), UNSUPPORTED),
+    ("vlc_decode_attn_fp4", DECODE4, dict(block=1 << 21), UNSUPPORTED),
+    ("vlc_gather_kvcache_fp4", GATHER, dict(block=1 << 21), UNSUPPORTED),
+    ("vlc_store_kvcache_fp4", STORE4, dict(block=1 << 21), UNSUPPORTED),
     ("vlc_decode_attn_fp4", DECODE4, dict(out_stride=256), STRIDE),
     ("vlc_decode_attn_fp4", DECODE4, dict(q=odd), ALIGN),
     ("vlc_decode_attn_fp4", DECODE4, dict(lens=None), NULL),

@@ -372,6 +372,36 @@ def test_decode_fp4_extreme_magnitudes(ops, size, qsize):
     _check_attention(out, q, kc, vc, bt, [1, 1], lens, scale, 1.0, 1.0, 2.0 ** -11)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+def test_decode_fp4_zero_and_negative_scale(ops, scale):
+    """A scale of 0 weighs every key alike; a negative one favours the least similar."""
+    lens, H, Hk = [700, 65, 1], 8, 2
+    kc, vc, bt = _paged(39, lens, Hk, 64)
+    q = torch.randn(3, H, D, generator=_gen(10)).to(torch.bfloat16)
+    out = ops.decode_attention_fp4(q.cuda(), kc.cuda(), vc.cuda(), bt.cuda(),
+                                   torch.tensor(lens, dtype=torch.int32).cuda(), np.int64(700), np.float32(scale))
+    for i, n in enumerate(lens):
+        k, v = (fp4.sequence(c.numpy(), bt[i].tolist(), n) for c in (kc, vc))
+        ref, size = fp4.attend(q[i:i + 1].double().numpy(), k, v, float(np.float32(scale)))
+        B = abs(scale) * float(np.abs(q[i].double().numpy()).max() * np.abs(k).sum(-1).max())
+        bound = 2.0 ** -8 * np.abs(ref) + (2.0 ** -11 + 2.0 ** -14 * B + 2.0 ** -15) * size
+        assert bool((np.abs(out[i:i + 1].double().cpu().numpy() - ref) <= bound).all())
+
+
+def test_image_rows_move_layer_by_layer_in_4_bits(ops):
+    """copy_image_kv_per_layer on its own stream gives copy_image_kv's bytes."""
+    from vlcache_b200.engine import kv_cache as kvc
+    kv = torch.stack([torch.stack([_pages(61 + 2 * x + y, 6, 2, 64) for x in range(3)]) for y in (0, 1)]).cuda()
+    src, dst = kvc.image_reuse_slots(10, 140, 13, [3, 4, 5], 7, [0, 1, 2], 64)
+    a, b = kv.clone(), kv.clone()
+    kvc.copy_image_kv(a, src, dst, (3, 3, 3))
+    events = kvc.copy_image_kv_per_layer(b, torch.from_numpy(src).cuda(), torch.from_numpy(dst).cuda(), (3, 3, 3),
+                                         torch.cuda.Stream())
+    for e in events:
+        torch.cuda.current_stream().wait_event(e)
+    assert len(events) == 3 and torch.equal(a, b) and not torch.equal(a, kv)
+
+
 def test_decode_fp4_order_and_sharing_of_the_caches(ops):
     """K before V, V before K, and one cache for both give what each place holds."""
     lens, H, Hk = [400, 129], 16, 2

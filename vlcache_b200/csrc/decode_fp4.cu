@@ -566,7 +566,7 @@ struct Joined {
 template <bool SPREAD>
 __global__ void __launch_bounds__(256, 3) decode_fp4_combine_kernel(const float* parts, const float2* part_ml,
                                                                  const int2* places, const int32_t* context_lens,
-                                                                 int num_heads, int num_kv_heads, float v_scale,
+                                                                 int num_warps, int num_heads, int num_kv_heads, float v_scale,
                                                                  __nv_bfloat16* out, int64_t out_seq_stride) {
   __shared__ float4 s_o[8][8];
   __shared__ float2 s_ml[8];
@@ -588,6 +588,9 @@ __global__ void __launch_bounds__(256, 3) decode_fp4_combine_kernel(const float*
     const int h = SPREAD ? blockIdx.y : blockIdx.y * 16 + x * 8 + warp;
     int2 place = make_int2(0, 0);
     if (h < num_heads && !empty) place = places[(int64_t)seq * num_kv_heads + h / G];
+    // A warp that gave up waiting for its copies (recorded) leaves pairs unnoted: nothing is read for them.
+    if ((uint32_t)place.x >= 2u * num_warps || (uint32_t)place.y > (uint32_t)(num_warps - (place.x >> 1)))
+      place = make_int2(0, 1);
     first[x] = (int64_t)place.x * G + h % G;
     rest[x] = (int64_t)(place.x & ~1) * G + h % G;
     count[x] = place.y;
@@ -687,7 +690,7 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
                                    int64_t out_seq_stride, void* workspace, int64_t workspace_bytes, void* stream) {
   if (num_seqs < 0 || max_context_len < 0 || max_context_len > (1 << 30) || block_table_width < 0)
     return VLC_ERR_SHAPE;
-  if (head_dim != HD || block_size <= 0 || block_size % CH != 0) return VLC_ERR_UNSUPPORTED;
+  if (head_dim != HD || block_size <= 0 || block_size % CH != 0 || block_size > fp4::MAX_BLOCK) return VLC_ERR_UNSUPPORTED;
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0) return VLC_ERR_SHAPE;
   const int G = num_heads / num_kv_heads;
   if (G > MAX_GROUP || !power_of_two(k_scale) || !power_of_two(v_scale)) return VLC_ERR_UNSUPPORTED;
@@ -777,7 +780,7 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, spread ? decode_fp4_combine_kernel<true> : decode_fp4_combine_kernel<false>,
-                         (const float*)p.parts, (const float2*)p.part_ml, (const int2*)p.places, context_lens,
+                         (const float*)p.parts, (const float2*)p.part_ml, (const int2*)p.places, context_lens, warps,
                          num_heads, num_kv_heads, v_scale, p.out, out_seq_stride) != cudaSuccess) {
     (void)cudaGetLastError();
     return VLC_ERR_CUDA;

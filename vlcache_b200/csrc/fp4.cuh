@@ -23,6 +23,7 @@ constexpr int GROUP = 16;
 constexpr int CODE_BYTES = HD / 2;
 constexpr int SCALE_BYTES = HD / GROUP;
 constexpr int ROW_BYTES = CODE_BYTES + SCALE_BYTES;
+constexpr int MAX_BLOCK = 1 << 20;  // a head's piece of a page stays within 32-bit offsets
 
 // Offset of a head's piece of a page, and of a row's codes and scales in it.
 __host__ __device__ __forceinline__ int64_t head_offset(int64_t page, int num_kv_heads, int head, int block_size) {

@@ -261,7 +261,7 @@ extern "C" int vlc_gather_kvcache_fp4(const void* k_cache, const void* v_cache, 
                                       int64_t out_layer_stride, void* stream) {
   if (num_seqs < 0 || total_k < 0 || num_layers < 0 || block_table_width < 0 || num_kv_heads <= 0)
     return VLC_ERR_SHAPE;
-  if (head_dim != HD || block_size <= 0 || block_size % TILE != 0) return VLC_ERR_UNSUPPORTED;
+  if (head_dim != HD || block_size <= 0 || block_size % TILE != 0 || block_size > fp4::MAX_BLOCK) return VLC_ERR_UNSUPPORTED;
   if (!power_of_two(k_scale) || !power_of_two(v_scale)) return VLC_ERR_UNSUPPORTED;
   if (num_seqs == 0 || total_k == 0 || num_layers == 0) return VLC_OK;
   if (!k_cache || !v_cache || !block_tables || !cu_seqlens_k || !k_out || !v_out) return VLC_ERR_NULL;
@@ -306,7 +306,7 @@ extern "C" int vlc_mrope_shift_fp4(void* k_cache, void* v_cache, int64_t layer_s
                                    const int32_t* delta_thw, const int32_t* mrope_section, float rope_theta,
                                    void* stream) {
   if (num_rows < 0 || num_layers < 0 || num_kv_heads <= 0) return VLC_ERR_SHAPE;
-  if (head_dim != HD || block_size <= 0 || block_size % TILE != 0) return VLC_ERR_UNSUPPORTED;
+  if (head_dim != HD || block_size <= 0 || block_size % TILE != 0 || block_size > fp4::MAX_BLOCK) return VLC_ERR_UNSUPPORTED;
   if (num_rows == 0 || num_layers == 0) return VLC_OK;
   if (!k_cache || !src_slots || !delta_thw || !mrope_section) return VLC_ERR_NULL;
   if (num_pages <= 0 || num_pages > 0x7fffffff / block_size || num_kv_heads > 65535 || num_layers > 65535)

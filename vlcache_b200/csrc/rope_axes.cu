@@ -446,7 +446,7 @@ static int cache_args(Params& p, const void* value, int64_t value_stride, void* 
 }
 
 static int fp4_args(Params& p, int64_t num_pages, int block_size, float k_scale, float v_scale) {
-  if (block_size <= 0 || block_size % 64 != 0) return VLC_ERR_UNSUPPORTED;
+  if (block_size <= 0 || block_size % 64 != 0 || block_size > fp4::MAX_BLOCK) return VLC_ERR_UNSUPPORTED;
   if (num_pages <= 0 || num_pages > 0x7fffffff / block_size) return VLC_ERR_SHAPE;
   if (!power_of_two(k_scale) || !power_of_two(v_scale)) return VLC_ERR_UNSUPPORTED;
   p.block_size = block_size;

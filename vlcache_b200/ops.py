@@ -766,7 +766,7 @@ def gather_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table
     _need(layers <= 1 or v_cache.stride(0) == layer_stride, "k_cache and v_cache: the same layer stride")
     _need(cu_seqlens_k.dtype == torch.int32 and cu_seqlens_k.dim() == 1 and cu_seqlens_k.is_contiguous()
           and cu_seqlens_k.numel() >= 1, "cu_seqlens_k: contiguous int32 [num_seqs + 1]")
-    seqs = cu_seqlens_k.numel() - 1
+    seqs, total_k = cu_seqlens_k.numel() - 1, int(total_k)
     stride, width = _tables(block_tables, seqs)
     shape = (layers, total_k, hk, HEAD_DIM) if many else (total_k, hk, HEAD_DIM)
     if k_out is None:
@@ -841,11 +841,12 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     _need(context_lens.dtype == torch.int32 and context_lens.numel() == b and context_lens.is_contiguous(),
           "context_lens: contiguous int32, one per sequence")
     out, os = _q_out(q, out)
+    max_context_len = int(max_context_len)
     need = lib().vlc_decode_fp4_workspace_size(b, h, hk, max_context_len)
     if need > 0 and (workspace is None or workspace.nbytes < need):
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     _launch(dev, "vlc_decode_attn_fp4", q.data_ptr(), qs, b, h, k_cache.data_ptr(), v_cache.data_ptr(), pages, block,
-            hk, d, block_tables.data_ptr(), stride, width, context_lens.data_ptr(), int(max_context_len),
+            hk, d, block_tables.data_ptr(), stride, width, context_lens.data_ptr(), max_context_len,
             float(softmax_scale), float(k_scale), float(v_scale), out.data_ptr(), os, _ptr(workspace),
             0 if workspace is None else workspace.nbytes)
     return out
