@@ -596,18 +596,23 @@ def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int, int]:
 _SECTIONS: dict = {}   # pairs per axis -> the C array of them
 
 
-def _rotary_args(positions, cos_sin_cache, sections, n: int, d: int):
-    """Positions and table of the rotating ops; returns (axis stride, axes, sections array, table rows)."""
-    if sections is None:
-        _need(positions.dim() == 1, "positions [tokens] (or [axes, tokens] with mrope_section)")
-        sections = (d // 2,)
+def _sections(sections):
     sections = tuple(sections)
     array = _SECTIONS.get(sections)
     if array is None:
         if len(_SECTIONS) > 64:
             _SECTIONS.clear()
         array = _SECTIONS[sections] = (ctypes.c_int32 * len(sections))(*[int(x) for x in sections])
-    axes = len(sections)
+    return array
+
+
+def _rotary_args(positions, cos_sin_cache, sections, n: int, d: int):
+    """Positions and table of the rotating ops; returns (axis stride, axes, sections array, table rows)."""
+    if sections is None:
+        _need(positions.dim() == 1, "positions [tokens] (or [axes, tokens] with mrope_section)")
+        sections = (d // 2,)
+    array = _sections(sections)
+    axes = len(array)
     shape, stride = positions.shape, positions.stride()
     _need(shape == (axes, n) or (axes == 1 and shape == (n,)), f"positions: [{axes}, {n}]")
     _need(positions.dtype == torch.int64 and (n <= 1 or stride[-1] == 1), "positions: int64, tokens contiguous")
@@ -696,9 +701,7 @@ def _fp4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dims: int = 3) -> 
         _need(k_cache[0].is_contiguous() and v_cache[0].is_contiguous(), "4-bit caches must be contiguous")
     else:
         _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "4-bit caches must be contiguous")
-    block = shape[-1] // FP4_ROW_BYTES
-    _need(block > 0 and shape[-1] == block * FP4_ROW_BYTES, "a 4-bit page is block_size * 72 bytes a head")
-    return shape[-3], shape[-2], block
+    return shape[-3], shape[-2], _fp4_block(shape[-1])
 
 
 def _tables(block_tables: torch.Tensor, num_seqs: int) -> tuple[int, int]:
@@ -783,16 +786,24 @@ def gather_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table
     return k_out, v_out
 
 
-def _shift_fp4(dev, k, v, layers, layer_stride, src_slots, dst_slots, delta_thw, mrope_section, rope_theta) -> None:
-    pages, hk, block = _fp4_caches(k, k if v is None else v, k.dim())
+def _fp4_block(page_bytes: int) -> int:
+    """Block size of a 4-bit page of that many bytes a head."""
+    block = page_bytes // FP4_ROW_BYTES
+    _need(block > 0 and page_bytes == block * FP4_ROW_BYTES, "a 4-bit page is block_size * 72 bytes a head")
+    return block
+
+
+def _shift_fp4(dev, k, v, layers, layer_stride, shape, src_slots, dst_slots, delta_thw, mrope_section,
+               rope_theta) -> None:
+    pages, hk, page_bytes = shape
     n = src_slots.numel()
     for t in (src_slots, dst_slots):
         _need(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n),
               "src_slots / dst_slots: contiguous int32 of one length")
+    _need(len(delta_thw) == 3 and len(mrope_section) == 3, "delta_thw and mrope_section: (t, h, w)")
     d = (ctypes.c_int32 * 3)(*[int(x) for x in delta_thw])
-    sec = (ctypes.c_int32 * 3)(*[int(x) for x in mrope_section])
-    _launch(dev, "vlc_mrope_shift_fp4", k.data_ptr(), _ptr(v), layer_stride, layers, pages, block, hk, HEAD_DIM,
-            src_slots.data_ptr(), _ptr(dst_slots), n, d, sec, float(rope_theta))
+    _launch(dev, "vlc_mrope_shift_fp4", k, v, layer_stride, layers, pages, _fp4_block(page_bytes), hk, HEAD_DIM,
+            src_slots.data_ptr(), _ptr(dst_slots), n, d, _sections(mrope_section), float(rope_theta))
 
 
 def mrope_shift_fp4(kv_cache: torch.Tensor, src_slots: torch.Tensor, dst_slots: torch.Tensor | None, delta_thw,
@@ -803,10 +814,12 @@ def mrope_shift_fp4(kv_cache: torch.Tensor, src_slots: torch.Tensor, dst_slots: 
     16 pairs whose delta is 0 keep their bits, so a zero delta copies.  No destination may
     be another row's source (``engine.kv_cache.check_reuse_slots``)."""
     dev = _device(kv_cache, src_slots, dst_slots)
-    _need(kv_cache.dim() == 5 and kv_cache.shape[0] == 2 and kv_cache.is_contiguous(),
+    shape, stride = kv_cache.shape, kv_cache.stride()
+    _need(kv_cache.dtype == torch.uint8 and len(shape) == 5 and shape[0] == 2 and kv_cache.is_contiguous(),
           "kv_cache: contiguous uint8 [2, layers, pages, Hk, block * 72]")
-    _shift_fp4(dev, kv_cache[0], kv_cache[1], kv_cache.shape[1], kv_cache.stride(1), src_slots, dst_slots, delta_thw,
-               mrope_section, rope_theta)
+    k = kv_cache.data_ptr()
+    _shift_fp4(dev, k, k + stride[0], shape[1], stride[1], shape[2:], src_slots, dst_slots, delta_thw, mrope_section,
+               rope_theta)
 
 
 def mrope_shift_layer_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor | None, src_slots: torch.Tensor,
@@ -815,8 +828,9 @@ def mrope_shift_layer_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor | None, s
     """``mrope_shift_fp4`` of one layer's caches uint8 [pages, Hk, block * 72] (``v_cache`` None:
     K alone)."""
     dev = _device(k_cache, v_cache, src_slots, dst_slots)
-    _need(k_cache.dim() == 3, "a 4-bit cache is uint8 [pages, num_kv_heads, block_size * 72]")
-    _shift_fp4(dev, k_cache, v_cache, 1, 0, src_slots, dst_slots, delta_thw, mrope_section, rope_theta)
+    _fp4_caches(k_cache, k_cache if v_cache is None else v_cache)
+    _shift_fp4(dev, k_cache.data_ptr(), _ptr(v_cache), 1, 0, k_cache.shape, src_slots, dst_slots, delta_thw,
+               mrope_section, rope_theta)
 
 
 def decode_fp4_workspace_bytes(num_seqs: int, num_heads: int, num_kv_heads: int, max_context_len: int) -> int:
