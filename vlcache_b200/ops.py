@@ -697,10 +697,10 @@ def _fp4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dims: int = 3) -> 
     if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8 or len(shape) != dims:
         raise ValueError("a 4-bit cache is uint8 [pages, num_kv_heads, block_size * 72]")
     _need(v_cache.shape == shape, "k_cache and v_cache: the same shape")
-    if dims == 4 and shape[0] > 0:   # the layers may lie apart
-        _need(k_cache[0].is_contiguous() and v_cache[0].is_contiguous(), "4-bit caches must be contiguous")
-    else:
-        _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "4-bit caches must be contiguous")
+    dense = (shape[-2] * shape[-1], shape[-1], 1)   # of a layer; layers may lie apart
+    for t in (k_cache, v_cache):
+        if t.stride()[-3:] != dense and not (t if dims == 3 or shape[0] == 0 else t[0]).is_contiguous():
+            raise ValueError("4-bit caches must be contiguous")
     return shape[-3], shape[-2], _fp4_block(shape[-1])
 
 
