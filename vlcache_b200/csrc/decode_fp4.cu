@@ -657,15 +657,19 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
 }
 
 // Joins the parts of the pairs that several warps shared and writes zeros for empty sequences.
-// SPREAD (few pairs of many parts): a block takes a quarter of one head's dims; its 32 groups of
-// eight lanes take the parts in turn.  Otherwise a block takes 16 heads of a sequence, a warp every
-// eighth of them.  The decode kernel fills the SMs to its end, so what a block does before the wait
+// kManyParts (few pairs): a block takes a quarter of one head's dims; its 32 groups of eight lanes
+// take the parts in turn.  Otherwise a block takes 8 or 16 heads of a sequence, a warp every eighth of
+// them, and loads eight parts of one head, or three of two, at once.  The decode kernel fills the SMs to its end, so what a block does before the wait
 // is not hidden: where a pair's parts are was noted by the warp that began it.
-template <bool SPREAD>
+enum Join { kFewParts, kSomeParts, kManyParts };
+template <Join JOIN>
 __global__ void __launch_bounds__(256, 3) decode_fp4_combine_kernel(const float* parts, const float2* part_ml,
                                                                  const int2* places, const int32_t* context_lens,
                                                                  int num_warps, int num_heads, int num_kv_heads, float v_scale,
                                                                  __nv_bfloat16* out, int64_t out_seq_stride) {
+  constexpr bool SPREAD = JOIN == kManyParts;
+  constexpr int HEADS = JOIN == kFewParts ? 2 : 1;  // of a warp
+  constexpr int PARTS = JOIN == kFewParts ? 3 : 8;  // of a head, loaded at once
   __shared__ float4 s_o[8][8];
   __shared__ float2 s_ml[8];
   const int seq = blockIdx.x, warp = warp_id(), lane = lane_id();
@@ -678,12 +682,11 @@ __global__ void __launch_bounds__(256, 3) decode_fp4_combine_kernel(const float*
   // Every block waits, those with nothing to join too: what follows in the stream may rely on this
   // grid's end for the decode kernel's.
   pdl_wait();
-  constexpr int HEADS = SPREAD ? 1 : 2;  // of a warp
   int64_t first[HEADS], rest[HEADS];     // rows of parts: part i > 0 is at rest + 2 G i
   int count[HEADS];                      // parts of the head
 #pragma unroll
   for (int x = 0; x < HEADS; ++x) {
-    const int h = SPREAD ? blockIdx.y : blockIdx.y * 16 + x * 8 + warp;
+    const int h = SPREAD ? blockIdx.y : blockIdx.y * (8 * HEADS) + x * 8 + warp;
     int2 place = make_int2(0, 0);
     if (h < num_heads && !empty) place = places[(int64_t)seq * num_kv_heads + h / G];
     // A warp that gave up waiting for its copies (recorded) leaves pairs unnoted: nothing is read for them.
@@ -723,9 +726,8 @@ __global__ void __launch_bounds__(256, 3) decode_fp4_combine_kernel(const float*
     dst[blockIdx.y * (HD / 4)] = sum.result(v_scale);
   }
   if constexpr (!SPREAD) {
-    constexpr int PARTS = 3;  // loads of that many parts of both heads at once: mostly all there are
     Joined sum[HEADS];
-    for (int i0 = 0; i0 < max(count[0], count[1]); i0 += PARTS) {
+    for (int i0 = 0; i0 < max(count[0], count[HEADS - 1]); i0 += PARTS) {
       float2 x[HEADS][PARTS];
       float4 v[HEADS][PARTS];
 #pragma unroll
@@ -745,7 +747,7 @@ __global__ void __launch_bounds__(256, 3) decode_fp4_combine_kernel(const float*
     }
 #pragma unroll
     for (int y = 0; y < HEADS; ++y) {
-      const int h = blockIdx.y * 16 + y * 8 + warp;
+      const int h = blockIdx.y * (8 * HEADS) + y * 8 + warp;
       if (h < num_heads && count[y] != 1) dst[h * (HD / 4)] = sum[y].result(v_scale);  // (0 parts: zeros)
     }
   }
@@ -758,9 +760,10 @@ static int grid_warps(int num_seqs, int num_heads, int num_kv_heads, int max_con
   return (int)std::max<int64_t>(1, std::min(resident, most));
 }
 
-// Whether clusters take whole pairs: where every block has an SM to itself.
+// Whether clusters take whole pairs.  Measured with up to 1024 keys against the line of chunks: 36
+// pairs 6.8 : 10.7 us, 128 pairs 10.8 : 20.8 (of 200 keys 9.8 : 9.5), 256 pairs 20.5 : 20.2 (16.0 : 10.2).
 static bool whole_pairs(int num_seqs, int num_kv_heads, int max_context_len, int num_sms) {
-  return max_context_len <= PAIR_KEYS && (int64_t)num_seqs * num_kv_heads * PAIR_BLOCKS <= num_sms;
+  return max_context_len <= PAIR_KEYS && (int64_t)num_seqs * num_kv_heads <= num_sms;
 }
 
 static int64_t workspace_bytes_for(int64_t warps, int group, int64_t pairs) {
@@ -883,10 +886,13 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   }
   int rc = launch_status();
   if (rc != VLC_OK) return rc;
-  // Few pairs: each has many parts, which several blocks read.
-  const bool spread = warps > 8ll * num_seqs * num_kv_heads;
+  // Parts of a pair on average, and whether four blocks a head are blocks enough to be there at once.
+  // 32 sequences of 1000 keys, 28 heads: 13.3 us with kSomeParts, 20.8 with kManyParts.
+  const int64_t parts = warps / ((int64_t)num_seqs * num_kv_heads) + 1;
+  const Join join = parts <= 4 ? kFewParts : (int64_t)num_seqs * num_heads <= sms ? kManyParts : kSomeParts;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = spread ? dim3(num_seqs, num_heads, 4) : dim3(num_seqs, (num_heads + 15) / 16);
+  cfg.gridDim = join == kManyParts ? dim3(num_seqs, num_heads, 4)
+                                   : dim3(num_seqs, (num_heads + (join == kFewParts ? 15 : 7)) / (join == kFewParts ? 16 : 8));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -894,7 +900,10 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, spread ? decode_fp4_combine_kernel<true> : decode_fp4_combine_kernel<false>,
+  if (cudaLaunchKernelEx(&cfg,
+                         join == kManyParts   ? decode_fp4_combine_kernel<kManyParts>
+                         : join == kSomeParts ? decode_fp4_combine_kernel<kSomeParts>
+                                              : decode_fp4_combine_kernel<kFewParts>,
                          (const float*)p.parts, (const float2*)p.part_ml, (const int2*)p.places, context_lens, warps,
                          num_heads, num_kv_heads, v_scale, p.out, out_seq_stride) != cudaSuccess) {
     (void)cudaGetLastError();
