@@ -360,6 +360,18 @@ def test_decode_fp4(ops, H, Hk, block, lens):
         _check_attention(out, q, kc, vc, bt, [1] * len(lens), lens, SCALE, 2.0, 0.25, 2.0 ** -11)
 
 
+@pytest.mark.parametrize("H,Hk", [(28, 4), (40, 4)])   # 7 and 10 query heads a KV head
+def test_decode_fp4_of_many_ragged_sequences(ops, H, Hk):
+    """More pairs than SMs, some of them in dozens of parts, some in one, some empty."""
+    lens = [int(x) for x in torch.randint(0, 300, (60,), generator=_gen(21))]
+    lens[7], lens[8], lens[59] = 2000, 0, 1500
+    kc, vc, bt = _paged(23, lens, Hk, 64)
+    q = torch.randn(len(lens), H, D, generator=_gen(5)).to(torch.bfloat16)
+    out = ops.decode_attention_fp4(q.cuda(), kc.cuda(), vc.cuda(), bt.cuda(),
+                                   torch.tensor(lens, dtype=torch.int32).cuda(), 2000, SCALE)
+    _check_attention(out, q, kc, vc, bt, [1] * len(lens), lens, SCALE, 1.0, 1.0, 2.0 ** -11)
+
+
 @pytest.mark.parametrize("size,qsize", [(300.0, 1e4), (2.0 ** -6, 2.0 ** -20), (1.0, 1e30)])
 def test_decode_fp4_extreme_magnitudes(ops, size, qsize):
     """Keys at the ends of the scales' range, queries far outside f16's: the power of two that q

@@ -657,58 +657,56 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
 }
 
 // Joins the parts of the pairs that several warps shared and writes zeros for empty sequences.
-// kManyParts (few pairs): a block takes a quarter of one head's dims; its 32 groups of eight lanes
-// take the parts in turn.  Otherwise a block takes 8 or 16 heads of a sequence, a warp every eighth of
-// them, and loads eight parts of one head, or three of two, at once.  The decode kernel fills the SMs to its end, so what a block does before the wait
-// is not hidden: where a pair's parts are was noted by the warp that began it.
+// kFewParts: a block takes eight heads of a sequence, a warp each, and loads eight parts at once.
+// kSomeParts: a block takes one head, and its warps take the parts in turn.  kManyParts: a block takes a
+// quarter of one head's dims, and its 32 groups of eight lanes take the parts in turn.  The decode kernel
+// fills the SMs to its end, so what a block does before the wait is not hidden: where a pair's parts are
+// was noted by the warp that began it.
+// Decode and join, us (few : some : many), 28 heads of 4 unless noted: parts 2, 256 sequences of
+// 100-1000 keys 35.1 : 47.5 : 101; parts 7, 64 of 3000-5000 37.5 : 40.2 : 55.2; parts 14, 32 of 3000-5000
+// 26.6 : 26.5 : 33.2; parts 28, 16 of 5000-8000 25.4 : 21.8 : 25.8; parts 112, 4 of 8000 25.8 : 13.9 : 14.0;
+// parts 223, 8 heads of 8, one of 32000 43 : 19.1 : 17.0; parts 445, one of 32000 67 : 18.6 : 14.9.
 enum Join { kFewParts, kSomeParts, kManyParts };
 template <Join JOIN>
 __global__ void __launch_bounds__(256, 3) decode_fp4_combine_kernel(const float* parts, const float2* part_ml,
                                                                  const int2* places, const int32_t* context_lens,
                                                                  int num_warps, int num_heads, int num_kv_heads, float v_scale,
                                                                  __nv_bfloat16* out, int64_t out_seq_stride) {
-  constexpr bool SPREAD = JOIN == kManyParts;
-  constexpr int HEADS = JOIN == kFewParts ? 2 : 1;  // of a warp
-  constexpr int PARTS = JOIN == kFewParts ? 3 : 8;  // of a head, loaded at once
-  __shared__ float4 s_o[8][8];
+  constexpr bool SPREAD = JOIN != kFewParts;
+  constexpr int LANES = JOIN == kManyParts ? 8 : 32;  // four dims each, of one part
+  constexpr int PARTS = 8;  // of a head, loaded at once by a warp of kFewParts
+  __shared__ float4 s_o[8][LANES];
   __shared__ float2 s_ml[8];
   const int seq = blockIdx.x, warp = warp_id(), lane = lane_id();
   const int G = num_heads / num_kv_heads;
-  // dims: 32 z + 4 (lane % 8) of a quarter, or 4 lane
-  const int dim4 = SPREAD ? blockIdx.z * 8 + (lane & 7) : lane;
+  const int dim4 = blockIdx.z * LANES + lane % LANES;  // all of the dims, or a quarter
   const float4* po = reinterpret_cast<const float4*>(parts) + dim4;
   uint2* const dst = reinterpret_cast<uint2*>(out + (int64_t)seq * out_seq_stride) + dim4;
   const bool empty = __ldg(context_lens + seq) <= 0;
   // Every block waits, those with nothing to join too: what follows in the stream may rely on this
   // grid's end for the decode kernel's.
   pdl_wait();
-  int64_t first[HEADS], rest[HEADS];     // rows of parts: part i > 0 is at rest + 2 G i
-  int count[HEADS];                      // parts of the head
-#pragma unroll
-  for (int x = 0; x < HEADS; ++x) {
-    const int h = SPREAD ? blockIdx.y : blockIdx.y * (8 * HEADS) + x * 8 + warp;
-    int2 place = make_int2(0, 0);
-    if (h < num_heads && !empty) place = places[(int64_t)seq * num_kv_heads + h / G];
-    // A warp that gave up waiting for its copies (recorded) leaves pairs unnoted: nothing is read for them.
-    if ((uint32_t)place.x >= 2u * num_warps || (uint32_t)place.y > (uint32_t)(num_warps - (place.x >> 1)))
-      place = make_int2(0, 1);
-    first[x] = (int64_t)place.x * G + h % G;
-    rest[x] = (int64_t)(place.x & ~1) * G + h % G;
-    count[x] = place.y;
-  }
+  const int h = SPREAD ? blockIdx.y : blockIdx.y * 8 + warp;
+  int2 place = make_int2(0, 0);
+  if (h < num_heads && !empty) place = places[(int64_t)seq * num_kv_heads + h / G];
+  // A warp that gave up waiting for its copies (recorded) leaves pairs unnoted: nothing is read for them.
+  if ((uint32_t)place.x >= 2u * num_warps || (uint32_t)place.y > (uint32_t)(num_warps - (place.x >> 1)))
+    place = make_int2(0, 1);
+  const int64_t first = (int64_t)place.x * G + h % G, rest = (int64_t)(place.x & ~1) * G + h % G;
+  const int count = place.y;  // parts of the head, of which part i > 0 is row rest + 2 G i
   if constexpr (SPREAD) {
-    if (empty && threadIdx.x < 8) dst[blockIdx.y * (HD / 4)] = make_uint2(0, 0);
-    if (count[0] <= 1) return;  // empty, or written by its warp
+    if (empty && threadIdx.x < LANES) dst[h * (HD / 4)] = make_uint2(0, 0);
+    if (count <= 1) return;  // empty, or written by its warp
     Joined sum;
 #pragma unroll 4
-    for (int i = threadIdx.x >> 3; i < count[0]; i += 32) {
-      const int64_t s = i == 0 ? first[0] : rest[0] + (int64_t)i * 2 * G;
+    for (int i = threadIdx.x / LANES; i < count; i += 256 / LANES) {
+      const int64_t s = i == 0 ? first : rest + (int64_t)i * 2 * G;
       const float2 x = part_ml[s];
       const float4 v = po[s * (HD / 4)];
       sum.add(x.x, x.y, v);
     }
 #pragma unroll
-    for (int d = 8; d < 32; d <<= 1) {
+    for (int d = LANES; d < 32; d <<= 1) {
       const float m = __shfl_xor_sync(0xffffffffu, sum.m, d), l = __shfl_xor_sync(0xffffffffu, sum.l, d);
       float4 v;
       v.x = __shfl_xor_sync(0xffffffffu, sum.o.x, d);
@@ -717,39 +715,32 @@ __global__ void __launch_bounds__(256, 3) decode_fp4_combine_kernel(const float*
       v.w = __shfl_xor_sync(0xffffffffu, sum.o.w, d);
       sum.add(m, l, v);
     }
-    if (lane < 8) s_o[warp][lane] = sum.o;
+    if (lane < LANES) s_o[warp][lane] = sum.o;
     if (lane == 0) s_ml[warp] = make_float2(sum.m, sum.l);
     __syncthreads();
-    if (threadIdx.x >= 8) return;
+    if (threadIdx.x >= LANES) return;
 #pragma unroll
     for (int w = 1; w < 8; ++w) sum.add(s_ml[w].x, s_ml[w].y, s_o[w][lane]);
-    dst[blockIdx.y * (HD / 4)] = sum.result(v_scale);
+    dst[h * (HD / 4)] = sum.result(v_scale);
   }
   if constexpr (!SPREAD) {
-    Joined sum[HEADS];
-    for (int i0 = 0; i0 < max(count[0], count[HEADS - 1]); i0 += PARTS) {
-      float2 x[HEADS][PARTS];
-      float4 v[HEADS][PARTS];
+    if (h >= num_heads || count == 1) return;  // (0 parts: zeros)
+    Joined sum;
+    for (int i0 = 0; i0 < count; i0 += PARTS) {
+      float2 x[PARTS];
+      float4 v[PARTS];
 #pragma unroll
-      for (int y = 0; y < HEADS; ++y)
+      for (int i = 0; i < PARTS; ++i) {
+        if (i0 + i >= count) continue;
+        const int64_t s = i0 + i == 0 ? first : rest + (int64_t)(i0 + i) * 2 * G;
+        x[i] = part_ml[s];
+        v[i] = po[s * (HD / 4)];
+      }
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) {
-          if (count[y] <= 1 || i0 + i >= count[y]) continue;
-          const int64_t s = i0 + i == 0 ? first[y] : rest[y] + (int64_t)(i0 + i) * 2 * G;
-          x[y][i] = part_ml[s];
-          v[y][i] = po[s * (HD / 4)];
-        }
-#pragma unroll
-      for (int y = 0; y < HEADS; ++y)
-#pragma unroll
-        for (int i = 0; i < PARTS; ++i)
-          if (count[y] > 1 && i0 + i < count[y]) sum[y].add(x[y][i].x, x[y][i].y, v[y][i]);
+      for (int i = 0; i < PARTS; ++i)
+        if (i0 + i < count) sum.add(x[i].x, x[i].y, v[i]);
     }
-#pragma unroll
-    for (int y = 0; y < HEADS; ++y) {
-      const int h = blockIdx.y * (8 * HEADS) + y * 8 + warp;
-      if (h < num_heads && count[y] != 1) dst[h * (HD / 4)] = sum[y].result(v_scale);  // (0 parts: zeros)
-    }
+    dst[h * (HD / 4)] = sum.result(v_scale);
   }
 }
 
@@ -760,10 +751,13 @@ static int grid_warps(int num_seqs, int num_heads, int num_kv_heads, int max_con
   return (int)std::max<int64_t>(1, std::min(resident, most));
 }
 
-// Whether clusters take whole pairs.  Measured with up to 1024 keys against the line of chunks: 36
-// pairs 6.8 : 10.7 us, 128 pairs 10.8 : 20.8 (of 200 keys 9.8 : 9.5), 256 pairs 20.5 : 20.2 (16.0 : 10.2).
-static bool whole_pairs(int num_seqs, int num_kv_heads, int max_context_len, int num_sms) {
-  return max_context_len <= PAIR_KEYS && (int64_t)num_seqs * num_kv_heads <= num_sms;
+// Whether clusters take whole pairs.  Measured against the line of chunks, us, of 1000 keys (of 200): 28
+// heads of 4, 4 pairs 5.2 : 7.2 (5.2 : 7.5), 64 pairs 7.4 : 9.4 (7.2 : 8.5), 128 pairs 10.7 : 13.8
+// (10.5 : 9.0), 256 pairs 20.4 : 18.8 (16.4 : 10.0).  With over 8 query heads a KV head (32 of 2) a block
+// takes more registers: 64 pairs 9.8 : 13.3 (9.6 : 10.1), 128 pairs 17.8 : 15.7 (17.3 : 11.6).
+static bool whole_pairs(int num_seqs, int num_heads, int num_kv_heads, int max_context_len, int num_sms) {
+  const int64_t most = num_heads / num_kv_heads <= 8 ? num_sms : num_sms / 2;
+  return max_context_len <= PAIR_KEYS && (int64_t)num_seqs * num_kv_heads <= most;
 }
 
 static int64_t workspace_bytes_for(int64_t warps, int group, int64_t pairs) {
@@ -784,7 +778,7 @@ using namespace vlc::decode_fp4;
 extern "C" int64_t vlc_decode_fp4_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int max_context_len) {
   if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_context_len < 0) return 0;
   const int sms = vlc_num_sms();
-  if (whole_pairs(num_seqs, num_kv_heads, max_context_len, sms)) return 0;
+  if (whole_pairs(num_seqs, num_heads, num_kv_heads, max_context_len, sms)) return 0;
   return workspace_bytes_for(grid_warps(num_seqs, num_heads, num_kv_heads, max_context_len, sms),
                              num_heads / num_kv_heads, (int64_t)num_seqs * num_kv_heads);
 }
@@ -812,7 +806,7 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   if (num_kv_heads > 65535 || num_seqs > 65535 || num_heads > 65535) return VLC_ERR_SHAPE;
   if (max_context_len == 0) max_context_len = 1;
   const int sms = vlc_num_sms();
-  const bool whole = whole_pairs(num_seqs, num_kv_heads, max_context_len, sms);
+  const bool whole = whole_pairs(num_seqs, num_heads, num_kv_heads, max_context_len, sms);
   const int warps = whole ? 0 : grid_warps(num_seqs, num_heads, num_kv_heads, max_context_len, sms);
   if (!whole) {
     if (!workspace || workspace_bytes < workspace_bytes_for(warps, G, (int64_t)num_seqs * num_kv_heads))
@@ -886,13 +880,12 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   }
   int rc = launch_status();
   if (rc != VLC_OK) return rc;
-  // Parts of a pair on average, and whether four blocks a head are blocks enough to be there at once.
-  // 32 sequences of 1000 keys, 28 heads: 13.3 us with kSomeParts, 20.8 with kManyParts.
+  // By the parts of a pair on average, and where quarters of all heads are at most two blocks an SM.
   const int64_t parts = warps / ((int64_t)num_seqs * num_kv_heads) + 1;
-  const Join join = parts <= 4 ? kFewParts : (int64_t)num_seqs * num_heads <= sms ? kManyParts : kSomeParts;
+  const Join join = parts <= 10 ? kFewParts : (int64_t)num_seqs * num_heads <= sms / 2 ? kManyParts : kSomeParts;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = join == kManyParts ? dim3(num_seqs, num_heads, 4)
-                                   : dim3(num_seqs, (num_heads + (join == kFewParts ? 15 : 7)) / (join == kFewParts ? 16 : 8));
+  cfg.gridDim = join == kFewParts ? dim3(num_seqs, (num_heads + 7) / 8)
+                                  : dim3(num_seqs, num_heads, join == kManyParts ? 4 : 1);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -901,9 +894,9 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg,
-                         join == kManyParts   ? decode_fp4_combine_kernel<kManyParts>
+                         join == kFewParts    ? decode_fp4_combine_kernel<kFewParts>
                          : join == kSomeParts ? decode_fp4_combine_kernel<kSomeParts>
-                                              : decode_fp4_combine_kernel<kFewParts>,
+                                              : decode_fp4_combine_kernel<kManyParts>,
                          (const float*)p.parts, (const float2*)p.part_ml, (const int2*)p.places, context_lens, warps,
                          num_heads, num_kv_heads, v_scale, p.out, out_seq_stride) != cudaSuccess) {
     (void)cudaGetLastError();
