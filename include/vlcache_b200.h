@@ -376,8 +376,8 @@ uint64_t vlc_xxh64(const void* data, int64_t nbytes, uint64_t seed);
  * nanovllm/layers/rotary_embedding.py:51-71); the rotation is HF transformers'
  * apply_multimodal_rotary_pos_emb (modeling_qwen2_5_vl.py:627-665).
  *   positions [num_axes][axis_stride] int64, num_axes 1 .. 4 (axis_stride 0: one row for
- *   every axis); sections[num_axes] pairs per axis, in order, summing to head_dim / 2: rotate-half pair j takes the position of
- *   the axis whose section holds it.
+ *   every axis); sections[num_axes] pairs per axis, in order, summing to head_dim / 2:
+ *   rotate-half pair j takes the position of the axis whose section holds it.
  * Everything else as vlc_rope_store_kvcache, whose result it gives, bit for bit, when a
  * row's positions are equal on all axes.  A row with a position outside the table on any
  * axis is recorded (VLC_DEV_ERR_POSITION) and its q and k are not stored.

@@ -724,6 +724,32 @@ def test_ops_refusals(ops):
     assert not bool(c.any())
 
 
+def test_bounds_outside_32_bits_are_refused(ops):
+    q = torch.zeros(1, 2, D, dtype=torch.bfloat16, device="cuda")
+    c = torch.zeros(1, 2, 64 * 72, dtype=torch.uint8, device="cuda")
+    s = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for bound in (-1, 2 ** 30 + 1, 2 ** 32 + 64):
+        with pytest.raises(ValueError):
+            ops.decode_attention_fp4(q, c, c, s.view(1, 1), s, bound, 0.1)
+
+
+def test_page_copies_of_host_lists_are_not_captured(ops):
+    from vlcache_b200.engine import kv_cache as kvc
+    kv = torch.arange(2 * 4 * 64 * 72, device="cuda").to(torch.uint8).view(2, 1, 4, 1, 64 * 72)
+    src, dst = (torch.tensor([x], dtype=torch.int32, device="cuda") for x in (1, 3))
+    before = kv.clone()
+    ops.copy_kv_pages(kv, dst, dst)   # (loads the kernel)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError):
+            kvc.copy_pages(kv, [1], [3])
+        ops.copy_kv_pages(kv, src, dst)
+    graph.replay()
+    before[:, :, 3] = before[:, :, 1]
+    assert torch.equal(kv, before)
+
+
 # ------------------------------------------------------------------ together, as an engine runs them
 @pytest.mark.parametrize("axes", [1, 3])
 def test_attention_layers_over_a_4bit_cache(ops, axes):

@@ -166,7 +166,8 @@ def check_reuse_slots(old_slots, new_slots) -> None:
 def copy_pages(kv_cache: torch.Tensor, src_pages, dst_pages) -> None:
     """Copy whole pages of every layer (host lists; ``PagePool.fork`` and ``PagePool.compact``
     return such lists), after checking them: destinations differ, and none is the source
-    of another pair."""
+    of another pair.  Not for graph capture: a replay would find other lists in the staging
+    memory (``ops.copy_kv_pages`` takes lists on the device)."""
     src, dst = np.asarray(src_pages, dtype=np.int64).ravel(), np.asarray(dst_pages, dtype=np.int64).ravel()
     if src.shape != dst.shape:
         raise ValueError("source and destination page lists differ in length")
@@ -180,6 +181,8 @@ def copy_pages(kv_cache: torch.Tensor, src_pages, dst_pages) -> None:
     moved = src != dst
     if np.intersect1d(src[moved], dst[moved]).size:
         raise ValueError("a page is the source of one copy and the destination of another")
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("copy_pages takes host lists, which a graph cannot hold: capture ops.copy_kv_pages")
     up = torch.from_numpy(np.stack([src, dst]).astype(np.int32)).pin_memory().to(kv_cache.device, non_blocking=True)
     ops.copy_kv_pages(kv_cache, up[0], up[1])
 

@@ -856,6 +856,7 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
           "context_lens: contiguous int32, one per sequence")
     out, os = _q_out(q, out)
     max_context_len = int(max_context_len)
+    _need(0 <= max_context_len <= 1 << 30, "max_context_len: 0 .. 2^30")
     need = lib().vlc_decode_fp4_workspace_size(b, h, hk, max_context_len)
     if need > 0 and (workspace is None or workspace.nbytes < need):
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
