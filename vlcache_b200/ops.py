@@ -572,7 +572,7 @@ def _device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
 def _launch(dev: int, name: str, *args) -> None:
     """Call a C-ABI entry point on device ``dev`` and its current stream (the last argument)."""
     fn = getattr(lib(), name)
-    if dev == torch.cuda.current_device():
+    if dev == (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
         status = fn(*args, _stream())
     else:
         with torch.cuda.device(dev):
@@ -593,6 +593,7 @@ def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int, int]:
     return n, h, d, stride[0] if n > 1 else h * d
 
 
+_INT3 = ctypes.c_int32 * 3
 _SECTIONS: dict = {}   # pairs per axis -> the C array of them
 
 
@@ -634,9 +635,12 @@ def _q_out(query: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Tensor,
 def _kv_rows(key: torch.Tensor, value: torch.Tensor, n: int, d: int) -> tuple[int, int, int]:
     """(KV heads, key's token stride, value's) of n tokens' key and value rows."""
     nk, hk, dk, ks = _rows(key, "key")
-    _need(nk == n and dk == d, "query and key: the same tokens and head_dim")
-    _need(value.shape == key.shape, "value: key's shape")
-    return hk, ks, _rows(value, "value")[3]
+    nv, hv, dv, vs = _rows(value, "value")
+    if nk != n or dk != d:
+        raise ValueError("query and key: the same tokens and head_dim")
+    if nv != n or hv != hk or dv != d:
+        raise ValueError("value: key's shape")
+    return hk, ks, vs
 
 
 def _slots(slot_mapping: torch.Tensor, n: int) -> None:
@@ -772,13 +776,13 @@ def gather_kvcache_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table
     seqs, total_k = cu_seqlens_k.numel() - 1, int(total_k)
     stride, width = _tables(block_tables, seqs)
     shape = (layers, total_k, hk, HEAD_DIM) if many else (total_k, hk, HEAD_DIM)
-    if k_out is None:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
-    if v_out is None:
-        v_out = torch.empty_like(k_out, memory_format=torch.contiguous_format)
     for t in (k_out, v_out):
-        if t.shape != shape or t.dtype != torch.bfloat16 or not t.is_contiguous():
+        if t is not None and (t.shape != shape or t.dtype != torch.bfloat16 or not t.is_contiguous()):
             raise ValueError(f"k_out / v_out: contiguous bf16 {list(shape)}")
+    if k_out is None:
+        k_out = torch.empty(*shape, dtype=torch.bfloat16, device=k_cache.device)
+    if v_out is None:
+        v_out = torch.empty_like(k_out)
     row = hk * HEAD_DIM
     _launch(dev, "vlc_gather_kvcache_fp4", k_cache.data_ptr(), v_cache.data_ptr(), layer_stride, layers, pages, block,
             hk, HEAD_DIM, block_tables.data_ptr(), stride, width, cu_seqlens_k.data_ptr(), seqs, total_k,
@@ -801,7 +805,7 @@ def _shift_fp4(dev, k, v, layers, layer_stride, shape, src_slots, dst_slots, del
         _need(t is None or (t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n),
               "src_slots / dst_slots: contiguous int32 of one length")
     _need(len(delta_thw) == 3 and len(mrope_section) == 3, "delta_thw and mrope_section: (t, h, w)")
-    d = (ctypes.c_int32 * 3)(*[int(x) for x in delta_thw])
+    d = _INT3(*[int(x) for x in delta_thw])
     _launch(dev, "vlc_mrope_shift_fp4", k, v, layer_stride, layers, pages, _fp4_block(page_bytes), hk, HEAD_DIM,
             src_slots.data_ptr(), _ptr(dst_slots), n, d, _sections(mrope_section), float(rope_theta))
 
