@@ -31,6 +31,7 @@
 // takes it) and cancels.  Sums are fp32.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "fp4.cuh"
 #include "runtime.h"
@@ -374,9 +375,12 @@ __device__ __forceinline__ void copy_chunk(const Params& p, uint8_t* st, uint64_
 }
 
 // Few pairs of few keys: a cluster of four blocks takes a pair, each of its warps one chunk of the
-// keys, and the warps join through the blocks' shared memory.  One launch where the line of chunks
-// takes two, and a scheduler for every warp: one sequence of 700 keys, 16 query and 2 KV heads:
-// 5.3 us against 7.1 with the line (and against 7.2 with sixteen warps in one block).
+// keys (chunk i block i % 4, so that few chunks spread over the SMs), and the warps join through the
+// blocks' shared memory, where a warp's O takes the place of its chunk: four blocks an SM.  One launch
+// where the line of chunks takes two, and a scheduler for every warp: one sequence of 700 keys, 16
+// query and 2 KV heads: 4.8 us against 7.1 with the line (and against 7.2 with sixteen warps in one
+// block).  Several chunks a warp, in clusters of 4 or 8, took a microsecond more for the loop and
+// gained 5 .. 14 % on the line at 2000 .. 4000 keys.
 constexpr int PAIR_BLOCKS = 4, PAIR_WARPS = 4;
 constexpr int PAIR_SMEM = PAIR_WARPS * STAGE_BYTES + 512;
 constexpr int PAIR_KEYS = PAIR_BLOCKS * PAIR_WARPS * CH;
@@ -400,17 +404,18 @@ __global__ void __launch_bounds__(PAIR_WARPS * 32) __cluster_dims__(PAIR_BLOCKS,
     decode_fp4_pair_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int HEADS = NT * 8;
+  static_assert(HEADS * HD * sizeof(float) <= STAGE_BYTES, "a warp's O takes the place of its chunk");
   __shared__ __align__(8) uint64_t full_all[PAIR_WARPS];
-  __shared__ __align__(16) float sm_o[PAIR_WARPS][HEADS][HD];  // static: at the same place in every block
   __shared__ __align__(8) float2 sm_ml[PAIR_WARPS][HEADS];
   const int warp = warp_id(), lane = lane_id();
   const int r = lane >> 2, t = lane & 3;
   const int rank = (int)cluster_ctarank();
   const int head = blockIdx.x / PAIR_BLOCKS, seq = blockIdx.y, G = p.group;
-  uint8_t* const st = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 511) & ~uintptr_t(511)) +
-                      warp * STAGE_BYTES;
+  // (at the same place in every block)
+  uint8_t* const first = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 511) & ~uintptr_t(511));
+  uint8_t* const st = first + warp * STAGE_BYTES;
   uint64_t* const full = full_all + warp;
-  const int key = (rank * PAIR_WARPS + warp) * CH, index = key / p.block_size, row = key - index * p.block_size;
+  const int key = (warp * PAIR_BLOCKS + rank) * CH, index = key / p.block_size, row = key - index * p.block_size;
   // loaded beside the length; unused where the chunk is past it
   const int page = index < p.table_width ? __ldg(p.block_tables + (int64_t)seq * p.table_stride + index) : -1;
   int len = __ldg(p.context_lens + seq);
@@ -437,11 +442,13 @@ __global__ void __launch_bounds__(PAIR_WARPS * 32) __cluster_dims__(PAIR_BLOCKS,
   if (valid > 0) {
     const bool came = mbar_wait_bounded(full, 0, VLC_DEV_ERR_TIMEOUT + 24, VLC_WAIT_LIMIT_CYCLES);
     if (__all_sync(0xffffffffu, came)) state.template step<true>(smem_u32(st), p.v_first, valid, r, t);
+    __syncwarp();  // every lane has read the chunk
   }
+  float(*const sm_o)[HD] = reinterpret_cast<float(*)[HD]>(st);
 #pragma unroll
   for (int x = 0; x < NT * 2; ++x) {
     const int nt = x >> 1, odd = x & 1, h = nt * 8 + 2 * t + odd;
-    float4* dst = reinterpret_cast<float4*>(&sm_o[warp][h][16 * r]);
+    float4* dst = reinterpret_cast<float4*>(&sm_o[h][16 * r]);
 #pragma unroll
     for (int mt = 0; mt < 8; mt += 2)
       dst[mt / 2] = make_float4(state.o[nt][mt][odd], state.o[nt][mt][2 + odd], state.o[nt][mt + 1][odd],
@@ -451,15 +458,22 @@ __global__ void __launch_bounds__(PAIR_WARPS * 32) __cluster_dims__(PAIR_BLOCKS,
   cluster_sync();
   const int h = rank * PAIR_WARPS + warp;  // a warp joins a head (at most 16)
   if (h < G) {
+    const uint32_t o_at = smem_u32(first) + (h * HD + 4 * lane) * (uint32_t)sizeof(float);
     Joined sum;
+    auto join = [&](auto rounds) {
 #pragma unroll
-    for (int b = 0; b < PAIR_BLOCKS; ++b)
+      for (int w = 0; w < decltype(rounds)::value; ++w)  // in the order of the chunks
 #pragma unroll
-      for (int w = 0; w < PAIR_WARPS; ++w) {
-        const float2 x = ld_cluster_v2(mapa_shared(smem_u32(&sm_ml[w][h]), b));
-        const float4 v = ld_cluster_v4(mapa_shared(smem_u32(&sm_o[w][h][4 * lane]), b));
-        sum.add(x.x, x.y, v);
-      }
+        for (int b = 0; b < PAIR_BLOCKS; ++b) {
+          const float2 x = ld_cluster_v2(mapa_shared(smem_u32(&sm_ml[w][h]), b));
+          const float4 v = ld_cluster_v4(mapa_shared(o_at + w * STAGE_BYTES, b));
+          sum.add(x.x, x.y, v);
+        }
+    };
+    static_assert(PAIR_WARPS == 4, "the rounds below");
+    if (len <= PAIR_BLOCKS * CH) join(std::integral_constant<int, 1>());
+    else if (len <= 2 * PAIR_BLOCKS * CH) join(std::integral_constant<int, 2>());
+    else join(std::integral_constant<int, 4>());
     reinterpret_cast<uint2*>(p.out + (int64_t)seq * p.out_seq_stride + ((int64_t)head * G + h) * HD)[lane] =
         sum.result(p.v_scale);  // (no key: zeros)
   }
@@ -752,9 +766,9 @@ static int grid_warps(int num_seqs, int num_heads, int num_kv_heads, int max_con
 }
 
 // Whether clusters take whole pairs.  Measured against the line of chunks, us, of 1000 keys (of 200): 28
-// heads of 4, 4 pairs 5.2 : 7.2 (5.2 : 7.5), 64 pairs 7.4 : 9.4 (7.2 : 8.5), 128 pairs 10.7 : 13.8
-// (10.5 : 9.0), 256 pairs 20.4 : 18.8 (16.4 : 10.0).  With over 8 query heads a KV head (32 of 2) a block
-// takes more registers: 64 pairs 9.8 : 13.3 (9.6 : 10.1), 128 pairs 17.8 : 15.7 (17.3 : 11.6).
+// heads of 4, 4 pairs 5.2 : 7.2 (4.2 : 7.1), 64 pairs 7.3 : 9.4 (5.4 : 8.5), 128 pairs 10.4 : 13.8
+// (6.4 : 9.0), 256 pairs 19.9 : 19.0 (11.6 : 10.1).  With over 8 query heads a KV head (32 of 2) a block
+// takes more registers: 64 pairs 10.0 : 13.3 (6.9 : 10.1), 128 pairs 17.3 : 15.8 (13.4 : 11.4).
 static bool whole_pairs(int num_seqs, int num_heads, int num_kv_heads, int max_context_len, int num_sms) {
   const int64_t most = num_heads / num_kv_heads <= 8 ? num_sms : num_sms / 2;
   return max_context_len <= PAIR_KEYS && (int64_t)num_seqs * num_kv_heads <= most;
