@@ -344,6 +344,8 @@ DECODE = [  # H, Hk, block, lens
     (8, 8, 64, [100, 33]),                   # one query head a KV head
     (28, 4, 256, [5000, 40, 2049]),          # several splits
     (4, 4, 128, [20011]),
+    (28, 4, 64, [255, 256, 257, 0, 768, 1023, 1024]),   # whole pairs of 4, 8 and 16 chunks
+    (32, 2, 128, [1024, 256, 3]),
 ]
 
 
