@@ -778,11 +778,6 @@ static int64_t workspace_bytes_for(int64_t warps, int group, int64_t pairs) {
   return warps * 2 * group * (HD + 2) * (int64_t)sizeof(float) + pairs * (int64_t)sizeof(int2);
 }
 
-static bool power_of_two(float g) {
-  int e;
-  return std::isfinite(g) && g > 0.f && std::frexp(g, &e) == 0.5f && e >= -63 && e <= 65;
-}
-
 }  // namespace decode_fp4
 }  // namespace vlc
 
@@ -808,7 +803,7 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   if (head_dim != HD || block_size <= 0 || block_size % CH != 0 || block_size > fp4::MAX_BLOCK) return VLC_ERR_UNSUPPORTED;
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0) return VLC_ERR_SHAPE;
   const int G = num_heads / num_kv_heads;
-  if (G > MAX_GROUP || !power_of_two(k_scale) || !power_of_two(v_scale)) return VLC_ERR_UNSUPPORTED;
+  if (G > MAX_GROUP || !fp4::power_of_two(k_scale) || !fp4::power_of_two(v_scale)) return VLC_ERR_UNSUPPORTED;
   if (num_seqs == 0) return VLC_OK;
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out) return VLC_ERR_NULL;
   if (q_seq_stride % 8 || out_seq_stride % 8 || q_seq_stride < (int64_t)num_heads * HD ||

@@ -13,6 +13,8 @@
 // head is one contiguous piece of codes and one of scales.
 #pragma once
 
+#include <cmath>
+
 #include "common.cuh"
 
 namespace vlc {
@@ -24,6 +26,12 @@ constexpr int CODE_BYTES = HD / 2;
 constexpr int SCALE_BYTES = HD / GROUP;
 constexpr int ROW_BYTES = CODE_BYTES + SCALE_BYTES;
 constexpr int MAX_BLOCK = 1 << 20;  // a head's piece of a page stays within 32-bit offsets
+
+// Whether g may be a cache's power of two: 2^-64 .. 2^64.
+inline bool power_of_two(float g) {
+  int e;
+  return std::isfinite(g) && g > 0.f && std::frexp(g, &e) == 0.5f && e >= -63 && e <= 65;
+}
 
 // Offset of a head's piece of a page, and of a row's codes and scales in it.
 __host__ __device__ __forceinline__ int64_t head_offset(int64_t page, int num_kv_heads, int head, int block_size) {

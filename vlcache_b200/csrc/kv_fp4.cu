@@ -242,11 +242,6 @@ __global__ void __launch_bounds__(256, 4) shift_fp4_kernel(const __grid_constant
 // inv_freq[j] in fp32 as the rotary table's builder has it: 1 / (theta ** (float(2j) / float(128))).
 static float inv_freq_f32(float theta, int j) { return 1.0f / powf(theta, (float)(2 * j) / (float)HD); }
 
-static bool power_of_two(float g) {
-  int e;
-  return std::isfinite(g) && g > 0.f && std::frexp(g, &e) == 0.5f && e >= -63 && e <= 65;
-}
-
 }  // namespace kv_fp4
 }  // namespace vlc
 
@@ -262,7 +257,7 @@ extern "C" int vlc_gather_kvcache_fp4(const void* k_cache, const void* v_cache, 
   if (num_seqs < 0 || total_k < 0 || num_layers < 0 || block_table_width < 0 || num_kv_heads <= 0)
     return VLC_ERR_SHAPE;
   if (head_dim != HD || block_size <= 0 || block_size % TILE != 0 || block_size > fp4::MAX_BLOCK) return VLC_ERR_UNSUPPORTED;
-  if (!power_of_two(k_scale) || !power_of_two(v_scale)) return VLC_ERR_UNSUPPORTED;
+  if (!fp4::power_of_two(k_scale) || !fp4::power_of_two(v_scale)) return VLC_ERR_UNSUPPORTED;
   if (num_seqs == 0 || total_k == 0 || num_layers == 0) return VLC_OK;
   if (!k_cache || !v_cache || !block_tables || !cu_seqlens_k || !k_out || !v_out) return VLC_ERR_NULL;
   if (num_pages <= 0 || num_pages > 0x7fffffff / block_size || num_kv_heads > 65535 || num_layers > 32767)

@@ -367,11 +367,6 @@ static bool set_sections(Params& p, const int32_t* sections, int num_axes) {
   return end == HALF;
 }
 
-static bool power_of_two(float g) {
-  int e;
-  return std::isfinite(g) && g > 0.f && std::frexp(g, &e) == 0.5f && e >= -63 && e <= 65;
-}
-
 template <int SINK, bool ROTATE>
 static int launch(Params& p, cudaStream_t stream) {
   const int heads = (ROTATE ? p.num_heads : 0) + (SINK == kRows ? 1 : 2) * p.num_kv_heads;
@@ -448,7 +443,7 @@ static int cache_args(Params& p, const void* value, int64_t value_stride, void* 
 static int fp4_args(Params& p, int64_t num_pages, int block_size, float k_scale, float v_scale) {
   if (block_size <= 0 || block_size % 64 != 0 || block_size > fp4::MAX_BLOCK) return VLC_ERR_UNSUPPORTED;
   if (num_pages <= 0 || num_pages > 0x7fffffff / block_size) return VLC_ERR_SHAPE;
-  if (!power_of_two(k_scale) || !power_of_two(v_scale)) return VLC_ERR_UNSUPPORTED;
+  if (!fp4::power_of_two(k_scale) || !fp4::power_of_two(v_scale)) return VLC_ERR_UNSUPPORTED;
   p.block_size = block_size;
   p.block_shift = -1;
   for (int s = 6; s < 31; ++s)
