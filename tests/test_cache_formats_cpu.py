@@ -267,3 +267,17 @@ def test_ops_refuse_cpu_tensors(cuda_lib):
                  lambda: ops.remap_block_tables(ints.view(1, 2), ints)):
         with pytest.raises(ValueError):
             call()
+
+
+# ------------------------------------------------------------------ bounds and arguments at their ends
+@pytest.mark.parametrize("seqs,heads,kv_heads", [(64, 28, 4), (200, 16, 2), (100, 32, 2), (1, 16, 2)])
+def test_decode_workspace_of_a_zero_bound(cuda_lib, seqs, heads, kv_heads):
+    """A bound of 0 (every sequence is empty) is a bound of 1 for the size as for the call, and a
+    byte less is refused."""
+    need = cuda_lib.vlc_decode_fp4_workspace_size(seqs, heads, kv_heads, 0)
+    assert need == cuda_lib.vlc_decode_fp4_workspace_size(seqs, heads, kv_heads, 1)
+    assert (need > 0) == (seqs > 1)          # one sequence: clusters take whole pairs, without a workspace
+    if need:
+        stride = heads * 128
+        assert _call(cuda_lib, "vlc_decode_attn_fp4", DECODE4, seqs=seqs, heads=heads, kv_heads=kv_heads, max_len=0,
+                     q_stride=stride, out_stride=stride, ws=P, ws_bytes=need - 1) == WORKSPACE

@@ -871,3 +871,19 @@ def test_projection_into_a_4bit_cache(ops):
             ops.store_kvcache(k_rot, v.contiguous(), other[0, 0], other[1, 0], slots)
         assert torch.equal(out, q_rot) and torch.equal(kv, other)
     ctx.reset_context()
+
+
+# ------------------------------------------------------------------ calls at the ends of their ranges
+@pytest.mark.parametrize("seqs,H,Hk", [(1, 16, 2), (64, 28, 4), (100, 32, 2)])
+def test_decode_fp4_zero_bound(ops, seqs, H, Hk):
+    """All sequences empty and a bound of 0, with fewer and with more pairs than SMs: zeros."""
+    c = torch.full((1, Hk, 64 * 72), 255, dtype=torch.uint8, device="cuda")
+    q = torch.randn(seqs, H, D, generator=_gen(1)).to(torch.bfloat16).cuda()
+    lens = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+    bt = torch.full((seqs, 1), -1, dtype=torch.int32, device="cuda")
+    out = torch.full((seqs, H, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(ops.decode_fp4_workspace_bytes(seqs, H, Hk, 0), dtype=torch.uint8, device="cuda")
+    for w in (None, ws):
+        ops.decode_attention_fp4(q, c, c, bt, lens, 0, SCALE, out=out, workspace=w)
+        assert not bool(out.any())           # (a NaN counts as true)
+        out.fill_(float("nan"))

@@ -774,6 +774,9 @@ static bool whole_pairs(int num_seqs, int num_heads, int num_kv_heads, int max_c
   return max_context_len <= PAIR_KEYS && (int64_t)num_seqs * num_kv_heads <= most;
 }
 
+// A bound of 0 (every sequence empty) runs as a bound of 1: the join writes the zeros.
+static int bound_of(int max_context_len) { return std::max(1, max_context_len); }
+
 static int64_t workspace_bytes_for(int64_t warps, int group, int64_t pairs) {
   return warps * 2 * group * (HD + 2) * (int64_t)sizeof(float) + pairs * (int64_t)sizeof(int2);
 }
@@ -786,6 +789,7 @@ using namespace vlc::decode_fp4;
 
 extern "C" int64_t vlc_decode_fp4_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int max_context_len) {
   if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_context_len < 0) return 0;
+  max_context_len = bound_of(max_context_len);
   const int sms = vlc_num_sms();
   if (whole_pairs(num_seqs, num_heads, num_kv_heads, max_context_len, sms)) return 0;
   return workspace_bytes_for(grid_warps(num_seqs, num_heads, num_kv_heads, max_context_len, sms),
@@ -813,7 +817,7 @@ extern "C" int vlc_decode_attn_fp4(const void* q, int64_t q_seq_stride, int num_
   if (num_pages <= 0 || num_pages > 0x7fffffff / block_size || num_pages * num_kv_heads > 0x7fffffff)
     return VLC_ERR_SHAPE;
   if (num_kv_heads > 65535 || num_seqs > 65535 || num_heads > 65535) return VLC_ERR_SHAPE;
-  if (max_context_len == 0) max_context_len = 1;
+  max_context_len = bound_of(max_context_len);
   const int sms = vlc_num_sms();
   const bool whole = whole_pairs(num_seqs, num_heads, num_kv_heads, max_context_len, sms);
   const int warps = whole ? 0 : grid_warps(num_seqs, num_heads, num_kv_heads, max_context_len, sms);
