@@ -281,3 +281,14 @@ def test_decode_workspace_of_a_zero_bound(cuda_lib, seqs, heads, kv_heads):
         stride = heads * 128
         assert _call(cuda_lib, "vlc_decode_attn_fp4", DECODE4, seqs=seqs, heads=heads, kv_heads=kv_heads, max_len=0,
                      q_stride=stride, out_stride=stride, ws=P, ws_bytes=need - 1) == WORKSPACE
+
+
+def test_get_mrope_takes_a_list():
+    """mrope_section as model configs hold it; the instance is the tuple's."""
+    from vlcache_b200.layers.rotary_embedding import get_mrope
+    rot = get_mrope(128, 128, 16, 1e4, [16, 24, 24])
+    assert rot.mrope_section == (16, 24, 24)
+    assert get_mrope(128, 128, 16, 1e4, (16, 24, 24)) is rot and get_mrope(128, 128, 16, 1e4) is rot
+    assert get_mrope(128, 128, 16, 1e4, [22, 21, 21]).mrope_section == (22, 21, 21)
+    with pytest.raises(ValueError):
+        get_mrope(128, 128, 16, 1e4, [16, 24, 23])

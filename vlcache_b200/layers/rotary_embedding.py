@@ -92,10 +92,16 @@ class MRotaryEmbedding(RotaryEmbedding):
         return ops.mrotary_embedding(positions, query, key, self.cos_sin_cache, self.mrope_section)
 
 
-@lru_cache(1)
 def get_mrope(head_size: int, rotary_dim: int, max_position: int, base: float,
-              mrope_section: tuple[int, ...] = ops.DEFAULT_MROPE_SECTION) -> MRotaryEmbedding:
-    """Shared instance per configuration, as ``get_rope``."""
+              mrope_section=ops.DEFAULT_MROPE_SECTION) -> MRotaryEmbedding:
+    """Shared instance per configuration, as ``get_rope``; ``mrope_section`` is any sequence (a model
+    config holds a list)."""
+    return _mrope_cached(head_size, rotary_dim, max_position, base, tuple(int(x) for x in mrope_section))
+
+
+@lru_cache(1)
+def _mrope_cached(head_size: int, rotary_dim: int, max_position: int, base: float,
+                  mrope_section: tuple[int, ...]) -> MRotaryEmbedding:
     return MRotaryEmbedding(head_size, rotary_dim, max_position, base, mrope_section)
 
 
