@@ -292,3 +292,23 @@ def test_get_mrope_takes_a_list():
     assert get_mrope(128, 128, 16, 1e4, [22, 21, 21]).mrope_section == (22, 21, 21)
     with pytest.raises(ValueError):
         get_mrope(128, 128, 16, 1e4, [16, 24, 23])
+
+
+@pytest.mark.parametrize("shape,swap", [((1, 2, 5, 4, 16), (0, 1)), ((2, 3, 1, 4, 16), None), ((2, 1, 5, 4, 16), None),
+                                        ((2, 5, 1, 4, 16), (1, 2)), ((3, 2, 5, 8), None)])
+def test_page_copies_stay_inside_the_cache(monkeypatch, shape, swap):
+    """The planes and pages that the launch is given tile the cache's own memory, also where a dim
+    of size 1 has a stride that says nothing (one layer of a cache allocated layer first; one page)."""
+    from vlcache_b200 import ops
+    cache = torch.zeros(shape, dtype=torch.bfloat16)
+    if swap:
+        cache = cache.transpose(*swap)
+    assert cache.is_contiguous()
+    calls = []
+    monkeypatch.setattr(ops, "_device", lambda *t: 0)
+    monkeypatch.setattr(ops, "_launch", lambda dev, name, *args: calls.append(args))
+    pages = torch.zeros(1, dtype=torch.int32)
+    ops.copy_kv_pages(cache, pages, pages)
+    base, plane_stride, planes, page_bytes, num_pages = calls[0][:5]
+    assert base == cache.data_ptr() and planes == cache.shape[0] * cache.shape[1] and num_pages == cache.shape[2]
+    assert page_bytes * num_pages == plane_stride and plane_stride * planes == cache.nbytes

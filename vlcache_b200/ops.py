@@ -7,6 +7,7 @@ the CPU are rejected (there is no CPU path in the product).
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 
 import numpy as np
@@ -929,9 +930,10 @@ def copy_kv_pages(kv_cache: torch.Tensor, src_pages: torch.Tensor, dst_pages: to
     for t in (src_pages, dst_pages):
         _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n,
               "src_pages / dst_pages: contiguous int32 of one length")
-    shape, stride, item = kv_cache.shape, kv_cache.stride(), kv_cache.element_size()
-    _launch(dev, "vlc_copy_pages", kv_cache.data_ptr(), stride[1] * item, shape[0] * shape[1], stride[2] * item,
-            shape[2], src_pages.data_ptr(), dst_pages.data_ptr(), n)
+    shape = kv_cache.shape
+    page = math.prod(shape[3:]) * kv_cache.element_size()   # (of a dim of size 1 the stride may be anything)
+    _launch(dev, "vlc_copy_pages", kv_cache.data_ptr(), shape[2] * page, shape[0] * shape[1], page, shape[2],
+            src_pages.data_ptr(), dst_pages.data_ptr(), n)
 
 
 def remap_block_tables(block_tables: torch.Tensor, page_map: torch.Tensor) -> None:
