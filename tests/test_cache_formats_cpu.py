@@ -312,3 +312,16 @@ def test_page_copies_stay_inside_the_cache(monkeypatch, shape, swap):
     base, plane_stride, planes, page_bytes, num_pages = calls[0][:5]
     assert base == cache.data_ptr() and planes == cache.shape[0] * cache.shape[1] and num_pages == cache.shape[2]
     assert page_bytes * num_pages == plane_stride and plane_stride * planes == cache.nbytes
+
+
+def test_remap_of_a_padded_host_table():
+    """Padding stays padding, as ops.remap_block_tables leaves it; other entries outside the pool are refused."""
+    from vlcache_b200.engine.page_pool import PagePool, remap
+    pool = PagePool(6, 4)
+    first, second = pool.allocate(2), pool.allocate(2)
+    pool.free(first)
+    page_map = pool.compact()[2]
+    assert remap(second + [-1, -1], page_map) == [0, 1, -1, -1]
+    for bad in ([6], [-2]):
+        with pytest.raises(ValueError):
+            remap(bad, page_map)

@@ -100,5 +100,8 @@ class PagePool:
 
 
 def remap(block_table: list[int], page_map: np.ndarray) -> list[int]:
-    """A host block table after ``PagePool.compact``."""
-    return [int(page_map[p]) for p in block_table]
+    """A host block table after ``PagePool.compact``; entries of -1 (padding) stay, as on the device."""
+    for p in block_table:
+        if not -1 <= p < len(page_map):
+            raise ValueError(f"page {p} is outside the pool's {len(page_map)}")
+    return [int(page_map[p]) if p >= 0 else -1 for p in block_table]
