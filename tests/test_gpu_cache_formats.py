@@ -887,3 +887,21 @@ def test_decode_fp4_zero_bound(ops, seqs, H, Hk):
         ops.decode_attention_fp4(q, c, c, bt, lens, 0, SCALE, out=out, workspace=w)
         assert not bool(out.any())           # (a NaN counts as true)
         out.fill_(float("nan"))
+
+
+def test_copy_kv_pages_of_a_large_pool(ops):
+    """More pairs than a grid has rows (65535): a compaction of a pool of small pages, bad pairs and
+    padding behind that border among them."""
+    n = 140010
+    cache = torch.randint(0, 256, (2, 2, n, 32), dtype=torch.uint8, generator=_gen(4)).cuda()
+    src = torch.arange(n - 70000, n, dtype=torch.int32, device="cuda")
+    dst = torch.randperm(n - 70000, generator=_gen(5))[:70000].to(torch.int32).cuda()
+    good = torch.ones(70000, dtype=torch.bool, device="cuda")
+    good[69990:69993] = False
+    want = cache.clone()
+    want[:, :, dst[good].long()] = cache[:, :, src[good].long()]
+    src[69990], dst[69991] = n, -3
+    src[69992] = dst[69992] = -1
+    ops.copy_kv_pages(cache, src, dst)
+    assert ops.device_error(reset=True) == 102
+    assert torch.equal(cache, want)
