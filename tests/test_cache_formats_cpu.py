@@ -325,3 +325,21 @@ def test_remap_of_a_padded_host_table():
     for bad in ([6], [-2]):
         with pytest.raises(ValueError):
             remap(bad, page_map)
+
+
+def test_decode_refuses_a_strided_workspace(cuda_lib, monkeypatch):
+    """The parts are written to consecutive bytes: a strided view's lie between another tensor's."""
+    from vlcache_b200 import ops
+    calls = []
+    monkeypatch.setattr(ops, "_device", lambda *t: 0)
+    monkeypatch.setattr(ops, "_launch", lambda dev, name, *args: calls.append(args))
+    q, cache = torch.zeros(3, 4, 128, dtype=torch.bfloat16), torch.zeros(2, 2, 64 * 72, dtype=torch.uint8)
+    ints = torch.zeros(3, dtype=torch.int32)
+    need = ops.decode_fp4_workspace_bytes(3, 4, 2, 5000)
+    call = lambda ws: ops.decode_attention_fp4(q, cache, cache, ints.view(3, 1), ints, 5000, 0.1, workspace=ws)  # noqa: E731
+    whole = torch.zeros(need, 2, dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        call(whole[:, 0])
+    assert not calls
+    call(whole.view(-1)[:need])
+    assert calls[0][-2:] == (whole.data_ptr(), need)

@@ -865,6 +865,7 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     need = lib().vlc_decode_fp4_workspace_size(b, h, hk, max_context_len)
     if need > 0 and (workspace is None or workspace.nbytes < need):
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _need(workspace is None or workspace.is_contiguous(), "workspace: contiguous")
     _launch(dev, "vlc_decode_attn_fp4", q.data_ptr(), qs, b, h, k_cache.data_ptr(), v_cache.data_ptr(), pages, block,
             hk, d, block_tables.data_ptr(), stride, width, context_lens.data_ptr(), max_context_len,
             float(softmax_scale), float(k_scale), float(v_scale), out.data_ptr(), os, _ptr(workspace),
