@@ -442,6 +442,7 @@ __global__ void __launch_bounds__(PAIR_WARPS * 32) __cluster_dims__(PAIR_BLOCKS,
   if (valid > 0) {
     const bool came = mbar_wait_bounded(full, 0, VLC_DEV_ERR_TIMEOUT + 24, VLC_WAIT_LIMIT_CYCLES);
     if (__all_sync(0xffffffffu, came)) state.template step<true>(smem_u32(st), p.v_first, valid, r, t);
+    else mbar_wait_bounded(full, 0, VLC_DEV_ERR_TIMEOUT + 24, VLC_WAIT_LIMIT_CYCLES);  // before O takes its place
     __syncwarp();  // every lane has read the chunk
   }
   float(*const sm_o)[HD] = reinterpret_cast<float(*)[HD]>(st);
@@ -609,8 +610,8 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm(NT)) decode_fp4_kern
   int first_slot = 0;  // the part's slot: 0 for the one that holds the warp's first chunk
 
   for (int i = 0; i < count; ++i) {
-    if (!__all_sync(0xffffffffu, arrived(i))) {  // the copies still in flight are given the same time
-      for (int x = i + 1; x < min(i + STAGES, count); ++x) arrived(x);
+    if (!__all_sync(0xffffffffu, arrived(i))) {  // the copies still in flight, this one's too, are given more time
+      for (int x = i; x < min(i + STAGES, count); ++x) arrived(x);
       return;
     }
     const uint32_t st = ring_u + (i % STAGES) * STAGE_BYTES;
