@@ -905,3 +905,31 @@ def test_copy_kv_pages_of_a_large_pool(ops):
     ops.copy_kv_pages(cache, src, dst)
     assert ops.device_error(reset=True) == 102
     assert torch.equal(cache, want)
+
+
+@pytest.mark.parametrize("H,Hk", [(8, 2), (20, 2)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_decode_fp4_non_finite_query(ops, H, Hk, bad):
+    """A head whose query holds an infinity has scores of +-infinity or NaN only, and a softmax of
+    those is NaN, all of them -infinity included (the keys have one sign where q is infinite).  The
+    other heads keep their bits, and a sequence without keys its zeros."""
+    lens, block = [700, 0, 65], 64
+    r = np.random.default_rng(7)
+    x = -np.abs(r.normal(size=(14, Hk, block, D))) - 0.5
+    kc = torch.from_numpy(fp4.join_pages(*fp4.quantise(x)))
+    vc = _pages(8, 14, Hk, block)
+    bt = torch.arange(14, dtype=torch.int32)
+    bt = torch.stack([bt[:11], torch.full((11,), -1, dtype=torch.int32), torch.cat([bt[11:13], bt[:1].expand(9)])]).cuda()
+    ctx = torch.tensor(lens, dtype=torch.int32).cuda()
+    q = torch.randn(3, H, D, generator=_gen(9)).to(torch.bfloat16).cuda()
+    for bound in (704, 5000):
+        call = lambda x: ops.decode_attention_fp4(x, kc.cuda(), vc.cuda(), bt, ctx, bound, SCALE)  # noqa: E731
+        good, other = call(q), q.clone()
+        other[:, 1, 0], other[:, H - 1, 3] = bad, bad
+        out = call(other)
+        assert not bool(out[1].any())
+        hit = torch.zeros(H, dtype=torch.bool)
+        hit[1] = hit[H - 1] = True
+        for i in (0, 2):
+            assert bool(torch.isnan(out[i, hit]).all())
+            assert bool(torch.isfinite(good[i]).all()) and torch.equal(out[i, ~hit], good[i, ~hit])

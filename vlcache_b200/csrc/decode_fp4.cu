@@ -185,10 +185,13 @@ struct State {
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^(141 - e) for a largest element with exponent field e puts it in [2^14, 2^15); e is kept
-      // where both that power and its inverse are normal.  All-zero and non-finite rows: power 1.
+      // where both that power and its inverse are normal.  All-zero rows: power 1.  A row with an
+      // infinity has scores of +-infinity or NaN only, whose softmax is NaN, also where all of them
+      // are -infinity (which would read as no key): such rows become NaN here.
       int e = (int)(top >> 7);
-      e = (top == 0 || e == 255) ? 141 : max(e, 15);
-      const float up = __uint_as_float((uint32_t)(127 + 141 - e) << 23) * sign;
+      const bool finite = e != 255;
+      e = (top == 0 || !finite) ? 141 : max(e, 15);
+      const float up = finite ? __uint_as_float((uint32_t)(127 + 141 - e) << 23) * sign : __int_as_float(0x7fffffff);
       const float down = __uint_as_float((uint32_t)(127 - 141 + e) << 23);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
