@@ -343,3 +343,21 @@ def test_decode_refuses_a_strided_workspace(cuda_lib, monkeypatch):
     assert not calls
     call(whole.view(-1)[:need])
     assert calls[0][-2:] == (whole.data_ptr(), need)
+
+
+@pytest.mark.parametrize("steps", [2, 3])
+def test_quantising_bears_the_approximate_reciprocal(steps):
+    """The codes with 1 / s off by two and three fp32 steps: the approximate division that makes it
+    is off by two units in the last place at most."""
+    f = np.float32
+    x = (np.arange(0x7f80, dtype=np.uint32) << 16).view(f)
+    grid = f(1.5 * 4096)
+    for s in fp4.E4M3[1:]:
+        y = x[x <= 20 * s]
+        want = fp4.nearest(y.astype(np.float64) / s, fp4.E2M1)
+        for end in (f(0), f(4096)):
+            inv = f(1) / f(s)
+            for _ in range(steps):
+                inv = np.nextafter(inv, end)
+            q = (y.astype(np.float64) * inv + grid).astype(f) - grid
+            assert np.array_equal(fp4.nearest(np.abs(q.astype(np.float64)), fp4.E2M1), want)

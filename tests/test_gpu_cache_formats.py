@@ -933,3 +933,148 @@ def test_decode_fp4_non_finite_query(ops, H, Hk, bad):
         for i in (0, 2):
             assert bool(torch.isnan(out[i, hit]).all())
             assert bool(torch.isfinite(good[i]).all()) and torch.equal(out[i, ~hit], good[i, ~hit])
+
+
+# ------------------------------------------------------------------ every scale and magnitude on the device
+def _sweep_rows(groups):
+    """bf16 rows [n, 1, 128] of groups of 16 (float32 values that bf16 holds), the last row filled up."""
+    flat = np.concatenate(groups).astype(np.float32)
+    flat = np.concatenate([flat, np.zeros(-len(flat) % D, np.float32)])
+    return torch.from_numpy(flat).view(-1, 1, D).to(torch.bfloat16)
+
+
+def _sweep_codes():
+    """For each scale s: groups whose largest element is 6 s (which makes the scale s) and whose others
+    sweep the bf16 magnitudes from 2^-4 s (below, the code is 0) to 6 s, in both signs."""
+    mags = (np.arange(0x7f80, dtype=np.uint32) << 16).view(np.float32)
+    out = []
+    for s in fp4.E4M3[1:]:
+        y = mags[(mags >= s / 16) & (mags <= 6 * s)]
+        y = np.concatenate([y, -y, np.zeros(-2 * len(y) % 15, np.float32)]).reshape(-1, 15)
+        out.append(np.concatenate([np.full((len(y), 1), 6 * s), y], 1).ravel())
+    return _sweep_rows(out)
+
+
+def _sweep_scales():
+    """A group for each bf16 magnitude, as its largest element among smaller ones."""
+    mags = (np.arange(0x7f80, dtype=np.uint32) << 16).view(np.float32)
+    part = (np.arange(16) % 8 / 8.0 * np.where(np.arange(16) < 8, 1, -1)).astype(np.float32)
+    part[0] = 1.0
+    x = torch.from_numpy(mags[:, None] * part[None]).to(torch.bfloat16).float().numpy()
+    return _sweep_rows([x.ravel()])
+
+
+@pytest.mark.parametrize("sweep", [_sweep_codes, _sweep_scales])
+@pytest.mark.parametrize("g", [1.0, 2.0 ** -5])
+def test_store_fp4_over_every_scale_and_magnitude(ops, sweep, g):
+    x = sweep()
+    n, block = x.shape[0], 64
+    rows = (x.float() * g).to(torch.bfloat16)
+    pages = (n + block - 1) // block
+    kc, vc = (torch.zeros(pages, 1, block * 72, dtype=torch.uint8, device="cuda") for _ in "kv")
+    slots = torch.randperm(pages * block, generator=_gen(n))[:n].to(torch.int32)
+    ops.store_kvcache_fp4(rows.cuda(), -rows.cuda(), kc, vc, slots.cuda(), g, g)
+    at = slots.long()
+    for cache, sign in ((kc, 1.0), (vc, -1.0)):
+        codes, scale = (a[at // block, :, at % block] for a in fp4.split_pages(cache.cpu().numpy()))
+        want_codes, want_scale = fp4.quantise(sign * rows.double().numpy(), g)
+        assert np.array_equal(scale, want_scale)
+        zero = (codes & 7 == 0) & (want_codes & 7 == 0)
+        assert bool(((codes == want_codes) | zero).all())
+
+
+# ------------------------------------------------------------------ axes that differ, through the layers
+@pytest.mark.parametrize("fmt", ["bf16", "fp4"])
+def test_attention_layers_at_image_positions(ops, fmt):
+    """A cold prompt with an image, a warm request that reuses the image further on, and a decode
+    step, with (time, height, width) positions that differ between the axes: the cache holds the
+    oracle's rotated rows, and the outputs are those of the attention over what the cache holds.
+    The moved rows are what new rows at their new positions would be: two bf16 roundings of the pair
+    (x1, x2) of radius r before the last turn's own, each 2^-8 of a component, give 2^-8 sqrt(2) r +
+    2 * 2^-8 |z|, and the fp32 angles 2^-16 r."""
+    from vlcache_b200.engine import kv_cache as kvc
+    from vlcache_b200.layers.attention import Attention
+    from vlcache_b200.layers.rotary_embedding import get_mrope, image_position_delta
+    from vlcache_b200.utils import context as ctx
+    H, Hk, gh, gw = 16, 2, 13, 17
+    image = gh * gw
+    g = _gen(71)
+    attn = Attention(H, D, SCALE, Hk)
+    kv = kvc.allocate_kv_cache(torch.nn.ModuleList([attn]), 1, 8, Hk, kv_format=fmt)
+    kv.zero_()
+    rot = get_mrope(D, D, 512, 1e6, [16, 24, 24])
+    table = rot.cos_sin_cache.cpu()
+    rot = rot.cuda()
+
+    def positions(start, tail):     # text, the image from `start` on, text from the image's largest position on
+        return torch.from_numpy(np.concatenate([omr.text_positions(0, start), omr.vision_positions(start, gh, gw),
+                                                omr.text_positions(start + max(gh, gw), tail)], 1))
+
+    def rows(n):
+        return torch.randn(n, H + 2 * Hk, D, generator=g).to(torch.bfloat16).cuda().split((H, Hk, Hk), 1)
+
+    def bf16(bits):
+        return torch.from_numpy(bits.view(np.int16).copy()).view(torch.bfloat16).cuda()
+
+    def held(x):                    # a row as the cache holds it
+        if fmt == "bf16":
+            return x
+        return torch.from_numpy(fp4.values(*fp4.quantise(x.double().cpu().numpy()))).to(torch.bfloat16).cuda()
+
+    def cached(pages, n):
+        if fmt == "fp4":
+            return ops.gather_kvcache_fp4(attn.k_cache, attn.v_cache, torch.tensor([pages], dtype=torch.int32).cuda(),
+                                          torch.tensor([0, n], dtype=torch.int32).cuda(), n)
+        return [c[pages].flatten(0, 1)[:n] for c in (attn.k_cache, attn.v_cache)]
+
+    builder = kvc.WarmPrefillBuilder(H, Hk)
+    # cold: 20 rows of text, the image, 30 rows of text
+    n = 20 + image + 30
+    old = [6, 1]
+    batch = builder.upload(builder.build([kvc.WarmRequest(n, old)]))
+    pos, (q, k, v) = positions(20, 30), rows(n)
+    assert len(set(map(tuple, pos.T.tolist()))) > image and bool((pos[0] != pos[1]).any())
+    o = attn(q, k, v, positions=pos.cuda(), rotary_emb=rot)
+    q_rot, k_rot = (bf16(_axes_reference(x.cpu(), pos, (16, 24, 24), table)) for x in (q, k))
+    assert torch.equal(o, ops.prefill_attention(q_rot, k_rot, v.contiguous(), None, batch.plan, SCALE))
+    for got, want in zip(cached(old, n), (k_rot, v)):
+        assert torch.equal(got, held(want))
+    raw_k, old_k = k, k_rot
+    # warm: the image from row 53 on, 40 of its rows again
+    start, again = 53, 40
+    n, new = start + image + 25, [0, 4]
+    src, dst = kvc.image_reuse_slots(start, start + image, again, new, 20, old)
+    kvc.copy_image_kv(kv, src, dst, image_position_delta(20, start))
+    batch = builder.upload(builder.build([kvc.WarmRequest(n, new, start, start + image, again, True)]))
+    pos = positions(start, 25)
+    fresh = torch.cat([torch.arange(start + again), torch.arange(start + image, n)])
+    q, k, v = rows(len(fresh))
+    o = attn(q, k, v, positions=pos[:, fresh].contiguous().cuda(), rotary_emb=rot)
+    q_rot, k_rot = (bf16(_axes_reference(x.cpu(), pos[:, fresh], (16, 24, 24), table)) for x in (q, k))
+    ck, cv = cached(new, n)
+    for got, want in ((ck, k_rot), (cv, v)):
+        assert torch.equal(got[fresh.cuda()], held(want))
+    both = [torch.cat([x[:start + again], x]) for x in (ck, cv)]
+    assert torch.equal(o, ops.prefill_attention(q_rot, *both, None, batch.plan, SCALE))
+    if fmt == "bf16":
+        mine = slice(start + again, start + image)
+        x = raw_k[20 + again:20 + image].float()
+        z = bf16(_axes_reference(x.to(torch.bfloat16).cpu(), pos[:, mine], (16, 24, 24), table)).float()
+        r = (x ** 2 + omr.rotate_half(x) ** 2).sqrt()
+        bound = 2.0 ** -8 * (math.sqrt(2) * r * 1.01 + 2 * z.abs() * 1.01) + 2.0 ** -16 * r
+        assert bool(((ck[mine].float() - z).abs() <= bound).all())
+        assert not torch.equal(ck[mine], old_k[20 + again:20 + image])
+    # decode: one token further, its axes apart
+    kvc.prepare_decode([n + 1], [new])
+    pos = torch.tensor([[90], [71], [85]])
+    q, k, v = rows(1)
+    o = attn(q, k, v, positions=pos.cuda(), rotary_emb=rot)
+    q_rot, k_rot = (bf16(_axes_reference(x.cpu(), pos, (16, 24, 24), table)) for x in (q, k))
+    ck2, cv2 = cached(new, n + 1)
+    assert torch.equal(ck2[:n], ck) and torch.equal(cv2[:n], cv)
+    assert torch.equal(ck2[n:], held(k_rot)) and torch.equal(cv2[n:], held(v))
+    bt, lens = torch.tensor([new], dtype=torch.int32).cuda(), torch.tensor([n + 1], dtype=torch.int32).cuda()
+    decode = ops.decode_attention_fp4 if fmt == "fp4" else ops.decode_attention
+    assert torch.equal(o[:, 0], decode(q_rot, attn.k_cache, attn.v_cache, bt, lens, ctx.get_context().max_context_len
+                                       or 512, SCALE))
+    ctx.reset_context()
