@@ -1078,3 +1078,166 @@ def test_attention_layers_at_image_positions(ops, fmt):
     assert torch.equal(o[:, 0], decode(q_rot, attn.k_cache, attn.v_cache, bt, lens, ctx.get_context().max_context_len
                                        or 512, SCALE))
     ctx.reset_context()
+
+
+# ------------------------------------------------------------------ forms that the tests above leave out
+@pytest.mark.parametrize("block", [192, 320])
+def test_blocks_that_are_no_power_of_two(ops, block):
+    """Store, read back, attend (both decode kernels and the prefill), move and copy in pages of a
+    multiple of 64 rows that is no power of two."""
+    H, Hk, lens = 12, 3, [700, 1, 383]
+    kc, vc, bt = _paged(81, lens, Hk, block)
+    cu_k = np.concatenate([[0], np.cumsum(lens)])
+    cu = torch.tensor(cu_k, dtype=torch.int32).cuda()
+    q = torch.randn(3, H, D, generator=_gen(1)).to(torch.bfloat16)
+    ctx = torch.tensor(lens, dtype=torch.int32).cuda()
+    dk, dv, dbt = kc.cuda(), vc.cuda(), bt.cuda()
+    for bound in (700, 5000):
+        out = ops.decode_attention_fp4(q.cuda(), dk, dv, dbt, ctx, bound, SCALE)
+        _check_attention(out, q, kc, vc, bt, [1] * 3, lens, SCALE, 1.0, 1.0, 2.0 ** -11)
+    q_lens = [40, 1, 300]
+    plan = ops.build_prefill_plan(np.concatenate([[0], np.cumsum(q_lens)]), cu_k, H, Hk, device="cuda")
+    q = torch.randn(sum(q_lens), H, D, generator=_gen(2)).to(torch.bfloat16)
+    out = ops.prefill_attention_fp4(q.cuda(), dk, dv, dbt, cu, plan, SCALE)
+    _check_attention(out, q, kc, vc, bt, q_lens, lens, SCALE, 1.0, 1.0, 2.0 ** -7)
+    # rows stored over the first sequence's, on both sides of its page borders, then read back
+    rows = torch.randn(300, Hk, D, generator=_gen(3)).to(torch.bfloat16)
+    at = torch.arange(150, 450)
+    slots = (bt[0].long()[at // block] * block + at % block).to(torch.int32)
+    kv = torch.stack([dk, dv]).unsqueeze(1)
+    ops.store_kvcache_fp4(rows.cuda(), rows.cuda(), kv[0, 0], kv[1, 0], slots.cuda())
+    k, v = ops.gather_kvcache_fp4(kv[0, 0], kv[1, 0], dbt, cu, int(cu_k[-1]))
+    want = fp4.values(*fp4.quantise(rows.double().numpy()))
+    assert np.array_equal(k[150:450].double().cpu().numpy(), want) and torch.equal(k[150:450], v[150:450])
+    assert np.array_equal(k[:150].double().cpu().numpy(), fp4.sequence(kc.numpy(), bt[0].tolist(), 150))
+    # moved without a turn to pages of their own, and those pages copied
+    free = [p for p in range(kc.shape[0]) if p not in bt.tolist()[0][:3]][:2]
+    if 2 * block >= 300:
+        to = (torch.tensor(free)[torch.arange(300) // block] * block + torch.arange(300) % block).to(torch.int32)
+        ops.mrope_shift_fp4(kv, slots.cuda(), to.cuda(), (0, 0, 0))
+        moved, _ = ops.gather_kvcache_fp4(kv[0, 0], kv[1, 0], torch.tensor([free], dtype=torch.int32).cuda(),
+                                          torch.tensor([0, 300], dtype=torch.int32).cuda(), 300)
+        assert torch.equal(moved, k[150:450])
+    page = kv[:, :, free[0]].clone()
+    ops.copy_kv_pages(kv, torch.tensor(free[:1], dtype=torch.int32).cuda(), torch.tensor(free[1:], dtype=torch.int32).cuda())
+    assert torch.equal(kv[:, :, free[1]], page)
+
+
+def test_gather_fp4_into_outputs_of_16_byte_alignment(ops):
+    kc, vc, bt = _paged(83, [200, 70], 2, 64)
+    cu = torch.tensor([0, 200, 270], dtype=torch.int32).cuda()
+    want = ops.gather_kvcache_fp4(kc.cuda(), vc.cuda(), bt.cuda(), cu, 270, 2.0, 0.5)
+    for a, b in ((8, 0), (0, 8), (8, 8)):
+        outs = [torch.full((270 * 2 * D + 24,), 7.0, dtype=torch.bfloat16, device="cuda") for _ in "kv"]
+        k, v = outs[0][a:a + 270 * 2 * D].view(270, 2, D), outs[1][b:b + 270 * 2 * D].view(270, 2, D)
+        assert (k.data_ptr() | v.data_ptr()) % 32 == 16
+        ops.gather_kvcache_fp4(kc.cuda(), vc.cuda(), bt.cuda(), cu, 270, 2.0, 0.5, k, v)
+        assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+        assert bool((outs[0][a + 270 * 2 * D:] == 7).all()) and bool((outs[1][b + 270 * 2 * D:] == 7).all())
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "fp4"])
+def test_rotary_of_many_tokens_in_place(ops, fmt):
+    """A prompt's q rotated where it lies, in the projection's rows, is the q of a separate output."""
+    from vlcache_b200.layers.rotary_embedding import rope_cos_sin_cache
+    N, H, Hk = 6011, 28, 4
+    g = _gen(91)
+    table = rope_cos_sin_cache(D, 1024, 1e6).cuda()
+    pos = torch.randint(0, 1024, (3, N), generator=g).cuda()
+    qkv = torch.randn(N, H + 2 * Hk, D, generator=g).to(torch.bfloat16).cuda()
+    slots = torch.randperm(24 * 256, generator=g)[:N].to(torch.int32).cuda()
+    shape, dtype = ((24, 256, Hk, D), torch.bfloat16) if fmt == "bf16" else ((24, Hk, 256 * 72), torch.uint8)
+    caches = [torch.zeros(shape, dtype=dtype, device="cuda") for _ in range(4)]
+    store = ops.mrope_store_kvcache if fmt == "bf16" else ops.rope_store_kvcache_fp4
+    q, k, v = qkv.split((H, Hk, Hk), 1)
+    apart = store(pos, q, k, v, table, *caches[:2], slots, (16, 24, 24))
+    mine = qkv.clone()
+    q, k, v = mine.split((H, Hk, Hk), 1)
+    out = store(pos, q, k, v, table, *caches[2:], slots, (16, 24, 24), out=q)
+    assert out.data_ptr() == mine.data_ptr() and torch.equal(out, apart) and not torch.equal(out, qkv[:, :H])
+    assert torch.equal(mine[:, H:], qkv[:, H:])
+    assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
+@pytest.mark.parametrize("hk", [1, 3])
+def test_shift_fp4_of_k_alone(ops, hk):
+    kv = torch.stack([_pages(93 + x, 4, hk, 64) for x in (0, 1)]).cuda()
+    src = torch.arange(5, 100, dtype=torch.int32).cuda()
+    both, alone = kv.clone(), kv.clone()
+    ops.mrope_shift_layer_fp4(both[0], both[1], src, src + 128, (3, 4, 5))
+    ops.mrope_shift_layer_fp4(alone[0], None, src, src + 128, (3, 4, 5))
+    assert torch.equal(alone[0], both[0]) and torch.equal(alone[1], kv[1]) and not torch.equal(both[1], kv[1])
+
+
+def test_prefill_fp4_without_mask_and_with_idle_sequences(ops):
+    """Every row sees all keys of its sequence; sequences without query rows, and without keys, between others."""
+    H, Hk, q_lens, k_lens = 16, 2, [3, 0, 0, 70, 0], [200, 65, 0, 70, 1]
+    kc, vc, bt = _paged(95, k_lens, Hk, 64)
+    cu_q, cu_k = np.concatenate([[0], np.cumsum(q_lens)]), np.concatenate([[0], np.cumsum(k_lens)])
+    cu = torch.tensor(cu_k, dtype=torch.int32).cuda()
+    q = torch.randn(73, H, D, generator=_gen(6)).to(torch.bfloat16)
+    for causal in (True, False):
+        plan = ops.build_prefill_plan(cu_q, cu_k, H, Hk, device="cuda", causal=causal)
+        out = ops.prefill_attention_fp4(q.cuda(), kc.cuda(), vc.cuda(), bt.cuda(), cu, plan, SCALE)
+        if causal:
+            _check_attention(out, q, kc, vc, bt, q_lens, k_lens, SCALE, 1.0, 1.0, 2.0 ** -7)
+        else:      # each row by itself is the last of its sequence
+            rows = [(i, r) for i, n in enumerate(q_lens) for r in range(n)]
+            for at, (i, _) in enumerate(rows):
+                _check_attention(out[at:at + 1], q[at:at + 1], kc, vc, bt[i:i + 1], [1], [k_lens[i]], SCALE, 1.0, 1.0,
+                                 2.0 ** -7)
+
+
+def test_prefill_fp4_of_no_rows(ops):
+    kc, vc, bt = _paged(97, [65], 2, 64)
+    plan = ops.build_prefill_plan([0, 0], [0, 65], 16, 2, device="cuda")
+    out = ops.prefill_attention_fp4(torch.empty(0, 16, D, dtype=torch.bfloat16, device="cuda"), kc.cuda(), vc.cuda(),
+                                    bt.cuda(), torch.tensor([0, 65], dtype=torch.int32).cuda(), plan, SCALE)
+    assert out.shape == (0, 16, D)
+
+
+def test_a_step_captured_and_replayed(ops):
+    """Rotary and scatter, prefill, decode, move and read-back captured together on a stream of their
+    own, and replayed with other rows, positions and slots, against the same calls made eagerly."""
+    from vlcache_b200.layers.rotary_embedding import rope_cos_sin_cache
+    H, Hk, block, n = 16, 2, 64, 300
+    g = _gen(99)
+    table = rope_cos_sin_cache(D, 512, 1e6).cuda()
+    pos = torch.randint(0, 512, (3, n), generator=g).cuda()
+    qkv = torch.randn(n, H + 2 * Hk, D, generator=g).to(torch.bfloat16).cuda()
+    kv = torch.stack([torch.stack([_pages(101 + x, 12, Hk, block)]) for x in (0, 1)]).cuda()
+    order = torch.randperm(12, generator=g).to(torch.int32)
+    bt, to = order[:5].view(1, 5).cuda(), order[5:10].view(1, 5).cuda()
+    row = torch.arange(n, device="cuda")
+    slots = (bt[0].long()[row // block] * block + row % block).to(torch.int32)
+    away = (to[0].long()[row // block] * block + row % block).to(torch.int32)
+    cu, lens = torch.tensor([0, n], dtype=torch.int32).cuda(), torch.tensor([n], dtype=torch.int32).cuda()
+    plan = ops.build_prefill_plan([0, n], [0, n], H, Hk, device="cuda")
+    ws = torch.empty(ops.prefill_fp4_workspace_bytes(plan, Hk), dtype=torch.uint8, device="cuda")
+    ws2 = torch.empty(ops.decode_fp4_workspace_bytes(1, H, Hk, 5000), dtype=torch.uint8, device="cuda")
+
+    def step(cache):
+        q, k, v = qkv.split((H, Hk, Hk), 1)
+        q = ops.rope_store_kvcache_fp4(pos, q, k, v, table, cache[0, 0], cache[1, 0], slots, (16, 24, 24))
+        a = ops.prefill_attention_fp4(q, cache[0, 0], cache[1, 0], bt, cu, plan, SCALE, workspace=ws)
+        ops.mrope_shift_fp4(cache, slots, away, (7, 3, 5))
+        b = ops.decode_attention_fp4(q[-1:], cache[0, 0], cache[1, 0], to, lens, 5000, SCALE, workspace=ws2)
+        c = ops.decode_attention_fp4(q[-1:], cache[0, 0], cache[1, 0], to, lens, 512, SCALE)
+        return (a, b, c) + ops.gather_kvcache_fp4(cache[0, 0], cache[1, 0], to, cu, n)
+
+    step(kv.clone())
+    mine = kv.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        outs = step(mine)
+    for seed in (1, 2):
+        qkv.copy_(torch.randn(qkv.shape, generator=_gen(seed)))
+        pos.copy_(torch.randint(0, 512, (3, n), generator=_gen(seed)))
+        want_cache = mine.clone()
+        want = step(want_cache)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(mine, want_cache) and all(torch.equal(x, y) for x, y in zip(outs, want))
+    del graph

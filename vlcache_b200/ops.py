@@ -900,6 +900,8 @@ def prefill_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
           "cu_seqlens_k: contiguous int32, the plan's sequences")
     stride, width = _tables(block_tables, seqs)
     out, os = _q_out(q, out)
+    if n == 0 and plan.num_units == 0:
+        return out
     need = prefill_fp4_workspace_bytes(plan, hk)
     if workspace is None or workspace.nbytes < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
