@@ -411,16 +411,17 @@ int vlc_mrope_store_kvcache(const int64_t* positions, int64_t axis_stride, int n
  *   cu_seqlens_k[b] + j of k_out / v_out ([total_k, num_kv_heads, 128] bf16, row stride
  *   out_row_stride elements), for num_layers layers (layer l of the caches at
  *   l * layer_stride bytes, of the outputs at l * out_layer_stride elements).
- *   cu_seqlens_k: device, num_seqs + 1.  Keys of a bad table entry read as 0 and are
- *   recorded (VLC_DEV_ERR_BLOCK_RANGE); rows past total_k are recorded
- *   (VLC_DEV_ERR_LENGTH) and not written.
+ *   cu_seqlens_k: device, num_seqs + 1.  Keys of a bad table entry read as 0, as in the bf16
+ *   prefill (the 4-bit decode leaves them out), and are recorded (VLC_DEV_ERR_BLOCK_RANGE);
+ *   rows past total_k are recorded (VLC_DEV_ERR_LENGTH) and not written.
  * vlc_mrope_shift_fp4: vlc_mrope_shift in such a cache: K rows of src_slots rotated by the
  *   delta, rounded to bf16, quantised again, written to dst_slots (NULL: in place); V rows
  *   copied when dst_slots is given.  A group whose 16 pairs the delta does not turn keeps
  *   its bits.  layer_stride in bytes.
  * vlc_decode_attn_fp4: vlc_decode_attn over such a cache: f16 products of exact K / V
  *   values with q (scaled per head by a power of two) and P, fp32 sums.  Keys of a chunk of
- *   64 whose table entry is bad are left out and recorded.  The workspace, 32-byte aligned,
+ *   64 whose table entry is bad are left out and recorded.  A head whose q holds an infinity or a
+ *   NaN gives NaN, unless its sequence has no key (zeros).  The workspace, 32-byte aligned,
  *   holds the parts of keys split over the grid; calls that may overlap take one each.
  * ------------------------------------------------------------------------ */
 int vlc_rope_store_kvcache_fp4(const int64_t* positions, int64_t axis_stride, int num_axes, const int32_t* sections,

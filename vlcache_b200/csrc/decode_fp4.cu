@@ -3,7 +3,7 @@
 //   o[h] = sum_j softmax_j(scale * g_k * q[h] . K[j]) * g_v * V[j],   K, V = s * code per group.
 //
 // The floor is HBM: 72 bytes per key and head for K and V each.  At that rate an SM has to take in
-// 4 times the keys a second of the bf16 decode, so the work per element counts:
+// 3.6 times the keys a second of the bf16 decode, so the work per element counts:
 //   * K and V are the A operands (16 rows) of m16n8k16 f16 MMAs and the query heads of the KV head
 //     the 8 columns: S^T = K Q^T and O^T = V^T P^T.  A KV head of up to 8 query heads then wastes
 //     no rows, and an MMA consumes 256 cache elements, twice what the transposed products would.
@@ -19,8 +19,7 @@
 // the lengths are (a grid of fixed splits left SMs idle at its end, paid a prologue and a join
 // every few chunks and merged in shared memory: 267 us for 256 sequences of 2700 .. 10700 keys, 28
 // query and 4 KV heads, against 178 us now).  A warp works alone: its own ring of chunks (TMA
-// tiles with the 64-byte swizzle for the codes, plain bulk copies for the scales, issued by its
-// lane 0), its own running maximum and sums, no barrier with any other warp.  A pair that a warp
+// tiles, with the 64-byte swizzle for the codes and without one for the scales, issued by its lane 0), its own running maximum and sums, no barrier with any other warp.  A pair that a warp
 // has to itself is written out; the parts of a pair that several warps share go to the workspace
 // and decode_fp4_combine_kernel, launched as a programmatic dependent, joins them.
 //
