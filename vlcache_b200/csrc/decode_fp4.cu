@@ -19,9 +19,10 @@
 // the lengths are (a grid of fixed splits left SMs idle at its end, paid a prologue and a join
 // every few chunks and merged in shared memory: 267 us for 256 sequences of 2700 .. 10700 keys, 28
 // query and 4 KV heads, against 178 us now).  A warp works alone: its own ring of chunks (TMA
-// tiles, with the 64-byte swizzle for the codes and without one for the scales, issued by its lane 0), its own running maximum and sums, no barrier with any other warp.  A pair that a warp
-// has to itself is written out; the parts of a pair that several warps share go to the workspace
-// and decode_fp4_combine_kernel, launched as a programmatic dependent, joins them.
+// tiles, with the 64-byte swizzle for the codes and without one for the scales, issued by its lane
+// 0), its own running maximum and sums, no barrier with any other warp.  A pair that a warp has to
+// itself is written out; the parts of a pair that several warps share go to the workspace and
+// decode_fp4_combine_kernel, launched as a programmatic dependent, joins them.
 //
 // f16 operands: K and V are exact in f16.  q is scaled per head by a power of two that puts its
 // largest element in [2^14, 2^15), so elements down to 2^-28 of it convert exactly; the power goes

@@ -849,8 +849,9 @@ def decode_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``decode_attention`` over a 4-bit cache: one query token per sequence, q / out [B, H, 128]
     (q may be [B, 1, H, 128]); sequences of length 0 give zeros, a head whose query holds an infinity
-    or a NaN gives NaN.  ``max_context_len`` bounds the lengths on the host and sizes the grid; ``workspace``: ``decode_fp4_workspace_bytes``,
-    32-byte aligned, one per call in flight."""
+    or a NaN gives NaN.  ``max_context_len`` bounds the lengths on the host and sizes the grid;
+    ``workspace``: ``decode_fp4_workspace_bytes``, contiguous and 32-byte aligned, one per call in
+    flight."""
     dev = _device(q, k_cache, v_cache, block_tables, context_lens, out, workspace)
     if q.dim() == 4:
         _need(q.shape[1] == 1, "q: one token per sequence")
