@@ -316,7 +316,7 @@ def _run_step(s):
     nth = (need.flatten().cumsum(0) - 1).view_as(need)
     count = s["num_free"].long()
     got = need & (nth < count)
-    pages = torch.where(got, free[(count - 1 - nth).clamp(min=0)], tables)
+    pages = torch.where(got, free[(count - 1 - nth).clamp(0, free.numel() - 1)], tables)
     count = count - got.sum()
     if c["window"]:
         behind = ((before - c["window"] + 1) // block).view(-1, 1)       # (floor: none where it is negative)
