@@ -45,6 +45,8 @@ extern "C" {
 #define VLC_DEV_ERR_BLOCK_RANGE 102  /* block table entry out of range where a key is needed */
 #define VLC_DEV_ERR_POSITION 103     /* rotary position outside the cos/sin cache */
 #define VLC_DEV_ERR_LENGTH 104       /* a device length exceeds the host-side bound the grid was sized for */
+#define VLC_DEV_ERR_PAGES 105        /* a free list without the pages that are needed (or without room for more) */
+#define VLC_DEV_ERR_TOKEN 106        /* a drafted token past the vocabulary */
 #define VLC_DEV_ERR_TIMEOUT 110      /* an mbarrier wait hit its bound (base; +role id) */
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -464,6 +466,73 @@ int vlc_copy_pages(void* base, int64_t plane_stride, int num_planes, int64_t pag
                    const int32_t* src_pages, const int32_t* dst_pages, int num_pairs, void* stream);
 int vlc_remap_block_tables(int32_t* block_tables, int64_t row_stride, int num_rows, int width,
                            const int32_t* page_map, int num_pages, void* stream);
+
+/* --------------------------------------------------------------------------
+ * A decode step with drafted tokens over a windowed cache.
+ *
+ * The mask of all of them: the row at position t of a sequence sees key j iff j <= t and
+ * (window == 0 or j > t - window or j < sinks).  Pages that no row sees are not read: their
+ * block-table entries may be -1.  A NaN or an infinity in V of a key that one row sees and
+ * another row of its tile does not reaches both (0 * NaN); keys that no row sees may hold anything.
+ *
+ * vlc_attention_plan_window: vlc_attention_plan with that mask (causal plans; capacity and
+ *   workspace as there); vlc_prefill_attn and vlc_prefill_attn_inflight follow the plan, and
+ *   take a positive softmax_scale only.  A window that no sequence outgrows gives the plan
+ *   without one.
+ * vlc_decode_attn_window: the last num_tokens tokens of each sequence (its key and value rows
+ *   are in the cache, context_lens counts them): q / out [num_seqs * num_tokens, num_heads, 128]
+ *   with any token stride, row i num_tokens + r being token context_lens[i] - num_tokens + r of
+ *   sequence i.  At most 128 rows num_tokens * num_heads / num_kv_heads; block_size a multiple of
+ *   16.  Tokens before a sequence's first and sequences of length 0 give zeros, a query row with
+ *   an infinity or a NaN gives NaN.  Keys of a bad page are left out and recorded
+ *   (VLC_DEV_ERR_BLOCK_RANGE), a length past max_context_len is cut to it and recorded
+ *   (VLC_DEV_ERR_LENGTH).  Sizes come from host values, so the launches can be captured; workspace:
+ *   vlc_decode_window_workspace_size bytes, 16-byte aligned, one per call in flight.
+ * vlc_step_metadata: sequence i of context_lens[i] tokens (below 0: an idle place of the batch)
+ *   takes new_lens[i] more.  Block-table entries below 0 where they fall are filled from the end
+ *   of the free list (free_pages[0 .. *num_free), the k-th missing page of the batch being
+ *   free_pages[*num_free - 1 - k], sequences in order), then pages wholly behind the window of
+ *   the first new row and behind the sinks go back to its end, in order, and their entries become
+ *   -1.  Writes positions and slots of the new rows one sequence after another (position 0 and
+ *   slot -1 in the rows behind the last, up to total_rows), their running sums cu_seqlens_q and
+ *   those of the lengths with them cu_seqlens_k (num_seqs + 1 each, below 2^31), and the lengths
+ *   new_context_lens.  Recorded, with slots of -1: pages that the list does not have
+ *   (VLC_DEV_ERR_PAGES), positions past the table (VLC_DEV_ERR_BLOCK_RANGE); with the rows left
+ *   out: more than total_rows (VLC_DEV_ERR_LENGTH).  The tables hold pages of their own: one that
+ *   several tables share would be given back by each.  new_context_lens is no input's memory.
+ * vlc_verify_drafts: draft i of a sequence (drafts[seq][i], -1: none from there on) is accepted iff
+ *   u[i] * draft_probs[i][d] < target_probs[i][d], up to the first refusal; then a token is sampled
+ *   from max(target - draft, 0) at the refused draft, or from the target's row behind the last
+ *   accepted one, at the random number u_last: probability x counts floor(clamp(x, 0, 1) 2^42), and
+ *   the token is the first whose running count passes floor(floor(u_last 2^24) total / 2^24).
+ *   tokens[seq] = accepted drafts, that token, -1 ..; emitted[seq] = accepted drafts + 1.  Without
+ *   draft_probs (NULL) a draft has probability 1, and refused it counts 0.  A difference without a
+ *   positive value is replaced by the target's row; a row without one gives token -1.  target_probs
+ *   [num_seqs][num_drafts + 1][vocab], draft_probs [num_seqs][num_drafts][vocab], strides in
+ *   elements, dtype 0 fp32, 1 bf16, 2 fp16; at most 31 drafts and 2^18 tokens.  A draft past the
+ *   vocabulary is recorded (VLC_DEV_ERR_TOKEN) and ends the drafts.
+ * ------------------------------------------------------------------------ */
+int vlc_attention_plan_window(const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int num_seqs, int num_heads,
+                              int num_kv_heads, int head_dim, int causal, int window, int sinks, int num_sms,
+                              int32_t* plan_out, int64_t plan_capacity, int64_t* plan_len);
+int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int num_seqs, int num_tokens, int num_heads,
+                           const void* k_cache, const void* v_cache, int64_t num_pages, int block_size,
+                           int num_kv_heads, int head_dim, const int32_t* block_tables, int64_t block_table_stride,
+                           int block_table_width, const int32_t* context_lens, int max_context_len, int window,
+                           int sinks, float softmax_scale, void* out, int64_t out_token_stride, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+int64_t vlc_decode_window_workspace_size(int num_seqs, int num_tokens, int num_heads, int num_kv_heads,
+                                         int max_context_len, int window, int sinks);
+int vlc_step_metadata(const int32_t* context_lens, const int32_t* new_lens, int num_seqs, int32_t* block_tables,
+                      int64_t block_table_stride, int block_table_width, int block_size, int window, int sinks,
+                      int32_t* free_pages, int free_capacity, int32_t* num_free, int64_t* positions,
+                      int32_t* slot_mapping, int total_rows, int32_t* cu_seqlens_q, int32_t* cu_seqlens_k,
+                      int32_t* new_context_lens, void* stream);
+int vlc_verify_drafts(const int64_t* drafts, int64_t draft_stride, int num_seqs, int num_drafts,
+                      const void* target_probs, int64_t target_seq_stride, int64_t target_row_stride,
+                      const void* draft_probs, int64_t draft_seq_stride, int64_t draft_row_stride, int vocab, int dtype,
+                      const float* u, int64_t u_stride, const float* u_last, int64_t* tokens, int32_t* emitted,
+                      void* stream);
 
 #ifdef __cplusplus
 }

@@ -79,6 +79,16 @@ SIGNATURES: dict[str, tuple] = {
     "vlc_decode_fp4_workspace_size": (c_i64, [c_int, c_int, c_int, c_int]),
     "vlc_copy_pages": (c_int, [c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_int, c_vp]),
     "vlc_remap_block_tables": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_int, c_vp]),
+    "vlc_attention_plan_window": (c_int, [c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp,
+                                          c_i64, c_vp]),
+    "vlc_decode_attn_window": (c_int, [c_vp, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_vp,
+                                       c_i64, c_int, c_vp, c_int, c_int, c_int, c_float, c_vp, c_i64, c_vp, c_i64,
+                                       c_vp]),
+    "vlc_decode_window_workspace_size": (c_i64, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "vlc_step_metadata": (c_int, [c_vp, c_vp, c_int, c_vp, c_i64, c_int, c_int, c_int, c_int, c_vp, c_int, c_vp, c_vp,
+                                  c_vp, c_int, c_vp, c_vp, c_vp, c_vp]),
+    "vlc_verify_drafts": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_int,
+                                  c_vp, c_i64, c_vp, c_vp, c_vp, c_vp]),
 }
 
 

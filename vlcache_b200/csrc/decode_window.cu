@@ -1,0 +1,724 @@
+// Paged decode attention of the last 1 .. n tokens of each sequence, with a sliding window and first
+// tokens (sinks) that stay visible, sm_100a.
+//
+//   Row r of a sequence's n has position t = len - n + r and sees key j iff j <= t and
+//   (window == 0 or j > t - window or j < sinks):   o = sum_j softmax_j(scale * q . K[j]) * V[j].
+//
+// The floor is HBM: 512 bytes a key and KV head, each key that any of the n rows sees read once.  So
+// the n tokens of a sequence and the G query heads of a KV head are the rows of one product, and a key
+// goes through shared memory once for all of them:
+//   * K and V are the A operands (16 rows) of m16n8k16 bf16 MMAs, the query rows (token-major, G heads
+//     each) the 8 columns: S^T = K Q^T and O^T = V^T P^T.  A tile of 8 rows wastes at most 7, where a
+//     tile of 16 would waste half of one token's 7 or 8 heads.
+//   * P^T in the layout of a B operand is S^T's accumulator transposed: one movmatrix an 8 x 8 tile.
+//   * The keys that a sequence sees are chunks of 16: those of the sinks, then those from the window's
+//     first on; what lies between is skipped, its pages are not touched.
+// The chunks of all (sequence, KV head) pairs form one line that the grid's teams share out evenly,
+// each a contiguous run of it, so that the shares are equal whatever the lengths are.  A team is one
+// warp for up to 32 rows and two or four for more (a warp's accumulators are 32 registers a tile of 8
+// rows); it has its own ring of chunks, one TMA copy each (K and V together), and no barrier with
+// other teams.  A pair that a team has to itself is written out; the parts of a pair that several
+// teams share go to the workspace, and window_join_kernel, a programmatic dependent, joins them.
+//
+// P is rounded to bf16, V's type, as an operand of its MMA has to be (by 2^-8 of itself at most); its sum
+// is taken over the rounded values, so that the error does not add up with the keys.  Scores, maxima
+// and sums are fp32.
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+#include "runtime.h"
+
+namespace vlc {
+namespace decode_window {
+
+constexpr int HD = 128;
+constexpr int CK = 16;                  // keys of a chunk
+constexpr int HALF_BYTES = CK * 128;    // 64 dims of the keys
+constexpr int TILE_BYTES = 2 * HALF_BYTES;
+constexpr int STAGE_BYTES = 2 * TILE_BYTES;  // K and V
+constexpr int WARPS = 4;                // of a block
+constexpr int RING_STAGES = 3 * WARPS;  // of a block, shared out among its teams
+constexpr int SMEM_BYTES = RING_STAGES * STAGE_BYTES + 1024;  // + alignment to the swizzle's period
+constexpr int BLOCKS_PER_SM = 2;
+constexpr int MAX_ROWS = 128;           // tokens x query heads of a KV head
+constexpr float SLACK = 8.f;            // log2 that the maximum may grow by before O is rescaled
+
+struct Params {
+  // {64 dims, Hk, slots, 2 halves of a row, caches}, box {64, 1, CK, 2, caches}.  Joined, the caches are
+  // the two, whose stride is their distance (v_first: V lies before K); else kv[0] is K and kv[1] V.
+  CUtensorMap kv[2];
+  bool joined, v_first;
+  const __nv_bfloat16* q;
+  int64_t q_token_stride;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  int table_width, block_size, num_pages;
+  const int32_t* context_lens;
+  int num_seqs, max_len, tokens, window, sinks;
+  int group, num_kv_heads, rows;  // rows = tokens * group
+  float scale_log2;               // |softmax scale| * log2(e)
+  uint32_t q_flip;                // the signs of a pair of q's elements where the scale is negative
+  __nv_bfloat16* out;
+  int64_t out_token_stride;
+  int num_teams;
+  // Workspace: a team's first pair and its last leave parts when they are not whole.
+  float* parts;     // [num_teams][2][rows][HD] sums of P V
+  float2* part_ml;  // [num_teams][2][rows] (maximum, sum of P)
+  int2* places;     // [num_seqs][num_kv_heads] of each pair with keys: (slot of its first part, parts)
+};
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// The chunks of a sequence that any of its rows sees: chunk v is v for v < first (of the sinks), and
+// v + jump from there on.
+struct Span {
+  int len;          // cut to the host's bound
+  int low;          // first key of the window of the sequence's first row
+  int first, jump;
+  int count;
+};
+__device__ __forceinline__ Span span_of(const Params& p, int len) {
+  Span s;
+  s.len = min(max(len, 0), p.max_len);
+  s.low = p.window > 0 ? max(0, s.len - p.tokens - p.window + 1) : 0;
+  const int wc = s.low / CK;
+  s.first = min(wc, (p.sinks + CK - 1) / CK);
+  s.jump = wc - s.first;
+  s.count = (s.len + CK - 1) / CK - s.jump;
+  return s;
+}
+
+// How the line of `total` chunks is shared: every team takes each() of them and the first extra()
+// one more.
+struct Shares {
+  int64_t each, extra;
+  __device__ __forceinline__ Shares(int64_t total, int teams) : each(total / teams), extra(total % teams) {}
+  __device__ __forceinline__ int64_t first(int64_t team) const { return team * each + min(team, extra); }
+  __device__ __forceinline__ int64_t count(int64_t team) const { return each + (team < extra ? 1 : 0); }
+  __device__ __forceinline__ int64_t team_of(int64_t chunk) const {
+    const int64_t big = extra * (each + 1);
+    return chunk < big ? chunk / (each + 1) : extra + (chunk - big) / each;
+  }
+};
+
+// A warp's rows: S^T, O^T and the softmax, and the step over one chunk.  Lane (r, t) = (lane / 4,
+// lane % 4) holds keys r and r + 8 of a chunk, dims 8c + r, and rows 2t and 2t + 1 of each tile.
+template <int NT>  // tiles of 8 rows
+struct State {
+  uint32_t qb[NT][8][2];  // Q as B fragments: dims 16k + 2t, + 1 (and 8 more) of row r
+  float o[NT][8][4];      // m-tile i: dims 16i + r of rows 2t, 2t + 1 (0, 1), dims 16i + 8 + r (2, 3)
+  float l[NT][4];         // sums of P: 0 and 1 of rows 2t, 2t + 1
+  float m[NT][2];         // the maximum that P is relative to
+  float shift[NT][2];     // -m (0 before the first key)
+
+  // Rows row0 .. of the pair, row x being token x / G's head x % G.
+  __device__ __forceinline__ void start(const Params& p, int seq, int head, int row0, int r, int t) {
+    const int G = p.group;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = row0 + n * 8 + r;
+      const int tok = row / G;
+      const bool live = row < p.rows;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(
+          p.q + ((int64_t)seq * p.tokens + (live ? tok : 0)) * p.q_token_stride +
+          ((int64_t)head * G + (live ? row - tok * G : 0)) * HD) + t;
+      uint32_t top = 0;  // largest bf16 magnitude
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t u = live ? __ldg(src + 8 * k + 4 * x) ^ p.q_flip : 0u;
+          qb[n][k][x] = u;
+          top = max(top, max(u & 0x7fffu, (u >> 16) & 0x7fffu));
+        }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // A row with an infinity has scores of +-infinity or NaN only, whose softmax is NaN, also where
+      // all of them are -infinity (which would read as no key): such rows become NaN here.
+      if (top >= 0x7f80u) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) qb[n][k][0] = qb[n][k][1] = 0x7fff7fffu;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      l[n][0] = l[n][1] = l[n][2] = l[n][3] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
+      shift[n][0] = shift[n][1] = 0.f;
+    }
+  }
+
+  // One chunk whose K and V tiles are at kt and vt.  CUT: key0 is its first key, and not every row
+  // sees all of it (`valid` 0: none of it counts).
+  template <bool CUT>
+  __device__ __forceinline__ void step(const Params& p, uint32_t kt, uint32_t vt, int key0, int valid, const Span& span,
+                                       int row0, int lane) {
+    const int r = lane >> 2, t = lane & 3, mi = lane >> 3, ri = lane & 7;
+    // ---- S^T = K Q^T
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    {
+      float s2[4] = {0.f, 0.f, 0.f, 0.f};  // one tile alone: two chains of MMAs
+      const uint32_t at = kt + ((mi & 1) * 8 + ri) * 128;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t a[4];
+        ldsm_x4(at + (k >> 2) * HALF_BYTES + ((((2 * k) & 7) + (mi >> 1) ^ ri) << 4), a);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_bf16(NT == 1 && (k & 1) ? s2 : s[n], a, qb[n][k][0], qb[n][k][1]);
+      }
+      if (NT == 1) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[0][x] += s2[x];
+      }
+    }
+    // ---- running softmax, log2 domain
+    uint32_t pb[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float(&x)[4] = s[n];
+      bool hide[4];
+      if (CUT) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + r + (e >> 1) * 8;
+          const int pos = span.len - p.tokens + (row0 + n * 8 + 2 * t + (e & 1)) / p.group;
+          hide[e] = valid == 0 || key > pos || (p.window > 0 && key <= pos - p.window && key >= p.sinks);
+          if (hide[e]) x[e] = -INFINITY;
+        }
+      }
+      const float top0 = fmaxf(x[0], x[2]) * p.scale_log2, top1 = fmaxf(x[1], x[3]) * p.scale_log2;
+      // The lanes' own maxima tell whether any grew past the slack; only then are they joined.
+      if (__any_sync(0xffffffffu, top0 > m[n][0] + SLACK || top1 > m[n][1] + SLACK)) {
+        float m0 = top0, m1 = top1;
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, d));
+          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, d));
+        }
+        m0 = fmaxf(m[n][0], m0);
+        m1 = fmaxf(m[n][1], m1);
+        const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m[n][0] - m0);  // (-inf: no key so far)
+        const float f1 = m1 == -INFINITY ? 0.f : fast_exp2(m[n][1] - m1);
+        m[n][0] = m0;
+        m[n][1] = m1;
+        shift[n][0] = m0 == -INFINITY ? 0.f : -m0;
+        shift[n][1] = m1 == -INFINITY ? 0.f : -m1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          o[n][i][0] *= f0;
+          o[n][i][1] *= f1;
+          o[n][i][2] *= f0;
+          o[n][i][3] *= f1;
+        }
+        l[n][0] *= f0;
+        l[n][1] *= f1;
+      }
+      x[0] = fast_exp2(fmaf(x[0], p.scale_log2, shift[n][0]));
+      x[1] = fast_exp2(fmaf(x[1], p.scale_log2, shift[n][1]));
+      x[2] = fast_exp2(fmaf(x[2], p.scale_log2, shift[n][0]));
+      x[3] = fast_exp2(fmaf(x[3], p.scale_log2, shift[n][1]));
+      if (CUT) {  // (not left to exp2(-inf): a scale of 0 would make it exp2(NaN))
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (hide[e]) x[e] = 0.f;
+      }
+      pb[n][0] = transpose8x8(pack_bf16x2(x[0], x[1]));
+      pb[n][1] = transpose8x8(pack_bf16x2(x[2], x[3]));
+    }
+    // ---- O^T += V^T P^T
+    const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mma_bf16(l[n], ones, pb[n][0], pb[n][1]);
+    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};  // of a lane's keys 2t, 2t + 1 (and 8 more)
+    if (CUT) {  // V rows that no row of the sequence sees may hold anything: their P is 0, and so is V then
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = key0 + 2 * t + (e & 1) + (e >> 1) * 8;
+        if (valid == 0 || key >= span.len || (key < span.low && key >= p.sinks))
+          keep[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+      }
+    }
+    const uint32_t at = vt + ((mi >> 1) * 8 + ri) * 128;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t a[4];
+      ldsm_x4_t(at + (i >> 2) * HALF_BYTES + ((((2 * i) & 7) + (mi & 1) ^ ri) << 4), a);
+      if (CUT) {
+        a[0] &= keep[0];
+        a[1] &= keep[0];
+        a[2] &= keep[1];
+        a[3] &= keep[1];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_bf16(o[n][i], a, pb[n][0], pb[n][1]);
+    }
+  }
+};
+
+// Grid: blocks of WARPS warps, WARPS / TEAM teams each; the warps of a team share its ring and its run
+// of the line, each with NT tiles of the pair's rows.
+template <int NT, int TEAM>
+__global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kernel(const __grid_constant__ Params p) {
+  constexpr int TEAMS = WARPS / TEAM, STAGES = RING_STAGES / TEAMS;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_all[RING_STAGES], empty_all[RING_STAGES];
+  __shared__ int valid_all[RING_STAGES];
+  pdl_launch_dependents();  // the join waits for this grid's end before it reads
+  const int warp = warp_id(), lane = lane_id();
+  const int r = lane >> 2, t = lane & 3;
+  const int G = p.group, Hk = p.num_kv_heads;
+  const int team = warp / TEAM, mate = warp % TEAM;
+  const int row0 = mate * NT * 8;
+  const int64_t my = (int64_t)blockIdx.x * TEAMS + team;
+  uint64_t* const full = full_all + team * STAGES;
+  uint64_t* const empty = empty_all + team * STAGES;
+  volatile int* const valid_of = valid_all + team * STAGES;
+  if (threadIdx.x < RING_STAGES) {
+    mbar_init(full_all + threadIdx.x, 1);
+    mbar_init(empty_all + threadIdx.x, TEAM);
+    fence_mbar_init();
+  }
+  __syncthreads();
+
+  // ---- this team's run [c0, c0 + count) of the line, and the sequence that c0 lies in
+  int64_t total = 0;
+  for (int i = lane; i < p.num_seqs; i += 32) {
+    const int len = __ldg(p.context_lens + i);
+    if (my == 0 && mate == 0 && len > p.max_len) record_error(VLC_DEV_ERR_LENGTH);
+    total += span_of(p, len).count;
+  }
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+  total *= Hk;
+  const Shares shares(total, p.num_teams);
+  const int64_t c0 = shares.first(my);
+  const int count = (int)shares.count(my);
+  if (my >= p.num_teams || count == 0) return;
+  int seq = 0;
+  int64_t at = c0;  // c0's place among the chunks from the sequence's first on
+  for (int base = 0;; base += 32) {
+    int64_t n = base + lane < p.num_seqs ? (int64_t)span_of(p, __ldg(p.context_lens + base + lane)).count * Hk : 0;
+    int64_t upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, upto > at);
+    if (past) {
+      const int first = __ffs(past) - 1;
+      seq = base + first;
+      at -= __shfl_sync(0xffffffffu, upto - n, first);
+      break;
+    }
+    at -= __shfl_sync(0xffffffffu, upto, 31);
+    if (base + 32 >= p.num_seqs) return;  // not reached: c0 < total
+  }
+  Span span = span_of(p, __ldg(p.context_lens + seq));
+  int head = (int)(at / span.count), j = (int)(at - (int64_t)head * span.count);
+
+  uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023)) +
+                        team * (STAGES * STAGE_BYTES);
+
+  // ---- the issuing side (lane 0 of the team's first warp): a cursor of its own
+  Span ahead = span;
+  int a_seq = seq, a_head = head, a_j = j, a_index = -1, a_page = -1, issued = 0;
+  auto issue = [&]() {  // chunk `issued` of the run
+    const int stage = issued % STAGES;
+    uint64_t* bar = full + stage;
+    const int key = (a_j < ahead.first ? a_j : a_j + ahead.jump) * CK;
+    const int index = key / p.block_size;
+    if (index != a_index) {
+      a_index = index;
+      a_page = index < p.table_width ? __ldg(p.block_tables + a_seq * p.table_stride + index) : -1;
+    }
+    if ((uint32_t)a_page < (uint32_t)p.num_pages) {
+      const int slot = a_page * p.block_size + (key - index * p.block_size);
+      uint8_t* st = ring + stage * STAGE_BYTES;
+      valid_of[stage] = 1;
+      mbar_expect_tx(bar, STAGE_BYTES);
+      tma_load_5d(st, &p.kv[0], bar, 0, a_head, slot, 0, 0);
+      if (!p.joined) tma_load_5d(st + TILE_BYTES, &p.kv[1], bar, 0, a_head, slot, 0, 0);
+    } else {  // the table has no usable page there: recorded, and none of the chunk's keys counts
+      valid_of[stage] = 0;
+      record_error(VLC_DEV_ERR_BLOCK_RANGE);
+      mbar_arrive(bar);
+    }
+    if (++issued == count || ++a_j < ahead.count) return;
+    a_j = 0;
+    a_index = -1;
+    if (++a_head < Hk) return;
+    a_head = 0;
+    do {
+      ahead = span_of(p, __ldg(p.context_lens + ++a_seq));  // a chunk follows: so does a sequence with keys
+    } while (ahead.count <= 0);
+  };
+  const bool issuer = mate == 0 && lane == 0;
+  // (team warps go on at their own pace: a stage is filled again one chunk late, when they are surely done)
+  constexpr int LAG = TEAM > 1 ? 1 : 0;
+  if (issuer) {
+    for (int i = 0; i < min(STAGES, count); ++i) issue();
+  }
+  // Whether chunk i came (recorded where it did not).
+  auto arrived = [&](int i) {
+    const uint32_t parity = (uint32_t)(i / STAGES) & 1u;
+    if (mbar_try_wait(full + i % STAGES, parity)) return true;
+    return mbar_wait_bounded(full + i % STAGES, parity, VLC_DEV_ERR_TIMEOUT + 26, VLC_WAIT_LIMIT_CYCLES);
+  };
+  // Copies still in flight are given more time before the block may end.
+  auto leave = [&](int i) {
+    if (issuer) {
+      for (int x = i; x < issued; ++x) arrived(x);
+    }
+  };
+
+  const uint32_t ring_u = smem_u32(ring);
+  State<NT> state;
+  state.start(p, seq, head, row0, r, t);
+  // The team with a pair's first chunk notes where its parts will be: one for each team up to that of
+  // its last chunk, in slot 0 but for this team's.
+  auto note = [&](int64_t chunk, int slot) {
+    if (issuer)
+      p.places[(int64_t)seq * Hk + head] =
+          make_int2((int)my * 2 + slot, (int)(shares.team_of(chunk + span.count - 1) - my) + 1);
+  };
+  if (j == 0) note(c0, 0);
+  int begin = j;       // first chunk of the pair that is in the state
+  int first_slot = 0;  // the part's slot: 0 for the one that holds the team's first chunk
+
+  for (int i = 0; i < count; ++i) {
+    if (!__all_sync(0xffffffffu, arrived(i))) {
+      leave(i);
+      return;
+    }
+    const int stage = i % STAGES;
+    const uint32_t st = ring_u + stage * STAGE_BYTES;
+    const uint32_t kt = st + (p.v_first ? TILE_BYTES : 0), vt = st + (p.v_first ? 0 : TILE_BYTES);
+    const int valid = valid_of[stage];
+    const int key0 = (j < span.first ? j : j + span.jump) * CK;
+    // Every row sees a chunk that ends by the first row's position and begins in the last row's window
+    // (or ends among the sinks).
+    const bool whole_chunk = valid && key0 + CK - 1 <= span.len - p.tokens &&
+                             (p.window == 0 || key0 >= span.len - p.window || key0 + CK <= p.sinks);
+    if (whole_chunk) state.template step<false>(p, kt, vt, key0, valid, span, row0, lane);
+    else state.template step<true>(p, kt, vt, key0, valid, span, row0, lane);
+    __syncwarp();  // every lane has read the stage
+    if (TEAM > 1) {
+      if (lane == 0) mbar_arrive(empty + stage);
+      bool ok = true;
+      if (issuer && i >= LAG && issued < count) {
+        const int x = i - LAG;  // chunk whose stage is filled again
+        ok = mbar_wait_bounded(empty + x % STAGES, (uint32_t)(x / STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 27,
+                               VLC_WAIT_LIMIT_CYCLES);
+        if (ok) issue();
+      }
+      if (!__all_sync(0xffffffffu, ok)) {
+        leave(i + 1);
+        return;
+      }
+    } else if (issuer && issued < count) {
+      issue();
+    }
+    if (++j < span.count && i + 1 < count) continue;
+
+    // ---- the pair ends, or the run does
+    const bool whole = begin == 0 && j == span.count;
+    float* const part_o = p.parts + (my * 2 + first_slot) * p.rows * HD;
+    float2* const part_ml = p.part_ml + (my * 2 + first_slot) * p.rows;
+#pragma unroll
+    for (int x = 0; x < NT * 2; ++x) {
+      const int n = x >> 1, odd = x & 1;
+      const int row = row0 + n * 8 + 2 * t + odd;
+      if (row >= p.rows) continue;
+      const float sum = state.l[n][odd];
+      if (whole) {
+        const int tok = row / G;
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;  // (NaN stays NaN)
+        __nv_bfloat16* dst = p.out + ((int64_t)seq * p.tokens + tok) * p.out_token_stride +
+                             ((int64_t)head * G + row - tok * G) * HD + r;
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {
+          dst[16 * mt] = __float2bfloat16(state.o[n][mt][odd] * inv);
+          dst[16 * mt + 8] = __float2bfloat16(state.o[n][mt][2 + odd] * inv);
+        }
+      } else {
+        float* dst = part_o + (int64_t)row * HD + r;
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {  // (eight lanes write a sector)
+          dst[16 * mt] = state.o[n][mt][odd];
+          dst[16 * mt + 8] = state.o[n][mt][2 + odd];
+        }
+        if (r == 0) part_ml[row] = make_float2(state.m[n][odd], sum);
+      }
+    }
+    if (i + 1 == count) break;
+    j = begin = 0;
+    first_slot = 1;
+    if (++head == Hk) {
+      head = 0;
+      do {
+        span = span_of(p, __ldg(p.context_lens + ++seq));
+      } while (span.count <= 0);
+    }
+    note(c0 + i + 1, 1);
+    state.start(p, seq, head, row0, r, t);
+  }
+}
+
+// A running (maximum, sum of P, four dims of O) and its union with another part's.
+struct Joined {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float m2, float l2, const float4& o2) {
+    const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.f : top;
+    const float f = fast_exp2(m - ref), g = fast_exp2(m2 - ref);
+    m = top;
+    l = l * f + l2 * g;
+    o = make_float4(o.x * f + o2.x * g, o.y * f + o2.y * g, o.z * f + o2.z * g, o.w * f + o2.w * g);
+  }
+  __device__ __forceinline__ uint2 result() const {
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    return make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  }
+};
+
+// Joins the parts of the pairs that several teams shared and writes zeros for empty sequences.  Grid
+// (pair, rows).  SPREAD: a block takes one row, its eight warps the row's parts in turn; else eight
+// rows, a warp each, which loads eight parts at once.
+template <bool SPREAD>
+__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ Params p) {
+  constexpr int PARTS = 8;
+  __shared__ float4 s_o[8][32];
+  __shared__ float2 s_ml[8];
+  const int pair = blockIdx.x, warp = warp_id(), lane = lane_id();
+  const int seq = pair / p.num_kv_heads, head = pair - seq * p.num_kv_heads;
+  const int row = SPREAD ? blockIdx.y : blockIdx.y * 8 + warp;
+  const bool empty = __ldg(p.context_lens + seq) <= 0;
+  // Every block waits, those with nothing to join too: what follows in the stream may rely on this
+  // grid's end for the decode kernel's.
+  pdl_wait();
+  if (row >= p.rows) return;
+  int2 place = make_int2(0, 0);
+  if (!empty) place = p.places[pair];
+  // A team that gave up waiting for its copies (recorded) leaves pairs unnoted: nothing is read for them.
+  if ((uint32_t)place.x >= 2u * p.num_teams || (uint32_t)place.y > (uint32_t)(p.num_teams - (place.x >> 1)))
+    place = make_int2(0, 1);
+  const int count = place.y;
+  if (count == 1) return;  // written by its team
+  const int tok = row / p.group;
+  uint2* const dst = reinterpret_cast<uint2*>(p.out + ((int64_t)seq * p.tokens + tok) * p.out_token_stride +
+                                              ((int64_t)head * p.group + row - tok * p.group) * HD) + lane;
+  // part i > 0 is in slot 0 of the team i after the first's
+  const int64_t first = (int64_t)place.x * p.rows + row, rest = (int64_t)(place.x & ~1) * p.rows + row;
+  const float4* const po = reinterpret_cast<const float4*>(p.parts) + lane;
+  Joined sum;
+  if constexpr (SPREAD) {
+#pragma unroll 4
+    for (int i = warp; i < count; i += 8) {
+      const int64_t s = i == 0 ? first : rest + (int64_t)i * 2 * p.rows;
+      const float2 x = p.part_ml[s];
+      const float4 v = po[s * (HD / 4)];
+      sum.add(x.x, x.y, v);
+    }
+    s_o[warp][lane] = sum.o;
+    if (lane == 0) s_ml[warp] = make_float2(sum.m, sum.l);
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) sum.add(s_ml[w].x, s_ml[w].y, s_o[w][lane]);
+    *dst = sum.result();  // (0 parts: zeros)
+  } else {
+    for (int i0 = 0; i0 < count; i0 += PARTS) {
+      float2 x[PARTS];
+      float4 v[PARTS];
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        if (i0 + i >= count) continue;
+        const int64_t s = i0 + i == 0 ? first : rest + (int64_t)(i0 + i) * 2 * p.rows;
+        x[i] = p.part_ml[s];
+        v[i] = po[s * (HD / 4)];
+      }
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i)
+        if (i0 + i < count) sum.add(x[i].x, x[i].y, v[i]);
+    }
+    *dst = sum.result();
+  }
+}
+
+// Warps of a team and row tiles of a warp: the fewest warps whose accumulators hold the rows.
+struct Shape {
+  int tiles, team;
+};
+static Shape shape_of(int rows) {
+  if (rows <= 8) return {1, 1};
+  if (rows <= 16) return {2, 1};
+  if (rows <= 32) return {4, 1};
+  if (rows <= 64) return {4, 2};
+  return {4, 4};
+}
+
+// Teams of the grid: from host values only, so that it is fixed for graph capture.
+static int grid_teams(int num_seqs, int num_kv_heads, int rows, int tokens, int max_context_len, int window, int sinks,
+                      int num_sms) {
+  int64_t chunks = ((int64_t)max_context_len + CK - 1) / CK;
+  if (window > 0) chunks = std::min(chunks, ((int64_t)sinks + CK - 1) / CK + ((int64_t)window + tokens + CK - 2) / CK + 1);
+  const int64_t resident = (int64_t)num_sms * BLOCKS_PER_SM * (WARPS / shape_of(rows).team);
+  return (int)std::max<int64_t>(1, std::min(resident, num_seqs * num_kv_heads * chunks));
+}
+
+static int64_t workspace_bytes_for(int64_t teams, int rows, int64_t pairs) {
+  return teams * 2 * rows * (HD + 2) * (int64_t)sizeof(float) + pairs * (int64_t)sizeof(int2);
+}
+
+// Bounds of the sizes that both entry points take.
+static bool sizes_ok(int num_seqs, int tokens, int num_heads, int num_kv_heads, int max_context_len, int window,
+                     int sinks) {
+  return num_seqs >= 0 && num_seqs <= 65535 && tokens > 0 && num_heads > 0 && num_kv_heads > 0 &&
+         num_heads % num_kv_heads == 0 && num_kv_heads <= 65535 && max_context_len >= 0 &&
+         max_context_len <= (1 << 30) && window >= 0 && sinks >= 0 && window <= (1 << 30) && sinks <= (1 << 30) &&
+         (int64_t)num_seqs * num_kv_heads <= 0x7fffffff;
+}
+
+template <int NT, int TEAM>
+static int launch(const Params& p, int grid, cudaStream_t st) {
+  static std::atomic<uint64_t> smem{0};
+  if (ensure_dynamic_smem((const void*)window_decode_kernel<NT, TEAM>, SMEM_BYTES, smem) != VLC_OK) return VLC_ERR_CUDA;
+  window_decode_kernel<NT, TEAM><<<grid, WARPS * 32, SMEM_BYTES, st>>>(p);
+  return launch_status();
+}
+
+}  // namespace decode_window
+}  // namespace vlc
+
+using namespace vlc;
+using namespace vlc::decode_window;
+
+extern "C" int64_t vlc_decode_window_workspace_size(int num_seqs, int num_tokens, int num_heads, int num_kv_heads,
+                                                    int max_context_len, int window, int sinks) {
+  if (num_seqs <= 0 || !sizes_ok(num_seqs, num_tokens, num_heads, num_kv_heads, max_context_len, window, sinks)) return 0;
+  const int64_t rows = (int64_t)num_heads / num_kv_heads * num_tokens;
+  if (rows > MAX_ROWS) return 0;
+  const int teams = grid_teams(num_seqs, num_kv_heads, (int)rows, num_tokens, std::max(1, max_context_len), window, sinks,
+                               vlc_num_sms());
+  return workspace_bytes_for(teams, (int)rows, (int64_t)num_seqs * num_kv_heads);
+}
+
+extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int num_seqs, int num_tokens,
+                                      int num_heads, const void* k_cache, const void* v_cache, int64_t num_pages,
+                                      int block_size, int num_kv_heads, int head_dim, const int32_t* block_tables,
+                                      int64_t block_table_stride, int block_table_width, const int32_t* context_lens,
+                                      int max_context_len, int window, int sinks, float softmax_scale, void* out,
+                                      int64_t out_token_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!sizes_ok(num_seqs, num_tokens, num_heads, num_kv_heads, max_context_len, window, sinks) || block_table_width < 0)
+    return VLC_ERR_SHAPE;
+  if (head_dim != HD || block_size <= 0 || block_size % CK != 0) return VLC_ERR_UNSUPPORTED;
+  const int G = num_heads / num_kv_heads;
+  if ((int64_t)G * num_tokens > MAX_ROWS || !std::isfinite(softmax_scale)) return VLC_ERR_UNSUPPORTED;
+  if (num_seqs == 0) return VLC_OK;
+  if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out) return VLC_ERR_NULL;
+  if (q_token_stride % 8 || out_token_stride % 8 || q_token_stride < (int64_t)num_heads * HD ||
+      out_token_stride < (int64_t)num_heads * HD || block_table_stride < block_table_width)
+    return VLC_ERR_STRIDE;
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out)) return VLC_ERR_ALIGN;
+  if (num_pages <= 0 || num_pages > 0x7fffffff / block_size) return VLC_ERR_SHAPE;
+  max_context_len = std::max(1, max_context_len);
+  const int sms = vlc_num_sms(), rows = G * num_tokens;
+  const int teams = grid_teams(num_seqs, num_kv_heads, rows, num_tokens, max_context_len, window, sinks, sms);
+  if (!workspace || workspace_bytes < workspace_bytes_for(teams, rows, (int64_t)num_seqs * num_kv_heads))
+    return VLC_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return VLC_ERR_ALIGN;
+
+  Params p;
+  const uint8_t* caches[2] = {(const uint8_t*)k_cache, (const uint8_t*)v_cache};
+  p.v_first = caches[1] < caches[0];
+  if (p.v_first) std::swap(caches[0], caches[1]);
+  const uint64_t apart = (uint64_t)(caches[1] - caches[0]);
+  p.joined = apart > 0 && apart < 1ull << 40;  // as a tensor map's strides may be
+  if (!p.joined && p.v_first) {
+    std::swap(caches[0], caches[1]);
+    p.v_first = false;
+  }
+  const uint64_t slots = (uint64_t)num_pages * block_size, row = (uint64_t)num_kv_heads * HD * 2;
+  for (int i = 0; i < (p.joined ? 1 : 2); ++i) {
+    const uint64_t both = p.joined ? 2 : 1;
+    const uint64_t dims[5] = {64, (uint64_t)num_kv_heads, slots, 2, both};
+    const uint64_t strides[4] = {HD * 2, row, 128, p.joined ? apart : 256};
+    const uint32_t box[5] = {64, 1, CK, 2, (uint32_t)both};
+    if (encode_tmap_bf16(&p.kv[i], caches[i], 5, dims, strides, box, 128) != VLC_OK) return VLC_ERR_CUDA;
+  }
+  p.q = (const __nv_bfloat16*)q;
+  p.q_token_stride = q_token_stride;
+  p.block_tables = block_tables;
+  p.table_stride = block_table_stride;
+  p.table_width = block_table_width;
+  p.block_size = block_size;
+  p.num_pages = (int)num_pages;
+  p.context_lens = context_lens;
+  p.num_seqs = num_seqs;
+  p.max_len = max_context_len;
+  p.tokens = num_tokens;
+  p.window = window;
+  p.sinks = window > 0 ? sinks : 0;
+  p.group = G;
+  p.num_kv_heads = num_kv_heads;
+  p.rows = rows;
+  p.scale_log2 = std::fabs(softmax_scale) * 1.4426950408889634f;
+  p.q_flip = softmax_scale < 0.f ? 0x80008000u : 0u;
+  p.out = (__nv_bfloat16*)out;
+  p.out_token_stride = out_token_stride;
+  p.num_teams = teams;
+  p.parts = (float*)workspace;
+  p.part_ml = (float2*)(p.parts + (int64_t)teams * 2 * rows * HD);
+  p.places = (int2*)(p.part_ml + (int64_t)teams * 2 * rows);
+
+  const Shape shape = shape_of(rows);
+  const int per_block = WARPS / shape.team, grid = (teams + per_block - 1) / per_block;
+  cudaStream_t st = (cudaStream_t)stream;
+  const int rc = shape.team == 4    ? launch<4, 4>(p, grid, st)
+                 : shape.team == 2  ? launch<4, 2>(p, grid, st)
+                 : shape.tiles == 4 ? launch<4, 1>(p, grid, st)
+                 : shape.tiles == 2 ? launch<2, 1>(p, grid, st)
+                                    : launch<1, 1>(p, grid, st);
+  if (rc != VLC_OK) return rc;
+  const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
+  const bool spread = teams / pairs + 1 > 10;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)pairs, spread ? rows : (rows + 7) / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, spread ? window_join_kernel<true> : window_join_kernel<false>, p) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return VLC_ERR_CUDA;
+  }
+  return VLC_OK;
+}

@@ -161,12 +161,18 @@ extern "C" int64_t vlc_prefill_plan_capacity(const int32_t* cu_q, const int32_t*
   return vlc_attention_plan_capacity(cu_q, cu_k, num_seqs, num_heads, num_kv_heads, 1, num_sms);
 }
 
-extern "C" int vlc_attention_plan(const int32_t* cu_q, const int32_t* cu_k, int num_seqs, int num_heads,
-                                  int num_kv_heads, int head_dim, int causal, int num_sms, int32_t* plan_out,
-                                  int64_t plan_capacity, int64_t* plan_len) {
+extern "C" int vlc_attention_plan_window(const int32_t* cu_q, const int32_t* cu_k, int num_seqs, int num_heads,
+                                         int num_kv_heads, int head_dim, int causal, int window, int sinks, int num_sms,
+                                         int32_t* plan_out, int64_t plan_capacity, int64_t* plan_len) {
   using namespace vlc;
   const int v = validate(cu_q, cu_k, num_seqs, num_heads, num_kv_heads, head_dim);
   if (v != VLC_OK) return v;
+  if (window < 0 || sinks < 0 || window > (1 << 30) || sinks > (1 << 30)) return VLC_ERR_SHAPE;
+  if (window > 0 && !causal) return VLC_ERR_UNSUPPORTED;
+  // A window that no sequence outgrows hides nothing.
+  bool outgrown = false;
+  for (int b = 0; b < num_seqs; ++b) outgrown |= cu_k[b + 1] - cu_k[b] > window;
+  if (!outgrown) window = 0;
   if (!plan_out || !plan_len) return VLC_ERR_NULL;
   if (num_sms <= 0) num_sms = vlc_num_sms();
   const int G = num_heads / num_kv_heads;
@@ -187,7 +193,7 @@ extern "C" int vlc_attention_plan(const int32_t* cu_q, const int32_t* cu_k, int 
   // Quad mode: per (sequence, KV head), from the end, tiles (a0, a1, b0, b1) = (last, last - 1,
   // last - 2, last - 3); the even CTA of a pair takes a0 and b0, the odd one a1 and b1, and the
   // pair's MMAs run over a0's (and b0's) key blocks.  `pairs` then holds (a0, b0), `odd` (a1, b1).
-  const bool quad = g_prefill_kernel.load() == 2 && !packed;
+  const bool quad = g_prefill_kernel.load() == 2 && !packed && window == 0;
   const int bins = quad ? std::max(1, num_sms / 2) : num_sms;
   std::vector<Pair> pairs, odd;
   pairs.reserve(tiles.size());
@@ -217,6 +223,15 @@ extern "C" int vlc_attention_plan(const int32_t* cu_q, const int32_t* cu_k, int 
       }
     }
     i = e;
+  }
+
+  // Under a window a pair's key blocks are those that its first row or a later one sees; the blocks of
+  // both its tiles are numbered without the skipped ones.
+  for (size_t i = 0; window > 0 && i < pairs.size(); ++i) {
+    const Pair& pr = pairs[i];
+    const int jump = window_blocks(tiles[pr.b >= 0 ? pr.b : pr.a].kpos0, window, sinks).jump;
+    tiles[pr.a].n_kb -= jump;
+    if (pr.b >= 0) tiles[pr.b].n_kb -= jump;
   }
 
   // Time model, in single-tile key-block steps (measured on B200: a step of a
@@ -384,6 +399,7 @@ extern "C" int vlc_attention_plan(const int32_t* cu_q, const int32_t* cu_k, int 
       u.f[kUKpos0A] = ta.kpos0;
       u.f[kUPartA] = np > 1 ? part_a + i : -1;
       u.f[kUPartB] = -1;
+      if (window > 0) u.f[kUKpos0B] = tiles[pr.b >= 0 ? pr.b : pr.a].kpos0;
       if (i < np_b) {
         const Tile& tb = tiles[pr.b];
         u.f[kUQBeginB] = tb.q_begin;
@@ -495,6 +511,8 @@ extern "C" int vlc_attention_plan(const int32_t* cu_q, const int32_t* cu_k, int 
   h[kPHeadDim] = head_dim;
   h[kPOffSegments] = (int32_t)off_segments;
   h[kPQuad] = quad ? 1 : 0;
+  h[kPWindow] = window;
+  h[kPSinks] = window > 0 ? sinks : 0;
   if (packed) {
     int32_t* seg = h + off_segments;
     for (int b = 0; b < num_seqs; ++b)
@@ -520,6 +538,13 @@ extern "C" int vlc_attention_plan(const int32_t* cu_q, const int32_t* cu_k, int 
   for (size_t i = 0; i < merge_blocks.size(); ++i) h[off_mblocks + i] = merge_blocks[i];
   *plan_len = total;
   return VLC_OK;
+}
+
+extern "C" int vlc_attention_plan(const int32_t* cu_q, const int32_t* cu_k, int num_seqs, int num_heads,
+                                  int num_kv_heads, int head_dim, int causal, int num_sms, int32_t* plan_out,
+                                  int64_t plan_capacity, int64_t* plan_len) {
+  return vlc_attention_plan_window(cu_q, cu_k, num_seqs, num_heads, num_kv_heads, head_dim, causal, 0, 0, num_sms,
+                                   plan_out, plan_capacity, plan_len);
 }
 
 extern "C" int vlc_prefill_plan(const int32_t* cu_q, const int32_t* cu_k, int num_seqs, int num_heads,

@@ -37,6 +37,8 @@ enum : int {
                           // sequence, for packed tiles (several short sequences in one tile)
   kPQuad = 21,            // 1: quad units on CTA pairs (prefill_attn_quad_kernel): the CTA
                           // ranges index CTA pairs, and unit i is records 2i (even CTA), 2i + 1
+  kPWindow = 22,          // 0, or the sliding window: row at position t sees keys j <= t with
+  kPSinks = 23,           // j > t - window or j < sinks
 };
 
 // A unit is one or two query tiles of one (sequence, KV head) over one range of
@@ -48,6 +50,9 @@ enum : int {
 // only): tile A holds whole consecutive sequences, tokens [q_begin, q_begin + q_count); its one
 // key block is the same tokens (k_base = q_begin, kv_len = q_count), and row t sees the keys of
 // its own sequence, [segments[t][0], segments[t][1]).
+// Windowed plan (kPWindow > 0): the key blocks that no row of the pair sees are skipped, and the
+// unit's block numbers count the others (window_block below); kUKpos0B of every unit is then the
+// position of the pair's first row, also where the unit has no tile B.
 constexpr int kUnitInts = 17;
 enum : int {
   kUSeq = 0,       // row of block_tables (-1: packed tile)
@@ -70,6 +75,22 @@ enum : int {
                    // first token in q, which is also its first key row in the in-flight K/V
                    // (the projection's output); -1 otherwise
 };
+
+// The 128-key blocks that a pair of tiles whose first row is at position `low` sees: those of the
+// sinks, then those from its window's first key on.  `first`: blocks of the sinks, `jump`: blocks
+// skipped behind them.
+struct WindowBlocks {
+  int first, jump;
+};
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline WindowBlocks window_blocks(int low, int window, int sinks) {
+  const int from = low - window + 1 > 0 ? (low - window + 1) / 128 : 0;
+  const int upto = (sinks + 127) / 128;
+  const int first = upto < from ? upto : from;
+  return WindowBlocks{first, from - first};
+}
 
 // kUPartA / kUPartB of a ghost tile: a quad's stand-in for a missing tile (computed, not written)
 constexpr int kGhostPart = -2;

@@ -100,6 +100,7 @@ struct Params {
   int tokens_per_tile;  // T
   int head_dim;         // d of q/k/v/out (64 < d <= 128); tiles are zero-padded to 128 columns
   int causal;           // 0: every row sees all of its sequence's keys
+  int window, sinks;    // windowed plans: a row at t sees keys j <= t with j > t - window or j < sinks
   const int32_t* segments;  // packed plans: {first, end} token of each query token's sequence
   __nv_bfloat16* out;
   int64_t out_token_stride;
@@ -199,6 +200,14 @@ __device__ __forceinline__ int key_block_slot(const Params& p, const int32_t* u,
   return (int)slot;
 }
 
+// The key block behind a unit's block number `kb`: its own, but for windowed plans.
+template <bool kWindow>
+__device__ __forceinline__ int key_block(const Params& p, const int32_t* u, int kb) {
+  if (!kWindow) return kb;
+  const WindowBlocks w = window_blocks(u[kUKpos0B], p.window, p.sinks);
+  return kb < w.first ? kb : kb + w.jump;
+}
+
 // Descriptor low words: q_lo / k_lo / v_lo address the tile's first byte; the K
 // steps of 16 add compile-time offsets (K-major: +32 B per step within a 64-column
 // half, +16 KB to the second half; MN-major V: +2 KB per 16 keys).
@@ -232,8 +241,9 @@ __device__ __forceinline__ void issue_pv_half(uint32_t o_tmem, uint32_t p_tmem, 
 // instantiation, so the causal path's code is not touched by it.  kDK: 16-column steps of
 // the head dim in the MMAs (5 for head dim 80: Q K^T over its 80 columns and P V with N =
 // 80, instead of the zero-padded 128; 8 otherwise).  O columns past 16 kDK are never
-// written (nor stored: the epilogue writes the head dim's columns only).
-template <bool kPacked, int kDK>
+// written (nor stored: the epilogue writes the head dim's columns only).  kWindow: a sliding window with
+// first tokens that stay visible; key blocks that no row of a unit's tiles sees are skipped.
+template <bool kPacked, int kDK, bool kWindow = false>
 __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __grid_constant__ Params p) {
   constexpr uint32_t kIdescPV = umma_idesc_bf16(128, 16 * kDK, false, true);
   extern __shared__ uint8_t smem_raw[];
@@ -362,7 +372,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
         kb0 = u[kUKbBegin];
         kb1 = u[kUKbEnd];
         infl = unit_inflight(p, u);
-        slot0 = kb0 < kb1 ? key_block_slot(p, u, kb0) : 0;
+        slot0 = kb0 < kb1 ? key_block_slot(p, u, key_block<kWindow>(p, u, kb0)) : 0;
       };
       if (u_begin < u_end) fetch(u_begin);
       bool waited = false;  // K/V rows (paged or contiguous) may be written by the preceding kernel
@@ -381,7 +391,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
         for (int kb = kb0; kb < kb_end; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (uint32_t)(it / STAGES) & 1u;
-          const int slot = kb == kb0 ? slot0 : kPacked ? u[kUQBeginB] : key_block_slot(p, u, kb);
+          const int slot = kb == kb0 ? slot0
+                           : kPacked ? u[kUQBeginB]
+                                     : key_block_slot(p, u, key_block<kWindow>(p, u, kb));
           if (it >= STAGES && !wait_or_abort(bars.k_empty + s, ph ^ 1u, VLC_DEV_ERR_TIMEOUT + 2, abort_flag)) {
             ok = false;
             break;
@@ -610,6 +622,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
       const int tok = row / p.group;
       const bool row_valid = row < p.rows && tok < q_count;
       const int qpos = p.causal ? kpos0 + tok : kpos0;  // non-causal: kpos0 = k_len - 1
+      // Windowed: the first key of the last row's window, and of the pair's first row's.
+      const int low_last = kWindow ? kpos0 + q_count - p.window : 0;
+      const int low_first = kWindow ? u[kUKpos0B] - p.window + 1 : 0;
 
       float m_use = -INFINITY;
       float l_row = 0.f;
@@ -621,7 +636,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
         }
         __syncwarp();
         tc_fence_after();
-        const int key0 = (kb0 + j) * BN;
+        const int key0 = key_block<kWindow>(p, u, kb0 + j) * BN;
         uint32_t sr[128];
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + q * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[q * 32]));
@@ -638,6 +653,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
 #pragma unroll
           for (int c = 0; c < 128; ++c)
             if (c < lo || c >= hi) sr[c] = __float_as_uint(-INFINITY);
+        } else if (kWindow && key0 < low_last && key0 + BN > p.sinks) {
+          // block begins behind the window of a row: the keys between the sinks and it are hidden
+          const int lim = qpos - key0, lo = lim - p.window + 1, hi = p.sinks - key0;
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c > lim || (c < lo && c >= hi)) sr[c] = __float_as_uint(-INFINITY);
         } else if (key0 + BN - 1 > kpos0) {  // block touches the causal diagonal
           const int lim = qpos - key0;
 #pragma unroll
@@ -660,15 +681,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
         m_use = m_new;
         const float mref = (m_use == -INFINITY) ? 0.f : m_use;
         // Keys past the sequence end: zero their V rows so 0 * garbage stays 0.  Tile A
-        // has every block of the unit, and its P*V runs first.
-        if ((kPacked || x == 0) && key0 + BN > kv_len) {
+        // has every block of the unit, and its P*V runs first.  So with keys behind every window.
+        const bool behind = kWindow && key0 < low_first && key0 + BN > p.sinks;
+        if ((kPacked || x == 0) && (key0 + BN > kv_len || behind)) {
           const int rb = kPacked ? ring0 : t;  // ring index of this block (tile A's count = the ring's)
           const int st = rb % STAGES;
           if (!wait_or_abort(bars.v_full + st, (uint32_t)(rb / STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 11, abort_flag)) {
             ok = false;
             break;
           }
-          if (key0 + row >= kv_len) {
+          if (key0 + row >= kv_len || (behind && key0 + row < low_first && key0 + row >= p.sinks)) {
             const uint4 z = make_uint4(0, 0, 0, 0);
             uint4* v0 = reinterpret_cast<uint4*>(smem + OFF_V + st * TILE_BYTES + row * 128);
             uint4* v1 = reinterpret_cast<uint4*>(smem + OFF_V + st * TILE_BYTES + HALF_BYTES + row * 128);
@@ -1674,12 +1696,16 @@ static int prefill_attn_impl(const void* q, int64_t q_token_stride, int total_q,
   prm.tokens_per_tile = T;
   prm.head_dim = head_dim;
   prm.causal = plan_host[kPCausal];
+  prm.window = plan_host[kPWindow];
+  prm.sinks = plan_host[kPSinks];
+  const bool windowed = prm.window > 0;
+  if (windowed && !(softmax_scale > 0.f)) return VLC_ERR_UNSUPPORTED;  // (hidden keys are scores of -infinity)
   prm.segments = plan_host[kPOffSegments] > 0 ? plan_dev + plan_host[kPOffSegments] : nullptr;
   if (prm.segments != nullptr && block_tables != nullptr) return VLC_ERR_PLAN;  // packed tiles: contiguous K/V
 
   const bool packed = prm.segments != nullptr;
   const bool quad_units = plan_host[kPQuad] != 0;
-  if (quad_units && (packed || grid % 2 != 0)) return VLC_ERR_PLAN;
+  if (quad_units && (packed || windowed || grid % 2 != 0)) return VLC_ERR_PLAN;
   if (quad_units) {
     // the K tensors again with a box of 64 keys: each CTA of a pair loads half of a block
     const uint64_t dims[3] = {(uint64_t)head_dim, (uint64_t)num_kv_heads, (uint64_t)num_slots};
@@ -1701,11 +1727,12 @@ static int prefill_attn_impl(const void* q, int64_t q_token_stride, int total_q,
   // the zero-padded 128 columns.
   const bool d80 = head_dim == 80;
   const void* kfn = quad_units ? (const void*)prefill_attn_quad_kernel<false>
+                    : windowed ? (const void*)prefill_attn_kernel<false, 8, true>
                     : packed   ? (d80 ? (const void*)prefill_attn_kernel<true, 5> : (const void*)prefill_attn_kernel<true, 8>)
                                : (d80 ? (const void*)prefill_attn_kernel<false, 5> : (const void*)prefill_attn_kernel<false, 8>);
   const int smem_bytes = quad_units ? quad::QD_SMEM_BYTES : SMEM_BYTES;
-  static std::atomic<uint64_t> smem_set[5];
-  const int kind = quad_units ? 4 : (packed ? 1 : 0) + (d80 ? 2 : 0);
+  static std::atomic<uint64_t> smem_set[6];
+  const int kind = quad_units ? 4 : windowed ? 5 : (packed ? 1 : 0) + (d80 ? 2 : 0);
   if (ensure_dynamic_smem(kfn, smem_bytes, smem_set[kind]) != VLC_OK) return VLC_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;
   // Both kernels are launched as programmatic dependents of their predecessor in the
