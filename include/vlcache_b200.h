@@ -483,9 +483,9 @@ int vlc_remap_block_tables(int32_t* block_tables, int64_t row_stride, int num_ro
  *   are in the cache, context_lens counts them): q / out [num_seqs * num_tokens, num_heads, 128]
  *   with any token stride, row i num_tokens + r being token context_lens[i] - num_tokens + r of
  *   sequence i.  At most 128 rows num_tokens * num_heads / num_kv_heads; block_size a multiple of
- *   16.  Tokens before a sequence's first and sequences of length 0 give zeros, a query row with
- *   an infinity or a NaN gives NaN.  Keys of a bad page are left out and recorded
- *   (VLC_DEV_ERR_BLOCK_RANGE), a length past max_context_len is cut to it and recorded
+ *   32.  Tokens before a sequence's first and sequences of length 0 give zeros, a query row with
+ *   an infinity or a NaN gives NaN.  Keys of a bad page that a row sees count as zeros and are
+ *   recorded (VLC_DEV_ERR_BLOCK_RANGE), a length past max_context_len is cut to it and recorded
  *   (VLC_DEV_ERR_LENGTH).  Sizes come from host values, so the launches can be captured; workspace:
  *   vlc_decode_window_workspace_size bytes, 16-byte aligned, one per call in flight.
  * vlc_step_metadata: sequence i of context_lens[i] tokens (below 0: an idle place of the batch)

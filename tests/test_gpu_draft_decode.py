@@ -85,14 +85,16 @@ CASES = [
     (28, 4, 1, 64, 100, 4, [1, 50, 100, 101, 104, 105, 164, 300, 999]),
     (28, 4, 5, 256, 512, 4, [5, 4, 1, 0, 511, 512, 513, 516, 517, 2000]),
     (28, 4, 2, 128, 1, 0, [2, 129, 1000]),
-    (16, 2, 3, 16, 33, 20, [3, 40, 53, 54, 200, 1000]),
+    (16, 2, 3, 32, 33, 20, [3, 40, 53, 54, 200, 1000]),
     (8, 8, 8, 256, 300, 300, [8, 299, 300, 301, 600, 601, 1500]),
     (12, 1, 1, 256, 64, 1, [700, 64, 65]),
     (12, 1, 5, 256, 700, 100, [3000, 701, 60]),
     (32, 2, 8, 256, 1000, 4, [5000, 8]),
     (16, 1, 8, 32, 77, 5, [400, 9, 1]),
-    (4, 4, 1, 48, 50, 3, [500, 47, 48, 49]),
+    (4, 4, 1, 96, 50, 3, [500, 47, 48, 49]),
     (2, 2, 31, 256, 20, 2, [500, 31, 12]),
+    (7, 1, 7, 64, 200, 33, [1000, 7, 300]),       # 49 rows: two tiles for four warps
+    (28, 4, 3, 256, 128, 0, [900, 3, 130]),       # 21: three tiles
 ]
 
 

@@ -11,20 +11,24 @@
 //     each) the 8 columns: S^T = K Q^T and O^T = V^T P^T.  A tile of 8 rows wastes at most 7, where a
 //     tile of 16 would waste half of one token's 7 or 8 heads.
 //   * P^T in the layout of a B operand is S^T's accumulator transposed: one movmatrix an 8 x 8 tile.
-//   * The keys that a sequence sees are chunks of 16: those of the sinks, then those from the window's
-//     first on; what lies between is skipped, its pages are not touched.
-// The chunks of all (sequence, KV head) pairs form one line that the grid's teams share out evenly,
-// each a contiguous run of it, so that the shares are equal whatever the lengths are.  A team is one
-// warp for up to 32 rows and two or four for more (a warp's accumulators are 32 registers a tile of 8
-// rows); it has its own ring of chunks, one TMA copy each (K and V together), and no barrier with
-// other teams.  A pair that a team has to itself is written out; the parts of a pair that several
-// teams share go to the workspace, and window_join_kernel, a programmatic dependent, joins them.
+//   * The keys that a sequence sees are chunks of 16 or 32: those of the sinks, then those from the
+//     window's first on; what lies between is skipped, its pages are not touched.
+// The chunks of all (sequence, KV head) pairs form one line that the grid's blocks share out evenly,
+// each a contiguous run of it, so that the shares are equal whatever the lengths are.  In a block a
+// team of warps takes every TEAMS-th chunk of the run, with a ring of its own (one TMA copy a chunk, K
+// and V together) and a running softmax of its own; at the end of a pair the teams' sums are added
+// through shared memory, lane by lane.  A team is one warp for up to 24 rows and two or four, which
+// share its chunks and have different rows, for more: a tile of 8 rows takes 32 registers of
+// accumulators and 16 of Q.  A pair that a block has to itself is written out; the parts of a pair
+// that several blocks share go to the workspace, and window_join_kernel, a programmatic dependent,
+// joins them.
 //
 // P is rounded to bf16, V's type, as an operand of its MMA has to be (by 2^-8 of itself at most); its sum
 // is taken over the rounded values, so that the error does not add up with the keys.  Scores, maxima
 // and sums are fp32.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 #include "common.cuh"
 #include "runtime.h"
@@ -33,19 +37,16 @@ namespace vlc {
 namespace decode_window {
 
 constexpr int HD = 128;
-constexpr int CK = 16;                  // keys of a chunk
-constexpr int HALF_BYTES = CK * 128;    // 64 dims of the keys
-constexpr int TILE_BYTES = 2 * HALF_BYTES;
-constexpr int STAGE_BYTES = 2 * TILE_BYTES;  // K and V
-constexpr int WARPS = 4;                // of a block
-constexpr int RING_STAGES = 3 * WARPS;  // of a block, shared out among its teams
-constexpr int SMEM_BYTES = RING_STAGES * STAGE_BYTES + 1024;  // + alignment to the swizzle's period
+constexpr int WARPS = 4;                 // of a block
+constexpr int RING_BYTES = 96 << 10;     // of a block, shared out among its teams
 constexpr int BLOCKS_PER_SM = 2;
+constexpr int MIN_BLOCK = 32;            // a page's tokens are a multiple of it
 constexpr int MAX_ROWS = 128;           // tokens x query heads of a KV head
 constexpr float SLACK = 8.f;            // log2 that the maximum may grow by before O is rescaled
+constexpr float NO_MAX = -3e38f;        // the maximum of no key (finite: differences of two are numbers)
 
 struct Params {
-  // {64 dims, Hk, slots, 2 halves of a row, caches}, box {64, 1, CK, 2, caches}.  Joined, the caches are
+  // {64 dims, Hk, slots, 2 halves of a row, caches}, box {64, 1, CK, 2, caches} of chunks of CK keys.  Joined, the caches are
   // the two, whose stride is their distance (v_first: V lies before K); else kv[0] is K and kv[1] V.
   CUtensorMap kv[2];
   bool joined, v_first;
@@ -57,14 +58,14 @@ struct Params {
   const int32_t* context_lens;
   int num_seqs, max_len, tokens, window, sinks;
   int group, num_kv_heads, rows;  // rows = tokens * group
-  float scale_log2;               // |softmax scale| * log2(e)
+  float scale_log2;               // |softmax scale| * log2(e), above 0: a hidden key's score stays -infinity
   uint32_t q_flip;                // the signs of a pair of q's elements where the scale is negative
   __nv_bfloat16* out;
   int64_t out_token_stride;
-  int num_teams;
-  // Workspace: a team's first pair and its last leave parts when they are not whole.
-  float* parts;     // [num_teams][2][rows][HD] sums of P V
-  float2* part_ml;  // [num_teams][2][rows] (maximum, sum of P)
+  int num_blocks;
+  // Workspace: a block's first pair and its last leave parts when they are not whole.
+  float* parts;     // [num_blocks][2][rows][HD] sums of P V
+  float2* part_ml;  // [num_blocks][2][rows] (maximum, sum of P)
   int2* places;     // [num_seqs][num_kv_heads] of each pair with keys: (slot of its first part, parts)
 };
 
@@ -94,14 +95,23 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
 
 // The chunks of a sequence that any of its rows sees: chunk v is v for v < first (of the sinks), and
 // v + jump from there on.
+template <int CK>  // keys of a chunk
 struct Span {
   int len;          // cut to the host's bound
   int low;          // first key of the window of the sequence's first row
   int first, jump;
   int count;
+  // Chunks whose keys every row sees: [0, all0) of the sinks and [all1, all2): they end by the first row's
+  // position and begin in the last row's window.
+  __device__ __forceinline__ int all0(const Params& p) const { return min(first, p.sinks / CK); }
+  __device__ __forceinline__ int all1(const Params& p) const {
+    return p.window > 0 ? max(first, (max(0, len - p.window) + CK - 1) / CK - jump) : 0;
+  }
+  __device__ __forceinline__ int all2(const Params& p) const { return (len - p.tokens + 1) / CK - jump; }
 };
-__device__ __forceinline__ Span span_of(const Params& p, int len) {
-  Span s;
+template <int CK>
+__device__ __forceinline__ Span<CK> span_of(const Params& p, int len) {
+  Span<CK> s;
   s.len = min(max(len, 0), p.max_len);
   s.low = p.window > 0 ? max(0, s.len - p.tokens - p.window + 1) : 0;
   const int wc = s.low / CK;
@@ -111,31 +121,36 @@ __device__ __forceinline__ Span span_of(const Params& p, int len) {
   return s;
 }
 
-// How the line of `total` chunks is shared: every team takes each() of them and the first extra()
+// How the line of `total` chunks is shared: every block takes each() of them and the first extra()
 // one more.
 struct Shares {
   int64_t each, extra;
-  __device__ __forceinline__ Shares(int64_t total, int teams) : each(total / teams), extra(total % teams) {}
-  __device__ __forceinline__ int64_t first(int64_t team) const { return team * each + min(team, extra); }
-  __device__ __forceinline__ int64_t count(int64_t team) const { return each + (team < extra ? 1 : 0); }
-  __device__ __forceinline__ int64_t team_of(int64_t chunk) const {
+  __device__ __forceinline__ Shares(int64_t total, int blocks) : each(total / blocks), extra(total % blocks) {}
+  __device__ __forceinline__ int64_t first(int64_t block) const { return block * each + min(block, extra); }
+  __device__ __forceinline__ int64_t count(int64_t block) const { return each + (block < extra ? 1 : 0); }
+  __device__ __forceinline__ int64_t block_of(int64_t chunk) const {
     const int64_t big = extra * (each + 1);
     return chunk < big ? chunk / (each + 1) : extra + (chunk - big) / each;
   }
 };
 
+// Byte of 16-byte piece `piece` of row `row` of a warp's Q in shared memory (rows of 256 bytes).
+__device__ __forceinline__ uint32_t q_at(int row, int piece) { return row * 256 + ((piece ^ (row & 7)) << 4); }
+
 // A warp's rows: S^T, O^T and the softmax, and the step over one chunk.  Lane (r, t) = (lane / 4,
 // lane % 4) holds keys r and r + 8 of a chunk, dims 8c + r, and rows 2t and 2t + 1 of each tile.
-template <int NT>  // tiles of 8 rows
+// Q_SMEM: Q in shared memory (four tiles leave no registers for it).
+template <int NT, int CK, bool Q_SMEM>  // NT: tiles of 8 rows, CK: keys of a chunk
 struct State {
-  uint32_t qb[NT][8][2];  // Q as B fragments: dims 16k + 2t, + 1 (and 8 more) of row r
-  float o[NT][8][4];      // m-tile i: dims 16i + r of rows 2t, 2t + 1 (0, 1), dims 16i + 8 + r (2, 3)
-  float l[NT][4];         // sums of P: 0 and 1 of rows 2t, 2t + 1
-  float m[NT][2];         // the maximum that P is relative to
-  float shift[NT][2];     // -m (0 before the first key)
+  static constexpr int KT = CK / 16;            // key tiles of a chunk
+  static constexpr int HALF_BYTES = CK * 128;   // 64 dims of its keys
+  uint32_t qb[Q_SMEM ? 1 : NT][8][2];  // Q as B fragments: dims 16k + 2t, + 1 (and 8 more) of row r
+  float o[NT][8][4];                   // m-tile i: dims 16i + r of rows 2t, 2t + 1 (0, 1), 16i + 8 + r (2, 3)
+  float l[NT][4];                      // sums of P: 0 and 1 of rows 2t, 2t + 1
+  float m[NT][2];                      // the maximum that P is relative to
 
   // Rows row0 .. of the pair, row x being token x / G's head x % G.
-  __device__ __forceinline__ void start(const Params& p, int seq, int head, int row0, int r, int t) {
+  __device__ __forceinline__ void start(const Params& p, int seq, int head, int row0, int r, int t, uint8_t* q_smem) {
     const int G = p.group;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -146,182 +161,253 @@ struct State {
           p.q + ((int64_t)seq * p.tokens + (live ? tok : 0)) * p.q_token_stride +
           ((int64_t)head * G + (live ? row - tok * G : 0)) * HD) + t;
       uint32_t top = 0;  // largest bf16 magnitude
+      uint32_t u[8][2];
 #pragma unroll
       for (int k = 0; k < 8; ++k)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint32_t u = live ? __ldg(src + 8 * k + 4 * x) ^ p.q_flip : 0u;
-          qb[n][k][x] = u;
-          top = max(top, max(u & 0x7fffu, (u >> 16) & 0x7fffu));
+          u[k][x] = live ? __ldg(src + 8 * k + 4 * x) ^ p.q_flip : 0u;
+          top = max(top, max(u[k][x] & 0x7fffu, (u[k][x] >> 16) & 0x7fffu));
         }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // A row with an infinity has scores of +-infinity or NaN only, whose softmax is NaN, also where
       // all of them are -infinity (which would read as no key): such rows become NaN here.
-      if (top >= 0x7f80u) {
+      const uint32_t spoil = top >= 0x7f80u ? 0x7fff7fffu : 0u;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) qb[n][k][0] = qb[n][k][1] = 0x7fff7fffu;
-      }
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (Q_SMEM) *reinterpret_cast<uint32_t*>(q_smem + q_at(n * 8 + r, 2 * k + x) + 4 * t) = u[k][x] | spoil;
+          else qb[n][k][x] = u[k][x] | spoil;
+        }
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
       l[n][0] = l[n][1] = l[n][2] = l[n][3] = 0.f;
-      m[n][0] = m[n][1] = -INFINITY;
-      shift[n][0] = shift[n][1] = 0.f;
+      m[n][0] = m[n][1] = NO_MAX;
+    }
+    if (Q_SMEM) __syncwarp();
+  }
+
+  // One chunk whose K and V tiles are at kt and vt; key0 is its first key.  `cut`: not every row sees all of it.
+  __device__ __forceinline__ void step(const Params& p, uint32_t kt, uint32_t vt, int key0, bool cut,
+                                       const Span<CK>& span, int row0, int lane, uint32_t q_smem) {
+    const int r = lane >> 2, t = lane & 3, mi = lane >> 3, ri = lane & 7;
+    // ---- S^T = K Q^T
+    float s[KT][NT][4];
+#pragma unroll
+    for (int c = 0; c < KT; ++c)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[c][n][0] = s[c][n][1] = s[c][n][2] = s[c][n][3] = 0.f;
+    {
+      float s2[4] = {0.f, 0.f, 0.f, 0.f};  // one tile alone: two chains of MMAs
+      // piece 2k + x of row ri is at (2k + x) ^ ri = 2k ^ (x ^ ri): an address, with bits of k exchanged
+      const uint32_t at = ((mi & 1) * 8 + ri) * 128 + (((mi >> 1) ^ ri) << 4);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t a[KT][4];
+#pragma unroll
+        for (int c = 0; c < KT; ++c) ldsm_x4(((kt + at) ^ ((k & 3) << 5)) + (k >> 2) * HALF_BYTES + c * 2048, a[c]);
+        if constexpr (Q_SMEM) {
+#pragma unroll
+          for (int n = 0; n < NT; n += 2) {  // two tiles' fragments in one load
+            uint32_t b[4];
+            ldsm_x4(q_smem + q_at(n * 8 + (mi >> 1) * 8 + ri, 2 * k + (mi & 1)), b);
+#pragma unroll
+            for (int c = 0; c < KT; ++c) {
+              mma_bf16(s[c][n], a[c], b[0], b[1]);
+              mma_bf16(s[c][n + 1], a[c], b[2], b[3]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < KT; ++c)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              mma_bf16(NT * KT == 1 && (k & 1) ? s2 : s[c][n], a[c], qb[n][k][0], qb[n][k][1]);
+        }
+      }
+      if (NT * KT == 1) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[0][0][x] += s2[x];
+      }
+    }
+    if (cut) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+          const int pos = span.len - p.tokens + (row0 + n * 8 + 2 * t + odd) / p.group;
+#pragma unroll
+          for (int c = 0; c < KT; ++c)
+#pragma unroll
+            for (int e = odd; e < 4; e += 2) {
+              const int key = key0 + c * 16 + r + (e >> 1) * 8;
+              if (key > pos || (p.window > 0 && key <= pos - p.window && key >= p.sinks)) s[c][n][e] = -INFINITY;
+            }
+        }
+      // V rows that no row of the sequence sees may hold anything: their P is 0, and so V is made.
+#pragma unroll
+      for (int x = lane; x < 2 * CK; x += 32) {
+        const int key = key0 + x % CK;
+        if (key >= span.len || (key < span.low && key >= p.sinks)) {
+#pragma unroll
+          for (int y = 0; y < 8; ++y)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vt + x * 128 + y * 16), "r"(0) : "memory");
+        }
+      }
+      fence_proxy_async_smem();  // before the next copy into the stage
+      __syncwarp();
+    }
+    // ---- running softmax, log2 domain
+    float top[NT][2], most = NO_MAX;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      top[n][0] = fmaxf(s[0][n][0], s[0][n][2]);
+      top[n][1] = fmaxf(s[0][n][1], s[0][n][3]);
+      if constexpr (KT == 2) {
+        top[n][0] = fmax3(top[n][0], s[1][n][0], s[1][n][2]);
+        top[n][1] = fmax3(top[n][1], s[1][n][1], s[1][n][3]);
+      }
+      most = fmax3(most, fmaf(top[n][0], p.scale_log2, -m[n][0]), fmaf(top[n][1], p.scale_log2, -m[n][1]));
+    }
+    // The lanes' own maxima tell whether any grew past the slack; only then are they joined.
+    if (__any_sync(0xffffffffu, most > SLACK)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          top[n][0] = fmaxf(top[n][0], __shfl_xor_sync(0xffffffffu, top[n][0], d));
+          top[n][1] = fmaxf(top[n][1], __shfl_xor_sync(0xffffffffu, top[n][1], d));
+        }
+        rescale(n, fmaxf(m[n][0], top[n][0] * p.scale_log2), fmaxf(m[n][1], top[n][1] * p.scale_log2));
+      }
+    }
+    uint32_t pb[KT][NT][2];
+#pragma unroll
+    for (int c = 0; c < KT; ++c)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float(&x)[4] = s[c][n];
+        x[0] = fast_exp2(fmaf(x[0], p.scale_log2, -m[n][0]));
+        x[1] = fast_exp2(fmaf(x[1], p.scale_log2, -m[n][1]));
+        x[2] = fast_exp2(fmaf(x[2], p.scale_log2, -m[n][0]));
+        x[3] = fast_exp2(fmaf(x[3], p.scale_log2, -m[n][1]));
+        pb[c][n][0] = transpose8x8(pack_bf16x2(x[0], x[1]));
+        pb[c][n][1] = transpose8x8(pack_bf16x2(x[2], x[3]));
+      }
+    // ---- O^T += V^T P^T
+    const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    const uint32_t at = ((mi >> 1) * 8 + ri) * 128 + (((mi & 1) ^ ri) << 4);
+#pragma unroll
+    for (int c = 0; c < KT; ++c) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_bf16(l[n], ones, pb[c][n][0], pb[c][n][1]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t a[4];
+        ldsm_x4_t(((vt + at) ^ ((i & 3) << 5)) + (i >> 2) * HALF_BYTES + c * 2048, a);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_bf16(o[n][i], a, pb[c][n][0], pb[c][n][1]);
+      }
     }
   }
 
-  // One chunk whose K and V tiles are at kt and vt.  CUT: key0 is its first key, and not every row
-  // sees all of it (`valid` 0: none of it counts).
-  template <bool CUT>
-  __device__ __forceinline__ void step(const Params& p, uint32_t kt, uint32_t vt, int key0, int valid, const Span& span,
-                                       int row0, int lane) {
-    const int r = lane >> 2, t = lane & 3, mi = lane >> 3, ri = lane & 7;
-    // ---- S^T = K Q^T
-    float s[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    {
-      float s2[4] = {0.f, 0.f, 0.f, 0.f};  // one tile alone: two chains of MMAs
-      const uint32_t at = kt + ((mi & 1) * 8 + ri) * 128;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        uint32_t a[4];
-        ldsm_x4(at + (k >> 2) * HALF_BYTES + ((((2 * k) & 7) + (mi >> 1) ^ ri) << 4), a);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma_bf16(NT == 1 && (k & 1) ? s2 : s[n], a, qb[n][k][0], qb[n][k][1]);
-      }
-      if (NT == 1) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[0][x] += s2[x];
-      }
-    }
-    // ---- running softmax, log2 domain
-    uint32_t pb[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float(&x)[4] = s[n];
-      bool hide[4];
-      if (CUT) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = key0 + r + (e >> 1) * 8;
-          const int pos = span.len - p.tokens + (row0 + n * 8 + 2 * t + (e & 1)) / p.group;
-          hide[e] = valid == 0 || key > pos || (p.window > 0 && key <= pos - p.window && key >= p.sinks);
-          if (hide[e]) x[e] = -INFINITY;
-        }
-      }
-      const float top0 = fmaxf(x[0], x[2]) * p.scale_log2, top1 = fmaxf(x[1], x[3]) * p.scale_log2;
-      // The lanes' own maxima tell whether any grew past the slack; only then are they joined.
-      if (__any_sync(0xffffffffu, top0 > m[n][0] + SLACK || top1 > m[n][1] + SLACK)) {
-        float m0 = top0, m1 = top1;
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, d));
-          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, d));
-        }
-        m0 = fmaxf(m[n][0], m0);
-        m1 = fmaxf(m[n][1], m1);
-        const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m[n][0] - m0);  // (-inf: no key so far)
-        const float f1 = m1 == -INFINITY ? 0.f : fast_exp2(m[n][1] - m1);
-        m[n][0] = m0;
-        m[n][1] = m1;
-        shift[n][0] = m0 == -INFINITY ? 0.f : -m0;
-        shift[n][1] = m1 == -INFINITY ? 0.f : -m1;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          o[n][i][0] *= f0;
-          o[n][i][1] *= f1;
-          o[n][i][2] *= f0;
-          o[n][i][3] *= f1;
-        }
-        l[n][0] *= f0;
-        l[n][1] *= f1;
-      }
-      x[0] = fast_exp2(fmaf(x[0], p.scale_log2, shift[n][0]));
-      x[1] = fast_exp2(fmaf(x[1], p.scale_log2, shift[n][1]));
-      x[2] = fast_exp2(fmaf(x[2], p.scale_log2, shift[n][0]));
-      x[3] = fast_exp2(fmaf(x[3], p.scale_log2, shift[n][1]));
-      if (CUT) {  // (not left to exp2(-inf): a scale of 0 would make it exp2(NaN))
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (hide[e]) x[e] = 0.f;
-      }
-      pb[n][0] = transpose8x8(pack_bf16x2(x[0], x[1]));
-      pb[n][1] = transpose8x8(pack_bf16x2(x[2], x[3]));
-    }
-    // ---- O^T += V^T P^T
-    const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-#pragma unroll
-    for (int n = 0; n < NT; ++n) mma_bf16(l[n], ones, pb[n][0], pb[n][1]);
-    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};  // of a lane's keys 2t, 2t + 1 (and 8 more)
-    if (CUT) {  // V rows that no row of the sequence sees may hold anything: their P is 0, and so is V then
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = key0 + 2 * t + (e & 1) + (e >> 1) * 8;
-        if (valid == 0 || key >= span.len || (key < span.low && key >= p.sinks))
-          keep[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
-      }
-    }
-    const uint32_t at = vt + ((mi >> 1) * 8 + ri) * 128;
+  // Tile n relative to other maxima.
+  __device__ __forceinline__ void rescale(int n, float m0, float m1) {
+    const float f0 = fast_exp2(m[n][0] - m0), f1 = fast_exp2(m[n][1] - m1);
+    m[n][0] = m0;
+    m[n][1] = m1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      uint32_t a[4];
-      ldsm_x4_t(at + (i >> 2) * HALF_BYTES + ((((2 * i) & 7) + (mi & 1) ^ ri) << 4), a);
-      if (CUT) {
-        a[0] &= keep[0];
-        a[1] &= keep[0];
-        a[2] &= keep[1];
-        a[3] &= keep[1];
-      }
+      o[n][i][0] *= f0;
+      o[n][i][1] *= f1;
+      o[n][i][2] *= f0;
+      o[n][i][3] *= f1;
+    }
+    l[n][0] *= f0;
+    l[n][1] *= f1;
+  }
+
+  // The sums to and from another warp's same lane, for one tile.
+  __device__ __forceinline__ void put(int n, float4* to, int lane) const {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_bf16(o[n][i], a, pb[n][0], pb[n][1]);
+    for (int i = 0; i < 8; ++i) to[i * 32 + lane] = make_float4(o[n][i][0], o[n][i][1], o[n][i][2], o[n][i][3]);
+    to[8 * 32 + lane] = make_float4(m[n][0], m[n][1], l[n][0], l[n][1]);
+  }
+  __device__ __forceinline__ void add(int n, const float4* from, int lane) {
+    const float4 ml = from[8 * 32 + lane];
+    rescale(n, fmaxf(m[n][0], ml.x), fmaxf(m[n][1], ml.y));
+    const float g0 = fast_exp2(ml.x - m[n][0]), g1 = fast_exp2(ml.y - m[n][1]);
+    l[n][0] = fmaf(ml.z, g0, l[n][0]);
+    l[n][1] = fmaf(ml.w, g1, l[n][1]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 v = from[i * 32 + lane];
+      o[n][i][0] = fmaf(v.x, g0, o[n][i][0]);
+      o[n][i][1] = fmaf(v.y, g1, o[n][i][1]);
+      o[n][i][2] = fmaf(v.z, g0, o[n][i][2]);
+      o[n][i][3] = fmaf(v.w, g1, o[n][i][3]);
     }
   }
 };
 
-// Grid: blocks of WARPS warps, WARPS / TEAM teams each; the warps of a team share its ring and its run
-// of the line, each with NT tiles of the pair's rows.
+// Q in shared memory takes a third of the ring; behind the ring are the sums (of a tile) that half of the block's
+// warps hand over to the other.
+constexpr int SUM_BYTES = 9 * 32 * 16;
+constexpr int SMEM_BYTES = RING_BYTES + WARPS / 2 * SUM_BYTES + 1024;  // + alignment to the swizzle's period
+
+// Keys of a chunk: where the rows take several warps a step's latency counts, so that it is made larger.
+__host__ __device__ constexpr int chunk_keys(int team) { return team > 1 ? 32 : 16; }
+
+// Grid: blocks of WARPS warps, WARPS / TEAM teams each; the warps of a team share its ring, each with NT
+// tiles of the pair's rows.
 template <int NT, int TEAM>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kernel(const __grid_constant__ Params p) {
-  constexpr int TEAMS = WARPS / TEAM, STAGES = RING_STAGES / TEAMS;
+  constexpr int TEAMS = WARPS / TEAM, CK = chunk_keys(TEAM);
+  constexpr int TILE_BYTES = CK * HD * 2, STAGE_BYTES = 2 * TILE_BYTES;  // K or V, and both
+  constexpr bool Q_SMEM = NT == 4;
+  constexpr int Q_BYTES = Q_SMEM ? WARPS * NT * 8 * HD * 2 : 0;
+  constexpr int STAGES = (RING_BYTES - Q_BYTES) / TEAMS / STAGE_BYTES;
+  static_assert(STAGES >= 3 && TEAMS * STAGES * STAGE_BYTES + Q_BYTES == RING_BYTES, "the ring is shared out");
+  using Span = Span<CK>;
+  auto span_of = [&](int len) { return decode_window::span_of<CK>(p, len); };
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_all[RING_STAGES], empty_all[RING_STAGES];
-  __shared__ int valid_all[RING_STAGES];
+  __shared__ __align__(8) uint64_t full_all[TEAMS * STAGES];
+  __shared__ uint32_t read_all[TEAMS * STAGES];  // how often a warp was done with the stage
   pdl_launch_dependents();  // the join waits for this grid's end before it reads
   const int warp = warp_id(), lane = lane_id();
   const int r = lane >> 2, t = lane & 3;
   const int G = p.group, Hk = p.num_kv_heads;
   const int team = warp / TEAM, mate = warp % TEAM;
   const int row0 = mate * NT * 8;
-  const int64_t my = (int64_t)blockIdx.x * TEAMS + team;
   uint64_t* const full = full_all + team * STAGES;
-  uint64_t* const empty = empty_all + team * STAGES;
-  volatile int* const valid_of = valid_all + team * STAGES;
-  if (threadIdx.x < RING_STAGES) {
+  uint32_t* const readers = read_all + team * STAGES;
+  if (threadIdx.x < TEAMS * STAGES) {
     mbar_init(full_all + threadIdx.x, 1);
-    mbar_init(empty_all + threadIdx.x, TEAM);
+    read_all[threadIdx.x] = 0;
     fence_mbar_init();
   }
   __syncthreads();
 
-  // ---- this team's run [c0, c0 + count) of the line, and the sequence that c0 lies in
+  // ---- this block's run [c0, c0 + count) of the line, and the sequence that c0 lies in (each warp for itself)
   int64_t total = 0;
   for (int i = lane; i < p.num_seqs; i += 32) {
     const int len = __ldg(p.context_lens + i);
-    if (my == 0 && mate == 0 && len > p.max_len) record_error(VLC_DEV_ERR_LENGTH);
-    total += span_of(p, len).count;
+    if (blockIdx.x == 0 && warp == 0 && len > p.max_len) record_error(VLC_DEV_ERR_LENGTH);
+    total += span_of(len).count;
   }
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
   total *= Hk;
-  const Shares shares(total, p.num_teams);
-  const int64_t c0 = shares.first(my);
-  const int count = (int)shares.count(my);
-  if (my >= p.num_teams || count == 0) return;
+  const Shares shares(total, p.num_blocks);
+  const int64_t c0 = shares.first(blockIdx.x);
+  const int count = (int)shares.count(blockIdx.x);
+  if (count == 0) return;
   int seq = 0;
   int64_t at = c0;  // c0's place among the chunks from the sequence's first on
   for (int base = 0;; base += 32) {
-    int64_t n = base + lane < p.num_seqs ? (int64_t)span_of(p, __ldg(p.context_lens + base + lane)).count * Hk : 0;
+    int64_t n = base + lane < p.num_seqs ? (int64_t)span_of(__ldg(p.context_lens + base + lane)).count * Hk : 0;
     int64_t upto = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -338,154 +424,169 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
     at -= __shfl_sync(0xffffffffu, upto, 31);
     if (base + 32 >= p.num_seqs) return;  // not reached: c0 < total
   }
-  Span span = span_of(p, __ldg(p.context_lens + seq));
-  int head = (int)(at / span.count), j = (int)(at - (int64_t)head * span.count);
+  Span span = span_of(__ldg(p.context_lens + seq));
+  int head = (int)(at / span.count), j0 = (int)(at - (int64_t)head * span.count);
 
-  uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023)) +
-                        team * (STAGES * STAGE_BYTES);
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* const ring = smem + team * (STAGES * STAGE_BYTES);
+  float4* const sums = reinterpret_cast<float4*>(smem + RING_BYTES);
+  uint8_t* const q_smem = smem + (RING_BYTES - Q_BYTES) + warp * (NT * 8 * HD * 2);  // (Q_SMEM)
 
-  // ---- the issuing side (lane 0 of the team's first warp): a cursor of its own
+  // ---- the issuing side (lane 0 of each warp): a cursor over the team's chunks.  The warp that is the last to be
+  // done with a chunk fills its stage again, so every warp moves the cursor along, and one of them issues.
+  const int mine = (count - team + TEAMS - 1) / TEAMS;  // chunks team, team + TEAMS, .. of the run
   Span ahead = span;
-  int a_seq = seq, a_head = head, a_j = j, a_index = -1, a_page = -1, issued = 0;
-  auto issue = [&]() {  // chunk `issued` of the run
+  int a_seq = seq, a_head = head, a_j = j0 + team, issued = 0;
+  int a_row = 0, a_index = 0, a_page = -1;  // its row in its page, the page of the sequence, the page's number
+  auto load_page = [&]() {
+    a_page = a_index < p.table_width ? __ldg(p.block_tables + a_seq * p.table_stride + a_index) : -1;
+  };
+  auto place = [&]() {  // a_j of another pair, or behind the sinks
+    while (a_j >= ahead.count) {  // past the pair's end: on to the pair that it lies in
+      a_j -= ahead.count;
+      if (++a_head < Hk) continue;
+      a_head = 0;
+      do {
+        ahead = span_of(__ldg(p.context_lens + ++a_seq));  // the chunk follows: so does a sequence with keys
+      } while (ahead.count <= 0);
+    }
+    const int key = (a_j < ahead.first ? a_j : a_j + ahead.jump) * CK;
+    a_index = key / p.block_size;
+    a_row = key - a_index * p.block_size;
+    load_page();
+  };
+  auto issue = [&](bool copy) {  // chunk `issued` of the team
     const int stage = issued % STAGES;
     uint64_t* bar = full + stage;
-    const int key = (a_j < ahead.first ? a_j : a_j + ahead.jump) * CK;
-    const int index = key / p.block_size;
-    if (index != a_index) {
-      a_index = index;
-      a_page = index < p.table_width ? __ldg(p.block_tables + a_seq * p.table_stride + index) : -1;
-    }
-    if ((uint32_t)a_page < (uint32_t)p.num_pages) {
-      const int slot = a_page * p.block_size + (key - index * p.block_size);
-      uint8_t* st = ring + stage * STAGE_BYTES;
-      valid_of[stage] = 1;
+    uint8_t* st = ring + stage * STAGE_BYTES;
+    if (copy) {
+      int slot = a_page * p.block_size + a_row;
+      if ((uint32_t)a_page >= (uint32_t)p.num_pages) {  // the table has no usable page there: recorded, zeros come
+        record_error(VLC_DEV_ERR_BLOCK_RANGE);
+        slot = p.num_pages * p.block_size;
+      }
       mbar_expect_tx(bar, STAGE_BYTES);
       tma_load_5d(st, &p.kv[0], bar, 0, a_head, slot, 0, 0);
       if (!p.joined) tma_load_5d(st + TILE_BYTES, &p.kv[1], bar, 0, a_head, slot, 0, 0);
-    } else {  // the table has no usable page there: recorded, and none of the chunk's keys counts
-      valid_of[stage] = 0;
-      record_error(VLC_DEV_ERR_BLOCK_RANGE);
-      mbar_arrive(bar);
     }
-    if (++issued == count || ++a_j < ahead.count) return;
-    a_j = 0;
-    a_index = -1;
-    if (++a_head < Hk) return;
-    a_head = 0;
-    do {
-      ahead = span_of(p, __ldg(p.context_lens + ++a_seq));  // a chunk follows: so does a sequence with keys
-    } while (ahead.count <= 0);
+    if (++issued == mine) return;
+    // the next chunk's place, whose page is there by the next call
+    a_j += TEAMS;
+    a_row += TEAMS * CK;
+    if (a_j >= ahead.count || (a_j >= ahead.first && a_j - TEAMS < ahead.first)) {
+      place();
+    } else if (a_row >= p.block_size) {
+      do {
+        a_row -= p.block_size;
+        ++a_index;
+      } while (a_row >= p.block_size);
+      load_page();
+    }
   };
-  const bool issuer = mate == 0 && lane == 0;
-  // (team warps go on at their own pace: a stage is filled again one chunk late, when they are surely done)
-  constexpr int LAG = TEAM > 1 ? 1 : 0;
-  if (issuer) {
-    for (int i = 0; i < min(STAGES, count); ++i) issue();
+  if (lane == 0 && mine > 0) {
+    place();
+    for (int i = 0; i < min(STAGES, mine); ++i) issue(mate == 0);
   }
-  // Whether chunk i came (recorded where it did not).
+  // Whether the team's chunk i came (recorded where it did not).
   auto arrived = [&](int i) {
     const uint32_t parity = (uint32_t)(i / STAGES) & 1u;
     if (mbar_try_wait(full + i % STAGES, parity)) return true;
     return mbar_wait_bounded(full + i % STAGES, parity, VLC_DEV_ERR_TIMEOUT + 26, VLC_WAIT_LIMIT_CYCLES);
   };
-  // Copies still in flight are given more time before the block may end.
-  auto leave = [&](int i) {
-    if (issuer) {
-      for (int x = i; x < issued; ++x) arrived(x);
-    }
-  };
 
-  const uint32_t ring_u = smem_u32(ring);
-  State<NT> state;
-  state.start(p, seq, head, row0, r, t);
-  // The team with a pair's first chunk notes where its parts will be: one for each team up to that of
-  // its last chunk, in slot 0 but for this team's.
-  auto note = [&](int64_t chunk, int slot) {
-    if (issuer)
-      p.places[(int64_t)seq * Hk + head] =
-          make_int2((int)my * 2 + slot, (int)(shares.team_of(chunk + span.count - 1) - my) + 1);
-  };
-  if (j == 0) note(c0, 0);
-  int begin = j;       // first chunk of the pair that is in the state
-  int first_slot = 0;  // the part's slot: 0 for the one that holds the team's first chunk
-
-  for (int i = 0; i < count; ++i) {
-    if (!__all_sync(0xffffffffu, arrived(i))) {
-      leave(i);
-      return;
-    }
-    const int stage = i % STAGES;
-    const uint32_t st = ring_u + stage * STAGE_BYTES;
-    const uint32_t kt = st + (p.v_first ? TILE_BYTES : 0), vt = st + (p.v_first ? 0 : TILE_BYTES);
-    const int valid = valid_of[stage];
-    const int key0 = (j < span.first ? j : j + span.jump) * CK;
-    // Every row sees a chunk that ends by the first row's position and begins in the last row's window
-    // (or ends among the sinks).
-    const bool whole_chunk = valid && key0 + CK - 1 <= span.len - p.tokens &&
-                             (p.window == 0 || key0 >= span.len - p.window || key0 + CK <= p.sinks);
-    if (whole_chunk) state.template step<false>(p, kt, vt, key0, valid, span, row0, lane);
-    else state.template step<true>(p, kt, vt, key0, valid, span, row0, lane);
-    __syncwarp();  // every lane has read the stage
-    if (TEAM > 1) {
-      if (lane == 0) mbar_arrive(empty + stage);
-      bool ok = true;
-      if (issuer && i >= LAG && issued < count) {
-        const int x = i - LAG;  // chunk whose stage is filled again
-        ok = mbar_wait_bounded(empty + x % STAGES, (uint32_t)(x / STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 27,
-                               VLC_WAIT_LIMIT_CYCLES);
-        if (ok) issue();
+  const uint32_t ring_u = smem_u32(ring), q_u = smem_u32(q_smem);
+  State<NT, CK, Q_SMEM> state;
+  int i = 0;        // the team's chunks so far
+  bool ok = true;   // its waits so far: a team that gave up takes no more chunks
+  for (int done = 0, first_slot = 0; done < count; first_slot = 1) {
+    // ---- the pair's chunks [done, done + n) of the run
+    const int n = min(span.count - j0, count - done);
+    // The block with a pair's first chunk notes where its parts will be: one for each block up to that
+    // of its last chunk, in slot 0 but for this block's.
+    if (j0 == 0 && threadIdx.x == 0)
+      p.places[(int64_t)seq * Hk + head] = make_int2((int)blockIdx.x * 2 + first_slot,
+                                                     (int)(shares.block_of(c0 + done + span.count - 1) - blockIdx.x) + 1);
+    state.start(p, seq, head, row0, r, t, q_smem);
+    const int all0 = span.all0(p), all1 = span.all1(p), all2 = span.all2(p);
+    const uint32_t k_off = p.v_first ? TILE_BYTES : 0, v_off = p.v_first ? 0 : TILE_BYTES;
+    for (int j = j0 + i * TEAMS + team - done; ok && j < j0 + n; j += TEAMS, ++i) {
+      if (!__all_sync(0xffffffffu, arrived(i))) {
+        ok = false;
+        break;
       }
-      if (!__all_sync(0xffffffffu, ok)) {
-        leave(i + 1);
-        return;
-      }
-    } else if (issuer && issued < count) {
-      issue();
-    }
-    if (++j < span.count && i + 1 < count) continue;
-
-    // ---- the pair ends, or the run does
-    const bool whole = begin == 0 && j == span.count;
-    float* const part_o = p.parts + (my * 2 + first_slot) * p.rows * HD;
-    float2* const part_ml = p.part_ml + (my * 2 + first_slot) * p.rows;
-#pragma unroll
-    for (int x = 0; x < NT * 2; ++x) {
-      const int n = x >> 1, odd = x & 1;
-      const int row = row0 + n * 8 + 2 * t + odd;
-      if (row >= p.rows) continue;
-      const float sum = state.l[n][odd];
-      if (whole) {
-        const int tok = row / G;
-        const float inv = sum != 0.f ? 1.f / sum : 0.f;  // (NaN stays NaN)
-        __nv_bfloat16* dst = p.out + ((int64_t)seq * p.tokens + tok) * p.out_token_stride +
-                             ((int64_t)head * G + row - tok * G) * HD + r;
-#pragma unroll
-        for (int mt = 0; mt < 8; ++mt) {
-          dst[16 * mt] = __float2bfloat16(state.o[n][mt][odd] * inv);
-          dst[16 * mt + 8] = __float2bfloat16(state.o[n][mt][2 + odd] * inv);
+      const int stage = i % STAGES;
+      const uint32_t st = ring_u + stage * STAGE_BYTES;
+      const int key0 = (j < span.first ? j : j + span.jump) * CK;
+      const bool all_seen = j < all0 || (j >= all1 && j < all2);
+      state.step(p, st + k_off, st + v_off, key0, !all_seen, span, row0, lane, q_u);
+      __syncwarp();  // every lane has read the stage
+      if (lane == 0 && issued < mine) {
+        bool last = true;
+        if (TEAM > 1) {
+          uint32_t before;  // (released to and acquired from the mates: their reads are done)
+          asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;"
+                       : "=r"(before)
+                       : "r"(smem_u32(readers + stage))
+                       : "memory");
+          last = (before + 1) % TEAM == 0;
         }
-      } else {
-        float* dst = part_o + (int64_t)row * HD + r;
-#pragma unroll
-        for (int mt = 0; mt < 8; ++mt) {  // (eight lanes write a sector)
-          dst[16 * mt] = state.o[n][mt][odd];
-          dst[16 * mt + 8] = state.o[n][mt][2 + odd];
-        }
-        if (r == 0) part_ml[row] = make_float2(state.m[n][odd], sum);
+        issue(last);
       }
     }
-    if (i + 1 == count) break;
-    j = begin = 0;
-    first_slot = 1;
-    if (++head == Hk) {
+    // ---- the teams' sums: the upper half of the warps hand theirs over until one team has them
+#pragma unroll
+    for (int half = WARPS / 2; half >= TEAM; half /= 2) {
+      float4* const to = sums + (warp % half) * (9 * 32);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        __syncthreads();
+        if (warp >= half && warp < 2 * half) state.put(x, to, lane);
+        __syncthreads();
+        if (warp < half) state.add(x, to, lane);
+      }
+    }
+    if (team == 0) {
+      const bool whole = j0 == 0 && n == span.count;
+      const int64_t slot = ((int64_t)blockIdx.x * 2 + first_slot) * p.rows;
+#pragma unroll
+      for (int x = 0; x < NT * 2; ++x) {
+        const int nt = x >> 1, odd = x & 1;
+        const int row = row0 + nt * 8 + 2 * t + odd;
+        if (row >= p.rows) continue;
+        const float sum = state.l[nt][odd];
+        if (whole) {
+          const int tok = row / G;
+          const float inv = sum != 0.f ? 1.f / sum : 0.f;  // (NaN stays NaN)
+          __nv_bfloat16* dst = p.out + ((int64_t)seq * p.tokens + tok) * p.out_token_stride +
+                               ((int64_t)head * G + row - tok * G) * HD + r;
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            dst[16 * mt] = __float2bfloat16(state.o[nt][mt][odd] * inv);
+            dst[16 * mt + 8] = __float2bfloat16(state.o[nt][mt][2 + odd] * inv);
+          }
+        } else {
+          float* dst = p.parts + (slot + row) * HD + r;
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {  // (eight lanes write a sector)
+            dst[16 * mt] = state.o[nt][mt][odd];
+            dst[16 * mt + 8] = state.o[nt][mt][2 + odd];
+          }
+          if (r == 0) p.part_ml[slot + row] = make_float2(state.m[nt][odd], sum);
+        }
+      }
+    }
+    done += n;
+    j0 = 0;
+    if (done < count && ++head == Hk) {
       head = 0;
       do {
-        span = span_of(p, __ldg(p.context_lens + ++seq));
+        span = span_of(__ldg(p.context_lens + ++seq));
       } while (span.count <= 0);
     }
-    note(c0 + i + 1, 1);
-    state.start(p, seq, head, row0, r, t);
+  }
+  // Copies still in flight are given more time before the block ends.
+  if (!ok && lane == 0) {
+    for (; i < issued; ++i) arrived(i);
   }
 }
 
@@ -506,7 +607,7 @@ struct Joined {
   }
 };
 
-// Joins the parts of the pairs that several teams shared and writes zeros for empty sequences.  Grid
+// Joins the parts of the pairs that several blocks shared and writes zeros for empty sequences.  Grid
 // (pair, rows).  SPREAD: a block takes one row, its eight warps the row's parts in turn; else eight
 // rows, a warp each, which loads eight parts at once.
 template <bool SPREAD>
@@ -524,15 +625,14 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
   if (row >= p.rows) return;
   int2 place = make_int2(0, 0);
   if (!empty) place = p.places[pair];
-  // A team that gave up waiting for its copies (recorded) leaves pairs unnoted: nothing is read for them.
-  if ((uint32_t)place.x >= 2u * p.num_teams || (uint32_t)place.y > (uint32_t)(p.num_teams - (place.x >> 1)))
-    place = make_int2(0, 1);
+  if ((uint32_t)place.x >= 2u * p.num_blocks || (uint32_t)place.y > (uint32_t)(p.num_blocks - (place.x >> 1)))
+    place = make_int2(0, 1);  // (not reached: every pair with keys is noted)
   const int count = place.y;
-  if (count == 1) return;  // written by its team
+  if (count == 1) return;  // written by its block
   const int tok = row / p.group;
   uint2* const dst = reinterpret_cast<uint2*>(p.out + ((int64_t)seq * p.tokens + tok) * p.out_token_stride +
                                               ((int64_t)head * p.group + row - tok * p.group) * HD) + lane;
-  // part i > 0 is in slot 0 of the team i after the first's
+  // part i > 0 is in slot 0 of the block i after the first's
   const int64_t first = (int64_t)place.x * p.rows + row, rest = (int64_t)(place.x & ~1) * p.rows + row;
   const float4* const po = reinterpret_cast<const float4*>(p.parts) + lane;
   Joined sum;
@@ -570,29 +670,38 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
   }
 }
 
-// Warps of a team and row tiles of a warp: the fewest warps whose accumulators hold the rows.
+// Warps of a team and row tiles of a warp: the fewest warps whose registers hold the rows.
 struct Shape {
   int tiles, team;
+  int keys() const { return chunk_keys(team); }
 };
 static Shape shape_of(int rows) {
   if (rows <= 8) return {1, 1};
   if (rows <= 16) return {2, 1};
-  if (rows <= 32) return {4, 1};
-  if (rows <= 64) return {4, 2};
+  if (rows <= 24) return {3, 1};
+  if (rows <= 32) return {2, 2};
+  if (rows <= 48) return {3, 2};
+  if (rows <= 64) return {2, 4};
+  if (rows <= 96) return {3, 4};
   return {4, 4};
 }
 
-// Teams of the grid: from host values only, so that it is fixed for graph capture.
-static int grid_teams(int num_seqs, int num_kv_heads, int rows, int tokens, int max_context_len, int window, int sinks,
-                      int num_sms) {
+// Blocks of the grid: from host values only, so that it is fixed for graph capture.  A block has at least
+// MIN_CHUNKS for each of its teams: few chunks, but fewer parts to join.
+constexpr int MIN_CHUNKS = 2;
+static int grid_blocks(int num_seqs, int num_kv_heads, int rows, int tokens, int max_context_len, int window, int sinks,
+                       int num_sms) {
+  const Shape shape = shape_of(rows);
+  const int CK = shape.keys();
   int64_t chunks = ((int64_t)max_context_len + CK - 1) / CK;
   if (window > 0) chunks = std::min(chunks, ((int64_t)sinks + CK - 1) / CK + ((int64_t)window + tokens + CK - 2) / CK + 1);
-  const int64_t resident = (int64_t)num_sms * BLOCKS_PER_SM * (WARPS / shape_of(rows).team);
-  return (int)std::max<int64_t>(1, std::min(resident, num_seqs * num_kv_heads * chunks));
+  const int least = MIN_CHUNKS * (WARPS / shape.team);
+  const int64_t most = (num_seqs * num_kv_heads * chunks + least - 1) / least;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)num_sms * BLOCKS_PER_SM, most));
 }
 
-static int64_t workspace_bytes_for(int64_t teams, int rows, int64_t pairs) {
-  return teams * 2 * rows * (HD + 2) * (int64_t)sizeof(float) + pairs * (int64_t)sizeof(int2);
+static int64_t workspace_bytes_for(int64_t blocks, int rows, int64_t pairs) {
+  return blocks * 2 * rows * (HD + 2) * (int64_t)sizeof(float) + pairs * (int64_t)sizeof(int2);
 }
 
 // Bounds of the sizes that both entry points take.
@@ -605,10 +714,10 @@ static bool sizes_ok(int num_seqs, int tokens, int num_heads, int num_kv_heads, 
 }
 
 template <int NT, int TEAM>
-static int launch(const Params& p, int grid, cudaStream_t st) {
+static int launch(const Params& p, cudaStream_t st) {
   static std::atomic<uint64_t> smem{0};
   if (ensure_dynamic_smem((const void*)window_decode_kernel<NT, TEAM>, SMEM_BYTES, smem) != VLC_OK) return VLC_ERR_CUDA;
-  window_decode_kernel<NT, TEAM><<<grid, WARPS * 32, SMEM_BYTES, st>>>(p);
+  window_decode_kernel<NT, TEAM><<<p.num_blocks, WARPS * 32, SMEM_BYTES, st>>>(p);
   return launch_status();
 }
 
@@ -623,9 +732,9 @@ extern "C" int64_t vlc_decode_window_workspace_size(int num_seqs, int num_tokens
   if (num_seqs <= 0 || !sizes_ok(num_seqs, num_tokens, num_heads, num_kv_heads, max_context_len, window, sinks)) return 0;
   const int64_t rows = (int64_t)num_heads / num_kv_heads * num_tokens;
   if (rows > MAX_ROWS) return 0;
-  const int teams = grid_teams(num_seqs, num_kv_heads, (int)rows, num_tokens, std::max(1, max_context_len), window, sinks,
+  const int blocks = grid_blocks(num_seqs, num_kv_heads, (int)rows, num_tokens, std::max(1, max_context_len), window, sinks,
                                vlc_num_sms());
-  return workspace_bytes_for(teams, (int)rows, (int64_t)num_seqs * num_kv_heads);
+  return workspace_bytes_for(blocks, (int)rows, (int64_t)num_seqs * num_kv_heads);
 }
 
 extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int num_seqs, int num_tokens,
@@ -636,7 +745,7 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
                                       int64_t out_token_stride, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!sizes_ok(num_seqs, num_tokens, num_heads, num_kv_heads, max_context_len, window, sinks) || block_table_width < 0)
     return VLC_ERR_SHAPE;
-  if (head_dim != HD || block_size <= 0 || block_size % CK != 0) return VLC_ERR_UNSUPPORTED;
+  if (head_dim != HD || block_size <= 0 || block_size % MIN_BLOCK != 0) return VLC_ERR_UNSUPPORTED;
   const int G = num_heads / num_kv_heads;
   if ((int64_t)G * num_tokens > MAX_ROWS || !std::isfinite(softmax_scale)) return VLC_ERR_UNSUPPORTED;
   if (num_seqs == 0) return VLC_OK;
@@ -648,8 +757,9 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
   if (num_pages <= 0 || num_pages > 0x7fffffff / block_size) return VLC_ERR_SHAPE;
   max_context_len = std::max(1, max_context_len);
   const int sms = vlc_num_sms(), rows = G * num_tokens;
-  const int teams = grid_teams(num_seqs, num_kv_heads, rows, num_tokens, max_context_len, window, sinks, sms);
-  if (!workspace || workspace_bytes < workspace_bytes_for(teams, rows, (int64_t)num_seqs * num_kv_heads))
+  const Shape shape = shape_of(rows);
+  const int blocks = grid_blocks(num_seqs, num_kv_heads, rows, num_tokens, max_context_len, window, sinks, sms);
+  if (!workspace || workspace_bytes < workspace_bytes_for(blocks, rows, (int64_t)num_seqs * num_kv_heads))
     return VLC_ERR_WORKSPACE;
   if (!aligned16(workspace)) return VLC_ERR_ALIGN;
 
@@ -668,7 +778,7 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
     const uint64_t both = p.joined ? 2 : 1;
     const uint64_t dims[5] = {64, (uint64_t)num_kv_heads, slots, 2, both};
     const uint64_t strides[4] = {HD * 2, row, 128, p.joined ? apart : 256};
-    const uint32_t box[5] = {64, 1, CK, 2, (uint32_t)both};
+    const uint32_t box[5] = {64, 1, (uint32_t)shape.keys(), 2, (uint32_t)both};
     if (encode_tmap_bf16(&p.kv[i], caches[i], 5, dims, strides, box, 128) != VLC_OK) return VLC_ERR_CUDA;
   }
   p.q = (const __nv_bfloat16*)q;
@@ -687,26 +797,30 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
   p.group = G;
   p.num_kv_heads = num_kv_heads;
   p.rows = rows;
-  p.scale_log2 = std::fabs(softmax_scale) * 1.4426950408889634f;
+  p.scale_log2 = std::max(std::fabs(softmax_scale) * 1.4426950408889634f, std::numeric_limits<float>::min());
   p.q_flip = softmax_scale < 0.f ? 0x80008000u : 0u;
   p.out = (__nv_bfloat16*)out;
   p.out_token_stride = out_token_stride;
-  p.num_teams = teams;
+  p.num_blocks = blocks;
   p.parts = (float*)workspace;
-  p.part_ml = (float2*)(p.parts + (int64_t)teams * 2 * rows * HD);
-  p.places = (int2*)(p.part_ml + (int64_t)teams * 2 * rows);
+  p.part_ml = (float2*)(p.parts + (int64_t)blocks * 2 * rows * HD);
+  p.places = (int2*)(p.part_ml + (int64_t)blocks * 2 * rows);
 
-  const Shape shape = shape_of(rows);
-  const int per_block = WARPS / shape.team, grid = (teams + per_block - 1) / per_block;
   cudaStream_t st = (cudaStream_t)stream;
-  const int rc = shape.team == 4    ? launch<4, 4>(p, grid, st)
-                 : shape.team == 2  ? launch<4, 2>(p, grid, st)
-                 : shape.tiles == 4 ? launch<4, 1>(p, grid, st)
-                 : shape.tiles == 2 ? launch<2, 1>(p, grid, st)
-                                    : launch<1, 1>(p, grid, st);
+  int rc;
+  switch (shape.team * 8 + shape.tiles) {
+    case 8 + 1: rc = launch<1, 1>(p, st); break;
+    case 8 + 2: rc = launch<2, 1>(p, st); break;
+    case 8 + 3: rc = launch<3, 1>(p, st); break;
+    case 16 + 2: rc = launch<2, 2>(p, st); break;
+    case 16 + 3: rc = launch<3, 2>(p, st); break;
+    case 32 + 2: rc = launch<2, 4>(p, st); break;
+    case 32 + 3: rc = launch<3, 4>(p, st); break;
+    default: rc = launch<4, 4>(p, st);
+  }
   if (rc != VLC_OK) return rc;
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
-  const bool spread = teams / pairs + 1 > 10;
+  const bool spread = blocks / pairs + 1 > 10;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)pairs, spread ? rows : (rows + 7) / 8);
   cfg.blockDim = dim3(256);
