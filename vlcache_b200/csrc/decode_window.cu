@@ -38,7 +38,7 @@ namespace decode_window {
 
 constexpr int HD = 128;
 constexpr int WARPS = 4;                 // of a block
-constexpr int RING_BYTES = 96 << 10;     // of a block, shared out among its teams
+constexpr int RING_BYTES = 64 << 10;     // of a block, shared out among its teams
 constexpr int BLOCKS_PER_SM = 2;
 constexpr int MIN_BLOCK = 32;            // a page's tokens are a multiple of it
 constexpr int MAX_ROWS = 128;           // tokens x query heads of a KV head
@@ -352,7 +352,7 @@ struct State {
   }
 };
 
-// Q in shared memory takes a third of the ring; behind the ring are the sums (of a tile) that half of the block's
+// Q in shared memory takes half of the ring; behind the ring are the sums (of a tile) that half of the block's
 // warps hand over to the other.
 constexpr int SUM_BYTES = 9 * 32 * 16;
 constexpr int SMEM_BYTES = RING_BYTES + WARPS / 2 * SUM_BYTES + 1024;  // + alignment to the swizzle's period
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
   constexpr bool Q_SMEM = NT == 4;
   constexpr int Q_BYTES = Q_SMEM ? WARPS * NT * 8 * HD * 2 : 0;
   constexpr int STAGES = (RING_BYTES - Q_BYTES) / TEAMS / STAGE_BYTES;
-  static_assert(STAGES >= 3 && TEAMS * STAGES * STAGE_BYTES + Q_BYTES == RING_BYTES, "the ring is shared out");
+  static_assert(STAGES >= 2 && TEAMS * STAGES * STAGE_BYTES + Q_BYTES == RING_BYTES, "the ring is shared out");
   using Span = Span<CK>;
   auto span_of = [&](int len) { return decode_window::span_of<CK>(p, len); };
   extern __shared__ uint8_t smem_raw[];
