@@ -202,10 +202,8 @@ __device__ __forceinline__ int key_block_slot(const Params& p, const int32_t* u,
 
 // The key block behind a unit's block number `kb`: its own, but for windowed plans.
 template <bool kWindow>
-__device__ __forceinline__ int key_block(const Params& p, const int32_t* u, int kb) {
-  if (!kWindow) return kb;
-  const WindowBlocks w = window_blocks(u[kUKpos0B], p.window, p.sinks);
-  return kb < w.first ? kb : kb + w.jump;
+__device__ __forceinline__ int key_block(const WindowBlocks& w, int kb) {
+  return !kWindow || kb < w.first ? kb : kb + w.jump;
 }
 
 // Descriptor low words: q_lo / k_lo / v_lo address the tile's first byte; the K
@@ -366,13 +364,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
       int g = 0, kb0 = 0, kb1 = 0, slot0 = 0;
       bool infl = false;
       const int32_t* u = nullptr;
+      WindowBlocks wb{0, 0};
       auto fetch = [&](int ui) {
         u = p.units + (int64_t)ui * kUnitInts;
         g = u[kUKvHead];
         kb0 = u[kUKbBegin];
         kb1 = u[kUKbEnd];
         infl = unit_inflight(p, u);
-        slot0 = kb0 < kb1 ? key_block_slot(p, u, key_block<kWindow>(p, u, kb0)) : 0;
+        if (kWindow) wb = window_blocks(u[kUKpos0B], p.window, p.sinks);
+        slot0 = kb0 < kb1 ? key_block_slot(p, u, key_block<kWindow>(wb, kb0)) : 0;
       };
       if (u_begin < u_end) fetch(u_begin);
       bool waited = false;  // K/V rows (paged or contiguous) may be written by the preceding kernel
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
           const uint32_t ph = (uint32_t)(it / STAGES) & 1u;
           const int slot = kb == kb0 ? slot0
                            : kPacked ? u[kUQBeginB]
-                                     : key_block_slot(p, u, key_block<kWindow>(p, u, kb));
+                                     : key_block_slot(p, u, key_block<kWindow>(wb, kb));
           if (it >= STAGES && !wait_or_abort(bars.k_empty + s, ph ^ 1u, VLC_DEV_ERR_TIMEOUT + 2, abort_flag)) {
             ok = false;
             break;
@@ -625,6 +625,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
       // Windowed: the first key of the last row's window, and of the pair's first row's.
       const int low_last = kWindow ? kpos0 + q_count - p.window : 0;
       const int low_first = kWindow ? u[kUKpos0B] - p.window + 1 : 0;
+      const WindowBlocks wb = kWindow ? window_blocks(u[kUKpos0B], p.window, p.sinks) : WindowBlocks{0, 0};
 
       float m_use = -INFINITY;
       float l_row = 0.f;
@@ -636,7 +637,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
         }
         __syncwarp();
         tc_fence_after();
-        const int key0 = key_block<kWindow>(p, u, kb0 + j) * BN;
+        const int key0 = key_block<kWindow>(wb, kb0 + j) * BN;
         uint32_t sr[128];
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + q * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[q * 32]));
@@ -654,11 +655,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
           for (int c = 0; c < 128; ++c)
             if (c < lo || c >= hi) sr[c] = __float_as_uint(-INFINITY);
         } else if (kWindow && key0 < low_last && key0 + BN > p.sinks) {
-          // block begins behind the window of a row: the keys between the sinks and it are hidden
+          // Block begins behind the window of a row: the keys between the sinks and it are hidden.  Where the
+          // block ends before the first row's position they are all on one side: one comparison a key.
           const int lim = qpos - key0, lo = lim - p.window + 1, hi = p.sinks - key0;
+          if (key0 + BN - 1 <= kpos0 && hi <= 0) {  // a window's first block
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c > lim || (c < lo && c >= hi)) sr[c] = __float_as_uint(-INFINITY);
+            for (int c = 0; c < 128; ++c)
+              if (c < lo) sr[c] = __float_as_uint(-INFINITY);
+          } else if (key0 + BN <= kpos0 - p.window + 1) {  // the sinks' last block
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              if (c >= hi) sr[c] = __float_as_uint(-INFINITY);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              if (c > lim || (c < lo && c >= hi)) sr[c] = __float_as_uint(-INFINITY);
+          }
         } else if (key0 + BN - 1 > kpos0) {  // block touches the causal diagonal
           const int lim = qpos - key0;
 #pragma unroll
@@ -771,10 +783,23 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
 #pragma unroll
       for (int q = 0; q < 4; ++q) tmem_ld32(o_addr + q * 32, *reinterpret_cast<uint32_t(*)[32]>(&orr[q * 32]));
       tmem_wait_ld();
+      const bool part32 = kWindow && part >= 0;
+      if (part32) {  // a windowed plan's parts keep 32 bits
+        float* dst32 = reinterpret_cast<float*>(p.part_o) + ((int64_t)part * BM + row) * HD;
+#pragma unroll
+        for (int c = 0; c < 128; c += 8) {
+          uint32_t v[8];
+#pragma unroll
+          for (int y = 0; y < 8; ++y) v[y] = __float_as_uint(__uint_as_float(orr[c + y]) * inv);
+          st_global_v8(dst32 + c, v);
+        }
+      }
 #pragma unroll
       for (int c = 0; c < 64; ++c)
         orr[c] = pack_bf16x2(__uint_as_float(orr[2 * c]) * inv, __uint_as_float(orr[2 * c + 1]) * inv);
-      if (own_slot && (part >= 0 || q_count == p.tokens_per_tile)) {
+      if (part32) {
+        // written above
+      } else if (own_slot && (part >= 0 || q_count == p.tokens_per_tile)) {
         // Full tile or split partial, Q slot free: the whole tile goes into the slot
         // in the Q load's layout (128-byte swizzle: 16-byte chunk c of row r of a
         // 64-column half at chunk c ^ (r % 8)) and leaves with two TMA stores.  The
@@ -1466,7 +1491,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
 }
 
 
-// Merge split units.  Part p holds O_p / l_p (bf16), its max m_p and sum l_p:
+// Merge split units.  Part p holds O_p / l_p (bf16, or fp32 in windowed plans), its max m_p and sum l_p:
 //   O = sum_p w_p (O_p / l_p) / sum_p w_p,   w_p = 2^(m_p - M) l_p.
 // 256-thread blocks listed by the planner as (merge, first row).  A warp is 4
 // groups of 8 lanes; lane c of a group owns dims [16 c, 16 c + 16) (one 32-byte
@@ -1474,13 +1499,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
 // group k folding parts k, k + K, ... with a running max, kMergeBatch parts per
 // round with their loads in flight together; the K states of a row combine
 // through shuffles.
-constexpr int kMergeBatch = 5;
-__global__ void __launch_bounds__(256, 3) prefill_merge_kernel(const int32_t* __restrict__ merges,
-                                                               const int32_t* __restrict__ blocks,
-                                                               const __nv_bfloat16* __restrict__ part_o,
-                                                               const float* __restrict__ part_ml, int group,
-                                                               __nv_bfloat16* __restrict__ out,
-                                                               int64_t out_token_stride, int head_dim) {
+template <bool F32>
+__global__ void __launch_bounds__(256, F32 ? 2 : 3)
+    prefill_merge_kernel(const int32_t* __restrict__ merges, const int32_t* __restrict__ blocks,
+                         const __nv_bfloat16* __restrict__ part_o, const float* __restrict__ part_ml, int group,
+                         __nv_bfloat16* __restrict__ out, int64_t out_token_stride, int head_dim) {
+  constexpr int kMergeBatch = 5;
+  constexpr int kLoads = F32 ? 4 : 2;  // 16-byte loads of a part's 16 dims
   const int entry = __ldg(blocks + blockIdx.x);
   const int32_t* m = merges + (int64_t)(entry >> 8) * kMergeInts;
   const int q_begin = __ldg(m + kMQBegin), g = __ldg(m + kMKvHead);
@@ -1506,19 +1531,21 @@ __global__ void __launch_bounds__(256, 3) prefill_merge_kernel(const int32_t* __
     // them is used, then the batch is folded with one rescale of the accumulator.
     for (int i0 = k0; i0 < nparts; i0 += kMergeBatch * K) {
       float2 v[kMergeBatch];
-      uint4 r0[kMergeBatch], r1[kMergeBatch];
+      uint4 r[kMergeBatch][kLoads];
 #pragma unroll
       for (int s = 0; s < kMergeBatch; ++s) {
         const int i = i0 + s * K;
         if (i < nparts) {
           const int64_t pr = (int64_t)(part0 + i) * BM + row;
-          const uint4* src = reinterpret_cast<const uint4*>(part_o + pr * HD) + 2 * c;
+          const uint4* src = F32 ? reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(part_o) + pr * HD) + 4 * c
+                                 : reinterpret_cast<const uint4*>(part_o + pr * HD) + 2 * c;
           v[s] = __ldg(&ml[pr]);
-          r0[s] = __ldg(src);
-          r1[s] = __ldg(src + 1);
+#pragma unroll
+          for (int y = 0; y < kLoads; ++y) r[s][y] = __ldg(src + y);
         } else {
           v[s] = make_float2(-INFINITY, 0.f);  // weight 0
-          r0[s] = r1[s] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int y = 0; y < kLoads; ++y) r[s][y] = make_uint4(0, 0, 0, 0);
         }
       }
       float m_new = m_run;
@@ -1534,12 +1561,19 @@ __global__ void __launch_bounds__(256, 3) prefill_merge_kernel(const int32_t* __
       for (int s = 0; s < kMergeBatch; ++s) {
         const float w = fast_exp2(v[s].x - mr) * v[s].y;  // weight of O_p / l_p (0 for an empty part)
         L += w;
-        const uint32_t wds[8] = {r0[s].x, r0[s].y, r0[s].z, r0[s].w, r1[s].x, r1[s].y, r1[s].z, r1[s].w};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float2 o = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wds[k]));
-          acc[2 * k] = fmaf(w, o.x, acc[2 * k]);
-          acc[2 * k + 1] = fmaf(w, o.y, acc[2 * k + 1]);
+        for (int y = 0; y < kLoads; ++y) {
+          const uint32_t wds[4] = {r[s][y].x, r[s][y].y, r[s][y].z, r[s][y].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (F32) {
+              acc[4 * y + k] = fmaf(w, __uint_as_float(wds[k]), acc[4 * y + k]);
+            } else {
+              const float2 o = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wds[k]));
+              acc[8 * y + 2 * k] = fmaf(w, o.x, acc[8 * y + 2 * k]);
+              acc[8 * y + 2 * k + 1] = fmaf(w, o.y, acc[8 * y + 2 * k + 1]);
+            }
+          }
         }
       }
     }
@@ -1588,7 +1622,8 @@ using namespace vlc::prefill;
 extern "C" int64_t vlc_prefill_workspace_size(const int32_t* plan_host) {
   if (!plan_host || plan_host[kPMagic] != kPlanMagic) return -1;
   const int64_t parts = plan_host[kPNumParts];
-  return parts * (int64_t)BM * (HD * (int64_t)sizeof(__nv_bfloat16) + 2 * (int64_t)sizeof(float));
+  const int64_t value = plan_host[kPWindow] > 0 ? sizeof(float) : sizeof(__nv_bfloat16);
+  return parts * (int64_t)BM * (HD * value + 2 * (int64_t)sizeof(float));
 }
 
 static int prefill_attn_impl(const void* q, int64_t q_token_stride, int total_q, int num_heads, const void* k_cache,
@@ -1770,7 +1805,7 @@ static int prefill_attn_impl(const void* q, int64_t q_token_stride, int total_q,
     mcfg.stream = st;
     mcfg.attrs = &pdl;
     mcfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&mcfg, prefill_merge_kernel, (const int32_t*)(plan_dev + plan_host[kPOffMerges]),
+    if (cudaLaunchKernelEx(&mcfg, windowed ? prefill_merge_kernel<true> : prefill_merge_kernel<false>, (const int32_t*)(plan_dev + plan_host[kPOffMerges]),
                            (const int32_t*)(plan_dev + plan_host[kPOffMergeBlocks]), (const __nv_bfloat16*)prm.part_o,
                            (const float*)prm.part_ml, group, prm.out, out_token_stride, head_dim) != cudaSuccess) {
       (void)cudaGetLastError();
