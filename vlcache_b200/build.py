@@ -4,7 +4,8 @@ Compiles every CUDA translation unit for sm_100a only (tcgen05/TMA code does not
 exist on other architectures) with nvcc, links the host planner, and links the
 CUDA runtime statically so the library has no torch dependency.  The driver API
 (cuTensorMapEncodeTiled) is reached through cudaGetDriverEntryPoint, so the
-library also loads on machines without a GPU (CPU-side tests use the planner).
+library also loads on machines without a GPU (CPU-side tests use the planner).  A small Python extension
+(``_binding``, g++ against torch's headers) calls it for the ops whose calls are short.
 
 Usage: ``python -m vlcache_b200.build [--force] [--verbose]``.
 """
@@ -13,10 +14,12 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -31,6 +34,8 @@ CUDA_SOURCES = ["runtime.cu", "kv_ops.cu", "prefill_attn.cu", "decode_attn.cu", 
                 "rope_axes.cu", "kv_fp4.cu", "decode_fp4.cu", "pages.cu", "decode_window.cu",
                 "step_metadata.cu", "verify.cu"]
 CPP_SOURCES = ["plan.cpp"]
+BINDING_SOURCE = "binding.cpp"
+BINDING_PATH = PKG_DIR / "_binding.so"
 
 
 def nvcc_path() -> str:
@@ -41,7 +46,7 @@ def nvcc_path() -> str:
 
 
 def _sources() -> list[Path]:
-    return [CSRC / s for s in CUDA_SOURCES + CPP_SOURCES]
+    return [CSRC / s for s in CUDA_SOURCES + CPP_SOURCES + [BINDING_SOURCE]]
 
 
 def _headers() -> list[Path]:
@@ -65,7 +70,7 @@ def source_hash() -> str:
 
 def is_fresh() -> bool:
     """True when the in-tree library exists and was built from the current sources."""
-    return LIB_PATH.exists() and STAMP_PATH.exists() and STAMP_PATH.read_text().strip() == source_hash()
+    return LIB_PATH.exists() and BINDING_PATH.exists() and STAMP_PATH.exists() and STAMP_PATH.read_text().strip() == source_hash()
 
 
 def _needs_build() -> bool:
@@ -90,13 +95,49 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _torch_dir() -> Path:
+    """Where torch is installed, without importing it."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        raise RuntimeError("torch not found; the vlcache_b200 binding cannot be built")
+    return Path(spec.submodule_search_locations[0])
+
+
+def _compile_binding(verbose: bool) -> Path:
+    torch = _torch_dir()
+    obj = BUILD_DIR / (BINDING_SOURCE + ".o")
+    BUILD_DIR.mkdir(parents=True, exist_ok=True)
+    include = [torch / "include", torch / "include/torch/csrc/api/include", sysconfig.get_paths()["include"],
+               Path(nvcc_path()).resolve().parent.parent / "include"]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-I", str(INCLUDE),
+           *[a for p in include for a in ("-isystem", str(p))], "-c", str(CSRC / BINDING_SOURCE), "-o", str(obj)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SOURCE}:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    if verbose and (res.stdout or res.stderr):
+        sys.stderr.write(res.stdout + res.stderr)
+    return obj
+
+
+def _link_binding(obj: Path) -> None:
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = ["g++", "-shared", "-o", str(tmp), str(obj), f"-L{_torch_dir() / 'lib'}", "-ltorch_python", "-ltorch_cpu",
+           "-lc10_cuda", "-lc10", f"-L{PKG_DIR}", f"-l:{LIB_PATH.name}", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"link of the binding failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING_PATH)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile (unless the library was built from exactly these sources) and return the
     path of the shared library."""
     if not force and not _needs_build():
         return LIB_PATH
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
-        objs = list(ex.map(lambda s: _compile(s, verbose), _sources()))
+        binding = ex.submit(_compile_binding, verbose)
+        objs = list(ex.map(lambda s: _compile(s, verbose), [CSRC / s for s in CUDA_SOURCES + CPP_SOURCES]))
+        binding_obj = binding.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [nvcc_path(), *ARCH_FLAGS, "-rdc=true", "-shared", "-cudart", "static", "-Xcompiler", "-fPIC",
            "-o", str(tmp), *map(str, objs)]
@@ -105,6 +146,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     digest = source_hash()
     os.replace(tmp, LIB_PATH)
+    _link_binding(binding_obj)
     STAMP_PATH.write_text(digest + "\n")
     return LIB_PATH
 

@@ -960,27 +960,17 @@ def remap_block_tables(block_tables: torch.Tensor, page_map: torch.Tensor) -> No
 
 
 # --------------------------------------------------------------------------- a decode step with drafted tokens
-def _tokens(t: torch.Tensor, name: str) -> tuple[int, int, int, int, int]:
-    """(sequences, tokens, heads, head_dim, token stride) of bf16 rows [B, n, H, D] (or [B, H, D]:
-    n = 1) with contiguous heads, one sequence's tokens behind another's."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) == 3:
-        shape, stride = (shape[0], 1, shape[1], shape[2]), (stride[0], stride[0], stride[1], stride[2])
-    if t.dtype != torch.bfloat16 or len(shape) != 4:
-        raise ValueError(f"{name}: bf16 [sequences, tokens, heads, head_dim]")
-    b, n, h, d = shape
-    if stride[3] != 1 or (h > 1 and stride[2] != d):
-        raise ValueError(f"{name}: the heads of a token must be contiguous")
-    step = stride[1] if n > 1 else stride[0] if b > 1 else h * d
-    if n > 1 and b > 1 and stride[0] != n * step:
-        raise ValueError(f"{name}: a sequence's tokens follow the one's before, at one token stride")
-    return b, n, h, d, step
+_compiled = None
 
 
-def _window(window, sinks) -> tuple[int, int]:
-    window, sinks = int(window), int(sinks)
-    _need(0 <= window <= 1 << 30 and 0 <= sinks <= 1 << 30, "window and sinks: 0 .. 2^30")
-    return window, sinks
+def _binding():
+    """The compiled binding (checks, allocations and launches of the ops below in C++)."""
+    global _compiled
+    if _compiled is None:
+        lib()   # raises where the kernels' library is missing
+        from . import _binding as module
+        _compiled = module
+    return _compiled
 
 
 def decode_window_workspace_bytes(num_seqs: int, num_tokens: int, num_heads: int, num_kv_heads: int,
@@ -1001,39 +991,9 @@ def decode_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     and sequences of length 0 give zeros, a head whose query holds an infinity or a NaN gives NaN.
     ``max_context_len`` bounds the lengths on the host and sizes the grid; ``workspace``:
     ``decode_window_workspace_bytes``, contiguous, one per call in flight."""
-    dev = _device(q, k_cache, v_cache, block_tables, context_lens, out, workspace)
-    b, n, h, d, qs = _tokens(q, "q")
-    shape = k_cache.shape
-    _need(k_cache.dtype == torch.bfloat16 and v_cache.dtype == torch.bfloat16 and len(shape) == 4
-          and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous() and shape[3] == d,
-          "k_cache / v_cache: contiguous bf16 [pages, block_size, num_kv_heads, head_dim]")
-    stride, width = _tables(block_tables, b)
-    _need(context_lens.dtype == torch.int32 and context_lens.numel() == b and context_lens.is_contiguous(),
-          "context_lens: contiguous int32, one per sequence")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        os = h * d
-    else:
-        _need(out.shape == q.shape, "out: q's shape")
-        os = _tokens(out, "out")[4]
-    max_context_len = int(max_context_len)
-    _need(0 <= max_context_len <= 1 << 30, "max_context_len: 0 .. 2^30")
-    window, sinks = _window(window, sinks)
-    need = lib().vlc_decode_window_workspace_size(b, n, h, shape[2], max_context_len, window, sinks)
-    if need > 0 and (workspace is None or workspace.nbytes < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _need(workspace is None or workspace.is_contiguous(), "workspace: contiguous")
-    _launch(dev, "vlc_decode_attn_window", q.data_ptr(), qs, b, n, h, k_cache.data_ptr(), v_cache.data_ptr(), shape[0],
-            shape[1], shape[2], d, block_tables.data_ptr(), stride, width, context_lens.data_ptr(), max_context_len,
-            window, sinks, float(softmax_scale), out.data_ptr(), os, _ptr(workspace),
-            0 if workspace is None else workspace.nbytes)
-    return out
-
-
-def _ints(t: torch.Tensor, n: int, name: str) -> int:
-    _need(t.dtype == torch.int32 and t.is_contiguous() and (n < 0 or t.numel() == n),
-          f"{name}: contiguous int32" + ("" if n < 0 else f" [{n}]"))
-    return t.data_ptr()
+    return (_compiled or _binding()).decode_attention_window(q, k_cache, v_cache, block_tables, context_lens,
+                                                             max_context_len, softmax_scale, window, sinks, out,
+                                                             workspace)
 
 
 def step_metadata(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor,
@@ -1052,37 +1012,8 @@ def step_metadata(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
     past the table and rows past ``total_rows`` are recorded (``device_error``) and have slot -1 or are
     left out (include/vlcache_b200.h).  The tables' pages are their own: forked requests, which share
     pages, stay with ``engine.page_pool``."""
-    dev = _device(context_lens, new_lens, block_tables, free_pages, num_free)
-    b = context_lens.numel()
-    lens = _ints(context_lens, b, "context_lens")
-    fresh = _ints(new_lens, b, "new_lens")
-    stride, width = _tables(block_tables, b)
-    free = _ints(free_pages, -1, "free_pages")
-    count = _ints(num_free, 1, "num_free")
-    block_size, total_rows = int(block_size), int(total_rows)
-    _need(block_size > 0, "block_size: positive")
-    _need(0 <= total_rows <= 1 << 30, "total_rows: 0 .. 2^30")
-    window, sinks = _window(window, sinks)
-    positions = torch.empty(total_rows, dtype=torch.int64, device=context_lens.device)
-    ints = torch.empty(total_rows + 3 * b + 2, dtype=torch.int32, device=context_lens.device)
-    slots, cu_q, cu_k, after = ints.split((total_rows, b + 1, b + 1, b))
-    at = ints.data_ptr()
-    _launch(dev, "vlc_step_metadata", lens, fresh, b, block_tables.data_ptr(), stride, width, block_size, window, sinks,
-            free, free_pages.numel(), count, positions.data_ptr(), at, total_rows, at + 4 * total_rows,
-            at + 4 * (total_rows + b + 1), at + 4 * (total_rows + 2 * b + 2))
-    return positions, slots, cu_q, cu_k, after
-
-
-_PROB_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _probs(t: torch.Tensor, b: int, rows: int, name: str) -> tuple[int, int, int]:
-    """(vocabulary, sequence stride, row stride) of probabilities [b, rows, vocabulary]."""
-    shape, stride = t.shape, t.stride()
-    _need(len(shape) == 3 and shape[0] == b and shape[1] == rows and t.dtype in _PROB_TYPES,
-          f"{name}: fp32, bf16 or fp16 [{b}, {rows}, vocabulary]")
-    _need(shape[2] <= 1 or stride[2] == 1, f"{name}: a row's values must be contiguous")
-    return shape[2], stride[0], stride[1]
+    return (_compiled or _binding()).step_metadata(context_lens, new_lens, block_tables, free_pages, num_free, block_size,
+                                                   total_rows, window, sinks)
 
 
 def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, draft_probs: torch.Tensor | None,
@@ -1098,21 +1029,4 @@ def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, draft_probs:
     [B, K + 1]: the accepted drafts, the sampled token, then -1; emitted int32 [B]: accepted + 1).
     Sums are whole numbers (include/vlcache_b200.h), so the answer is the same in every run and
     whatever the order of summation.  At most 31 drafts and 2^18 tokens of vocabulary."""
-    dev = _device(drafts, target_probs, draft_probs, u, u_last)
-    _need(drafts.dtype == torch.int64 and drafts.dim() == 2, "drafts: int64 [sequences, drafts]")
-    b, k = drafts.shape
-    _need(k <= 1 or drafts.stride(1) == 1, "drafts: a sequence's tokens must be contiguous")
-    vocab, ps, pr = _probs(target_probs, b, k + 1, "target_probs")
-    qs = qr = 0
-    if draft_probs is not None:
-        other, qs, qr = _probs(draft_probs, b, k, "draft_probs")
-        _need(other == vocab and draft_probs.dtype == target_probs.dtype, "draft_probs: target_probs' vocabulary and type")
-    _need(u.dtype == torch.float32 and u.shape == (b, k) and (k <= 1 or u.stride(1) == 1), f"u: fp32 [{b}, {k}]")
-    _need(u_last.dtype == torch.float32 and u_last.shape == (b,) and (b <= 1 or u_last.stride(0) == 1),
-          f"u_last: fp32 [{b}]")
-    tokens = torch.empty(b, k + 1, dtype=torch.int64, device=drafts.device)
-    emitted = torch.empty(b, dtype=torch.int32, device=drafts.device)
-    _launch(dev, "vlc_verify_drafts", drafts.data_ptr(), drafts.stride(0), b, k, target_probs.data_ptr(), ps, pr,
-            _ptr(draft_probs), qs, qr, vocab, _PROB_TYPES[target_probs.dtype], u.data_ptr(), u.stride(0),
-            u_last.data_ptr(), tokens.data_ptr(), emitted.data_ptr())
-    return tokens, emitted
+    return (_compiled or _binding()).verify_drafts(drafts, target_probs, draft_probs, u, u_last)
