@@ -21,7 +21,8 @@
 // share its chunks and have different rows, for more: a tile of 8 rows takes 32 registers of
 // accumulators and 16 of Q.  A pair that a block has to itself is written out; the parts of a pair
 // that several blocks share go to the workspace, and window_join_kernel, a programmatic dependent,
-// joins them.
+// joins them.  Few pairs of few keys are taken by clusters instead, a pair each, whose blocks join through
+// their shared memory: one launch.
 //
 // P is rounded to bf16, V's type, as an operand of its MMA has to be (by 2^-8 of itself at most); its sum
 // is taken over the rounded values, so that the error does not add up with the keys.  Scores, maxima
@@ -58,6 +59,9 @@ struct Params {
   const int32_t* context_lens;
   int num_seqs, max_len, tokens, window, sinks;
   int group, num_kv_heads, rows;  // rows = tokens * group
+  uint32_t group_inverse;         // 2^16 / group, rounded up: exact for rows below 128
+  __device__ __forceinline__ int token_of(int row) const { return (int)((uint32_t)row * group_inverse >> 16); }
+  int cluster;                    // blocks of a pair's cluster (0: the line)
   float scale_log2;               // |softmax scale| * log2(e), above 0: a hidden key's score stays -infinity
   uint32_t q_flip;                // the signs of a pair of q's elements where the scale is negative
   __nv_bfloat16* out;
@@ -155,7 +159,7 @@ struct State {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = row0 + n * 8 + r;
-      const int tok = row / G;
+      const int tok = p.token_of(row);
       const bool live = row < p.rows;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(
           p.q + ((int64_t)seq * p.tokens + (live ? tok : 0)) * p.q_token_stride +
@@ -237,7 +241,7 @@ struct State {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int odd = 0; odd < 2; ++odd) {
-          const int pos = span.len - p.tokens + (row0 + n * 8 + 2 * t + odd) / p.group;
+          const int pos = span.len - p.tokens + p.token_of(row0 + n * 8 + 2 * t + odd);
 #pragma unroll
           for (int c = 0; c < KT; ++c)
 #pragma unroll
@@ -352,17 +356,29 @@ struct State {
   }
 };
 
-// Q in shared memory takes half of the ring; behind the ring are the sums (of a tile) that half of the block's
-// warps hand over to the other.
-constexpr int SUM_BYTES = 9 * 32 * 16;
-constexpr int SMEM_BYTES = RING_BYTES + WARPS / 2 * SUM_BYTES + 1024;  // + alignment to the swizzle's period
+// Q in shared memory takes half of the ring; behind the ring are the sums that half of the block's warps hand over
+// to the other.
+constexpr int SUM_BYTES = 9 * 32 * 16;  // of a tile
+__host__ __device__ constexpr int smem_bytes(int tiles) {
+  return RING_BYTES + WARPS / 2 * (tiles < 2 ? 2 : tiles) * SUM_BYTES + 1024;  // + alignment to the swizzle's period
+}
 
 // Keys of a chunk: where the rows take several warps a step's latency counts, so that it is made larger.
 __host__ __device__ constexpr int chunk_keys(int team) { return team > 1 ? 32 : 16; }
 
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
 // Grid: blocks of WARPS warps, WARPS / TEAM teams each; the warps of a team share its ring, each with NT
-// tiles of the pair's rows.
-template <int NT, int TEAM>
+// tiles of the pair's rows.  PAIR: clusters, each with a pair (y: sequence, x: head and rank) whose chunks its
+// blocks share; else blocks with equal shares of the line.
+template <int NT, int TEAM, bool PAIR>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kernel(const __grid_constant__ Params p) {
   constexpr int TEAMS = WARPS / TEAM, CK = chunk_keys(TEAM);
   constexpr int TILE_BYTES = CK * HD * 2, STAGE_BYTES = 2 * TILE_BYTES;  // K or V, and both
@@ -375,7 +391,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_all[TEAMS * STAGES];
   __shared__ uint32_t read_all[TEAMS * STAGES];  // how often a warp was done with the stage
-  pdl_launch_dependents();  // the join waits for this grid's end before it reads
+  if (!PAIR) pdl_launch_dependents();  // the join waits for this grid's end before it reads
   const int warp = warp_id(), lane = lane_id();
   const int r = lane >> 2, t = lane & 3;
   const int G = p.group, Hk = p.num_kv_heads;
@@ -391,41 +407,57 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
   __syncthreads();
 
   // ---- this block's run [c0, c0 + count) of the line, and the sequence that c0 lies in (each warp for itself)
-  int64_t total = 0;
-  for (int i = lane; i < p.num_seqs; i += 32) {
-    const int len = __ldg(p.context_lens + i);
-    if (blockIdx.x == 0 && warp == 0 && len > p.max_len) record_error(VLC_DEV_ERR_LENGTH);
-    total += span_of(len).count;
-  }
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-  total *= Hk;
-  const Shares shares(total, p.num_blocks);
-  const int64_t c0 = shares.first(blockIdx.x);
-  const int count = (int)shares.count(blockIdx.x);
-  if (count == 0) return;
-  int seq = 0;
-  int64_t at = c0;  // c0's place among the chunks from the sequence's first on
-  for (int base = 0;; base += 32) {
-    int64_t n = base + lane < p.num_seqs ? (int64_t)span_of(__ldg(p.context_lens + base + lane)).count * Hk : 0;
-    int64_t upto = n;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += x;
+  int seq = 0, head = 0, j0 = 0, count = 0;
+  int64_t c0 = 0;
+  Span span;
+  const Shares shares = [&] {
+    if constexpr (PAIR) {
+      seq = blockIdx.y;
+      head = blockIdx.x / p.cluster;
+      const int len = __ldg(p.context_lens + seq), rank = (int)cluster_ctarank();
+      if (blockIdx.x == 0 && threadIdx.x == 0 && len > p.max_len) record_error(VLC_DEV_ERR_LENGTH);
+      span = span_of(len);
+      j0 = (int)((int64_t)span.count * rank / p.cluster);
+      count = (int)((int64_t)span.count * (rank + 1) / p.cluster) - j0;
+      return Shares(0, 1);
     }
-    const uint32_t past = __ballot_sync(0xffffffffu, upto > at);
-    if (past) {
-      const int first = __ffs(past) - 1;
-      seq = base + first;
-      at -= __shfl_sync(0xffffffffu, upto - n, first);
-      break;
+    int64_t total = 0;
+    for (int i = lane; i < p.num_seqs; i += 32) {
+      const int len = __ldg(p.context_lens + i);
+      if (blockIdx.x == 0 && warp == 0 && len > p.max_len) record_error(VLC_DEV_ERR_LENGTH);
+      total += span_of(len).count;
     }
-    at -= __shfl_sync(0xffffffffu, upto, 31);
-    if (base + 32 >= p.num_seqs) return;  // not reached: c0 < total
-  }
-  Span span = span_of(__ldg(p.context_lens + seq));
-  int head = (int)(at / span.count), j0 = (int)(at - (int64_t)head * span.count);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    const Shares all(total * Hk, p.num_blocks);
+    c0 = all.first(blockIdx.x);
+    count = (int)all.count(blockIdx.x);
+    int64_t at = c0;  // c0's place among the chunks from the sequence's first on
+    for (int base = 0; count > 0 && base < p.num_seqs; base += 32) {
+      const int64_t n = base + lane < p.num_seqs ? (int64_t)span_of(__ldg(p.context_lens + base + lane)).count * Hk : 0;
+      int64_t upto = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += x;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, upto > at);
+      if (past) {
+        const int first = __ffs(past) - 1;
+        seq = base + first;
+        at -= __shfl_sync(0xffffffffu, upto - n, first);
+        break;
+      }
+      at -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    span = span_of(__ldg(p.context_lens + seq));
+    if (count > 0) {
+      head = (int)(at / span.count);
+      j0 = (int)(at - (int64_t)head * span.count);
+    }
+    return all;
+  }();
+  if (!PAIR && count == 0) return;
 
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const ring = smem + team * (STAGES * STAGE_BYTES);
@@ -498,12 +530,12 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
   State<NT, CK, Q_SMEM> state;
   int i = 0;        // the team's chunks so far
   bool ok = true;   // its waits so far: a team that gave up takes no more chunks
-  for (int done = 0, first_slot = 0; done < count; first_slot = 1) {
+  for (int done = 0, first_slot = 0; PAIR || done < count; first_slot = 1) {
     // ---- the pair's chunks [done, done + n) of the run
-    const int n = min(span.count - j0, count - done);
+    const int n = PAIR ? count : min(span.count - j0, count - done);
     // The block with a pair's first chunk notes where its parts will be: one for each block up to that
     // of its last chunk, in slot 0 but for this block's.
-    if (j0 == 0 && threadIdx.x == 0)
+    if (!PAIR && j0 == 0 && threadIdx.x == 0)
       p.places[(int64_t)seq * Hk + head] = make_int2((int)blockIdx.x * 2 + first_slot,
                                                      (int)(shares.block_of(c0 + done + span.count - 1) - blockIdx.x) + 1);
     state.start(p, seq, head, row0, r, t, q_smem);
@@ -536,16 +568,73 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
     // ---- the teams' sums: the upper half of the warps hand theirs over until one team has them
 #pragma unroll
     for (int half = WARPS / 2; half >= TEAM; half /= 2) {
-      float4* const to = sums + (warp % half) * (9 * 32);
+      float4* const to = sums + (warp % half) * (NT * 9 * 32);
+      __syncthreads();
+      if (warp >= half && warp < 2 * half) {
 #pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        __syncthreads();
-        if (warp >= half && warp < 2 * half) state.put(x, to, lane);
-        __syncthreads();
-        if (warp < half) state.add(x, to, lane);
+        for (int x = 0; x < NT; ++x) state.put(x, to + x * (9 * 32), lane);
+      }
+      __syncthreads();
+      if (warp < half) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x) state.add(x, to + x * (9 * 32), lane);
       }
     }
-    if (team == 0) {
+    if constexpr (PAIR) {
+      // ---- the blocks' sums: each block leaves its in its shared memory and adds some dims of all of them
+      if (!ok && lane == 0) {  // (copies still in flight are given more time before the sums take their place)
+        for (; i < issued; ++i) arrived(i);
+      }
+      __syncthreads();
+      float4* const own = reinterpret_cast<float4*>(smem);
+      if (team == 0) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x) state.put(x, own + (mate * NT + x) * (9 * 32), lane);
+      }
+      cluster_sync();
+      for (int tile = warp; tile * 8 < p.rows; tile += WARPS) {
+        const uint32_t at = smem_u32(own + tile * (9 * 32) + lane);
+        for (int mt = (int)cluster_ctarank(); mt < 8; mt += p.cluster) {
+          float4 ml[8], v[8];
+#pragma unroll
+          for (int b = 0; b < 8; ++b) {
+            if (b >= p.cluster) continue;
+            const uint32_t from = mapa_shared(at, b);
+            ml[b] = ld_cluster_v4(from + 8 * 32 * 16);
+            v[b] = ld_cluster_v4(from + mt * 32 * 16);
+          }
+          float m0 = NO_MAX, m1 = NO_MAX, l0 = 0.f, l1 = 0.f;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int b = 0; b < 8; ++b) {
+            if (b >= p.cluster) continue;
+            m0 = fmaxf(m0, ml[b].x);
+            m1 = fmaxf(m1, ml[b].y);
+          }
+#pragma unroll
+          for (int b = 0; b < 8; ++b) {
+            if (b >= p.cluster) continue;
+            const float f0 = fast_exp2(ml[b].x - m0), f1 = fast_exp2(ml[b].y - m1);
+            l0 = fmaf(ml[b].z, f0, l0);
+            l1 = fmaf(ml[b].w, f1, l1);
+            o = make_float4(fmaf(v[b].x, f0, o.x), fmaf(v[b].y, f1, o.y), fmaf(v[b].z, f0, o.z), fmaf(v[b].w, f1, o.w));
+          }
+          const float inv0 = l0 != 0.f ? 1.f / l0 : 0.f, inv1 = l1 != 0.f ? 1.f / l1 : 0.f;  // (NaN stays NaN)
+#pragma unroll
+          for (int odd = 0; odd < 2; ++odd) {
+            const int row = tile * 8 + 2 * t + odd, tok = p.token_of(row);
+            if (row >= p.rows) continue;
+            __nv_bfloat16* dst = p.out + ((int64_t)seq * p.tokens + tok) * p.out_token_stride +
+                                 ((int64_t)head * G + row - tok * G) * HD + r + 16 * mt;
+            dst[0] = __float2bfloat16(odd ? o.y * inv1 : o.x * inv0);
+            dst[8] = __float2bfloat16(odd ? o.w * inv1 : o.z * inv0);
+          }
+        }
+      }
+      cluster_sync();  // the others have read this block's sums
+      return;
+    }
+    if (!PAIR && team == 0) {
       const bool whole = j0 == 0 && n == span.count;
       const int64_t slot = ((int64_t)blockIdx.x * 2 + first_slot) * p.rows;
 #pragma unroll
@@ -555,7 +644,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
         if (row >= p.rows) continue;
         const float sum = state.l[nt][odd];
         if (whole) {
-          const int tok = row / G;
+          const int tok = p.token_of(row);
           const float inv = sum != 0.f ? 1.f / sum : 0.f;  // (NaN stays NaN)
           __nv_bfloat16* dst = p.out + ((int64_t)seq * p.tokens + tok) * p.out_token_stride +
                                ((int64_t)head * G + row - tok * G) * HD + r;
@@ -629,7 +718,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
     place = make_int2(0, 1);  // (not reached: every pair with keys is noted)
   const int count = place.y;
   if (count == 1) return;  // written by its block
-  const int tok = row / p.group;
+  const int tok = p.token_of(row);
   uint2* const dst = reinterpret_cast<uint2*>(p.out + ((int64_t)seq * p.tokens + tok) * p.out_token_stride +
                                               ((int64_t)head * p.group + row - tok * p.group) * HD) + lane;
   // part i > 0 is in slot 0 of the block i after the first's
@@ -686,15 +775,37 @@ static Shape shape_of(int rows) {
   return {4, 4};
 }
 
+// Most chunks that any sequence has under the host's bound.
+static int64_t most_chunks(int CK, int tokens, int max_context_len, int window, int sinks) {
+  const int64_t chunks = ((int64_t)max_context_len + CK - 1) / CK;
+  if (window == 0) return chunks;
+  return std::min(chunks, ((int64_t)sinks + CK - 1) / CK + ((int64_t)window + tokens + CK - 2) / CK + 1);
+}
+
+// Blocks of the cluster that takes a pair, or 0 for the line.  The line's shares are even whatever the lengths
+// are, and its blocks many where the pairs are few; a pair's cluster saves the second launch.  Pair : line, us, of
+// 16 query and 2 KV heads, one token (five): one sequence of 500 keys 6.3 : 8.0 (10.6 : 11.2), of 2000 7.8 : 9.9
+// (13.7 : 15.1), of 4000 9.9 : 9.6 (17.7 : 15.0), of 8000 14.3 : 10.6 (25.8 : 15.7); eight of 4000 11.1 : 13.1
+// (20.7 : 22.1); sixteen of 8000 26.2 : 30.8 (35.0 : 40.8); 64 of 4000 46.3 : 48.4 (59.7 : 61.0).  So a team takes
+// up to 8 chunks, or 16 where the clusters fill half of the GPU (beyond that ragged lengths would leave it idle).
+static int cluster_of(int num_seqs, int num_kv_heads, int rows, int tokens, int max_context_len, int window, int sinks,
+                      int num_sms) {
+  const Shape shape = shape_of(rows);
+  const int64_t pairs = (int64_t)num_seqs * num_kv_heads, resident = (int64_t)num_sms * BLOCKS_PER_SM;
+  int cluster = 8;
+  while (cluster > 1 && pairs * cluster > resident) cluster /= 2;
+  const int64_t chunks = most_chunks(shape.keys(), tokens, max_context_len, window, sinks);
+  const int64_t most = (2 * pairs * cluster >= resident ? 16 : 8) * cluster * (WARPS / shape.team);
+  return cluster > 1 && chunks <= most ? cluster : 0;
+}
+
 // Blocks of the grid: from host values only, so that it is fixed for graph capture.  A block has at least
 // MIN_CHUNKS for each of its teams: few chunks, but fewer parts to join.
 constexpr int MIN_CHUNKS = 2;
 static int grid_blocks(int num_seqs, int num_kv_heads, int rows, int tokens, int max_context_len, int window, int sinks,
                        int num_sms) {
   const Shape shape = shape_of(rows);
-  const int CK = shape.keys();
-  int64_t chunks = ((int64_t)max_context_len + CK - 1) / CK;
-  if (window > 0) chunks = std::min(chunks, ((int64_t)sinks + CK - 1) / CK + ((int64_t)window + tokens + CK - 2) / CK + 1);
+  const int64_t chunks = most_chunks(shape.keys(), tokens, max_context_len, window, sinks);
   const int least = MIN_CHUNKS * (WARPS / shape.team);
   const int64_t most = (num_seqs * num_kv_heads * chunks + least - 1) / least;
   return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)num_sms * BLOCKS_PER_SM, most));
@@ -715,10 +826,27 @@ static bool sizes_ok(int num_seqs, int tokens, int num_heads, int num_kv_heads, 
 
 template <int NT, int TEAM>
 static int launch(const Params& p, cudaStream_t st) {
-  static std::atomic<uint64_t> smem{0};
-  if (ensure_dynamic_smem((const void*)window_decode_kernel<NT, TEAM>, SMEM_BYTES, smem) != VLC_OK) return VLC_ERR_CUDA;
-  window_decode_kernel<NT, TEAM><<<p.num_blocks, WARPS * 32, SMEM_BYTES, st>>>(p);
-  return launch_status();
+  static std::atomic<uint64_t> smem[2];
+  const bool pair = p.cluster > 0;
+  const auto kernel = pair ? window_decode_kernel<NT, TEAM, true> : window_decode_kernel<NT, TEAM, false>;
+  if (ensure_dynamic_smem((const void*)kernel, smem_bytes(NT), smem[pair]) != VLC_OK) return VLC_ERR_CUDA;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = pair ? dim3(p.cluster * p.num_kv_heads, p.num_seqs) : dim3(p.num_blocks);
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = smem_bytes(NT);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pair ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return VLC_ERR_CUDA;
+  }
+  return VLC_OK;
 }
 
 }  // namespace decode_window
@@ -732,8 +860,10 @@ extern "C" int64_t vlc_decode_window_workspace_size(int num_seqs, int num_tokens
   if (num_seqs <= 0 || !sizes_ok(num_seqs, num_tokens, num_heads, num_kv_heads, max_context_len, window, sinks)) return 0;
   const int64_t rows = (int64_t)num_heads / num_kv_heads * num_tokens;
   if (rows > MAX_ROWS) return 0;
-  const int blocks = grid_blocks(num_seqs, num_kv_heads, (int)rows, num_tokens, std::max(1, max_context_len), window, sinks,
-                               vlc_num_sms());
+  const int sms = vlc_num_sms();
+  max_context_len = std::max(1, max_context_len);
+  if (cluster_of(num_seqs, num_kv_heads, (int)rows, num_tokens, max_context_len, window, sinks, sms)) return 0;
+  const int blocks = grid_blocks(num_seqs, num_kv_heads, (int)rows, num_tokens, max_context_len, window, sinks, sms);
   return workspace_bytes_for(blocks, (int)rows, (int64_t)num_seqs * num_kv_heads);
 }
 
@@ -759,9 +889,12 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
   const int sms = vlc_num_sms(), rows = G * num_tokens;
   const Shape shape = shape_of(rows);
   const int blocks = grid_blocks(num_seqs, num_kv_heads, rows, num_tokens, max_context_len, window, sinks, sms);
-  if (!workspace || workspace_bytes < workspace_bytes_for(blocks, rows, (int64_t)num_seqs * num_kv_heads))
-    return VLC_ERR_WORKSPACE;
-  if (!aligned16(workspace)) return VLC_ERR_ALIGN;
+  const int cluster = cluster_of(num_seqs, num_kv_heads, rows, num_tokens, max_context_len, window, sinks, sms);
+  if (!cluster) {
+    if (!workspace || workspace_bytes < workspace_bytes_for(blocks, rows, (int64_t)num_seqs * num_kv_heads))
+      return VLC_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return VLC_ERR_ALIGN;
+  }
 
   Params p;
   const uint8_t* caches[2] = {(const uint8_t*)k_cache, (const uint8_t*)v_cache};
@@ -795,8 +928,10 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
   p.window = window;
   p.sinks = window > 0 ? sinks : 0;
   p.group = G;
+  p.group_inverse = (65536 + G - 1) / G;
   p.num_kv_heads = num_kv_heads;
   p.rows = rows;
+  p.cluster = cluster;
   p.scale_log2 = std::max(std::fabs(softmax_scale) * 1.4426950408889634f, std::numeric_limits<float>::min());
   p.q_flip = softmax_scale < 0.f ? 0x80008000u : 0u;
   p.out = (__nv_bfloat16*)out;
@@ -818,7 +953,7 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
     case 32 + 3: rc = launch<3, 4>(p, st); break;
     default: rc = launch<4, 4>(p, st);
   }
-  if (rc != VLC_OK) return rc;
+  if (rc != VLC_OK || cluster) return rc;
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
   const bool spread = blocks / pairs + 1 > 10;
   cudaLaunchConfig_t cfg{};
