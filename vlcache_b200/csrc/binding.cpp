@@ -132,6 +132,16 @@ void check(const char* function, int status) {
 
 at::TensorOptions like(const Tensor& t, at::ScalarType type) { return at::TensorOptions().dtype(type).device(t.device()); }
 
+// A tensor of a part of a buffer, from byte `at` on (a multiple of the type's size): one allocation for several
+// outputs, each some 1 us on the host.
+Tensor part(const Tensor& buffer, int64_t at, at::ScalarType type, at::IntArrayRef sizes) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(),
+                                                      c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
 // ---- the ops
 PyObject* decode_attention_window(PyObject* const* a) {
   const Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k_cache"), &v = tensor(a[2], "v_cache"),
@@ -203,9 +213,16 @@ PyObject* step_metadata(PyObject* const* a) {
   const int block = bounded(a[5], "block_size", 1, 0x7fffffff), rows = bounded(a[6], "total_rows", 0, 1 << 30);
   const int window = bounded(a[7], "window", 0, 1 << 30), sinks = bounded(a[8], "sinks", 0, 1 << 30);
   const On on(device);
-  const at::TensorOptions i32 = like(lens, at::kInt);
-  Tensor positions = at::empty({rows}, like(lens, at::kLong)), slots = at::empty({rows}, i32);
-  Tensor cu_q = at::empty({b + 1}, i32), cu_k = at::empty({b + 1}, i32), after = at::empty({b}, i32);
+  int64_t at = 0;
+  const int64_t rows16 = (rows + 3) / 4 * 4;
+  const Tensor buffer = at::empty({rows16 * 12 + (3 * b + 2) * 4}, like(lens, at::kByte));
+  auto next = [&](at::ScalarType type, int64_t n, int64_t room) {
+    const Tensor t = part(buffer, at, type, {n});
+    at += room * (int64_t)c10::elementSize(type);
+    return t;
+  };
+  const Tensor positions = next(at::kLong, rows, rows16), slots = next(at::kInt, rows, rows16);
+  const Tensor cu_q = next(at::kInt, b + 1, b + 1), cu_k = next(at::kInt, b + 1, b + 1), after = next(at::kInt, b, b);
   check("vlc_step_metadata",
         vlc_step_metadata(context_lens, new_lens, (int)b, t.data, t.stride, t.width, block, window, sinks,
                           const_cast<int32_t*>(free_pages), (int)pages.numel(), const_cast<int32_t*>(num_free),
@@ -248,7 +265,8 @@ PyObject* verify_drafts(PyObject* const* a) {
   need(u_last.scalar_type() == at::kFloat && u_last.dim() == 1 && u_last.size(0) == b && u_last.is_contiguous(), "u_last",
        "contiguous fp32 [" + std::to_string(b) + "]");
   const On on(device);
-  Tensor tokens = at::empty({b, n + 1}, like(drafts, at::kLong)), emitted = at::empty({b}, like(drafts, at::kInt));
+  const Tensor buffer = at::empty({b * ((n + 1) * 8 + 4)}, like(drafts, at::kByte));
+  const Tensor tokens = part(buffer, 0, at::kLong, {b, n + 1}), emitted = part(buffer, b * (n + 1) * 8, at::kInt, {b});
   check("vlc_verify_drafts",
         vlc_verify_drafts((const int64_t*)drafts.data_ptr(), drafts.stride(0), (int)b, (int)n, target.data_ptr(), p.seq,
                           p.row, draft.defined() ? draft.data_ptr() : nullptr, q.seq, q.row, p.vocab, p.type,

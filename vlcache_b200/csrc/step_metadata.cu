@@ -7,9 +7,12 @@
 //     (p + 1) block <= L_i - window + 1, go back to the end of the list in the same order.
 //   * Every new row gets its position and its slot, table[t / block] * block + t % block.
 // The work is a few integer operations a row; what counts is latency.  So it is one launch: a cluster of
-// blocks shares the sequences, counts, joins the counts through its blocks' shared memory, fills the
-// tables and then writes the rows, with cluster barriers in between (pages are taken before any is
-// given back into the same places).
+// blocks shares the sequences, counts, joins the counts through its blocks' shared memory and fills the
+// tables, with a cluster barrier before pages go back (into the places that pages are taken from).  Rows of
+// a few tokens a sequence are written by the warp that has just filled its table; where a sequence takes
+// more, all warps share all rows behind a barrier, four a lane.  Many rows (whole prompts) are written by
+// a second launch over all SMs, a programmatic dependent: 64 prompts of up to 10,617 tokens in NEW us,
+// by the cluster alone in 24.
 #include <algorithm>
 #include <climits>
 
@@ -23,6 +26,8 @@ constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_BLOCKS = 8;
 constexpr int MAX_LEN = 1 << 30;
+constexpr int MANY_ROWS = 16384;  // of a step, for the second launch
+constexpr int FEW_ROWS = 64;  // of a sequence, that its warp writes by itself
 
 struct Params {
   const int32_t* context_lens;
@@ -40,6 +45,7 @@ struct Params {
   int32_t* cu_q;
   int32_t* cu_k;
   int32_t* new_context_lens;
+  bool rows_apart;  // rows are written by the second launch
 };
 
 // What a sequence's step is made of: its tokens, the pages of the new ones, and the pages behind the
@@ -49,10 +55,10 @@ struct Seq {
   int first, last;    // pages of the new rows, cut to the table
   int gone0, gone1;   // pages behind the window
 };
-__device__ __forceinline__ Seq seq_of(const Params& p, int i) {
+__device__ __forceinline__ Seq seq_of(const Params& p, int2 lens) {  // context and new lengths
   Seq s;
-  s.len = __ldg(p.context_lens + i);
-  s.fresh = max(0, __ldg(p.new_lens + i));
+  s.len = lens.x;
+  s.fresh = max(0, lens.y);
   if (s.len < 0) s.len = s.fresh = 0;  // an idle place of the batch
   if (s.len > MAX_LEN || s.fresh > MAX_LEN) {
     record_error(VLC_DEV_ERR_LENGTH);
@@ -71,20 +77,92 @@ __device__ __forceinline__ int ld_cluster_i32(uint32_t addr) {
   return v;
 }
 
-enum : int { kNeed = 0, kGone = 1, kRows = 2, kKeys = 3, kCounts = 4 };
+enum : int { kNeed = 0, kGone = 1, kRows = 2, kKeys = 3, kMany = 4, kCounts = 5 };  // kMany: sequences of many rows
 
-// Dynamic shared memory: [kCounts][per_block] counts of the block's sequences, then their exclusive sums.
+// Slot of position t, -1 where the table has no page there.
+__device__ __forceinline__ int32_t slot_at(const Params& p, int number, int t, int page) {
+  const int64_t at = (int64_t)number * p.block_size + (t - page * p.block_size);
+  if (number >= 0 && at > INT_MAX) record_error(VLC_DEV_ERR_SLOT_RANGE);
+  return number >= 0 && at <= INT_MAX ? (int32_t)at : -1;
+}
+
+// Positions and slots of rows, from the sums and the tables that are in memory.
+struct Rows {
+  const Params& p;
+  const int rows;  // of all sequences
+  int seq = -1, begin = 0, end = 0, len = 0;
+  const bool aligned;
+  __device__ __forceinline__ Rows(const Params& p, int rows)
+      : p(p), rows(rows),
+        aligned((reinterpret_cast<uintptr_t>(p.positions) % 32 | reinterpret_cast<uintptr_t>(p.slots) % 16) == 0) {}
+  __device__ __forceinline__ void take(int s) {
+    seq = s;
+    begin = p.cu_q[s];
+    end = p.cu_q[s + 1];
+    len = p.new_context_lens[s] - (end - begin);
+  }
+  // Rows r .. r + n - 1 (n up to 4; r a multiple of 4, and not below that of the call before).
+  __device__ __forceinline__ void write(int64_t r, int n) {
+    if (r < rows && seq < 0) {  // the last sequence that begins at or before the first row
+      int lo = 0, hi = p.num_seqs - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.cu_q[mid] <= r) lo = mid;
+        else hi = mid - 1;
+      }
+      take(lo);
+    }
+    int page = -1, first = 0, number = -1;  // of the row before, and the page's first position
+    int32_t position[4] = {0, 0, 0, 0}, slot[4] = {-1, -1, -1, -1};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (r + x >= rows) continue;
+      if (r + x >= end) {
+        while (r + x >= end && seq + 1 < p.num_seqs) take(seq + 1);
+        page = -1;
+      }
+      const int t = len + (int)(r + x - begin);
+      if (page < 0 || t - first >= p.block_size) {
+        page = t / p.block_size;
+        first = page * p.block_size;
+        number = (uint32_t)page < (uint32_t)p.width ? p.block_tables[seq * p.table_stride + page] : -1;
+      }
+      position[x] = t;
+      slot[x] = slot_at(p, number, t, page);
+    }
+    if (n == 4 && aligned) {
+      const uint32_t wide[8] = {(uint32_t)position[0], 0, (uint32_t)position[1], 0,
+                                (uint32_t)position[2], 0, (uint32_t)position[3], 0};
+      st_global_v8(p.positions + r, wide);
+      *reinterpret_cast<int4*>(p.slots + r) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (x >= n) continue;
+        p.positions[r + x] = position[x];
+        p.slots[r + x] = slot[x];
+      }
+    }
+  }
+};
+
+// Dynamic shared memory: the block's sequences' lengths, [kCounts][per_block] counts of them, then their exclusive sums.
 __global__ void __launch_bounds__(THREADS) step_metadata_kernel(const Params p, int per_block) {
-  extern __shared__ int counts[];
+  extern __shared__ int2 lens[];
+  int* const counts = reinterpret_cast<int*>(lens + per_block);
   __shared__ int totals[kCounts];
+  if (p.rows_apart) pdl_launch_dependents();
   const int rank = (int)cluster_ctarank(), blocks = gridDim.x;
   const int warp = warp_id(), lane = lane_id();
   const int seq0 = rank * per_block, mine = max(0, min(per_block, p.num_seqs - seq0));
   const int num_free = min(max(0, __ldg(p.num_free)), p.free_capacity);  // (written behind the last barrier)
 
+  for (int i = threadIdx.x; i < mine; i += THREADS)
+    lens[i] = make_int2(__ldg(p.context_lens + seq0 + i), __ldg(p.new_lens + seq0 + i));
+  __syncthreads();
   // ---- counts of each sequence, a warp each
   for (int i = warp; i < mine; i += WARPS) {
-    const Seq s = seq_of(p, seq0 + i);
+    const Seq s = seq_of(p, lens[i]);
     const int32_t* table = p.block_tables + (seq0 + i) * p.table_stride;
     int need = 0, gone = 0;
     for (int x = s.first + lane; x < s.last; x += 32) need += table[x] < 0;
@@ -96,6 +174,7 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(const Params p, 
       counts[kGone * per_block + i] = gone;
       counts[kRows * per_block + i] = s.fresh;
       counts[kKeys * per_block + i] = s.len + s.fresh;
+      counts[kMany * per_block + i] = s.fresh > FEW_ROWS;
     }
   }
   __syncthreads();
@@ -117,21 +196,24 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(const Params p, 
     if (lane == 0) totals[warp] = before;
   }
   cluster_sync();
-  int base[kCounts] = {0, 0, 0, 0}, total[kCounts] = {0, 0, 0, 0};
-  for (int b = 0; b < blocks; ++b) {
-    const uint32_t at = mapa_shared(smem_u32(totals), b);
+  int base[kCounts], total[kCounts];
+  {  // lane b: block b's
+    const uint32_t at = mapa_shared(smem_u32(totals), min(lane, blocks - 1));
+    int v[kCounts];
+#pragma unroll
+    for (int k = 0; k < kCounts; ++k) v[k] = ld_cluster_i32(at + 4 * k);
 #pragma unroll
     for (int k = 0; k < kCounts; ++k) {
-      const int v = ld_cluster_i32(at + 4 * k);
-      if (b < rank) base[k] += v;
-      total[k] += v;
+      total[k] = (int)__reduce_add_sync(0xffffffffu, (unsigned)(lane < blocks ? v[k] : 0));
+      base[k] = (int)__reduce_add_sync(0xffffffffu, (unsigned)(lane < rank ? v[k] : 0));
     }
   }
   const int taken = min(total[kNeed], num_free);
+  const bool shared_rows = p.rows_apart || total[kMany] > 0;
 
   // ---- missing pages, lengths and their running sums
   for (int i = warp; i < mine; i += WARPS) {
-    const Seq s = seq_of(p, seq0 + i);
+    const Seq s = seq_of(p, lens[i]);
     int32_t* table = p.block_tables + (seq0 + i) * p.table_stride;
     int nth = base[kNeed] + counts[kNeed * per_block + i];
     for (int x0 = s.first; x0 < s.last; x0 += 32) {
@@ -144,8 +226,19 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(const Params p, 
       }
       nth += __popc(who);
     }
+    const int q = base[kRows] + counts[kRows * per_block + i];
+    if (!shared_rows) {
+      __syncwarp();  // (the lanes' entries are there)
+      for (int r = lane; r < s.fresh; r += 32) {
+        const int t = s.len + r, page = t / p.block_size;
+        if (q + r < p.total_rows) {
+          p.positions[q + r] = t;
+          p.slots[q + r] = slot_at(p, page < p.width ? table[page] : -1, t, page);
+        }
+      }
+    }
     if (lane == 0) {
-      const int q = base[kRows] + counts[kRows * per_block + i], k = base[kKeys] + counts[kKeys * per_block + i];
+      const int k = base[kKeys] + counts[kKeys * per_block + i];
       p.cu_q[seq0 + i] = q;
       p.cu_k[seq0 + i] = k;
       p.new_context_lens[seq0 + i] = s.len + s.fresh;
@@ -158,12 +251,13 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(const Params p, 
     if (total[kNeed] > num_free || num_free - taken + total[kGone] > p.free_capacity) record_error(VLC_DEV_ERR_PAGES);
     if (total[kRows] > p.total_rows) record_error(VLC_DEV_ERR_LENGTH);
   }
-  cluster_sync();  // every page is taken, every table filled
+  // Every page is taken, every table filled; and the sums of this block have been read.
+  cluster_sync();
 
   // ---- pages behind the window
   if (p.window > 0) {
     for (int i = warp; i < mine; i += WARPS) {
-      const Seq s = seq_of(p, seq0 + i);
+      const Seq s = seq_of(p, lens[i]);
       int32_t* table = p.block_tables + (seq0 + i) * p.table_stride;
       int nth = num_free - taken + base[kGone] + counts[kGone * per_block + i];
       for (int x0 = s.gone0; x0 < s.gone1; x0 += 32) {
@@ -181,45 +275,23 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(const Params p, 
   }
   if (rank == 0 && threadIdx.x == 0) *p.num_free = min(num_free - taken + total[kGone], p.free_capacity);
 
-  // ---- rows: a warp takes a run of them
-  const int rows = min(total[kRows], p.total_rows);
-  const int warps = blocks * WARPS;
-  const int run = ((p.total_rows + warps - 1) / warps + 31) / 32 * 32;
-  const int64_t r0 = (int64_t)(rank * WARPS + warp) * run;
-  int seq = 0, begin = 0, end = 0, len = 0;
-  if (r0 < rows) {  // the last sequence that begins at or before the lane's first row
-    const int row = min((int)r0 + lane, rows - 1);
-    int lo = 0, hi = p.num_seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (p.cu_q[mid] <= row) lo = mid;
-      else hi = mid - 1;
-    }
-    seq = lo;
-    begin = p.cu_q[seq];
-    end = p.cu_q[seq + 1];
-    len = p.new_context_lens[seq] - (end - begin);
-  }
-  for (int64_t r = r0 + lane; r < r0 + run && r < p.total_rows; r += 32) {
-    int64_t position = 0;
-    int32_t slot = -1;
-    if (r < rows) {
-      while (r >= end && seq + 1 < p.num_seqs) {
-        begin = end;
-        end = p.cu_q[++seq + 1];
-        len = p.new_context_lens[seq] - (end - begin);
-      }
-      const int t = len + (int)(r - begin);
-      const int page = t / p.block_size;
-      position = t;
-      const int number = (uint32_t)page < (uint32_t)p.width ? p.block_tables[seq * p.table_stride + page] : -1;
-      const int64_t at = (int64_t)number * p.block_size + (t - page * p.block_size);
-      if (number >= 0 && at <= INT_MAX) slot = (int32_t)at;
-      else if (number >= 0) record_error(VLC_DEV_ERR_SLOT_RANGE);
-    }
-    p.positions[r] = position;
-    p.slots[r] = slot;
-  }
+  // ---- rows behind the last, and all rows where a sequence has many: a warp takes a run of them, a lane four at once
+  if (p.rows_apart) return;
+  const int rows = min(max(total[kRows], 0), p.total_rows);
+  const int from = shared_rows ? 0 : rows / 4 * 4, warps = blocks * WARPS;
+  const int run = ((p.total_rows - from + warps - 1) / warps + 127) / 128 * 128;
+  const int64_t r0 = from + (int64_t)(rank * WARPS + warp) * run, r1 = min(r0 + run, (int64_t)p.total_rows);
+  Rows at(p, rows);
+  for (int64_t r = r0 + lane * 4; r < r1; r += 128) at.write(r, (int)min(r1 - r, (int64_t)4));
+}
+
+// Many rows: a thread four of them.
+__global__ void __launch_bounds__(THREADS) step_rows_kernel(const Params p) {
+  pdl_wait();  // the tables and sums are the launch before's
+  const int64_t r = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * 4;
+  if (r >= p.total_rows) return;
+  Rows at(p, min(max(p.cu_q[p.num_seqs], 0), p.total_rows));
+  at.write(r, (int)min(p.total_rows - r, (int64_t)4));
 }
 
 }  // namespace step_meta
@@ -262,13 +334,14 @@ extern "C" int vlc_step_metadata(const int32_t* context_lens, const int32_t* new
   p.cu_q = cu_seqlens_q;
   p.cu_k = cu_seqlens_k;
   p.new_context_lens = new_context_lens;
+  p.rows_apart = total_rows > MANY_ROWS;
   // A block a sequence for each of its warps, or for as many rows as its threads write at once.
   int blocks = 1;
-  while (blocks < MAX_BLOCKS && (num_seqs > blocks * WARPS || total_rows > blocks * THREADS)) blocks *= 2;
+  while (blocks < MAX_BLOCKS && (num_seqs > blocks * WARPS || (!p.rows_apart && total_rows > blocks * THREADS))) blocks *= 2;
   const int per_block = (num_seqs + blocks - 1) / blocks;
-  const int bytes = kCounts * per_block * (int)sizeof(int);
+  const int bytes = (kCounts + 2) * per_block * (int)sizeof(int);
   static std::atomic<uint64_t> smem{0};
-  if (ensure_dynamic_smem((const void*)step_metadata_kernel, kCounts * ((65535 + MAX_BLOCKS - 1) / MAX_BLOCKS) * 4,
+  if (ensure_dynamic_smem((const void*)step_metadata_kernel, (kCounts + 2) * ((65535 + MAX_BLOCKS - 1) / MAX_BLOCKS) * 4,
                           smem) != VLC_OK)
     return VLC_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
@@ -284,6 +357,15 @@ extern "C" int vlc_step_metadata(const int32_t* context_lens, const int32_t* new
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, step_metadata_kernel, (const Params)p, per_block) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return VLC_ERR_CUDA;
+  }
+  if (!p.rows_apart) return VLC_OK;
+  cfg.gridDim = dim3((unsigned)(((int64_t)total_rows + 4 * THREADS - 1) / (4 * THREADS)));
+  cfg.dynamicSmemBytes = 0;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  if (cudaLaunchKernelEx(&cfg, step_rows_kernel, (const Params)p) != cudaSuccess) {
     (void)cudaGetLastError();
     return VLC_ERR_CUDA;
   }
