@@ -488,8 +488,8 @@ int vlc_remap_block_tables(int32_t* block_tables, int64_t row_stride, int num_ro
  *   recorded (VLC_DEV_ERR_BLOCK_RANGE), a length past max_context_len is cut to it and recorded
  *   (VLC_DEV_ERR_LENGTH).  Sizes come from host values, so the launches can be captured; workspace:
  *   vlc_decode_window_workspace_size bytes, 16-byte aligned, one per call in flight.
- * vlc_step_metadata: sequence i of context_lens[i] tokens (below 0: an idle place of the batch)
- *   takes new_lens[i] more.  Block-table entries below 0 where they fall are filled from the end
+ * vlc_step_metadata: sequence i of context_lens[i] tokens takes new_lens[i] more (below 0: an idle place
+ *   of the batch, whose rows have position 0 and slot -1, and which takes no page and has length 0 after).  Block-table entries below 0 where they fall are filled from the end
  *   of the free list (free_pages[0 .. *num_free), the k-th missing page of the batch being
  *   free_pages[*num_free - 1 - k], sequences in order), then pages wholly behind the window of
  *   the first new row and behind the sinks go back to its end, in order, and their entries become
@@ -505,7 +505,8 @@ int vlc_remap_block_tables(int32_t* block_tables, int64_t row_stride, int num_ro
  *   from max(target - draft, 0) at the refused draft, or from the target's row behind the last
  *   accepted one, at the random number u_last: probability x counts floor(clamp(x, 0, 1) 2^42), and
  *   the token is the first whose running count passes floor(floor(u_last 2^24) total / 2^24).
- *   tokens[seq] = accepted drafts, that token, -1 ..; emitted[seq] = accepted drafts + 1.  Without
+ *   tokens[seq] = accepted drafts, that token, -1 ..; emitted[seq] = accepted drafts + 1, which
+ *   context_lens[seq] (unless NULL, or below 0: an idle place) is moved on by.  Without
  *   draft_probs (NULL) a draft has probability 1, and refused it counts 0.  A difference without a
  *   positive value is replaced by the target's row; a row without one gives token -1.  target_probs
  *   [num_seqs][num_drafts + 1][vocab], draft_probs [num_seqs][num_drafts][vocab], strides in
@@ -532,7 +533,7 @@ int vlc_verify_drafts(const int64_t* drafts, int64_t draft_stride, int num_seqs,
                       const void* target_probs, int64_t target_seq_stride, int64_t target_row_stride,
                       const void* draft_probs, int64_t draft_seq_stride, int64_t draft_row_stride, int vocab, int dtype,
                       const float* u, int64_t u_stride, const float* u_last, int64_t* tokens, int32_t* emitted,
-                      void* stream);
+                      int32_t* context_lens, void* stream);
 
 #ifdef __cplusplus
 }

@@ -50,14 +50,13 @@ def step(context_lens, new_lens, tables, free_pages, num_free, block, total_rows
     tables, free = [list(t) for t in tables], list(free_pages)
     context = [max(n, 0) for n in context_lens]
     fresh = [0 if n < 0 else max(m, 0) for n, m in zip(context_lens, new_lens)]
+    rows = [max(m, 0) for m in new_lens]     # idle places (below 0) have rows too
     for table, n, m in zip(tables, context, fresh):
         for t in range(n, n + m):
             page = t // block
             if page < len(table) and table[page] < 0 and num_free > 0:
                 num_free -= 1
                 table[page] = free[num_free]
-            elif page < len(table) and table[page] < 0:
-                pass
     if window:
         for table, n in zip(tables, context):
             for page in range(len(table)):
@@ -67,12 +66,14 @@ def step(context_lens, new_lens, tables, free_pages, num_free, block, total_rows
                     num_free += 1
                     table[page] = -1
     positions, slots, cu_q, cu_k = [], [], [0], [0]
-    for table, n, m in zip(tables, context, fresh):
+    for table, n, m, k in zip(tables, context, fresh, rows):
         for t in range(n, n + m):
             page = table[t // block] if t // block < len(table) else -1
             positions.append(t)
             slots.append(page * block + t % block if page >= 0 else -1)
-        cu_q.append(cu_q[-1] + m)
+        positions += [0] * (k - m)
+        slots += [-1] * (k - m)
+        cu_q.append(cu_q[-1] + k)
         cu_k.append(cu_k[-1] + n + m)
     pad = max(0, total_rows - len(positions))
     return (positions[:total_rows] + [0] * pad, slots[:total_rows] + [-1] * pad, cu_q, cu_k,

@@ -65,15 +65,15 @@ def _decode(tables, lens, new, q, k_cache, v_cache, window, sinks, scale, **kw):
                                           window, sinks, **kw)
 
 
-def _check_decode(got, tables, lens, n, q, k_cache, v_cache, window, sinks, scale):
+def _check_decode(got, tables, lens, n, q, k_cache, v_cache, window, sinks, scale, scores=0.0):
     for i, m in enumerate(lens):
         k, v = (oracle.sequence_keys(c, tables[i], m) for c in (k_cache, v_cache))
         pos = torch.arange(m - n, m, device="cuda")
         want, rms = oracle.attention(q[i].double().view(n, -1, D), k, v, pos, window, sinks, scale)
         # P is off by STEP of itself in numerator and denominator alike: STEP * sum p |v - o| <= STEP * rms;
         # the output's rounding is STEP of it; fp32 scores and sums of up to 2^8 natural logs are off by less
-        # than 2^-12 of the terms.
-        tol = (STEP + 2.0 ** -12) * (rms + want.abs()) + 1e-30
+        # than 2^-12 of the terms.  `scores`: what scores are off by beyond that, and so the logarithms of P.
+        tol = (STEP + 2.0 ** -12) * (rms + want.abs()) + 2 * math.expm1(scores) * rms + 1e-30
         off = (got[i].double().view(n, -1, D) - want).abs()
         assert bool((off <= tol).all()), (i, m, float((off / tol).max()))
 
@@ -234,7 +234,7 @@ def test_step_metadata(b, most_new, longest, block, window, sinks):
     ops = _ops()
     r = np.random.default_rng(b + most_new)
     lens, new, tables, free, count = _step_case(r, b, most_new, longest, block, window, sinks)
-    total = sum(max(n, 0) for n, m in zip(new, lens) if m >= 0) + 5
+    total = sum(new) + 5
     want = oracle.step(lens, new, tables, free, count, block, total, window, sinks)
     i32 = dict(dtype=torch.int32, device="cuda")
     # a row stride of its own, with guards behind the tables' rows
@@ -279,3 +279,440 @@ def test_verify_drafts(dtype, b, k, vocab, sampled):
         want = oracle.verify(drafts[i].tolist(), p[i].cpu(), q[i].cpu() if sampled else None, u[i].tolist(),
                              float(u_last[i]))
         assert int(emitted[i]) == len(want) and tokens[i].tolist() == want + [-1] * (k + 1 - len(want))
+
+
+# ------------------------------------------------------------------ decode: what a call may bring
+def _small(seed=1, lens=(200, 70, 333), n=2, heads=16, kv_heads=2, block=64):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    lens = list(lens)
+    tables, pages = _tables(g, lens, block)
+    k_cache, v_cache = _caches(g, pages, block, kv_heads)
+    q = torch.randn(len(lens), n, heads, D, generator=g, device="cuda").to(torch.bfloat16)
+    return g, lens, tables, k_cache, v_cache, q
+
+
+@pytest.mark.parametrize("lens", [(200, 70, 333), (9000,) * 40])   # clusters, and the line of chunks
+def test_decode_window_strides_out_and_workspace(lens):
+    g, lens, tables, k_cache, v_cache, q = _small(lens=lens)
+    b, n, heads, _ = q.shape
+    want = _decode(tables, lens, None, q, k_cache, v_cache, 50, 3, 0.1)
+    rows = torch.full((b * n, 20 * D), math.nan, dtype=torch.bfloat16, device="cuda")   # a projection's rows
+    view = rows[:, :heads * D].view(b, n, heads, D)
+    view.copy_(q)
+    into = torch.full((b * n + 1, heads + 1, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = into[:b * n, :heads].view(b, n, heads, D)
+    need = _ops().decode_window_workspace_bytes(b, n, heads, 2, max(lens), 50, 3)
+    wide = torch.full((b, tables.shape[1] + 5), -3, dtype=torch.int32, device="cuda")
+    wide[:, :tables.shape[1]] = tables
+    got = _decode(wide[:, :tables.shape[1]], lens, None, view, k_cache, v_cache, 50, 3, 0.1, out=out,
+                  workspace=torch.empty(need + 16, dtype=torch.uint8, device="cuda"))
+    assert got.data_ptr() == out.data_ptr() and torch.equal(out, want)
+    assert bool((into[b * n:] == 7).all()) and bool((into[:, heads:] == 7).all())   # rows behind stay as they were
+    three = _decode(tables, lens, None, q[:, 1].contiguous(), k_cache, v_cache, 50, 3, 0.1)
+    assert three.shape == (b, heads, D)
+    _check_decode(three.unsqueeze(1), tables, lens, 1, q[:, 1:].contiguous(), k_cache, v_cache, 50, 3, 0.1)
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        got = _decode(tables, lens, None, q, k_cache, v_cache, 50, 3, 0.1)
+    other.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("scale", [0.3, -0.3, 0.0])
+def test_decode_window_scales_and_broken_queries(scale):
+    g, lens, tables, k_cache, v_cache, q = _small()
+    q[0, 1, 3, 5], q[1, 0, 0, 0], q[2, 1, 15, 127] = math.inf, math.nan, -math.inf
+    got = _decode(tables, lens, None, q, k_cache, v_cache, 40, 0, scale)
+    broken = ~torch.isfinite(q).all(-1)
+    assert int(broken.sum()) == 3 and bool(torch.isnan(got[broken]).all()) and bool(torch.isfinite(got[~broken]).all())
+    clean = torch.where(broken.unsqueeze(-1), torch.zeros_like(q), q)
+    got = torch.where(broken.unsqueeze(-1), _decode(tables, lens, None, clean, k_cache, v_cache, 40, 0, scale), got)
+    _check_decode(got, tables, lens, 2, clean, k_cache, v_cache, 40, 0, scale)
+
+
+def test_decode_window_large_scores():
+    """Scores that rise by some 2 a key to well over a thousand: the maximum keeps moving."""
+    g, lens, tables, k_cache, v_cache, q = _small(lens=(700,))
+    for j in range(700):
+        k_cache[tables[0, j // 64], j % 64] = q[0, 0, 0] * (j / 64)
+    got = _decode(tables, lens, None, q, k_cache, v_cache, 0, 0, 1.0)
+    # A score is a sum of 128 products in fp32, each sum off by 2^-24 of sum |q k| at most, then scaled in two
+    # roundings: 130 steps of it.
+    most = float(q[0].double().abs().sum(-1).max() * k_cache.double().abs().max())
+    most = min(most, float((q[0].double().abs() @ (q[0, 0, 0].double().abs() * 11)).max()) * 1.01)
+    _check_decode(got, tables, lens, 2, q, k_cache, v_cache, 0, 0, 1.0, scores=130 * 2.0 ** -24 * most)
+
+
+@pytest.mark.parametrize("lens", [(200, 70, 333), (9000,) * 40])
+def test_decode_window_bad_pages_and_lengths(lens):
+    ops = _ops()
+    g, lens, tables, k_cache, v_cache, q = _small(lens=lens)
+    pages = k_cache.shape[0]
+    for bad in (-1, pages, 1 << 30, -(1 << 31)):
+        broken = tables.clone()
+        broken[1, 0] = bad
+        got = _decode(broken, lens, None, q, k_cache, v_cache, 0, 0, 0.1)
+        assert ops.device_error() == 102
+        keys = k_cache.clone(), v_cache.clone()   # its keys count as zeros
+        for c in keys:
+            c[tables[1, 0].long()] = 0
+        _check_decode(got, tables, lens, 2, q, *keys, 0, 0, 0.1)
+    # a table too narrow for the length: the same
+    narrow = tables[:, :1].contiguous()
+    got = _decode(narrow, lens, None, q, k_cache, v_cache, 0, 0, 0.1)
+    assert ops.device_error() == 102 and bool(torch.isfinite(got).all())
+    # a length past the host's bound is cut to it
+    got = _decode(tables, lens, None, q, k_cache, v_cache, 30, 2, 0.1, bound=100)
+    assert ops.device_error() == 104
+    cut = [min(n, 100) for n in lens]
+    _check_decode(got, tables, cut, 2, q, k_cache, v_cache, 30, 2, 0.1)
+    lens_t = torch.tensor([-5] + lens[1:], dtype=torch.int32, device="cuda")
+    got = ops.decode_attention_window(q, k_cache, v_cache, tables, lens_t, max(lens), 0.1)
+    assert ops.device_error() == 0 and bool((got[0] == 0).all())
+
+
+def test_decode_window_no_sequences():
+    _, _, tables, k_cache, v_cache, q = _small()
+    got = _decode(tables[:0], [], None, q[:0], k_cache, v_cache, 8, 0, 0.1)
+    assert got.shape == (0, 2, 16, D)
+
+
+@pytest.mark.parametrize("lens", [(200, 70, 333), (6000,) * 40])
+def test_decode_window_captured(lens):
+    """Two graphs of their own workspaces, replayed in turn and at once, follow lengths and tables that change."""
+    g, lens, tables, k_cache, v_cache, q = _small(lens=lens)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qs, graphs, outs = [q, q.flip(0).contiguous()], [], []
+    for x in qs:
+        _ops().decode_attention_window(x, k_cache, v_cache, tables, lens_t, max(lens), 0.1, 60, 4)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_ops().decode_attention_window(x, k_cache, v_cache, tables, lens_t, max(lens), 0.1, 60, 4))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for cut in (0, 3, 64):
+        lens_t.copy_(torch.tensor([max(0, n - cut) for n in lens], dtype=torch.int32))
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for x, out in zip(qs, outs):
+            _check_decode(out, tables, [max(0, n - cut) for n in lens][:3], 2, x, k_cache, v_cache, 60, 4, 0.1)
+    assert _ops().device_error() == 0
+
+
+def test_decode_window_pages_beyond_4_gb():
+    """Pages whose byte offset passes 32 bits, the caches in either order."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pages, block, kv_heads = 9000, 256, 4
+    both = torch.empty(2, pages, block, kv_heads, D, dtype=torch.bfloat16, device="cuda")
+    both[:, -4:].normal_(generator=g)
+    tables = torch.tensor([[pages - 1, pages - 3], [pages - 2, pages - 4]], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 1, 28, D, generator=g, device="cuda").to(torch.bfloat16)
+    for k_cache, v_cache in ((both[0], both[1]), (both[1], both[0])):
+        got = _decode(tables, [400, 512], None, q, k_cache, v_cache, 300, 4, 0.1)
+        _check_decode(got, tables, [400, 512], 1, q, k_cache, v_cache, 300, 4, 0.1)
+
+
+# ------------------------------------------------------------------ step: what goes wrong
+def test_step_metadata_without_room():
+    ops = _ops()
+    i32 = dict(dtype=torch.int32, device="cuda")
+
+    def step(lens, new, tables, free, count, total, **kw):
+        a = [torch.tensor(x, **i32) for x in (lens, new, tables, free, [count])]
+        return ops.step_metadata(*a, 4, total, **kw), a
+    # two pages for three that are missing: the last sequence's slots are -1
+    got, a = step([3, 0], [2, 5], [[5, -1], [-1, -1]], [9, 8, 7], 2, 7)
+    assert ops.device_error() == 105 and got[1].tolist() == [23, 32, 36, 37, 38, 39, -1] and int(a[4]) == 0
+    assert a[2].tolist() == [[5, 8], [9, -1]] and got[0].tolist() == [3, 4, 0, 1, 2, 3, 4]
+    # past the table
+    got, a = step([7], [3], [[5, 6]], [9], 1, 3)
+    assert ops.device_error() == 102 and got[1].tolist() == [27, -1, -1] and int(a[4]) == 1
+    # fewer rows than the step has
+    got, a = step([0, 0], [2, 2], [[-1], [-1]], [9, 8], 2, 3)
+    assert ops.device_error() == 104 and got[1].tolist() == [32, 33, 36] and got[2].tolist() == [0, 2, 4]
+    # a free list that is full takes nothing more
+    got, a = step([9], [0], [[1, 2, 3]], [4, 5], 2, 0, window=1)
+    assert ops.device_error() == 105 and a[3].tolist() == [4, 5] and a[2].tolist() == [[-1, -1, 3]] and int(a[4]) == 2
+    # slots past 32 bits
+    got, a = step([0], [1], [[1 << 30]], [9], 0, 1)
+    assert ops.device_error() == 101 and got[1].tolist() == [-1]
+    # idle places have rows; negative new lengths are none
+    got, a = step([-1, 2, -7, 4], [2, -3, 1, 1], [[-1], [1], [-1], [-1]], [9], 1, 5)
+    assert ops.device_error() == 102 and got[0].tolist() == [0, 0, 0, 4, 0] and got[1].tolist() == [-1] * 5
+    assert got[2].tolist() == [0, 2, 2, 3, 4] and got[4].tolist() == [0, 2, 0, 5]
+    # no sequences
+    got = ops.step_metadata(*(torch.empty(n, **i32) for n in ((0,), (0,), (0, 4), (2,))), torch.zeros(1, **i32), 4, 3)
+    assert ops.device_error() == 0 and got[0].tolist() == [0] * 3 and got[1].tolist() == [-1] * 3 and got[2].tolist() == [0]
+
+
+def test_step_metadata_many_rows_of_idle_places():
+    """The second launch (many rows) with idle places, empty ones and rows to spare."""
+    ops = _ops()
+    r = np.random.default_rng(5)
+    lens = [int(x) for x in r.integers(0, 300, 40)]
+    new = [int(x) for x in r.integers(0, 900, 40)]
+    for i in (0, 7, 39):
+        lens[i] = -1
+    new[3] = new[38] = 0
+    tables = [[-1] * 40 for _ in lens]
+    free = r.permutation(1700).tolist()
+    for t, n in zip(tables, lens):
+        for p in range((max(n, 0) + 31) // 32):
+            t[p] = free.pop()
+    count = len(free)
+    free += [0] * 300
+    total = sum(new) + 4097
+    want = oracle.step(lens, new, tables, free, count, 32, total, 100, 4)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    a = [torch.tensor(x, **i32) for x in (lens, new, tables, free, [count])]
+    got = ops.step_metadata(*a, 32, total, 100, 4)
+    assert ops.device_error() == 0
+    for x, w in zip(got + (a[2], a[3], a[4]), want[:7] + ([want[7]],)):
+        assert x.tolist() == w
+
+
+# ------------------------------------------------------------------ verification: what goes wrong
+def _verify_one(drafts, p, q, u, u_last, dtype=torch.float32):
+    p = torch.tensor([p], dtype=dtype, device="cuda")
+    q = None if q is None else torch.tensor([q], dtype=dtype, device="cuda")
+    k = len(drafts)
+    got = _ops().verify_drafts(torch.tensor([drafts], dtype=torch.int64, device="cuda").view(1, k), p, q,
+                               torch.tensor([u], dtype=torch.float32, device="cuda").view(1, k),
+                               torch.tensor([u_last], dtype=torch.float32, device="cuda"))
+    want = oracle.verify(drafts, p[0].cpu(), None if q is None else q[0].cpu(), torch.tensor(u).tolist(),
+                         float(torch.tensor(u_last)))
+    assert int(got[1]) == len(want) and got[0][0].tolist() == want + [-1] * (k + 1 - len(want))
+    return want
+
+
+def test_verify_drafts_borders():
+    half = [0.5, 0.5, 0.0]
+    assert _verify_one([], [half], None, [], 0.5) == [1]                   # half of the counts belong to token 0
+    assert _verify_one([], [half], None, [], 0.5 - 2.0 ** -24) == [0]
+    assert _verify_one([], [[0.0, 0.25, 0.0, 0.75]], None, [], 0.0) == [1]  # the first with any weight
+    assert _verify_one([0], [half, half], [half], [1.0 - 2.0 ** -24], 0.0) == [0, 0]   # equal: accepted below 1
+    assert _verify_one([2], [half, half], [half], [0.0], 0.9) == [1]      # 0 < 0 does not hold, and p - q is 0: p
+    assert _verify_one([0], [[0.25, 0.5, 0.25], half], None, [0.25], 0.0) == [1]      # 0.25 < 0.25 does not hold
+    assert _verify_one([0], [[0.25, 0.5, 0.25], half], None, [0.2499], 0.0) == [0, 0]
+    assert _verify_one([1], [[1.0, 0.0], half[:2]], [[0.0, 1.0]], [0.0], 0.99) == [0]
+    assert _verify_one([0, 1], [half, half, half], [half, half], [0.1, 0.1], 0.7) == [0, 1, 1]
+    assert _verify_one([0, -1, 1], [half] * 4, None, [0.1, 0.1, 0.1], 0.7) == [0, 1]   # -1 ends the drafts
+
+
+def test_verify_drafts_rows_that_are_no_probabilities():
+    nan, inf = math.nan, math.inf
+    assert _verify_one([], [[nan, -1.0, 0.5, inf]], None, [], 0.2) == [2]   # NaN and below 0 count 0, above 1 as 1
+    assert _verify_one([], [[nan, -1.0, 0.5, inf]], None, [], 0.9) == [3]
+    assert _verify_one([], [[0.0, 0.0]], None, [], 0.5) == [-1]
+    assert _verify_one([], [[nan, nan]], None, [], 0.5) == [-1]
+    assert _verify_one([1], [[0.0, nan], [0.5, 0.5]], [[0.5, 0.5]], [0.5], 0.5) == [-1]
+    assert _verify_one([0], [[nan, 1.0], [0.5, 0.5]], [[0.5, 0.5]], [0.5], 0.5) == [1]   # NaN accepts nothing
+    for u in (1.0, 2.0, inf):
+        assert _verify_one([], [[0.5, 0.5]], None, [], u) == [1]
+    for u in (-0.5, nan, -inf):
+        assert _verify_one([], [[0.5, 0.5]], None, [], u) == [0]
+    assert _verify_one([], [[1e-30, 2.0 ** -42, 2.0 ** -43]], None, [], 0.9) == [1]   # what counts below one is nothing
+    assert _ops().device_error() == 0
+
+
+def test_verify_drafts_past_the_vocabulary():
+    ops = _ops()
+    p = torch.full((2, 3, 5), 0.2, device="cuda")
+    drafts = torch.tensor([[1, 5], [1 << 40, 0]], device="cuda")
+    tokens, emitted = ops.verify_drafts(drafts, p, None, torch.zeros(2, 2, device="cuda"), torch.zeros(2, device="cuda"))
+    assert ops.device_error() == 106 and emitted.tolist() == [2, 1] and tokens.tolist() == [[1, 0, -1], [0, -1, -1]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("vocab", [1, 2, 7, 8, 9, 15, 16, 17, 1023, 8191, 8193, 1 << 18])
+def test_verify_drafts_alignments(dtype, vocab):
+    """Rows that begin at every place of a 16-byte word, p's and q's alike and apart; every token can come."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    b, k = 9, 1
+    for apart in (0, 1):
+        room = vocab + 16
+        big_p = torch.full((b, k + 1, room), math.nan, dtype=dtype, device="cuda")
+        big_q = torch.full((b, k, room), math.nan, dtype=dtype, device="cuda")
+        drafts = torch.randint(0, vocab, (b, k), generator=g, device="cuda")
+        u, u_last = torch.rand(b, k, generator=g, device="cuda"), torch.rand(b, generator=g, device="cuda")
+        u_last[0], u_last[1] = 0.0, 1 - 2.0 ** -24   # the first and the last token that have weight
+        flat = torch.full((2, vocab), 1 / vocab, device="cuda")
+        for shift in range(8):
+            p, q = big_p[..., shift:shift + vocab], big_q[..., (shift + apart) % 8:(shift + apart) % 8 + vocab]
+            p.copy_(_probabilities(g, b, k + 1, vocab, dtype))
+            p[:2] = flat.to(dtype)
+            q.copy_(_probabilities(g, b, k, vocab, dtype))
+            for draft in (q, None):
+                tokens, emitted = ops.verify_drafts(drafts, p, draft, u, u_last)
+                some = range(b) if vocab < 10000 else range(0, 3)
+                for i in some:
+                    want = oracle.verify(drafts[i].tolist(), p[i].cpu(), None if draft is None else draft[i].cpu(),
+                                         u[i].tolist(), float(u_last[i]))
+                    assert tokens[i, :len(want)].tolist() == want and int(emitted[i]) == len(want)
+            if vocab > 10000 and shift == 2:
+                break
+    assert ops.device_error() == 0
+
+
+def test_verify_drafts_many_sequences_and_lengths():
+    """More sequences than clusters fit at once, lengths moved on in place, the call captured."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    b, k, vocab = 700, 2, 900
+    p, q = _probabilities(g, b, k + 1, vocab, torch.float32), _probabilities(g, b, k, vocab, torch.float32)
+    drafts = torch.randint(0, vocab, (b, k), generator=g, device="cuda")
+    u, u_last = torch.rand(b, k, generator=g, device="cuda") ** 4, torch.rand(b, generator=g, device="cuda")
+    lens = torch.arange(-2, b - 2, dtype=torch.int32, device="cuda")
+    before = lens.clone()
+    tokens, emitted = ops.verify_drafts(drafts, p, q, u, u_last, lens)
+    assert torch.equal(lens, torch.where(before < 0, before, before + emitted))
+    for i in range(0, b, 7):
+        want = oracle.verify(drafts[i].tolist(), p[i].cpu(), q[i].cpu(), u[i].tolist(), float(u_last[i]))
+        assert tokens[i].tolist() == want + [-1] * (k + 1 - len(want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.verify_drafts(drafts, p, q, u, u_last)
+    p.copy_(p.flip(0)), q.copy_(q.flip(0)), drafts.copy_(drafts.flip(0)), u.copy_(u.flip(0)), u_last.copy_(u_last.flip(0))
+    graph.replay()
+    assert torch.equal(out[0], tokens.flip(0)) and torch.equal(out[1], emitted.flip(0))
+    empty = ops.verify_drafts(drafts[:0], p[:0], q[:0], u[:0], u_last[:0])
+    assert empty[0].shape == (0, k + 1) and empty[1].shape == (0,)
+
+
+# ------------------------------------------------------------------ a run of them together
+class _Model:
+    """Two attention layers over embeddings of the tokens, one with a sliding window; logits from their outputs."""
+
+    def __init__(self, seed, vocab=97, heads=8, kv_heads=2, window=40, sinks=3, all_windowed=True):
+        from vlcache_b200.layers.attention import Attention
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.heads, self.kv_heads, self.vocab = heads, kv_heads, vocab
+        self.embed = torch.randn(vocab, (heads + 2 * kv_heads) * D, generator=g, device="cuda").to(torch.bfloat16)
+        self.head = torch.randn(heads * D, vocab, generator=g, device="cuda") * 0.08
+        self.layers = [Attention(heads, D, 0.1, kv_heads, window, sinks),
+                       Attention(heads, D, 0.1, kv_heads, window if all_windowed else None, sinks)]
+
+    def rows(self, tokens, positions):
+        x = self.embed[tokens.clamp(min=0)] * (1 + 0.1 * torch.sin(positions)).unsqueeze(-1).to(torch.bfloat16)
+        x = x.view(-1, self.heads + 2 * self.kv_heads, D)
+        return x[:, :self.heads], x[:, self.heads:-self.kv_heads], x[:, -self.kv_heads:]
+
+    def caches(self, pages, block):
+        for i, layer in enumerate(self.layers):
+            layer.k_cache, layer.v_cache = (torch.zeros(pages, block, self.kv_heads, D, dtype=torch.bfloat16, device="cuda")
+                                            for _ in range(2))
+
+    def __call__(self, tokens, positions):
+        q, k, v = self.rows(tokens, positions)
+        o = sum(layer(q, k.contiguous(), v.contiguous()).reshape(-1, self.heads * D).float() for layer in self.layers)
+        return torch.softmax(o @ self.head, -1)
+
+    def plain(self, tokens):
+        """Probabilities behind each token of one sequence, from 64-bit attention over all of it."""
+        pos = torch.arange(len(tokens), device="cuda")
+        q, k, v = (x.double() for x in self.rows(torch.tensor(tokens, device="cuda"), pos))
+        o = sum(oracle.attention(q, k, v, pos, l.sliding_window, l.num_sinks, 0.1)[0] for l in self.layers)
+        return torch.softmax(o.flatten(1) @ self.head.double(), -1)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("all_windowed", [True, False])
+def test_draft_decode_together(captured, all_windowed):
+    """Prompts through the windowed prefill, then steps of drafts: what is emitted is what each sequence alone, by
+    64-bit attention over all of its tokens, gives its probabilities to; pages go back and are used again."""
+    from vlcache_b200.engine.draft_decode import DraftDecode
+    from vlcache_b200.engine.page_pool import PagePool
+    from vlcache_b200.utils.context import reset_context, set_context
+    ops = _ops()
+    block, places, drafts_n = 32, 4, 3
+    model = _Model(7, all_windowed=all_windowed)
+    pool = PagePool(200, block)
+    model.caches(200, block)
+    window = 40 if all_windowed else 0
+    d = DraftDecode(pool, places, 16, drafts_n, window, 3 if window else 0)
+    assert d.lend(40)
+    r = np.random.default_rng(4)
+    histories = {0: [int(x) for x in r.integers(0, 97, 50)], 1: [int(x) for x in r.integers(0, 97, 7)],
+                 3: [int(x) for x in r.integers(0, 97, 133)]}
+
+    def prompt(place, tokens):
+        table = pool.allocate(pool.pages_for(len(tokens)))
+        n = len(tokens)
+        slots = torch.tensor([table[t // block] * block + t % block for t in range(n)], dtype=torch.int32, device="cuda")
+        cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        # this layer stack has no residual path, so one call fills every layer's cache
+        set_context(True, cu, cu, n, n, slots, None, None, cu_seqlens_q_host=[0, n], cu_seqlens_k_host=[0, n])
+        probs = model(torch.tensor(tokens, device="cuda"), torch.arange(n, device="cuda"))
+        want = model.plain(tokens)
+        assert float((probs.double() - want).abs().max()) < 0.05
+        d.admit(place, table, n)
+        return int(probs[-1].argmax())
+
+    last = {p: prompt(p, h) for p, h in histories.items()}
+    tokens_in = torch.zeros(places, drafts_n + 1, dtype=torch.int64, device="cuda")
+    u, u_last = torch.zeros(places, drafts_n, device="cuda"), torch.zeros(places, device="cuda")
+
+    def step():
+        positions = d.begin()
+        probs = model(tokens_in.flatten(), positions).view(places, drafts_n + 1, -1)
+        return (probs,) + d.finish(tokens_in[:, 1:].contiguous(), probs, None, u, u_last)
+
+    graph = None
+    for turn in range(14):
+        guess = torch.full((places, drafts_n + 1), -1, dtype=torch.int64)
+        for p in histories:   # drafts: the right ones up to somewhere, then others
+            row, good = [last[p]], int(r.integers(0, drafts_n + 1))
+            for i in range(drafts_n):
+                best = int(model.plain(histories[p] + row)[-1].argmax())
+                row.append(best if i < good else int(r.integers(0, 97)))
+            guess[p] = torch.tensor(row)
+        tokens_in.copy_(guess)
+        u.copy_(torch.tensor(r.random((places, drafts_n)) * 0.2, dtype=torch.float32))
+        u_last.copy_(torch.tensor(r.random(places), dtype=torch.float32))
+        lens = {p: len(h) for p, h in histories.items()}
+        if captured and graph is None:
+            saved = [t.clone() for t in (d.context_lens, d.block_tables, d.free_pages, d.num_free)]
+            step()   # what a first call sets up
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                probs, tokens, emitted = step()
+            for t, s in zip((d.context_lens, d.block_tables, d.free_pages, d.num_free), saved):
+                t.copy_(s)
+        if graph is not None:
+            graph.replay()
+        else:
+            probs, tokens, emitted = step()
+        assert ops.device_error() == 0
+        for p in histories:
+            want = model.plain(histories[p] + guess[p].tolist())[lens[p]:]
+            # An output is off by STEP * (2 rms + |o|) < 0.02 a layer, of either sign; a logit sums 512 of each of the
+            # two layers' (8 heads of 128, summed by pairs) times 0.08: 0.02 * 0.08 * sqrt(2048) = 0.07 would be
+            # the deviation if all were that far off, and a probability moves by a quarter of it at most.
+            assert float((probs[p].double() - want).abs().max()) < 0.05, (turn, p)
+            out = oracle.verify(guess[p, 1:].tolist(), probs[p].cpu(), None, u[p].tolist(), float(u_last[p]))
+            assert tokens[p].tolist() == out + [-1] * (drafts_n + 1 - len(out)) and int(emitted[p]) == len(out)
+            histories[p] += guess[p, :len(out)].tolist()
+            last[p] = out[-1]
+            assert int(d.context_lens[p]) == len(histories[p])
+        if window:   # pages wholly behind the window went back, the first stays (its sinks)
+            for p, h in histories.items():
+                live = [i for i, x in enumerate(d.block_tables[p].tolist()) if x >= 0]
+                gone = (lens[p] - window + 1) // block
+                assert 0 in live and all(i == 0 or i >= gone for i in live)
+        pages = [x for row in d.block_tables.tolist() for x in row if x >= 0] + d.free_pages[:int(d.num_free)].tolist()
+        assert len(pages) == len(set(pages))   # no page is twice in use
+        if turn == 8:   # one leaves, another comes
+            d.retire(0)
+            del histories[0]
+            histories[2] = [int(x) for x in r.integers(0, 97, 64)]
+            last[2] = prompt(2, histories[2])
+    for p in histories:
+        d.retire(p)
+    d.settle()
+    assert pool.num_free == 200 and pool.refs == [0] * 200
+    reset_context()

@@ -88,7 +88,7 @@ SIGNATURES: dict[str, tuple] = {
     "vlc_step_metadata": (c_int, [c_vp, c_vp, c_int, c_vp, c_i64, c_int, c_int, c_int, c_int, c_vp, c_int, c_vp, c_vp,
                                   c_vp, c_int, c_vp, c_vp, c_vp, c_vp]),
     "vlc_verify_drafts": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_int,
-                                  c_vp, c_i64, c_vp, c_vp, c_vp, c_vp]),
+                                  c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp]),
 }
 
 

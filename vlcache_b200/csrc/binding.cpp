@@ -68,7 +68,7 @@ double number(PyObject* o) {
 }
 
 // ---- checks
-// Index of the CUDA device that all the tensors (undefined: none given) are on.
+// Index of the CUDA device that all the tensors (undefined: none given) are on; the ops' last check.
 int device_of(const Tensor& first, std::initializer_list<const Tensor*> others) {
   const at::Device device = first.device();
   if (!device.is_cuda()) throw Refused("vlcache_b200 ops run on CUDA tensors only (no CPU fallback)");
@@ -147,7 +147,6 @@ PyObject* decode_attention_window(PyObject* const* a) {
   const Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k_cache"), &v = tensor(a[2], "v_cache"),
                &tables = tensor(a[3], "block_tables"), &lens = tensor(a[4], "context_lens");
   Tensor out = optional(a[9], "out"), workspace = optional(a[10], "workspace");
-  const int device = device_of(q, {&k, &v, &tables, &lens, &out, &workspace});
   const Rows r = rows_of(q, "q");
   need(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && k.dim() == 4 && k.sizes() == v.sizes() &&
            k.is_contiguous() && v.is_contiguous() && k.size(3) == r.dim,
@@ -159,19 +158,18 @@ PyObject* decode_attention_window(PyObject* const* a) {
   const int window = bounded(a[7], "window", 0, 1 << 30), sinks = bounded(a[8], "sinks", 0, 1 << 30);
   for (const int64_t n : {r.seqs, r.tokens, r.heads, r.dim, k.size(1), k.size(2)})
     need(n <= 0x7fffffff, "sizes below 2^31");
-  const On on(device);
   int64_t out_stride = r.heads * r.dim;
   if (out.defined()) {
     need(out.sizes() == q.sizes(), "out: q's shape");
     out_stride = rows_of(out, "out").stride;
-  } else {
-    out = at::empty(q.sizes(), like(q, at::kBFloat16));
   }
+  need(!workspace.defined() || workspace.is_contiguous(), "workspace: contiguous");
+  const On on(device_of(q, {&k, &v, &tables, &lens, &out, &workspace}));
+  if (!out.defined()) out = at::empty(q.sizes(), like(q, at::kBFloat16));
   const int64_t bytes = vlc_decode_window_workspace_size((int)r.seqs, (int)r.tokens, (int)r.heads, (int)k.size(2), max_len,
                                                          window, sinks);
   if (bytes > 0 && (!workspace.defined() || (int64_t)workspace.nbytes() < bytes))
     workspace = at::empty({bytes}, like(q, at::kByte));
-  need(!workspace.defined() || workspace.is_contiguous(), "workspace: contiguous");
   check("vlc_decode_attn_window",
         vlc_decode_attn_window(q.data_ptr(), r.stride, (int)r.seqs, (int)r.tokens, (int)r.heads, k.data_ptr(),
                                v.data_ptr(), k.size(0), (int)k.size(1), (int)k.size(2), (int)r.dim, t.data, t.stride,
@@ -201,7 +199,6 @@ PyObject* step_metadata(PyObject* const* a) {
   const Tensor &lens = tensor(a[0], "context_lens"), &fresh = tensor(a[1], "new_lens"),
                &tables = tensor(a[2], "block_tables"), &pages = tensor(a[3], "free_pages"),
                &count = tensor(a[4], "num_free");
-  const int device = device_of(lens, {&fresh, &tables, &pages, &count});
   const int64_t b = lens.numel();
   need(b <= 65535, "at most 65535 sequences");
   const int32_t* const context_lens = ints_of(lens, b, "context_lens");
@@ -212,7 +209,7 @@ PyObject* step_metadata(PyObject* const* a) {
   need(pages.numel() <= 0x7fffffff, "free_pages: too many");
   const int block = bounded(a[5], "block_size", 1, 0x7fffffff), rows = bounded(a[6], "total_rows", 0, 1 << 30);
   const int window = bounded(a[7], "window", 0, 1 << 30), sinks = bounded(a[8], "sinks", 0, 1 << 30);
-  const On on(device);
+  const On on(device_of(lens, {&fresh, &tables, &pages, &count}));
   int64_t at = 0;
   const int64_t rows16 = (rows + 3) / 4 * 4;
   const Tensor buffer = at::empty({rows16 * 12 + (3 * b + 2) * 4}, like(lens, at::kByte));
@@ -249,7 +246,7 @@ PyObject* verify_drafts(PyObject* const* a) {
   const Tensor &drafts = tensor(a[0], "drafts"), &target = tensor(a[1], "target_probs");
   const Tensor draft = optional(a[2], "draft_probs");
   const Tensor &u = tensor(a[3], "u"), &u_last = tensor(a[4], "u_last");
-  const int device = device_of(drafts, {&target, &draft, &u, &u_last});
+  const Tensor lens = optional(a[5], "context_lens");
   need(drafts.scalar_type() == at::kLong && drafts.dim() == 2, "drafts: int64 [sequences, drafts]");
   const int64_t b = drafts.size(0), n = drafts.size(1);
   need(b <= 65535 && n <= 31, "at most 65535 sequences and 31 drafts");
@@ -264,14 +261,16 @@ PyObject* verify_drafts(PyObject* const* a) {
        "u", "fp32 [" + std::to_string(b) + ", " + std::to_string(n) + "]");
   need(u_last.scalar_type() == at::kFloat && u_last.dim() == 1 && u_last.size(0) == b && u_last.is_contiguous(), "u_last",
        "contiguous fp32 [" + std::to_string(b) + "]");
-  const On on(device);
+  const int32_t* const context_lens = lens.defined() ? ints_of(lens, b, "context_lens") : nullptr;
+  const On on(device_of(drafts, {&target, &draft, &u, &u_last, &lens}));
   const Tensor buffer = at::empty({b * ((n + 1) * 8 + 4)}, like(drafts, at::kByte));
   const Tensor tokens = part(buffer, 0, at::kLong, {b, n + 1}), emitted = part(buffer, b * (n + 1) * 8, at::kInt, {b});
   check("vlc_verify_drafts",
         vlc_verify_drafts((const int64_t*)drafts.data_ptr(), drafts.stride(0), (int)b, (int)n, target.data_ptr(), p.seq,
                           p.row, draft.defined() ? draft.data_ptr() : nullptr, q.seq, q.row, p.vocab, p.type,
                           (const float*)u.data_ptr(), u.stride(0), (const float*)u_last.data_ptr(),
-                          (int64_t*)tokens.data_ptr(), (int32_t*)emitted.data_ptr(), on.stream));
+                          (int64_t*)tokens.data_ptr(), (int32_t*)emitted.data_ptr(),
+                          const_cast<int32_t*>(context_lens), on.stream));
   return tuple_of({tokens, emitted});
 }
 
@@ -324,7 +323,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef kMethods[] = {
     {"decode_attention_window", (PyCFunction)(void (*)(void))call<decode_attention_window, 11>, METH_FASTCALL, nullptr},
     {"step_metadata", (PyCFunction)(void (*)(void))call<step_metadata, 9>, METH_FASTCALL, nullptr},
-    {"verify_drafts", (PyCFunction)(void (*)(void))call<verify_drafts, 5>, METH_FASTCALL, nullptr},
+    {"verify_drafts", (PyCFunction)(void (*)(void))call<verify_drafts, 6>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -51,19 +51,20 @@ struct Params {
 // What a sequence's step is made of: its tokens, the pages of the new ones, and the pages behind the
 // window (as ranges of table entries).
 struct Seq {
-  int len, fresh;
+  int len, fresh;     // tokens it has, and that it takes
+  int rows;           // of the step: also an idle place's
   int first, last;    // pages of the new rows, cut to the table
   int gone0, gone1;   // pages behind the window
 };
 __device__ __forceinline__ Seq seq_of(const Params& p, int2 lens) {  // context and new lengths
   Seq s;
   s.len = lens.x;
-  s.fresh = max(0, lens.y);
-  if (s.len < 0) s.len = s.fresh = 0;  // an idle place of the batch
+  s.rows = s.fresh = max(0, lens.y);
   if (s.len > MAX_LEN || s.fresh > MAX_LEN) {
     record_error(VLC_DEV_ERR_LENGTH);
-    s.len = s.fresh = 0;
+    s.len = s.rows = s.fresh = 0;
   }
+  if (s.len < 0) s.len = s.fresh = 0;  // an idle place of the batch
   s.first = s.len / p.block_size;
   s.last = s.fresh > 0 ? min(p.width, (s.len + s.fresh - 1) / p.block_size + 1) : s.first;
   s.gone0 = (p.sinks + p.block_size - 1) / p.block_size;
@@ -122,6 +123,7 @@ struct Rows {
         page = -1;
       }
       const int t = len + (int)(r + x - begin);
+      if (t < 0) continue;  // an idle place's
       if (page < 0 || t - first >= p.block_size) {
         page = t / p.block_size;
         first = page * p.block_size;
@@ -172,9 +174,9 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(const Params p, 
     if (lane == 0) {
       counts[kNeed * per_block + i] = need;
       counts[kGone * per_block + i] = gone;
-      counts[kRows * per_block + i] = s.fresh;
+      counts[kRows * per_block + i] = s.rows;
       counts[kKeys * per_block + i] = s.len + s.fresh;
-      counts[kMany * per_block + i] = s.fresh > FEW_ROWS;
+      counts[kMany * per_block + i] = s.rows > FEW_ROWS;
     }
   }
   __syncthreads();
@@ -229,11 +231,12 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(const Params p, 
     const int q = base[kRows] + counts[kRows * per_block + i];
     if (!shared_rows) {
       __syncwarp();  // (the lanes' entries are there)
-      for (int r = lane; r < s.fresh; r += 32) {
+      for (int r = lane; r < s.rows; r += 32) {
         const int t = s.len + r, page = t / p.block_size;
+        const bool idle = s.fresh == 0;
         if (q + r < p.total_rows) {
-          p.positions[q + r] = t;
-          p.slots[q + r] = slot_at(p, page < p.width ? table[page] : -1, t, page);
+          p.positions[q + r] = idle ? 0 : t;
+          p.slots[q + r] = slot_at(p, !idle && page < p.width ? table[page] : -1, t, page);
         }
       }
     }

@@ -44,6 +44,7 @@ struct Params {
   const float* u_last;
   int64_t* tokens;   // [num_seqs][num_drafts + 1]
   int32_t* emitted;
+  int32_t* context_lens;  // null, or moved on by emitted (idle places, below 0, stay)
   int num_drafts, vocab;
   int tiles;         // of a warp
 };
@@ -334,6 +335,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) verify_kernel(const Pa
       int64_t* const out = a.tokens + (int64_t)seq * (a.num_drafts + 1);
       for (int i = 0; i <= a.num_drafts; ++i) out[i] = i < taken ? drafts[i] : i == taken ? token : -1;
       a.emitted[seq] = taken + 1;
+      if (a.context_lens && a.context_lens[seq] >= 0) a.context_lens[seq] += taken + 1;
     }
     return;
   }
@@ -369,7 +371,7 @@ extern "C" int vlc_verify_drafts(const int64_t* drafts, int64_t draft_stride, in
                                  const void* target_probs, int64_t target_seq_stride, int64_t target_row_stride,
                                  const void* draft_probs, int64_t draft_seq_stride, int64_t draft_row_stride, int vocab,
                                  int dtype, const float* u, int64_t u_stride, const float* u_last, int64_t* tokens,
-                                 int32_t* emitted, void* stream) {
+                                 int32_t* emitted, int32_t* context_lens, void* stream) {
   if (num_seqs < 0 || num_seqs > 65535 || num_drafts < 0 || vocab <= 0) return VLC_ERR_SHAPE;
   if (num_drafts > MAX_DRAFTS - 1 || vocab > MAX_VOCAB || dtype < 0 || dtype > 2) return VLC_ERR_UNSUPPORTED;
   if (num_seqs == 0) return VLC_OK;
@@ -389,6 +391,7 @@ extern "C" int vlc_verify_drafts(const int64_t* drafts, int64_t draft_stride, in
   a.u_last = u_last;
   a.tokens = tokens;
   a.emitted = emitted;
+  a.context_lens = context_lens;
   a.num_drafts = num_drafts;
   a.vocab = vocab;
   const int tile = dtype == 0 ? kTile<float> : kTile<__half>;

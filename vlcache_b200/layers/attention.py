@@ -16,6 +16,10 @@ A ``rotary_emb`` with several axes (``layers.rotary_embedding.MRotaryEmbedding``
 A 4-bit cache (``allocate_kv_cache(..., kv_format="fp4")``: ``k_cache`` / ``v_cache`` uint8) is
 written by vlc_rope_store_kvcache_fp4 / vlc_store_kvcache_fp4 and read by the 4-bit prefill
 and decode; ``k_scale`` / ``v_scale`` are its powers of two.
+``sliding_window`` / ``num_sinks`` (no counterpart in the reference): a row sees the last
+``sliding_window`` keys, its own among them, and the first ``num_sinks``; such layers, and decode
+steps of several tokens a sequence (``engine.draft_decode``), run vlc_decode_attn_window and
+windowed prefill plans, over a bf16 cache.
 ``forward(q, None, None)`` attends over a cache that already holds this step's K/V
 (stored by ``layers.linear.QKVParallelLinear.forward_rope_store``, which fuses the
 QKV projection, RoPE and the scatter).
@@ -49,9 +53,10 @@ def rope_store(positions, q, k, v, rotary_emb: nn.Module, attn: nn.Module, slot_
     return ops.rope_store_kvcache(positions, q, k, v, table, k_cache, v_cache, slot_mapping)
 
 
-def _prefill_plan(context: Context, num_heads: int, num_kv_heads: int, device: torch.device) -> ops.PrefillPlan:
-    """Plan once per step and cache it on the context (every layer shares it)."""
-    plan = context.prefill_plan
+def _prefill_plan(context: Context, num_heads: int, num_kv_heads: int, device: torch.device, window: int = 0,
+                  sinks: int = 0) -> ops.PrefillPlan:
+    """Plan once per step and cache it on the context (every layer of the same window shares it)."""
+    plan = context.window_plans.get((window, sinks)) if window else context.prefill_plan
     if plan is None:
         cq = context.cu_seqlens_q_host
         ck = context.cu_seqlens_k_host
@@ -60,8 +65,11 @@ def _prefill_plan(context: Context, num_heads: int, num_kv_heads: int, device: t
         if ck is None:
             ck = context.cu_seqlens_k.cpu().numpy()
         plan = ops.build_prefill_plan(np.asarray(cq), np.asarray(ck), num_heads, num_kv_heads,
-                                      device=device)
-        context.prefill_plan = plan
+                                      device=device, window=window, sinks=sinks)
+        if window:
+            context.window_plans[window, sinks] = plan
+        else:
+            context.prefill_plan = plan
     elif plan.dev is None or plan.dev.device != device:
         plan.dev = torch.from_numpy(plan.host).to(device)
     return plan
@@ -79,8 +87,12 @@ def _workspace(context: Context, nbytes: int, device: torch.device) -> torch.Ten
 
 class Attention(nn.Module):
 
-    def __init__(self, num_heads, head_dim, scale, num_kv_heads):
+    def __init__(self, num_heads, head_dim, scale, num_kv_heads, sliding_window=None, num_sinks=0):
         super().__init__()
+        if (sliding_window is not None and sliding_window <= 0) or num_sinks < 0:
+            raise ValueError("sliding_window must be positive (or None), num_sinks not negative")
+        self.sliding_window = int(sliding_window or 0)   # 0: every key is visible
+        self.num_sinks = int(num_sinks) if sliding_window else 0
         self.num_heads = num_heads
         self.head_dim = head_dim
         self.scale = scale
@@ -105,6 +117,14 @@ class Attention(nn.Module):
             torch.cuda.current_stream().wait_event(context.kv_ready[self.layer_id])
         have_cache = bool(k_cache.numel() and v_cache.numel()) and k is not None
         fp4 = k_cache.dtype == torch.uint8
+        tokens = 1   # of a sequence in a decode step
+        if not context.is_prefill and q.shape[0] > context.context_lens.numel():
+            tokens, rest = divmod(q.shape[0], max(1, context.context_lens.numel()))
+            if rest:
+                raise ValueError(f"decode: {q.shape[0]} rows for {context.context_lens.numel()} sequences")
+        windowed = self.sliding_window > 0 or tokens > 1
+        if fp4 and windowed:
+            raise ValueError("a 4-bit cache takes no sliding window and one token a sequence")
         if rotary_emb is not None:
             assert positions is not None, "rotary_emb needs the positions"
             if have_cache and (context.block_tables is not None or not context.is_prefill):
@@ -120,7 +140,8 @@ class Attention(nn.Module):
             store_kvcache(k, v, k_cache, v_cache, context.slot_mapping)
             stored_plain = True
         if context.is_prefill:
-            plan = _prefill_plan(context, self.num_heads, self.num_kv_heads, q.device)
+            plan = _prefill_plan(context, self.num_heads, self.num_kv_heads, q.device, self.sliding_window,
+                                 self.num_sinks)
             paged = context.block_tables is not None
             ws = _workspace(context, ops.prefill_fp4_workspace_bytes(plan, self.num_kv_heads) if fp4 and paged
                             else plan.workspace_bytes, q.device)
@@ -147,6 +168,15 @@ class Attention(nn.Module):
                 o = ops.decode_attention_fp4(q, k_cache, v_cache, context.block_tables, context.context_lens, max_len,
                                              self.scale, self.k_scale, self.v_scale, workspace=ws)
                 return o.unsqueeze(1)
+            if windowed:
+                seqs = q.shape[0] // tokens
+                q = q.unflatten(0, (seqs, tokens))
+                ws = _workspace(context, ops.decode_window_workspace_bytes(seqs, tokens, self.num_heads,
+                                                                           self.num_kv_heads, max_len,
+                                                                           self.sliding_window, self.num_sinks), q.device)
+                return ops.decode_attention_window(q, k_cache, v_cache, context.block_tables[:seqs],
+                                                   context.context_lens[:seqs], max_len, self.scale,
+                                                   self.sliding_window, self.num_sinks, workspace=ws)
             ws = _workspace(context, ops.decode_workspace_bytes(q.shape[0], self.num_heads, self.num_kv_heads,
                                                                 max_len), q.device)
             o = ops.decode_attention(q, k_cache, v_cache, context.block_tables, context.context_lens, max_len,

@@ -1000,8 +1000,9 @@ def step_metadata(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
                   free_pages: torch.Tensor, num_free: torch.Tensor, block_size: int, total_rows: int, window: int = 0,
                   sinks: int = 0) -> tuple[torch.Tensor, ...]:
     """Block tables and slot maps of a step, built on the device from the sequences' lengths, without a
-    host read (so that it can be captured): sequence i of ``context_lens[i]`` tokens (below 0: an idle
-    place of the batch) takes ``new_lens[i]`` more.
+    host read (so that it can be captured): sequence i of ``context_lens[i]`` tokens takes
+    ``new_lens[i]`` more (below 0: an idle place of the batch, whose rows have position 0 and slot -1,
+    and which takes no page and has length 0 after).
 
     Missing entries (below 0) of ``block_tables`` [B, width] where they fall are filled from the end of
     the free list (``free_pages[:num_free]``, sequences in order), then pages wholly behind the
@@ -1017,7 +1018,8 @@ def step_metadata(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
 
 
 def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, draft_probs: torch.Tensor | None,
-                  u: torch.Tensor, u_last: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+                  u: torch.Tensor, u_last: torch.Tensor,
+                  context_lens: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Speculative sampling's verification, from given random numbers: draft i of each sequence
     (``drafts`` int64 [B, K], -1 from a sequence's end on) is accepted iff ``u[b, i] * draft_probs[b, i,
     d] < target_probs[b, i, d]``, up to the first refusal; then one token is sampled at ``u_last[b]``, from
@@ -1027,6 +1029,8 @@ def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, draft_probs:
     bf16 or fp16); without ``draft_probs`` (drafts looked up, not sampled) a draft has probability 1,
     and refused it counts 0.  ``u`` [B, K] and ``u_last`` [B] are fp32 in [0, 1).  Returns (tokens int64
     [B, K + 1]: the accepted drafts, the sampled token, then -1; emitted int32 [B]: accepted + 1).
+    ``context_lens`` (int32 [B], when given) is moved on by emitted in place: the step's first token and
+    the accepted drafts are in the cache then (idle places, below 0, stay).
     Sums are whole numbers (include/vlcache_b200.h), so the answer is the same in every run and
     whatever the order of summation.  At most 31 drafts and 2^18 tokens of vocabulary."""
-    return (_compiled or _binding()).verify_drafts(drafts, target_probs, draft_probs, u, u_last)
+    return (_compiled or _binding()).verify_drafts(drafts, target_probs, draft_probs, u, u_last, context_lens)

@@ -13,10 +13,11 @@ keep working):
   * ``workspace``       — scratch tensor reused by every layer of the step;
   * ``kv_ready``        — per-layer CUDA events (``engine.kv_cache.copy_image_kv_per_layer``):
                           layer i's attention waits for event i before it reads the cache.
+``window_plans`` holds the prefill plans of layers with a sliding window, by (window, sinks).
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Any
 
 import torch
@@ -39,6 +40,7 @@ class Context:
     max_context_len: int | None = None
     workspace: torch.Tensor | None = None
     kv_ready: Any = None
+    window_plans: dict = field(default_factory=dict)
 
 
 _CONTEXT = Context()
