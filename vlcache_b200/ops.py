@@ -254,7 +254,7 @@ def build_prefill_plan(cu_seqlens_q, cu_seqlens_k, num_heads: int, num_kv_heads:
                                         1 if causal else 0, sms)
     if cap < 0:
         raise ValueError("invalid prefill metadata (cu_seqlens / heads)")
-    plan = np.zeros(int(cap), dtype=np.int32)
+    plan = np.empty(int(cap), dtype=np.int32)   # (the planner writes all that it uses; zeroing 15 MB took 0.7 ms)
     used = ctypes.c_int64(0)
     st = L.vlc_attention_plan_window(cq.ctypes.data, ck.ctypes.data, nseq, num_heads, num_kv_heads, head_dim,
                                      1 if causal else 0, int(window), int(sinks), sms, plan.ctypes.data, int(cap),
