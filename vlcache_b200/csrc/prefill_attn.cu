@@ -695,13 +695,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
         // Keys past the sequence end: zero their V rows so 0 * garbage stays 0.  Tile A
         // has every block of the unit, and its P*V runs first.  So with keys behind every window.
         const bool behind = kWindow && key0 < low_first && key0 + BN > p.sinks;
-        if ((kPacked || x == 0) && (key0 + BN > kv_len || behind)) {
+        const bool zero_v = (kPacked || x == 0) && (key0 + BN > kv_len || behind);
+        auto clear_v = [&]() {
           const int rb = kPacked ? ring0 : t;  // ring index of this block (tile A's count = the ring's)
           const int st = rb % STAGES;
-          if (!wait_or_abort(bars.v_full + st, (uint32_t)(rb / STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 11, abort_flag)) {
-            ok = false;
-            break;
-          }
+          if (!wait_or_abort(bars.v_full + st, (uint32_t)(rb / STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 11, abort_flag))
+            return false;
           if (key0 + row >= kv_len || (behind && key0 + row < low_first && key0 + row >= p.sinks)) {
             const uint4 z = make_uint4(0, 0, 0, 0);
             uint4* v0 = reinterpret_cast<uint4*>(smem + OFF_V + st * TILE_BYTES + row * 128);
@@ -713,6 +712,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
             }
           }
           fence_proxy_async_smem();
+          return true;
+        };
+        // (A window's first block is a unit's first, whose V is still on its way: there it is waited for only
+        // when the first half of P is there.)
+        if (!kWindow && zero_v && !clear_v()) {
+          ok = false;
+          break;
         }
         // P = exp2(s * scale_log2 - mref) as bf16 pairs: key pair (2c, 2c+1) goes to S
         // column c (its register is free: pair c reads registers 2c and 2c+1 >= c).  Each
@@ -754,8 +760,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
           }
           tmem_wait_st();
           tc_fence_before();
+          if (kWindow && half == 0 && zero_v && !clear_v()) ok = false;
           mbar_arrive(half == 0 ? bars.p_lo + x : bars.p_hi + x);
         }
+        if (kWindow && !ok) break;
         {
           float l0, l1;
           f2_unpack(lsum, l0, l1);
