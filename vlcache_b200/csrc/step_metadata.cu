@@ -11,8 +11,9 @@
 // tables, with a cluster barrier before pages go back (into the places that pages are taken from).  Rows of
 // a few tokens a sequence are written by the warp that has just filled its table; where a sequence takes
 // more, all warps share all rows behind a barrier, four a lane.  Many rows (whole prompts) are written by
-// a second launch over all SMs, a programmatic dependent: 64 prompts of up to 10,617 tokens in NEW us,
-// by the cluster alone in 24.
+// a second launch over all SMs, a programmatic dependent: 64 prompts of up to 10,617 tokens (295,000 rows) in
+// 8.5 us, by the cluster alone in 24.  What bounds it is the chain of dependent loads and barriers (lengths, table
+// entries, sums, pages, slots): 4.9 us for 8 sequences, 9.6 for 256 of five tokens under a window.
 #include <algorithm>
 #include <climits>
 

@@ -13,7 +13,11 @@
 // warp sums a run of the row, tile by tile, the next tile's loads in flight; the warps' sums are pushed to all
 // blocks of the cluster, and the block whose warp's run holds the token finds the tile by its kept sum and
 // reads that again (from L2), a thread a few values.  As many blocks a request as are resident at once: a
-// second wave would wait for its acceptance again.
+// second wave would wait for its acceptance again.  One request of 151,936 tokens takes 7.8 us (a chain of drafts,
+// their probabilities, the row, the cluster's sums and the tile), 64 with four drafts 16.2 (floor 10.0), 256
+// without draft probabilities, in bf16, 24 (floor 11.9: one block a request, 256 on 148 SMs).  With conversions to
+// whole numbers instead of the additions in 64-bit floating point 16.9 and 39; four blocks an SM (spilling) 18.0
+// and 25.4.
 #include <algorithm>
 #include <type_traits>
 
