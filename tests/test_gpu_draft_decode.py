@@ -716,3 +716,144 @@ def test_draft_decode_together(captured, all_windowed):
     d.settle()
     assert pool.num_free == 200 and pool.refs == [0] * 200
     reset_context()
+
+
+# ------------------------------------------------------------------ further calls that the documentation allows
+@pytest.mark.parametrize("lens", [(200, 70, 333), (9000,) * 40])
+def test_decode_window_in_place(lens):
+    """The output over the query."""
+    g, lens, tables, k_cache, v_cache, q = _small(lens=lens)
+    want = _decode(tables, lens, None, q, k_cache, v_cache, 70, 4, 0.1)
+    got = _decode(tables, lens, None, q, k_cache, v_cache, 70, 4, 0.1, out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(q, want)
+
+
+def test_decode_window_many_short_sequences():
+    g = torch.Generator(device="cuda").manual_seed(11)
+    lens = [int(x) for x in np.random.default_rng(1).integers(0, 40, 2500)]
+    tables, pages = _tables(g, lens, 32)
+    k_cache, v_cache = _caches(g, pages, 32, 1)
+    q = torch.randn(len(lens), 2, 8, D, generator=g, device="cuda").to(torch.bfloat16)
+    got = _decode(tables, lens, None, q, k_cache, v_cache, 9, 2, 0.1)
+    assert _ops().device_error() == 0
+    pick = list(range(0, 2500, 37))
+    _check_decode(got[pick], tables[pick], [lens[i] for i in pick], 2, q[pick], k_cache, v_cache, 9, 2, 0.1)
+    assert bool((got[[i for i, n in enumerate(lens) if n == 0]] == 0).all())
+
+
+@pytest.mark.parametrize("lens", [(500, 77), (20000, 9999)])
+def test_decode_window_one_cache_for_both(lens):
+    """Keys that are the values (one tensor): copied apart, since their distance is 0."""
+    g, lens, tables, k_cache, _, q = _small(lens=lens)
+    got = _decode(tables, lens, None, q, k_cache, k_cache, 0, 0, 0.1)
+    _check_decode(got, tables, lens, 2, q, k_cache, k_cache, 0, 0, 0.1)
+
+
+@pytest.mark.parametrize("head_dim", [80, 96, 128])
+def test_prefill_window_head_dims(head_dim):
+    """Contiguous keys and values of narrower heads, whole and split tiles."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(head_dim)
+    new, lens = [300, 9], [300, 5000]
+    cu_q, cu_k = np.cumsum([0] + new), np.cumsum([0] + lens)
+    q, k, v = (torch.randn(n, h, head_dim, generator=g, device="cuda").to(torch.bfloat16)
+               for n, h in ((309, 16), (5300, 2), (5300, 2)))
+    plan = ops.build_prefill_plan(cu_q, cu_k, 16, 2, head_dim, device="cuda", window=1500, sinks=4)
+    assert plan.num_parts > 0
+    got = ops.prefill_attention(q, k, v, None, plan, 0.1)
+    assert ops.device_error() == 0
+    for i, (n, m) in enumerate(zip(new, lens)):
+        want, rms = oracle.attention(q[cu_q[i]:cu_q[i + 1]].double(), k[cu_k[i]:cu_k[i + 1]].double(),
+                                     v[cu_k[i]:cu_k[i + 1]].double(), torch.arange(m - n, m, device="cuda"), 1500, 4, 0.1)
+        tol = (STEP + 2.0 ** -12) * (2 * rms + want.abs()) + 1e-30   # (as test_prefill_window)
+        assert bool(((got[cu_q[i]:cu_q[i + 1]].double() - want).abs() <= tol).all())
+
+
+def test_prefill_window_over_a_4_bit_cache_and_refusals():
+    """A windowed plan over keys read back from 4 bits is the one over those keys in bf16; scales that are not
+    positive are refused."""
+    ops = _ops()
+    from vlcache_b200._lib import VLCError
+    from vlcache_b200.layers.attention import Attention
+    from vlcache_b200.utils.context import reset_context, set_context
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n, block = 700, 128
+    k, v = (torch.randn(n, 2, D, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(300, 16, D, generator=g, device="cuda").to(torch.bfloat16)
+    k4, v4 = (torch.zeros(6, 2, block * 72, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ops.store_kvcache_fp4(k, v, k4, v4, torch.arange(n, dtype=torch.int32, device="cuda"))
+    tables = torch.arange(6, dtype=torch.int32, device="cuda").view(1, 6)
+    cu_k = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    plan = ops.build_prefill_plan([0, 300], [0, n], 16, 2, device="cuda", window=200, sinks=4)
+    a = ops.prefill_attention_fp4(q, k4, v4, tables, cu_k, plan, 0.1)
+    kb, vb = ops.gather_kvcache_fp4(k4, v4, tables, cu_k, n)
+    assert torch.equal(a, ops.prefill_attention(q, kb, vb, None, plan, 0.1)) and ops.device_error() == 0
+    for scale in (0.0, -0.1, math.nan):
+        with pytest.raises(VLCError):
+            ops.prefill_attention(q, kb, vb, None, plan, scale)
+    layer = Attention(16, D, 0.1, 2, 200)
+    layer.k_cache, layer.v_cache = k4, v4
+    set_context(False, slot_mapping=torch.full((1,), -1, dtype=torch.int32, device="cuda"), context_lens=cu_k[1:],
+                block_tables=tables)
+    with pytest.raises(ValueError, match="4-bit"):
+        layer(q[:1], k[:1], v[:1])
+    layer = Attention(16, D, 0.1, 2)
+    layer.k_cache, layer.v_cache = (torch.zeros(6, block, 2, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    set_context(False, slot_mapping=torch.full((3,), -1, dtype=torch.int32, device="cuda"),
+                context_lens=cu_k.clone(), block_tables=tables.expand(2, 6).contiguous())
+    with pytest.raises(ValueError, match="3 rows for 2 sequences"):
+        layer(q[:3], k[:3], v[:3])
+    reset_context()
+
+
+def test_prefill_window_plans_are_pairs(cuda_lib):
+    ops = _ops()
+    try:
+        ops.set_prefill_kernel(ops.PREFILL_QUADS)
+        plan = ops.build_prefill_plan([0, 700], [0, 900], 16, 2, device="cuda", window=100)
+        assert int(plan.host[21]) == 0 and int(plan.host[22]) == 100
+    finally:
+        ops.set_prefill_kernel(ops.PREFILL_DEFAULT)
+
+
+@pytest.mark.parametrize("b", [8193, 65535])
+def test_step_metadata_many_sequences(b):
+    """The most sequences: a page of two tokens each."""
+    ops = _ops()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    lens = torch.arange(b, **i32) % 3 - 1              # idle, empty, one token
+    tables = torch.full((b, 2), -1, **i32)
+    one = (lens == 1).nonzero().flatten()
+    tables[one, 0] = one.int()
+    free = torch.arange(b, 3 * b, **i32)
+    count, new = torch.tensor([2 * b], **i32), torch.full((b,), 2, **i32)
+    positions, slots, cu_q, cu_k, after = ops.step_metadata(lens, new, tables, free, count, 2, 2 * b)
+    assert ops.device_error() == 0
+    missing = (lens >= 0).long()                        # empty: its first page; one token: its second
+    nth = missing.cumsum(0) - 1
+    page = torch.where(missing > 0, 3 * b - 1 - nth, -1)
+    want = torch.full((b, 2), -1, dtype=torch.int64, device="cuda")
+    want[:, 0] = torch.where(lens == 0, page, torch.where(lens == 1, torch.arange(b, device="cuda"), -1))
+    want[:, 1] = torch.where(lens == 1, page, -1)
+    assert torch.equal(tables.long(), want) and int(count) == 2 * b - int(missing.sum())
+    start = lens.clamp(min=0).long()
+    pos = torch.stack((start, start + 1), 1)
+    live = (lens >= 0).view(-1, 1)
+    assert torch.equal(positions.view(b, 2), torch.where(live, pos, 0))
+    slot = want.gather(1, (pos // 2).clamp(max=1)) * 2 + pos % 2
+    assert torch.equal(slots.view(b, 2).long(), torch.where(live, slot, -1))
+    assert torch.equal(cu_q.long(), 2 * torch.arange(b + 1, device="cuda"))
+    assert torch.equal(after.long(), torch.where(lens >= 0, start + 2, 0)) and int(cu_k[-1]) == int(after.sum())
+
+
+def test_verify_drafts_shared_rows():
+    """One distribution for all sequences (strides of 0), and random numbers likewise."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(6)
+    p = _probabilities(g, 1, 3, 5000, torch.float32).expand(50, 3, 5000)
+    u = torch.rand(1, 2, generator=g, device="cuda").expand(50, 2)
+    drafts = torch.randint(0, 5000, (1, 2), generator=g, device="cuda").expand(50, 2)
+    tokens, emitted = ops.verify_drafts(drafts, p, None, u, torch.full((50,), 0.3, device="cuda"))
+    assert bool((tokens == tokens[0]).all()) and bool((emitted == emitted[0]).all())
+    want = oracle.verify(drafts[0].tolist(), p[0].cpu(), None, u[0].tolist(), float(torch.tensor(0.3)))
+    assert tokens[0].tolist() == want + [-1] * (3 - len(want))
