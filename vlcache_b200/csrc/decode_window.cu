@@ -34,7 +34,8 @@
 // (76 % of DRAM's nominal rate); with more the steps' latency counts: 8 warps an SM, whose registers hold the rows,
 // the tensor pipe half busy.  Tried for five tokens: chunks of 16 keys 136, a ring of 96 KB 107.6, tiles as 3 + 2
 // instead of 3 + 3 of which one is empty 110, three warps of 2 tiles a team (12 warps an SM) 114, three blocks an SM
-// (spilling) 169.
+// (spilling) 169, Q of three tiles in shared memory 110.  (A ninth warp that only copies would cap the others at
+// 168 registers.)
 #include <algorithm>
 #include <cmath>
 #include <limits>

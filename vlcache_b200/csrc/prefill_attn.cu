@@ -688,7 +688,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
                              p.scale_log2;
         // Lazy rescaling: only move the reference max when it grows by > 2^8.
         const bool need = m_tile > m_use + 8.0f;
-        const float m_new = need ? m_tile : m_use;
+        // (A window's first block may show a row a few keys only: its reference is put above them, so that the
+        // next block's maximum does not move it.)
+        const float above = kWindow && m_use == -INFINITY ? 8.0f : 0.f;
+        const float m_new = need ? m_tile + above : m_use;
         const float f = (need && m_use != -INFINITY) ? fast_exp2(m_use - m_new) : 1.0f;
         m_use = m_new;
         const float mref = (m_use == -INFINITY) ? 0.f : m_use;
