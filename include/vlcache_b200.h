@@ -488,8 +488,9 @@ int vlc_remap_block_tables(int32_t* block_tables, int64_t row_stride, int num_ro
  *   recorded (VLC_DEV_ERR_BLOCK_RANGE), a length past max_context_len is cut to it and recorded
  *   (VLC_DEV_ERR_LENGTH).  Sizes come from host values, so the launches can be captured; workspace:
  *   vlc_decode_window_workspace_size bytes, 16-byte aligned, one per call in flight.
- * vlc_step_metadata: sequence i of context_lens[i] tokens takes new_lens[i] more (below 0: an idle place
- *   of the batch, whose rows have position 0 and slot -1, and which takes no page and has length 0 after).  Block-table entries below 0 where they fall are filled from the end
+ * vlc_step_metadata: sequence i of context_lens[i] tokens takes new_lens[i] more (a context_lens[i] below 0: an
+ *   idle place of the batch, whose new_lens[i] rows have position 0 and slot -1, and which takes no page and
+ *   has length 0 after).  Block-table entries below 0 where they fall are filled from the end
  *   of the free list (free_pages[0 .. *num_free), the k-th missing page of the batch being
  *   free_pages[*num_free - 1 - k], sequences in order), then pages wholly behind the window of
  *   the first new row and behind the sinks go back to its end, in order, and their entries become

@@ -14,6 +14,7 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import hashlib
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -57,9 +58,10 @@ STAMP_PATH = LIB_PATH.with_name(LIB_PATH.name + ".srchash")
 
 
 def source_hash() -> str:
-    """SHA-256 over the bytes of every source, header and this recipe (names included):
-    the library is rebuilt exactly when this differs from the hash it was built from."""
-    h = hashlib.sha256()
+    """SHA-256 over the bytes of every source, header and this recipe (names included), and the versions of
+    Python and torch that the binding is built for: the library is rebuilt exactly when this differs
+    from the hash it was built from."""
+    h = hashlib.sha256(f"{sys.implementation.cache_tag} {importlib.metadata.version('torch')}\0".encode())
     for p in _sources() + _headers() + [Path(__file__)]:
         h.update(p.name.encode())
         h.update(b"\0")
@@ -70,7 +72,8 @@ def source_hash() -> str:
 
 def is_fresh() -> bool:
     """True when the in-tree library exists and was built from the current sources."""
-    return LIB_PATH.exists() and BINDING_PATH.exists() and STAMP_PATH.exists() and STAMP_PATH.read_text().strip() == source_hash()
+    return (LIB_PATH.exists() and BINDING_PATH.exists() and STAMP_PATH.exists()
+            and STAMP_PATH.read_text().strip() == source_hash())
 
 
 def _needs_build() -> bool:

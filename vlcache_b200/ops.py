@@ -1001,8 +1001,8 @@ def step_metadata(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
                   sinks: int = 0) -> tuple[torch.Tensor, ...]:
     """Block tables and slot maps of a step, built on the device from the sequences' lengths, without a
     host read (so that it can be captured): sequence i of ``context_lens[i]`` tokens takes
-    ``new_lens[i]`` more (below 0: an idle place of the batch, whose rows have position 0 and slot -1,
-    and which takes no page and has length 0 after).
+    ``new_lens[i]`` more (a ``context_lens[i]`` below 0: an idle place of the batch, whose
+    ``new_lens[i]`` rows have position 0 and slot -1, and which takes no page and has length 0 after).
 
     Missing entries (below 0) of ``block_tables`` [B, width] where they fall are filled from the end of
     the free list (``free_pages[:num_free]``, sequences in order), then pages wholly behind the
