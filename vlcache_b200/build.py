@@ -32,7 +32,7 @@ LIB_PATH = PKG_DIR / "libvlcache_b200.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CUDA_SOURCES = ["runtime.cu", "kv_ops.cu", "prefill_attn.cu", "decode_attn.cu", "metadata.cu", "gemm.cu", "content_hash.cu",
-                "rope_axes.cu", "kv_fp4.cu", "decode_fp4.cu", "pages.cu", "decode_window.cu",
+                "rope_axes.cu", "kv_fp4.cu", "decode_fp4.cu", "pages.cu", "decode_window.cu", "decode_window_wide.cu",
                 "step_metadata.cu", "verify.cu"]
 CPP_SOURCES = ["plan.cpp"]
 BINDING_SOURCE = "binding.cpp"

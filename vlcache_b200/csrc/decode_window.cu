@@ -40,47 +40,16 @@
 #include <cmath>
 #include <limits>
 
-#include "common.cuh"
+#include "decode_window.cuh"
 #include "runtime.h"
 
 namespace vlc {
 namespace decode_window {
 
-constexpr int HD = 128;
 constexpr int WARPS = 4;                 // of a block
 constexpr int RING_BYTES = 64 << 10;     // of a block, shared out among its teams
 constexpr int BLOCKS_PER_SM = 2;
-constexpr int MIN_BLOCK = 32;            // a page's tokens are a multiple of it
-constexpr int MAX_ROWS = 128;           // tokens x query heads of a KV head
-constexpr float SLACK = 8.f;            // log2 that the maximum may grow by before O is rescaled
-constexpr float NO_MAX = -3e38f;        // the maximum of no key (finite: differences of two are numbers)
-
-struct Params {
-  // {64 dims, Hk, slots, 2 halves of a row, caches}, box {64, 1, CK, 2, caches} of chunks of CK keys.  Joined, the caches are
-  // the two, whose stride is their distance (v_first: V lies before K); else kv[0] is K and kv[1] V.
-  CUtensorMap kv[2];
-  bool joined, v_first;
-  const __nv_bfloat16* q;
-  int64_t q_token_stride;
-  const int32_t* block_tables;
-  int64_t table_stride;
-  int table_width, block_size, num_pages;
-  const int32_t* context_lens;
-  int num_seqs, max_len, tokens, window, sinks;
-  int group, num_kv_heads, rows;  // rows = tokens * group
-  uint32_t group_inverse;         // 2^16 / group, rounded up: exact for rows below 128
-  __device__ __forceinline__ int token_of(int row) const { return (int)((uint32_t)row * group_inverse >> 16); }
-  int cluster;                    // blocks of a pair's cluster (0: the line)
-  float scale_log2;               // |softmax scale| * log2(e), above 0: a hidden key's score stays -infinity
-  uint32_t q_flip;                // the signs of a pair of q's elements where the scale is negative
-  __nv_bfloat16* out;
-  int64_t out_token_stride;
-  int num_blocks;
-  // Workspace: a block's first pair and its last leave parts when they are not whole.
-  float* parts;     // [num_blocks][2][rows][HD] sums of P V
-  float2* part_ml;  // [num_blocks][2][rows] (maximum, sum of P)
-  int2* places;     // [num_seqs][num_kv_heads] of each pair with keys: (slot of its first part, parts)
-};
+constexpr int WIDE_ROWS = 24;            // more rows go to decode_window_wide.cu
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -105,47 +74,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-
-// The chunks of a sequence that any of its rows sees: chunk v is v for v < first (of the sinks), and
-// v + jump from there on.
-template <int CK>  // keys of a chunk
-struct Span {
-  int len;          // cut to the host's bound
-  int low;          // first key of the window of the sequence's first row
-  int first, jump;
-  int count;
-  // Chunks whose keys every row sees: [0, all0) of the sinks and [all1, all2): they end by the first row's
-  // position and begin in the last row's window.
-  __device__ __forceinline__ int all0(const Params& p) const { return min(first, p.sinks / CK); }
-  __device__ __forceinline__ int all1(const Params& p) const {
-    return p.window > 0 ? max(first, (max(0, len - p.window) + CK - 1) / CK - jump) : 0;
-  }
-  __device__ __forceinline__ int all2(const Params& p) const { return (len - p.tokens + 1) / CK - jump; }
-};
-template <int CK>
-__device__ __forceinline__ Span<CK> span_of(const Params& p, int len) {
-  Span<CK> s;
-  s.len = min(max(len, 0), p.max_len);
-  s.low = p.window > 0 ? max(0, s.len - p.tokens - p.window + 1) : 0;
-  const int wc = s.low / CK;
-  s.first = min(wc, (p.sinks + CK - 1) / CK);
-  s.jump = wc - s.first;
-  s.count = (s.len + CK - 1) / CK - s.jump;
-  return s;
-}
-
-// How the line of `total` chunks is shared: every block takes each() of them and the first extra()
-// one more.
-struct Shares {
-  int64_t each, extra;
-  __device__ __forceinline__ Shares(int64_t total, int blocks) : each(total / blocks), extra(total % blocks) {}
-  __device__ __forceinline__ int64_t first(int64_t block) const { return block * each + min(block, extra); }
-  __device__ __forceinline__ int64_t count(int64_t block) const { return each + (block < extra ? 1 : 0); }
-  __device__ __forceinline__ int64_t block_of(int64_t chunk) const {
-    const int64_t big = extra * (each + 1);
-    return chunk < big ? chunk / (each + 1) : extra + (chunk - big) / each;
-  }
-};
 
 // Byte of 16-byte piece `piece` of row `row` of a warp's Q in shared memory (rows of 256 bytes).
 __device__ __forceinline__ uint32_t q_at(int row, int piece) { return row * 256 + ((piece ^ (row & 7)) << 4); }
@@ -430,40 +358,14 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
       count = (int)((int64_t)span.count * (rank + 1) / p.cluster) - j0;
       return Shares(0, 1);
     }
-    int64_t total = 0;
-    for (int i = lane; i < p.num_seqs; i += 32) {
-      const int len = __ldg(p.context_lens + i);
-      if (blockIdx.x == 0 && warp == 0 && len > p.max_len) record_error(VLC_DEV_ERR_LENGTH);
-      total += span_of(len).count;
-    }
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    const Shares all(total * Hk, p.num_blocks);
-    c0 = all.first(blockIdx.x);
-    count = (int)all.count(blockIdx.x);
-    int64_t at = c0;  // c0's place among the chunks from the sequence's first on
-    for (int base = 0; count > 0 && base < p.num_seqs; base += 32) {
-      const int64_t n = base + lane < p.num_seqs ? (int64_t)span_of(__ldg(p.context_lens + base + lane)).count * Hk : 0;
-      int64_t upto = n;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += x;
-      }
-      const uint32_t past = __ballot_sync(0xffffffffu, upto > at);
-      if (past) {
-        const int first = __ffs(past) - 1;
-        seq = base + first;
-        at -= __shfl_sync(0xffffffffu, upto - n, first);
-        break;
-      }
-      at -= __shfl_sync(0xffffffffu, upto, 31);
-    }
-    span = span_of(__ldg(p.context_lens + seq));
-    if (count > 0) {
-      head = (int)(at / span.count);
-      j0 = (int)(at - (int64_t)head * span.count);
-    }
+    Run<CK> run;
+    const Shares all = run_of(p, run, warp, lane);
+    seq = run.seq;
+    head = run.head;
+    j0 = run.j0;
+    count = run.count;
+    c0 = run.c0;
+    span = run.span;
     return all;
   }();
   if (!PAIR && count == 0) return;
@@ -808,16 +710,20 @@ static int cluster_of(int num_seqs, int num_kv_heads, int rows, int tokens, int 
   return cluster > 1 && chunks <= most ? cluster : 0;
 }
 
+// Whether decode_window_wide.cu takes the line.
+static bool wide_of(int rows) { return rows > WIDE_ROWS; }
+
 // Blocks of the grid: from host values only, so that it is fixed for graph capture.  A block has at least
 // MIN_CHUNKS for each of its teams: few chunks, but fewer parts to join.
 constexpr int MIN_CHUNKS = 2;
 static int grid_blocks(int num_seqs, int num_kv_heads, int rows, int tokens, int max_context_len, int window, int sinks,
                        int num_sms) {
+  const bool wide = wide_of(rows);
   const Shape shape = shape_of(rows);
-  const int64_t chunks = most_chunks(shape.keys(), tokens, max_context_len, window, sinks);
-  const int least = MIN_CHUNKS * (WARPS / shape.team);
+  const int64_t chunks = most_chunks(wide ? WIDE_CHUNK : shape.keys(), tokens, max_context_len, window, sinks);
+  const int least = wide ? 1 : MIN_CHUNKS * (WARPS / shape.team);
   const int64_t most = (num_seqs * num_kv_heads * chunks + least - 1) / least;
-  return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)num_sms * BLOCKS_PER_SM, most));
+  return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)num_sms * (wide ? 1 : BLOCKS_PER_SM), most));
 }
 
 static int64_t workspace_bytes_for(int64_t blocks, int rows, int64_t pairs) {
@@ -905,23 +811,25 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
     if (!aligned16(workspace)) return VLC_ERR_ALIGN;
   }
 
+  const bool wide = !cluster && wide_of(rows);
   Params p;
   const uint8_t* caches[2] = {(const uint8_t*)k_cache, (const uint8_t*)v_cache};
-  p.v_first = caches[1] < caches[0];
+  p.v_first = !wide && caches[1] < caches[0];
   if (p.v_first) std::swap(caches[0], caches[1]);
   const uint64_t apart = (uint64_t)(caches[1] - caches[0]);
-  p.joined = apart > 0 && apart < 1ull << 40;  // as a tensor map's strides may be
+  p.joined = !wide && apart > 0 && apart < 1ull << 40;  // as a tensor map's strides may be
   if (!p.joined && p.v_first) {
     std::swap(caches[0], caches[1]);
     p.v_first = false;
   }
+  p.box = wide ? block_size % 64 == 0 ? 64 : 32 : shape.keys();
   const uint64_t slots = (uint64_t)num_pages * block_size, row = (uint64_t)num_kv_heads * HD * 2;
   for (int i = 0; i < (p.joined ? 1 : 2); ++i) {
     const uint64_t both = p.joined ? 2 : 1;
     const uint64_t dims[5] = {64, (uint64_t)num_kv_heads, slots, 2, both};
     const uint64_t strides[4] = {HD * 2, row, 128, p.joined ? apart : 256};
-    const uint32_t box[5] = {64, 1, (uint32_t)shape.keys(), 2, (uint32_t)both};
-    if (encode_tmap_bf16(&p.kv[i], caches[i], 5, dims, strides, box, 128) != VLC_OK) return VLC_ERR_CUDA;
+    const uint32_t box[5] = {64, 1, (uint32_t)p.box, wide ? 1u : 2u, (uint32_t)both};
+    if (encode_tmap_bf16(&p.kv[i], caches[i], wide ? 4 : 5, dims, strides, box, 128) != VLC_OK) return VLC_ERR_CUDA;
   }
   p.q = (const __nv_bfloat16*)q;
   p.q_token_stride = q_token_stride;
@@ -952,7 +860,8 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
 
   cudaStream_t st = (cudaStream_t)stream;
   int rc;
-  switch (shape.team * 8 + shape.tiles) {
+  if (wide) rc = launch_wide(p, st);
+  else switch (shape.team * 8 + shape.tiles) {
     case 8 + 1: rc = launch<1, 1>(p, st); break;
     case 8 + 2: rc = launch<2, 1>(p, st); break;
     case 8 + 3: rc = launch<3, 1>(p, st); break;

@@ -147,21 +147,6 @@ __device__ __forceinline__ Bars make_bars(uint8_t* smem) {
   return r;
 }
 
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, int code,
-                                              volatile int* abort_flag) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*abort_flag) return false;
-    if (clock64() - t0 > VLC_WAIT_LIMIT_CYCLES) {
-      record_error(code);
-      *abort_flag = 1;
-      return false;
-    }
-  }
-}
-
 // Unit fields the roles need.
 struct UnitView {
   int n_a, n_b;  // key blocks of tile A (the unit's length) and of tile B (0: no tile B)
