@@ -857,3 +857,130 @@ def test_verify_drafts_shared_rows():
     assert bool((tokens == tokens[0]).all()) and bool((emitted == emitted[0]).all())
     want = oracle.verify(drafts[0].tolist(), p[0].cpu(), None, u[0].tolist(), float(torch.tensor(0.3)))
     assert tokens[0].tolist() == want + [-1] * (3 - len(want))
+
+
+# ------------------------------------------------------------------ decode of more than 24 rows a KV head
+MANY_ROWS = [
+    # heads, kv_heads, tokens, block, window, sinks: 28, 35, 48, 56, 72, 91, 112 and 128 rows
+    (14, 2, 4, 256, 700, 4),
+    (14, 2, 5, 32, 129, 20),
+    (32, 2, 3, 96, 0, 0),
+    (7, 1, 8, 160, 128, 0),
+    (24, 2, 6, 128, 300, 130),
+    (14, 2, 13, 64, 1, 0),
+    (7, 1, 16, 256, 1000, 1),
+    (16, 1, 8, 32, 255, 300),
+]
+
+
+@pytest.mark.parametrize("case", MANY_ROWS, ids=lambda c: "-".join(map(str, c)))
+def test_decode_window_many_rows(case):
+    """Lengths around the chunks' borders, pairs that blocks share, rows that see nothing, and NaN and infinities
+    in every key and value that no row sees."""
+    heads, kv_heads, n, block, window, sinks = case
+    g = torch.Generator(device="cuda").manual_seed(heads + n + block)
+    lens = [0, 1, n, 127, 128, 129, 255, 256, 257, 383, 4000] + [int(x) for x in np.random.default_rng(n).integers(1, 2500, 50)]
+    tables, pages = _tables(g, lens, block)
+    k_cache, v_cache = _caches(g, pages, block, kv_heads, joined=n % 2 == 0)
+    q = (1.5 * torch.randn(len(lens), n, heads, D, generator=g, device="cuda")).to(torch.bfloat16)
+    new = [min(n, m) for m in lens]
+    _spoil(k_cache, tables, lens, new, window, sinks, math.nan)
+    _spoil(v_cache, tables, lens, new, window, sinks, math.inf)
+    _release(tables, lens, new, block, window, sinks)
+    got = _decode(tables, lens, new, q, k_cache, v_cache, window, sinks, 0.09)
+    assert _ops().device_error() == 0
+    _check_decode(got, tables, lens, n, q, k_cache, v_cache, window, sinks, 0.09)
+    assert torch.equal(got, _decode(tables, lens, new, q, k_cache, v_cache, window, sinks, 0.09, out=q))   # in place
+
+
+@pytest.mark.parametrize("scale", [0.3, -0.3, 0.0])
+def test_decode_window_many_rows_scales_and_broken_queries(scale):
+    g, lens, tables, k_cache, v_cache, q = _small(lens=(200, 70, 3330), n=5)
+    q[0, 1, 3, 5], q[1, 0, 0, 0], q[2, 4, 15, 127] = math.inf, math.nan, -math.inf
+    got = _decode(tables, lens, None, q, k_cache, v_cache, 40, 0, scale)
+    broken = ~torch.isfinite(q).all(-1)
+    assert int(broken.sum()) == 3 and bool(torch.isnan(got[broken]).all()) and bool(torch.isfinite(got[~broken]).all())
+    clean = torch.where(broken.unsqueeze(-1), torch.zeros_like(q), q)
+    again = _decode(tables, lens, None, clean, k_cache, v_cache, 40, 0, scale)
+    _check_decode(again, tables, lens, 5, clean, k_cache, v_cache, 40, 0, scale)
+    assert torch.equal(got[~broken], again[~broken])
+
+
+def test_decode_window_many_rows_large_scores():
+    """Scores that rise along the keys: the maxima move again and again."""
+    g, lens, tables, k_cache, v_cache, q = _small(lens=(3000, 2000), n=4)
+    rising = torch.linspace(0.1, 3, 3000, device="cuda")
+    for i, m in enumerate(lens):
+        at, row = tables[i].long()[torch.arange(m, device="cuda") // 64], torch.arange(m, device="cuda") % 64
+        k_cache[at, row] = (k_cache[at, row].float() * rising[:m, None, None]).to(torch.bfloat16)
+    got = _decode(tables, lens, None, q, k_cache, v_cache, 0, 0, 0.5)
+    # a score is off by 130 steps of fp32 of sum |q k| at most (128 products, two roundings of the scale)
+    most = 0.5 * float(q.double().abs().sum(-1).max() * k_cache.double().abs().max())
+    most = min(most, 0.5 * float((q.double() ** 2).sum(-1).max().sqrt() * (k_cache.double() ** 2).sum(-1).max().sqrt()))
+    _check_decode(got, tables, lens, 4, q, k_cache, v_cache, 0, 0, 0.5, scores=130 * 2.0 ** -24 * most)
+
+
+def test_decode_window_many_rows_bad_pages_and_lengths():
+    ops = _ops()
+    g, lens, tables, k_cache, v_cache, q = _small(lens=(200, 70, 5000), n=4, block=32)
+    for bad in (-1, k_cache.shape[0], 1 << 30, -(1 << 31)):
+        broken = tables.clone()
+        broken[2, 7], broken[1, 1] = bad, bad
+        got = _decode(broken, lens, None, q, k_cache, v_cache, 0, 0, 0.1)
+        assert ops.device_error() == 102
+        keys = k_cache.clone(), v_cache.clone()   # their keys count as zeros, the others of their chunks stay
+        for c in keys:
+            c[tables[2, 7].long()] = 0
+            c[tables[1, 1].long()] = 0
+        _check_decode(got, tables, lens, 4, q, *keys, 0, 0, 0.1)
+    got = _decode(tables[:, :1].contiguous(), lens, None, q, k_cache, v_cache, 0, 0, 0.1)
+    assert ops.device_error() == 102 and bool(torch.isfinite(got).all())
+    got = _decode(tables, lens, None, q, k_cache, v_cache, 30, 2, 0.1, bound=100)
+    assert ops.device_error() == 104
+    _check_decode(got, tables, [min(m, 100) for m in lens], 4, q, k_cache, v_cache, 30, 2, 0.1)
+
+
+def test_decode_window_many_rows_strides_and_captured():
+    """A projection's rows, a caller's output and workspace; two graphs at once that follow changed lengths."""
+    ops = _ops()
+    g, lens, tables, k_cache, v_cache, q = _small(lens=(900, 70, 5000), n=4)
+    rows = torch.full((12, 20 * D), math.nan, dtype=torch.bfloat16, device="cuda")
+    view = rows[:, :16 * D].view(3, 4, 16, D)
+    view.copy_(q)
+    into = torch.full((13, 17, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = into[:12, :16].view(3, 4, 16, D)
+    need = ops.decode_window_workspace_bytes(3, 4, 16, 2, 5000, 600, 3)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ops.decode_attention_window(view, k_cache, v_cache, tables, lens_t, 5000, 0.1, 600, 3, out,
+                                torch.empty(need, dtype=torch.uint8, device="cuda"))
+    _check_decode(out, tables, lens, 4, q, k_cache, v_cache, 600, 3, 0.1)
+    assert bool((into[12:] == 7).all()) and bool((into[:, 16:] == 7).all())
+    qs, graphs, outs = [q, q.flip(0).contiguous()], [], []
+    for x in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.decode_attention_window(x, k_cache, v_cache, tables, lens_t, 5000, 0.1, 600, 3))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for cut in (0, 3, 64):
+        now = [max(0, m - cut * 2) for m in lens]
+        lens_t.copy_(torch.tensor(now, dtype=torch.int32))
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for x, o in zip(qs, outs):
+            _check_decode(o, tables, now, 4, x, k_cache, v_cache, 600, 3, 0.1)
+    assert ops.device_error() == 0
+
+
+def test_decode_window_many_rows_pages_beyond_4_gb():
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pages, block, kv_heads = 9000, 256, 4
+    both = torch.empty(2, pages, block, kv_heads, D, dtype=torch.bfloat16, device="cuda")
+    both[:, -4:].normal_(generator=g)
+    tables = torch.tensor([[pages - 1, pages - 3], [pages - 2, pages - 4]], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 5, 28, D, generator=g, device="cuda").to(torch.bfloat16)
+    got = _decode(tables, [400, 512], None, q, both[0], both[1], 300, 4, 0.1)
+    _check_decode(got, tables, [400, 512], 5, q, both[0], both[1], 300, 4, 0.1)

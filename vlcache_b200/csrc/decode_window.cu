@@ -11,31 +11,26 @@
 //     each) the 8 columns: S^T = K Q^T and O^T = V^T P^T.  A tile of 8 rows wastes at most 7, where a
 //     tile of 16 would waste half of one token's 7 or 8 heads.
 //   * P^T in the layout of a B operand is S^T's accumulator transposed: one movmatrix an 8 x 8 tile.
-//   * The keys that a sequence sees are chunks of 16 or 32: those of the sinks, then those from the
+//   * The keys that a sequence sees are chunks of 16: those of the sinks, then those from the
 //     window's first on; what lies between is skipped, its pages are not touched.
 // The chunks of all (sequence, KV head) pairs form one line that the grid's blocks share out evenly,
 // each a contiguous run of it, so that the shares are equal whatever the lengths are.  In a block a
-// team of warps takes every TEAMS-th chunk of the run, with a ring of its own (one TMA copy a chunk, K
-// and V together) and a running softmax of its own; at the end of a pair the teams' sums are added
-// through shared memory, lane by lane.  A team is one warp for up to 24 rows and two or four, which
-// share its chunks and have different rows, for more: a tile of 8 rows takes 32 registers of
-// accumulators and 16 of Q.  A pair that a block has to itself is written out; the parts of a pair
+// warp takes every fourth chunk of the run, with a ring of its own (one TMA copy a chunk, K and V
+// together) and a running softmax of its own; at the end of a pair the warps' sums are added through
+// shared memory, lane by lane.  A pair that a block has to itself is written out; the parts of a pair
 // that several blocks share go to the workspace, and window_join_kernel, a programmatic dependent,
 // joins them.  Few pairs of few keys are taken by clusters instead, a pair each, whose blocks join through
-// their shared memory: one launch.
+// their shared memory: one launch.  A tile of 8 rows takes 32 registers of accumulators and 16 of Q: up to three
+// tiles, 24 rows, are here; more go to decode_window_wide.cu, which shares the line and the join.
 //
 // P is rounded to bf16, V's type, as an operand of its MMA has to be (by 2^-8 of itself at most); its sum
 // is taken over the rounded values, so that the error does not add up with the keys.  Scores, maxima
 // and sums are fp32.
 //
 // Measured (64 sequences of 2700 .. 10700 keys, window 4096, 28 query and 4 KV heads; floor 82 .. 83 us): one token
-// 86.6 us, two 91, three and four 96, five and six 106 .. 108, eight 142; two sequences of 100,003 .. 131,071 keys,
-// 16 and 2 heads, four tokens without a window 50.5 (floor 36, 7 of them the join).  One token is bound by HBM
-// (76 % of DRAM's nominal rate); with more the steps' latency counts: 8 warps an SM, whose registers hold the rows,
-// the tensor pipe half busy.  Tried for five tokens: chunks of 16 keys 136, a ring of 96 KB 107.6, tiles as 3 + 2
-// instead of 3 + 3 of which one is empty 110, three warps of 2 tiles a team (12 warps an SM) 114, three blocks an SM
-// (spilling) 169, Q of three tiles in shared memory 110.  (A ninth warp that only copies would cap the others at
-// 168 registers.)
+// 86.6 us, two 91, three 95 (decode_window_wide.cu: two 93.6, three 95.1); four, which it takes, 94.5 (here, by teams of
+// two warps: 96), five 96 (106), eight 101 (142).  One token is bound by HBM (76 % of DRAM's nominal rate); with more
+// the steps' latency counts: 8 warps an SM, whose registers hold the rows.
 #include <algorithm>
 #include <cmath>
 #include <limits>
@@ -47,9 +42,10 @@ namespace vlc {
 namespace decode_window {
 
 constexpr int WARPS = 4;                 // of a block
-constexpr int RING_BYTES = 64 << 10;     // of a block, shared out among its teams
+constexpr int RING_BYTES = 64 << 10;     // of a block, shared out among its warps
+constexpr int CK = 16;                   // keys of a chunk
 constexpr int BLOCKS_PER_SM = 2;
-constexpr int WIDE_ROWS = 24;            // more rows go to decode_window_wide.cu
+constexpr int WIDE_ROWS = 24;            // more rows go to decode_window_wide.cu, whatever the lengths are
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -75,27 +71,22 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   return d;
 }
 
-// Byte of 16-byte piece `piece` of row `row` of a warp's Q in shared memory (rows of 256 bytes).
-__device__ __forceinline__ uint32_t q_at(int row, int piece) { return row * 256 + ((piece ^ (row & 7)) << 4); }
-
 // A warp's rows: S^T, O^T and the softmax, and the step over one chunk.  Lane (r, t) = (lane / 4,
 // lane % 4) holds keys r and r + 8 of a chunk, dims 8c + r, and rows 2t and 2t + 1 of each tile.
-// Q_SMEM: Q in shared memory (four tiles leave no registers for it).
-template <int NT, int CK, bool Q_SMEM>  // NT: tiles of 8 rows, CK: keys of a chunk
+template <int NT>  // tiles of 8 rows
 struct State {
-  static constexpr int KT = CK / 16;            // key tiles of a chunk
   static constexpr int HALF_BYTES = CK * 128;   // 64 dims of its keys
-  uint32_t qb[Q_SMEM ? 1 : NT][8][2];  // Q as B fragments: dims 16k + 2t, + 1 (and 8 more) of row r
+  uint32_t qb[NT][8][2];  // Q as B fragments: dims 16k + 2t, + 1 (and 8 more) of row r
   float o[NT][8][4];                   // m-tile i: dims 16i + r of rows 2t, 2t + 1 (0, 1), 16i + 8 + r (2, 3)
   float l[NT][4];                      // sums of P: 0 and 1 of rows 2t, 2t + 1
   float m[NT][2];                      // the maximum that P is relative to
 
-  // Rows row0 .. of the pair, row x being token x / G's head x % G.
-  __device__ __forceinline__ void start(const Params& p, int seq, int head, int row0, int r, int t, uint8_t* q_smem) {
+  // The pair's rows, row x being token x / G's head x % G.
+  __device__ __forceinline__ void start(const Params& p, int seq, int head, int r, int t) {
     const int G = p.group;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int row = row0 + n * 8 + r;
+      const int row = n * 8 + r;
       const int tok = p.token_of(row);
       const bool live = row < p.rows;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(
@@ -118,59 +109,36 @@ struct State {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (Q_SMEM) *reinterpret_cast<uint32_t*>(q_smem + q_at(n * 8 + r, 2 * k + x) + 4 * t) = u[k][x] | spoil;
-          else qb[n][k][x] = u[k][x] | spoil;
-        }
+        for (int x = 0; x < 2; ++x) qb[n][k][x] = u[k][x] | spoil;
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
       l[n][0] = l[n][1] = l[n][2] = l[n][3] = 0.f;
       m[n][0] = m[n][1] = NO_MAX;
     }
-    if (Q_SMEM) __syncwarp();
   }
 
   // One chunk whose K and V tiles are at kt and vt; key0 is its first key.  `cut`: not every row sees all of it.
   __device__ __forceinline__ void step(const Params& p, uint32_t kt, uint32_t vt, int key0, bool cut,
-                                       const Span<CK>& span, int row0, int lane, uint32_t q_smem) {
+                                       const Span<CK>& span, int lane) {
     const int r = lane >> 2, t = lane & 3, mi = lane >> 3, ri = lane & 7;
     // ---- S^T = K Q^T
-    float s[KT][NT][4];
+    float s[NT][4];
 #pragma unroll
-    for (int c = 0; c < KT; ++c)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[c][n][0] = s[c][n][1] = s[c][n][2] = s[c][n][3] = 0.f;
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
     {
       float s2[4] = {0.f, 0.f, 0.f, 0.f};  // one tile alone: two chains of MMAs
       // piece 2k + x of row ri is at (2k + x) ^ ri = 2k ^ (x ^ ri): an address, with bits of k exchanged
       const uint32_t at = ((mi & 1) * 8 + ri) * 128 + (((mi >> 1) ^ ri) << 4);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        uint32_t a[KT][4];
+        uint32_t a[4];
+        ldsm_x4(((kt + at) ^ ((k & 3) << 5)) + (k >> 2) * HALF_BYTES, a);
 #pragma unroll
-        for (int c = 0; c < KT; ++c) ldsm_x4(((kt + at) ^ ((k & 3) << 5)) + (k >> 2) * HALF_BYTES + c * 2048, a[c]);
-        if constexpr (Q_SMEM) {
-#pragma unroll
-          for (int n = 0; n < NT; n += 2) {  // two tiles' fragments in one load
-            uint32_t b[4];
-            ldsm_x4(q_smem + q_at(n * 8 + (mi >> 1) * 8 + ri, 2 * k + (mi & 1)), b);
-#pragma unroll
-            for (int c = 0; c < KT; ++c) {
-              mma_bf16(s[c][n], a[c], b[0], b[1]);
-              mma_bf16(s[c][n + 1], a[c], b[2], b[3]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < KT; ++c)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              mma_bf16(NT * KT == 1 && (k & 1) ? s2 : s[c][n], a[c], qb[n][k][0], qb[n][k][1]);
-        }
+        for (int n = 0; n < NT; ++n) mma_bf16(NT == 1 && (k & 1) ? s2 : s[n], a, qb[n][k][0], qb[n][k][1]);
       }
-      if (NT * KT == 1) {
+      if (NT == 1) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s[0][0][x] += s2[x];
+        for (int x = 0; x < 4; ++x) s[0][x] += s2[x];
       }
     }
     if (cut) {
@@ -178,24 +146,19 @@ struct State {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int odd = 0; odd < 2; ++odd) {
-          const int pos = span.len - p.tokens + p.token_of(row0 + n * 8 + 2 * t + odd);
+          const int pos = span.len - p.tokens + p.token_of(n * 8 + 2 * t + odd);
 #pragma unroll
-          for (int c = 0; c < KT; ++c)
-#pragma unroll
-            for (int e = odd; e < 4; e += 2) {
-              const int key = key0 + c * 16 + r + (e >> 1) * 8;
-              if (key > pos || (p.window > 0 && key <= pos - p.window && key >= p.sinks)) s[c][n][e] = -INFINITY;
-            }
+          for (int e = odd; e < 4; e += 2) {
+            const int key = key0 + r + (e >> 1) * 8;
+            if (key > pos || (p.window > 0 && key <= pos - p.window && key >= p.sinks)) s[n][e] = -INFINITY;
+          }
         }
       // V rows that no row of the sequence sees may hold anything: their P is 0, and so V is made.
+      const int key = key0 + lane % CK;  // (a lane half a row)
+      if (key >= span.len || (key < span.low && key >= p.sinks)) {
 #pragma unroll
-      for (int x = lane; x < 2 * CK; x += 32) {
-        const int key = key0 + x % CK;
-        if (key >= span.len || (key < span.low && key >= p.sinks)) {
-#pragma unroll
-          for (int y = 0; y < 8; ++y)
-            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vt + x * 128 + y * 16), "r"(0) : "memory");
-        }
+        for (int y = 0; y < 8; ++y)
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vt + lane * 128 + y * 16), "r"(0) : "memory");
       }
       fence_proxy_async_smem();  // before the next copy into the stage
       __syncwarp();
@@ -204,12 +167,8 @@ struct State {
     float top[NT][2], most = NO_MAX;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      top[n][0] = fmaxf(s[0][n][0], s[0][n][2]);
-      top[n][1] = fmaxf(s[0][n][1], s[0][n][3]);
-      if constexpr (KT == 2) {
-        top[n][0] = fmax3(top[n][0], s[1][n][0], s[1][n][2]);
-        top[n][1] = fmax3(top[n][1], s[1][n][1], s[1][n][3]);
-      }
+      top[n][0] = fmaxf(s[n][0], s[n][2]);
+      top[n][1] = fmaxf(s[n][1], s[n][3]);
       most = fmax3(most, fmaf(top[n][0], p.scale_log2, -m[n][0]), fmaf(top[n][1], p.scale_log2, -m[n][1]));
     }
     // The lanes' own maxima tell whether any grew past the slack; only then are they joined.
@@ -224,33 +183,28 @@ struct State {
         rescale(n, fmaxf(m[n][0], top[n][0] * p.scale_log2), fmaxf(m[n][1], top[n][1] * p.scale_log2));
       }
     }
-    uint32_t pb[KT][NT][2];
+    uint32_t pb[NT][2];
 #pragma unroll
-    for (int c = 0; c < KT; ++c)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float(&x)[4] = s[c][n];
-        x[0] = fast_exp2(fmaf(x[0], p.scale_log2, -m[n][0]));
-        x[1] = fast_exp2(fmaf(x[1], p.scale_log2, -m[n][1]));
-        x[2] = fast_exp2(fmaf(x[2], p.scale_log2, -m[n][0]));
-        x[3] = fast_exp2(fmaf(x[3], p.scale_log2, -m[n][1]));
-        pb[c][n][0] = transpose8x8(pack_bf16x2(x[0], x[1]));
-        pb[c][n][1] = transpose8x8(pack_bf16x2(x[2], x[3]));
-      }
+    for (int n = 0; n < NT; ++n) {
+      float(&x)[4] = s[n];
+      x[0] = fast_exp2(fmaf(x[0], p.scale_log2, -m[n][0]));
+      x[1] = fast_exp2(fmaf(x[1], p.scale_log2, -m[n][1]));
+      x[2] = fast_exp2(fmaf(x[2], p.scale_log2, -m[n][0]));
+      x[3] = fast_exp2(fmaf(x[3], p.scale_log2, -m[n][1]));
+      pb[n][0] = transpose8x8(pack_bf16x2(x[0], x[1]));
+      pb[n][1] = transpose8x8(pack_bf16x2(x[2], x[3]));
+    }
     // ---- O^T += V^T P^T
     const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
     const uint32_t at = ((mi >> 1) * 8 + ri) * 128 + (((mi & 1) ^ ri) << 4);
 #pragma unroll
-    for (int c = 0; c < KT; ++c) {
+    for (int n = 0; n < NT; ++n) mma_bf16(l[n], ones, pb[n][0], pb[n][1]);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_bf16(l[n], ones, pb[c][n][0], pb[c][n][1]);
+    for (int i = 0; i < 8; ++i) {
+      uint32_t a[4];
+      ldsm_x4_t(((vt + at) ^ ((i & 3) << 5)) + (i >> 2) * HALF_BYTES, a);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t a[4];
-        ldsm_x4_t(((vt + at) ^ ((i & 3) << 5)) + (i >> 2) * HALF_BYTES + c * 2048, a);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma_bf16(o[n][i], a, pb[c][n][0], pb[c][n][1]);
-      }
+      for (int n = 0; n < NT; ++n) mma_bf16(o[n][i], a, pb[n][0], pb[n][1]);
     }
   }
 
@@ -293,15 +247,11 @@ struct State {
   }
 };
 
-// Q in shared memory takes half of the ring; behind the ring are the sums that half of the block's warps hand over
-// to the other.
+// Behind the ring are the sums that half of the block's warps hand over to the other.
 constexpr int SUM_BYTES = 9 * 32 * 16;  // of a tile
-__host__ __device__ constexpr int smem_bytes(int tiles) {
+constexpr int smem_bytes(int tiles) {
   return RING_BYTES + WARPS / 2 * (tiles < 2 ? 2 : tiles) * SUM_BYTES + 1024;  // + alignment to the swizzle's period
 }
-
-// Keys of a chunk: where the rows take several warps a step's latency counts, so that it is made larger.
-__host__ __device__ constexpr int chunk_keys(int team) { return team > 1 ? 32 : 16; }
 
 __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
   float4 v;
@@ -312,33 +262,23 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
   return v;
 }
 
-// Grid: blocks of WARPS warps, WARPS / TEAM teams each; the warps of a team share its ring, each with NT
-// tiles of the pair's rows.  PAIR: clusters, each with a pair (y: sequence, x: head and rank) whose chunks its
-// blocks share; else blocks with equal shares of the line.
-template <int NT, int TEAM, bool PAIR>
+// Grid: blocks of WARPS warps, each with a ring and every WARPS-th chunk of the block's.  PAIR: clusters, each with a
+// pair (y: sequence, x: head and rank) whose chunks its blocks share; else blocks with equal shares of the line.
+template <int NT, bool PAIR>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kernel(const __grid_constant__ Params p) {
-  constexpr int TEAMS = WARPS / TEAM, CK = chunk_keys(TEAM);
   constexpr int TILE_BYTES = CK * HD * 2, STAGE_BYTES = 2 * TILE_BYTES;  // K or V, and both
-  constexpr bool Q_SMEM = NT == 4;
-  constexpr int Q_BYTES = Q_SMEM ? WARPS * NT * 8 * HD * 2 : 0;
-  constexpr int STAGES = (RING_BYTES - Q_BYTES) / TEAMS / STAGE_BYTES;
-  static_assert(STAGES >= 2 && TEAMS * STAGES * STAGE_BYTES + Q_BYTES == RING_BYTES, "the ring is shared out");
+  constexpr int STAGES = RING_BYTES / WARPS / STAGE_BYTES;
   using Span = Span<CK>;
   auto span_of = [&](int len) { return decode_window::span_of<CK>(p, len); };
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_all[TEAMS * STAGES];
-  __shared__ uint32_t read_all[TEAMS * STAGES];  // how often a warp was done with the stage
+  __shared__ __align__(8) uint64_t full_all[WARPS * STAGES];
   if (!PAIR) pdl_launch_dependents();  // the join waits for this grid's end before it reads
   const int warp = warp_id(), lane = lane_id();
   const int r = lane >> 2, t = lane & 3;
   const int G = p.group, Hk = p.num_kv_heads;
-  const int team = warp / TEAM, mate = warp % TEAM;
-  const int row0 = mate * NT * 8;
-  uint64_t* const full = full_all + team * STAGES;
-  uint32_t* const readers = read_all + team * STAGES;
-  if (threadIdx.x < TEAMS * STAGES) {
+  uint64_t* const full = full_all + warp * STAGES;
+  if (threadIdx.x < WARPS * STAGES) {
     mbar_init(full_all + threadIdx.x, 1);
-    read_all[threadIdx.x] = 0;
     fence_mbar_init();
   }
   __syncthreads();
@@ -371,15 +311,13 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
   if (!PAIR && count == 0) return;
 
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* const ring = smem + team * (STAGES * STAGE_BYTES);
+  uint8_t* const ring = smem + warp * (STAGES * STAGE_BYTES);
   float4* const sums = reinterpret_cast<float4*>(smem + RING_BYTES);
-  uint8_t* const q_smem = smem + (RING_BYTES - Q_BYTES) + warp * (NT * 8 * HD * 2);  // (Q_SMEM)
 
-  // ---- the issuing side (lane 0 of each warp): a cursor over the team's chunks.  The warp that is the last to be
-  // done with a chunk fills its stage again, so every warp moves the cursor along, and one of them issues.
-  const int mine = (count - team + TEAMS - 1) / TEAMS;  // chunks team, team + TEAMS, .. of the run
+  // ---- the issuing side (lane 0): a cursor over the warp's chunks
+  const int mine = (count - warp + WARPS - 1) / WARPS;  // chunks warp, warp + WARPS, .. of the run
   Span ahead = span;
-  int a_seq = seq, a_head = head, a_j = j0 + team, issued = 0;
+  int a_seq = seq, a_head = head, a_j = j0 + warp, issued = 0;
   int a_row = 0, a_index = 0, a_page = -1;  // its row in its page, the page of the sequence, the page's number
   auto load_page = [&]() {
     a_page = a_index < p.table_width ? __ldg(p.block_tables + a_seq * p.table_stride + a_index) : -1;
@@ -398,25 +336,23 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
     a_row = key - a_index * p.block_size;
     load_page();
   };
-  auto issue = [&](bool copy) {  // chunk `issued` of the team
+  auto issue = [&]() {  // chunk `issued` of the warp
     const int stage = issued % STAGES;
     uint64_t* bar = full + stage;
     uint8_t* st = ring + stage * STAGE_BYTES;
-    if (copy) {
-      int slot = a_page * p.block_size + a_row;
-      if ((uint32_t)a_page >= (uint32_t)p.num_pages) {  // the table has no usable page there: recorded, zeros come
-        record_error(VLC_DEV_ERR_BLOCK_RANGE);
-        slot = p.num_pages * p.block_size;
-      }
-      mbar_expect_tx(bar, STAGE_BYTES);
-      tma_load_5d(st, &p.kv[0], bar, 0, a_head, slot, 0, 0);
-      if (!p.joined) tma_load_5d(st + TILE_BYTES, &p.kv[1], bar, 0, a_head, slot, 0, 0);
+    int slot = a_page * p.block_size + a_row;
+    if ((uint32_t)a_page >= (uint32_t)p.num_pages) {  // the table has no usable page there: recorded, zeros come
+      record_error(VLC_DEV_ERR_BLOCK_RANGE);
+      slot = p.num_pages * p.block_size;
     }
+    mbar_expect_tx(bar, STAGE_BYTES);
+    tma_load_5d(st, &p.kv[0], bar, 0, a_head, slot, 0, 0);
+    if (!p.joined) tma_load_5d(st + TILE_BYTES, &p.kv[1], bar, 0, a_head, slot, 0, 0);
     if (++issued == mine) return;
     // the next chunk's place, whose page is there by the next call
-    a_j += TEAMS;
-    a_row += TEAMS * CK;
-    if (a_j >= ahead.count || (a_j >= ahead.first && a_j - TEAMS < ahead.first)) {
+    a_j += WARPS;
+    a_row += WARPS * CK;
+    if (a_j >= ahead.count || (a_j >= ahead.first && a_j - WARPS < ahead.first)) {
       place();
     } else if (a_row >= p.block_size) {
       do {
@@ -428,19 +364,19 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
   };
   if (lane == 0 && mine > 0) {
     place();
-    for (int i = 0; i < min(STAGES, mine); ++i) issue(mate == 0);
+    for (int i = 0; i < min(STAGES, mine); ++i) issue();
   }
-  // Whether the team's chunk i came (recorded where it did not).
+  // Whether the warp's chunk i came (recorded where it did not).
   auto arrived = [&](int i) {
     const uint32_t parity = (uint32_t)(i / STAGES) & 1u;
     if (mbar_try_wait(full + i % STAGES, parity)) return true;
     return mbar_wait_bounded(full + i % STAGES, parity, VLC_DEV_ERR_TIMEOUT + 26, VLC_WAIT_LIMIT_CYCLES);
   };
 
-  const uint32_t ring_u = smem_u32(ring), q_u = smem_u32(q_smem);
-  State<NT, CK, Q_SMEM> state;
-  int i = 0;        // the team's chunks so far
-  bool ok = true;   // its waits so far: a team that gave up takes no more chunks
+  const uint32_t ring_u = smem_u32(ring);
+  State<NT> state;
+  int i = 0;        // the warp's chunks so far
+  bool ok = true;   // its waits so far: a warp that gave up takes no more chunks
   for (int done = 0, first_slot = 0; PAIR || done < count; first_slot = 1) {
     // ---- the pair's chunks [done, done + n) of the run
     const int n = PAIR ? count : min(span.count - j0, count - done);
@@ -449,10 +385,10 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
     if (!PAIR && j0 == 0 && threadIdx.x == 0)
       p.places[(int64_t)seq * Hk + head] = make_int2((int)blockIdx.x * 2 + first_slot,
                                                      (int)(shares.block_of(c0 + done + span.count - 1) - blockIdx.x) + 1);
-    state.start(p, seq, head, row0, r, t, q_smem);
+    state.start(p, seq, head, r, t);
     const int all0 = span.all0(p), all1 = span.all1(p), all2 = span.all2(p);
     const uint32_t k_off = p.v_first ? TILE_BYTES : 0, v_off = p.v_first ? 0 : TILE_BYTES;
-    for (int j = j0 + i * TEAMS + team - done; ok && j < j0 + n; j += TEAMS, ++i) {
+    for (int j = j0 + i * WARPS + warp - done; ok && j < j0 + n; j += WARPS, ++i) {
       if (!__all_sync(0xffffffffu, arrived(i))) {
         ok = false;
         break;
@@ -461,24 +397,13 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
       const uint32_t st = ring_u + stage * STAGE_BYTES;
       const int key0 = (j < span.first ? j : j + span.jump) * CK;
       const bool all_seen = j < all0 || (j >= all1 && j < all2);
-      state.step(p, st + k_off, st + v_off, key0, !all_seen, span, row0, lane, q_u);
+      state.step(p, st + k_off, st + v_off, key0, !all_seen, span, lane);
       __syncwarp();  // every lane has read the stage
-      if (lane == 0 && issued < mine) {
-        bool last = true;
-        if (TEAM > 1) {
-          uint32_t before;  // (released to and acquired from the mates: their reads are done)
-          asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;"
-                       : "=r"(before)
-                       : "r"(smem_u32(readers + stage))
-                       : "memory");
-          last = (before + 1) % TEAM == 0;
-        }
-        issue(last);
-      }
+      if (lane == 0 && issued < mine) issue();
     }
-    // ---- the teams' sums: the upper half of the warps hand theirs over until one team has them
+    // ---- the warps' sums: the upper half hand theirs over until one warp has them
 #pragma unroll
-    for (int half = WARPS / 2; half >= TEAM; half /= 2) {
+    for (int half = WARPS / 2; half >= 1; half /= 2) {
       float4* const to = sums + (warp % half) * (NT * 9 * 32);
       __syncthreads();
       if (warp >= half && warp < 2 * half) {
@@ -498,9 +423,9 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
       }
       __syncthreads();
       float4* const own = reinterpret_cast<float4*>(smem);
-      if (team == 0) {
+      if (warp == 0) {
 #pragma unroll
-        for (int x = 0; x < NT; ++x) state.put(x, own + (mate * NT + x) * (9 * 32), lane);
+        for (int x = 0; x < NT; ++x) state.put(x, own + x * (9 * 32), lane);
       }
       cluster_sync();
       for (int tile = warp; tile * 8 < p.rows; tile += WARPS) {
@@ -545,13 +470,13 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) window_decode_kerne
       cluster_sync();  // the others have read this block's sums
       return;
     }
-    if (!PAIR && team == 0) {
+    if (!PAIR && warp == 0) {
       const bool whole = j0 == 0 && n == span.count;
       const int64_t slot = ((int64_t)blockIdx.x * 2 + first_slot) * p.rows;
 #pragma unroll
       for (int x = 0; x < NT * 2; ++x) {
         const int nt = x >> 1, odd = x & 1;
-        const int row = row0 + nt * 8 + 2 * t + odd;
+        const int row = nt * 8 + 2 * t + odd;
         if (row >= p.rows) continue;
         const float sum = state.l[nt][odd];
         if (whole) {
@@ -670,21 +595,11 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
   }
 }
 
-// Warps of a team and row tiles of a warp: the fewest warps whose registers hold the rows.
-struct Shape {
-  int tiles, team;
-  int keys() const { return chunk_keys(team); }
-};
-static Shape shape_of(int rows) {
-  if (rows <= 8) return {1, 1};
-  if (rows <= 16) return {2, 1};
-  if (rows <= 24) return {3, 1};
-  if (rows <= 32) return {2, 2};
-  if (rows <= 48) return {3, 2};
-  if (rows <= 64) return {2, 4};
-  if (rows <= 96) return {3, 4};
-  return {4, 4};
-}
+// Whether decode_window_wide.cu takes the call.  40 rows, there : here (by teams of warps, clusters where they were
+// faster), us: one sequence of 500 keys and 2 KV heads 9.8 : 9.4, of 2000 10.2 : 12.9, of 8000 12.8 : 15.2; eight of 2000
+// 14.7 : 14.9; sixteen of 8000 32.0 : 34.4; 32 of 4000 32.7 : 34.4.  64 rows: 11.2 : 9.8, 11.6 : 11.9, 14.1 : 14.1; 16.0 : 18.7;
+// 34.0 : 44.8; 35.9 : 45.1.
+static bool wide_of(int rows) { return rows > WIDE_ROWS; }
 
 // Most chunks that any sequence has under the host's bound.
 static int64_t most_chunks(int CK, int tokens, int max_context_len, int window, int sinks) {
@@ -695,33 +610,28 @@ static int64_t most_chunks(int CK, int tokens, int max_context_len, int window, 
 
 // Blocks of the cluster that takes a pair, or 0 for the line.  The line's shares are even whatever the lengths
 // are, and its blocks many where the pairs are few; a pair's cluster saves the second launch.  Pair : line, us, of
-// 16 query and 2 KV heads, one token (five): one sequence of 500 keys 6.3 : 8.0 (10.6 : 11.2), of 2000 7.8 : 9.9
-// (13.7 : 15.1), of 4000 9.9 : 9.6 (17.7 : 15.0), of 8000 14.3 : 10.6 (25.8 : 15.7); eight of 4000 11.1 : 13.1
-// (20.7 : 22.1); sixteen of 8000 26.2 : 30.8 (35.0 : 40.8); 64 of 4000 46.3 : 48.4 (59.7 : 61.0).  So a team takes
+// 16 query and 2 KV heads, one token: one sequence of 500 keys 6.3 : 8.0, of 2000 7.8 : 9.9, of 4000 9.9 : 9.6, of
+// 8000 14.3 : 10.6; eight of 4000 11.1 : 13.1; sixteen of 8000 26.2 : 30.8; 64 of 4000 46.3 : 48.4.  So a warp takes
 // up to 8 chunks, or 16 where the clusters fill half of the GPU (beyond that ragged lengths would leave it idle).
 static int cluster_of(int num_seqs, int num_kv_heads, int rows, int tokens, int max_context_len, int window, int sinks,
                       int num_sms) {
-  const Shape shape = shape_of(rows);
+  if (wide_of(rows)) return 0;
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads, resident = (int64_t)num_sms * BLOCKS_PER_SM;
   int cluster = 8;
   while (cluster > 1 && pairs * cluster > resident) cluster /= 2;
-  const int64_t chunks = most_chunks(shape.keys(), tokens, max_context_len, window, sinks);
-  const int64_t most = (2 * pairs * cluster >= resident ? 16 : 8) * cluster * (WARPS / shape.team);
+  const int64_t chunks = most_chunks(CK, tokens, max_context_len, window, sinks);
+  const int64_t most = (2 * pairs * cluster >= resident ? 16 : 8) * cluster * WARPS;
   return cluster > 1 && chunks <= most ? cluster : 0;
 }
 
-// Whether decode_window_wide.cu takes the line.
-static bool wide_of(int rows) { return rows > WIDE_ROWS; }
-
 // Blocks of the grid: from host values only, so that it is fixed for graph capture.  A block has at least
-// MIN_CHUNKS for each of its teams: few chunks, but fewer parts to join.
+// MIN_CHUNKS for each of its warps: few chunks, but fewer parts to join.
 constexpr int MIN_CHUNKS = 2;
 static int grid_blocks(int num_seqs, int num_kv_heads, int rows, int tokens, int max_context_len, int window, int sinks,
                        int num_sms) {
   const bool wide = wide_of(rows);
-  const Shape shape = shape_of(rows);
-  const int64_t chunks = most_chunks(wide ? WIDE_CHUNK : shape.keys(), tokens, max_context_len, window, sinks);
-  const int least = wide ? 1 : MIN_CHUNKS * (WARPS / shape.team);
+  const int64_t chunks = most_chunks(wide ? WIDE_CHUNK : CK, tokens, max_context_len, window, sinks);
+  const int least = wide ? 1 : MIN_CHUNKS * WARPS;
   const int64_t most = (num_seqs * num_kv_heads * chunks + least - 1) / least;
   return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)num_sms * (wide ? 1 : BLOCKS_PER_SM), most));
 }
@@ -739,11 +649,11 @@ static bool sizes_ok(int num_seqs, int tokens, int num_heads, int num_kv_heads, 
          (int64_t)num_seqs * num_kv_heads <= 0x7fffffff;
 }
 
-template <int NT, int TEAM>
+template <int NT>
 static int launch(const Params& p, cudaStream_t st) {
   static std::atomic<uint64_t> smem[2];
   const bool pair = p.cluster > 0;
-  const auto kernel = pair ? window_decode_kernel<NT, TEAM, true> : window_decode_kernel<NT, TEAM, false>;
+  const auto kernel = pair ? window_decode_kernel<NT, true> : window_decode_kernel<NT, false>;
   if (ensure_dynamic_smem((const void*)kernel, smem_bytes(NT), smem[pair]) != VLC_OK) return VLC_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = pair ? dim3(p.cluster * p.num_kv_heads, p.num_seqs) : dim3(p.num_blocks);
@@ -802,7 +712,6 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
   if (num_pages <= 0 || num_pages > 0x7fffffff / block_size) return VLC_ERR_SHAPE;
   max_context_len = std::max(1, max_context_len);
   const int sms = vlc_num_sms(), rows = G * num_tokens;
-  const Shape shape = shape_of(rows);
   const int blocks = grid_blocks(num_seqs, num_kv_heads, rows, num_tokens, max_context_len, window, sinks, sms);
   const int cluster = cluster_of(num_seqs, num_kv_heads, rows, num_tokens, max_context_len, window, sinks, sms);
   if (!cluster) {
@@ -811,7 +720,7 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
     if (!aligned16(workspace)) return VLC_ERR_ALIGN;
   }
 
-  const bool wide = !cluster && wide_of(rows);
+  const bool wide = wide_of(rows);
   Params p;
   const uint8_t* caches[2] = {(const uint8_t*)k_cache, (const uint8_t*)v_cache};
   p.v_first = !wide && caches[1] < caches[0];
@@ -822,7 +731,7 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
     std::swap(caches[0], caches[1]);
     p.v_first = false;
   }
-  p.box = wide ? block_size % 64 == 0 ? 64 : 32 : shape.keys();
+  p.box = wide ? block_size % 64 == 0 ? 64 : 32 : CK;
   const uint64_t slots = (uint64_t)num_pages * block_size, row = (uint64_t)num_kv_heads * HD * 2;
   for (int i = 0; i < (p.joined ? 1 : 2); ++i) {
     const uint64_t both = p.joined ? 2 : 1;
@@ -859,18 +768,7 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
   p.places = (int2*)(p.part_ml + (int64_t)blocks * 2 * rows);
 
   cudaStream_t st = (cudaStream_t)stream;
-  int rc;
-  if (wide) rc = launch_wide(p, st);
-  else switch (shape.team * 8 + shape.tiles) {
-    case 8 + 1: rc = launch<1, 1>(p, st); break;
-    case 8 + 2: rc = launch<2, 1>(p, st); break;
-    case 8 + 3: rc = launch<3, 1>(p, st); break;
-    case 16 + 2: rc = launch<2, 2>(p, st); break;
-    case 16 + 3: rc = launch<3, 2>(p, st); break;
-    case 32 + 2: rc = launch<2, 4>(p, st); break;
-    case 32 + 3: rc = launch<3, 4>(p, st); break;
-    default: rc = launch<4, 4>(p, st);
-  }
+  const int rc = wide ? launch_wide(p, st) : rows <= 8 ? launch<1>(p, st) : rows <= 16 ? launch<2>(p, st) : launch<3>(p, st);
   if (rc != VLC_OK || cluster) return rc;
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads;
   const bool spread = blocks / pairs + 1 > 10;

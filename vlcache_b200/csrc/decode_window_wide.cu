@@ -10,6 +10,19 @@
 // its row's maximum by 2^8; P goes to shared memory as the second product's B operand, 16 bytes a store.  Roles (a
 // block an SM, 12 warps): K and V copies, products, Q, softmax (8).  The next chunk's S is made while this one's
 // softmax runs; S, O and Q have two buffers each, so that the next pair starts while this one's O is written.
+//
+// P is rounded to bf16 as an operand has to be, and its sums are of the rounded values; scores, maxima, sums and O are
+// fp32.
+//
+// Measured (64 sequences of 2700 .. 10700 keys, window 4096, 28 query and 4 KV heads; floor 83 us): 28 rows 94.5 us, 35
+// 96, 56 101, 63 102, 91 120, 112 178.  Up to 48 rows HBM bounds it: 4.5 us until the first S, the join and the last
+// chunks 5, between them 0.96 of the floor (a ring of 4 slots instead of 5 costs 0.5).  With more the softmax's time
+// counts (2000 cycles a chunk of 64 rows), then registers: a thread's sums of P.  Tried: the exponentials or the products
+// left out, for a time only: no change, so the chains of waits count and not the pipes; pages' numbers four chunks ahead,
+// unrolled: 98 and 104 for 35 and 56 rows (more code, which the roles' caches feel); P and the slow path in one loop, one
+// copy of each: 99 and 107; one copy of 32 KB a tile instead of four of 8: no change; four shares of the rows: no change
+// for 56, 127 for 91, but 178 instead of 195 for 112.  Rows' output offsets and 1 / sum made once, not by each thread, and
+// maxima and sums over lanes that halve the columns: 112 -> 96.
 #include <algorithm>
 #include <cmath>
 
@@ -21,20 +34,21 @@ namespace decode_window {
 namespace wide {
 
 constexpr int CK = WIDE_CHUNK;
-constexpr int THREADS = 384;
-constexpr int FIRST_SOFTMAX = 4;              // warp; the eight from there on, four for each half of the rows
+constexpr int FIRST_SOFTMAX = 4;              // warp; four for each share of the rows from there on
 constexpr int HALF_BYTES = CK * 128;          // 64 dims of a chunk's keys
 constexpr int TILE_BYTES = 2 * HALF_BYTES;    // K or V
 constexpr uint32_t DESC_HI = umma_desc_sw128_hi(1024);
 
 template <int N>
 struct Layout {
+  static constexpr int SIDES = N <= 96 ? 2 : 4;  // shares of the rows: a thread's sums of P are registers
+  static constexpr int THREADS = (FIRST_SOFTMAX + 4 * SIDES) * 32;
   static constexpr int SLOTS = N <= 64 ? 5 : 4;  // of the ring of K and V
   static constexpr int Q_BUFFERS = N <= 96 ? 2 : 1, Q_BYTES = N * HD * 2;
   static constexpr int P_BYTES = (N + 63) / 64 * HALF_BYTES;  // 64 rows of each key, then the next 64
   static constexpr int Q = SLOTS * TILE_BYTES, P = Q + Q_BUFFERS * Q_BYTES;
   static constexpr int ROWS = P + P_BYTES;       // where a row's output is, from the pair's on
-  static constexpr int FLOATS = ROWS + N * 8;    // m[N], factor[N], tops[2 halves][4 warps][N / 2]
+  static constexpr int FLOATS = ROWS + N * 8;    // m[N], factor[N], tops[SIDES][4 warps][N / SIDES]
   static constexpr int BARS = FLOATS + 6 * N * 4;
   static constexpr int NUM_BARS = 2 * SLOTS + 13;
   static constexpr int MISC = BARS + NUM_BARS * 8;
@@ -104,9 +118,10 @@ __device__ __forceinline__ int k_load(int i) { return i == 0 ? 0 : 2 * i - 1; }
 __device__ __forceinline__ int v_load(int i, int n) { return i + 1 < n ? 2 * i + 2 : 2 * n - 1; }
 
 template <int N>  // columns: rows, padded
-__global__ void __launch_bounds__(THREADS, 1) window_decode_wide_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kernel(const __grid_constant__ Params p) {
   using L = Layout<N>;
-  constexpr int NC = N / 2;  // of a softmax thread
+  constexpr int SIDES = L::SIDES, THREADS = L::THREADS;
+  constexpr int NC = N / SIDES;  // of a softmax thread
   constexpr uint32_t IDESC_S = umma_idesc_bf16(128, N, false, false);
   constexpr uint32_t IDESC_O = umma_idesc_bf16(128, N, true, true);
   extern __shared__ uint8_t smem_raw[];
@@ -137,10 +152,10 @@ __global__ void __launch_bounds__(THREADS, 1) window_decode_wide_kernel(const __
       mbar_init(q_full + x, 64);
       mbar_init(q_empty + x, 1);
       mbar_init(s_full + x, 1);
-      mbar_init(s_empty + x, 8);
-      mbar_init(o_empty + x, 8);
+      mbar_init(s_empty + x, 4 * SIDES);
+      mbar_init(o_empty + x, 4 * SIDES);
     }
-    mbar_init(p_full, 8);
+    mbar_init(p_full, 4 * SIDES);
     mbar_init(p_empty, 1);
     mbar_init(drain, 1);
     fence_mbar_init();
@@ -289,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, 1) window_decode_wide_kernel(const __
       const int b = pair % L::Q_BUFFERS;
       if (pair >= L::Q_BUFFERS && !wait(q_empty + b, pair / L::Q_BUFFERS - 1, 35)) break;
       uint8_t* const to = smem + L::Q + b * L::Q_BYTES + (piece >> 3) * (N * 128);
-      constexpr int LOADS = N <= 64 ? N / 4 : N / 8;  // at once
+      constexpr int LOADS = N <= 64 ? N / 4 : 8;  // at once
 #pragma unroll
       for (int first = 0; first < N; first += LOADS * 4) {
         uint4 v[LOADS];
@@ -321,7 +336,7 @@ __global__ void __launch_bounds__(THREADS, 1) window_decode_wide_kernel(const __
       if (done < count) at.next_pair(p);
     }
   } else {
-    // ------------------------------------------------------------ softmax: a thread has a key, and a half of the rows.
+    // ------------------------------------------------------------ softmax: a thread has a key, and a share of the rows.
     // After a wait that gave up a thread goes on through all chunks (later waits end at once), so that the named
     // barriers stay matched.
     const int side = (warp - FIRST_SOFTMAX) >> 2, quarter = warp & 3, key_lane = quarter * 32 + lane;
@@ -443,9 +458,10 @@ __global__ void __launch_bounds__(THREADS, 1) window_decode_wide_kernel(const __
           const int load = v_load(i, count), ring_slot = load % L::SLOTS;
           wait(full + ring_slot, load / L::SLOTS, 38);
           if (key >= span.len || (key < span.low && key >= p.sinks)) {
-            uint4* const v = reinterpret_cast<uint4*>(smem + ring_slot * TILE_BYTES + side * HALF_BYTES + key_lane * 128);
+            uint4* const v = reinterpret_cast<uint4*>(smem + ring_slot * TILE_BYTES + side * 2 / SIDES * HALF_BYTES +
+                                                          key_lane * 128 + side % (SIDES / 2) * (256 / SIDES));
 #pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] = make_uint4(0, 0, 0, 0);
+            for (int x = 0; x < 16 / SIDES; ++x) v[x] = make_uint4(0, 0, 0, 0);
           }
         }
         fence_proxy_async_smem();
@@ -496,7 +512,7 @@ static int launch(const Params& p, cudaStream_t st) {
   static std::atomic<uint64_t> smem{0};
   const auto kernel = window_decode_wide_kernel<N>;
   if (ensure_dynamic_smem((const void*)kernel, Layout<N>::BYTES, smem) != VLC_OK) return VLC_ERR_CUDA;
-  kernel<<<p.num_blocks, THREADS, Layout<N>::BYTES, st>>>(p);
+  kernel<<<p.num_blocks, Layout<N>::THREADS, Layout<N>::BYTES, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? VLC_OK : VLC_ERR_CUDA;
 }
 
