@@ -477,8 +477,8 @@ int vlc_remap_block_tables(int32_t* block_tables, int64_t row_stride, int num_ro
  *
  * vlc_attention_plan_window: vlc_attention_plan with that mask (causal plans; capacity and
  *   workspace as there); vlc_prefill_attn and vlc_prefill_attn_inflight follow the plan, and
- *   take a positive softmax_scale only.  A window that no sequence outgrows gives the plan
- *   without one.
+ *   take a positive softmax_scale only.  A window that no sequence outgrows, and a window of 0, give the
+ *   plan without one, unless tiles are split there: parts of split tiles keep 32 bits in windowed plans.
  * vlc_decode_attn_window: the last num_tokens tokens of each sequence (its key and value rows
  *   are in the cache, context_lens counts them): q / out [num_seqs * num_tokens, num_heads, 128]
  *   with any token stride, row i num_tokens + r being token context_lens[i] - num_tokens + r of

@@ -100,6 +100,22 @@ def test_window_that_hides_nothing_is_the_plan_without(cuda_lib):
     assert c.num_parts > 0 and c.workspace_bytes == c.num_parts * 128 * (128 * 4 + 8)   # parts in fp32
 
 
+def test_window_of_0_is_the_plan_without_but_for_split_tiles(cuda_lib):
+    from vlcache_b200 import ops
+    a = ops.build_prefill_plan([0, 700], [0, 900], 16, 2, num_sms=16, window=0)
+    b = ops.build_prefill_plan([0, 700], [0, 900], 16, 2, num_sms=16)
+    assert a.num_parts == 0 and np.array_equal(a.host, b.host)
+    for window in (0, 9000):
+        a = ops.build_prefill_plan([0, 20], [0, 9000], 16, 2, num_sms=148, window=window)
+        b = ops.build_prefill_plan([0, 20], [0, 9000], 16, 2, num_sms=148)
+        assert a.num_parts == b.num_parts > 0 and a.num_units == b.num_units
+        assert a.workspace_bytes == a.num_parts * 128 * (128 * 4 + 8)
+        assert b.workspace_bytes == b.num_parts * 128 * (128 * 2 + 8)   # bf16, as plans without a window were
+    a = ops.build_prefill_plan([0, 20], [0, 9000], 16, 2, num_sms=148, window=0, causal=False)
+    b = ops.build_prefill_plan([0, 20], [0, 9000], 16, 2, num_sms=148, causal=False)
+    assert np.array_equal(a.host, b.host)
+
+
 def test_window_plan_refusals(cuda_lib):
     from vlcache_b200 import ops
     from vlcache_b200._lib import VLCError

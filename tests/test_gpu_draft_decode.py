@@ -984,3 +984,25 @@ def test_decode_window_many_rows_pages_beyond_4_gb():
     q = torch.randn(2, 5, 28, D, generator=g, device="cuda").to(torch.bfloat16)
     got = _decode(tables, [400, 512], None, q, both[0], both[1], 300, 4, 0.1)
     _check_decode(got, tables, [400, 512], 5, q, both[0], both[1], 300, 4, 0.1)
+
+
+@pytest.mark.parametrize("head_dim", [80, 128])
+@pytest.mark.parametrize("window", [0, 6000, 20000])
+def test_prefill_window_split_tiles_that_see_all_keys(head_dim, window):
+    """No window, and windows that hide nothing: the parts of split tiles are fp32, P's rounding and the output's
+    are the only ones."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(head_dim)
+    new, lens = [48, 9], [6000, 500]
+    cu_q, cu_k = np.cumsum([0] + new), np.cumsum([0] + lens)
+    q, k, v = (torch.randn(n, h, head_dim, generator=g, device="cuda").to(torch.bfloat16)
+               for n, h in ((57, 16), (6500, 2), (6500, 2)))
+    plan = ops.build_prefill_plan(cu_q, cu_k, 16, 2, head_dim, device="cuda", window=window)
+    assert plan.num_parts > 0
+    got = ops.prefill_attention(q, k, v, None, plan, 0.1)
+    assert ops.device_error() == 0
+    for i, (n, m) in enumerate(zip(new, lens)):
+        want, rms = oracle.attention(q[cu_q[i]:cu_q[i + 1]].double(), k[cu_k[i]:cu_k[i + 1]].double(),
+                                     v[cu_k[i]:cu_k[i + 1]].double(), torch.arange(m - n, m, device="cuda"), 0, 0, 0.1)
+        tol = (STEP + 2.0 ** -12) * (rms + want.abs()) + 1e-30
+        assert bool(((got[cu_q[i]:cu_q[i + 1]].double() - want).abs() <= tol).all())

@@ -65,7 +65,7 @@ def _prefill_plan(context: Context, num_heads: int, num_kv_heads: int, device: t
         if ck is None:
             ck = context.cu_seqlens_k.cpu().numpy()
         plan = ops.build_prefill_plan(np.asarray(cq), np.asarray(ck), num_heads, num_kv_heads,
-                                      device=device, window=window, sinks=sinks)
+                                      device=device, window=window or None, sinks=sinks)
         if window:
             context.window_plans[window, sinks] = plan
         else:

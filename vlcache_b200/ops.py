@@ -238,12 +238,13 @@ def set_prefill_kernel(mode: int) -> None:
 
 def build_prefill_plan(cu_seqlens_q, cu_seqlens_k, num_heads: int, num_kv_heads: int, head_dim: int = HEAD_DIM,
                        num_sms: int = 0, device: torch.device | str | None = None, causal: bool = True,
-                       window: int = 0, sinks: int = 0) -> PrefillPlan:
+                       window: int | None = None, sinks: int = 0) -> PrefillPlan:
     """Plan the warm-prefill attention launch from HOST cu_seqlens (lists/arrays/CPU tensors).
     ``causal=False`` plans the non-causal varlen attention (every row sees all keys of its
     sequence); ``head_dim`` may be 80..128 in steps of 16.  ``window`` > 0: a row at position t sees
     key j <= t iff j > t - window or j < ``sinks``; pages that no row sees are not read (their
-    block-table entries may be -1)."""
+    block-table entries may be -1).  Parts of tiles that several CTAs share are bf16 without
+    ``window`` and fp32 with one, 0 (every key is visible) among them."""
     cq = np.ascontiguousarray(np.asarray(cu_seqlens_q, dtype=np.int32))
     ck = np.ascontiguousarray(np.asarray(cu_seqlens_k, dtype=np.int32))
     nseq = len(cq) - 1
@@ -256,10 +257,12 @@ def build_prefill_plan(cu_seqlens_q, cu_seqlens_k, num_heads: int, num_kv_heads:
         raise ValueError("invalid prefill metadata (cu_seqlens / heads)")
     plan = np.empty(int(cap), dtype=np.int32)   # (the planner writes all that it uses; zeroing 15 MB took 0.7 ms)
     used = ctypes.c_int64(0)
-    st = L.vlc_attention_plan_window(cq.ctypes.data, ck.ctypes.data, nseq, num_heads, num_kv_heads, head_dim,
-                                     1 if causal else 0, int(window), int(sinks), sms, plan.ctypes.data, int(cap),
-                                     ctypes.byref(used))
-    check("vlc_attention_plan_window", st)
+    sizes = (cq.ctypes.data, ck.ctypes.data, nseq, num_heads, num_kv_heads, head_dim, 1 if causal else 0)
+    room = (sms, plan.ctypes.data, int(cap), ctypes.byref(used))
+    if window is None:
+        check("vlc_attention_plan", L.vlc_attention_plan(*sizes, *room))
+    else:
+        check("vlc_attention_plan_window", L.vlc_attention_plan_window(*sizes, int(window), int(sinks), *room))
     plan = plan[: used.value].copy()
     ws = int(L.vlc_prefill_workspace_size(plan.ctypes.data))
     dev = None
