@@ -595,10 +595,10 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
   }
 }
 
-// Whether decode_window_wide.cu takes the call.  40 rows, there : here (by teams of warps, clusters where they were
-// faster), us: one sequence of 500 keys and 2 KV heads 9.8 : 9.4, of 2000 10.2 : 12.9, of 8000 12.8 : 15.2; eight of 2000
-// 14.7 : 14.9; sixteen of 8000 32.0 : 34.4; 32 of 4000 32.7 : 34.4.  64 rows: 11.2 : 9.8, 11.6 : 11.9, 14.1 : 14.1; 16.0 : 18.7;
-// 34.0 : 44.8; 35.9 : 45.1.
+// Whether decode_window_wide.cu takes the call.  There : here (by teams of warps, by clusters where they were faster), us.
+// 40 rows: one sequence of 500 keys and 2 KV heads 9.8 : 9.4, of 2000 10.2 : 12.9, of 8000 12.8 : 15.2; eight of 2000
+// 14.7 : 14.9; sixteen of 8000 32.0 : 34.4; 32 of 4000 32.7 : 34.4.  64 rows, the same: 11.2 : 9.8, 11.6 : 11.9,
+// 14.1 : 14.1, 16.0 : 18.7, 34.0 : 44.8, 35.9 : 45.1.
 static bool wide_of(int rows) { return rows > WIDE_ROWS; }
 
 // Most chunks that any sequence has under the host's bound.
@@ -731,13 +731,12 @@ extern "C" int vlc_decode_attn_window(const void* q, int64_t q_token_stride, int
     std::swap(caches[0], caches[1]);
     p.v_first = false;
   }
-  p.box = wide ? block_size % 64 == 0 ? 64 : 32 : CK;
   const uint64_t slots = (uint64_t)num_pages * block_size, row = (uint64_t)num_kv_heads * HD * 2;
   for (int i = 0; i < (p.joined ? 1 : 2); ++i) {
     const uint64_t both = p.joined ? 2 : 1;
     const uint64_t dims[5] = {64, (uint64_t)num_kv_heads, slots, 2, both};
     const uint64_t strides[4] = {HD * 2, row, 128, p.joined ? apart : 256};
-    const uint32_t box[5] = {64, 1, (uint32_t)p.box, wide ? 1u : 2u, (uint32_t)both};
+    const uint32_t box[5] = {64, 1, (uint32_t)(wide ? WIDE_BOX : CK), wide ? 1u : 2u, (uint32_t)both};
     if (encode_tmap_bf16(&p.kv[i], caches[i], wide ? 4 : 5, dims, strides, box, 128) != VLC_OK) return VLC_ERR_CUDA;
   }
   p.q = (const __nv_bfloat16*)q;

@@ -14,8 +14,9 @@ constexpr float SLACK = 8.f;            // log2 that the maximum may grow by bef
 constexpr float NO_MAX = -3e38f;        // the maximum of no key (finite: differences of two are numbers)
 
 struct Params {
-  // {64 dims, Hk, slots, 2 halves of a row, caches}, box {64, 1, CK, 2, caches} of chunks of CK keys.  Joined, the caches are
+  // decode_window.cu: {64 dims, Hk, slots, 2 halves of a row, caches}, box {64, 1, 16, 2, caches}.  Joined, the caches are
   // the two, whose stride is their distance (v_first: V lies before K); else kv[0] is K and kv[1] V.
+  // decode_window_wide.cu: K and V, {64 dims, Hk, slots, 2 halves}, box {64, 1, WIDE_BOX, 1}.
   CUtensorMap kv[2];
   bool joined, v_first;
   const __nv_bfloat16* q;
@@ -28,7 +29,6 @@ struct Params {
   int group, num_kv_heads, rows;  // rows = tokens * group
   uint32_t group_inverse;         // 2^16 / group, rounded up: exact for rows below 128
   __device__ __forceinline__ int token_of(int row) const { return (int)((uint32_t)row * group_inverse >> 16); }
-  int box;                        // keys of a copy (decode_window_wide.cu)
   int cluster;                    // blocks of a pair's cluster (0: the line)
   float scale_log2;               // |softmax scale| * log2(e), above 0: a hidden key's score stays -infinity
   uint32_t q_flip;                // the signs of a pair of q's elements where the scale is negative
@@ -143,6 +143,7 @@ __device__ __forceinline__ Shares run_of(const Params& p, Run<CK>& run, int warp
 
 // decode_window_wide.cu: chunks of WIDE_CHUNK keys, a block an SM.
 constexpr int WIDE_CHUNK = 128;
+constexpr int WIDE_BOX = 32;  // keys of a copy; a box of keys that no row sees is not read
 int launch_wide(const Params& p, cudaStream_t st);
 
 }  // namespace decode_window

@@ -14,9 +14,10 @@
 // P is rounded to bf16 as an operand has to be, and its sums are of the rounded values; scores, maxima, sums and O are
 // fp32.
 //
-// Measured (64 sequences of 2700 .. 10700 keys, window 4096, 28 query and 4 KV heads; floor 83 us): 28 rows 94.5 us, 35
-// 96, 56 101, 63 102, 91 120, 112 178.  Up to 48 rows HBM bounds it: 4.5 us until the first S, the join and the last
-// chunks 5, between them 0.96 of the floor (a ring of 4 slots instead of 5 costs 0.5).  With more the softmax's time
+// Measured (64 sequences of 2700 .. 10700 keys, window 4096, 28 query and 4 KV heads; floor 83 us): 28 rows 93 us, 35
+// 95, 56 100, 63 101, 91 121, 112 178.  Up to 48 rows HBM bounds it: 4.5 us until the first S, the join and the last
+// chunks 5, between them 0.97 of the floor (a ring of 4 slots instead of 5 costs 0.5).  Copies of 32 keys: of 64, a window's ends
+// waste more (96.7 -> 94.6 on one GPU, 97.9 on another), of 16 the copies count (112).  With more the softmax's time
 // counts (2000 cycles a chunk of 64 rows), then registers: a thread's sums of P.  Tried: the exponentials or the products
 // left out, for a time only: no change, so the chains of waits count and not the pipes; pages' numbers four chunks ahead,
 // unrolled: 98 and 104 for 35 and 56 rows (more code, which the roles' caches feel); P and the slow path in one loop, one
@@ -177,8 +178,9 @@ __global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kern
   };
 
   if (warp == 0) {
-    // ------------------------------------------------------------ K and V copies: a lane each box of `box` keys
-    const int boxes = CK / p.box;
+    // ------------------------------------------------------------ K and V copies: a lane each box of keys
+    constexpr int BOXES = CK / WIDE_BOX;
+    static_assert(MIN_BLOCK % WIDE_BOX == 0, "a box lies in one page");
     struct Entry {
       int page, row, head;
       bool seen;  // some row sees some key of the box
@@ -186,11 +188,11 @@ __global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kern
     Run<CK> at = run;
     int left = count;
     auto fetch = [&]() {  // the box of the cursor's chunk, and on
-      const int j = at.j0, key = (j < at.span.first ? j : j + at.span.jump) * CK + lane * p.box;
+      const int j = at.j0, key = (j < at.span.first ? j : j + at.span.jump) * CK + lane * WIDE_BOX;
       const int index = key / p.block_size;
       Entry e{-1, key - index * p.block_size, at.head,
-              key < at.span.len && (key + p.box > at.span.low || key < p.sinks)};
-      if (lane < boxes && e.seen && index < p.table_width)
+              key < at.span.len && (key + WIDE_BOX > at.span.low || key < p.sinks)};
+      if (lane < BOXES && e.seen && index < p.table_width)
         e.page = __ldg(p.block_tables + at.seq * p.table_stride + index);
       if (--left > 0 && ++at.j0 == at.span.count) at.next_pair(p);
       return e;
@@ -201,13 +203,13 @@ __global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kern
       if (loads >= L::SLOTS && !wait(empty + slot, loads / L::SLOTS - 1, 27)) return false;
       if (lane == 0) mbar_expect_tx(full + slot, TILE_BYTES);
       __syncwarp();
-      if (lane < boxes) {
+      if (lane < BOXES) {
         int row = e.page * p.block_size + e.row;
         if ((uint32_t)e.page >= (uint32_t)p.num_pages) {  // no usable page there: zeros come
           if (e.seen) record_error(VLC_DEV_ERR_BLOCK_RANGE);
           row = p.num_pages * p.block_size;
         }
-        uint8_t* const to = smem + slot * TILE_BYTES + lane * p.box * 128;
+        uint8_t* const to = smem + slot * TILE_BYTES + lane * WIDE_BOX * 128;
         tma_load_4d(to, map, full + slot, 0, e.head, row, 0);
         tma_load_4d(to + HALF_BYTES, map, full + slot, 0, e.head, row, 1);
       }
@@ -485,7 +487,8 @@ __global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kern
       arrive(o_empty + (pair & 1));
       const int rows = min(NC, p.rows - row0);
       if (whole) {
-        __nv_bfloat16* const out = p.out + (int64_t)at.seq * p.tokens * p.out_token_stride + at.head * p.group * HD + key_lane;
+        __nv_bfloat16* const out =
+            p.out + (int64_t)at.seq * p.tokens * p.out_token_stride + (int64_t)at.head * p.group * HD + key_lane;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
           if (c < rows) out[row_at[row0 + c]] = __float2bfloat16(__uint_as_float(o[c]) * fs[c]);
