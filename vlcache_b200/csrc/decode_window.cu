@@ -28,7 +28,7 @@
 // and sums are fp32.
 //
 // Measured (64 sequences of 2700 .. 10700 keys, window 4096, 28 query and 4 KV heads; floor 82 .. 83 us): one token
-// 86.6 us, two 91, three 95 (decode_window_wide.cu: two 93.6, three 95.1); four, which it takes, 94.5 (here, by teams of
+// 86.6 us, two 91, three 95 (decode_window_wide.cu: two 93.6, three 95.1); four, which it takes, 94 (here, by teams of
 // two warps: 96), five 96 (106), eight 101 (142).  One token is bound by HBM (76 % of DRAM's nominal rate); with more
 // the steps' latency counts: 8 warps an SM, whose registers hold the rows.
 #include <algorithm>

@@ -14,16 +14,16 @@
 // P is rounded to bf16 as an operand has to be, and its sums are of the rounded values; scores, maxima, sums and O are
 // fp32.
 //
-// Measured (64 sequences of 2700 .. 10700 keys, window 4096, 28 query and 4 KV heads; floor 83 us): 28 rows 93 us, 35
-// 95, 56 100, 63 101, 91 121, 112 178.  Up to 48 rows HBM bounds it: 4.5 us until the first S, the join and the last
-// chunks 5, between them 0.97 of the floor (a ring of 4 slots instead of 5 costs 0.5).  Copies of 32 keys: of 64, a window's ends
-// waste more (96.7 -> 94.6 on one GPU, 97.9 on another), of 16 the copies count (112).  With more the softmax's time
-// counts (2000 cycles a chunk of 64 rows), then registers: a thread's sums of P.  Tried: the exponentials or the products
-// left out, for a time only: no change, so the chains of waits count and not the pipes; pages' numbers four chunks ahead,
-// unrolled: 98 and 104 for 35 and 56 rows (more code, which the roles' caches feel); P and the slow path in one loop, one
-// copy of each: 99 and 107; one copy of 32 KB a tile instead of four of 8: no change; four shares of the rows: no change
-// for 56, 127 for 91, but 178 instead of 195 for 112.  Rows' output offsets and 1 / sum made once, not by each thread, and
-// maxima and sums over lanes that halve the columns: 112 -> 96.
+// Measured (64 sequences of 2700 .. 10700 keys, window 4096, 28 query and 4 KV heads; floor 83 us): 28 rows 93 .. 95 us by
+// the GPU, 35 95 .. 97, 56 100 .. 102, 63 102, 91 121, 112 178.  Up to 48 rows HBM bounds it: 4.5 us until the first S, the
+// join and the last chunks 5, between them 0.97 of the floor (a ring of 4 slots instead of 5 costs 0.5).  Copies of 32
+// keys: of 64, a window's ends waste more (35 rows 97.9 against 96.6), of 16 the copies count (112); chunks that lie in a
+// page in one copy: no change.  With more rows the softmax's time counts (2000 cycles a chunk of 64 rows), then
+// registers: a thread's sums of P.  Tried: the exponentials or the products left out, for a time only: no change, so
+// the chains of waits count and not the pipes; pages' numbers four chunks ahead, unrolled: 98 and 104 for 35 and 56
+// rows (more code, which the roles' caches feel); P and the slow path in one loop, one copy of each: 99 and 107; four
+// shares of the rows: no change for 56, 127 for 91, but 178 instead of 195 for 112.  Rows' output offsets and 1 / sum made
+// once, not by each thread, and maxima and sums over lanes that halve the columns: 112 -> 96.
 #include <algorithm>
 #include <cmath>
 
