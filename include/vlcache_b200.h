@@ -512,7 +512,12 @@ int vlc_remap_block_tables(int32_t* block_tables, int64_t row_stride, int num_ro
  *   positive value is replaced by the target's row; a row without one gives token -1.  target_probs
  *   [num_seqs][num_drafts + 1][vocab], draft_probs [num_seqs][num_drafts][vocab], strides in
  *   elements, dtype 0 fp32, 1 bf16, 2 fp16; at most 31 drafts and 2^18 tokens.  A draft past the
- *   vocabulary is recorded (VLC_DEV_ERR_TOKEN) and ends the drafts.
+ *   vocabulary is recorded (VLC_DEV_ERR_TOKEN) and ends the drafts.  Every row of the step counts as stored.
+ * vlc_verify_stored_drafts: the same of rows that have a page: row r of a sequence (its last token, then its
+ *   drafts) is at position context_lens[seq] + r, and from the first on whose entry of the step's
+ *   block tables is below 0 or past their width nothing is in the cache.  A draft there is none, and a sequence
+ *   whose first row is there emits nothing: emitted 0, tokens -1, its length stays, and its next step
+ *   begins with the same token.  So the lengths count stored tokens only, whatever the step's free list lacked.
  * ------------------------------------------------------------------------ */
 int vlc_attention_plan_window(const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int num_seqs, int num_heads,
                               int num_kv_heads, int head_dim, int causal, int window, int sinks, int num_sms,
@@ -535,6 +540,12 @@ int vlc_verify_drafts(const int64_t* drafts, int64_t draft_stride, int num_seqs,
                       const void* draft_probs, int64_t draft_seq_stride, int64_t draft_row_stride, int vocab, int dtype,
                       const float* u, int64_t u_stride, const float* u_last, int64_t* tokens, int32_t* emitted,
                       int32_t* context_lens, void* stream);
+int vlc_verify_stored_drafts(const int64_t* drafts, int64_t draft_stride, int num_seqs, int num_drafts,
+                             const void* target_probs, int64_t target_seq_stride, int64_t target_row_stride,
+                             const void* draft_probs, int64_t draft_seq_stride, int64_t draft_row_stride, int vocab,
+                             int dtype, const float* u, int64_t u_stride, const float* u_last, int64_t* tokens,
+                             int32_t* emitted, int32_t* context_lens, const int32_t* block_tables,
+                             int64_t block_table_stride, int block_table_width, int block_size, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,43 @@
+"""Host side of a decode step with drafted tokens, further: refusals and bookkeeping, none of which needs a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+
+# ------------------------------------------------------------------ verification with block tables
+def _verify_args(**kw):
+    a = dict(drafts=torch.zeros(3, 2, dtype=torch.int64), target_probs=torch.zeros(3, 3, 50), draft_probs=None,
+             u=torch.zeros(3, 2), u_last=torch.zeros(3), context_lens=torch.zeros(3, dtype=torch.int32),
+             block_tables=torch.zeros(3, 4, dtype=torch.int32), block_size=32)
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(context_lens=None), "with context_lens"), (dict(block_tables=torch.zeros(2, 4, dtype=torch.int32)), "block_tables"),
+    (dict(block_tables=torch.zeros(3, 4)), "block_tables"),
+    (dict(block_tables=torch.zeros(4, 3, dtype=torch.int32).T), "rows must be contiguous"),
+    (dict(block_size=0), "block_size"), (dict(block_size=1 << 31), "block_size"), ({}, "CUDA tensors only"),
+])
+def test_verify_refuses_tables(cuda_lib, change, what):
+    from vlcache_b200 import ops
+    with pytest.raises(ValueError, match=what):
+        ops.verify_drafts(**_verify_args(**change))
+
+
+def test_verify_takes_a_block_size_with_tables(cuda_lib):
+    from vlcache_b200 import ops
+    with pytest.raises(TypeError):
+        ops.verify_drafts(**_verify_args(block_size=None))
+
+
+def test_c_abi_verify_refuses_tables(cuda_lib):
+    one = ctypes.c_void_p(64)   # never dereferenced: validation fails first
+
+    def verify(seqs=2, lens=one, tables=one, stride=4, width=4, block=32, vocab=100):
+        return cuda_lib.vlc_verify_stored_drafts(one, 2, seqs, 2, one, 300, 100, one, 200, 100, vocab, 0, one, 2, one, one,
+                                                 one, lens, tables, stride, width, block, None)
+    assert verify(block=0) == 2 and verify(width=-1) == 2 and verify(vocab=0) == 2
+    assert verify(lens=None) == 1 and verify(tables=None) == 1 and verify(stride=3) == 3
+    assert verify(seqs=0) == 0 and verify(seqs=0, lens=None, tables=None) == 0

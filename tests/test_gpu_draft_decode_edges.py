@@ -1,0 +1,139 @@
+"""A decode step with drafted tokens on the device, further: what its inputs may hold and which calls may follow one
+another."""
+import math
+
+import pytest
+import torch
+
+from oracle import draft_decode as oracle
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+
+
+def _ops():
+    from vlcache_b200 import ops
+    return ops
+
+
+# ------------------------------------------------------------------ steps that find no page
+def _stored(table, length, rows, block):
+    """Leading rows of a step at positions length .. that the table has pages for."""
+    for r in range(rows):
+        if (length + r) // block >= len(table) or table[(length + r) // block] < 0:
+            return r
+    return rows
+
+
+@pytest.mark.parametrize("blocks", [1, 8])   # of the cluster that takes a sequence
+def test_verify_drafts_of_rows_without_pages(blocks):
+    """A draft in a row without a page is none, a sequence without a page for its first row emits nothing; idle places
+    and sequences whose rows have pages are verified as without tables."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    b, k, vocab, block, width = (600 if blocks == 1 else 12), 3, 517, 4, 5
+    p = torch.softmax(2 * torch.randn(b, k + 1, vocab, generator=g, device="cuda"), -1)
+    q = torch.softmax(2 * torch.randn(b, k, vocab, generator=g, device="cuda"), -1)
+    drafts = torch.randint(0, vocab, (b, k), generator=g, device="cuda")
+    u, u_last = torch.rand(b, k, generator=g, device="cuda") ** 4, torch.rand(b, generator=g, device="cuda")
+    lens = (torch.arange(b, device="cuda") * 7 % 23 - 1).int()   # -1: idle; up to 21, past the table of 20 tokens
+    tables = torch.where(torch.rand(b, width, generator=g, device="cuda") < 0.3, -1, 9).int()
+    wide = torch.full((b, width + 2), 7, dtype=torch.int32, device="cuda")   # pages behind a row's end are not its own
+    wide[:, :width] = tables
+    before = lens.clone()
+    tokens, emitted = ops.verify_drafts(drafts, p, q, u, u_last, lens, wide[:, :width], block)
+    seen = set()
+    for i in range(b):
+        n = int(before[i])
+        rows = k + 1 if n < 0 else _stored(tables[i].tolist(), n, k + 1, block)
+        seen.add(rows)
+        ds = [d if r + 1 < rows else -1 for r, d in enumerate(drafts[i].tolist())]
+        want = [] if rows == 0 else oracle.verify(ds, p[i].cpu(), q[i].cpu(), u[i].tolist(), float(u_last[i]))
+        assert tokens[i].tolist() == want + [-1] * (k + 1 - len(want)) and int(emitted[i]) == len(want), i
+        assert int(lens[i]) == (n if n < 0 else n + len(want))
+    assert seen >= {0, 4} and ops.device_error() == 0
+    # slots past 32 bits are none
+    far = torch.full((1, 1), 1 << 29, dtype=torch.int32, device="cuda")
+    got = ops.verify_drafts(drafts[:1], p[:1], q[:1], u[:1], u_last[:1], torch.zeros(1, dtype=torch.int32, device="cuda"),
+                            far, block)
+    assert int(got[1]) == 0
+    # no table at all
+    none = ops.verify_drafts(drafts[:2], p[:2], q[:2], u[:2], u_last[:2], before[1:3].clone(), tables[:2, :0], block)
+    assert none[1].tolist() == [0, 0] and none[0].tolist() == [[-1] * (k + 1)] * 2
+
+
+@pytest.mark.parametrize("all_windowed", [True, False])
+def test_draft_decode_without_pages(all_windowed):
+    """Steps while the lent pages run out, and at a table's end: rows without a page are not verified, no length
+    counts a token that is not in the cache, and sequences go on when pages are lent, from the same token."""
+    from test_gpu_draft_decode import _Model
+
+    from vlcache_b200.engine.draft_decode import DraftDecode
+    from vlcache_b200.engine.page_pool import PagePool
+    from vlcache_b200.utils.context import reset_context, set_context
+    import numpy as np
+    ops = _ops()
+    block, places, k, most = 32, 3, 3, 4
+    model = _Model(11, all_windowed=all_windowed)
+    pool = PagePool(60, block)
+    model.caches(60, block)
+    for layer in model.layers:   # what a recycled page holds
+        layer.k_cache.fill_(3.0)
+        layer.v_cache.fill_(30.0)
+    window = 40 if all_windowed else 0
+    d = DraftDecode(pool, places, most, k, window, 3 if window else 0)
+    r = np.random.default_rng(9)
+    histories = {0: [int(x) for x in r.integers(0, 97, 61)], 1: [int(x) for x in r.integers(0, 97, 95)],
+                 2: [int(x) for x in r.integers(0, 97, 30)]}
+    last = {}
+    for place, tokens in histories.items():
+        table, n = pool.allocate(pool.pages_for(len(tokens))), len(tokens)
+        slots = torch.tensor([table[t // block] * block + t % block for t in range(n)], dtype=torch.int32, device="cuda")
+        cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        set_context(True, cu, cu, n, n, slots, None, None, cu_seqlens_q_host=[0, n], cu_seqlens_k_host=[0, n])
+        last[place] = int(model(torch.tensor(tokens, device="cuda"), torch.arange(n, device="cuda"))[-1].argmax())
+        d.admit(place, table, n)
+    seen, errors = set(), set()
+    for turn in range(250):
+        if all(len(h) == most * block for h in histories.values()) and 0 in seen:
+            break
+        if turn in (6, 9, 30):
+            assert d.lend(1)
+        if turn == 40:
+            assert d.lend(20)
+        guess = torch.full((places, k + 1), -1, dtype=torch.int64)
+        for p in histories:
+            row = [last[p]]
+            for _ in range(k):   # the right drafts, mostly
+                best = int(model.plain(histories[p] + row)[-1].argmax())
+                row.append(best if r.random() < 0.7 else int(r.integers(0, 97)))
+            guess[p] = torch.tensor(row)
+        tokens_in = guess.cuda()
+        u = torch.tensor(r.random((places, k)) * 0.2, dtype=torch.float32, device="cuda")
+        u_last = torch.tensor(r.random(places), dtype=torch.float32, device="cuda")
+        positions = d.begin()
+        tables = d.block_tables.tolist()
+        probs = model(tokens_in.flatten(), positions).view(places, k + 1, -1)
+        tokens, emitted = d.finish(tokens_in[:, 1:].contiguous(), probs, None, u, u_last)
+        errors.add(ops.device_error())
+        for p, h in histories.items():
+            rows = _stored(tables[p], len(h), k + 1, block)
+            seen.add(rows)
+            want = model.plain(h + guess[p].tolist())[len(h):]
+            # (an output's error as in the test of steps with pages: below 0.05)
+            assert float((probs[p].double() - want)[:rows].abs().max() if rows else 0.0) < 0.05, (turn, p, rows)
+            ds = [x if i + 1 < rows else -1 for i, x in enumerate(guess[p, 1:].tolist())]
+            out = [] if rows == 0 else oracle.verify(ds, probs[p].cpu(), None, u[p].tolist(), float(u_last[p]))
+            assert tokens[p].tolist() == out + [-1] * (k + 1 - len(out)) and int(emitted[p]) == len(out), (turn, p)
+            if out:
+                h += guess[p, :len(out)].tolist()
+                last[p] = out[-1]
+            assert int(d.context_lens[p]) == len(h) <= most * block
+    assert 0 in seen and k + 1 in seen and len(seen) > 2 and errors - {0} <= {102, 105} and len(errors) > 1
+    assert all(len(h) == most * block for h in histories.values())   # and every table ended full
+    for p in histories:
+        d.retire(p)
+    d.settle()
+    assert pool.num_free == 60 and pool.refs == [0] * 60
+    reset_context()

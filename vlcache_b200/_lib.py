@@ -89,6 +89,8 @@ SIGNATURES: dict[str, tuple] = {
                                   c_vp, c_int, c_vp, c_vp, c_vp, c_vp]),
     "vlc_verify_drafts": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_int,
                                   c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "vlc_verify_stored_drafts": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_int,
+                                         c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_int, c_vp]),
 }
 
 

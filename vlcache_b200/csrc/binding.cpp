@@ -246,7 +246,7 @@ PyObject* verify_drafts(PyObject* const* a) {
   const Tensor &drafts = tensor(a[0], "drafts"), &target = tensor(a[1], "target_probs");
   const Tensor draft = optional(a[2], "draft_probs");
   const Tensor &u = tensor(a[3], "u"), &u_last = tensor(a[4], "u_last");
-  const Tensor lens = optional(a[5], "context_lens");
+  const Tensor lens = optional(a[5], "context_lens"), tables = optional(a[6], "block_tables");
   need(drafts.scalar_type() == at::kLong && drafts.dim() == 2, "drafts: int64 [sequences, drafts]");
   const int64_t b = drafts.size(0), n = drafts.size(1);
   need(b <= 65535 && n <= 31, "at most 65535 sequences and 31 drafts");
@@ -262,15 +262,30 @@ PyObject* verify_drafts(PyObject* const* a) {
   need(u_last.scalar_type() == at::kFloat && u_last.dim() == 1 && u_last.size(0) == b && u_last.is_contiguous(), "u_last",
        "contiguous fp32 [" + std::to_string(b) + "]");
   const int32_t* const context_lens = lens.defined() ? ints_of(lens, b, "context_lens") : nullptr;
-  const On on(device_of(drafts, {&target, &draft, &u, &u_last, &lens}));
+  Tables t{};
+  int block = 0;
+  if (tables.defined()) {
+    need(lens.defined(), "block_tables: with context_lens");
+    t = tables_of(tables, b);
+    block = bounded(a[7], "block_size", 1, 0x7fffffff);
+  }
+  const On on(device_of(drafts, {&target, &draft, &u, &u_last, &lens, &tables}));
   const Tensor buffer = at::empty({b * ((n + 1) * 8 + 4)}, like(drafts, at::kByte));
   const Tensor tokens = part(buffer, 0, at::kLong, {b, n + 1}), emitted = part(buffer, b * (n + 1) * 8, at::kInt, {b});
-  check("vlc_verify_drafts",
-        vlc_verify_drafts((const int64_t*)drafts.data_ptr(), drafts.stride(0), (int)b, (int)n, target.data_ptr(), p.seq,
-                          p.row, draft.defined() ? draft.data_ptr() : nullptr, q.seq, q.row, p.vocab, p.type,
-                          (const float*)u.data_ptr(), u.stride(0), (const float*)u_last.data_ptr(),
-                          (int64_t*)tokens.data_ptr(), (int32_t*)emitted.data_ptr(),
-                          const_cast<int32_t*>(context_lens), on.stream));
+  if (tables.defined())
+    check("vlc_verify_stored_drafts",
+          vlc_verify_stored_drafts((const int64_t*)drafts.data_ptr(), drafts.stride(0), (int)b, (int)n, target.data_ptr(),
+                                   p.seq, p.row, draft.defined() ? draft.data_ptr() : nullptr, q.seq, q.row, p.vocab,
+                                   p.type, (const float*)u.data_ptr(), u.stride(0), (const float*)u_last.data_ptr(),
+                                   (int64_t*)tokens.data_ptr(), (int32_t*)emitted.data_ptr(),
+                                   const_cast<int32_t*>(context_lens), t.data, t.stride, t.width, block, on.stream));
+  else
+    check("vlc_verify_drafts",
+          vlc_verify_drafts((const int64_t*)drafts.data_ptr(), drafts.stride(0), (int)b, (int)n, target.data_ptr(), p.seq,
+                            p.row, draft.defined() ? draft.data_ptr() : nullptr, q.seq, q.row, p.vocab, p.type,
+                            (const float*)u.data_ptr(), u.stride(0), (const float*)u_last.data_ptr(),
+                            (int64_t*)tokens.data_ptr(), (int32_t*)emitted.data_ptr(),
+                            const_cast<int32_t*>(context_lens), on.stream));
   return tuple_of({tokens, emitted});
 }
 
@@ -323,7 +338,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef kMethods[] = {
     {"decode_attention_window", (PyCFunction)(void (*)(void))call<decode_attention_window, 11>, METH_FASTCALL, nullptr},
     {"step_metadata", (PyCFunction)(void (*)(void))call<step_metadata, 9>, METH_FASTCALL, nullptr},
-    {"verify_drafts", (PyCFunction)(void (*)(void))call<verify_drafts, 6>, METH_FASTCALL, nullptr},
+    {"verify_drafts", (PyCFunction)(void (*)(void))call<verify_drafts, 8>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

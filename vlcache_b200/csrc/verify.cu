@@ -19,6 +19,7 @@
 // whole numbers instead of the additions in 64-bit floating point 16.9 and 39; four blocks an SM (spilling) 18.0
 // and 25.4.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "common.cuh"
@@ -49,6 +50,9 @@ struct Params {
   int64_t* tokens;   // [num_seqs][num_drafts + 1]
   int32_t* emitted;
   int32_t* context_lens;  // null, or moved on by emitted (idle places, below 0, stay)
+  const int32_t* block_tables;  // of the step's rows, with block_size; block_size 0: every row is in the cache
+  int64_t table_stride;
+  int table_width, block_size;
   int num_drafts, vocab;
   int tiles;         // of a warp
 };
@@ -223,8 +227,19 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) verify_kernel(const Pa
   // ---- acceptance, in every block
   if (warp == 0) {
     bool live = false, taken = false;
+    // Row r of the step (its last token, then the drafts) is in the cache iff the table has a page for it; what is
+    // behind the first that is not, was computed without its key.
+    int stored = 32;
+    const int len = a.block_size > 0 ? a.context_lens[seq] : -1;
+    if (len >= 0) {  // (idle places have no rows)
+      const uint32_t t = (uint32_t)len + lane, page = t / (uint32_t)a.block_size;
+      const int number = page < (uint32_t)a.table_width ? __ldg(a.block_tables + seq * a.table_stride + page) : -1;
+      const bool there = number >= 0 && (int64_t)number * a.block_size + t % (uint32_t)a.block_size <= INT_MAX;
+      const uint32_t none = ~__ballot_sync(0xffffffffu, there);
+      stored = none ? __ffs(none) - 1 : 32;
+    }
     if (lane < a.num_drafts) {
-      const int64_t d = drafts[lane];
+      const int64_t d = lane + 1 < stored ? drafts[lane] : -1;
       live = d >= 0 && d < a.vocab;
       if (d >= a.vocab && rank == 0) record_error(VLC_DEV_ERR_TOKEN);
       const int64_t v = live ? d : 0;
@@ -235,12 +250,18 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) verify_kernel(const Pa
     const uint32_t yes = __ballot_sync(0xffffffffu, taken), have = __ballot_sync(0xffffffffu, live);
     const int n = __ffs(~yes) == 0 ? 32 : __ffs(~yes) - 1;
     if (lane == 0) {
-      s_taken = n;
+      s_taken = stored > 0 ? n : -1;
       s_refused = n < a.num_drafts && (have >> n & 1);
     }
   }
   __syncthreads();
   const int taken = s_taken;
+  if (taken < 0) {  // the sequence's own token is not in the cache: it waits for a page
+    if (rank == 0 && threadIdx.x <= a.num_drafts) a.tokens[(int64_t)seq * (a.num_drafts + 1) + threadIdx.x] = -1;
+    if (rank == 0 && threadIdx.x == 0) a.emitted[seq] = 0;
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    return;
+  }
   const bool refused = s_refused != 0;
   Row<T> row;
   row.p = p0 + taken * a.p_row;
@@ -371,11 +392,13 @@ static int launch(const Params& a, int num_seqs, int blocks, cudaStream_t st) {
 using namespace vlc;
 using namespace vlc::verify;
 
-extern "C" int vlc_verify_drafts(const int64_t* drafts, int64_t draft_stride, int num_seqs, int num_drafts,
-                                 const void* target_probs, int64_t target_seq_stride, int64_t target_row_stride,
-                                 const void* draft_probs, int64_t draft_seq_stride, int64_t draft_row_stride, int vocab,
-                                 int dtype, const float* u, int64_t u_stride, const float* u_last, int64_t* tokens,
-                                 int32_t* emitted, int32_t* context_lens, void* stream) {
+// block_size 0: without block tables.
+static int verify_drafts(const int64_t* drafts, int64_t draft_stride, int num_seqs, int num_drafts,
+                         const void* target_probs, int64_t target_seq_stride, int64_t target_row_stride,
+                         const void* draft_probs, int64_t draft_seq_stride, int64_t draft_row_stride, int vocab, int dtype,
+                         const float* u, int64_t u_stride, const float* u_last, int64_t* tokens, int32_t* emitted,
+                         int32_t* context_lens, const int32_t* block_tables, int64_t block_table_stride,
+                         int block_table_width, int block_size, void* stream) {
   if (num_seqs < 0 || num_seqs > 65535 || num_drafts < 0 || vocab <= 0) return VLC_ERR_SHAPE;
   if (num_drafts > MAX_DRAFTS - 1 || vocab > MAX_VOCAB || dtype < 0 || dtype > 2) return VLC_ERR_UNSUPPORTED;
   if (num_seqs == 0) return VLC_OK;
@@ -396,6 +419,10 @@ extern "C" int vlc_verify_drafts(const int64_t* drafts, int64_t draft_stride, in
   a.tokens = tokens;
   a.emitted = emitted;
   a.context_lens = context_lens;
+  a.block_tables = block_tables;
+  a.table_stride = block_table_stride;
+  a.table_width = block_table_width;
+  a.block_size = block_size;
   a.num_drafts = num_drafts;
   a.vocab = vocab;
   const int tile = dtype == 0 ? kTile<float> : kTile<__half>;
@@ -408,4 +435,29 @@ extern "C" int vlc_verify_drafts(const int64_t* drafts, int64_t draft_stride, in
   return dtype == 0 ? launch<float>(a, num_seqs, blocks, st)
          : dtype == 1 ? launch<__nv_bfloat16>(a, num_seqs, blocks, st)
                       : launch<__half>(a, num_seqs, blocks, st);
+}
+
+extern "C" int vlc_verify_drafts(const int64_t* drafts, int64_t draft_stride, int num_seqs, int num_drafts,
+                                 const void* target_probs, int64_t target_seq_stride, int64_t target_row_stride,
+                                 const void* draft_probs, int64_t draft_seq_stride, int64_t draft_row_stride, int vocab,
+                                 int dtype, const float* u, int64_t u_stride, const float* u_last, int64_t* tokens,
+                                 int32_t* emitted, int32_t* context_lens, void* stream) {
+  return verify_drafts(drafts, draft_stride, num_seqs, num_drafts, target_probs, target_seq_stride, target_row_stride,
+                       draft_probs, draft_seq_stride, draft_row_stride, vocab, dtype, u, u_stride, u_last, tokens, emitted,
+                       context_lens, nullptr, 0, 0, 0, stream);
+}
+
+extern "C" int vlc_verify_stored_drafts(const int64_t* drafts, int64_t draft_stride, int num_seqs, int num_drafts,
+                                        const void* target_probs, int64_t target_seq_stride, int64_t target_row_stride,
+                                        const void* draft_probs, int64_t draft_seq_stride, int64_t draft_row_stride,
+                                        int vocab, int dtype, const float* u, int64_t u_stride, const float* u_last,
+                                        int64_t* tokens, int32_t* emitted, int32_t* context_lens,
+                                        const int32_t* block_tables, int64_t block_table_stride, int block_table_width,
+                                        int block_size, void* stream) {
+  if (block_table_width < 0 || block_size <= 0) return VLC_ERR_SHAPE;
+  if (num_seqs > 0 && (!context_lens || (block_table_width > 0 && !block_tables))) return VLC_ERR_NULL;
+  if (num_seqs > 1 && block_table_stride < block_table_width) return VLC_ERR_STRIDE;
+  return verify_drafts(drafts, draft_stride, num_seqs, num_drafts, target_probs, target_seq_stride, target_row_stride,
+                       draft_probs, draft_seq_stride, draft_row_stride, vocab, dtype, u, u_stride, u_last, tokens, emitted,
+                       context_lens, block_tables, block_table_stride, block_table_width, block_size, stream);
 }

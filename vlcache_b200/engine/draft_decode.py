@@ -106,15 +106,21 @@ class DraftDecode:
         positions, slots, _, _, lens = ops.step_metadata(self.context_lens, self.new_lens, self.block_tables,
                                                          self.free_pages, self.num_free, self.pool.block_size, rows,
                                                          self.window, self.sinks)
+        # (Rows past a table's end are in the lengths too: a bound without them would cut the lengths, and so move
+        # the rows before them.)
         set_context(False, slot_mapping=slots, context_lens=lens, block_tables=self.block_tables,
-                    max_context_len=self.max_pages * self.pool.block_size)
+                    max_context_len=self.max_pages * self.pool.block_size + self.num_tokens)
         return positions
 
     def finish(self, drafts: torch.Tensor, target_probs: torch.Tensor, draft_probs: torch.Tensor | None,
                u: torch.Tensor, u_last: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """Verify the step's drafts (``ops.verify_drafts``; int64 [places, num_drafts], -1 where a place
         has fewer) and keep what was accepted: the lengths move on by emitted.  Returns (tokens, emitted);
-        of a place's tokens the last is its next step's first row."""
+        of a place's tokens the last is its next step's first row.  A place that found no page for some of its rows
+        (the free list ran out, or its table ended: ``ops.device_error``) has no drafts from there on; one that found
+        none for its first row emits nothing (emitted 0, tokens -1) and begins its next step with the same
+        token, when pages were lent."""
         if drafts.shape != (self.places, self.num_tokens - 1):
             raise ValueError(f"drafts: [{self.places}, {self.num_tokens - 1}]")
-        return ops.verify_drafts(drafts, target_probs, draft_probs, u, u_last, self.context_lens)
+        return ops.verify_drafts(drafts, target_probs, draft_probs, u, u_last, self.context_lens, self.block_tables,
+                                 self.pool.block_size)

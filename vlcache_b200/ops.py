@@ -1021,8 +1021,9 @@ def step_metadata(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
 
 
 def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, draft_probs: torch.Tensor | None,
-                  u: torch.Tensor, u_last: torch.Tensor,
-                  context_lens: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                  u: torch.Tensor, u_last: torch.Tensor, context_lens: torch.Tensor | None = None,
+                  block_tables: torch.Tensor | None = None,
+                  block_size: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Speculative sampling's verification, from given random numbers: draft i of each sequence
     (``drafts`` int64 [B, K], -1 from a sequence's end on) is accepted iff ``u[b, i] * draft_probs[b, i,
     d] < target_probs[b, i, d]``, up to the first refusal; then one token is sampled at ``u_last[b]``, from
@@ -1033,7 +1034,11 @@ def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, draft_probs:
     and refused it counts 0.  ``u`` [B, K] and ``u_last`` [B] are fp32 in [0, 1).  Returns (tokens int64
     [B, K + 1]: the accepted drafts, the sampled token, then -1; emitted int32 [B]: accepted + 1).
     ``context_lens`` (int32 [B], when given) is moved on by emitted in place: the step's first token and
-    the accepted drafts are in the cache then (idle places, below 0, stay).
+    the accepted drafts are in the cache then (idle places, below 0, stay).  With the step's
+    ``block_tables`` [B, width] and ``block_size`` (and ``context_lens``) that is so also where the free list ran out or
+    a table ended: from the first row without a page on there are no drafts, and a sequence whose first row has
+    none emits nothing (emitted 0, tokens -1, its length stays); its next step begins with the same token.
     Sums are whole numbers (include/vlcache_b200.h), so the answer is the same in every run and
     whatever the order of summation.  At most 31 drafts and 2^18 tokens of vocabulary."""
-    return (_compiled or _binding()).verify_drafts(drafts, target_probs, draft_probs, u, u_last, context_lens)
+    return (_compiled or _binding()).verify_drafts(drafts, target_probs, draft_probs, u, u_last, context_lens, block_tables,
+                                                   block_size)
