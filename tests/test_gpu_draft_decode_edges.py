@@ -17,6 +17,33 @@ def _ops():
     return ops
 
 
+# ------------------------------------------------------------------ verification
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("vocab", [5, 64, 1000, 40003])
+@pytest.mark.parametrize("sampled", [True, False])
+def test_verify_drafts_counts_negative_zeros_as_none(dtype, vocab, sampled):
+    """Probabilities of -0.0 (and -0.0 - 0.0 at a refused draft) count 0, in whole vectors and at a row's ends."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    b, k = 12, 2
+    p = torch.softmax(2 * torch.randn(b, k + 1, vocab, generator=g, device="cuda"), -1).to(dtype)
+    q = torch.softmax(2 * torch.randn(b, k, vocab, generator=g, device="cuda"), -1).to(dtype)
+    zero = torch.rand(p.shape, generator=g, device="cuda") < 0.5
+    zero[..., 0] = zero[..., -1] = True
+    zero[..., vocab // 2] = False
+    p = torch.where(zero, torch.full_like(p, -0.0), p)
+    q = torch.where(zero[:, :k] & (torch.rand(q.shape, generator=g, device="cuda") < 0.7), torch.zeros_like(q), q)
+    assert bool(torch.signbit(p[..., 0]).all())
+    drafts = torch.randint(0, vocab, (b, k), generator=g, device="cuda")
+    u, u_last = torch.rand(b, k, generator=g, device="cuda"), torch.rand(b, generator=g, device="cuda")
+    tokens, emitted = ops.verify_drafts(drafts, p, q if sampled else None, u, u_last)
+    assert ops.device_error() == 0
+    for i in range(b):
+        want = oracle.verify(drafts[i].tolist(), p[i].cpu(), q[i].cpu() if sampled else None, u[i].tolist(),
+                             float(u_last[i]))
+        assert tokens[i].tolist() == want + [-1] * (k + 1 - len(want)) and int(emitted[i]) == len(want)
+
+
 # ------------------------------------------------------------------ steps that find no page
 def _stored(table, length, rows, block):
     """Leading rows of a step at positions length .. that the table has pages for."""

@@ -67,7 +67,7 @@ struct Counter {
   double at = 1024.0;
   template <bool SHORT>  // x is a 16-bit number
   __device__ __forceinline__ void add(float x) {
-    const uint32_t b = __float_as_uint(__saturatef(x));  // (NaN counts as 0)
+    const uint32_t b = __float_as_uint(__saturatef(x));  // (NaN counts as 0, -0.0 saturates to 0.0: tested)
     // the same number in 64 bits, but 2^-127 for 0 and less than 2^-126 for smaller ones
     at = __dadd_rd(at, __hiloint2double((int)((b >> 3) + 0x38000000u), SHORT ? 0 : (int)(b << 29)));
   }
