@@ -41,3 +41,31 @@ def test_c_abi_verify_refuses_tables(cuda_lib):
     assert verify(block=0) == 2 and verify(width=-1) == 2 and verify(vocab=0) == 2
     assert verify(lens=None) == 1 and verify(tables=None) == 1 and verify(stride=3) == 3
     assert verify(seqs=0) == 0 and verify(seqs=0, lens=None, tables=None) == 0
+
+
+# ------------------------------------------------------------------ waits that give up
+def _source(name):
+    from pathlib import Path
+
+    import vlcache_b200
+    return (Path(vlcache_b200.__file__).parent / "csrc" / name).read_text()
+
+
+def test_wide_decode_warps_give_up_together():
+    """A wait that gives up ends a role for all lanes of a warp or for none: lanes that left alone would be waited for by
+    the others at their next vote, for ever.  Only the products' role, which is one lane, leaves by itself; the softmax
+    warps, whose barriers need all of them, never leave."""
+    import re
+    src = _source("decode_window_wide.cu")
+    kernel = src[src.index("window_decode_wide_kernel(const"):src.index("static int launch(")]
+    roles = re.split(r"  // -{20,} (?=K and V copies|products|Q:|softmax)", kernel)
+    assert len(roles) == 5
+    copies, products, queries, softmax = roles[1:]
+    leaves = r"!wait\(|= wait\(|return wait\("   # something depends on a lane's own result
+    for role in (copies, queries):
+        assert "!warp_wait(" in role and not re.search(leaves, role)
+    assert "if (lane == 0 && count > 0)" in products and "!wait(" in products
+    assert not re.search(leaves, softmax) and "break;" not in softmax and "return;" not in softmax
+    common = _source("common.cuh")
+    helper = common[common.index("bool warp_wait_or_abort("):]
+    assert "__all_sync(0xffffffffu, wait_or_abort(" in helper[:helper.index("}")]

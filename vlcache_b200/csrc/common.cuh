@@ -104,6 +104,13 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, in
   }
 }
 
+// The same by a whole warp that goes on to something its lanes do together (a vote, a warp or block barrier, a
+// tcgen05 load): all of its lanes see the wait succeed, or none, whichever of them gave up.
+__device__ __forceinline__ bool warp_wait_or_abort(uint64_t* bar, uint32_t parity, int code,
+                                                   volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, wait_or_abort(bar, parity, code, abort_flag));
+}
+
 // ---------------------------------------------------------------- proxies / fences
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

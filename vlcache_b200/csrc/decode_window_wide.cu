@@ -176,6 +176,10 @@ __global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kern
   auto wait = [&](uint64_t* bar, int phase, int role) {
     return wait_or_abort(bar, (uint32_t)phase & 1u, VLC_DEV_ERR_TIMEOUT + role, abort_flag);
   };
+  // By a warp that leaves its role where it gave up: its lanes leave together or not at all.
+  auto warp_wait = [&](uint64_t* bar, int phase, int role) {
+    return warp_wait_or_abort(bar, (uint32_t)phase & 1u, VLC_DEV_ERR_TIMEOUT + role, abort_flag);
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ K and V copies: a lane each box of keys
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kern
     int loads = 0;
     auto issue = [&](const CUtensorMap* map, const Entry& e) {
       const int slot = loads % L::SLOTS;
-      if (loads >= L::SLOTS && !wait(empty + slot, loads / L::SLOTS - 1, 27)) return false;
+      if (loads >= L::SLOTS && !warp_wait(empty + slot, loads / L::SLOTS - 1, 27)) return false;
       if (lane == 0) mbar_expect_tx(full + slot, TILE_BYTES);
       __syncwarp();
       if (lane < BOXES) {
@@ -236,7 +240,7 @@ __global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kern
                           VLC_WAIT_LIMIT_CYCLES);
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ products
+    // ------------------------------------------------------------ products, by one lane
     if (lane == 0 && count > 0) {
       const uint32_t ring = umma_desc_sw128_lo(smem_u32(smem), 16);
       const uint32_t ring_v = umma_desc_sw128_lo(smem_u32(smem), HALF_BYTES);
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kern
     Run<CK> at = run;
     for (int done = 0, pair = 0; done < count; ++pair) {
       const int b = pair % L::Q_BUFFERS;
-      if (pair >= L::Q_BUFFERS && !wait(q_empty + b, pair / L::Q_BUFFERS - 1, 35)) break;
+      if (pair >= L::Q_BUFFERS && !warp_wait(q_empty + b, pair / L::Q_BUFFERS - 1, 35)) break;
       uint8_t* const to = smem + L::Q + b * L::Q_BYTES + (piece >> 3) * (N * 128);
       constexpr int LOADS = N <= 64 ? N / 4 : 8;  // at once
 #pragma unroll
