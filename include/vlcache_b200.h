@@ -182,8 +182,8 @@ int64_t vlc_prefill_workspace_size(const int32_t* plan_host);
  * The plan's causal flag selects the mask (vlc_attention_plan).
  * Launch order: the attention is a programmatic dependent launch of the kernel
  * enqueued just before it on `stream` (its setup overlaps that kernel's tail).
- * That kernel may write q, k and v; plan_dev and block_tables must have been
- * written by a copy or by an earlier kernel.
+ * That kernel may write q, k, v and block_tables (vlc_step_metadata makes them on the
+ * device); plan_dev must have been written by a copy or by an earlier kernel.
  * ------------------------------------------------------------------------ */
 int vlc_prefill_attn(const void* q, int64_t q_token_stride, int total_q, int num_heads,
                      const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,

@@ -164,3 +164,36 @@ def test_draft_decode_without_pages(all_windowed):
     d.settle()
     assert pool.num_free == 60 and pool.refs == [0] * 60
     reset_context()
+
+
+# ------------------------------------------------------------------ one call behind another
+@pytest.mark.parametrize("rows,window", [(700, 0), (700, 100), (20000, 0), (20000, 1000)])   # one launch of metadata, and two
+def test_prefill_reads_tables_of_the_step_before(rows, window):
+    """Block tables that vlc_step_metadata has just written, by the prefill launched directly behind it, which starts
+    before that kernel has ended."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    seqs, block = 4, 256
+    each = rows // seqs
+    held = (each + block - 1) // block
+    pages = 2 * seqs * held
+    k_cache, v_cache = (torch.randn(pages, block, 2, D, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(seqs * each, 16, D, generator=g, device="cuda").to(torch.bfloat16)
+    cu = [i * each for i in range(seqs + 1)]
+    plan = ops.build_prefill_plan(cu, cu, 16, 2, device="cuda", window=window or None)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    lens, new = torch.zeros(seqs, **i32), torch.full((seqs,), each, **i32)
+    tables = torch.full((seqs, held), -1, **i32)
+    out = torch.empty_like(q)
+    workspace = torch.empty(max(1, plan.workspace_bytes), dtype=torch.uint8, device="cuda")
+    for turn in range(6):
+        free = torch.randperm(pages, generator=g, device="cuda").int()
+        count = torch.tensor([pages], **i32)
+        tables.fill_(-1)   # a stale entry would be an error, or another turn's page
+        torch.cuda.synchronize()
+        ops.step_metadata(lens, new, tables, free, count, block, seqs * each)
+        ops.prefill_attention(q, k_cache, v_cache, tables, plan, 0.1, out=out, workspace=workspace)
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert ops.device_error() == 0 and int((tables < 0).sum()) == 0
+        assert torch.equal(got, ops.prefill_attention(q, k_cache, v_cache, tables, plan, 0.1)), turn

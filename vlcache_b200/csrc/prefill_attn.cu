@@ -173,7 +173,8 @@ __device__ __forceinline__ int key_block_slot(const Params& p, const int32_t* u,
   if (unit_inflight(p, u)) {
     slot = (int64_t)u[kUSelfRow] + key0;  // box may run past the end: zero fill, masked
   } else if (p.block_tables != nullptr) {
-    const int page = __ldg(p.block_tables + (int64_t)u[kUSeq] * p.bt_stride + key0 / p.block_size);
+    // (an ordinary load, behind pdl_wait: the kernel launched just before may have written the tables)
+    const int page = p.block_tables[(int64_t)u[kUSeq] * p.bt_stride + key0 / p.block_size];
     slot = (int64_t)page * p.block_size + (key0 % p.block_size);
     if (page < 0 || slot + BN > p.num_slots) {
       record_error(VLC_DEV_ERR_BLOCK_RANGE);
@@ -183,6 +184,13 @@ __device__ __forceinline__ int key_block_slot(const Params& p, const int32_t* u,
     slot = (int64_t)u[kUKBase] + key0;  // box may run past the end: zero fill, masked
   }
   return (int)slot;
+}
+
+// Asks L2 for the table entry of a unit's key block, so that it is near when pdl_wait is over.
+__device__ __forceinline__ void prefetch_page(const Params& p, const int32_t* u, int kb) {
+  if (p.block_tables == nullptr || unit_inflight(p, u)) return;
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p.block_tables + (int64_t)u[kUSeq] * p.bt_stride +
+                                                kb * BN / p.block_size));
 }
 
 // The key block behind a unit's block number `kb`: its own, but for windowed plans.
@@ -344,9 +352,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
   } else if (warp == 8) {
     // ------------------------------------------------------------ K/V producer
     if (lane == 0) {
-      // Plan and block tables are never written by the kernel launched just before:
-      // the first unit's fields and its first page are read while the wait runs.
-      int g = 0, kb0 = 0, kb1 = 0, slot0 = 0;
+      // The plan is never written by the kernel launched just before: the first unit's
+      // fields are read while the wait runs.  Block tables may be (step metadata is made on
+      // the device): their entries are read behind it.
+      int g = 0, kb0 = 0, kb1 = 0;
       bool infl = false;
       const int32_t* u = nullptr;
       WindowBlocks wb{0, 0};
@@ -357,9 +366,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
         kb1 = u[kUKbEnd];
         infl = unit_inflight(p, u);
         if (kWindow) wb = window_blocks(u[kUKpos0B], p.window, p.sinks);
-        slot0 = kb0 < kb1 ? key_block_slot(p, u, key_block<kWindow>(wb, kb0)) : 0;
       };
-      if (u_begin < u_end) fetch(u_begin);
+      if (u_begin < u_end) {
+        fetch(u_begin);
+        if (kb0 < kb1) prefetch_page(p, u, key_block<kWindow>(wb, kb0));
+      }
       bool waited = false;  // K/V rows (paged or contiguous) may be written by the preceding kernel
       int it = 0;
       for (int ui = u_begin; ui < u_end; ++ui) {
@@ -376,9 +387,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
         for (int kb = kb0; kb < kb_end; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (uint32_t)(it / STAGES) & 1u;
-          const int slot = kb == kb0 ? slot0
-                           : kPacked ? u[kUQBeginB]
-                                     : key_block_slot(p, u, key_block<kWindow>(wb, kb));
+          const int slot = kPacked && kb > kb0 ? u[kUQBeginB] : key_block_slot(p, u, key_block<kWindow>(wb, kb));
           if (it >= STAGES && !wait_or_abort(bars.k_empty + s, ph ^ 1u, VLC_DEV_ERR_TIMEOUT + 2, abort_flag)) {
             ok = false;
             break;
@@ -1059,9 +1068,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
   } else if (warp == 8) {
     // ------------------------------------------------------------ K/V producer
     if (lane == 0) {
-      // Plan and block tables are never written by the kernel launched just before:
-      // the first unit's fields and its first page are read while the wait runs.
-      int g = 0, kb0 = 0, kb1 = 0, slot0 = 0;
+      // The plan is never written by the kernel launched just before: the first unit's
+      // fields are read while the wait runs.  Block tables may be (step metadata is made on
+      // the device): their entries are read behind it.
+      int g = 0, kb0 = 0, kb1 = 0;
       bool infl = false;
       const int32_t* u = nullptr;
       auto fetch = [&](int ui) {
@@ -1070,9 +1080,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
         kb0 = u[kUKbBegin];
         kb1 = u[kUKbEnd];
         infl = unit_inflight(p, u);
-        slot0 = kb0 < kb1 ? key_block_slot(p, u, kb0) : 0;
       };
-      if (u_begin < u_end) fetch(u_begin);
+      if (u_begin < u_end) {
+        fetch(u_begin);
+        if (kb0 < kb1) prefetch_page(p, u, kb0);
+      }
       bool waited = false;  // K/V rows (paged or contiguous) may be written by the preceding kernel
       int it = 0;
       for (int ui = u_begin; ui < u_end; ++ui) {
@@ -1087,7 +1099,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (uint32_t)(it / STAGES) & 1u;
-          const int slot = kb == kb0 ? slot0 : key_block_slot(p, u, kb);
+          const int slot = key_block_slot(p, u, kb);
           if (it >= STAGES && !wait_or_abort(bars.k_empty + s, ph ^ 1u, VLC_DEV_ERR_TIMEOUT + 2, abort_flag)) {
             ok = false;
             break;

@@ -281,7 +281,7 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_t
     ``block_tables`` maps sequences to pages.  Contiguous (``block_tables`` None): ``k``/``v``
     are ``[total_k, Hk, D]`` (any token stride) laid out by cu_seqlens_k.
     The kernel is a programmatic dependent launch of the previous kernel on the
-    stream: that kernel may produce q/k/v, but not the plan or ``block_tables``.
+    stream: that kernel may produce q/k/v and ``block_tables``, but not the plan.
 
     Paged with ``k_new``/``v_new`` (the step's in-flight ``[total_q, Hk, D]`` rows, row i
     for query row i): sequences with q_len == k_len read their keys from those rows and
