@@ -62,10 +62,27 @@ def test_wide_decode_warps_give_up_together():
     assert len(roles) == 5
     copies, products, queries, softmax = roles[1:]
     leaves = r"!wait\(|= wait\(|return wait\("   # something depends on a lane's own result
-    for role in (copies, queries):
-        assert "!warp_wait(" in role and not re.search(leaves, role)
+    assert re.search(r"empty_now = .*\|\| wait\(.*\n.*\n *if \(!__all_sync\(0xffffffffu, empty_now\)\) return false;", copies)
+    assert not re.search(leaves, copies)
+    assert "!warp_wait(" in queries and not re.search(leaves, queries)
     assert "if (lane == 0 && count > 0)" in products and "!wait(" in products
     assert not re.search(leaves, softmax) and "break;" not in softmax and "return;" not in softmax
     common = _source("common.cuh")
     helper = common[common.index("bool warp_wait_or_abort("):]
     assert "__all_sync(0xffffffffu, wait_or_abort(" in helper[:helper.index("}")]
+
+
+def test_prefill_softmax_warps_never_leave_a_wait():
+    """The prefill's softmax warps meet at warp and named barriers: none of them leaves its role where a wait gave up.
+    The copies' roles give theirs in flight more time."""
+    import re
+    src = _source("prefill_attn.cu")
+    kernels = re.split(r"__global__ void", src)[1:3]
+    for kernel in kernels:
+        roles = re.split(r"  // -{20,} (?=Q producer|K/V producer|MMA issuer|softmax)", kernel)
+        assert len(roles) == 5
+        softmax = roles[4]
+        assert softmax.count("wait_or_abort(") == 3
+        assert not re.search(r"!\s*wait_or_abort\(|return wait_or_abort\(|\bok\b|\bbreak;", softmax)
+        assert "drain_ring(bars.q_full" in roles[1]
+        assert "drain_ring(bars.k_full" in roles[2] and "drain_ring(bars.v_full" in roles[2]

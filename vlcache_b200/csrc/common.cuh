@@ -111,6 +111,13 @@ __device__ __forceinline__ bool warp_wait_or_abort(uint64_t* bar, uint32_t parit
   return __all_sync(0xffffffffu, wait_or_abort(bar, parity, code, abort_flag));
 }
 
+// Where a role gave up, its block's copies in flight, the last of `loads` into a ring, are given more time before
+// the block ends (until one does not come).  Not inlined: the roles' loops stay as they are.
+__device__ __noinline__ static void drain_ring(uint64_t* full, int loads, int slots, int code) {
+  for (int x = loads > slots ? loads - slots : 0; x < loads; ++x)
+    if (!mbar_wait_bounded(full + x % slots, (uint32_t)(x / slots) & 1u, code, VLC_WAIT_LIMIT_CYCLES)) return;
+}
+
 // ---------------------------------------------------------------- proxies / fences
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

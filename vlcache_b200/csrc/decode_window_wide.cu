@@ -204,9 +204,9 @@ __global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kern
     int loads = 0;
     auto issue = [&](const CUtensorMap* map, const Entry& e) {
       const int slot = loads % L::SLOTS;
-      if (loads >= L::SLOTS && !warp_wait(empty + slot, loads / L::SLOTS - 1, 27)) return false;
-      if (lane == 0) mbar_expect_tx(full + slot, TILE_BYTES);
-      __syncwarp();
+      const bool empty_now = loads < L::SLOTS || wait(empty + slot, loads / L::SLOTS - 1, 27);
+      if (lane == 0 && empty_now) mbar_expect_tx(full + slot, TILE_BYTES);
+      if (!__all_sync(0xffffffffu, empty_now)) return false;  // (a lane alone may have given up: all leave, or none)
       if (lane < BOXES) {
         int row = e.page * p.block_size + e.row;
         if ((uint32_t)e.page >= (uint32_t)p.num_pages) {  // no usable page there: zeros come
@@ -234,11 +234,7 @@ __global__ void __launch_bounds__(Layout<N>::THREADS, 1) window_decode_wide_kern
       }
     }
     // Where a role gave up, the copies in flight are given more time before the block ends.
-    if (!ok || *abort_flag) {
-      for (int x = max(0, loads - L::SLOTS); x < loads; ++x)
-        mbar_wait_bounded(full + x % L::SLOTS, (uint32_t)(x / L::SLOTS) & 1u, VLC_DEV_ERR_TIMEOUT + 28,
-                          VLC_WAIT_LIMIT_CYCLES);
-    }
+    if (!ok || *abort_flag) drain_ring(full, loads, L::SLOTS, VLC_DEV_ERR_TIMEOUT + 28);
   } else if (warp == 1) {
     // ------------------------------------------------------------ products, by one lane
     if (lane == 0 && count > 0) {

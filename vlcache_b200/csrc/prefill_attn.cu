@@ -346,7 +346,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
           tma_load_3d(qdst, &p.tm_q, bars.q_full + slot, 0, g * p.group, q_begin);
           tma_load_3d(qdst + HALF_BYTES, &p.tm_q, bars.q_full + slot, 64, g * p.group, q_begin);
         }
-        if (!ok) break;
+        if (!ok) {
+          drain_ring(bars.q_full, load, QSLOTS, VLC_DEV_ERR_TIMEOUT + 1);
+          break;
+        }
       }
     }
   } else if (warp == 8) {
@@ -397,6 +400,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
           tma_load_3d(kdst, tk, bars.k_full + s, 0, g, slot);
           tma_load_3d(kdst + HALF_BYTES, tk, bars.k_full + s, 64, g, slot);
           if (it >= STAGES && !wait_or_abort(bars.v_empty + s, ph ^ 1u, VLC_DEV_ERR_TIMEOUT + 3, abort_flag)) {
+            drain_ring(bars.k_full, it + 1, STAGES, VLC_DEV_ERR_TIMEOUT + 2);
             ok = false;
             break;
           }
@@ -410,7 +414,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
           tma_load_3d(vdst, tv, bars.v_full + s, 0, g, slot);
           tma_load_3d(vdst + HALF_BYTES, tv, bars.v_full + s, 64, g, slot);
         }
-        if (!ok) break;
+        if (!ok) {
+          drain_ring(bars.k_full, it, STAGES, VLC_DEV_ERR_TIMEOUT + 2);
+          drain_ring(bars.v_full, it, STAGES, VLC_DEV_ERR_TIMEOUT + 3);
+          break;
+        }
       }
     }
   } else if (warp == 9) {
@@ -623,12 +631,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
 
       float m_use = -INFINITY;
       float l_row = 0.f;
-      bool ok = true;
       for (int j = 0; j < n; ++j, ++t) {
-        if (!wait_or_abort(bars.s_full + x, (uint32_t)t & 1u, VLC_DEV_ERR_TIMEOUT + 9, abort_flag)) {
-          ok = false;
-          break;
-        }
+        // Where a wait gave up (its error is recorded, the outputs are void) the warps go on through all blocks, later
+        // waits ending at once: their votes and named barriers need all of them.
+        wait_or_abort(bars.s_full + x, (uint32_t)t & 1u, VLC_DEV_ERR_TIMEOUT + 9, abort_flag);
         __syncwarp();
         tc_fence_after();
         const int key0 = key_block<kWindow>(wb, kb0 + j) * BN;
@@ -696,8 +702,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
         auto clear_v = [&]() {
           const int rb = kPacked ? ring0 : t;  // ring index of this block (tile A's count = the ring's)
           const int st = rb % STAGES;
-          if (!wait_or_abort(bars.v_full + st, (uint32_t)(rb / STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 11, abort_flag))
-            return false;
+          wait_or_abort(bars.v_full + st, (uint32_t)(rb / STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 11, abort_flag);
           if (key0 + row >= kv_len || (behind && key0 + row < low_first && key0 + row >= p.sinks)) {
             const uint4 z = make_uint4(0, 0, 0, 0);
             uint4* v0 = reinterpret_cast<uint4*>(smem + OFF_V + st * TILE_BYTES + row * 128);
@@ -709,14 +714,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
             }
           }
           fence_proxy_async_smem();
-          return true;
         };
         // (A window's first block is a unit's first, whose V is still on its way: there it is waited for only
         // when the first half of P is there.)
-        if (!kWindow && zero_v && !clear_v()) {
-          ok = false;
-          break;
-        }
+        if (!kWindow && zero_v) clear_v();
         // P = exp2(s * scale_log2 - mref) as bf16 pairs: key pair (2c, 2c+1) goes to S
         // column c (its register is free: pair c reads registers 2c and 2c+1 >= c).  Each
         // half of the keys is released to the MMA as soon as it is in TMEM.
@@ -757,19 +758,17 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
           }
           tmem_wait_st();
           tc_fence_before();
-          if (kWindow && half == 0 && zero_v && !clear_v()) ok = false;
+          if (kWindow && half == 0 && zero_v) clear_v();
           mbar_arrive(half == 0 ? bars.p_lo + x : bars.p_hi + x);
         }
-        if (kWindow && !ok) break;
         {
           float l0, l1;
           f2_unpack(lsum, l0, l1);
           l_row += l0 + l1;
         }
       }
-      if (!ok) break;
       // ---------------------------------------------------------- epilogue
-      if (!wait_or_abort(bars.o_done + x, (uint32_t)nunit & 1u, VLC_DEV_ERR_TIMEOUT + 12, abort_flag)) break;
+      wait_or_abort(bars.o_done + x, (uint32_t)nunit & 1u, VLC_DEV_ERR_TIMEOUT + 12, abort_flag);
       ++nunit;
       __syncwarp();
       tc_fence_after();
@@ -1062,7 +1061,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
           tma_load_3d_pair(qdst, &p.tm_q, qbar, 0, g * p.group, q_begin);
           tma_load_3d_pair(qdst + HALF_BYTES, &p.tm_q, qbar, 64, g * p.group, q_begin);
         }
-        if (!ok) break;
+        if (!ok) {
+          if (leader) drain_ring(bars.q_full, load, QSLOTS, VLC_DEV_ERR_TIMEOUT + 1);
+          break;
+        }
       }
     }
   } else if (warp == 8) {
@@ -1111,6 +1113,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
           tma_load_3d_pair(kdst, tk, kbar, 0, g, slot + 64 * (int)rank);
           tma_load_3d_pair(kdst + quad::KHALF_BYTES, tk, kbar, 64, g, slot + 64 * (int)rank);
           if (it >= STAGES && !wait_or_abort(bars.v_empty + s, ph ^ 1u, VLC_DEV_ERR_TIMEOUT + 3, abort_flag)) {
+            if (leader) drain_ring(bars.k_full, it + 1, STAGES, VLC_DEV_ERR_TIMEOUT + 2);
             ok = false;
             break;
           }
@@ -1124,7 +1127,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
           if (leader) mbar_expect_tx(bars.v_full + s, TILE_BYTES);  // both CTAs' halves
           tma_load_3d_pair(vdst, tv, mapa_shared(smem_u32(bars.v_full + s), 0), 64 * (int)rank, g, slot);
         }
-        if (!ok) break;
+        if (!ok) {
+          if (leader) {  // (the pair's other CTA waits for this one before it ends)
+            drain_ring(bars.k_full, it, STAGES, VLC_DEV_ERR_TIMEOUT + 2);
+            drain_ring(bars.v_full, it, STAGES, VLC_DEV_ERR_TIMEOUT + 3);
+          }
+          break;
+        }
       }
     }
   } else if (warp == 9) {
@@ -1279,12 +1288,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
 
       float m_use = -INFINITY;
       float l_row = 0.f;
-      bool ok = true;
       for (int j = 0; j < n; ++j, ++t) {
-        if (!wait_or_abort(bars.s_full + x, (uint32_t)t & 1u, VLC_DEV_ERR_TIMEOUT + 9, abort_flag)) {
-          ok = false;
-          break;
-        }
+        // (warps go on where a wait gave up, as in prefill_attn_kernel)
+        wait_or_abort(bars.s_full + x, (uint32_t)t & 1u, VLC_DEV_ERR_TIMEOUT + 9, abort_flag);
         __syncwarp();
         tc_fence_after();
         const int key0 = (kb0 + j) * BN;
@@ -1329,11 +1335,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
         // has every block of the unit, and its P*V runs first.
         if (x == 0 && key0 + BN > kv_len) {
           const int st = t % STAGES;
-          if (!wait_or_abort(leader ? bars.v_full + st : v_landed + st, (uint32_t)(t / STAGES) & 1u,
-                             VLC_DEV_ERR_TIMEOUT + 11, abort_flag)) {
-            ok = false;
-            break;
-          }
+          wait_or_abort(leader ? bars.v_full + st : v_landed + st, (uint32_t)(t / STAGES) & 1u,
+                             VLC_DEV_ERR_TIMEOUT + 11, abort_flag);
           if (key0 + row >= kv_len) {
             const uint4 z = make_uint4(0, 0, 0, 0);
             uint4* v0 = reinterpret_cast<uint4*>(smem + OFF_V + st * TILE_BYTES + row * 128);
@@ -1394,9 +1397,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_quad_kernel(const
           l_row += l0 + l1;
         }
       }
-      if (!ok) break;
       // ---------------------------------------------------------- epilogue
-      if (!wait_or_abort(bars.o_done + x, (uint32_t)nunit & 1u, VLC_DEV_ERR_TIMEOUT + 12, abort_flag)) break;
+      wait_or_abort(bars.o_done + x, (uint32_t)nunit & 1u, VLC_DEV_ERR_TIMEOUT + 12, abort_flag);
       ++nunit;
       __syncwarp();
       tc_fence_after();
