@@ -86,3 +86,14 @@ def test_prefill_softmax_warps_never_leave_a_wait():
         assert not re.search(r"!\s*wait_or_abort\(|return wait_or_abort\(|\bok\b|\bbreak;", softmax)
         assert "drain_ring(bars.q_full" in roles[1]
         assert "drain_ring(bars.k_full" in roles[2] and "drain_ring(bars.v_full" in roles[2]
+
+
+def test_projection_epilogues_never_leave_a_wait():
+    """The projections' epilogue warps meet at named barriers and take tickets that the next launch relies on."""
+    import re
+    src = _source("gemm.cu")
+    epilogues = re.findall(r"  // -{20,} epilogue \(warps 2-5.*?\n  __syncthreads\(\);", src, flags=re.S)
+    assert len(epilogues) == 2
+    for role in epilogues:
+        assert role.count("wait_or_abort(") == 1 and not re.search(r"!\s*wait_or_abort\(|\bbreak;", role)
+    assert src.count("drain_ring(full, it, ") == 2

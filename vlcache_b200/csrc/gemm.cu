@@ -97,20 +97,6 @@ struct Params {
   int num_heads, num_kv_heads;
 };
 
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int code, volatile int* abort_flag) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*abort_flag) return false;
-    if (clock64() - t0 > VLC_WAIT_LIMIT_CYCLES) {
-      record_error(code);
-      *abort_flag = 1;
-      return false;
-    }
-  }
-}
-
 __device__ __forceinline__ float bf16_round(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -298,7 +284,7 @@ __device__ __forceinline__ void stage_parts(const Params& p, const Fixup& fx, in
       ++j;
     }
   }
-  // a timeout records the error; the CTA then unwinds after this tile (its values are void)
+  // a timeout records the error, and the other roles' waits end too (the values are void)
   if (!mbar_wait_bounded(fx.bar, (uint32_t)h, VLC_DEV_ERR_TIMEOUT + 51, VLC_WAIT_LIMIT_CYCLES)) *fx.abort_flag = 1;
 }
 
@@ -544,7 +530,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_kernel(const __grid_const
         for (int kb = sg.kb_lo; kb < sg.kb_hi; ++kb, ++it) {
           const int s = it % TL::STAGES;
           if (it >= TL::STAGES &&
-              !wait_bar(empty + s, (uint32_t)((it / TL::STAGES) & 1) ^ 1u, VLC_DEV_ERR_TIMEOUT + 40, abort_flag)) {
+              !wait_or_abort(empty + s, (uint32_t)((it / TL::STAGES) & 1) ^ 1u, VLC_DEV_ERR_TIMEOUT + 40, abort_flag)) {
+            drain_ring(full, it, TL::STAGES, VLC_DEV_ERR_TIMEOUT + 40);
             ok = false;
             break;
           }
@@ -572,7 +559,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_kernel(const __grid_const
       for (bool more = seg_first(p, sg); ok && more; more = seg_next(p, sg), ++local) {
         const int buf = local & 1;
         if (local >= 2 &&
-            !wait_bar(acc_empty + buf, (uint32_t)((local >> 1) & 1) ^ 1u, VLC_DEV_ERR_TIMEOUT + 41, abort_flag)) {
+            !wait_or_abort(acc_empty + buf, (uint32_t)((local >> 1) & 1) ^ 1u, VLC_DEV_ERR_TIMEOUT + 41, abort_flag)) {
           ok = false;
           break;
         }
@@ -580,7 +567,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_kernel(const __grid_const
         const uint32_t d = tmem_base + (uint32_t)buf * TN;
         for (int kb = sg.kb_lo; kb < sg.kb_hi; ++kb, ++it) {
           const int s = it % TL::STAGES;
-          if (!wait_bar(full + s, (uint32_t)(it / TL::STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 42, abort_flag)) {
+          if (!wait_or_abort(full + s, (uint32_t)(it / TL::STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 42, abort_flag)) {
             ok = false;
             break;
           }
@@ -617,7 +604,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_kernel(const __grid_const
       // inputs of the epilogue that do not depend on the accumulator: loaded while the MMAs run
       if (bias_s != nullptr) stage_bias<TN>(p.bias, nt * TN, p.n, bias_s);
       qkv_prefetch<EPI>(p, row, qr);
-      if (!wait_bar(acc_full + buf, (uint32_t)(local >> 1) & 1u, VLC_DEV_ERR_TIMEOUT + 43, abort_flag)) break;
+      // Where a wait gave up (its error is recorded, the output is void) the epilogue's warps go on through all tiles,
+      // later waits ending at once: their named barriers need all of them, and a later launch the tickets.
+      wait_or_abort(acc_full + buf, (uint32_t)(local >> 1) & 1u, VLC_DEV_ERR_TIMEOUT + 43, abort_flag);
       __syncwarp();
       tc_fence_after();
       const uint32_t tacc = tmem_base + lane_off + (uint32_t)buf * TN;
@@ -662,7 +651,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_kernel(const __grid_const
         if (!*ticket_last) {
           tc_fence_before();
           mbar_arrive(acc_empty + buf);
-          if (*abort_flag) break;
           continue;
         }
         fx.c_lo = c_lo;
@@ -677,7 +665,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_kernel(const __grid_const
       epilogue_tile<EPI, TN>(p, tacc, fx, r_in, row, nt, bias_s, qr);
       tc_fence_before();
       mbar_arrive(acc_empty + buf);
-      if (*abort_flag) break;
     }
   }
 
@@ -770,7 +757,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_pair_kernel(const __grid_
         for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
           const int s = it % PAIR_STAGES;
           if (it >= PAIR_STAGES &&
-              !wait_bar(empty + s, (uint32_t)((it / PAIR_STAGES) & 1) ^ 1u, VLC_DEV_ERR_TIMEOUT + 44, abort_flag)) {
+              !wait_or_abort(empty + s, (uint32_t)((it / PAIR_STAGES) & 1) ^ 1u, VLC_DEV_ERR_TIMEOUT + 44, abort_flag)) {
+            if (rank == 0) drain_ring(full, it, PAIR_STAGES, VLC_DEV_ERR_TIMEOUT + 44);
             ok = false;
             break;
           }
@@ -792,7 +780,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_pair_kernel(const __grid_
       for (int t = pair; ok && t < p.tiles; t += npairs, ++local) {
         const int buf = local & 1;
         if (local >= 2 &&
-            !wait_bar(acc_empty + buf, (uint32_t)((local >> 1) & 1) ^ 1u, VLC_DEV_ERR_TIMEOUT + 45, abort_flag)) {
+            !wait_or_abort(acc_empty + buf, (uint32_t)((local >> 1) & 1) ^ 1u, VLC_DEV_ERR_TIMEOUT + 45, abort_flag)) {
           ok = false;
           break;
         }
@@ -800,7 +788,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_pair_kernel(const __grid_
         const uint32_t d = tmem_base + (uint32_t)buf * BN;
         for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
           const int s = it % PAIR_STAGES;
-          if (!wait_bar(full + s, (uint32_t)(it / PAIR_STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 46, abort_flag)) {
+          if (!wait_or_abort(full + s, (uint32_t)(it / PAIR_STAGES) & 1u, VLC_DEV_ERR_TIMEOUT + 46, abort_flag)) {
             ok = false;
             break;
           }
@@ -841,7 +829,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_pair_kernel(const __grid_
       const int row = mt * PM + (int)rank * BM + r_in;
       if (bias_s != nullptr) stage_bias<BN>(p.bias, nt * BN, p.n, bias_s);
       qkv_prefetch<EPI>(p, row, qr);
-      if (!wait_bar(acc_full + buf, (uint32_t)(local >> 1) & 1u, VLC_DEV_ERR_TIMEOUT + 47, abort_flag)) break;
+      // (warps go on where a wait gave up, as in the kernel above)
+      wait_or_abort(acc_full + buf, (uint32_t)(local >> 1) & 1u, VLC_DEV_ERR_TIMEOUT + 47, abort_flag);
       __syncwarp();
       tc_fence_after();
       const uint32_t tacc = tmem_base + lane_off + (uint32_t)buf * BN;
@@ -851,7 +840,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) gemm_pair_kernel(const __grid_
         mbar_arrive(acc_empty + buf);
       else
         mbar_arrive_cluster(mapa_shared(smem_u32(acc_empty + buf), 0));
-      if (*abort_flag) break;
     }
   }
 
