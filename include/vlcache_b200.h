@@ -416,6 +416,10 @@ int vlc_mrope_store_kvcache(const int64_t* positions, int64_t axis_stride, int n
  *   cu_seqlens_k: device, num_seqs + 1.  Keys of a bad table entry read as 0, as in the bf16
  *   prefill (the 4-bit decode leaves them out), and are recorded (VLC_DEV_ERR_BLOCK_RANGE);
  *   rows past total_k are recorded (VLC_DEV_ERR_LENGTH) and not written.
+ * vlc_gather_seen_kvcache_fp4: the same for an attention with a window (vlc_attention_plan_window): of each
+ *   sequence, keys from the sinks up to lows[b] (device; the first key that its first row's window
+ *   shows) are seen by no row, and lows[b] < 0 says that none is seen (no rows): tiles of 64 keys of
+ *   them are not read, their table entries may be -1, and their rows of the outputs stay as they were.
  * vlc_mrope_shift_fp4: vlc_mrope_shift in such a cache: K rows of src_slots rotated by the
  *   delta, rounded to bf16, quantised again, written to dst_slots (NULL: in place); V rows
  *   copied when dst_slots is given.  A group whose 16 pairs the delta does not turn keeps
@@ -441,6 +445,12 @@ int vlc_gather_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t lay
                            const int32_t* block_tables, int64_t block_table_stride, int block_table_width,
                            const int32_t* cu_seqlens_k, int num_seqs, int64_t total_k, float k_scale, float v_scale,
                            void* k_out, void* v_out, int64_t out_row_stride, int64_t out_layer_stride, void* stream);
+int vlc_gather_seen_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t layer_stride, int num_layers,
+                                int64_t num_pages, int block_size, int num_kv_heads, int head_dim,
+                                const int32_t* block_tables, int64_t block_table_stride, int block_table_width,
+                                const int32_t* cu_seqlens_k, int num_seqs, int64_t total_k, float k_scale, float v_scale,
+                                void* k_out, void* v_out, int64_t out_row_stride, int64_t out_layer_stride,
+                                const int32_t* lows, int sinks, void* stream);
 int vlc_mrope_shift_fp4(void* k_cache, void* v_cache, int64_t layer_stride, int num_layers, int64_t num_pages,
                         int block_size, int num_kv_heads, int head_dim, const int32_t* src_slots,
                         const int32_t* dst_slots, int num_rows, const int32_t* delta_thw,

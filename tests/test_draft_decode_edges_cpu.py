@@ -97,3 +97,23 @@ def test_projection_epilogues_never_leave_a_wait():
     for role in epilogues:
         assert role.count("wait_or_abort(") == 1 and not re.search(r"!\s*wait_or_abort\(|\bbreak;", role)
     assert src.count("drain_ring(full, it, ") == 2
+
+
+# ------------------------------------------------------------------ windowed plans
+def test_windowed_plan_holds_first_keys(cuda_lib):
+    from vlcache_b200 import ops
+    cu_q, cu_k = [0, 5, 5, 300, 301], [0, 1000, 1400, 1695, 1700]
+    plan = ops.build_prefill_plan(cu_q, cu_k, 16, 2, num_sms=8, window=100, sinks=4)
+    assert plan.host[plan.lows_at:].tolist() == [1000 - 5 - 99, -1, 0, 0] and plan.lows_at == int(plan.host[15])
+    assert ops.build_prefill_plan(cu_q, cu_k, 16, 2, num_sms=8).lows_at is None
+    hides_nothing = ops.build_prefill_plan([0, 20], [0, 9000], 16, 2, num_sms=148, window=0)   # split: parts in 32 bits
+    assert hides_nothing.host[hides_nothing.lows_at:].tolist() == [0]
+
+
+def test_c_abi_gather_of_seen_keys_refuses(cuda_lib):
+    one = ctypes.c_void_p(64)   # never dereferenced: validation fails first
+
+    def gather(seqs=1, lows=one, sinks=0, block=64):
+        return cuda_lib.vlc_gather_seen_kvcache_fp4(one, one, 0, 1, 4, block, 2, 128, one, 4, 4, one, seqs, 100, 1.0, 1.0,
+                                                    one, one, 256, 0, lows, sinks, None)
+    assert gather(sinks=-1) == 2 and gather(lows=None) == 1 and gather(block=48) == 5 and gather(seqs=0, lows=None) == 0

@@ -197,3 +197,44 @@ def test_prefill_reads_tables_of_the_step_before(rows, window):
         torch.cuda.synchronize()
         assert ops.device_error() == 0 and int((tables < 0).sum()) == 0
         assert torch.equal(got, ops.prefill_attention(q, k_cache, v_cache, tables, plan, 0.1)), turn
+
+
+# ------------------------------------------------------------------ windowed prefill over a 4-bit cache
+@pytest.mark.parametrize("window,sinks", [(100, 0), (200, 4), (64, 130), (1, 0), (333, 64)])
+def test_prefill_window_over_a_4_bit_cache_without_hidden_pages(window, sinks):
+    """Pages that no row sees are not read: entries of -1 change nothing and record nothing; pages that rows see are."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(window)
+    block, seqs = 64, [(50, 1500), (0, 400), (130, 130), (1, 700), (300, 2000)]
+    new, lens = [a for a, _ in seqs], [b for _, b in seqs]
+    cu_q, cu_k = ([sum(x[:i]) for i in range(len(x) + 1)] for x in (new, lens))
+    widths = [(n + block - 1) // block for n in lens]
+    pages = sum(widths)
+    k4, v4 = (torch.randint(0, 256, (pages, 2, block * 72), generator=g, device="cuda", dtype=torch.int32)
+              .to(torch.uint8) for _ in range(2))
+    k, v = (torch.randn(pages * block, 2, D, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    ops.store_kvcache_fp4(k, v, k4, v4, torch.arange(pages * block, dtype=torch.int32, device="cuda"))
+    order = torch.randperm(pages, generator=g, device="cuda").tolist()
+    tables = torch.full((len(seqs), max(widths)), -1, dtype=torch.int32, device="cuda")
+    for i, w in enumerate(widths):
+        tables[i, :w] = torch.tensor([order.pop() for _ in range(w)], dtype=torch.int32)
+    q = torch.randn(sum(new), 16, D, generator=g, device="cuda").to(torch.bfloat16)
+    cu = torch.tensor(cu_k, dtype=torch.int32, device="cuda")
+    plan = ops.build_prefill_plan(cu_q, cu_k, 16, 2, device="cuda", window=window, sinks=sinks)
+    want = ops.prefill_attention_fp4(q, k4, v4, tables, cu, plan, 0.1)
+    kb, vb = ops.gather_kvcache_fp4(k4, v4, tables, cu, cu_k[-1])
+    assert torch.equal(want, ops.prefill_attention(q, kb, vb, None, plan, 0.1)) and ops.device_error() == 0
+    gone = 0
+    for i, (n, m) in enumerate(seqs):
+        for page in range(widths[i]):
+            if n == 0 or (page * block >= sinks and (page + 1) * block <= m - n - window + 1):
+                tables[i, page] = -1
+                gone += 1
+    assert gone > 20
+    # (what the workspace holds where nothing is read is not seen)
+    workspace = torch.full((ops.prefill_fp4_workspace_bytes(plan, 2),), 255, dtype=torch.uint8, device="cuda")
+    got = ops.prefill_attention_fp4(q, k4, v4, tables, cu, plan, 0.1, workspace=workspace)
+    assert torch.equal(got, want) and ops.device_error() == 0
+    tables[4, widths[4] - 1] = -1   # one that its rows see
+    ops.prefill_attention_fp4(q, k4, v4, tables, cu, plan, 0.1, workspace=workspace)
+    assert ops.device_error() == 102

@@ -72,6 +72,8 @@ SIGNATURES: dict[str, tuple] = {
                                       c_int, c_int, c_int, c_vp]),
     "vlc_gather_kvcache_fp4": (c_int, [c_vp, c_vp, c_i64, c_int, c_i64, c_int, c_int, c_int, c_vp, c_i64, c_int, c_vp,
                                        c_int, c_i64, c_float, c_float, c_vp, c_vp, c_i64, c_i64, c_vp]),
+    "vlc_gather_seen_kvcache_fp4": (c_int, [c_vp, c_vp, c_i64, c_int, c_i64, c_int, c_int, c_int, c_vp, c_i64, c_int, c_vp,
+                                            c_int, c_i64, c_float, c_float, c_vp, c_vp, c_i64, c_i64, c_vp, c_int, c_vp]),
     "vlc_mrope_shift_fp4": (c_int, [c_vp, c_vp, c_i64, c_int, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_int, c_vp,
                                     c_vp, c_float, c_vp]),
     "vlc_decode_attn_fp4": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_i64,

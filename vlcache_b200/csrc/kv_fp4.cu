@@ -56,6 +56,10 @@ struct GatherParams {
   __nv_bfloat16* out[2];
   int64_t out_row_stride, out_layer_stride;
   bool wide;  // outputs 32-byte aligned
+  // Null, or of each sequence the first key that a row's window shows (below 0: no row sees any): tiles between the
+  // sinks and it are left out.
+  const int32_t* lows;
+  int sinks;
 };
 
 __global__ void __launch_bounds__(256) gather_fp4_kernel(const __grid_constant__ GatherParams p) {
@@ -70,6 +74,10 @@ __global__ void __launch_bounds__(256) gather_fp4_kernel(const __grid_constant__
   const int len = __ldg(p.cu_seqlens_k + lo + 1) - (int)begin;
   const int64_t j0 = ((int64_t)blockIdx.x - (begin / TILE + lo)) * TILE;
   if (j0 < 0 || j0 >= len) return;
+  if (p.lows != nullptr) {
+    const int low = __ldg(p.lows + lo);
+    if (low < 0 || (j0 >= p.sinks && j0 + TILE <= low)) return;
+  }
   const int head = blockIdx.y, layer = blockIdx.z;
   const int table_index = (int)j0 / p.block_size;
   const int page = table_index < p.table_width ? __ldg(p.block_tables + lo * p.table_stride + table_index) : -1;
@@ -248,12 +256,13 @@ static float inv_freq_f32(float theta, int j) { return 1.0f / powf(theta, (float
 using namespace vlc;
 using namespace vlc::kv_fp4;
 
-extern "C" int vlc_gather_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t layer_stride, int num_layers,
-                                      int64_t num_pages, int block_size, int num_kv_heads, int head_dim,
-                                      const int32_t* block_tables, int64_t block_table_stride, int block_table_width,
-                                      const int32_t* cu_seqlens_k, int num_seqs, int64_t total_k, float k_scale,
-                                      float v_scale, void* k_out, void* v_out, int64_t out_row_stride,
-                                      int64_t out_layer_stride, void* stream) {
+// lows null: all keys.
+static int gather_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t layer_stride, int num_layers,
+                              int64_t num_pages, int block_size, int num_kv_heads, int head_dim,
+                              const int32_t* block_tables, int64_t block_table_stride, int block_table_width,
+                              const int32_t* cu_seqlens_k, int num_seqs, int64_t total_k, float k_scale, float v_scale,
+                              void* k_out, void* v_out, int64_t out_row_stride, int64_t out_layer_stride,
+                              const int32_t* lows, int sinks, void* stream) {
   if (num_seqs < 0 || total_k < 0 || num_layers < 0 || block_table_width < 0 || num_kv_heads <= 0)
     return VLC_ERR_SHAPE;
   if (head_dim != HD || block_size <= 0 || block_size % TILE != 0 || block_size > fp4::MAX_BLOCK) return VLC_ERR_UNSUPPORTED;
@@ -290,9 +299,36 @@ extern "C" int vlc_gather_kvcache_fp4(const void* k_cache, const void* v_cache, 
   p.out_layer_stride = out_layer_stride;
   p.wide = reinterpret_cast<uintptr_t>(k_out) % 32 == 0 && reinterpret_cast<uintptr_t>(v_out) % 32 == 0 &&
            out_row_stride % 16 == 0 && out_layer_stride % 16 == 0;
+  p.lows = lows;
+  p.sinks = sinks;
   const dim3 grid((unsigned)(total_k / TILE + num_seqs), num_kv_heads, num_layers);
   gather_fp4_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(p);
   return launch_status();
+}
+
+extern "C" int vlc_gather_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t layer_stride, int num_layers,
+                                      int64_t num_pages, int block_size, int num_kv_heads, int head_dim,
+                                      const int32_t* block_tables, int64_t block_table_stride, int block_table_width,
+                                      const int32_t* cu_seqlens_k, int num_seqs, int64_t total_k, float k_scale,
+                                      float v_scale, void* k_out, void* v_out, int64_t out_row_stride,
+                                      int64_t out_layer_stride, void* stream) {
+  return gather_kvcache_fp4(k_cache, v_cache, layer_stride, num_layers, num_pages, block_size, num_kv_heads, head_dim,
+                            block_tables, block_table_stride, block_table_width, cu_seqlens_k, num_seqs, total_k, k_scale,
+                            v_scale, k_out, v_out, out_row_stride, out_layer_stride, nullptr, 0, stream);
+}
+
+extern "C" int vlc_gather_seen_kvcache_fp4(const void* k_cache, const void* v_cache, int64_t layer_stride,
+                                           int num_layers, int64_t num_pages, int block_size, int num_kv_heads,
+                                           int head_dim, const int32_t* block_tables, int64_t block_table_stride,
+                                           int block_table_width, const int32_t* cu_seqlens_k, int num_seqs,
+                                           int64_t total_k, float k_scale, float v_scale, void* k_out, void* v_out,
+                                           int64_t out_row_stride, int64_t out_layer_stride, const int32_t* lows,
+                                           int sinks, void* stream) {
+  if (sinks < 0) return VLC_ERR_SHAPE;
+  if (num_seqs > 0 && !lows) return VLC_ERR_NULL;
+  return gather_kvcache_fp4(k_cache, v_cache, layer_stride, num_layers, num_pages, block_size, num_kv_heads, head_dim,
+                            block_tables, block_table_stride, block_table_width, cu_seqlens_k, num_seqs, total_k, k_scale,
+                            v_scale, k_out, v_out, out_row_stride, out_layer_stride, lows, sinks, stream);
 }
 
 extern "C" int vlc_mrope_shift_fp4(void* k_cache, void* v_cache, int64_t layer_stride, int num_layers,

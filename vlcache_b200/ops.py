@@ -187,12 +187,14 @@ def mrope_shift_all_layers(kv_cache: torch.Tensor, src_slots: torch.Tensor, dst_
 @dataclass
 class PrefillPlan:
     """Host plan (numpy int32) plus its device copy and workspace size (bytes), and the key
-    rows and sequences it was built for."""
+    rows and sequences it was built for.  Behind a windowed plan, at ``lows_at``, stands the first key of each
+    sequence that its first row's window shows (-1: it has no rows)."""
     host: np.ndarray
     dev: torch.Tensor | None
     workspace_bytes: int
     total_k: int = 0
     num_seqs: int = 0
+    lows_at: int | None = None
 
     @property
     def host_ptr(self) -> int:
@@ -226,6 +228,7 @@ class PrefillPlan:
         return [(int(r[0]), int(r[1]), int(r[2])) for r in rec]
 
 
+PLAN_WINDOW, PLAN_SINKS = 22, 23   # of a plan's header (csrc/plan.h)
 PREFILL_DEFAULT, PREFILL_PAIRS, PREFILL_QUADS = 0, 1, 2
 
 
@@ -265,10 +268,16 @@ def build_prefill_plan(cu_seqlens_q, cu_seqlens_k, num_heads: int, num_kv_heads:
         check("vlc_attention_plan_window", L.vlc_attention_plan_window(*sizes, int(window), int(sinks), *room))
     plan = plan[: used.value].copy()
     ws = int(L.vlc_prefill_workspace_size(plan.ctypes.data))
+    lows_at = None
+    if plan[PLAN_WINDOW] > 0:
+        rows, keys = np.diff(cq), np.diff(ck)
+        lows = np.where(rows > 0, np.maximum(0, keys - rows - int(plan[PLAN_WINDOW]) + 1), -1).astype(np.int32)
+        lows_at, plan = len(plan), np.concatenate((plan, lows))
     dev = None
     if device is not None:
         dev = torch.from_numpy(plan).pin_memory().to(device, non_blocking=True)
-    return PrefillPlan(host=plan, dev=dev, workspace_bytes=ws, total_k=int(ck[-1]), num_seqs=nseq)
+    return PrefillPlan(host=plan, dev=dev, workspace_bytes=ws, total_k=int(ck[-1]), num_seqs=nseq,
+                       lows_at=lows_at)
 
 
 def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_tables: torch.Tensor | None,
@@ -899,7 +908,8 @@ def prefill_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     to bf16 once (``gather_kvcache_fp4``, exact), then the tcgen05 attention kernel runs on
     them.  A prompt's query tiles share each key, so each is converted once.  The read-back
     writes 512 bytes a key and KV head: 12 MB for one warm 4K-image request of 2 KV heads, which
-    stay in L2 (4 of 24 us), 222 MB for 64 warm 1080p requests, which do not (48 of 263 us).  As in
+    stay in L2 (4 of 24 us), 222 MB for 64 warm 1080p requests, which do not (48 of 263 us).  Under a plan's
+    window, keys that no row sees are not read (their block-table entries may be -1).  As in
     ``prefill_attention``, P and the partial outputs of split tiles are bf16 (off by 2^-8 of
     themselves at most, each), where the 4-bit decode keeps P in f16 and its parts in fp32.
     ``cu_seqlens_k``: the plan's, on the device; ``workspace``: ``prefill_fp4_workspace_bytes``,
@@ -923,9 +933,13 @@ def prefill_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     row = hk * HEAD_DIM
     k = workspace.data_ptr() + _round_up(plan.workspace_bytes, 256)
     v = k + 2 * total_k * row
-    _launch(dev, "vlc_gather_kvcache_fp4", k_cache.data_ptr(), v_cache.data_ptr(), 0, 1, pages, block, hk, d,
-            block_tables.data_ptr(), stride, width, cu_seqlens_k.data_ptr(), seqs, total_k, float(k_scale),
-            float(v_scale), k, v, row, 0)
+    gather = (k_cache.data_ptr(), v_cache.data_ptr(), 0, 1, pages, block, hk, d, block_tables.data_ptr(), stride, width,
+              cu_seqlens_k.data_ptr(), seqs, total_k, float(k_scale), float(v_scale), k, v, row, 0)
+    if plan.lows_at is None:
+        _launch(dev, "vlc_gather_kvcache_fp4", *gather)
+    else:   # (keys that no row sees, whose pages may be gone, are left out)
+        _launch(dev, "vlc_gather_seen_kvcache_fp4", *gather, plan.dev.data_ptr() + 4 * plan.lows_at,
+                int(plan.host[PLAN_SINKS]))
     _launch(dev, "vlc_prefill_attn", q.data_ptr(), qs, n, h, k, v, row, row, total_k, hk, d, None, 0, 0,
             plan.dev.data_ptr(), plan.host_ptr, float(softmax_scale), out.data_ptr(), os, workspace.data_ptr(),
             plan.workspace_bytes)
