@@ -117,3 +117,41 @@ def test_c_abi_gather_of_seen_keys_refuses(cuda_lib):
         return cuda_lib.vlc_gather_seen_kvcache_fp4(one, one, 0, 1, 4, block, 2, 128, one, 4, 4, one, seqs, 100, 1.0, 1.0,
                                                     one, one, 256, 0, lows, sinks, None)
     assert gather(sinks=-1) == 2 and gather(lows=None) == 1 and gather(block=48) == 5 and gather(seqs=0, lows=None) == 0
+
+
+# ------------------------------------------------------------------ the engine's bookkeeping
+def _decoder(pages=20, **kw):
+    from vlcache_b200.engine.draft_decode import DraftDecode
+    from vlcache_b200.engine.page_pool import PagePool
+    pool = PagePool(pages, 32)
+    return pool, DraftDecode(pool, **{**dict(places=3, max_pages=6, num_drafts=2, device="cpu"), **kw})
+
+
+@pytest.mark.parametrize("window,sinks,tokens", [(40, 3, 170), (40, 0, 170), (1, 0, 161), (33, 64, 192), (100, 5, 190)])
+def test_admit_takes_a_table_whose_hidden_pages_are_gone(window, sinks, tokens):
+    """Entries of -1 where no later row sees a key, and nowhere else: the pages that a step would give back."""
+    pool, d = _decoder(window=window, sinks=sinks)
+    full = pool.allocate(6)
+    seen = {j // 32 for j in range(tokens + 1) if j > tokens - window or j < sinks}
+    hidden = [i for i in range(6) if i not in seen]
+    assert hidden or window == 100
+    table = [-1 if i in hidden else p for i, p in enumerate(full)]
+    pool.free([full[i] for i in hidden])
+    for i in sorted(seen & set(range(6))):
+        with pytest.raises(ValueError, match="not this table's alone"):
+            d.admit(0, [-1 if x == i else p for x, p in enumerate(table)], tokens)
+    assert int(d.context_lens[0]) == -1
+    for bad in (-2, 20):
+        for i in hidden:
+            with pytest.raises(ValueError, match="not this table's alone"):
+                d.admit(0, [bad if x == i else p for x, p in enumerate(table)], tokens)
+    d.admit(0, table, tokens)
+    assert d.block_tables[0].tolist() == table and int(d.context_lens[0]) == tokens
+    assert d.retire(0) == tokens and pool.num_free == 20 and pool.refs == [0] * 20
+
+
+def test_admit_without_a_window_needs_every_page():
+    pool, d = _decoder()
+    table = pool.allocate(3)
+    with pytest.raises(ValueError, match="not this table's alone"):
+        d.admit(0, [-1] + table[1:], 96)

@@ -10,7 +10,8 @@ emitted tokens whenever it wants to.
 Pages come from a ``PagePool``: ``lend`` moves some to the device's free list, which the steps take
 pages from and give those behind the window back to; ``settle`` returns them.  A sequence enters with
 the block table that its prompt was stored through (``admit``) and leaves with ``retire``.  The
-tables own their pages: a forked table, which shares some, cannot enter.
+tables own their pages: a forked table, which shares some, cannot enter.  After ``PagePool.compact``
+the block tables and the free list go through ``ops.remap_block_tables`` as every device table does.
 """
 from __future__ import annotations
 
@@ -66,7 +67,8 @@ class DraftDecode:
     def admit(self, place: int, block_table: list[int], num_tokens: int) -> None:
         """A sequence of ``num_tokens`` tokens in the cache, stored through ``block_table`` (its pages are the
         decoder's from here on), takes an idle place.  Its next token, not in the cache yet, is the
-        first of its rows in the next step."""
+        first of its rows in the next step.  Entries of pages that it no longer sees, behind the window and the sinks,
+        may be -1."""
         if not 0 <= place < self.places:
             raise ValueError(f"place {place} is outside the {self.places}")
         if int(self.context_lens[place]) >= 0:
@@ -75,15 +77,22 @@ class DraftDecode:
             raise ValueError("the block table does not hold that many tokens")
         if len(block_table) > self.max_pages:
             raise ValueError(f"a block table of {len(block_table)} pages, {self.max_pages} at most")
-        shared = [p for p in block_table if not 0 <= p < self.pool.num_pages or self.pool.refs[p] != 1]
+        gone = [p == -1 and self._behind(i, num_tokens) for i, p in enumerate(block_table)]
+        pages = [p for p, g in zip(block_table, gone) if not g]
+        shared = [p for p in pages if not 0 <= p < self.pool.num_pages or self.pool.refs[p] != 1]
         if shared:
             raise ValueError(f"page {shared[0]} is not this table's alone")
-        if len(set(block_table)) != len(block_table):
+        if len(set(pages)) != len(pages):
             raise ValueError("a page is in the block table twice")
         row = torch.full((self.max_pages,), -1, dtype=torch.int32)
         row[:len(block_table)] = torch.tensor(block_table, dtype=torch.int32)
         self.block_tables[place] = row.to(self.block_tables.device)
         self.context_lens[place] = num_tokens
+
+    def _behind(self, page: int, num_tokens: int) -> bool:
+        """Whether entry ``page`` of a table is one that no row at position ``num_tokens`` or later sees."""
+        block = self.pool.block_size
+        return self.window > 0 and page * block >= self.sinks and (page + 1) * block <= num_tokens - self.window + 1
 
     def retire(self, place: int) -> int:
         """A sequence leaves: its pages go back to the pool, its place is idle.  Returns its tokens in the cache."""
