@@ -155,3 +155,24 @@ def test_admit_without_a_window_needs_every_page():
     table = pool.allocate(3)
     with pytest.raises(ValueError, match="not this table's alone"):
         d.admit(0, [-1] + table[1:], 96)
+
+
+def test_admit_refuses_pages_that_the_decoder_has():
+    """A page of another place's table, or one that was lent, would be written by two sequences and given back twice."""
+    pool, d = _decoder()
+    table = pool.allocate(2)
+    d.admit(0, table, 64)
+    for other in (table, pool.allocate(1) + table[1:]):
+        with pytest.raises(ValueError, match="another place's table"):
+            d.admit(1, other, 40)
+    assert d.lend(2)
+    lent = d.free_pages[:2].tolist()
+    with pytest.raises(ValueError, match="was lent"):
+        d.admit(1, lent, 40)
+    d.settle()   # now they are the pool's, and nobody's
+    assert d.retire(0) == 64
+    d.admit(1, table[:0], 0)
+    assert int(d.context_lens[1]) == 0
+    again = pool.allocate(4)   # pages that the decoder had are a table's again
+    d.admit(2, again, 100)
+    assert d.block_tables[2].tolist() == again + [-1, -1]

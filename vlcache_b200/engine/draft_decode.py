@@ -84,6 +84,9 @@ class DraftDecode:
             raise ValueError(f"page {shared[0]} is not this table's alone")
         if len(set(pages)) != len(pages):
             raise ValueError("a page is in the block table twice")
+        mine = torch.cat((self.block_tables.flatten(), self.free_pages[:int(self.num_free)]))
+        if pages and bool(torch.isin(torch.tensor(pages, dtype=torch.int32).to(mine.device), mine).any()):
+            raise ValueError("a page is in another place's table or was lent")
         row = torch.full((self.max_pages,), -1, dtype=torch.int32)
         row[:len(block_table)] = torch.tensor(block_table, dtype=torch.int32)
         self.block_tables[place] = row.to(self.block_tables.device)
