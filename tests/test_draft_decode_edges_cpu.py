@@ -176,3 +176,50 @@ def test_admit_refuses_pages_that_the_decoder_has():
     again = pool.allocate(4)   # pages that the decoder had are a table's again
     d.admit(2, again, 100)
     assert d.block_tables[2].tolist() == again + [-1, -1]
+
+
+# ------------------------------------------------------------------ rows of a decode step
+@pytest.mark.parametrize("rows,lens,tokens,refused", [
+    (4, 2, None, True), (3, 2, None, True), (4, 2, 2, False), (2, 2, 2, False), (6, 2, 2, True), (3, 2, 2, True),
+    (2, 2, None, False), (1, 2, None, False), (2, 2, 0, True),
+])
+def test_attention_takes_the_tokens_that_the_context_says(rows, lens, tokens, refused, monkeypatch):
+    """Twice as many rows as lengths are no two tokens each unless the context says so: a slip in the lengths is
+    refused before anything runs."""
+    from vlcache_b200 import ops
+    from vlcache_b200.layers.attention import Attention
+    from vlcache_b200.utils.context import reset_context, set_context
+    calls = []
+    monkeypatch.setattr(ops, "decode_workspace_bytes", lambda *a: 0)
+    monkeypatch.setattr(ops, "decode_window_workspace_bytes", lambda *a: 0)
+    monkeypatch.setattr(ops, "decode_attention", lambda q, *a, **k: calls.append(q.shape) or q)
+    monkeypatch.setattr(ops, "decode_attention_window", lambda q, *a, **k: calls.append((q.shape, a[2].shape, a[3].shape)) or q)
+    layer = Attention(4, 128, 0.1, 2)
+    layer.k_cache, layer.v_cache = (torch.zeros(2, 32, 2, 128, dtype=torch.bfloat16) for _ in range(2))
+    kw = {} if tokens is None else dict(num_tokens=tokens)
+    try:
+        set_context(False, context_lens=torch.ones(lens, dtype=torch.int32),
+                    block_tables=torch.zeros(lens, 1, dtype=torch.int32), **kw)
+        q = torch.zeros(rows, 4, 128, dtype=torch.bfloat16)
+        if refused:
+            with pytest.raises(ValueError, match=f"decode: {rows} rows for {lens} sequences"):
+                layer(q, None, None)
+            assert not calls
+        else:
+            layer(q, None, None)
+            n = tokens or 1
+            assert calls == ([((rows // n, n, 4, 128), (rows // n, 1), (rows // n,))] if n > 1 else [(rows, 4, 128)])
+    finally:
+        reset_context()
+
+
+def test_draft_decode_says_its_tokens(monkeypatch):
+    from vlcache_b200 import ops
+    from vlcache_b200.utils.context import get_context, reset_context
+    _, d = _decoder()
+    monkeypatch.setattr(ops, "step_metadata", lambda *a: (torch.zeros(9),) * 4 + (d.context_lens,))
+    try:
+        d.begin()
+        assert get_context().num_tokens == 3 and not get_context().is_prefill
+    finally:
+        reset_context()

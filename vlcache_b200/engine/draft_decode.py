@@ -121,7 +121,7 @@ class DraftDecode:
         # (Rows past a table's end are in the lengths too: a bound without them would cut the lengths, and so move
         # the rows before them.)
         set_context(False, slot_mapping=slots, context_lens=lens, block_tables=self.block_tables,
-                    max_context_len=self.max_pages * self.pool.block_size + self.num_tokens)
+                    max_context_len=self.max_pages * self.pool.block_size + self.num_tokens, num_tokens=self.num_tokens)
         return positions
 
     def finish(self, drafts: torch.Tensor, target_probs: torch.Tensor, draft_probs: torch.Tensor | None,

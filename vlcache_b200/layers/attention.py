@@ -118,10 +118,10 @@ class Attention(nn.Module):
         have_cache = bool(k_cache.numel() and v_cache.numel()) and k is not None
         fp4 = k_cache.dtype == torch.uint8
         tokens = 1   # of a sequence in a decode step
-        if not context.is_prefill and q.shape[0] > context.context_lens.numel():
-            tokens, rest = divmod(q.shape[0], max(1, context.context_lens.numel()))
-            if rest:
-                raise ValueError(f"decode: {q.shape[0]} rows for {context.context_lens.numel()} sequences")
+        if not context.is_prefill:
+            tokens, lens = context.num_tokens, context.context_lens.numel()
+            if tokens < 1 or q.shape[0] % tokens or q.shape[0] > tokens * lens:
+                raise ValueError(f"decode: {q.shape[0]} rows for {lens} sequences of {tokens} tokens")
         windowed = self.sliding_window > 0 or tokens > 1
         if fp4 and windowed:
             raise ValueError("a 4-bit cache takes no sliding window and one token a sequence")

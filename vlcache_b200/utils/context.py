@@ -12,7 +12,9 @@ keep working):
                           block-table width times the block size: no device read);
   * ``workspace``       — scratch tensor reused by every layer of the step;
   * ``kv_ready``        — per-layer CUDA events (``engine.kv_cache.copy_image_kv_per_layer``):
-                          layer i's attention waits for event i before it reads the cache.
+                          layer i's attention waits for event i before it reads the cache;
+  * ``num_tokens``      — query rows of each sequence in a decode step (its last tokens: drafted
+                          ones to verify, ``engine.draft_decode``), 1 unless said.
 ``window_plans`` holds the prefill plans of layers with a sliding window, by (window, sinks).
 """
 from __future__ import annotations
@@ -40,6 +42,7 @@ class Context:
     max_context_len: int | None = None
     workspace: torch.Tensor | None = None
     kv_ready: Any = None
+    num_tokens: int = 1
     window_plans: dict = field(default_factory=dict)
 
 
@@ -53,11 +56,11 @@ def get_context() -> Context:
 def set_context(is_prefill, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0, max_seqlen_k=0,
                 slot_mapping=None, context_lens=None, block_tables=None, *, prefill_plan=None,
                 cu_seqlens_q_host=None, cu_seqlens_k_host=None, max_context_len=None, workspace=None,
-                kv_ready=None):
+                kv_ready=None, num_tokens=1):
     global _CONTEXT
     _CONTEXT = Context(is_prefill, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, slot_mapping,
                        context_lens, block_tables, prefill_plan, cu_seqlens_q_host, cu_seqlens_k_host,
-                       max_context_len, workspace, kv_ready)
+                       max_context_len, workspace, kv_ready, num_tokens)
 
 
 def reset_context():
