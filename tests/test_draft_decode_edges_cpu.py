@@ -223,3 +223,40 @@ def test_draft_decode_says_its_tokens(monkeypatch):
         assert get_context().num_tokens == 3 and not get_context().is_prefill
     finally:
         reset_context()
+
+
+# ------------------------------------------------------------------ the build
+@pytest.mark.parametrize("torch_there", [True, False])
+def test_library_is_built_without_torch(torch_there, monkeypatch, tmp_path):
+    """The library needs no torch: without it the build leaves the binding out (and says so in its stamp)."""
+    from pathlib import Path
+
+    from vlcache_b200 import build
+    for name in ("LIB_PATH", "BINDING_PATH", "STAMP_PATH", "BUILD_DIR"):
+        monkeypatch.setattr(build, name, tmp_path / name)
+    with_torch = build.source_hash()
+    if not torch_there:
+        real_spec, real_version = build.importlib.util.find_spec, build.importlib.metadata.version
+
+        def version(name):
+            if name == "torch":
+                raise build.importlib.metadata.PackageNotFoundError(name)
+            return real_version(name)
+        monkeypatch.setattr(build.importlib.util, "find_spec", lambda n, *a: None if n == "torch" else real_spec(n, *a))
+        monkeypatch.setattr(build.importlib.metadata, "version", version)
+    tools = []
+
+    def run(cmd, **kw):
+        tools.append(Path(cmd[0]).name)
+        out = Path(cmd[cmd.index("-o") + 1])
+        out.parent.mkdir(parents=True, exist_ok=True)
+        out.write_text("built")
+        return build.subprocess.CompletedProcess(cmd, 0, "", "")
+    monkeypatch.setattr(build.subprocess, "run", run)
+    assert build.build() == build.LIB_PATH and build.LIB_PATH.exists() and build.is_fresh()
+    assert build.BINDING_PATH.exists() == torch_there and tools.count("g++") == (2 if torch_there else 0)
+    assert tools.count("nvcc") == len(build.CUDA_SOURCES) + len(build.CPP_SOURCES) + 1
+    assert (build.source_hash() == with_torch) == torch_there
+    tools.clear()
+    build.build()
+    assert not tools   # fresh

@@ -5,7 +5,8 @@ exist on other architectures) with nvcc, links the host planner, and links the
 CUDA runtime statically so the library has no torch dependency.  The driver API
 (cuTensorMapEncodeTiled) is reached through cudaGetDriverEntryPoint, so the
 library also loads on machines without a GPU (CPU-side tests use the planner).  A small Python extension
-(``_binding``, g++ against torch's headers) calls it for the ops whose calls are short.
+(``_binding``, g++ against torch's headers) calls it for the ops whose calls are short; where torch is not installed,
+the library is built without it.
 
 Usage: ``python -m vlcache_b200.build [--force] [--verbose]``.
 """
@@ -59,9 +60,10 @@ STAMP_PATH = LIB_PATH.with_name(LIB_PATH.name + ".srchash")
 
 def source_hash() -> str:
     """SHA-256 over the bytes of every source, header and this recipe (names included), and the versions of
-    Python and torch that the binding is built for: the library is rebuilt exactly when this differs
-    from the hash it was built from."""
-    h = hashlib.sha256(f"{sys.implementation.cache_tag} {importlib.metadata.version('torch')}\0".encode())
+    Python and torch that the binding is built for (none: no binding): the library is rebuilt exactly when this
+    differs from the hash it was built from."""
+    torch = importlib.metadata.version("torch") if _torch_dir() else "none"
+    h = hashlib.sha256(f"{sys.implementation.cache_tag} {torch}\0".encode())
     for p in _sources() + _headers() + [Path(__file__)]:
         h.update(p.name.encode())
         h.update(b"\0")
@@ -72,7 +74,7 @@ def source_hash() -> str:
 
 def is_fresh() -> bool:
     """True when the in-tree library exists and was built from the current sources."""
-    return (LIB_PATH.exists() and BINDING_PATH.exists() and STAMP_PATH.exists()
+    return (LIB_PATH.exists() and (BINDING_PATH.exists() or not _torch_dir()) and STAMP_PATH.exists()
             and STAMP_PATH.read_text().strip() == source_hash())
 
 
@@ -98,12 +100,10 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
-def _torch_dir() -> Path:
-    """Where torch is installed, without importing it."""
+def _torch_dir() -> Path | None:
+    """Where torch is installed (None: nowhere), without importing it."""
     spec = importlib.util.find_spec("torch")
-    if spec is None or not spec.submodule_search_locations:
-        raise RuntimeError("torch not found; the vlcache_b200 binding cannot be built")
-    return Path(spec.submodule_search_locations[0])
+    return Path(spec.submodule_search_locations[0]) if spec and spec.submodule_search_locations else None
 
 
 def _compile_binding(verbose: bool) -> Path:
@@ -138,9 +138,9 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not _needs_build():
         return LIB_PATH
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
-        binding = ex.submit(_compile_binding, verbose)
+        binding = ex.submit(_compile_binding, verbose) if _torch_dir() else None
         objs = list(ex.map(lambda s: _compile(s, verbose), [CSRC / s for s in CUDA_SOURCES + CPP_SOURCES]))
-        binding_obj = binding.result()
+        binding_obj = binding.result() if binding else None
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [nvcc_path(), *ARCH_FLAGS, "-rdc=true", "-shared", "-cudart", "static", "-Xcompiler", "-fPIC",
            "-o", str(tmp), *map(str, objs)]
@@ -149,7 +149,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
     digest = source_hash()
     os.replace(tmp, LIB_PATH)
-    _link_binding(binding_obj)
+    if binding_obj:
+        _link_binding(binding_obj)
     STAMP_PATH.write_text(digest + "\n")
     return LIB_PATH
 
