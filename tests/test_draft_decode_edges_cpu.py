@@ -110,6 +110,31 @@ def test_windowed_plan_holds_first_keys(cuda_lib):
     assert hides_nothing.host[hides_nothing.lows_at:].tolist() == [0]
 
 
+@pytest.mark.parametrize("window,parts,wide", [
+    (None, None, False), (0, None, True), (None, torch.float32, True), (0, torch.float32, True),
+    (None, torch.bfloat16, False), (0, torch.bfloat16, False), (4000, None, True), (4000, torch.float32, True),
+    (9000, torch.float32, True),
+])
+def test_plan_parts_have_a_named_type(cuda_lib, window, parts, wide):
+    """What split tiles are kept in goes by a name; no window and a window of 0 are the same mask under either."""
+    from vlcache_b200 import ops
+    plan = ops.build_prefill_plan([0, 20], [0, 9000], 16, 2, num_sms=148, window=window, parts=parts)
+    assert plan.num_parts > 0 and plan.workspace_bytes == plan.num_parts * 128 * (128 * (4 if wide else 2) + 8)
+    if not window:   # the same mask, and so the same plan
+        other = ops.build_prefill_plan([0, 20], [0, 9000], 16, 2, num_sms=148, window=0 if wide else None)
+        assert plan.host.tolist() == other.host.tolist()
+    whole = ops.build_prefill_plan([0, 700], [0, 900], 16, 2, num_sms=16, window=window, parts=parts)
+    assert whole.num_parts == 0 and whole.workspace_bytes == 0
+
+
+def test_plan_parts_refusals(cuda_lib):
+    from vlcache_b200 import ops
+    for kw in (dict(parts=torch.float16), dict(parts="fp32"), dict(parts=torch.bfloat16, window=100),
+               dict(parts=torch.float32, causal=False)):
+        with pytest.raises(ValueError, match="parts"):
+            ops.build_prefill_plan([0, 64], [0, 64], 16, 2, num_sms=8, **kw)
+
+
 def test_c_abi_gather_of_seen_keys_refuses(cuda_lib):
     one = ctypes.c_void_p(64)   # never dereferenced: validation fails first
 

@@ -241,13 +241,23 @@ def set_prefill_kernel(mode: int) -> None:
 
 def build_prefill_plan(cu_seqlens_q, cu_seqlens_k, num_heads: int, num_kv_heads: int, head_dim: int = HEAD_DIM,
                        num_sms: int = 0, device: torch.device | str | None = None, causal: bool = True,
-                       window: int | None = None, sinks: int = 0) -> PrefillPlan:
+                       window: int | None = None, sinks: int = 0, parts: torch.dtype | None = None) -> PrefillPlan:
     """Plan the warm-prefill attention launch from HOST cu_seqlens (lists/arrays/CPU tensors).
     ``causal=False`` plans the non-causal varlen attention (every row sees all keys of its
     sequence); ``head_dim`` may be 80..128 in steps of 16.  ``window`` > 0: a row at position t sees
     key j <= t iff j > t - window or j < ``sinks``; pages that no row sees are not read (their
-    block-table entries may be -1).  Parts of tiles that several CTAs share are bf16 without
-    ``window`` and fp32 with one, 0 (every key is visible) among them."""
+    block-table entries may be -1).
+    ``parts``: the type in which tiles that several CTAs share are kept until they are joined,
+    torch.bfloat16 or torch.float32 (error against 64 bits 2.7e-3 or 1.7e-3; 48 rows behind 8000 keys 23.9 or
+    27.8 us, and positive softmax scales only).  Unless said, fp32 where ``window`` is given, 0 (every key is
+    visible, as without) among them, and bf16 else, as ``layers.attention`` plans layers without a window.
+    A ``window`` above 0 and non-causal plans have one type only, fp32 and bf16."""
+    if parts not in (None, torch.bfloat16, torch.float32):
+        raise ValueError("parts: torch.bfloat16 or torch.float32")
+    if (parts == torch.bfloat16 and window) or (parts == torch.float32 and not causal):
+        raise ValueError("parts: fp32 under a window, bf16 in a non-causal plan")
+    if parts is not None and not window:
+        window = 0 if parts == torch.float32 else None
     cq = np.ascontiguousarray(np.asarray(cu_seqlens_q, dtype=np.int32))
     ck = np.ascontiguousarray(np.asarray(cu_seqlens_k, dtype=np.int32))
     nseq = len(cq) - 1
