@@ -238,3 +238,61 @@ def test_prefill_window_over_a_4_bit_cache_without_hidden_pages(window, sinks):
     tables[4, widths[4] - 1] = -1   # one that its rows see
     ops.prefill_attention_fp4(q, k4, v4, tables, cu, plan, 0.1, workspace=workspace)
     assert ops.device_error() == 102
+
+
+# ------------------------------------------------------------------ windowed prefill, to the bound of 32-bit parts
+STEP = 2.0 ** -8   # half a step of bf16, relative
+
+
+def _prefill_cases():
+    from test_gpu_draft_decode import PREFILL
+    return [(*c, D) for c in PREFILL] + [(16, 2, 256, 40, 3, [(300, 300), (9, 5000)], d) for d in (80, 96, 112)] + \
+        [(16, 2, 256, 3000, 4, [(48, 9000)], D), (28, 4, 256, 6000, 300, [(20, 12000), (7, 30)], D)]
+
+
+@pytest.mark.parametrize("case", _prefill_cases(), ids=lambda c: "-".join(map(str, (c[0], c[1], c[3], c[4], c[6]))))
+def test_prefill_window_keeps_parts_in_32_bits(case):
+    """P's rounding (STEP of itself, sum p |v| <= rms) and the output's (STEP of it) are the only ones, also where a
+    window hides keys and tiles are split: 2^-12 for what fp32 scores, sums and parts are off by."""
+    ops = _ops()
+    heads, kv_heads, _, window, sinks, seqs, head_dim = case
+    g = torch.Generator(device="cuda").manual_seed(heads + window + head_dim)
+    cu_q, cu_k = ([sum(x[:i]) for i in range(len(x) + 1)] for x in ([a for a, _ in seqs], [b for _, b in seqs]))
+    q = (1.5 * torch.randn(cu_q[-1], heads, head_dim, generator=g, device="cuda")).to(torch.bfloat16)
+    k, v = (torch.randn(cu_k[-1], kv_heads, head_dim, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    plan = ops.build_prefill_plan(cu_q, cu_k, heads, kv_heads, head_dim, device="cuda", window=window, sinks=sinks)
+    assert plan.num_parts > 0 or window < 3000
+    got = ops.prefill_attention(q, k, v, None, plan, 0.09)
+    assert ops.device_error() == 0
+    for i, (n, m) in enumerate(seqs):
+        want, rms = oracle.attention(q[cu_q[i]:cu_q[i + 1]].double(), k[cu_k[i]:cu_k[i + 1]].double(),
+                                     v[cu_k[i]:cu_k[i + 1]].double(), torch.arange(m - n, m, device="cuda"), window, sinks,
+                                     0.09)
+        off = (got[cu_q[i]:cu_q[i + 1]].double() - want).abs()
+        assert bool((off <= (STEP + 2.0 ** -12) * (rms + want.abs()) + 1e-30).all()), i
+
+
+# ------------------------------------------------------------------ positions of several axes
+def test_draft_decode_positions_of_several_axes():
+    """A step's rows behind images: each place's offset on the device makes [axes, rows] of the positions."""
+    from vlcache_b200.engine.draft_decode import DraftDecode
+    from vlcache_b200.engine.page_pool import PagePool
+    from vlcache_b200.layers.rotary_embedding import get_mrope
+    from vlcache_b200.utils.context import reset_context
+    ops = _ops()
+    pool = PagePool(12, 32)
+    d = DraftDecode(pool, 3, 4, 2)
+    assert d.lend(4)
+    d.admit(0, pool.allocate(2), 50)
+    d.admit(2, pool.allocate(1), 9)
+    offsets = torch.tensor([-30, 0, 7], device="cuda")   # (idle places: 0)
+    positions = d.begin()
+    axes = (positions.view(3, -1) + offsets.view(-1, 1)).view(1, -1).expand(3, -1)
+    assert axes.tolist() == [[20, 21, 22, 0, 0, 0, 16, 17, 18]] * 3
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k = (torch.randn(9, h, D, generator=g, device="cuda").to(torch.bfloat16) for h in (4, 2))
+    rot = get_mrope(D, D, 64, 1e6).cuda()
+    for a, b in zip(rot(axes, q, k), rot(axes.contiguous(), q, k)):
+        assert torch.equal(a, b)
+    assert ops.device_error() == 0
+    reset_context()
