@@ -285,3 +285,19 @@ def test_library_is_built_without_torch(torch_there, monkeypatch, tmp_path):
     tools.clear()
     build.build()
     assert not tools   # fresh
+
+
+@pytest.mark.parametrize("num_drafts", [0, 1, 5])
+def test_draft_decode_bounds_lengths_by_its_tables(num_drafts, monkeypatch):
+    """A step that begins in a table is not cut, one that begins at its end is: a single token's length never passes
+    the table, which the one-token decode reads unchecked."""
+    from vlcache_b200 import ops
+    from vlcache_b200.utils.context import get_context, reset_context
+    _, d = _decoder(num_drafts=num_drafts)
+    monkeypatch.setattr(ops, "step_metadata", lambda *a: (torch.zeros(9),) * 4 + (d.context_lens,))
+    try:
+        d.begin()
+        bound, room = get_context().max_context_len, 6 * 32
+        assert (room - 1) + (num_drafts + 1) <= bound < room + (num_drafts + 1)
+    finally:
+        reset_context()

@@ -166,6 +166,53 @@ def test_draft_decode_without_pages(all_windowed):
     reset_context()
 
 
+def test_one_token_steps_to_the_table_end():
+    """Steps without drafts over layers without a window (the one-token decode), up to and past a full table."""
+    from test_gpu_draft_decode import _Model
+
+    from vlcache_b200.engine.draft_decode import DraftDecode
+    from vlcache_b200.engine.page_pool import PagePool
+    from vlcache_b200.layers.attention import Attention
+    from vlcache_b200.utils.context import reset_context, set_context
+    import numpy as np
+    ops = _ops()
+    block, places = 256, 2
+    model = _Model(5)
+    model.layers = [Attention(model.heads, D, 0.1, model.kv_heads) for _ in range(2)]
+    pool = PagePool(6, block)
+    model.caches(6, block)
+    d = DraftDecode(pool, places, 2, 0)
+    r = np.random.default_rng(2)
+    histories = {0: [int(x) for x in r.integers(0, 97, 505)], 1: [int(x) for x in r.integers(0, 97, 254)]}
+    last = {}
+    for place, tokens in histories.items():
+        table, n = pool.allocate(pool.pages_for(len(tokens))), len(tokens)
+        slots = torch.tensor([table[t // block] * block + t % block for t in range(n)], dtype=torch.int32, device="cuda")
+        cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        set_context(True, cu, cu, n, n, slots, None, None, cu_seqlens_q_host=[0, n], cu_seqlens_k_host=[0, n])
+        last[place] = int(model(torch.tensor(tokens, device="cuda"), torch.arange(n, device="cuda"))[-1].argmax())
+        d.admit(place, table, n)
+    none = torch.zeros(places, 0, device="cuda")
+    for turn in range(12):
+        if turn == 5:
+            assert d.lend(1)   # place 1 stands at 256 tokens until now
+        positions = d.begin()
+        probs = model(torch.tensor([last[0], last[1]], device="cuda"), positions).view(places, 1, -1)
+        tokens, emitted = d.finish(none.long(), probs, None, none, torch.full((places,), 0.5, device="cuda"))
+        assert ops.device_error() in (0, 102, 104, 105)
+        for p, h in histories.items():
+            stored = len(h) < 512 and (p == 0 or len(h) < 256 or turn >= 5)
+            assert int(emitted[p]) == int(stored), (turn, p)
+            if stored:
+                want = model.plain(h + [last[p]])[-1]
+                assert float((probs[p, 0].double() - want).abs().max()) < 0.05   # (as in the test of steps with pages)
+                h.append(last[p])
+                last[p] = int(tokens[p, 0])
+            assert int(d.context_lens[p]) == len(h)
+    assert len(histories[0]) == 512 and len(histories[1]) == 256 + 7
+    reset_context()
+
+
 # ------------------------------------------------------------------ one call behind another
 @pytest.mark.parametrize("rows,window", [(700, 0), (700, 100), (20000, 0), (20000, 1000)])   # one launch of metadata, and two
 def test_prefill_reads_tables_of_the_step_before(rows, window):

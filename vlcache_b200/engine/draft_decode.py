@@ -118,10 +118,11 @@ class DraftDecode:
         positions, slots, _, _, lens = ops.step_metadata(self.context_lens, self.new_lens, self.block_tables,
                                                          self.free_pages, self.num_free, self.pool.block_size, rows,
                                                          self.window, self.sinks)
-        # (Rows past a table's end are in the lengths too: a bound without them would cut the lengths, and so move
-        # the rows before them.)
+        # The bound takes in a step that reaches past a table's end (cut lengths would move the rows before the end), but
+        # no more: a step that begins there is cut, none of whose rows count, so that a sequence's single token stays in
+        # its table (vlc_decode_attn has no width to look at).
         set_context(False, slot_mapping=slots, context_lens=lens, block_tables=self.block_tables,
-                    max_context_len=self.max_pages * self.pool.block_size + self.num_tokens, num_tokens=self.num_tokens)
+                    max_context_len=self.max_pages * self.pool.block_size + self.num_tokens - 1, num_tokens=self.num_tokens)
         return positions
 
     def finish(self, drafts: torch.Tensor, target_probs: torch.Tensor, draft_probs: torch.Tensor | None,
