@@ -301,3 +301,10 @@ def test_draft_decode_bounds_lengths_by_its_tables(num_drafts, monkeypatch):
         assert (room - 1) + (num_drafts + 1) <= bound < room + (num_drafts + 1)
     finally:
         reset_context()
+
+
+def test_draft_decode_refuses_more_drafts_than_a_verification_takes():
+    for bad in (dict(num_drafts=32), dict(places=65536)):
+        with pytest.raises(ValueError, match="places"):
+            _decoder(**bad)
+    _decoder(num_drafts=31)

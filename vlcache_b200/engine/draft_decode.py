@@ -29,8 +29,8 @@ class DraftDecode:
 
     def __init__(self, pool: PagePool, places: int, max_pages: int, num_drafts: int, window: int = 0, sinks: int = 0,
                  device: torch.device | str = "cuda"):
-        if places <= 0 or max_pages <= 0 or num_drafts < 0:
-            raise ValueError("places and max_pages must be positive, num_drafts not negative")
+        if not 0 < places <= 65535 or max_pages <= 0 or not 0 <= num_drafts <= 31:
+            raise ValueError("places: 1 .. 65535, max_pages: positive, num_drafts: 0 .. 31")
         if pool.block_size % 32:
             raise ValueError("block_size must be a multiple of 32")
         self.pool, self.places, self.max_pages = pool, places, max_pages
