@@ -5,7 +5,8 @@
 // Everything here is sm_100a inline PTX written for this library.  Every wait
 // on an mbarrier is bounded: after VLC_WAIT_LIMIT_CYCLES the waiting thread
 // records an error code in the library's device error word and reports failure
-// so the kernel can unwind instead of hanging the GPU.
+// so the kernel can end instead of hanging the GPU.  Warps that meet others at
+// votes or barriers leave their role together, or go on to its end.
 #pragma once
 
 #include <cuda.h>

@@ -45,7 +45,7 @@ constexpr int WARPS = 4;                 // of a block
 constexpr int RING_BYTES = 64 << 10;     // of a block, shared out among its warps
 constexpr int CK = 16;                   // keys of a chunk
 constexpr int BLOCKS_PER_SM = 2;
-constexpr int WIDE_ROWS = 24;            // more rows go to decode_window_wide.cu, whatever the lengths are
+constexpr int WIDE_ROWS = 24;            // more rows go to decode_window_wide.cu, whatever the lengths are (wide_of)
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -595,10 +595,12 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
   }
 }
 
-// Whether decode_window_wide.cu takes the call.  There : here (by teams of warps, by clusters where they were faster), us.
-// 40 rows: one sequence of 500 keys and 2 KV heads 9.8 : 9.4, of 2000 10.2 : 12.9, of 8000 12.8 : 15.2; eight of 2000
-// 14.7 : 14.9; sixteen of 8000 32.0 : 34.4; 32 of 4000 32.7 : 34.4.  64 rows, the same: 11.2 : 9.8, 11.6 : 11.9,
-// 14.1 : 14.1, 16.0 : 18.7, 34.0 : 44.8, 35.9 : 45.1.
+// Whether decode_window_wide.cu takes the call: it does where the rows are more than three tiles here.  Below that both
+// could; here : there, us (WIDE_ROWS lowered), 16 query and 2 KV heads without a window, caches out of L2.  16 rows: one
+// sequence of 500 keys 7.2 : 8.4, of 2000 9.3 : 9.4, of 8000 13.3 : 10.9; eight of 2000 11.4 : 13.3; sixteen of 8000
+// 28.4 : 30.1.  24 rows: 8.8 : 8.7, 11.0 : 9.4, 15.9 : 11.4, 13.7 : 13.7, 30.6 : 29.9.  64 sequences under a window (28 and 4
+// heads): 14 rows 91.2 : 93.6, 21 rows 95.5 : 95.1.  So up to 16 rows batches are faster here, and 24 are near even but
+// for one long sequence.
 static bool wide_of(int rows) { return rows > WIDE_ROWS; }
 
 // Most chunks that any sequence has under the host's bound.

@@ -34,7 +34,7 @@
 //   warps 2-5  epilogue: thread = TMEM lane = tile row; reads its row 32 columns at a
 //              time, applies the epilogue, stores to global memory, then releases the
 //              TMEM half so the issuer can start the tile after next in it.
-// Every mbarrier wait is bounded; a timeout records a device error and the CTA unwinds.
+// Every mbarrier wait is bounded; a timeout records a device error, the epilogue goes on to its end and the CTA returns.
 #include <algorithm>
 #include <cmath>
 

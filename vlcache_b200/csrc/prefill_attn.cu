@@ -720,7 +720,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) prefill_attn_kernel(const __gr
         if (!kWindow && zero_v) clear_v();
         // P = exp2(s * scale_log2 - mref) as bf16 pairs: key pair (2c, 2c+1) goes to S
         // column c (its register is free: pair c reads registers 2c and 2c+1 >= c).  Each
-        // half of the keys is released to the MMA as soon as it is in TMEM.
+        // half of the keys is released to the MMA as soon as it is in TMEM.  The sum is of the
+        // exponentials before their rounding: P, which the MMA takes in bf16 only, is off by 2^-8 of itself at
+        // most, of either sign, in O alone, so that a row's weights add to 1 but for that (summing the rounded
+        // ones, as the windowed decode does, is two more instructions a pair in a loop that they bound).
         const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
         const uint64_t negm2 = f2_pack(-mref, -mref);
         uint64_t lsum = f2_pack(0.f, 0.f);

@@ -113,7 +113,10 @@ class DraftDecode:
     def begin(self) -> torch.Tensor:
         """Take the step's pages, make its metadata and install it (``set_context``); returns the rows'
         positions int64 [places * (num_drafts + 1)].  The rows are the places' tokens, one place behind
-        another: its last token, then its drafts; idle places have rows too, which nothing is stored for."""
+        another: its last token, then its drafts; idle places have rows too, which nothing is stored for.
+        A rotary with several axes, whose positions behind an image differ from the tokens' numbers by an offset of
+        each sequence, takes ``(positions.view(places, -1) + offsets.view(-1, 1)).view(1, -1).expand(axes, -1)``,
+        ``offsets`` int64 [places] on the device (0 in idle places)."""
         rows = self.places * self.num_tokens
         positions, slots, _, _, lens = ops.step_metadata(self.context_lens, self.new_lens, self.block_tables,
                                                          self.free_pages, self.num_free, self.pool.block_size, rows,

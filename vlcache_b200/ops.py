@@ -1039,7 +1039,8 @@ def step_metadata(context_lens: torch.Tensor, new_lens: torch.Tensor, block_tabl
     ``total_rows`` bounds the new tokens on the host.  Pages that the list does not have, positions
     past the table and rows past ``total_rows`` are recorded (``device_error``) and have slot -1 or are
     left out (include/vlcache_b200.h).  The tables' pages are their own: forked requests, which share
-    pages, stay with ``engine.page_pool``."""
+    pages, stay with ``engine.page_pool``.  Any kernel may follow on the stream, the prefill too, which starts before
+    this one has ended but reads the tables behind it."""
     return (_compiled or _binding()).step_metadata(context_lens, new_lens, block_tables, free_pages, num_free, block_size,
                                                    total_rows, window, sinks)
 
