@@ -19,6 +19,7 @@ def _verify_args(**kw):
     (dict(block_tables=torch.zeros(3, 4)), "block_tables"),
     (dict(block_tables=torch.zeros(4, 3, dtype=torch.int32).T), "rows must be contiguous"),
     (dict(block_size=0), "block_size"), (dict(block_size=1 << 31), "block_size"), ({}, "CUDA tensors only"),
+    (dict(block_tables=None), "block_size: with block_tables"),   # rows that it was to leave out would count
 ])
 def test_verify_refuses_tables(cuda_lib, change, what):
     from vlcache_b200 import ops

@@ -62,8 +62,7 @@ def source_hash() -> str:
     """SHA-256 over the bytes of every source, header and this recipe (names included), and the versions of
     Python and torch that the binding is built for (none: no binding): the library is rebuilt exactly when this
     differs from the hash it was built from."""
-    torch = importlib.metadata.version("torch") if _torch_dir() else "none"
-    h = hashlib.sha256(f"{sys.implementation.cache_tag} {torch}\0".encode())
+    h = hashlib.sha256(f"{sys.implementation.cache_tag} {_torch_version()}\0".encode())
     for p in _sources() + _headers() + [Path(__file__)]:
         h.update(p.name.encode())
         h.update(b"\0")
@@ -104,6 +103,15 @@ def _torch_dir() -> Path | None:
     """Where torch is installed (None: nowhere), without importing it."""
     spec = importlib.util.find_spec("torch")
     return Path(spec.submodule_search_locations[0]) if spec and spec.submodule_search_locations else None
+
+
+def _torch_version() -> str:
+    if not _torch_dir():
+        return "none"
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:   # a tree that was not installed
+        return "unnamed"
 
 
 def _compile_binding(verbose: bool) -> Path:

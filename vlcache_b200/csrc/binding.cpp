@@ -264,6 +264,7 @@ PyObject* verify_drafts(PyObject* const* a) {
   const int32_t* const context_lens = lens.defined() ? ints_of(lens, b, "context_lens") : nullptr;
   Tables t{};
   int block = 0;
+  need(tables.defined() || a[7] == Py_None, "block_size: with block_tables");
   if (tables.defined()) {
     need(lens.defined(), "block_tables: with context_lens");
     t = tables_of(tables, b);
