@@ -211,7 +211,8 @@ struct Row {
   }
 };
 
-template <typename T>
+// PAGED: rows of the step without a page are left out.
+template <typename T, bool PAGED>
 __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) verify_kernel(const Params a) {
   __shared__ uint64_t sums[MAX_BLOCKS * WARPS];  // of all warps of the cluster
   __shared__ uint64_t kept[WARPS][MAX_TILES];    // of the tiles of this block's warps
@@ -227,19 +228,21 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) verify_kernel(const Pa
   // ---- acceptance, in every block
   if (warp == 0) {
     bool live = false, taken = false;
-    // Row r of the step (its last token, then the drafts) is in the cache iff the table has a page for it; what is
-    // behind the first that is not, was computed without its key.
     int stored = 32;
-    const int len = a.block_size > 0 ? a.context_lens[seq] : -1;
-    if (len >= 0) {  // (idle places have no rows)
-      const uint32_t t = (uint32_t)len + lane, page = t / (uint32_t)a.block_size;
-      const int number = page < (uint32_t)a.table_width ? __ldg(a.block_tables + seq * a.table_stride + page) : -1;
-      const bool there = number >= 0 && (int64_t)number * a.block_size + t % (uint32_t)a.block_size <= INT_MAX;
-      const uint32_t none = ~__ballot_sync(0xffffffffu, there);
-      stored = none ? __ffs(none) - 1 : 32;
+    if constexpr (PAGED) {
+      // Row r of the step (its last token, then the drafts) is in the cache iff the table has a page for it; what is
+      // behind the first that is not, was computed without its key.
+      const int len = a.context_lens[seq];
+      if (len >= 0) {  // (idle places have no rows)
+        const uint32_t t = (uint32_t)len + lane, page = t / (uint32_t)a.block_size;
+        const int number = page < (uint32_t)a.table_width ? __ldg(a.block_tables + seq * a.table_stride + page) : -1;
+        const bool there = number >= 0 && (int64_t)number * a.block_size + t % (uint32_t)a.block_size <= INT_MAX;
+        const uint32_t none = ~__ballot_sync(0xffffffffu, there);
+        stored = none ? __ffs(none) - 1 : 32;
+      }
     }
     if (lane < a.num_drafts) {
-      const int64_t d = lane + 1 < stored ? drafts[lane] : -1;
+      const int64_t d = !PAGED || lane + 1 < stored ? drafts[lane] : -1;
       live = d >= 0 && d < a.vocab;
       if (d >= a.vocab && rank == 0) record_error(VLC_DEV_ERR_TOKEN);
       const int64_t v = live ? d : 0;
@@ -250,13 +253,13 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) verify_kernel(const Pa
     const uint32_t yes = __ballot_sync(0xffffffffu, taken), have = __ballot_sync(0xffffffffu, live);
     const int n = __ffs(~yes) == 0 ? 32 : __ffs(~yes) - 1;
     if (lane == 0) {
-      s_taken = stored > 0 ? n : -1;
+      s_taken = !PAGED || stored > 0 ? n : -1;
       s_refused = n < a.num_drafts && (have >> n & 1);
     }
   }
   __syncthreads();
   const int taken = s_taken;
-  if (taken < 0) {  // the sequence's own token is not in the cache: it waits for a page
+  if (PAGED && taken < 0) {  // the sequence's own token is not in the cache: it waits for a page
     if (rank == 0 && threadIdx.x <= a.num_drafts) a.tokens[(int64_t)seq * (a.num_drafts + 1) + threadIdx.x] = -1;
     if (rank == 0 && threadIdx.x == 0) a.emitted[seq] = 0;
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -368,6 +371,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) verify_kernel(const Pa
 
 template <typename T>
 static int launch(const Params& a, int num_seqs, int blocks, cudaStream_t st) {
+  const auto kernel = a.block_size > 0 ? verify_kernel<T, true> : verify_kernel<T, false>;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(blocks, num_seqs);
   cfg.blockDim = dim3(THREADS);
@@ -379,7 +383,7 @@ static int launch(const Params& a, int num_seqs, int blocks, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, verify_kernel<T>, a) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) {
     (void)cudaGetLastError();
     return VLC_ERR_CUDA;
   }
