@@ -213,6 +213,38 @@ def test_one_token_steps_to_the_table_end():
     reset_context()
 
 
+def test_draft_decode_over_a_compacted_pool():
+    """Tables and free list through the page map: lent pages and sequences' are the pool's still, each once."""
+    from vlcache_b200.engine.draft_decode import DraftDecode
+    from vlcache_b200.engine.page_pool import PagePool
+    from vlcache_b200.utils.context import reset_context
+    ops = _ops()
+    pool = PagePool(30, 32)
+    d = DraftDecode(pool, 3, 6, 2)
+    filler = pool.allocate(9)
+    assert d.lend(4)
+    tables = {0: pool.allocate(3), 2: pool.allocate(2)}
+    d.admit(0, tables[0], 95)   # the next step takes a page
+    d.admit(2, tables[2], 33)
+    pool.free(filler)
+    src, dst, page_map = pool.compact()
+    assert src and max(dst) < 9
+    on_device = torch.from_numpy(page_map).cuda()
+    for t in (d.block_tables, d.free_pages.view(1, -1)):
+        ops.remap_block_tables(t, on_device)
+    assert ops.device_error() == 0
+    d.begin()
+    assert ops.device_error() == 0 and int(d.num_free) == 3
+    held = [p for row in d.block_tables.tolist() for p in row if p >= 0] + d.free_pages[:3].tolist()
+    assert sorted(held) == list(range(9)) and all(pool.refs[p] == 1 for p in held)
+    assert d.block_tables[0, :3].tolist() == [int(page_map[p]) for p in tables[0]]
+    for p in (0, 2):
+        d.retire(p)
+    d.settle()
+    assert pool.num_free == 30 and pool.refs == [0] * 30
+    reset_context()
+
+
 # ------------------------------------------------------------------ one call behind another
 @pytest.mark.parametrize("rows,window", [(700, 0), (700, 100), (20000, 0), (20000, 1000)])   # one launch of metadata, and two
 def test_prefill_reads_tables_of_the_step_before(rows, window):

@@ -11,7 +11,7 @@ Pages come from a ``PagePool``: ``lend`` moves some to the device's free list, w
 pages from and give those behind the window back to; ``settle`` returns them.  A sequence enters with
 the block table that its prompt was stored through (``admit``) and leaves with ``retire``.  The
 tables own their pages: a forked table, which shares some, cannot enter.  After ``PagePool.compact``
-the block tables and the free list go through ``ops.remap_block_tables`` as every device table does.
+``block_tables`` and ``free_pages.view(1, -1)`` go through ``ops.remap_block_tables`` as every device table does.
 """
 from __future__ import annotations
 
